@@ -6,9 +6,12 @@ A case is a plain dict; `op` names the operator:
 
   quant      rows (fp32 or bf16, `ldx` >= `k`) to e4m3 rows and their scales
   linear     a product with an f8 weight: `m` rows, `k` -> `n`; `x`: "f32" rows quantized by the call or "f8" rows
-             that an earlier operator left; `epi`: "store", "resid" (out += r) or "gated" (out += gate * r)
-  glu        the gated half of a feed-forward block: act(x Wg^T) * (x Wu^T), `f` columns wide, as fp32 or f8 rows
-  norm       the seam between two blocks: x += res_scale * gate * post(y), h = norm(x), h as fp32 or f8 rows
+             that an earlier operator left; `epi`: "store", "resid" (out += r) or "gated" (out += gate * r);
+             `out`: "bf16" rows (stored), from sums as exact as that needs, or "f32" rows from 32-bit sums
+  glu        the gated half of a feed-forward block: act(x Wg^T) * (x Wu^T), `f` columns wide, as fp32 or f8 rows,
+             from 32-bit sums
+  norm       the seam between two blocks: x += res_scale * gate * post(y), h = norm(x), h as fp32 or f8 rows;
+             `y`: "bf16" or "f32" rows of a product, or "" (the norm alone)
 
 Definition of the 8-bit rows (all operations in 32 bits, rounded to nearest even): for a block of 128 columns with
 largest magnitude a (at least 2^-100), s = a / 448 and q = e4m3(x * (448 / a)).
@@ -33,25 +36,35 @@ def listed():
         # a short prompt's q columns inside its stacked q/k/v rows: a strided slice of few rows
         {"name": "quant_43x2048_of_4096", "op": "quant", "m": 43, "k": 2048, "ldx": 4096, "bf16": False},
         # one token through the text encoder's stacked q/k/v projection: the latency of a single row
-        {"name": "linear_1x4096x1024", "op": "linear", "m": 1, "n": 4096, "k": 1024, "x": "f32", "epi": "store", "act": "none"},
+        {"name": "linear_1x4096x1024", "op": "linear", "m": 1, "n": 4096, "k": 1024, "x": "f32", "epi": "store",
+         "act": "none", "out": "f32"},
         # a short prompt through the output projection, added to the residual stream
-        {"name": "linear_43x1024x2048_resid", "op": "linear", "m": 43, "n": 1024, "k": 2048, "x": "f32", "epi": "resid", "act": "none"},
-        # sizes that divide nothing: a cropped image's tokens, a last block of 16 columns of k, 36 of n
-        {"name": "linear_3013x1316x1424_gelu", "op": "linear", "m": 3013, "n": 1316, "k": 1424, "x": "f8", "epi": "store", "act": "gelu"},
-        # the second MLP product of a DiT step, two images of 1024 x 1024, gated into the residual stream
-        {"name": "linear_8192x2048x8192_gated", "op": "linear", "m": 8192, "n": 2048, "k": 8192, "x": "f8", "epi": "gated", "act": "none"},
+        {"name": "linear_43x1024x2048_resid", "op": "linear", "m": 43, "n": 1024, "k": 2048, "x": "f32",
+         "epi": "resid", "act": "none", "out": "f32"},
+        # sizes that divide nothing: a cropped image's tokens, a last block of 16 columns of k, 36 of n; gated into the
+        # residual stream
+        {"name": "linear_3013x1316x1424_gated", "op": "linear", "m": 3013, "n": 1316, "k": 1424, "x": "f8",
+         "epi": "gated", "act": "none", "out": "f32"},
+        # the second MLP product of a DiT step, two images of 1024 x 1024, for the seam behind it
+        {"name": "linear_8192x2048x8192_bf16", "op": "linear", "m": 8192, "n": 2048, "k": 8192, "x": "f8",
+         "epi": "store", "act": "none", "out": "bf16"},
         # one token through a gated feed-forward block's first half
         {"name": "glu_1x4096x1024", "op": "glu", "m": 1, "f": 4096, "k": 1024, "x": "f32", "out": "f32", "act": "silu"},
         # a prompt padded to the context length
-        {"name": "glu_512x4096x1024_f8", "op": "glu", "m": 512, "f": 4096, "k": 1024, "x": "f8", "out": "f8", "act": "silu"},
+        {"name": "glu_512x4096x1024_f8", "op": "glu", "m": 512, "f": 4096, "k": 1024, "x": "f8", "out": "f8",
+         "act": "silu"},
         # an image model's gated MLP at two images of 1024 x 1024: the largest
-        {"name": "glu_8192x8192x2048_f8", "op": "glu", "m": 8192, "f": 8192, "k": 2048, "x": "f8", "out": "f8", "act": "silu"},
+        {"name": "glu_8192x8192x2048_f8", "op": "glu", "m": 8192, "f": 8192, "k": 2048, "x": "f8", "out": "f8",
+         "act": "silu"},
         # one token between two blocks of the text encoder
-        {"name": "norm_1x1024_f8", "op": "norm", "m": 1, "c": 1024, "y": True, "post": False, "gate": False, "mod": False, "layer": False, "groups": 1, "out": "f8"},
+        {"name": "norm_1x1024_f8", "op": "norm", "m": 1, "c": 1024, "y": "f32", "post": False, "gate": False,
+         "mod": False, "layer": False, "groups": 1, "out": "f8"},
         # a prompt between two blocks with a norm on both sides of the seam, fp32 rows out
-        {"name": "norm_512x1600_post", "op": "norm", "m": 512, "c": 1600, "y": True, "post": True, "gate": False, "mod": False, "layer": False, "groups": 1, "out": "f32"},
+        {"name": "norm_512x1600_post", "op": "norm", "m": 512, "c": 1600, "y": "f32", "post": True, "gate": False,
+         "mod": False, "layer": False, "groups": 1, "out": "f32"},
         # two images of 1024 x 1024 with modulation vectors of their own
-        {"name": "norm_8192x2048_mod_f8", "op": "norm", "m": 8192, "c": 2048, "y": True, "post": False, "gate": True, "mod": True, "layer": True, "groups": 2, "out": "f8"},
+        {"name": "norm_8192x2048_mod_f8", "op": "norm", "m": 8192, "c": 2048, "y": "bf16", "post": False,
+         "gate": True, "mod": True, "layer": True, "groups": 2, "out": "f8"},
     ]
 
 
@@ -63,12 +76,15 @@ def draw(rng):
     op = rng.choice(["quant", "linear", "linear", "glu", "glu", "norm", "norm"])
     if op == "quant":
         m, k = _log_int(rng, 1, 8192), _log_int(rng, 64, 8192, 16)
-        return {"op": op, "m": m, "k": k, "ldx": k + 8 * rng.choice([0, 0, rng.randint(1, 256)]), "bf16": rng.choice([True, False])}
+        return {"op": op, "m": m, "k": k, "ldx": k + 8 * rng.choice([0, 0, rng.randint(1, 256)]),
+                "bf16": rng.choice([True, False])}
     if op == "linear":
         m, n, k = _log_int(rng, 1, 8192), _log_int(rng, 64, 8192, 4), _log_int(rng, 64, 8192, 16)
         n = max(64, min(n, (1 << 37) // (m * k) // 4 * 4))
-        return {"op": op, "m": m, "n": n, "k": k, "x": rng.choice(["f8", "f32"]), "epi": rng.choice(["store", "resid", "gated"]),
-                "act": rng.choice(["none", "none", "gelu", "silu"])}
+        epi = rng.choice(["store", "store", "resid", "gated"])
+        return {"op": op, "m": m, "n": n, "k": k, "x": rng.choice(["f8", "f32"]), "epi": epi,
+                "act": rng.choice(["none", "none", "gelu", "silu"]),
+                "out": rng.choice(["bf16", "bf16", "f32"]) if epi == "store" else "f32"}
     if op == "glu":
         m, f, k = _log_int(rng, 1, 8192), _log_int(rng, 64, 8192, 16), _log_int(rng, 64, 8192, 16)
         f = max(64, min(f, (1 << 36) // (m * k) // 16 * 16))
@@ -76,9 +92,9 @@ def draw(rng):
                 "act": rng.choice(["silu", "silu", "gelu"])}
     m, c = _log_int(rng, 1, 8192), _log_int(rng, 64, 8192, 16)
     groups = rng.choice([1, 1, 2, 4])
-    return {"op": op, "m": -(-m // groups) * groups, "c": c, "y": rng.choice([True, True, False]), "post": rng.choice([True, False]),
-            "gate": rng.choice([True, False]), "mod": rng.choice([True, False]), "layer": rng.choice([True, False]), "groups": groups,
-            "out": rng.choice(["f8", "f32"])}
+    return {"op": op, "m": -(-m // groups) * groups, "c": c, "y": rng.choice(["bf16", "f32", ""]),
+            "post": rng.choice([True, False]), "gate": rng.choice([True, False]), "mod": rng.choice([True, False]),
+            "layer": rng.choice([True, False]), "groups": groups, "out": rng.choice(["f8", "f32"])}
 
 
 # ---------------------------------------------------------------- inputs
@@ -126,7 +142,8 @@ def _inputs(case, seed):
         c = case["c"]
         t["x"] = g.rows(m, c) * 3.0
         if case["y"]:
-            t["y"] = g.rows(m, c)
+            y = g.rows(m, c)
+            t["y"] = y.to(torch.bfloat16) if case["y"] == "bf16" else y
         if case["post"]:
             t["post"] = g.normal((c,), 0.1, 1.0)
         if case["gate"]:
@@ -165,7 +182,7 @@ def prepare(case, seed):
     elif op == "linear" and case["epi"] != "store":
         s.out = s.t["out"]
     else:
-        s.out = torch.empty((m, n), device="cuda")
+        s.out = torch.empty((m, n), device="cuda", dtype=torch.bfloat16 if case["out"] == "bf16" else torch.float32)
     s.weights = None
     torch.cuda.synchronize()
     return s
@@ -222,7 +239,7 @@ def _plain(s):
     if op == "linear":
         r = _act(_plain_x(s) @ _weight32(t["w"]).t() + t["bias"], case["act"])
         if case["epi"] == "store":
-            return r
+            return r.to(s.out.dtype)
         return s.out.add_(r * t["gate"] if case["epi"] == "gated" else r)
     if op == "glu":
         x = _plain_x(s)
@@ -230,7 +247,7 @@ def _plain(s):
         return _quantize(h) if case["out"] == "f8" else h
     x = t["x"]
     if case["y"]:
-        y = t["y"]
+        y = t["y"].float()
         if case["post"]:
             y = y / torch.sqrt((y * y).mean(1, keepdim=True) + EPS) * t["post"]
         if case["gate"]:
@@ -284,17 +301,18 @@ def _own(s):
     if op == "linear":
         epi = {"store": _module.EPI_STORE, "resid": _module.EPI_RESID, "gated": _module.EPI_GATED}[case["epi"]]
         ctx.linear(_weights(s)[0], m, _ptr(s.out), x=_ptr(t.get("x")), xq=_ptr(t.get("xq")), xs=_ptr(t.get("xs")),
-                   act=case["act"], epilogue=epi, gate=_ptr(t.get("gate")))
+                   act=case["act"], epilogue=epi, gate=_ptr(t.get("gate")), out_bf16=case["out"] == "bf16",
+                   precision=_module.PREC_BF16 if case["out"] == "bf16" else _module.PREC_FP32)
         return s.out
     if op == "glu":
         wg, wu = _weights(s)
         f8 = case["out"] == "f8"
         ctx.linear_glu(wg, wu, m, x=_ptr(t.get("x")), xq=_ptr(t.get("xq")), xs=_ptr(t.get("xs")), act=case["act"],
-                       out=None if f8 else _ptr(s.out), out_q=_ptr(s.q) if f8 else None, out_s=_ptr(s.s) if f8 else None)
+                       precision=_module.PREC_FP32, out=None if f8 else _ptr(s.out), out_q=_ptr(s.q) if f8 else None, out_s=_ptr(s.s) if f8 else None)
         return _f8(s) if f8 else s.out
     f8 = case["out"] == "f8"
-    ctx.residual_norm(m, case["c"], _ptr(t["x"]), y=_ptr(t.get("y")), post_w=_ptr(t.get("post")) if case["y"] else None,
-                      gate=_ptr(t.get("gate")) if case["y"] else None, res_scale=0.5,
+    ctx.residual_norm(m, case["c"], _ptr(t["x"]), y=_ptr(t.get("y")), y_bf16=case["y"] == "bf16",
+                      post_w=_ptr(t.get("post")) if case["y"] else None, gate=_ptr(t.get("gate")) if case["y"] else None, res_scale=0.5,
                       norm="layer" if case["layer"] else "rms", norm_w=_ptr(t.get("w")), shift=_ptr(t.get("shift")),
                       scale=_ptr(t.get("scale")), group_rows=m // case["groups"], eps=EPS,
                       h=None if f8 else _ptr(s.out), q=_ptr(s.q) if f8 else None, s=_ptr(s.s) if f8 else None)
@@ -316,12 +334,12 @@ def work(case):
         c = case["c"]
         out = m * c + 4 * m * -(-c // 128) if case["out"] == "f8" else 4 * m * c
         vectors = 4 * c * (case["groups"] * (case["gate"] + 2 * case["mod"]) + case["post"] + (not case["layer"]))
-        return {"bytes": 4 * m * c * (3 if case["y"] else 1) + out + vectors, "flops": 10 * m * c}
+        return {"bytes": m * c * {"f32": 12, "bf16": 10, "": 4}[case["y"]] + out + vectors, "flops": 10 * m * c}
     k = case["k"]
     x = m * k + 4 * m * -(-k // 128) if case["x"] == "f8" else 4 * m * k
     if op == "linear":
         n = case["n"]
-        out = 4 * m * n * (1 if case["epi"] == "store" else 2)
+        out = m * n * (2 if case["out"] == "bf16" else 4 if case["epi"] == "store" else 8)
         return {"bytes": x + n * k + out + 4 * n, "flops": 2 * m * n * k}
     f = case["f"]
     out = m * f + 4 * m * -(-f // 128) if case["out"] == "f8" else 4 * m * f
