@@ -20,10 +20,11 @@ HEADER = os.path.join(os.path.dirname(HERE), "include", "anima.h")
 ANIMA_OK = 0
 PREC_BF16 = 0
 PREC_FP32 = 1
-W_BF16, W_I8, W_W4, W_F32, W_F32S3 = 0, 1, 2, 3, 4
+W_BF16, W_I8, W_W4, W_F32, W_F32S3, W_F8 = 0, 1, 2, 3, 4, 5
 W4_GRID_SCRATCH, W4_IN_GEMM = 0, 1
 ACT = {"none": 0, "gelu": 1, "silu": 2}
 EPI_STORE, EPI_RESID, EPI_GATED = 0, 1, 2
+NORM = {"rms": 0, "layer": 1}
 EW = {"silu_mul": 0, "add": 1, "silu": 2, "copy": 3}
 
 _i64 = ctypes.c_int64
@@ -74,7 +75,8 @@ class LinearDesc(ctypes.Structure):
                 ("xq", _vp), ("xs", _vp), ("out", _vp), ("ldc", _i64), ("alpha", ctypes.c_float),
                 ("act", ctypes.c_int), ("epilogue", ctypes.c_int), ("gate", _vp), ("gate_off", _i64),
                 ("acc_out", _vp), ("add", _vp), ("ld_add", _i64), ("lora_xa", _vp), ("ld_lora_xa", _i64),
-                ("lora_b", _vp), ("lora_r", ctypes.c_int), ("lora_cols", ctypes.c_int)]
+                ("lora_b", _vp), ("lora_r", ctypes.c_int), ("lora_cols", ctypes.c_int), ("precision", ctypes.c_int),
+                ("out_bf16", ctypes.c_int)]
 
 
 SAMPLER = {"euler": 0, "euler_a": 1, "dpmpp_2m": 2, "er_sde": 3}
@@ -101,9 +103,23 @@ class QkvDesc(ctypes.Structure):
                 ("q_norm", _vp), ("q_prep", _vp), ("q_scale", ctypes.c_float)]
 
 
+class GluDesc(ctypes.Structure):
+    _fields_ = [("M", _i64), ("gate", ctypes.POINTER(Weight)), ("up", ctypes.POINTER(Weight)), ("x", _vp), ("xq", _vp),
+                ("xs", _vp), ("ldx", _i64), ("act", ctypes.c_int), ("out", _vp), ("ldc", _i64), ("out_q", _vp),
+                ("out_s", _vp), ("precision", ctypes.c_int)]
+
+
+class ResNormDesc(ctypes.Structure):
+    _fields_ = [("rows", _i64), ("cols", ctypes.c_int), ("x", _vp), ("ldx", _i64), ("y", _vp), ("ldy", _i64),
+                ("post_w", _vp), ("gate", _vp), ("gate_ld", _i64), ("res_scale", ctypes.c_float), ("norm", ctypes.c_int),
+                ("norm_w", _vp), ("shift", _vp), ("scale", _vp), ("mod_ld", _i64), ("group_rows", _i64),
+                ("eps", ctypes.c_float), ("h", _vp), ("ldh", _i64), ("q", _vp), ("s", _vp),
+                ("y_bf16", ctypes.c_int)]
+
+
 ABI_STRUCTS = {"anima_attn_desc": AttnDesc, "anima_linear_desc": LinearDesc, "anima_weight": Weight,
                "anima_sampler_desc": SamplerDesc, "anima_conv_desc": ConvDesc, "anima_limits": Limits,
-               "anima_qkv_desc": QkvDesc}
+               "anima_qkv_desc": QkvDesc, "anima_glu_desc": GluDesc, "anima_resnorm_desc": ResNormDesc}
 
 
 def abi_mismatches(L):
@@ -189,6 +205,10 @@ def lib():
         L.anima_conv3x3.argtypes = [_vp, ctypes.POINTER(ConvDesc)]
         L.anima_channel_norm.argtypes = [_vp, _vp, _vp, _vp, _i64, ctypes.c_int, ctypes.c_int]
         L.anima_fill_random.argtypes = [_vp, _vp, _i64, ctypes.c_int, ctypes.c_uint64, ctypes.c_float, ctypes.c_float]
+        L.anima_quant_rows_f8.argtypes = [_vp, _vp, ctypes.c_int, _i64, ctypes.c_int, _i64, _vp, _vp]
+        L.anima_weight_quant_f8.argtypes = [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp]
+        L.anima_linear_glu.argtypes = [_vp, P(GluDesc)]
+        L.anima_residual_norm.argtypes = [_vp, P(ResNormDesc)]
         L.anima_graph_begin.argtypes = [_vp]
         L.anima_graph_end.argtypes = [_vp, P(_vp)]
         L.anima_graph_launch.argtypes = [_vp, _vp]
@@ -440,8 +460,8 @@ class Context:
 
     def linear(self, W, M, out, *, x=None, ldx=0, x_rotated=True, xq=None, xs=None, ldc=0, alpha=0.0, act="none",
                epilogue=EPI_STORE, gate=None, gate_off=0, acc_out=None, add=None, ld_add=0, lora_xa=None,
-               ld_lora_xa=0, lora_b=None, lora_r=0, lora_cols=0):
-        """anima_linear; lora_xa / lora_b / lora_r: the LoRA delta's factors for the quantized
+               ld_lora_xa=0, lora_b=None, lora_r=0, lora_cols=0, precision=PREC_BF16, out_bf16=False):
+        """anima_linear; precision, out_bf16: of f8 weights (sums in 32 bits; bf16 rows out); lora_xa / lora_b / lora_r: the LoRA delta's factors for the quantized
         GEMM's epilogue (A products [M][ld_lora_xa] fp32, B as three bf16 planes [3][N][lora_r]);
         lora_cols > 0: block-diagonal ranks, column n reading xa columns (n // lora_cols) * lora_r
         + k."""
@@ -449,7 +469,7 @@ class Context:
                        xs=_ptr(xs), out=_ptr(out), ldc=ldc, alpha=alpha, act=ACT[act] if isinstance(act, str) else act,
                        epilogue=epilogue, gate=_ptr(gate), gate_off=gate_off, acc_out=_ptr(acc_out), add=_ptr(add),
                        ld_add=ld_add, lora_xa=_ptr(lora_xa), ld_lora_xa=ld_lora_xa, lora_b=_ptr(lora_b),
-                       lora_r=lora_r, lora_cols=lora_cols)
+                       lora_r=lora_r, lora_cols=lora_cols, precision=precision, out_bf16=int(out_bf16))
         return self._check(lib().anima_linear(self.h, ctypes.byref(d)))
 
     def linear_qkv(self, W, M, out, *, B, L, H, k_norm=None, rope_cs=None, rope_sin_off=0, kv_prep=None, eps=1e-6,
@@ -472,6 +492,34 @@ class Context:
     def weight_unpack_w4(self, W, grid):
         """The int8 grid [N][K] of a W4 weight (anima_weight_unpack_w4)."""
         return self._check(lib().anima_weight_unpack_w4(self.h, ctypes.byref(W), _ptr(grid)))
+
+    def quant_rows_f8(self, x, M, K, q, s, *, ldx=0, bf16=False):
+        """anima_quant_rows_f8: fp32 (bf16) rows to e4m3 rows q[M][K] and scales s[ceil(K/128)][M]."""
+        return self._check(lib().anima_quant_rows_f8(self.h, _ptr(x), int(bf16), M, K, ldx, _ptr(q), _ptr(s)))
+
+    def weight_quant_f8(self, w, N, K, q, scale, *, bf16=True):
+        """anima_weight_quant_f8: a bf16 (fp32) weight to the data and block scales of a W_F8 weight."""
+        return self._check(lib().anima_weight_quant_f8(self.h, _ptr(w), int(bf16), N, K, _ptr(q), _ptr(scale)))
+
+    def linear_glu(self, gate, up, M, *, x=None, xq=None, xs=None, ldx=0, act="silu", out=None, ldc=0, out_q=None,
+                   out_s=None, precision=PREC_BF16):
+        """anima_linear_glu: act(x W_gate^T) * (x W_up^T) of two W_F8 weights, from fp32 rows x or e4m3 rows
+        xq, xs, into fp32 rows out or e4m3 rows out_q, out_s."""
+        d = GluDesc(M=M, gate=ctypes.pointer(gate), up=ctypes.pointer(up), x=_ptr(x), xq=_ptr(xq), xs=_ptr(xs), ldx=ldx,
+                    act=ACT[act] if isinstance(act, str) else act, out=_ptr(out), ldc=ldc, out_q=_ptr(out_q),
+                    out_s=_ptr(out_s), precision=precision)
+        return self._check(lib().anima_linear_glu(self.h, ctypes.byref(d)))
+
+    def residual_norm(self, rows, cols, x, *, ldx=0, y=None, ldy=0, y_bf16=False, post_w=None, gate=None, gate_ld=0, res_scale=0.0,
+                      norm="rms", norm_w=None, shift=None, scale=None, mod_ld=0, group_rows=0, eps=1e-6, h=None, ldh=0,
+                      q=None, s=None):
+        """anima_residual_norm: x += res_scale * gate * post(y) in place, then the norm of x (norm "rms" /
+        "layer", norm_w, shift / scale) as fp32 rows h and / or e4m3 rows q, s."""
+        d = ResNormDesc(rows=rows, cols=cols, x=_ptr(x), ldx=ldx, y=_ptr(y), ldy=ldy, post_w=_ptr(post_w), gate=_ptr(gate),
+                        gate_ld=gate_ld, res_scale=res_scale, norm=NORM[norm] if isinstance(norm, str) else norm,
+                        norm_w=_ptr(norm_w), shift=_ptr(shift), scale=_ptr(scale), mod_ld=mod_ld, group_rows=group_rows,
+                        eps=eps, h=_ptr(h), ldh=ldh, q=_ptr(q), s=_ptr(s), y_bf16=int(y_bf16))
+        return self._check(lib().anima_residual_norm(self.h, ctypes.byref(d)))
 
     def split3_bf16(self, src, dst, n):
         return self._check(lib().anima_split3_bf16(self.h, _ptr(src), _ptr(dst), n))

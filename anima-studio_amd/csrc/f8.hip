@@ -1,0 +1,608 @@
+// The e4m3 operators for gfx950: rows and weights to 8-bit floating point with a scale per block of 128,
+// the products of such rows and weights, the gated half of a feed-forward block, and the residual / norm
+// seam that leaves e4m3 rows.  No reference counterpart (see anima.h).
+//
+// Quantization of a block with largest magnitude a: a' = max(a, 2^-100), scale = a' / 448,
+// value = e4m3(x * (448 / a')).  The maximum is taken on the bit patterns of |x| (as unsigned integers they
+// order like the values, an infinity above every finite value and NaN above that), so a NaN reaches the
+// scale.  |x| * (448 / a') is at most 448 (1 + 2^-22), which rounds to 448: no clamp.
+//
+// Products: D = sum over the 128 k of a block on the matrix cores, then acc = fma(xs * scale, D, acc) in fp32.
+// ANIMA_PREC_BF16 takes v_mfma_f32_16x16x128_f8f6f4, exactly one block of k: within each eight k it aligns the
+// products to the largest and drops what lies 2^-13 below (measured: 2^16 + 2^3 is exact, 2^16 + 2^2 gives 2^16;
+// relative L2 error of a block of normal values 1.5e-5, mean 1e-7), between the eights it adds in 32 bits.
+// ANIMA_PREC_FP32 widens e4m3 to bf16 (exact: 4 significant bits) and takes v_mfma_f32_16x16x32_bf16, whose
+// products of such values are exact and sums 32 bits (error of a block 9e-9), at half the rate.  The weight is
+// the first operand, so D's rows are outputs n and its columns rows m of x: a lane holds four consecutive n of
+// one m, and its xs is one value.
+#include <cmath>
+
+#include "common.h"
+#include "f8_args.h"
+#include "internal.h"
+
+namespace anima {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float F8_TOP = 448.0f;                     // largest e4m3 value
+constexpr uint32_t F8_TINY = (127u - 100u) << 23;    // bits of 2^-100
+
+struct F8Args {
+  const uint8_t* xq;  // e4m3 rows, ldx bytes apart, and xs [KB][M]; or fp32 rows x, ldx floats apart
+  const float* xs;
+  const float* x;
+  int64_t ldx;
+  const uint8_t* w;   // [N][K], ws [ceil(N/128)][KB]; GLU: the gate's
+  const float* ws;
+  const float* bias;
+  const uint8_t* w2;  // GLU: the up projection
+  const float* ws2;
+  const float* bias2;
+  float* out;
+  int64_t ldc;
+  float alpha;
+  int act, epi;
+  const float* gate;  // [N]
+  const float* add;
+  int64_t ld_add;
+  int M, N, K, KB;
+  int vec;            // four columns of out, add, bias and gate at a time
+  int obf;            // out is bf16 rows
+};
+
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+
+// A block's scale and the factor its values are multiplied with, from the bits of its largest magnitude.
+__device__ __forceinline__ void f8_scale(uint32_t amax, float& scale, float& mul) {
+  const float a = __builtin_bit_cast(float, umax(amax, F8_TINY));
+  scale = a / F8_TOP;
+  mul = F8_TOP / a;
+}
+
+// four values to e4m3 bytes, the first in the lowest
+__device__ __forceinline__ uint32_t f8_pack(f32x4 v, float mul) {
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * mul, v[1] * mul, 0, false);
+  r = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * mul, v[3] * mul, r, true);
+  return (uint32_t)r;
+}
+
+__device__ __forceinline__ uint32_t amax4(f32x4 v, uint32_t m) {
+  return umax(umax(abs_bits(v[0]), abs_bits(v[1])), umax(umax(abs_bits(v[2]), abs_bits(v[3])), m));
+}
+
+// maximum over the 32 lanes of a half wave
+__device__ __forceinline__ uint32_t half_umax(uint32_t v) {
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) v = umax(v, (uint32_t)__shfl_xor((int)v, s));
+  return v;
+}
+
+__device__ __forceinline__ float f8_act(float r, int act) {
+  if (act == ANIMA_ACT_GELU) return gelu_erf(r);
+  if (act == ANIMA_ACT_SILU) return silu_f(r);
+  return r;
+}
+
+// ------------------------------------------------------------------ rows and weights to e4m3
+
+__device__ __forceinline__ f32x4 ld4(const float* p) { return *(const f32x4*)p; }
+__device__ __forceinline__ f32x4 ld4(const uint16_t* p) {
+  const uint2 u = *(const uint2*)p;
+  return f32x4{__builtin_bit_cast(float, u.x << 16), __builtin_bit_cast(float, u.x & 0xffff0000u),
+               __builtin_bit_cast(float, u.y << 16), __builtin_bit_cast(float, u.y & 0xffff0000u)};
+}
+
+// A half wave per block of 128 columns (a lane: four of them), blocks in row order.
+template <class T>
+__global__ __launch_bounds__(256) void quant_rows_f8_kernel(const T* X, int64_t ldx, int M, int K, int KB, uint8_t* Q, float* S) {
+  const int l = threadIdx.x & 31;
+  const int64_t b = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int64_t m = b / KB;
+  const int kb = (int)(b - m * KB), k = kb * 128 + 4 * l;
+  const bool in = m < M && k < K;
+  const f32x4 v = in ? ld4(X + m * ldx + k) : f32x4{};
+  float scale, mul;
+  f8_scale(half_umax(amax4(v, 0)), scale, mul);
+  if (in) *(uint32_t*)(Q + m * K + k) = f8_pack(v, mul);
+  if (l == 0 && m < M) S[(int64_t)kb * M + m] = scale;
+}
+
+// A workgroup per 128 x 128 block: thread t holds columns 4 (t % 32) .. + 3 of rows t / 32 + 8 i.
+template <class T>
+__global__ __launch_bounds__(256) void weight_quant_f8_kernel(const T* W, int N, int K, int KB, uint8_t* Q, float* S) {
+  __shared__ uint32_t red[8];
+  const int kb = blockIdx.x % KB, nb = blockIdx.x / KB;
+  const int k = kb * 128 + 4 * (threadIdx.x & 31), n0 = nb * 128 + (threadIdx.x >> 5);
+  f32x4 v[16];
+  uint32_t a = 0;
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    const int n = n0 + 8 * i;
+    v[i] = n < N && k < K ? ld4(W + (int64_t)n * K + k) : f32x4{};
+    a = amax4(v[i], a);
+  }
+  a = half_umax(a);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; i++) a = umax(a, red[i]);
+  float scale, mul;
+  f8_scale(a, scale, mul);
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    const int n = n0 + 8 * i;
+    if (n < N && k < K) *(uint32_t*)(Q + (int64_t)n * K + k) = f8_pack(v[i], mul);
+  }
+  if (threadIdx.x == 0) S[(int64_t)nb * KB + kb] = scale;
+}
+
+// ------------------------------------------------------------------ residual + norm
+
+struct NormArgs {
+  float* x;
+  const void* y;
+  const float *post_w, *gate, *norm_w, *shift, *scale;
+  float* h;
+  uint8_t* q;
+  float* s;
+  int64_t ldx, ldy, ldh, gate_ld, mod_ld, group_rows;
+  float res_scale, eps;
+  int rows, cols, layer, y_bf16;
+};
+
+// Sum over the workgroup of T threads; `red` holds T / 64 floats, of its own for each use.
+template <int T>
+__device__ __forceinline__ float group_sum(float v, float* red) {
+  v = wave_sum(v);
+  if constexpr (T == 64) return v;
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0.0f;
+#pragma unroll
+  for (int i = 0; i < T / 64; i++) v += red[i];
+  return v;
+}
+
+// A workgroup per row, the row in registers: thread t holds the four-column groups t + T i, i < NV.
+template <int T, int NV>
+__global__ __launch_bounds__(T) void residual_norm_kernel(NormArgs a) {
+  __shared__ float red[3][T / 64];
+  const int t = threadIdx.x;
+  const int64_t row = blockIdx.x, grp = row / a.group_rows;
+  const float inv = 1.0f / (float)a.cols;
+  f32x4 x[NV];
+  float* xr = a.x + row * a.ldx;
+#pragma unroll
+  for (int i = 0; i < NV; i++) {
+    const int c = 4 * (t + T * i);
+    x[i] = c < a.cols ? ld4(xr + c) : f32x4{};
+  }
+  if (a.y) {
+    f32x4 y[NV];
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const int c = 4 * (t + T * i);
+      y[i] = f32x4{};
+      if (c < a.cols) y[i] = a.y_bf16 ? ld4((const uint16_t*)a.y + row * a.ldy + c) : ld4((const float*)a.y + row * a.ldy + c);
+    }
+    if (a.post_w) {
+      float ss = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NV; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) ss = __builtin_fmaf(y[i][e], y[i][e], ss);
+      const float r = 1.0f / sqrtf(group_sum<T>(ss, red[0]) * inv + a.eps);
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        const int c = 4 * (t + T * i);
+        if (c < a.cols) y[i] = y[i] * r * ld4(a.post_w + c);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const int c = 4 * (t + T * i);
+      if (c < a.cols) {
+        if (a.gate) y[i] = y[i] * ld4(a.gate + grp * a.gate_ld + c);
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[i][e] = __builtin_fmaf(a.res_scale, y[i][e], x[i][e]);
+        *(f32x4*)(xr + c) = x[i];
+      }
+    }
+  }
+  float mean = 0.0f;
+  if (a.layer) {
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; i++) s += (x[i][0] + x[i][1]) + (x[i][2] + x[i][3]);
+    mean = group_sum<T>(s, red[1]) * inv;
+  }
+  float ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; i++) {
+    const int c = 4 * (t + T * i);
+    if (c < a.cols) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        x[i][e] -= mean;
+        ss = __builtin_fmaf(x[i][e], x[i][e], ss);
+      }
+    }
+  }
+  const float r = 1.0f / sqrtf(group_sum<T>(ss, red[2]) * inv + a.eps);
+#pragma unroll
+  for (int i = 0; i < NV; i++) {
+    const int c = 4 * (t + T * i);
+    const bool in = c < a.cols;
+    f32x4 h = x[i] * r;
+    if (in) {
+      if (a.norm_w) h = h * ld4(a.norm_w + c);
+      if (a.scale) {
+        const f32x4 sc = ld4(a.scale + grp * a.mod_ld + c), sh = ld4(a.shift + grp * a.mod_ld + c);
+#pragma unroll
+        for (int e = 0; e < 4; e++) h[e] = __builtin_fmaf(h[e], 1.0f + sc[e], sh[e]);
+      }
+      if (a.h) *(f32x4*)(a.h + row * a.ldh + c) = h;
+    }
+    if (a.q) {  // 32 lanes hold one block of 128 columns (zeros past the row)
+      float scale, mul;
+      f8_scale(half_umax(amax4(in ? h : f32x4{}, 0)), scale, mul);
+      if (in) {
+        *(uint32_t*)(a.q + row * a.cols + c) = f8_pack(h, mul);
+        if ((t & 31) == 0) a.s[(int64_t)(c >> 7) * a.rows + row] = scale;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ products
+
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+
+// eight e4m3 values as bf16
+__device__ __forceinline__ bf16x8 widen8(int lo, int hi) {
+  const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true),
+                 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+  return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// a fragment of mfma_f8 as four of v_mfma_f32_16x16x32_bf16 (any order of k that both operands share will do)
+struct Wide {
+  bf16x8 v[4];
+};
+__device__ __forceinline__ Wide widen(i32x8 a) {
+  Wide w;
+#pragma unroll
+  for (int i = 0; i < 4; i++) w.v[i] = widen8(a[2 * i], a[2 * i + 1]);
+  return w;
+}
+__device__ __forceinline__ f32x4 mfma_wide(const Wide& a, const Wide& b) {
+  f32x4 d{};
+#pragma unroll
+  for (int i = 0; i < 4; i++) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[i], b.v[i], d, 0, 0, 0);
+  return d;
+}
+
+__device__ __forceinline__ f32x4 fma4(float s, f32x4 d, f32x4 c) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) c[e] = __builtin_fmaf(s, d[e], c[e]);
+  return c;
+}
+
+__device__ __forceinline__ uint32_t bf16_bits(float v) { return __builtin_bit_cast(uint16_t, to_bf16(v)); }
+
+// Columns n .. n + 3 of row m of a linear's output from their sums.
+__device__ __forceinline__ void f8_store(const F8Args& a, int m, int n, f32x4 r) {
+  if (m >= a.M) return;
+  const int64_t at = (int64_t)m * a.ldc + n;
+  float* o = a.out + at;
+  uint16_t* ob = (uint16_t*)a.out + at;
+  const float* add = a.add ? a.add + (int64_t)m * a.ld_add + n : nullptr;
+  r = r * a.alpha;
+  if (a.vec) {
+    if (n >= a.N) return;
+    if (a.bias) r = r + ld4(a.bias + n);
+    if (add) r = r + ld4(add);
+#pragma unroll
+    for (int e = 0; e < 4; e++) r[e] = f8_act(r[e], a.act);
+    if (a.epi == ANIMA_EPI_RESID) {
+      r = r + ld4(o);
+    } else if (a.epi == ANIMA_EPI_GATED) {
+      const f32x4 g = ld4(a.gate + n), c = ld4(o);
+#pragma unroll
+      for (int e = 0; e < 4; e++) r[e] = __builtin_fmaf(g[e], r[e], c[e]);
+    }
+    if (a.obf) *(uint2*)ob = make_uint2(bf16_bits(r[0]) | bf16_bits(r[1]) << 16, bf16_bits(r[2]) | bf16_bits(r[3]) << 16);
+    else *(f32x4*)o = r;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    if (n + e >= a.N) return;
+    float v = r[e];
+    if (a.bias) v += a.bias[n + e];
+    if (add) v += add[e];
+    v = f8_act(v, a.act);
+    if (a.epi == ANIMA_EPI_RESID) v += o[e];
+    else if (a.epi == ANIMA_EPI_GATED) v = __builtin_fmaf(a.gate[n + e], v, o[e]);
+    if (a.obf) ob[e] = (uint16_t)bf16_bits(v);
+    else o[e] = v;
+  }
+}
+
+// Columns n .. n + 3 of row m of h = act(g + b_gate) * (u + b_up); zeros past the row.
+__device__ __forceinline__ f32x4 f8_glu(const F8Args& a, int n, f32x4 g, f32x4 u) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const bool in = n + e < a.N;
+    const float gv = g[e] + (a.bias && in ? a.bias[n + e] : 0.0f), uv = u[e] + (a.bias2 && in ? a.bias2[n + e] : 0.0f);
+    g[e] = f8_act(gv, a.act) * uv;
+  }
+  return g;
+}
+
+__device__ __forceinline__ void f8_glu_store(const F8Args& a, int m, int n, f32x4 h) {
+  if (m >= a.M || n >= a.N) return;
+  float* o = a.out + (int64_t)m * a.ldc + n;
+  if (a.vec) {
+    *(f32x4*)o = h;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; e++)
+    if (n + e < a.N) o[e] = h[e];
+}
+
+// f8_skinny: 16 outputs of 16 rows per workgroup, up to 8 waves that share the blocks of k; operands straight
+// from memory into the matrix cores' registers (a lane: 32 consecutive k of one row), the waves' sums
+// added through LDS in wave order.  QX: fp32 rows, each wave quantizing the blocks that it multiplies.  Sums in
+// 32 bits whatever the precision asked for: these products wait for the weight's bytes.
+constexpr int SKW = 8;
+template <bool QX, bool GLU>
+__global__ __launch_bounds__(64 * SKW) void f8_skinny(F8Args a) {
+  constexpr int TT = GLU ? 2 : 1;
+  __shared__ f32x4 part[SKW][TT][64];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, nw = blockDim.x >> 6;
+  const int r = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16, m = m0 + r;
+  const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w + (int64_t)n0 * a.K), (short)0,
+                                                                     min(16, a.N - n0) * a.K, 0x00020000);
+  __amdgpu_buffer_rsrc_t rw2 = rw, rx = rw;
+  if constexpr (GLU)
+    rw2 = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w2 + (int64_t)n0 * a.K), (short)0, min(16, a.N - n0) * a.K, 0x00020000);
+  if constexpr (!QX)
+    rx = __builtin_amdgcn_make_buffer_rsrc((void*)(a.xq + (int64_t)m0 * a.ldx), (short)0,
+                                           (min(16, a.M - m0) - 1) * (int)a.ldx + a.K, 0x00020000);
+  const float* xrow = QX ? a.x + (int64_t)min(m, a.M - 1) * a.ldx : nullptr;
+  const float* ws = a.ws + (int64_t)(n0 >> 7) * a.KB;
+  const float* ws2 = GLU ? a.ws2 + (int64_t)(n0 >> 7) * a.KB : nullptr;
+  constexpr uint32_t PAST = 0x80000000u;  // an offset past every resource's end: reads as zero
+  const auto frag = [&](__amdgpu_buffer_rsrc_t rs, uint32_t off, int k) {
+    const u32x4 lo = __builtin_amdgcn_raw_buffer_load_b128(rs, k < a.K ? off + k : PAST, 0, 0);
+    const u32x4 hi = __builtin_amdgcn_raw_buffer_load_b128(rs, k + 16 < a.K ? off + k + 16 : PAST, 0, 0);
+    return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+  };
+  f32x4 acc[TT];
+#pragma unroll
+  for (int t = 0; t < TT; t++) acc[t] = f32x4{};
+  for (int kb = wave; kb < a.KB; kb += nw) {
+    const int k = kb * 128 + 32 * g;
+    const i32x8 w = frag(rw, r * a.K, k);
+    i32x8 w2 = w, x;
+    if constexpr (GLU) w2 = frag(rw2, r * a.K, k);
+    float sx;
+    if constexpr (QX) {
+      f32x4 v[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = m < a.M && k + 4 * i < a.K ? ld4(xrow + k + 4 * i) : f32x4{};
+      uint32_t am = 0;
+#pragma unroll
+      for (int i = 0; i < 8; i++) am = amax4(v[i], am);
+      am = umax(am, (uint32_t)__shfl_xor((int)am, 16));
+      am = umax(am, (uint32_t)__shfl_xor((int)am, 32));
+      float mul;
+      f8_scale(am, sx, mul);
+#pragma unroll
+      for (int i = 0; i < 8; i++) x[i] = (int)f8_pack(v[i], mul);
+    } else {
+      x = frag(rx, r * (uint32_t)a.ldx, k);
+      sx = a.xs[(int64_t)kb * a.M + min(m, a.M - 1)];
+    }
+    const Wide xw = widen(x);
+    acc[0] = fma4(sx * ws[kb], mfma_wide(widen(w), xw), acc[0]);
+    if constexpr (GLU) acc[1] = fma4(sx * ws2[kb], mfma_wide(widen(w2), xw), acc[1]);
+  }
+#pragma unroll
+  for (int t = 0; t < TT; t++) part[wave][t][lane] = acc[t];
+  __syncthreads();
+  if (tid >= 64) return;
+#pragma unroll
+  for (int t = 0; t < TT; t++)
+    for (int w = 1; w < nw; w++) acc[t] = acc[t] + part[w][t][lane];
+  const int n = n0 + 4 * g;
+  if constexpr (GLU) f8_glu_store(a, m, n, f8_glu(a, n, acc[0], acc[1]));
+  else f8_store(a, m, n, acc[0]);
+}
+
+// ------------------------------------------------------------------ host
+
+namespace {
+
+// Makes the context's device the current one for a call's launches.
+struct OnDevice {
+  int before = -1;
+  explicit OnDevice(const anima_ctx* c) {
+    if (hipGetDevice(&before) != hipSuccess || before == c->device || hipSetDevice(c->device) != hipSuccess) before = -1;
+  }
+  ~OnDevice() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
+
+int refused(anima_ctx* c, int rc, const char* msg) { return fail(c, rc, "%s", msg); }
+
+constexpr int64_t GRID_Y = 65535;
+
+}  // namespace
+
+int quant_rows_f8_launch(anima_ctx* c, const void* x, int x_bf16, int64_t M, int K, int64_t ldx, uint8_t* q, float* s) {
+  char msg[256];
+  if (int rc = check_quant_rows_f8(x, x_bf16, M, K, ldx, q, s, F8Msg{msg, sizeof msg})) return refused(c, rc, msg);
+  if (M == 0) return ANIMA_OK;
+  OnDevice on(c);
+  const int KB = (K + 127) / 128;
+  const int64_t groups = (M * KB + 7) / 8, ld = ldx ? ldx : K;
+  if (groups > 0x7fffffff) return fail(c, ANIMA_E_UNSUPPORTED, "anima_quant_rows_f8: %lld blocks", (long long)(M * KB));
+  Launch L(c, x_bf16 ? "quant.f8.bf16" : "quant.f8", 0.0, (double)M * K * (x_bf16 ? 3 : 5));
+  if (x_bf16)
+    hipLaunchKernelGGL(quant_rows_f8_kernel<uint16_t>, dim3((unsigned)groups), dim3(256), 0, c->stream, (const uint16_t*)x, ld, (int)M, K,
+                       KB, q, s);
+  else
+    hipLaunchKernelGGL(quant_rows_f8_kernel<float>, dim3((unsigned)groups), dim3(256), 0, c->stream, (const float*)x, ld, (int)M, K, KB, q, s);
+  return L.end();
+}
+
+int weight_quant_f8_launch(anima_ctx* c, const void* w, int w_bf16, int N, int K, uint8_t* q, float* scale) {
+  char msg[256];
+  if (int rc = check_weight_quant_f8(w, w_bf16, N, K, q, scale, F8Msg{msg, sizeof msg})) return refused(c, rc, msg);
+  OnDevice on(c);
+  const int KB = (K + 127) / 128;
+  const int64_t blocks = (int64_t)((N + 127) / 128) * KB;
+  if (blocks > 0x7fffffff) return fail(c, ANIMA_E_UNSUPPORTED, "anima_weight_quant_f8: %lld blocks", (long long)blocks);
+  Launch L(c, "weight_quant.f8", 0.0, (double)N * K * (w_bf16 ? 3 : 5));
+  if (w_bf16)
+    hipLaunchKernelGGL(weight_quant_f8_kernel<uint16_t>, dim3((unsigned)blocks), dim3(256), 0, c->stream, (const uint16_t*)w, N, K, KB, q,
+                       scale);
+  else
+    hipLaunchKernelGGL(weight_quant_f8_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, c->stream, (const float*)w, N, K, KB, q, scale);
+  return L.end();
+}
+
+int residual_norm_launch(anima_ctx* c, const anima_resnorm_desc* d) {
+  char msg[256];
+  if (int rc = check_residual_norm(d, F8Msg{msg, sizeof msg})) return refused(c, rc, msg);
+  if (d->rows == 0) return ANIMA_OK;
+  OnDevice on(c);
+  const int64_t C = d->cols;
+  const auto ld = [&](int64_t v) { return v ? v : C; };
+  const NormArgs a{d->x,
+                   d->y,
+                   d->post_w,
+                   d->gate,
+                   d->norm_w,
+                   d->shift,
+                   d->scale,
+                   d->h,
+                   d->q,
+                   d->s,
+                   ld(d->ldx),
+                   ld(d->ldy),
+                   ld(d->ldh),
+                   ld(d->gate_ld),
+                   ld(d->mod_ld),
+                   d->group_rows ? d->group_rows : d->rows,
+                   d->res_scale != 0.0f ? d->res_scale : 1.0f,
+                   d->eps,
+                   (int)d->rows,
+                   d->cols,
+                   d->norm == ANIMA_NORM_LAYER,
+                   d->y_bf16};
+  const dim3 grid((unsigned)d->rows);
+  Launch L(c, "residual_norm", 0.0, (double)d->rows * C * ((d->y ? d->y_bf16 ? 10.0 : 12.0 : 4.0) + (d->h ? 4 : 0) + (d->q ? 1 : 0)));
+#define RN(T, NV) hipLaunchKernelGGL((residual_norm_kernel<T, NV>), grid, dim3(T), 0, c->stream, a)
+  if (C <= 256) RN(64, 1);
+  else if (C <= 512) RN(64, 2);
+  else if (C <= 1024) RN(64, 4);
+  else if (C <= 2048) RN(128, 4);
+  else if (C <= 4096) RN(256, 4);
+  else if (C <= 8192) RN(512, 4);
+  else RN(1024, 4);
+#undef RN
+  return L.end();
+}
+
+// The product's input as e4m3 rows: those given, or fp32 rows in `a` as they are.
+static void f8_input(F8Args& a, const anima_weight* W, const float* x, int64_t ldx, const int8_t* xq, const float* xs) {
+  a.xq = (const uint8_t*)xq;
+  a.xs = xs;
+  a.x = xq ? nullptr : x;
+  a.ldx = ldx ? ldx : W->K;
+  a.N = W->N;
+  a.K = W->K;
+  a.KB = (W->K + 127) / 128;
+}
+
+// The kernel for a product's sizes.
+template <bool GLU>
+static int f8_product(anima_ctx* c, const F8Args& a) {
+  const char* name = GLU ? "gemm.f8.glu.skinny" : "gemm.f8.skinny";
+  const int64_t mt = ((int64_t)a.M + 15) / 16;
+  if (mt > GRID_Y) return fail(c, ANIMA_E_UNSUPPORTED, "f8 product: M=%d", a.M);
+  Launch L(c, name, (GLU ? 4.0 : 2.0) * a.M * a.N * a.K, (double)a.N * a.K * (GLU ? 2 : 1));
+  const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)mt), block(64 * (a.KB < SKW ? a.KB : SKW));
+  if (a.x) hipLaunchKernelGGL((f8_skinny<true, GLU>), grid, block, 0, c->stream, a);
+  else hipLaunchKernelGGL((f8_skinny<false, GLU>), grid, block, 0, c->stream, a);
+  return L.end();
+}
+
+int linear_f8_launch(anima_ctx* c, const anima_linear_desc* d) {
+  char msg[256];
+  if (int rc = check_linear_f8(d, F8Msg{msg, sizeof msg})) return refused(c, rc, msg);
+  OnDevice on(c);
+  const anima_weight* W = d->W;
+  F8Args a{};
+  f8_input(a, W, d->x, d->ldx, d->xq, d->xs);
+  a.M = (int)d->M;
+  a.w = (const uint8_t*)W->w;
+  a.ws = W->scale;
+  a.bias = W->bias;
+  a.out = d->out;
+  a.ldc = d->ldc ? d->ldc : W->N;
+  a.alpha = d->alpha != 0.0f ? d->alpha : 1.0f;
+  a.act = d->act;
+  a.epi = d->epilogue;
+  a.gate = d->gate ? d->gate + d->gate_off : nullptr;
+  a.add = d->add;
+  a.ld_add = d->ld_add ? d->ld_add : W->N;
+  a.obf = d->out_bf16;
+  a.vec = a.N % 4 == 0 && a.ldc % 4 == 0 && f8_al(a.out, a.obf ? 8 : 16) && f8_al(a.bias, 16) && (!a.add || (a.ld_add % 4 == 0 && f8_al(a.add, 16))) &&
+          (a.epi != ANIMA_EPI_GATED || f8_al(a.gate, 16));
+  return f8_product<false>(c, a);
+}
+
+int linear_glu_launch(anima_ctx* c, const anima_glu_desc* d) {
+  char msg[256];
+  if (int rc = check_linear_glu(d, F8Msg{msg, sizeof msg})) return refused(c, rc, msg);
+  if (d->M == 0) return ANIMA_OK;
+  OnDevice on(c);
+  const anima_weight *G = d->gate, *U = d->up;
+  F8Args a{};
+  f8_input(a, G, d->x, d->ldx, d->xq, d->xs);
+  a.M = (int)d->M;
+  a.w = (const uint8_t*)G->w;
+  a.ws = G->scale;
+  a.bias = G->bias;
+  a.w2 = (const uint8_t*)U->w;
+  a.ws2 = U->scale;
+  a.bias2 = U->bias;
+  a.act = d->act;
+  a.out = d->out;
+  a.ldc = d->ldc ? d->ldc : a.N;
+  void* tmp = nullptr;
+  if (d->out_q) {  // fp32 rows first (pooled scratch), then their e4m3 rows
+    if (int rc = anima_alloc(c, (size_t)a.M * a.N * 4, &tmp)) return rc;
+    a.out = (float*)tmp;
+    a.ldc = a.N;
+  }
+  a.vec = a.N % 4 == 0 && a.ldc % 4 == 0 && f8_al(a.out, 16);
+  int rc = f8_product<true>(c, a);
+  if (tmp) {
+    if (rc == ANIMA_OK) rc = quant_rows_f8_launch(c, tmp, 0, a.M, a.N, 0, d->out_q, d->out_s);
+    anima_free(c, tmp);
+  }
+  return rc;
+}
+
+}  // namespace anima

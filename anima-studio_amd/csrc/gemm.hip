@@ -2731,6 +2731,7 @@ int linear_launch(anima_ctx* c, const anima_linear_desc* d, int64_t s3_plane) {
   }
   if (M == 0) return ANIMA_OK;
 
+  if (W->kind == ANIMA_W_F8) return linear_f8_launch(c, d);
   if (W->kind == ANIMA_W_F32S3) {
     // x: fp32 rows, or per-token int8 rows xq with their scales xs (y = xs[m] * (q W^T)[m])
     const bool q8 = d->xq != nullptr;

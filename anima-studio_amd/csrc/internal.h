@@ -150,4 +150,12 @@ int linear_grouped_bf16_launch(anima_ctx* c, int G, int64_t M, int N, int K, con
 int gemv_grouped_f32_launch(anima_ctx* c, int G, int N, int K, const float* x, int64_t x_gs, const float* w, int64_t w_gs,
                             float* y, int64_t y_gs, float alpha, int accumulate);
 
+// ---- kernel launchers (f8.hip)
+int quant_rows_f8_launch(anima_ctx* c, const void* x, int x_bf16, int64_t M, int K, int64_t ldx, uint8_t* q, float* s);
+int weight_quant_f8_launch(anima_ctx* c, const void* w, int w_bf16, int N, int K, uint8_t* q, float* scale);
+// (linear_launch has made the checks that every kind of weight shares)
+int linear_f8_launch(anima_ctx* c, const anima_linear_desc* d);
+int linear_glu_launch(anima_ctx* c, const anima_glu_desc* d);
+int residual_norm_launch(anima_ctx* c, const anima_resnorm_desc* d);
+
 }  // namespace anima

@@ -662,6 +662,26 @@ int anima_linear_qkv(anima_ctx* c, const anima_linear_desc* d, const anima_qkv_d
   return linear_qkv_launch(c, d, p);
 }
 
+int anima_quant_rows_f8(anima_ctx* c, const void* x, int x_bf16, int64_t M, int K, int64_t ldx, uint8_t* q, float* s) {
+  CHECK_CTX(c);
+  return quant_rows_f8_launch(c, x, x_bf16, M, K, ldx, q, s);
+}
+
+int anima_weight_quant_f8(anima_ctx* c, const void* w, int w_bf16, int N, int K, uint8_t* q, float* scale) {
+  CHECK_CTX(c);
+  return weight_quant_f8_launch(c, w, w_bf16, N, K, q, scale);
+}
+
+int anima_linear_glu(anima_ctx* c, const anima_glu_desc* d) {
+  CHECK_CTX(c);
+  return linear_glu_launch(c, d);
+}
+
+int anima_residual_norm(anima_ctx* c, const anima_resnorm_desc* d) {
+  CHECK_CTX(c);
+  return residual_norm_launch(c, d);
+}
+
 int anima_linear_grouped_bf16(anima_ctx* c, int G, int64_t M, int N, int K, const float* x, int64_t ldx,
                               int64_t x_gstride, const uint16_t* w, int64_t w_gstride, const float* bias,
                               int64_t bias_gstride, float* out, int64_t ldc, int64_t out_gstride) {
@@ -706,6 +726,7 @@ static const struct {
     ABI_FIELD(anima_linear_desc, acc_out), ABI_FIELD(anima_linear_desc, add), ABI_FIELD(anima_linear_desc, ld_add),
     ABI_FIELD(anima_linear_desc, lora_xa), ABI_FIELD(anima_linear_desc, ld_lora_xa), ABI_FIELD(anima_linear_desc, lora_b),
     ABI_FIELD(anima_linear_desc, lora_r), ABI_FIELD(anima_linear_desc, lora_cols),
+    ABI_FIELD(anima_linear_desc, precision), ABI_FIELD(anima_linear_desc, out_bf16),
     ABI_SIZE(anima_sampler_desc), ABI_FIELD(anima_sampler_desc, kind), ABI_FIELD(anima_sampler_desc, n),
     ABI_FIELD(anima_sampler_desc, x), ABI_FIELD(anima_sampler_desc, v), ABI_FIELD(anima_sampler_desc, v_uncond),
     ABI_FIELD(anima_sampler_desc, cfg), ABI_FIELD(anima_sampler_desc, sigma), ABI_FIELD(anima_sampler_desc, final_step),
@@ -724,6 +745,19 @@ static const struct {
     ABI_FIELD(anima_qkv_desc, k_norm), ABI_FIELD(anima_qkv_desc, rope_cs), ABI_FIELD(anima_qkv_desc, rope_sin_off),
     ABI_FIELD(anima_qkv_desc, eps), ABI_FIELD(anima_qkv_desc, kv_prep), ABI_FIELD(anima_qkv_desc, kv_prep_bytes),
     ABI_FIELD(anima_qkv_desc, q_norm), ABI_FIELD(anima_qkv_desc, q_prep), ABI_FIELD(anima_qkv_desc, q_scale),
+    ABI_SIZE(anima_glu_desc), ABI_FIELD(anima_glu_desc, M), ABI_FIELD(anima_glu_desc, gate),
+    ABI_FIELD(anima_glu_desc, up), ABI_FIELD(anima_glu_desc, x), ABI_FIELD(anima_glu_desc, xq),
+    ABI_FIELD(anima_glu_desc, xs), ABI_FIELD(anima_glu_desc, ldx), ABI_FIELD(anima_glu_desc, act),
+    ABI_FIELD(anima_glu_desc, out), ABI_FIELD(anima_glu_desc, ldc), ABI_FIELD(anima_glu_desc, out_q),
+    ABI_FIELD(anima_glu_desc, out_s), ABI_FIELD(anima_glu_desc, precision),
+    ABI_SIZE(anima_resnorm_desc), ABI_FIELD(anima_resnorm_desc, rows), ABI_FIELD(anima_resnorm_desc, cols),
+    ABI_FIELD(anima_resnorm_desc, x), ABI_FIELD(anima_resnorm_desc, ldx), ABI_FIELD(anima_resnorm_desc, y),
+    ABI_FIELD(anima_resnorm_desc, ldy), ABI_FIELD(anima_resnorm_desc, post_w), ABI_FIELD(anima_resnorm_desc, gate),
+    ABI_FIELD(anima_resnorm_desc, gate_ld), ABI_FIELD(anima_resnorm_desc, res_scale),
+    ABI_FIELD(anima_resnorm_desc, norm), ABI_FIELD(anima_resnorm_desc, norm_w), ABI_FIELD(anima_resnorm_desc, shift),
+    ABI_FIELD(anima_resnorm_desc, scale), ABI_FIELD(anima_resnorm_desc, mod_ld),
+    ABI_FIELD(anima_resnorm_desc, group_rows), ABI_FIELD(anima_resnorm_desc, eps), ABI_FIELD(anima_resnorm_desc, h),
+    ABI_FIELD(anima_resnorm_desc, ldh), ABI_FIELD(anima_resnorm_desc, q), ABI_FIELD(anima_resnorm_desc, s), ABI_FIELD(anima_resnorm_desc, y_bf16),
 };
 #undef ABI_FIELD
 #undef ABI_SIZE

@@ -105,8 +105,8 @@ int anima_timer_stop(anima_ctx* ctx, float* ms);
 
 /* ABI self-description, for bindings that restate the descriptor structs below (ctypes, FFI):
  * the byte offset of `field` in the struct named `type` -- "anima_attn_desc", "anima_linear_desc",
- * "anima_weight", "anima_sampler_desc", "anima_conv_desc", "anima_limits", "anima_qkv_desc" -- or the
- * struct's size when `field` is
+ * "anima_weight", "anima_sampler_desc", "anima_conv_desc", "anima_limits", "anima_qkv_desc",
+ * "anima_glu_desc", "anima_resnorm_desc" -- or the struct's size when `field` is
  * NULL; -1 for a name this library does not know.  No counterpart in the reference (its op layer
  * has no C ABI); it lets a binding refuse to load when its layout differs from the library's. */
 int64_t anima_abi_offset(const char* type, const char* field);
@@ -373,6 +373,9 @@ int anima_to_rgba(anima_ctx* ctx, const float* x, int64_t n, uint8_t* out);
                            cores as sum_{i+j<=2} x_i w_j with x split the same way on the fly, fp32
                            accumulation: fp32-level accuracy (not bit-identical to ANIMA_W_F32) at
                            ~1/3 of the fp32 matrix-core time.  K % 8 == 0.  The same LoRA matrices. */
+#define ANIMA_W_F8 5 /* e4m3 [N][K] + scale [ceil(N/128)][ceil(K/128)], one for each 128 x 128 block; the
+                        activations are e4m3 rows with one scale per 128 columns (anima_quant_rows_f8).
+                        K % 16 == 0.  No reference counterpart (its loader knows comfy_quant formats only) */
 #define ANIMA_ACT_NONE 0
 #define ANIMA_ACT_GELU 1 /* erf GELU (kernels.js:9-20) */
 #define ANIMA_ACT_SILU 2
@@ -384,7 +387,7 @@ int anima_to_rgba(anima_ctx* ctx, const float* x, int64_t n, uint8_t* out);
 typedef struct {
   int kind, N, K;
   const void* w;
-  const float* scale;      /* i8: weight_scale [N]; w4: weight_s_channel [N] */
+  const float* scale;      /* i8: weight_scale [N]; w4: weight_s_channel [N]; f8: the block scales */
   const uint8_t* srel;     /* w4: [N][K/16] fp8 e4m3 */
   const float* codebook;   /* w4: [16] */
   const float* bias;       /* [N] or NULL */
@@ -401,7 +404,10 @@ typedef struct {
   /* i8/w4: pre-quantized rotated activations (anima_quant_rows / anima_layernorm_mod); when set,
    * x is ignored.  f32s3 (split) weights take them in place of x as well (x NULL; K % 16 == 0,
    * ldx % 16 == 0 in bytes, xq 16-byte aligned): y = xs[m] * sum_k xq[m][k] W[n][k], the LoRA A
-   * product of a quantized linear over the int8 rows its GEMM reads, with the rotated A. */
+   * product of a quantized linear over the int8 rows its GEMM reads, with the rotated A.
+   * f8 weights: e4m3 rows (ldx bytes apart, 0 -> K, ldx % 16 == 0, 16-byte aligned) with xs
+   * [ceil(K/128)][M] as anima_quant_rows_f8 writes them; without xq the fp32 rows x (ldx % 4 == 0,
+   * 16-byte aligned) are quantized the same way by the call.  x_rotated is not read. */
   const int8_t* xq;
   const float* xs;
   float* out;
@@ -431,13 +437,25 @@ typedef struct {
   const uint16_t* lora_b;
   int lora_r;
   int lora_cols;
+  /* f8 weights only (0 otherwise).  precision: ANIMA_PREC_BF16 lets the 8-bit matrix instructions add the
+   * products, which keep 2^-13 of the largest of each eight (about 1.5e-5 of the result, far below a bf16
+   * rounding); ANIMA_PREC_FP32 adds them in 32 bits, at the rate of bf16 products.  out_bf16 = 1: out is
+   * bf16 rows (round to nearest even; out and ldc then address uint16 elements), store epilogue only. */
+  int precision;
+  int out_bf16;
 } anima_linear_desc;
 
 /* ops.linear (app/gpu/ops.js:48-66) -> matmulShader (gemm.js:166-280):
  * r = alpha * (x @ dec(W)^T); i8/w4: dec is the int8 grid and r is scaled by s_x[m] * s_w[n]
  * (W8A8: activations quantized per token after the ConvRot rotation); then + bias[n], act,
  * and the store / residual / gated-residual epilogue of gemm.js:186-192.
- * i8/w4 need K % 64 == 0 (and K <= 8192 when x is quantized here). */
+ * i8/w4 need K % 64 == 0 (and K <= 8192 when x is quantized here).
+ * f8: r = alpha * sum_b xs[b][m] scale[n / 128][b] * (sum of xq[m][k] w[n][k] over the 128 k of block b):
+ * each block's products summed on the matrix cores (see precision), the blocks added in fp32.  Any M and N;
+ * K % 16 == 0, K <= 2^20.  fp32 rows x are quantized as anima_quant_rows_f8 does, few of them inside the
+ * product's kernel, more in a pass before it (pooled scratch).  The order in which a result's blocks are
+ * added, and so its last bits, depends on the sizes.  No acc_out and no LoRA factors (`add` carries a
+ * delta). */
 int anima_linear(anima_ctx* ctx, const anima_linear_desc* desc);
 
 /* The stacked QKV projection of a DiT block with the attention's operand preparation in its
@@ -496,6 +514,82 @@ int anima_weight_unpack_w4(anima_ctx* ctx, const anima_weight* w4, int8_t* grid)
 #define ANIMA_W4_GRID_SCRATCH 0
 #define ANIMA_W4_IN_GEMM 1
 int anima_set_w4_path(anima_ctx* ctx, int path);
+
+/* ---------------------------------------------------------------- e4m3 rows and weights
+ * No reference counterpart.  8-bit floating point (e4m3: 4 exponent and 3 mantissa bits, no infinity,
+ * largest value 448) with one fp32 scale for each block of 128.  Of a block with largest magnitude a,
+ *   a' = max(a, 2^-100),  scale = a' / 448,  value = e4m3(x * (448 / a'))
+ * in fp32, every step rounded to nearest even; the block stands for scale * value, off by at most 2^-4 of
+ * each value (2^-10 scale below 2^-6 scale).  A NaN makes its block's scale and values NaN, an infinity the
+ * scale infinite: such a row's products are NaN. */
+
+/* Rows x[M] (fp32, or bf16 with x_bf16 = 1; ldx elements apart, 0 -> K) to e4m3 rows q[M][K] with a scale for
+ * every 128 columns, s[ceil(K/128)][M]: block-major, since a product's k step reads one block of many rows.
+ * K % 16 == 0; x and q 16-byte aligned, ldx a multiple of 16 bytes. */
+int anima_quant_rows_f8(anima_ctx* ctx, const void* x, int x_bf16, int64_t M, int K, int64_t ldx, uint8_t* q, float* s);
+/* A weight w[N][K] (fp32, or bf16 with w_bf16 = 1) to the data q[N][K] and scales [ceil(N/128)][ceil(K/128)]
+ * of an ANIMA_W_F8 weight, one scale per 128 x 128 block: a loader's conversion of a bf16 checkpoint. */
+int anima_weight_quant_f8(anima_ctx* ctx, const void* w, int w_bf16, int N, int K, uint8_t* q, float* scale);
+
+/* The first half of a gated feed-forward block (the gate / up linears and the silu_mul of
+ * app/models/qwen3.js:66-72) in one kernel:
+ *   h[m][n] = act(x W_gate^T + b_gate) * (x W_up^T + b_up)
+ * both products as anima_linear's of f8 weights, h as fp32 rows or as the e4m3 rows that the following
+ * product reads.  The two weights have equal N and K and biases of their own. */
+typedef struct {
+  int64_t M;
+  const anima_weight* gate;
+  const anima_weight* up;
+  const float* x;      /* fp32 rows, or */
+  const int8_t* xq;    /* e4m3 rows (then x is not read) with their scales, as anima_linear_desc's */
+  const float* xs;
+  int64_t ldx;         /* of x in floats, of xq in bytes; 0 -> K */
+  int act;             /* ANIMA_ACT_* of the gate */
+  float* out;          /* fp32 [M][ldc], or */
+  int64_t ldc;         /* 0 -> N */
+  uint8_t* out_q;      /* e4m3 [M][N] (N % 16 == 0, 16-byte aligned) with */
+  float* out_s;        /* [ceil(N/128)][M] */
+  int precision;       /* as anima_linear_desc's */
+} anima_glu_desc;
+int anima_linear_glu(anima_ctx* ctx, const anima_glu_desc* desc);
+
+/* The seam between two blocks of a transformer in one pass over the rows: the residual addition of a block's
+ * output y (with a norm of its own, a gate and a scale), and the next block's input norm.
+ *   x += res_scale * gate * post(y)               post(y) = y / sqrt(mean(y^2) + eps) * post_w, or y
+ *   h  = n(x) * norm_w * (1 + scale) + shift      n: RMSNorm or LayerNorm (no affine part of its own), eps
+ * Every factor is optional (NULL: left out; without y, x is only read and stays as it is).  Row r takes the
+ * gate and modulation vectors of group r / group_rows.  Sums in fp32.  h leaves as fp32 rows and / or as
+ * e4m3 rows q, s (as anima_quant_rows_f8 of those fp32 rows: the same values).  In the reference these are
+ * the residual epilogues of ops.linear, ops.rmsnorm and ops.layernormMod (app/gpu/ops.js:48-66, 111-137).
+ * cols % 4 == 0 (q: % 16), cols <= 16384; rows and vectors 16-byte aligned (bf16 y: 8), strides multiples of 4.
+ * h may be an fp32 y; other outputs overlap no input. */
+#define ANIMA_NORM_RMS 0
+#define ANIMA_NORM_LAYER 1
+typedef struct {
+  int64_t rows;
+  int cols;
+  float* x;             /* [rows][ldx], updated in place when y is given */
+  int64_t ldx;          /* (every stride here: 0 -> cols) */
+  const void* y;        /* [rows][ldy] fp32, or bf16 with y_bf16 = 1, or NULL */
+  int64_t ldy;
+  const float* post_w;  /* [cols] or NULL: no norm of y */
+  const float* gate;    /* [groups][gate_ld] or NULL */
+  int64_t gate_ld;
+  float res_scale;      /* 0 -> 1 */
+  int norm;             /* ANIMA_NORM_* */
+  const float* norm_w;  /* [cols] or NULL */
+  const float* shift;   /* [groups][mod_ld] or NULL (both or neither) */
+  const float* scale;
+  int64_t mod_ld;
+  int64_t group_rows;   /* 0: one group */
+  float eps;
+  float* h;             /* fp32 [rows][ldh] and / or */
+  int64_t ldh;
+  uint8_t* q;           /* e4m3 [rows][cols] with */
+  float* s;             /* [ceil(cols/128)][rows] */
+  int y_bf16;
+} anima_resnorm_desc;
+int anima_residual_norm(anima_ctx* ctx, const anima_resnorm_desc* desc);
 
 /* G independent small-M bf16-weight products in one launch, for the adaLN modulation linears of
  * timeCond (app/models/dit.js:196-225 runs one per block and kind, all on the same sigma):
