@@ -3,9 +3,10 @@
 // seam that leaves e4m3 rows.  No reference counterpart (see anima.h).
 //
 // Quantization of a block with largest magnitude a: a' = max(a, 2^-100), scale = a' / 448,
-// value = e4m3(x * (448 / a')).  The maximum is taken on the bit patterns of |x| (as unsigned integers they
+// value = e4m3(x * (448 * (1 / a'))).  The maximum is taken on the bit patterns of |x| (as unsigned integers they
 // order like the values, an infinity above every finite value and NaN above that), so a NaN reaches the
-// scale.  |x| * (448 / a') is at most 448 (1 + 2^-22), which rounds to 448: no clamp.
+// scale.  |x| * (448 * (1 / a')) is at most 448 (1 + 2^-21) (1 / a' has 22 bits at the least, as a subnormal of
+// the largest a'), which rounds to 448: no clamp.
 //
 // Products: D = sum over the 128 k of a block on the matrix cores, then acc = fma(xs * scale, D, acc) in fp32.
 // ANIMA_PREC_BF16 takes v_mfma_f32_16x16x128_f8f6f4, exactly one block of k: within each eight k it aligns the
@@ -59,7 +60,7 @@ __device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b 
 __device__ __forceinline__ void f8_scale(uint32_t amax, float& scale, float& mul) {
   const float a = __builtin_bit_cast(float, umax(amax, F8_TINY));
   scale = a / F8_TOP;
-  mul = F8_TOP / a;
+  mul = F8_TOP * (1.0f / a);
 }
 
 // four values to e4m3 bytes, the first in the lowest

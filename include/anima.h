@@ -518,7 +518,7 @@ int anima_set_w4_path(anima_ctx* ctx, int path);
 /* ---------------------------------------------------------------- e4m3 rows and weights
  * No reference counterpart.  8-bit floating point (e4m3: 4 exponent and 3 mantissa bits, no infinity,
  * largest value 448) with one fp32 scale for each block of 128.  Of a block with largest magnitude a,
- *   a' = max(a, 2^-100),  scale = a' / 448,  value = e4m3(x * (448 / a'))
+ *   a' = max(a, 2^-100),  scale = a' / 448,  value = e4m3(x * (448 * (1 / a')))
  * in fp32, every step rounded to nearest even; the block stands for scale * value, off by at most 2^-4 of
  * each value (2^-10 scale below 2^-6 scale).  A NaN makes its block's scale and values NaN, an infinity the
  * scale infinite: such a row's products are NaN. */

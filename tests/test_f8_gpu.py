@@ -74,7 +74,7 @@ def quant_ref(x):
             v = x[:, 128 * b:128 * b + 128]
             a = np.maximum(np.abs(v).max(1), TINY)  # (a NaN stays)
             s[b] = a / np.float32(448)
-            q[:, 128 * b:128 * b + 128] = to_e4m3(v * (np.float32(448) / a)[:, None])
+            q[:, 128 * b:128 * b + 128] = to_e4m3(v * (np.float32(448) * (np.float32(1) / a))[:, None])
     return q, s
 
 
@@ -208,7 +208,7 @@ def test_weight_quant(ctx, N, K, wide):
             v = vals[128 * i:128 * i + 128, 128 * j:128 * j + 128]
             a = max(np.abs(v).max(), TINY)
             assert gs[i, j] == a / np.float32(448)
-            assert np.array_equal(gq[128 * i:128 * i + 128, 128 * j:128 * j + 128], to_e4m3(v * (np.float32(448) / a)))
+            assert np.array_equal(gq[128 * i:128 * i + 128, 128 * j:128 * j + 128], to_e4m3(v * (np.float32(448) * (np.float32(1) / a))))
 
 
 # ------------------------------------------------------------------ products
