@@ -17,6 +17,7 @@
 // the first operand, so D's rows are outputs n and its columns rows m of x: a lane holds four consecutive n of
 // one m, and its xs is one value.
 #include <cmath>
+#include <cstdlib>
 
 #include "common.h"
 #include "f8_args.h"
@@ -51,6 +52,8 @@ struct F8Args {
   int M, N, K, KB;
   int vec;            // four columns of out, add, bias and gate at a time
   int obf;            // out is bf16 rows
+  uint8_t* oq;        // GLU: e4m3 rows [M][N] instead, and their scales
+  float* os;
 };
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
@@ -333,14 +336,26 @@ __device__ __forceinline__ void f8_store(const F8Args& a, int m, int n, f32x4 r)
   }
 }
 
-// Columns n .. n + 3 of row m of h = act(g + b_gate) * (u + b_up); zeros past the row.
-__device__ __forceinline__ f32x4 f8_glu(const F8Args& a, int n, f32x4 g, f32x4 u) {
+// The biases of columns n .. n + 3 of both projections.
+struct GluBias {
+  f32x4 g, u;
+};
+__device__ __forceinline__ GluBias f8_glu_bias(const F8Args& a, int n) {
+  GluBias b{};
 #pragma unroll
   for (int e = 0; e < 4; e++) {
-    const bool in = n + e < a.N;
-    const float gv = g[e] + (a.bias && in ? a.bias[n + e] : 0.0f), uv = u[e] + (a.bias2 && in ? a.bias2[n + e] : 0.0f);
-    g[e] = f8_act(gv, a.act) * uv;
+    if (a.bias && n + e < a.N) b.g[e] = a.bias[n + e];
+    if (a.bias2 && n + e < a.N) b.u[e] = a.bias2[n + e];
   }
+  return b;
+}
+
+// h = act(g + b_gate) * (u + b_up)
+__device__ __forceinline__ f32x4 f8_glu(const F8Args& a, const GluBias& b, f32x4 g, f32x4 u) {
+  g = g + b.g;
+  u = u + b.u;
+#pragma unroll
+  for (int e = 0; e < 4; e++) g[e] = f8_act(g[e], a.act) * u[e];
   return g;
 }
 
@@ -423,8 +438,222 @@ __global__ __launch_bounds__(64 * SKW) void f8_skinny(F8Args a) {
   for (int t = 0; t < TT; t++)
     for (int w = 1; w < nw; w++) acc[t] = acc[t] + part[w][t][lane];
   const int n = n0 + 4 * g;
-  if constexpr (GLU) f8_glu_store(a, m, n, f8_glu(a, n, acc[0], acc[1]));
+  if constexpr (GLU) f8_glu_store(a, m, n, f8_glu(a, f8_glu_bias(a, n), acc[0], acc[1]));
   else f8_store(a, m, n, acc[0]);
+}
+
+// f8_tile: one BM x BN output tile per workgroup (GLU: BN / 2 columns of each projection), waves of WM x WN.
+// A stage is one block of 128 k: BM rows of x, BN of the weight (128 bytes each) and BM scales, filled NST - 1
+// stages ahead by buffer_load ... lds.  LDS row r holds eight 16-byte units, unit u at slot u ^ (r % 8): a copy
+// (eight whole rows, 1 KiB) is contiguous in LDS as the instruction needs it, and eight consecutive rows' reads
+// of one unit touch every bank once.  Rows past M (N) lie past their resource's end and units past K are sent
+// there: they read as zero.  GLU: each 64 rows of the weight tile are 32 of the gate and the same 32 of the up
+// projection, so that a lane holds both values of an output.
+typedef __attribute__((address_space(3))) void f8_lds_t;
+#define F8_WAIT_VM(n) __builtin_amdgcn_s_waitcnt(((n) & 15) | (7 << 4) | (15 << 8) | (((n) >> 4) << 14))
+
+__device__ __forceinline__ void f8_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+__device__ __forceinline__ f32x4 mfma_f8(i32x8 a, i32x8 b) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, f32x4{}, 0, 0, 0, 0, 0, 0);
+}
+
+// a wave's copy of 64 x 16 (x 4) bytes into LDS
+__device__ __forceinline__ void f8_copy16(__amdgpu_buffer_rsrc_t rs, char* dst, uint32_t off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (f8_lds_t*)dst, 16, off, 0, 0, 0);
+}
+__device__ __forceinline__ void f8_copy4(__amdgpu_buffer_rsrc_t rs, char* dst, uint32_t off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (f8_lds_t*)dst, 4, off, 0, 0, 0);
+}
+
+template <int BM, int BN, int WM, int WN, int NST, bool WIDE, bool GLU>
+__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void f8_tile(F8Args a) {
+  constexpr int NWM = BM / WM, NW = NWM * (BN / WN), MT = WM / 16, NT = WN / 16;
+  constexpr int ST = (BM + BN) * 128 + BM * 4;            // bytes of a stage
+  constexpr int CPW = (BM + BN) / 8 / NW, SPW = BM / 64;  // copies per wave: rows; waves that copy 64 scales each
+  constexpr int FN = GLU ? BN / 2 : BN;                   // output columns of a tile
+  constexpr uint32_t PAST = 0x80000000u;
+  static_assert(CPW * NW * 8 == BM + BN && SPW <= NW && WN <= 64 && (!GLU || WN == 64), "copies and waves");
+  __shared__ __attribute__((aligned(1024))) char smem[NST * ST];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int r = lane & 15, g = lane >> 4;
+  const int ntn = (a.N + FN - 1) / FN, ntm = (a.M + BM - 1) / BM;
+  int tm, tn;
+  {
+    // XCD x takes a contiguous range of tiles (dispatch is round-robin over the 8 XCDs), in groups of 8 row
+    // tiles, column-major inside a group: the tiles in flight on one XCD share rows of both operands in its L2
+    const int total = ntn * ntm, q = total >> 3, rem = total & 7, x = blockIdx.x & 7;
+    const int t = x * q + min(x, rem) + (int)(blockIdx.x >> 3);
+    const int grp = t / (8 * ntn), row0 = 8 * grp, gm = min(8, ntm - row0), local = t - grp * 8 * ntn;
+    tn = local / gm;
+    tm = row0 + (local - tn * gm);
+  }
+  const int bm = tm * BM, bn = tn * FN, K = a.K, KB = a.KB;
+  const int wm = (wave % NWM) * WM, wn = (wave / NWM) * WN;
+
+  const int mrows = min(BM, a.M - bm), nrows = min(FN, a.N - bn);
+  const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc((void*)(a.xq + (int64_t)bm * a.ldx), (short)0,
+                                                                     (mrows - 1) * (int)a.ldx + K, 0x00020000);
+  const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w + (int64_t)bn * K), (short)0, nrows * K, 0x00020000);
+  const __amdgpu_buffer_rsrc_t rw2 =
+      GLU ? __builtin_amdgcn_make_buffer_rsrc((void*)(a.w2 + (int64_t)bn * K), (short)0, nrows * K, 0x00020000) : rw;
+  const int unit = (lane & 7) ^ (lane >> 3);
+  uint32_t voff[CPW];
+  int src[CPW];  // 0: x, 1: the weight, 2: the up projection
+#pragma unroll
+  for (int c = 0; c < CPW; c++) {
+    const int row = 8 * (wave * CPW + c), b = row - BM;
+    src[c] = b < 0 ? 0 : GLU && (b & 32) ? 2 : 1;
+    const int rr = b < 0 ? row : GLU ? (b >> 6) * 32 + (b & 31) : b;
+    voff[c] = (uint32_t)(rr + (lane >> 3)) * (uint32_t)(b < 0 ? (int)a.ldx : K) + 16 * unit;
+  }
+  int icur = 0, ikb = 0;  // the next stage to fill: its buffer and block
+  const auto issue = [&]() __attribute__((always_inline)) {
+    char* st = smem + icur * ST;
+    icur = icur + 1 == NST ? 0 : icur + 1;
+    const int k = ikb * 128;
+    const uint32_t kl = k + 16 * unit < K ? (uint32_t)k : PAST;
+#pragma unroll
+    for (int c = 0; c < CPW; c++)
+      f8_copy16(src[c] == 0 ? rx : src[c] == 1 ? rw : rw2, st + (wave * CPW + c) * 1024, voff[c] + kl);
+    const int kbc = min(ikb, KB - 1);  // (past the last block its scales again, unused)
+    const __amdgpu_buffer_rsrc_t rs =
+        __builtin_amdgcn_make_buffer_rsrc((void*)(a.xs + (int64_t)kbc * a.M + bm), (short)0, mrows * 4, 0x00020000);
+    // every wave issues one, so that the wait counts are the same: waves past the scales repeat the last
+    const int sw = min(wave, SPW - 1);
+    f8_copy4(rs, st + (BM + BN) * 128 + sw * 256, 4 * (64 * sw + lane));
+    ikb++;
+  };
+  // block scales of the wave's columns: 64 blocks in a register, one per lane
+  const float* ws = a.ws + (int64_t)((bn + (GLU ? wn / 2 : wn)) >> 7) * KB;
+  const float* ws2 = GLU ? a.ws2 + (int64_t)((bn + wn / 2) >> 7) * KB : nullptr;
+  const bool wcols = bn + (GLU ? wn / 2 : wn) < a.N;  // (a wave past N has no scales)
+  float swv = 0.0f, swv2 = 0.0f;
+
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; i++)
+#pragma unroll
+    for (int j = 0; j < NT; j++) acc[i][j] = f32x4{};
+  const int f0 = r * 128 + 16 * (g ^ (r & 7));
+  const auto frag = [&](const char* p) __attribute__((always_inline)) {
+    const i32x4 lo = *(const i32x4*)(p + f0), hi = *(const i32x4*)(p + (f0 ^ 64));
+    return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  };
+
+#pragma unroll
+  for (int p = 0; p < NST - 1; p++) issue();
+  int cur = 0;
+  for (int kb = 0; kb < KB; kb++) {
+    if ((kb & 63) == 0) {
+      swv = wcols && kb + lane < KB ? ws[kb + lane] : 0.0f;
+      if constexpr (GLU) swv2 = wcols && kb + lane < KB ? ws2[kb + lane] : 0.0f;
+    }
+    // stage kb has arrived once at most the copies of the NST - 2 stages after it pend; the barrier also ends
+    // every wave's reads of stage kb - 1, whose buffer is refilled
+    F8_WAIT_VM((NST - 2) * (CPW + 1));
+    f8_barrier();
+    issue();
+    const char* st = smem + cur * ST;
+    cur = cur + 1 == NST ? 0 : cur + 1;
+    const float sw = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, swv), kb & 63));
+    const float sw2 = GLU ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, swv2), kb & 63)) : 0.0f;
+    const float* sxs = (const float*)(st + (BM + BN) * 128) + wm + r;
+    if constexpr (WIDE) {
+      Wide wf[NT];
+#pragma unroll
+      for (int j = 0; j < NT; j++) wf[j] = widen(frag(st + (BM + wn + 16 * j) * 128));
+#pragma unroll
+      for (int i = 0; i < MT; i++) {
+        const Wide xf = widen(frag(st + (wm + 16 * i) * 128));
+        const float sx = sxs[16 * i];
+#pragma unroll
+        for (int j = 0; j < NT; j++) acc[i][j] = fma4(sx * (GLU && j >= NT / 2 ? sw2 : sw), mfma_wide(wf[j], xf), acc[i][j]);
+      }
+    } else {
+      i32x8 wf[NT];
+#pragma unroll
+      for (int j = 0; j < NT; j++) wf[j] = frag(st + (BM + wn + 16 * j) * 128);
+#pragma unroll
+      for (int i = 0; i < MT; i++) {
+        const i32x8 xf = frag(st + (wm + 16 * i) * 128);
+        const float sx = sxs[16 * i];
+#pragma unroll
+        for (int j = 0; j < NT; j++) acc[i][j] = fma4(sx * (GLU && j >= NT / 2 ? sw2 : sw), mfma_f8(wf[j], xf), acc[i][j]);
+      }
+    }
+  }
+  F8_WAIT_VM(0);  // no copy into LDS outlives the loop
+
+  // fp32 (bf16) rows leave through LDS, 16 HR rows of a wave at a time: a loop over rows with whole 16-byte columns
+  // of one row in neighbouring lanes, where the accumulators' layout would need the epilogue's code MT * NT times
+  constexpr int OC = GLU ? WN / 2 : WN, HR = MT < 2 ? MT : 2, RS = OC + 4, LR = OC / 4;
+  static_assert(NW * 16 * HR * RS * 4 <= NST * ST, "the waves' rows fit the stages");
+  const int n0 = bn + (GLU ? wn / 2 : wn);
+  if constexpr (GLU) {
+    GluBias b[NT / 2];
+#pragma unroll
+    for (int j = 0; j < NT / 2; j++) b[j] = f8_glu_bias(a, n0 + 16 * j + 4 * g);
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+      for (int j = 0; j < NT / 2; j++) acc[i][j] = f8_glu(a, b[j], acc[i][j], acc[i][j + NT / 2]);
+  }
+  f8_barrier();  // every wave's reads of the last stage are done
+  if (a.out) {
+    float* rows = (float*)smem + wave * (16 * HR * RS);
+#pragma unroll
+    for (int i0 = 0; i0 < MT; i0 += HR) {
+#pragma unroll
+      for (int i = 0; i < HR; i++)
+#pragma unroll
+        for (int j = 0; j < OC / 16; j++) *(f32x4*)(rows + (16 * i + r) * RS + 16 * j + 4 * g) = acc[i0 + i][j];
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll 2
+      for (int q = lane / LR; q < 16 * HR; q += 64 / LR) {
+        const f32x4 v = *(const f32x4*)(rows + q * RS + 4 * (lane % LR));
+        const int m = bm + wm + 16 * i0 + q, n = n0 + 4 * (lane % LR);
+        if constexpr (GLU) f8_glu_store(a, m, n, v);
+        else f8_store(a, m, n, v);
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+  if constexpr (GLU) {
+    if constexpr (FN == 128) {
+      if (a.oq) {  // a tile is one block of 128 columns: its waves' maxima meet in LDS
+        uint32_t* red = (uint32_t*)smem;  // [NW / NWM][BM]
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+          uint32_t m = 0;
+#pragma unroll
+          for (int j = 0; j < NT / 2; j++) m = amax4(n0 + 16 * j < a.N ? acc[i][j] : f32x4{}, m);  // (N % 16 == 0)
+          m = umax(m, (uint32_t)__shfl_xor((int)m, 16));
+          m = umax(m, (uint32_t)__shfl_xor((int)m, 32));
+          if (g == 0) red[(wave / NWM) * BM + wm + 16 * i + r] = m;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+          const int ml = wm + 16 * i + r, m = bm + ml;
+          uint32_t am = 0;
+#pragma unroll
+          for (int w = 0; w < NW / NWM; w++) am = umax(am, red[w * BM + ml]);
+          float scale, mul;
+          f8_scale(am, scale, mul);
+          if (m >= a.M) continue;
+#pragma unroll
+          for (int j = 0; j < NT / 2; j++)
+            if (n0 + 16 * j < a.N) *(uint32_t*)(a.oq + (int64_t)m * a.N + n0 + 16 * j + 4 * g) = f8_pack(acc[i][j], mul);
+          if (wave < NWM && g == 0) a.os[(int64_t)tn * a.M + m] = scale;
+        }
+      }
+    }
+  }
 }
 
 // ------------------------------------------------------------------ host
@@ -443,8 +672,6 @@ struct OnDevice {
 };
 
 int refused(anima_ctx* c, int rc, const char* msg) { return fail(c, rc, "%s", msg); }
-
-constexpr int64_t GRID_Y = 65535;
 
 }  // namespace
 
@@ -535,17 +762,59 @@ static void f8_input(F8Args& a, const anima_weight* W, const float* x, int64_t l
   a.KB = (W->K + 127) / 128;
 }
 
-// The kernel for a product's sizes.
+// The kernel for a product's sizes: f8_skinny's 16 rows, or tiles.
+enum { F8_SKINNY, F8_256, F8_128, F8_64x256, F8_64, F8_COUNT };
+
+static int f8_choose(anima_ctx* c, bool glu, int64_t M, int N, int K, int precision) {
+  if (const char* e = getenv("F8_TILE")) return atoi(e);
+  if (M <= 64) return F8_SKINNY;
+  return F8_256;
+}
+
+template <int BM, int BN, int WM, int WN, int NST, bool GLU>
+static void f8_tile_launch(anima_ctx* c, const F8Args& a, int precision) {
+  constexpr int FN = GLU ? BN / 2 : BN;
+  const dim3 grid((unsigned)((int64_t)((a.N + FN - 1) / FN) * ((a.M + BM - 1) / BM))), block(64 * (BM / WM) * (BN / WN));
+  if (precision == ANIMA_PREC_FP32) hipLaunchKernelGGL((f8_tile<BM, BN, WM, WN, NST, true, GLU>), grid, block, 0, c->stream, a);
+  else hipLaunchKernelGGL((f8_tile<BM, BN, WM, WN, NST, false, GLU>), grid, block, 0, c->stream, a);
+}
+
+// Runs the product of a's rows, quantizing fp32 rows first where the kernel takes e4m3 rows.
 template <bool GLU>
-static int f8_product(anima_ctx* c, const F8Args& a) {
-  const char* name = GLU ? "gemm.f8.glu.skinny" : "gemm.f8.skinny";
-  const int64_t mt = ((int64_t)a.M + 15) / 16;
-  if (mt > GRID_Y) return fail(c, ANIMA_E_UNSUPPORTED, "f8 product: M=%d", a.M);
-  Launch L(c, name, (GLU ? 4.0 : 2.0) * a.M * a.N * a.K, (double)a.N * a.K * (GLU ? 2 : 1));
-  const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)mt), block(64 * (a.KB < SKW ? a.KB : SKW));
-  if (a.x) hipLaunchKernelGGL((f8_skinny<true, GLU>), grid, block, 0, c->stream, a);
-  else hipLaunchKernelGGL((f8_skinny<false, GLU>), grid, block, 0, c->stream, a);
-  return L.end();
+static int f8_product(anima_ctx* c, F8Args a, int kind, int precision) {
+  static const char* const names[2][F8_COUNT] = {{"gemm.f8.skinny", "gemm.f8.256x256", "gemm.f8.128x128", "gemm.f8.64x256", "gemm.f8.64x64"},
+                                                 {"glu.f8.skinny", "glu.f8.256x256", "glu.f8.128x128", "glu.f8.64x256", "glu.f8.64x64"}};
+  void* scratch = nullptr;
+  if (kind != F8_SKINNY && a.x) {
+    const size_t qb = ((size_t)a.M * a.K + 255) / 256 * 256;
+    if (int rc = anima_alloc(c, qb + (size_t)a.M * a.KB * 4, &scratch)) return rc;
+    a.xq = (const uint8_t*)scratch;
+    a.xs = (const float*)((char*)scratch + qb);
+    const int rc = quant_rows_f8_launch(c, a.x, 0, a.M, a.K, a.ldx, (uint8_t*)scratch, (float*)((char*)scratch + qb));
+    if (rc != ANIMA_OK) {
+      anima_free(c, scratch);
+      return rc;
+    }
+    a.ldx = a.K;
+  }
+  Launch L(c, names[GLU][kind], (GLU ? 4.0 : 2.0) * a.M * a.N * a.K, (double)a.N * a.K * (GLU ? 2 : 1));
+  if (kind == F8_SKINNY) {
+    const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)((a.M + 15) / 16)), block(64 * (a.KB < SKW ? a.KB : SKW));
+    if (a.x) hipLaunchKernelGGL((f8_skinny<true, GLU>), grid, block, 0, c->stream, a);
+    else hipLaunchKernelGGL((f8_skinny<false, GLU>), grid, block, 0, c->stream, a);
+  } else if (kind == F8_256) {
+    f8_tile_launch<256, 256, 128, 64, 2, GLU>(c, a, precision);
+  } else if (kind == F8_128) {
+    f8_tile_launch<128, 128, 64, 64, 2, GLU>(c, a, precision);
+  } else if (kind == F8_64x256) {
+    f8_tile_launch<64, 256, 64, 64, 2, GLU>(c, a, precision);
+  } else {
+    if constexpr (GLU) f8_tile_launch<64, 64, 16, 64, 3, GLU>(c, a, precision);
+    else f8_tile_launch<64, 64, 32, 32, 3, GLU>(c, a, precision);
+  }
+  const int rc = L.end();
+  if (scratch) anima_free(c, scratch);
+  return rc;
 }
 
 int linear_f8_launch(anima_ctx* c, const anima_linear_desc* d) {
@@ -570,7 +839,7 @@ int linear_f8_launch(anima_ctx* c, const anima_linear_desc* d) {
   a.obf = d->out_bf16;
   a.vec = a.N % 4 == 0 && a.ldc % 4 == 0 && f8_al(a.out, a.obf ? 8 : 16) && f8_al(a.bias, 16) && (!a.add || (a.ld_add % 4 == 0 && f8_al(a.add, 16))) &&
           (a.epi != ANIMA_EPI_GATED || f8_al(a.gate, 16));
-  return f8_product<false>(c, a);
+  return f8_product<false>(c, a, f8_choose(c, false, a.M, a.N, a.K, d->precision), d->precision);
 }
 
 int linear_glu_launch(anima_ctx* c, const anima_glu_desc* d) {
@@ -592,13 +861,18 @@ int linear_glu_launch(anima_ctx* c, const anima_glu_desc* d) {
   a.out = d->out;
   a.ldc = d->ldc ? d->ldc : a.N;
   void* tmp = nullptr;
-  if (d->out_q) {  // fp32 rows first (pooled scratch), then their e4m3 rows
+  const int kind = f8_choose(c, true, a.M, a.N, a.K, d->precision);
+  if (d->out_q && (kind == F8_256 || kind == F8_64x256)) {  // a tile is one block of 128 columns
+    a.oq = d->out_q;
+    a.os = d->out_s;
+    a.out = nullptr;
+  } else if (d->out_q) {  // fp32 rows first (pooled scratch), then their e4m3 rows
     if (int rc = anima_alloc(c, (size_t)a.M * a.N * 4, &tmp)) return rc;
     a.out = (float*)tmp;
     a.ldc = a.N;
   }
   a.vec = a.N % 4 == 0 && a.ldc % 4 == 0 && f8_al(a.out, 16);
-  int rc = f8_product<true>(c, a);
+  int rc = f8_product<true>(c, a, kind, d->precision);
   if (tmp) {
     if (rc == ANIMA_OK) rc = quant_rows_f8_launch(c, tmp, 0, a.M, a.N, 0, d->out_q, d->out_s);
     anima_free(c, tmp);
