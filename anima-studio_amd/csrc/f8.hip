@@ -9,15 +9,16 @@
 // the largest a'), which rounds to 448: no clamp.
 //
 // Products: D = sum over the 128 k of a block on the matrix cores, then acc = fma(xs * scale, D, acc) in fp32.
-// ANIMA_PREC_BF16 takes v_mfma_f32_16x16x128_f8f6f4, exactly one block of k: within each eight k it aligns the
+// ANIMA_PREC_BF16 takes v_mfma_f32_32x32x64_f8f6f4, two of them a block of k: within each eight k it aligns the
 // products to the largest and drops what lies 2^-13 below (measured: 2^16 + 2^3 is exact, 2^16 + 2^2 gives 2^16;
 // relative L2 error of a block of normal values 1.5e-5, mean 1e-7), between the eights it adds in 32 bits.
-// ANIMA_PREC_FP32 widens e4m3 to bf16 (exact: 4 significant bits) and takes v_mfma_f32_16x16x32_bf16, whose
+// ANIMA_PREC_FP32 widens e4m3 to bf16 (exact: 4 significant bits) and takes v_mfma_f32_32x32x16_bf16, whose
 // products of such values are exact and sums 32 bits (error of a block 9e-9), at half the rate.  The weight is
 // the first operand, so D's rows are outputs n and its columns rows m of x: a lane holds four consecutive n of
 // one m, and its xs is one value.
 #include <cmath>
 #include <cstdlib>
+#include <type_traits>
 
 #include "common.h"
 #include "f8_args.h"
@@ -84,9 +85,16 @@ __device__ __forceinline__ uint32_t half_umax(uint32_t v) {
   return v;
 }
 
+// SiLU as r * rcp(1 + 2^(-r log2 e)) on v_exp_f32 and v_rcp_f32 (1 ulp each): within 2^-22 (1 + |r| / 2) of itself for
+// negative r (the rounding of the exponent), 2^-22 for others; 5 instructions, where silu_f's expf and quotient take 40
+// (of a 256 x 256 tile's epilogue 25000 cycles, and 9000).
+__device__ __forceinline__ float f8_silu(float r) {
+  return r * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(r * -1.4426950408889634f));
+}
+
 __device__ __forceinline__ float f8_act(float r, int act) {
   if (act == ANIMA_ACT_GELU) return gelu_erf(r);
-  if (act == ANIMA_ACT_SILU) return silu_f(r);
+  if (act == ANIMA_ACT_SILU) return f8_silu(r);
   return r;
 }
 
@@ -272,7 +280,8 @@ __device__ __forceinline__ bf16x8 widen8(int lo, int hi) {
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// a fragment of mfma_f8 as four of v_mfma_f32_16x16x32_bf16 (any order of k that both operands share will do)
+// 32 values of k of a lane as four fragments of v_mfma_f32_16x16x32_bf16 (any order of k that both operands share
+// will do)
 struct Wide {
   bf16x8 v[4];
 };
@@ -297,42 +306,49 @@ __device__ __forceinline__ f32x4 fma4(float s, f32x4 d, f32x4 c) {
 
 __device__ __forceinline__ uint32_t bf16_bits(float v) { return __builtin_bit_cast(uint16_t, to_bf16(v)); }
 
-// Columns n .. n + 3 of row m of a linear's output from their sums.
-__device__ __forceinline__ void f8_store(const F8Args& a, int m, int n, f32x4 r) {
-  if (m >= a.M) return;
+// Columns n .. n + 3 of a row of N values; zeros past it.
+__device__ __forceinline__ f32x4 f8_ld4(const float* p, int n, int N, int vec) {
+  if (vec) return n < N ? ld4(p + n) : f32x4{};
+  f32x4 v{};
+#pragma unroll
+  for (int e = 0; e < 4; e++)
+    if (n + e < N) v[e] = p[n + e];
+  return v;
+}
+
+// What is in columns n .. n + 3 of row m of the output.
+__device__ __forceinline__ f32x4 f8_ld_out(const F8Args& a, int m, int n) {
+  return m < a.M ? f8_ld4(a.out + (int64_t)m * a.ldc, n, a.N, a.vec) : f32x4{};
+}
+
+// Columns n .. n + 3 of row m of a linear's output from their sums, bias, gate and what is there.
+__device__ __forceinline__ void f8_store(const F8Args& a, int m, int n, f32x4 r, f32x4 bias, f32x4 gate, f32x4 c) {
+  if (m >= a.M || n >= a.N) return;
   const int64_t at = (int64_t)m * a.ldc + n;
-  float* o = a.out + at;
-  uint16_t* ob = (uint16_t*)a.out + at;
-  const float* add = a.add ? a.add + (int64_t)m * a.ld_add + n : nullptr;
-  r = r * a.alpha;
-  if (a.vec) {
-    if (n >= a.N) return;
-    if (a.bias) r = r + ld4(a.bias + n);
-    if (add) r = r + ld4(add);
+#pragma unroll
+  for (int e = 0; e < 4; e++) r[e] = __builtin_fmaf(r[e], a.alpha, bias[e]);
+  if (a.add) r = r + f8_ld4(a.add + (int64_t)m * a.ld_add, n, a.N, a.vec);
+  if (a.act) {
 #pragma unroll
     for (int e = 0; e < 4; e++) r[e] = f8_act(r[e], a.act);
-    if (a.epi == ANIMA_EPI_RESID) {
-      r = r + ld4(o);
-    } else if (a.epi == ANIMA_EPI_GATED) {
-      const f32x4 g = ld4(a.gate + n), c = ld4(o);
+  }
+  if (a.epi == ANIMA_EPI_RESID) {
+    r = r + c;
+  } else if (a.epi == ANIMA_EPI_GATED) {
 #pragma unroll
-      for (int e = 0; e < 4; e++) r[e] = __builtin_fmaf(g[e], r[e], c[e]);
-    }
+    for (int e = 0; e < 4; e++) r[e] = __builtin_fmaf(gate[e], r[e], c[e]);
+  }
+  uint16_t* ob = (uint16_t*)a.out + at;
+  if (a.vec) {
     if (a.obf) *(uint2*)ob = make_uint2(bf16_bits(r[0]) | bf16_bits(r[1]) << 16, bf16_bits(r[2]) | bf16_bits(r[3]) << 16);
-    else *(f32x4*)o = r;
+    else *(f32x4*)(a.out + at) = r;
     return;
   }
 #pragma unroll
   for (int e = 0; e < 4; e++) {
     if (n + e >= a.N) return;
-    float v = r[e];
-    if (a.bias) v += a.bias[n + e];
-    if (add) v += add[e];
-    v = f8_act(v, a.act);
-    if (a.epi == ANIMA_EPI_RESID) v += o[e];
-    else if (a.epi == ANIMA_EPI_GATED) v = __builtin_fmaf(a.gate[n + e], v, o[e]);
-    if (a.obf) ob[e] = (uint16_t)bf16_bits(v);
-    else o[e] = v;
+    if (a.obf) ob[e] = (uint16_t)bf16_bits(r[e]);
+    else a.out[at + e] = r[e];
   }
 }
 
@@ -351,12 +367,20 @@ __device__ __forceinline__ GluBias f8_glu_bias(const F8Args& a, int n) {
 }
 
 // h = act(g + b_gate) * (u + b_up)
-__device__ __forceinline__ f32x4 f8_glu(const F8Args& a, const GluBias& b, f32x4 g, f32x4 u) {
+__device__ __forceinline__ f32x4 f8_glu(int act, const GluBias& b, f32x4 g, f32x4 u) {
   g = g + b.g;
   u = u + b.u;
 #pragma unroll
-  for (int e = 0; e < 4; e++) g[e] = f8_act(g[e], a.act) * u[e];
+  for (int e = 0; e < 4; e++) g[e] = f8_act(g[e], act) * u[e];
   return g;
+}
+
+// f(the activation as a constant)
+template <class F>
+__device__ __forceinline__ void f8_with_act(int act, const F& f) {
+  if (act == ANIMA_ACT_SILU) f(std::integral_constant<int, ANIMA_ACT_SILU>{});
+  else if (act == ANIMA_ACT_GELU) f(std::integral_constant<int, ANIMA_ACT_GELU>{});
+  else f(std::integral_constant<int, ANIMA_ACT_NONE>{});
 }
 
 __device__ __forceinline__ void f8_glu_store(const F8Args& a, int m, int n, f32x4 h) {
@@ -438,8 +462,9 @@ __global__ __launch_bounds__(64 * SKW) void f8_skinny(F8Args a) {
   for (int t = 0; t < TT; t++)
     for (int w = 1; w < nw; w++) acc[t] = acc[t] + part[w][t][lane];
   const int n = n0 + 4 * g;
-  if constexpr (GLU) f8_glu_store(a, m, n, f8_glu(a, f8_glu_bias(a, n), acc[0], acc[1]));
-  else f8_store(a, m, n, acc[0]);
+  if constexpr (GLU) f8_glu_store(a, m, n, f8_glu(a.act, f8_glu_bias(a, n), acc[0], acc[1]));
+  else f8_store(a, m, n, acc[0], a.bias ? f8_ld4(a.bias, n, a.N, a.vec) : f32x4{}, a.epi == ANIMA_EPI_GATED ? f8_ld4(a.gate, n, a.N, a.vec) : f32x4{},
+                a.epi != ANIMA_EPI_STORE ? f8_ld_out(a, m, n) : f32x4{});
 }
 
 // f8_tile: one BM x BN output tile per workgroup (GLU: BN / 2 columns of each projection), waves of WM x WN.
@@ -458,10 +483,6 @@ __device__ __forceinline__ void f8_barrier() {
   asm volatile("" ::: "memory");
 }
 
-__device__ __forceinline__ f32x4 mfma_f8(i32x8 a, i32x8 b) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, f32x4{}, 0, 0, 0, 0, 0, 0);
-}
-
 // a wave's copy of 64 x 16 (x 4) bytes into LDS
 __device__ __forceinline__ void f8_copy16(__amdgpu_buffer_rsrc_t rs, char* dst, uint32_t off) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (f8_lds_t*)dst, 16, off, 0, 0, 0);
@@ -471,16 +492,21 @@ __device__ __forceinline__ void f8_copy4(__amdgpu_buffer_rsrc_t rs, char* dst, u
 }
 
 template <int BM, int BN, int WM, int WN, int NST, bool WIDE, bool GLU>
-__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void f8_tile(F8Args a) {
-  constexpr int NWM = BM / WM, NW = NWM * (BN / WN), MT = WM / 16, NT = WN / 16;
-  constexpr int ST = (BM + BN) * 128 + BM * 4;            // bytes of a stage
+__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void f8_tile(F8Args a) {
+  constexpr int NWM = BM / WM, NW = NWM * (BN / WN), MT = WM / 32, NT = WN / 32;
+  // LDS: the stages' rows of x, then those of the weight, the scales of x, the scales of the weight; each address is
+  // a lane's register plus a constant
+  constexpr int XB = BM * 128, WB = BN * 128, SB = GLU ? 512 : 256;  // bytes of a stage
+  constexpr int WO = NST * XB, XSO = WO + NST * WB, WSO = XSO + NST * BM * 4;
+  constexpr int EPL = NW * 32 * (MT < 2 ? 1 : 2) * ((GLU ? WN / 2 : WN) + 4) * 4;  // the epilogue's rows
+  constexpr int LDS = WSO + NST * SB > EPL ? WSO + NST * SB : EPL;
   constexpr int CPW = (BM + BN) / 8 / NW, SPW = BM / 64;  // copies per wave: rows; waves that copy 64 scales each
   constexpr int FN = GLU ? BN / 2 : BN;                   // output columns of a tile
   constexpr uint32_t PAST = 0x80000000u;
-  static_assert(CPW * NW * 8 == BM + BN && SPW <= NW && WN <= 64 && (!GLU || WN == 64), "copies and waves");
-  __shared__ __attribute__((aligned(1024))) char smem[NST * ST];
+  static_assert(CPW * NW * 8 == BM + BN && SPW + (GLU ? 1 : 0) < NW && WN <= 64 && (!GLU || WN == 64), "copies and waves");
+  __shared__ __attribute__((aligned(1024))) char smem[LDS];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int r = lane & 15, g = lane >> 4;
+  const int r = lane & 31, hf = lane >> 5;
   const int ntn = (a.N + FN - 1) / FN, ntm = (a.M + BM - 1) / BM;
   int tm, tn;
   {
@@ -501,156 +527,311 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void f8_tile(F8Args a) 
   const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w + (int64_t)bn * K), (short)0, nrows * K, 0x00020000);
   const __amdgpu_buffer_rsrc_t rw2 =
       GLU ? __builtin_amdgcn_make_buffer_rsrc((void*)(a.w2 + (int64_t)bn * K), (short)0, nrows * K, 0x00020000) : rw;
-  const int unit = (lane & 7) ^ (lane >> 3);
-  uint32_t voff[CPW];
-  int src[CPW];  // 0: x, 1: the weight, 2: the up projection
+  // copy c of this wave: eight rows of one operand, row lane / 8 at (lane / 8) * ld + 16 * unit past their start
+  int src[CPW];        // 0: x, 1: the weight, 2: the up projection
+  uint32_t roff[CPW];  // where the rows start
 #pragma unroll
   for (int c = 0; c < CPW; c++) {
     const int row = 8 * (wave * CPW + c), b = row - BM;
     src[c] = b < 0 ? 0 : GLU && (b & 32) ? 2 : 1;
-    const int rr = b < 0 ? row : GLU ? (b >> 6) * 32 + (b & 31) : b;
-    voff[c] = (uint32_t)(rr + (lane >> 3)) * (uint32_t)(b < 0 ? (int)a.ldx : K) + 16 * unit;
+    roff[c] = b < 0 ? (uint32_t)row * (uint32_t)a.ldx : (uint32_t)(GLU ? (b >> 6) * 32 + (b & 31) : b) * (uint32_t)K;
   }
-  int icur = 0, ikb = 0;  // the next stage to fill: its buffer and block
-  const auto issue = [&]() __attribute__((always_inline)) {
-    char* st = smem + icur * ST;
-    icur = icur + 1 == NST ? 0 : icur + 1;
-    const int k = ikb * 128;
-    const uint32_t kl = k + 16 * unit < K ? (uint32_t)k : PAST;
+  // One more copy in every wave, so that the wait counts are the same: 64 scales of x each, then the block scales of
+  // the tile's columns (even lanes the first block of 128, odd lanes the second) and of the up projection's.  No
+  // branch: a stage is one basic block, or its sums would move behind it.
+  const bool up = GLU && wave > SPW;
+  const float* sbase = wave < SPW ? a.xs + bm : (up ? a.ws2 : a.ws) + (int64_t)(bn >> 7) * KB;
+  const int64_t sstep = wave < SPW ? a.M : 1;
+  const int srec = wave < SPW ? mrows * 4 : min((a.N + 127) / 128 - (bn >> 7), 2) * KB * 4;
+  const int sdst = wave < SPW ? XSO + wave * 256 : WSO + (up ? 256 : 0), sdstep = wave < SPW ? BM * 4 : SB;
+  // The lanes' parts of the addresses are formed again for every stage (the asm keeps them there): registers are
+  // what the sums leave, and a spilled one waits for all copies in flight.
+  int ikb = 0;  // the next block to copy (into buffer p = ikb % NST)
+  const auto issue = [&](int p) __attribute__((always_inline)) {
+    int l;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
+    const int unit = (l & 7) ^ (l >> 3), k = ikb * 128;
+    const uint32_t kl = k + 16 * unit < K ? (uint32_t)(k + 16 * unit) : PAST;
+    const uint32_t lx = (uint32_t)(l >> 3) * (uint32_t)a.ldx + kl, lw = (uint32_t)(l >> 3) * (uint32_t)K + kl;
+    const uint32_t soff = wave < SPW ? 4 * (64 * wave + l) : 4 * ((l & 1) * KB);
 #pragma unroll
     for (int c = 0; c < CPW; c++)
-      f8_copy16(src[c] == 0 ? rx : src[c] == 1 ? rw : rw2, st + (wave * CPW + c) * 1024, voff[c] + kl);
+      f8_copy16(src[c] == 0 ? rx : src[c] == 1 ? rw : rw2, smem + (wave * CPW + c) * 1024 + (src[c] ? WO - XB + p * WB : p * XB),
+                (src[c] ? lw : lx) + roff[c]);
     const int kbc = min(ikb, KB - 1);  // (past the last block its scales again, unused)
-    const __amdgpu_buffer_rsrc_t rs =
-        __builtin_amdgcn_make_buffer_rsrc((void*)(a.xs + (int64_t)kbc * a.M + bm), (short)0, mrows * 4, 0x00020000);
-    // every wave issues one, so that the wait counts are the same: waves past the scales repeat the last
-    const int sw = min(wave, SPW - 1);
-    f8_copy4(rs, st + (BM + BN) * 128 + sw * 256, 4 * (64 * sw + lane));
+    f8_copy4(__builtin_amdgcn_make_buffer_rsrc((void*)(sbase + (int64_t)kbc * sstep), (short)0, srec - (wave < SPW ? 0 : 4 * kbc), 0x00020000),
+             smem + sdst + p * sdstep, soff);
     ikb++;
   };
-  // block scales of the wave's columns: 64 blocks in a register, one per lane
-  const float* ws = a.ws + (int64_t)((bn + (GLU ? wn / 2 : wn)) >> 7) * KB;
-  const float* ws2 = GLU ? a.ws2 + (int64_t)((bn + wn / 2) >> 7) * KB : nullptr;
-  const bool wcols = bn + (GLU ? wn / 2 : wn) < a.N;  // (a wave past N has no scales)
-  float swv = 0.0f, swv2 = 0.0f;
-
-  f32x4 acc[MT][NT];
+  f32x16 acc[MT][NT];
 #pragma unroll
   for (int i = 0; i < MT; i++)
 #pragma unroll
-    for (int j = 0; j < NT; j++) acc[i][j] = f32x4{};
-  const int f0 = r * 128 + 16 * (g ^ (r & 7));
-  const auto frag = [&](const char* p) __attribute__((always_inline)) {
-    const i32x4 lo = *(const i32x4*)(p + f0), hi = *(const i32x4*)(p + (f0 ^ 64));
-    return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    for (int j = 0; j < NT; j++) acc[i][j] = f32x16{};
+  // a fragment: units 2 c + hf (c = 0 .. 3) of row r, 64 of the block's k in 16 registers
+  int xa[4], wa[4];
+#pragma unroll
+  for (int c = 0; c < 4; c++) {
+    const int f = r * 128 + 16 * ((2 * c + hf) ^ (r & 7));
+    xa[c] = f + wm * 128;
+    wa[c] = f + wn * 128 + WO;
+  }
+  const auto axpy = [](float s, const f32x16& d, f32x16& c, int e0, int e1) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = e0; e < e1; e++) c[e] = __builtin_fmaf(s, d[e], c[e]);
   };
 
+  const int xsa = XSO + 4 * (wm + r), wsa = WSO + 4 * (((bn + (GLU ? wn / 2 : wn)) >> 7) - (bn >> 7));
+  const auto wscale = [&](int p, int up) __attribute__((always_inline)) { return *(const float*)(smem + wsa + p * SB + 256 * up); };
+  const auto xscale = [&](int p, int i) __attribute__((always_inline)) { return *(const float*)(smem + xsa + p * BM * 4 + 128 * i); };
+  const auto xunit = [&](int p, int i, int c) __attribute__((always_inline)) { return *(const i32x4*)(smem + xa[c] + p * XB + 4096 * i); };
+  const auto wunit = [&](int p, int j, int c) __attribute__((always_inline)) { return *(const i32x4*)(smem + wa[c] + p * WB + 4096 * j); };
+
+  // The order of a stage is written out (sched_barrier): a tile's sums are scaled and added between the products of
+  // the tiles after it.
 #pragma unroll
-  for (int p = 0; p < NST - 1; p++) issue();
-  int cur = 0;
-  for (int kb = 0; kb < KB; kb++) {
-    if ((kb & 63) == 0) {
-      swv = wcols && kb + lane < KB ? ws[kb + lane] : 0.0f;
-      if constexpr (GLU) swv2 = wcols && kb + lane < KB ? ws2[kb + lane] : 0.0f;
+  for (int p = 0; p < NST; p++) issue(p);
+  const auto stages = [&](const auto& stage) __attribute__((always_inline)) {  // the buffer as a constant
+    int kb = 0;
+    for (; kb + NST <= KB; kb += NST) {
+      stage(std::integral_constant<int, 0>{});
+      stage(std::integral_constant<int, 1>{});
+      if constexpr (NST == 3) stage(std::integral_constant<int, 2>{});
     }
-    // stage kb has arrived once at most the copies of the NST - 2 stages after it pend; the barrier also ends
-    // every wave's reads of stage kb - 1, whose buffer is refilled
+    if (kb < KB) stage(std::integral_constant<int, 0>{});
+    if constexpr (NST == 3)
+      if (kb + 1 < KB) stage(std::integral_constant<int, 1>{});
+  };
+  // Stages overlap: before the last tiles of stage kb, whose fragments are in registers by then, a barrier ends every
+  // wave's reads of the stage (its buffer is refilled) and publishes stage kb + 1 (arrived once at most the copies of
+  // the NST - 2 stages after it pend), whose first fragments are then read under those tiles' products.
+  const auto turn = [&](int p) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
     F8_WAIT_VM((NST - 2) * (CPW + 1));
     f8_barrier();
-    issue();
-    const char* st = smem + cur * ST;
-    cur = cur + 1 == NST ? 0 : cur + 1;
-    const float sw = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, swv), kb & 63));
-    const float sw2 = GLU ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, swv2), kb & 63)) : 0.0f;
-    const float* sxs = (const float*)(st + (BM + BN) * 128) + wm + r;
-    if constexpr (WIDE) {
-      Wide wf[NT];
+    issue(p);
+  };
+  F8_WAIT_VM((NST - 1) * (CPW + 1));
+  f8_barrier();
+  constexpr int T = MT * NT;
+  static_assert((MT == 1 || MT % 2 == 0) && (T == 1 || T % 2 == 0), "fragments and sums alternate");
+  f32x16 d[2];
+  float sp = 0.0f;  // the scale of the tile in the other d
+  d[1] = f32x16{};
+  if constexpr (WIDE) {
+    // One column of tiles after the other, so that the widened weight is one fragment; x is widened again
+    // for each column, and its registers take the next row's units one by one.
+    i32x4 xr[4], wr[4];
+    bf16x8 wf[8];
 #pragma unroll
-      for (int j = 0; j < NT; j++) wf[j] = widen(frag(st + (BM + wn + 16 * j) * 128));
-#pragma unroll
-      for (int i = 0; i < MT; i++) {
-        const Wide xf = widen(frag(st + (wm + 16 * i) * 128));
-        const float sx = sxs[16 * i];
-#pragma unroll
-        for (int j = 0; j < NT; j++) acc[i][j] = fma4(sx * (GLU && j >= NT / 2 ? sw2 : sw), mfma_wide(wf[j], xf), acc[i][j]);
-      }
-    } else {
-      i32x8 wf[NT];
-#pragma unroll
-      for (int j = 0; j < NT; j++) wf[j] = frag(st + (BM + wn + 16 * j) * 128);
-#pragma unroll
-      for (int i = 0; i < MT; i++) {
-        const i32x8 xf = frag(st + (wm + 16 * i) * 128);
-        const float sx = sxs[16 * i];
-#pragma unroll
-        for (int j = 0; j < NT; j++) acc[i][j] = fma4(sx * (GLU && j >= NT / 2 ? sw2 : sw), mfma_f8(wf[j], xf), acc[i][j]);
-      }
+    for (int c = 0; c < 4; c++) {
+      xr[c] = xunit(0, 0, c);
+      wr[c] = wunit(0, 0, c);
     }
+    stages([&](auto buffer) __attribute__((always_inline)) {
+      constexpr int p = decltype(buffer)::value, pn = (p + 1) % NST;
+#pragma unroll
+      for (int t = 0; t < T; t++) {
+        const int j = t / MT, i = t % MT, pt = (t + T - 1) % T;
+        const bool last = t + 1 == T;
+        const float s = xscale(p, i) * wscale(p, GLU && j >= NT / 2);
+        if (last) turn(p);
+#pragma unroll
+        for (int q = 0; q < 8; q++) {
+          const bf16x8 xq = widen8(xr[q / 2][q % 2 * 2], xr[q / 2][q % 2 * 2 + 1]);
+          if (i == 0) wf[q] = widen8(wr[q / 2][q % 2 * 2], wr[q / 2][q % 2 * 2 + 1]);
+          if (q % 2 == 1) {  // the unit is done with
+            xr[q / 2] = xunit(last ? pn : p, (i + 1) % MT, q / 2);
+            if (i + 1 == MT) wr[q / 2] = wunit(last ? pn : p, (j + 1) % NT, q / 2);
+          }
+          d[t & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[q], xq, q ? d[t & 1] : f32x16{}, 0, 0, 0);
+          if constexpr (T > 1) axpy(sp, d[(t + 1) & 1], acc[pt % MT][pt / MT], 2 * q, 2 * q + 2);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        sp = s;
+        if constexpr (T == 1) axpy(sp, d[0], acc[0][0], 0, 16);
+      }
+    });
+  } else {
+    i32x8 wf[NT][2], xf[2][2];
+    const auto two = [](i32x4 lo, i32x4 hi) __attribute__((always_inline)) { return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7); };
+    const auto x64 = [&](int p, int i, int h) __attribute__((always_inline)) { return two(xunit(p, i, 2 * h), xunit(p, i, 2 * h + 1)); };
+    const auto w64 = [&](int p, int j, int h) __attribute__((always_inline)) { return two(wunit(p, j, 2 * h), wunit(p, j, 2 * h + 1)); };
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      xf[0][h] = x64(0, 0, h);
+#pragma unroll
+      for (int j = 0; j < NT; j++) wf[j][h] = w64(0, j, h);
+    }
+    stages([&](auto buffer) __attribute__((always_inline)) {
+      constexpr int p = decltype(buffer)::value, pn = (p + 1) % NST;
+      float s[NT];
+#pragma unroll
+      for (int t = 0; t < T; t++) {
+        const int i = t / NT, j = t % NT, pt = (t + T - 1) % T;
+        if (j == 0) {
+#pragma unroll
+          for (int n = 0; n < NT; n++) s[n] = xscale(p, i) * wscale(p, GLU && n >= NT / 2);
+          if (i + 1 == MT) turn(p);
+          if constexpr (MT > 1) {  // (past the last row: the next stage's first)
+#pragma unroll
+            for (int h = 0; h < 2; h++) xf[(i + 1) & 1][h] = i + 1 == MT ? x64(pn, 0, h) : x64(p, i + 1, h);
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          d[t & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[j][h], xf[i & 1][h], h ? d[t & 1] : f32x16{}, 0, 0, 0, 0, 0, 0);
+          if constexpr (T > 1) axpy(sp, d[(t + 1) & 1], acc[pt / NT][pt % NT], 8 * h, 8 * h + 8);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (i + 1 == MT) {
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            wf[j][h] = w64(pn, j, h);
+            if (MT == 1 && j + 1 == NT) xf[0][h] = x64(pn, 0, h);
+          }
+        }
+        sp = s[j];
+        if constexpr (T == 1) axpy(sp, d[0], acc[0][0], 0, 16);
+      }
+    });
   }
+  if constexpr (T > 1) axpy(sp, d[1], acc[MT - 1][NT - 1], 0, 16);
   F8_WAIT_VM(0);  // no copy into LDS outlives the loop
 
-  // fp32 (bf16) rows leave through LDS, 16 HR rows of a wave at a time: a loop over rows with whole 16-byte columns
-  // of one row in neighbouring lanes, where the accumulators' layout would need the epilogue's code MT * NT times
-  constexpr int OC = GLU ? WN / 2 : WN, HR = MT < 2 ? MT : 2, RS = OC + 4, LR = OC / 4;
-  static_assert(NW * 16 * HR * RS * 4 <= NST * ST, "the waves' rows fit the stages");
+  // fp32 (bf16) rows leave through LDS, 64 rows of a wave at a time: a loop with 16 bytes of one row in neighbouring
+  // lanes (whole lines; the accumulators' layout has 16 bytes of 32 rows), a lane keeping its four columns.
+  constexpr int OC = GLU ? WN / 2 : WN, RS = OC + 4, LR = OC / 4, PR = 64 / LR, HR = MT < 2 ? 1 : 2;
+  static_assert(NW * 32 * HR * RS * 4 <= LDS && 32 * HR * LR % 256 == 0, "the waves' rows fit; four passes at a time");
   const int n0 = bn + (GLU ? wn / 2 : wn);
-  if constexpr (GLU) {
-    GluBias b[NT / 2];
+  const auto quad = [](const f32x16& v, int q) __attribute__((always_inline)) {
+    return f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+  };
+  if constexpr (GLU) {  // (NT = 2: a lane's gate and up values of columns n0 + 8 q + 4 hf + e)
+    GluBias b[4];
 #pragma unroll
-    for (int j = 0; j < NT / 2; j++) b[j] = f8_glu_bias(a, n0 + 16 * j + 4 * g);
+    for (int q = 0; q < 4; q++) b[q] = f8_glu_bias(a, n0 + 8 * q + 4 * hf);
+    f8_with_act(a.act, [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < MT; i++)
+      for (int i = 0; i < MT; i++)
 #pragma unroll
-      for (int j = 0; j < NT / 2; j++) acc[i][j] = f8_glu(a, b[j], acc[i][j], acc[i][j + NT / 2]);
+        for (int q = 0; q < 4; q++) {
+          const f32x4 h = f8_glu(decltype(act)::value, b[q], quad(acc[i][0], q), quad(acc[i][1], q));
+#pragma unroll
+          for (int e = 0; e < 4; e++) acc[i][0][4 * q + e] = h[e];
+        }
+    });
   }
   f8_barrier();  // every wave's reads of the last stage are done
   if (a.out) {
-    float* rows = (float*)smem + wave * (16 * HR * RS);
+    float* rows = (float*)smem + wave * (32 * HR * RS);
+    const int n = n0 + 4 * (lane % LR);
+    const float* line = rows + (lane / LR) * RS + 4 * (lane % LR);
+    // rows 32 i ... of the wave into LDS, and `pass` for each four of a lane's rows (row in the tile, their values)
+    const auto leave = [&](const auto& pass) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i0 = 0; i0 < MT; i0 += HR) {
+      for (int i = 0; i < MT; i += HR) {
 #pragma unroll
-      for (int i = 0; i < HR; i++)
+        for (int k = 0; k < HR; k++)
 #pragma unroll
-        for (int j = 0; j < OC / 16; j++) *(f32x4*)(rows + (16 * i + r) * RS + 16 * j + 4 * g) = acc[i0 + i][j];
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll 2
-      for (int q = lane / LR; q < 16 * HR; q += 64 / LR) {
-        const f32x4 v = *(const f32x4*)(rows + q * RS + 4 * (lane % LR));
-        const int m = bm + wm + 16 * i0 + q, n = n0 + 4 * (lane % LR);
-        if constexpr (GLU) f8_glu_store(a, m, n, v);
-        else f8_store(a, m, n, v);
+          for (int j = 0; j < OC / 32; j++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) *(f32x4*)(rows + (32 * k + r) * RS + 32 * j + 8 * q + 4 * hf) = quad(acc[i + k][j], q);
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int q = 0; q < 32 * HR; q += 4 * PR) {
+          f32x4 v[4];
+#pragma unroll
+          for (int u = 0; u < 4; u++) v[u] = *(const f32x4*)(line + (q + u * PR) * RS);
+          pass(bm + wm + 32 * i + q + lane / LR, v);
+        }
+        __builtin_amdgcn_wave_barrier();
       }
-      __builtin_amdgcn_wave_barrier();
+    };
+    if constexpr (GLU) {
+      leave([&](int m, const f32x4 (&v)[4]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < 4; u++) f8_glu_store(a, m + u * PR, n, v[u]);
+      });
+    } else {
+      const f32x4 bias = a.bias ? f8_ld4(a.bias, n, a.N, a.vec) : f32x4{};
+      const f32x4 gate = a.epi == ANIMA_EPI_GATED ? f8_ld4(a.gate, n, a.N, a.vec) : f32x4{};
+      if (a.vec && !a.add) {
+        // the plain rows, each kind with code of its own: four rows' loads before the first store, one address each
+        const int64_t step = (int64_t)PR * a.ldc;
+        int M = n < a.N ? a.M : 0;
+        float alpha = a.alpha;
+        const auto plain = [&](auto kind, auto act) __attribute__((always_inline)) {
+          constexpr int E = decltype(kind)::value;  // ANIMA_EPI_*, 3: bf16 rows
+          leave([&](int m, f32x4 (&v)[4]) __attribute__((always_inline)) {
+            const int64_t at = (int64_t)m * a.ldc + n;
+            f32x4 c[4];
+            if constexpr (E == ANIMA_EPI_RESID || E == ANIMA_EPI_GATED) {
+#pragma unroll
+              for (int u = 0; u < 4; u++) c[u] = m + u * PR < M ? ld4(a.out + at + u * step) : f32x4{};
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                const float t = f8_act(__builtin_fmaf(v[u][e], alpha, bias[e]), decltype(act)::value);
+                v[u][e] = E == ANIMA_EPI_RESID ? t + c[u][e] : E == ANIMA_EPI_GATED ? __builtin_fmaf(gate[e], t, c[u][e]) : t;
+              }
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+              if (m + u * PR < M) {
+                if constexpr (E == 3)
+                  *(uint2*)((uint16_t*)a.out + at + u * step) =
+                      make_uint2(bf16_bits(v[u][0]) | bf16_bits(v[u][1]) << 16, bf16_bits(v[u][2]) | bf16_bits(v[u][3]) << 16);
+                else
+                  *(f32x4*)(a.out + at + u * step) = v[u];
+              }
+          });
+        };
+        f8_with_act(a.act, [&](auto act) __attribute__((always_inline)) {
+          if (a.epi == ANIMA_EPI_RESID) plain(std::integral_constant<int, ANIMA_EPI_RESID>{}, act);
+          else if (a.epi == ANIMA_EPI_GATED) plain(std::integral_constant<int, ANIMA_EPI_GATED>{}, act);
+          else if (a.obf) plain(std::integral_constant<int, 3>{}, act);
+          else plain(std::integral_constant<int, ANIMA_EPI_STORE>{}, act);
+        });
+      } else {
+        leave([&](int m, const f32x4 (&v)[4]) __attribute__((always_inline)) {
+#pragma unroll
+          for (int u = 0; u < 4; u++)
+            f8_store(a, m + u * PR, n, v[u], bias, gate, a.epi != ANIMA_EPI_STORE ? f8_ld_out(a, m + u * PR, n) : f32x4{});
+        });
+      }
     }
   }
-  if constexpr (GLU) {
-    if constexpr (FN == 128) {
-      if (a.oq) {  // a tile is one block of 128 columns: its waves' maxima meet in LDS
-        uint32_t* red = (uint32_t*)smem;  // [NW / NWM][BM]
+  if constexpr (GLU && FN == 128) {
+    if (a.oq) {  // a tile is one block of 128 columns: its waves' maxima meet in LDS
+      uint32_t* red = (uint32_t*)smem;  // [NW / NWM][BM]
 #pragma unroll
-        for (int i = 0; i < MT; i++) {
-          uint32_t m = 0;
+      for (int i = 0; i < MT; i++) {
+        uint32_t m = 0;
 #pragma unroll
-          for (int j = 0; j < NT / 2; j++) m = amax4(n0 + 16 * j < a.N ? acc[i][j] : f32x4{}, m);  // (N % 16 == 0)
-          m = umax(m, (uint32_t)__shfl_xor((int)m, 16));
-          m = umax(m, (uint32_t)__shfl_xor((int)m, 32));
-          if (g == 0) red[(wave / NWM) * BM + wm + 16 * i + r] = m;
-        }
-        __syncthreads();
+        for (int q = 0; q < 4; q++) m = amax4(n0 + 8 * q + 4 * hf < a.N ? quad(acc[i][0], q) : f32x4{}, m);  // (N % 16 == 0)
+        m = umax(m, (uint32_t)__shfl_xor((int)m, 32));
+        if (hf == 0) red[(wave / NWM) * BM + wm + 32 * i + r] = m;
+      }
+      __syncthreads();
 #pragma unroll
-        for (int i = 0; i < MT; i++) {
-          const int ml = wm + 16 * i + r, m = bm + ml;
-          uint32_t am = 0;
+      for (int i = 0; i < MT; i++) {
+        const int ml = wm + 32 * i + r, m = bm + ml;
+        uint32_t am = 0;
 #pragma unroll
-          for (int w = 0; w < NW / NWM; w++) am = umax(am, red[w * BM + ml]);
-          float scale, mul;
-          f8_scale(am, scale, mul);
-          if (m >= a.M) continue;
+        for (int w = 0; w < NW / NWM; w++) am = umax(am, red[w * BM + ml]);
+        float scale, mul;
+        f8_scale(am, scale, mul);
+        // lane hf of a row holds columns 8 q + 4 hf: it gives away two quads and stores 16 columns from 16 hf on
+        uint32_t p[4];
 #pragma unroll
-          for (int j = 0; j < NT / 2; j++)
-            if (n0 + 16 * j < a.N) *(uint32_t*)(a.oq + (int64_t)m * a.N + n0 + 16 * j + 4 * g) = f8_pack(acc[i][j], mul);
-          if (wave < NWM && g == 0) a.os[(int64_t)tn * a.M + m] = scale;
-        }
+        for (int q = 0; q < 4; q++) p[q] = f8_pack(quad(acc[i][0], q), mul);
+        const uint32_t g0 = (uint32_t)__shfl_xor((int)(hf ? p[0] : p[2]), 32), g1 = (uint32_t)__shfl_xor((int)(hf ? p[1] : p[3]), 32);
+        if (m >= a.M) continue;
+        const u32x4 o = hf ? u32x4{g0, p[2], g1, p[3]} : u32x4{p[0], g0, p[1], g1};
+        if (n0 + 16 * hf < a.N) *(u32x4*)(a.oq + (int64_t)m * a.N + n0 + 16 * hf) = o;
+        if (wave < NWM && hf == 0) a.os[(int64_t)tn * a.M + m] = scale;
       }
     }
   }
@@ -763,7 +944,7 @@ static void f8_input(F8Args& a, const anima_weight* W, const float* x, int64_t l
 }
 
 // The kernel for a product's sizes: f8_skinny's 16 rows, or tiles.
-enum { F8_SKINNY, F8_256, F8_128, F8_64x256, F8_64, F8_COUNT };
+enum { F8_SKINNY, F8_256, F8_128, F8_64x256, F8_64, F8_128x256, F8_COUNT };
 
 static int f8_choose(anima_ctx* c, bool glu, int64_t M, int N, int K, int precision) {
   if (const char* e = getenv("F8_TILE")) return atoi(e);
@@ -782,8 +963,8 @@ static void f8_tile_launch(anima_ctx* c, const F8Args& a, int precision) {
 // Runs the product of a's rows, quantizing fp32 rows first where the kernel takes e4m3 rows.
 template <bool GLU>
 static int f8_product(anima_ctx* c, F8Args a, int kind, int precision) {
-  static const char* const names[2][F8_COUNT] = {{"gemm.f8.skinny", "gemm.f8.256x256", "gemm.f8.128x128", "gemm.f8.64x256", "gemm.f8.64x64"},
-                                                 {"glu.f8.skinny", "glu.f8.256x256", "glu.f8.128x128", "glu.f8.64x256", "glu.f8.64x64"}};
+  static const char* const names[2][F8_COUNT] = {{"gemm.f8.skinny", "gemm.f8.256x256", "gemm.f8.128x128", "gemm.f8.64x256", "gemm.f8.64x64", "c"},
+                                                 {"glu.f8.skinny", "glu.f8.256x256", "glu.f8.128x128", "glu.f8.64x256", "glu.f8.64x64", "c"}};
   void* scratch = nullptr;
   if (kind != F8_SKINNY && a.x) {
     const size_t qb = ((size_t)a.M * a.K + 255) / 256 * 256;
@@ -808,8 +989,10 @@ static int f8_product(anima_ctx* c, F8Args a, int kind, int precision) {
     f8_tile_launch<128, 128, 64, 64, 2, GLU>(c, a, precision);
   } else if (kind == F8_64x256) {
     f8_tile_launch<64, 256, 64, 64, 2, GLU>(c, a, precision);
+  } else if (kind == F8_128x256) {
+    f8_tile_launch<128, 256, 64, 64, 3, GLU>(c, a, precision);
   } else {
-    if constexpr (GLU) f8_tile_launch<64, 64, 16, 64, 3, GLU>(c, a, precision);
+    if constexpr (GLU) f8_tile_launch<64, 128, 32, 64, 3, GLU>(c, a, precision);
     else f8_tile_launch<64, 64, 32, 32, 3, GLU>(c, a, precision);
   }
   const int rc = L.end();
@@ -862,7 +1045,7 @@ int linear_glu_launch(anima_ctx* c, const anima_glu_desc* d) {
   a.ldc = d->ldc ? d->ldc : a.N;
   void* tmp = nullptr;
   const int kind = f8_choose(c, true, a.M, a.N, a.K, d->precision);
-  if (d->out_q && (kind == F8_256 || kind == F8_64x256)) {  // a tile is one block of 128 columns
+  if (d->out_q && (kind == F8_256 || kind == F8_64x256 || kind == F8_128x256)) {  // a tile is one block of 128 columns
     a.oq = d->out_q;
     a.os = d->out_s;
     a.out = nullptr;
