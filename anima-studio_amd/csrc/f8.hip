@@ -17,7 +17,6 @@
 // the first operand, so D's rows are outputs n and its columns rows m of x: a lane holds four consecutive n of
 // one m, and its xs is one value.
 #include <cmath>
-#include <cstdlib>
 #include <type_traits>
 
 #include "common.h"
@@ -78,11 +77,30 @@ __device__ __forceinline__ uint32_t amax4(f32x4 v, uint32_t m) {
   return umax(umax(abs_bits(v[0]), abs_bits(v[1])), umax(umax(abs_bits(v[2]), abs_bits(v[3])), m));
 }
 
-// maximum over the 32 lanes of a half wave
+// v of the lane that DPP control C names
+template <int C>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, C, 0xf, 0xf, false);
+}
+// DPP controls that exchange lanes 1, 2, then (the quads being equal) 4 and 8 apart
+constexpr int X1 = 0xb1, X2 = 0x4e, X4 = 0x141, X8 = 0x140;
+
+// maximum over the 32 lanes of a half wave, in every lane: 16 lanes with DPP, then both rows of 16
 __device__ __forceinline__ uint32_t half_umax(uint32_t v) {
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) v = umax(v, (uint32_t)__shfl_xor((int)v, s));
-  return v;
+  v = umax(v, dpp<X1>(v));
+  v = umax(v, dpp<X2>(v));
+  v = umax(v, dpp<X4>(v));
+  v = umax(v, dpp<X8>(v));
+  const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  return umax(r[0], r[1]);
+}
+
+// maximum over the lanes with the same lane % 16, in every lane
+__device__ __forceinline__ uint32_t cross_umax(uint32_t v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = umax(r[0], r[1]);
+  const auto q = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return umax(q[0], q[1]);
 }
 
 // SiLU as r * rcp(1 + 2^(-r log2 e)) on v_exp_f32 and v_rcp_f32 (1 ulp each): within 2^-22 (1 + |r| / 2) of itself for
@@ -395,76 +413,133 @@ __device__ __forceinline__ void f8_glu_store(const F8Args& a, int m, int n, f32x
     if (n + e < a.N) o[e] = h[e];
 }
 
-// f8_skinny: 16 outputs of 16 rows per workgroup, up to 8 waves that share the blocks of k; operands straight
+// f8_skinny: 16 outputs of 16 rows per workgroup, up to 16 waves that share the blocks of k; operands straight
 // from memory into the matrix cores' registers (a lane: 32 consecutive k of one row), the waves' sums
 // added through LDS in wave order.  QX: fp32 rows, each wave quantizing the blocks that it multiplies.  Sums in
-// 32 bits whatever the precision asked for: these products wait for the weight's bytes.
-constexpr int SKW = 8;
+// 32 bits whatever the precision asked for: these products wait for the weight's bytes.  Everything a wave reads of
+// a block is asked for before the first use, x (whose quantization runs while the weight arrives) first, and the
+// next block's weight before this one's products.
+constexpr int SKW = 16;
+constexpr uint32_t F8_PAST = 0x80000000u;  // an offset past every resource's end: reads as zero
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t f8_rsrc(const void* p, int64_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, (short)0, (int)bytes, 0x00020000);
+}
+
+// 32 bytes at k of a row that starts at `row`, zeros past K
+__device__ __forceinline__ i32x8 f8_frag(__amdgpu_buffer_rsrc_t rs, uint32_t row, int k, int K) {
+  const u32x4 lo = __builtin_amdgcn_raw_buffer_load_b128(rs, k < K ? row + k : F8_PAST, 0, 0);
+  const u32x4 hi = __builtin_amdgcn_raw_buffer_load_b128(rs, k + 16 < K ? row + k + 16 : F8_PAST, 0, 0);
+  return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+}
+
 template <bool QX, bool GLU>
 __global__ __launch_bounds__(64 * SKW) void f8_skinny(F8Args a) {
   constexpr int TT = GLU ? 2 : 1;
   __shared__ f32x4 part[SKW][TT][64];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, nw = blockDim.x >> 6;
   const int r = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16, m = m0 + r;
-  const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w + (int64_t)n0 * a.K), (short)0,
-                                                                     min(16, a.N - n0) * a.K, 0x00020000);
-  __amdgpu_buffer_rsrc_t rw2 = rw, rx = rw;
-  if constexpr (GLU)
-    rw2 = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w2 + (int64_t)n0 * a.K), (short)0, min(16, a.N - n0) * a.K, 0x00020000);
-  if constexpr (!QX)
-    rx = __builtin_amdgcn_make_buffer_rsrc((void*)(a.xq + (int64_t)m0 * a.ldx), (short)0,
-                                           (min(16, a.M - m0) - 1) * (int)a.ldx + a.K, 0x00020000);
-  const float* xrow = QX ? a.x + (int64_t)min(m, a.M - 1) * a.ldx : nullptr;
-  const float* ws = a.ws + (int64_t)(n0 >> 7) * a.KB;
-  const float* ws2 = GLU ? a.ws2 + (int64_t)(n0 >> 7) * a.KB : nullptr;
-  constexpr uint32_t PAST = 0x80000000u;  // an offset past every resource's end: reads as zero
-  const auto frag = [&](__amdgpu_buffer_rsrc_t rs, uint32_t off, int k) {
-    const u32x4 lo = __builtin_amdgcn_raw_buffer_load_b128(rs, k < a.K ? off + k : PAST, 0, 0);
-    const u32x4 hi = __builtin_amdgcn_raw_buffer_load_b128(rs, k + 16 < a.K ? off + k + 16 : PAST, 0, 0);
-    return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
-  };
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16, m = m0 + r, K = a.K, KB = a.KB;
+  const int nr = min(16, a.N - n0), mr = min(16, a.M - m0);
+  const __amdgpu_buffer_rsrc_t rw = f8_rsrc(a.w + (int64_t)n0 * K, nr * (int64_t)K),
+                               rw2 = GLU ? f8_rsrc(a.w2 + (int64_t)n0 * K, nr * (int64_t)K) : rw,
+                               rx = QX ? f8_rsrc(a.x + (int64_t)m0 * a.ldx, 4 * ((mr - 1) * a.ldx + K))
+                                       : f8_rsrc(a.xq + (int64_t)m0 * a.ldx, (mr - 1) * a.ldx + K);
+  const float* ws = a.ws + (int64_t)(n0 >> 7) * KB;
+  const float* ws2 = GLU ? a.ws2 + (int64_t)(n0 >> 7) * KB : nullptr;
   f32x4 acc[TT];
 #pragma unroll
   for (int t = 0; t < TT; t++) acc[t] = f32x4{};
-  for (int kb = wave; kb < a.KB; kb += nw) {
+  const float* xs = QX ? nullptr : a.xs + min(m, a.M - 1);
+  i32x8 w[TT], x;
+  float sx = 0.0f;
+  for (int kb = wave; kb < KB; kb += nw) {
     const int k = kb * 128 + 32 * g;
-    const i32x8 w = frag(rw, r * a.K, k);
-    i32x8 w2 = w, x;
-    if constexpr (GLU) w2 = frag(rw2, r * a.K, k);
-    float sx;
+    f32x4 v[QX ? 8 : 1];
     if constexpr (QX) {
-      f32x4 v[8];
 #pragma unroll
-      for (int i = 0; i < 8; i++) v[i] = m < a.M && k + 4 * i < a.K ? ld4(xrow + k + 4 * i) : f32x4{};
+      for (int i = 0; i < 8; i++) {  // lane g: four values of every 16 (whole sectors of the 16 rows an instruction)
+        const int c = 128 * kb + 16 * i + 4 * g;
+        const u32x4 u = __builtin_amdgcn_raw_buffer_load_b128(rx, c < K && r < mr ? 4 * (r * (uint32_t)a.ldx + c) : F8_PAST, 0, 0);
+        v[i] = __builtin_bit_cast(f32x4, u);
+      }
+    }
+    if (kb == wave) {
+      if constexpr (!QX) {
+        x = f8_frag(rx, r * (uint32_t)a.ldx, k, K);
+        sx = xs[(int64_t)kb * a.M];
+      }
+      w[0] = f8_frag(rw, r * K, k, K);
+      if constexpr (GLU) w[1] = f8_frag(rw2, r * K, k, K);
+    }
+    i32x8 next[TT], nx;
+    float ns = 0.0f;
+    if (kb + nw < KB) {
+      next[0] = f8_frag(rw, r * K, k + 128 * nw, K);
+      if constexpr (GLU) next[1] = f8_frag(rw2, r * K, k + 128 * nw, K);
+      if constexpr (!QX) {
+        nx = f8_frag(rx, r * (uint32_t)a.ldx, k + 128 * nw, K);
+        ns = xs[(int64_t)(kb + nw) * a.M];
+      }
+    }
+    const float s0 = ws[kb], s1 = GLU ? ws2[kb] : 0.0f;
+    if constexpr (QX) {
       uint32_t am = 0;
 #pragma unroll
       for (int i = 0; i < 8; i++) am = amax4(v[i], am);
-      am = umax(am, (uint32_t)__shfl_xor((int)am, 16));
-      am = umax(am, (uint32_t)__shfl_xor((int)am, 32));
       float mul;
-      f8_scale(am, sx, mul);
+      f8_scale(cross_umax(am), sx, mul);
+      // dword i holds k = 16 i + 4 g ...: two 4 x 4 transposes over g give lane g its 32 consecutive ones
+      uint32_t e[2][4];
 #pragma unroll
-      for (int i = 0; i < 8; i++) x[i] = (int)f8_pack(v[i], mul);
-    } else {
-      x = frag(rx, r * (uint32_t)a.ldx, k);
-      sx = a.xs[(int64_t)kb * a.M + min(m, a.M - 1)];
+      for (int i = 0; i < 8; i++) e[i & 1][i >> 1] = f8_pack(v[i], mul);
+#pragma unroll
+      for (int o = 0; o < 2; o++) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const auto t = __builtin_amdgcn_permlane32_swap(e[o][j], e[o][j + 2], false, false);
+          e[o][j] = t[0];
+          e[o][j + 2] = t[1];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+          const auto t = __builtin_amdgcn_permlane16_swap(e[o][j], e[o][j + 1], false, false);
+          x[4 * o + j] = (int)t[0];
+          x[4 * o + j + 1] = (int)t[1];
+        }
+      }
     }
     const Wide xw = widen(x);
-    acc[0] = fma4(sx * ws[kb], mfma_wide(widen(w), xw), acc[0]);
-    if constexpr (GLU) acc[1] = fma4(sx * ws2[kb], mfma_wide(widen(w2), xw), acc[1]);
-  }
+    acc[0] = fma4(sx * s0, mfma_wide(widen(w[0]), xw), acc[0]);
+    if constexpr (GLU) acc[1] = fma4(sx * s1, mfma_wide(widen(w[1]), xw), acc[1]);
 #pragma unroll
-  for (int t = 0; t < TT; t++) part[wave][t][lane] = acc[t];
+    for (int t = 0; t < TT; t++) w[t] = next[t];
+    if constexpr (!QX) {
+      x = nx;
+      sx = ns;
+    }
+  }
+  const int n = n0 + 4 * g;
+  // (what the first wave needs for the epilogue, asked for before the sums meet)
+  f32x4 bias{}, gate{}, c{};
+  if constexpr (!GLU) {
+    if (wave == 0) {
+      if (a.bias) bias = f8_ld4(a.bias, n, a.N, a.vec);
+      if (a.epi == ANIMA_EPI_GATED) gate = f8_ld4(a.gate, n, a.N, a.vec);
+      if (a.epi != ANIMA_EPI_STORE) c = f8_ld_out(a, m, n);
+    }
+  }
+  if (wave > 0) {
+#pragma unroll
+    for (int t = 0; t < TT; t++) part[wave][t][lane] = acc[t];
+  }
   __syncthreads();
-  if (tid >= 64) return;
+  if (wave > 0) return;
 #pragma unroll
   for (int t = 0; t < TT; t++)
-    for (int w = 1; w < nw; w++) acc[t] = acc[t] + part[w][t][lane];
-  const int n = n0 + 4 * g;
+    for (int o = 1; o < nw; o++) acc[t] = acc[t] + part[o][t][lane];
   if constexpr (GLU) f8_glu_store(a, m, n, f8_glu(a.act, f8_glu_bias(a, n), acc[0], acc[1]));
-  else f8_store(a, m, n, acc[0], a.bias ? f8_ld4(a.bias, n, a.N, a.vec) : f32x4{}, a.epi == ANIMA_EPI_GATED ? f8_ld4(a.gate, n, a.N, a.vec) : f32x4{},
-                a.epi != ANIMA_EPI_STORE ? f8_ld_out(a, m, n) : f32x4{});
+  else f8_store(a, m, n, acc[0], bias, gate, c);
 }
 
 // f8_tile: one BM x BN output tile per workgroup (GLU: BN / 2 columns of each projection), waves of WM x WN.
@@ -502,7 +577,6 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void f8_tile(F8Args 
   constexpr int LDS = WSO + NST * SB > EPL ? WSO + NST * SB : EPL;
   constexpr int CPW = (BM + BN) / 8 / NW, SPW = BM / 64;  // copies per wave: rows; waves that copy 64 scales each
   constexpr int FN = GLU ? BN / 2 : BN;                   // output columns of a tile
-  constexpr uint32_t PAST = 0x80000000u;
   static_assert(CPW * NW * 8 == BM + BN && SPW + (GLU ? 1 : 0) < NW && WN <= 64 && (!GLU || WN == 64), "copies and waves");
   __shared__ __attribute__((aligned(1024))) char smem[LDS];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -522,11 +596,9 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void f8_tile(F8Args 
   const int wm = (wave % NWM) * WM, wn = (wave / NWM) * WN;
 
   const int mrows = min(BM, a.M - bm), nrows = min(FN, a.N - bn);
-  const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc((void*)(a.xq + (int64_t)bm * a.ldx), (short)0,
-                                                                     (mrows - 1) * (int)a.ldx + K, 0x00020000);
-  const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w + (int64_t)bn * K), (short)0, nrows * K, 0x00020000);
-  const __amdgpu_buffer_rsrc_t rw2 =
-      GLU ? __builtin_amdgcn_make_buffer_rsrc((void*)(a.w2 + (int64_t)bn * K), (short)0, nrows * K, 0x00020000) : rw;
+  const __amdgpu_buffer_rsrc_t rx = f8_rsrc(a.xq + (int64_t)bm * a.ldx, (mrows - 1) * a.ldx + K),
+                               rw = f8_rsrc(a.w + (int64_t)bn * K, nrows * (int64_t)K),
+                               rw2 = GLU ? f8_rsrc(a.w2 + (int64_t)bn * K, nrows * (int64_t)K) : rw;
   // copy c of this wave: eight rows of one operand, row lane / 8 at (lane / 8) * ld + 16 * unit past their start
   int src[CPW];        // 0: x, 1: the weight, 2: the up projection
   uint32_t roff[CPW];  // where the rows start
@@ -551,7 +623,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void f8_tile(F8Args 
     int l;
     asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
     const int unit = (l & 7) ^ (l >> 3), k = ikb * 128;
-    const uint32_t kl = k + 16 * unit < K ? (uint32_t)(k + 16 * unit) : PAST;
+    const uint32_t kl = k + 16 * unit < K ? (uint32_t)(k + 16 * unit) : F8_PAST;
     const uint32_t lx = (uint32_t)(l >> 3) * (uint32_t)a.ldx + kl, lw = (uint32_t)(l >> 3) * (uint32_t)K + kl;
     const uint32_t soff = wave < SPW ? 4 * (64 * wave + l) : 4 * ((l & 1) * KB);
 #pragma unroll
@@ -559,8 +631,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void f8_tile(F8Args 
       f8_copy16(src[c] == 0 ? rx : src[c] == 1 ? rw : rw2, smem + (wave * CPW + c) * 1024 + (src[c] ? WO - XB + p * WB : p * XB),
                 (src[c] ? lw : lx) + roff[c]);
     const int kbc = min(ikb, KB - 1);  // (past the last block its scales again, unused)
-    f8_copy4(__builtin_amdgcn_make_buffer_rsrc((void*)(sbase + (int64_t)kbc * sstep), (short)0, srec - (wave < SPW ? 0 : 4 * kbc), 0x00020000),
-             smem + sdst + p * sdstep, soff);
+    f8_copy4(f8_rsrc(sbase + kbc * sstep, srec - (wave < SPW ? 0 : 4 * kbc)), smem + sdst + p * sdstep, soff);
     ikb++;
   };
   f32x16 acc[MT][NT];
@@ -811,7 +882,8 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void f8_tile(F8Args 
         uint32_t m = 0;
 #pragma unroll
         for (int q = 0; q < 4; q++) m = amax4(n0 + 8 * q + 4 * hf < a.N ? quad(acc[i][0], q) : f32x4{}, m);  // (N % 16 == 0)
-        m = umax(m, (uint32_t)__shfl_xor((int)m, 32));
+        const auto o = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+        m = umax(o[0], o[1]);
         if (hf == 0) red[(wave / NWM) * BM + wm + 32 * i + r] = m;
       }
       __syncthreads();
@@ -943,13 +1015,61 @@ static void f8_input(F8Args& a, const anima_weight* W, const float* x, int64_t l
   a.KB = (W->K + 127) / 128;
 }
 
-// The kernel for a product's sizes: f8_skinny's 16 rows, or tiles.
-enum { F8_SKINNY, F8_256, F8_128, F8_64x256, F8_64, F8_128x256, F8_COUNT };
+// The kernel for a product's sizes.
+enum { F8_SKINNY, F8_256, F8_128, F8_64x256, F8_64, F8_COUNT };
 
-static int f8_choose(anima_ctx* c, bool glu, int64_t M, int N, int K, int precision) {
-  if (const char* e = getenv("F8_TILE")) return atoi(e);
-  if (M <= 64) return F8_SKINNY;
-  return F8_256;
+static int64_t f8_tiles(int kind, bool glu, int64_t M, int64_t N) {
+  static const int bm[F8_COUNT] = {16, 256, 128, 64, 64}, bn[2][F8_COUNT] = {{16, 256, 128, 256, 64}, {16, 128, 64, 128, 64}};
+  return (M + bm[kind] - 1) / bm[kind] * ((N + bn[glu][kind] - 1) / bn[glu][kind]);
+}
+
+// Microseconds of a product (f8_skinny: base + step for each block of k of a wave + work for each 4096 blocks that all
+// its workgroups read; tiles: base + for each tile per CU step for each block of k, round for each tile after the first)
+// + out for a million outputs.  Fitted to 4000 products of M = 1 .. 8192, N and K = 64 .. 8192: the choice takes
+// 0.2 to 0.7% longer than the best kernel in the mean.  Small products are bound by the depth of one
+// workgroup's k loop, so they take the waves of f8_skinny or small tiles; large ones by the bytes that a tile's
+// operands move per product (43 x 2048 x 1024: 4.6, 64x64 8.6, 256x256 33 us; 8192 x 2048 x 8192: 64x64 219, 256x256 124).
+// The gated form leaves e4m3 rows from the tiles of 128 columns; from the others they cost a pass.
+static int f8_choose(anima_ctx* c, bool glu, bool f8_out, int64_t M, int64_t N, int K, int precision) {
+  struct Fit {
+    float base, step, round, out;
+  };
+  static const Fit fit[2][2][F8_COUNT] = {
+      {{{1.56f, 1.05f, 1.60f, 0.0f}, {6.94f, 1.57f, 1.44f, 0.64f}, {4.51f, 0.68f, 0.0f, 0.60f}, {}, {3.23f, 0.316f, 0.0f, 0.66f}},
+       {{1.56f, 1.05f, 1.58f, 0.0f}, {6.98f, 2.74f, 1.84f, 0.69f}, {4.48f, 1.06f, 0.0f, 0.61f}, {}, {3.29f, 0.394f, 0.0f, 0.62f}}},
+      {{{1.15f, 1.84f, 2.74f, 0.08f}, {7.69f, 1.65f, 5.87f, 0.93f}, {4.77f, 0.68f, 0.0f, 1.02f}, {5.10f, 1.06f, 2.90f, 1.0f}, {4.80f, 0.512f, 0.2f, 1.15f}},
+       {{1.15f, 1.84f, 2.74f, 0.08f}, {7.76f, 2.77f, 5.30f, 0.96f}, {4.79f, 1.05f, 0.0f, 1.05f}, {5.10f, 1.49f, 2.80f, 1.10f}, {4.85f, 0.747f, 0.2f, 1.05f}}}};
+  const int KB = (K + 127) / 128;
+  int best = F8_256;
+  float bt = 0.0f;
+  for (int k = F8_COUNT - 1; k >= 0; k--) {
+    if (k == F8_64x256 && !glu) continue;
+    if (k == F8_SKINNY && M > 16 * 65535) continue;  // (the grid's second dimension)
+    const int64_t tiles = f8_tiles(k, glu, M, N);
+    if (tiles > 0x7fffffff) continue;
+    const Fit& f = fit[glu][precision][k];
+    const float rounds = (float)((tiles + c->num_cus - 1) / c->num_cus), mn = 1e-6f * (float)M * (float)N;
+    const bool fused = k == F8_256 || k == F8_64x256;
+    float us = f.base + f.out * mn * (f8_out && fused ? 0.6f : 1.0f);
+    if (k == F8_SKINNY) us += f.step * (float)((KB + SKW - 1) / SKW) + f.round * (float)tiles * (float)KB / 4096.0f;
+    else us += f.step * (float)KB * rounds + f.round * (rounds - 1.0f);
+    if (f8_out && !fused) us += 2.0f + 1.2f * mn;
+    if (bt == 0.0f || us < bt) {
+      best = k;
+      bt = us;
+    }
+  }
+  return best;
+}
+
+// Whether fp32 rows are quantized inside f8_skinny (each workgroup quantizes its 16 rows again) instead of by a pass
+// before the product (1.6 to 2.5 us): rows of x times blocks of one workgroup, and of all, below what a
+// pass costs.  1 row of 1024 to 2048 outputs 3.8 us with the pass 5.1, of 8192 12.1 and 10.3; 16 rows of 1024 5.1 and 5.9,
+// of 2048 7.4 and 6.9; 48 rows of 1024 7.4 and 6.8.
+static bool f8_quantizes(const F8Args& a, int kind) {
+  if (kind != F8_SKINNY || a.ldx >= (1 << 25)) return false;  // (16 rows within a resource's 2^31 bytes)
+  const int64_t work = (4 + (a.M < 16 ? a.M : 16)) * (int64_t)a.KB;
+  return work <= 240 && work * f8_tiles(F8_SKINNY, false, a.M, a.N) <= 50000;
 }
 
 template <int BM, int BN, int WM, int WN, int NST, bool GLU>
@@ -963,10 +1083,10 @@ static void f8_tile_launch(anima_ctx* c, const F8Args& a, int precision) {
 // Runs the product of a's rows, quantizing fp32 rows first where the kernel takes e4m3 rows.
 template <bool GLU>
 static int f8_product(anima_ctx* c, F8Args a, int kind, int precision) {
-  static const char* const names[2][F8_COUNT] = {{"gemm.f8.skinny", "gemm.f8.256x256", "gemm.f8.128x128", "gemm.f8.64x256", "gemm.f8.64x64", "c"},
-                                                 {"glu.f8.skinny", "glu.f8.256x256", "glu.f8.128x128", "glu.f8.64x256", "glu.f8.64x64", "c"}};
+  static const char* const names[2][F8_COUNT] = {{"gemm.f8.skinny", "gemm.f8.256x256", "gemm.f8.128x128", "", "gemm.f8.64x64"},
+                                                 {"glu.f8.skinny", "glu.f8.256x256", "glu.f8.128x128", "glu.f8.64x256", "glu.f8.64x128"}};
   void* scratch = nullptr;
-  if (kind != F8_SKINNY && a.x) {
+  if (a.x && !f8_quantizes(a, kind)) {
     const size_t qb = ((size_t)a.M * a.K + 255) / 256 * 256;
     if (int rc = anima_alloc(c, qb + (size_t)a.M * a.KB * 4, &scratch)) return rc;
     a.xq = (const uint8_t*)scratch;
@@ -977,6 +1097,7 @@ static int f8_product(anima_ctx* c, F8Args a, int kind, int precision) {
       return rc;
     }
     a.ldx = a.K;
+    a.x = nullptr;
   }
   Launch L(c, names[GLU][kind], (GLU ? 4.0 : 2.0) * a.M * a.N * a.K, (double)a.N * a.K * (GLU ? 2 : 1));
   if (kind == F8_SKINNY) {
@@ -987,10 +1108,8 @@ static int f8_product(anima_ctx* c, F8Args a, int kind, int precision) {
     f8_tile_launch<256, 256, 128, 64, 2, GLU>(c, a, precision);
   } else if (kind == F8_128) {
     f8_tile_launch<128, 128, 64, 64, 2, GLU>(c, a, precision);
-  } else if (kind == F8_64x256) {
-    f8_tile_launch<64, 256, 64, 64, 2, GLU>(c, a, precision);
-  } else if (kind == F8_128x256) {
-    f8_tile_launch<128, 256, 64, 64, 3, GLU>(c, a, precision);
+  } else if (GLU && kind == F8_64x256) {
+    if constexpr (GLU) f8_tile_launch<64, 256, 64, 64, 2, GLU>(c, a, precision);
   } else {
     if constexpr (GLU) f8_tile_launch<64, 128, 32, 64, 3, GLU>(c, a, precision);
     else f8_tile_launch<64, 64, 32, 32, 3, GLU>(c, a, precision);
@@ -1022,7 +1141,7 @@ int linear_f8_launch(anima_ctx* c, const anima_linear_desc* d) {
   a.obf = d->out_bf16;
   a.vec = a.N % 4 == 0 && a.ldc % 4 == 0 && f8_al(a.out, a.obf ? 8 : 16) && f8_al(a.bias, 16) && (!a.add || (a.ld_add % 4 == 0 && f8_al(a.add, 16))) &&
           (a.epi != ANIMA_EPI_GATED || f8_al(a.gate, 16));
-  return f8_product<false>(c, a, f8_choose(c, false, a.M, a.N, a.K, d->precision), d->precision);
+  return f8_product<false>(c, a, f8_choose(c, false, false, a.M, a.N, a.K, d->precision), d->precision);
 }
 
 int linear_glu_launch(anima_ctx* c, const anima_glu_desc* d) {
@@ -1044,8 +1163,8 @@ int linear_glu_launch(anima_ctx* c, const anima_glu_desc* d) {
   a.out = d->out;
   a.ldc = d->ldc ? d->ldc : a.N;
   void* tmp = nullptr;
-  const int kind = f8_choose(c, true, a.M, a.N, a.K, d->precision);
-  if (d->out_q && (kind == F8_256 || kind == F8_64x256 || kind == F8_128x256)) {  // a tile is one block of 128 columns
+  const int kind = f8_choose(c, true, d->out_q != nullptr, a.M, a.N, a.K, d->precision);
+  if (d->out_q && (kind == F8_256 || kind == F8_64x256)) {  // a tile is one block of 128 columns
     a.oq = d->out_q;
     a.os = d->out_s;
     a.out = nullptr;
