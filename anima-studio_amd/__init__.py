@@ -465,11 +465,11 @@ class Context:
         GEMM's epilogue (A products [M][ld_lora_xa] fp32, B as three bf16 planes [3][N][lora_r]);
         lora_cols > 0: block-diagonal ranks, column n reading xa columns (n // lora_cols) * lora_r
         + k."""
-        d = LinearDesc(M=M, W=ctypes.pointer(W), x=_ptr(x), ldx=ldx, x_rotated=int(x_rotated), xq=_ptr(xq),
-                       xs=_ptr(xs), out=_ptr(out), ldc=ldc, alpha=alpha, act=ACT[act] if isinstance(act, str) else act,
-                       epilogue=epilogue, gate=_ptr(gate), gate_off=gate_off, acc_out=_ptr(acc_out), add=_ptr(add),
-                       ld_add=ld_add, lora_xa=_ptr(lora_xa), ld_lora_xa=ld_lora_xa, lora_b=_ptr(lora_b),
-                       lora_r=lora_r, lora_cols=lora_cols, precision=precision, out_bf16=int(out_bf16))
+        # (the fields in order, absent pointers as they are: half the time of keywords, on every short call)
+        d = LinearDesc(M, ctypes.pointer(W), x and _ptr(x), ldx, int(x_rotated), xq and _ptr(xq), xs and _ptr(xs),
+                       _ptr(out), ldc, alpha, ACT[act] if isinstance(act, str) else act, epilogue, gate and _ptr(gate),
+                       gate_off, acc_out and _ptr(acc_out), add and _ptr(add), ld_add, lora_xa and _ptr(lora_xa),
+                       ld_lora_xa, lora_b and _ptr(lora_b), lora_r, lora_cols, precision, int(out_bf16))
         return self._check(lib().anima_linear(self.h, ctypes.byref(d)))
 
     def linear_qkv(self, W, M, out, *, B, L, H, k_norm=None, rope_cs=None, rope_sin_off=0, kv_prep=None, eps=1e-6,
@@ -505,9 +505,9 @@ class Context:
                    out_s=None, precision=PREC_BF16):
         """anima_linear_glu: act(x W_gate^T) * (x W_up^T) of two W_F8 weights, from fp32 rows x or e4m3 rows
         xq, xs, into fp32 rows out or e4m3 rows out_q, out_s."""
-        d = GluDesc(M=M, gate=ctypes.pointer(gate), up=ctypes.pointer(up), x=_ptr(x), xq=_ptr(xq), xs=_ptr(xs), ldx=ldx,
-                    act=ACT[act] if isinstance(act, str) else act, out=_ptr(out), ldc=ldc, out_q=_ptr(out_q),
-                    out_s=_ptr(out_s), precision=precision)
+        d = GluDesc(M, ctypes.pointer(gate), ctypes.pointer(up), x and _ptr(x), xq and _ptr(xq), xs and _ptr(xs), ldx,
+                    ACT[act] if isinstance(act, str) else act, out and _ptr(out), ldc, out_q and _ptr(out_q),
+                    out_s and _ptr(out_s), precision)
         return self._check(lib().anima_linear_glu(self.h, ctypes.byref(d)))
 
     def residual_norm(self, rows, cols, x, *, ldx=0, y=None, ldy=0, y_bf16=False, post_w=None, gate=None, gate_ld=0, res_scale=0.0,
@@ -515,10 +515,10 @@ class Context:
                       q=None, s=None):
         """anima_residual_norm: x += res_scale * gate * post(y) in place, then the norm of x (norm "rms" /
         "layer", norm_w, shift / scale) as fp32 rows h and / or e4m3 rows q, s."""
-        d = ResNormDesc(rows=rows, cols=cols, x=_ptr(x), ldx=ldx, y=_ptr(y), ldy=ldy, post_w=_ptr(post_w), gate=_ptr(gate),
-                        gate_ld=gate_ld, res_scale=res_scale, norm=NORM[norm] if isinstance(norm, str) else norm,
-                        norm_w=_ptr(norm_w), shift=_ptr(shift), scale=_ptr(scale), mod_ld=mod_ld, group_rows=group_rows,
-                        eps=eps, h=_ptr(h), ldh=ldh, q=_ptr(q), s=_ptr(s), y_bf16=int(y_bf16))
+        d = ResNormDesc(rows, cols, _ptr(x), ldx, y and _ptr(y), ldy, post_w and _ptr(post_w), gate and _ptr(gate), gate_ld,
+                        res_scale, NORM[norm] if isinstance(norm, str) else norm, norm_w and _ptr(norm_w),
+                        shift and _ptr(shift), scale and _ptr(scale), mod_ld, group_rows, eps, h and _ptr(h), ldh,
+                        q and _ptr(q), s and _ptr(s), int(y_bf16))
         return self._check(lib().anima_residual_norm(self.h, ctypes.byref(d)))
 
     def split3_bf16(self, src, dst, n):
@@ -576,8 +576,8 @@ def dit_rope_table(Hp: int, Wp: int) -> np.ndarray:
 
 
 def _ptr(b):
-    if b is None:
-        return None
+    if b is None or type(b) is int:
+        return b
     if isinstance(b, DeviceBuffer):
         return b.ptr
     return int(b)

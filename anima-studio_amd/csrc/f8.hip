@@ -62,7 +62,11 @@ __device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b 
 // A block's scale and the factor its values are multiplied with, from the bits of its largest magnitude.
 __device__ __forceinline__ void f8_scale(uint32_t amax, float& scale, float& mul) {
   const float a = __builtin_bit_cast(float, umax(amax, F8_TINY));
-  scale = a / F8_TOP;
+  // a / 448 rounded once: the product with 1 / 448 corrected by its exact remainder (equal to the quotient for all 2^23
+  // fractions of a; a is no subnormal), an infinity or NaN as the quotient's
+  constexpr float y = 1.0f / F8_TOP;
+  const float q = a * y;
+  scale = __builtin_amdgcn_div_fixupf(__builtin_fmaf(__builtin_fmaf(-F8_TOP, q, a), y, q), F8_TOP, a);
   mul = F8_TOP * (1.0f / a);
 }
 
@@ -75,6 +79,10 @@ __device__ __forceinline__ uint32_t f8_pack(f32x4 v, float mul) {
 
 __device__ __forceinline__ uint32_t amax4(f32x4 v, uint32_t m) {
   return umax(umax(abs_bits(v[0]), abs_bits(v[1])), umax(umax(abs_bits(v[2]), abs_bits(v[3])), m));
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t f8_rsrc(const void* p, int64_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, (short)0, (int)bytes, 0x00020000);
 }
 
 // v of the lane that DPP control C names
@@ -125,19 +133,66 @@ __device__ __forceinline__ f32x4 ld4(const uint16_t* p) {
                __builtin_bit_cast(float, u.y << 16), __builtin_bit_cast(float, u.y & 0xffff0000u)};
 }
 
-// A half wave per block of 128 columns (a lane: four of them), blocks in row order.
-template <class T>
-__global__ __launch_bounds__(256) void quant_rows_f8_kernel(const T* X, int64_t ldx, int M, int K, int KB, uint8_t* Q, float* S) {
-  const int l = threadIdx.x & 31;
-  const int64_t b = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int64_t m = b / KB;
-  const int kb = (int)(b - m * KB), k = kb * 128 + 4 * l;
-  const bool in = m < M && k < K;
-  const f32x4 v = in ? ld4(X + m * ldx + k) : f32x4{};
-  float scale, mul;
-  f8_scale(half_umax(amax4(v, 0)), scale, mul);
-  if (in) *(uint32_t*)(Q + m * K + k) = f8_pack(v, mul);
-  if (l == 0 && m < M) S[(int64_t)kb * M + m] = scale;
+// n / d for n < 2^31 by a multiplication: d = 1, or (n * mul >> 32) >> shift with mul = floor(2^(32 + shift) / d) + 1 and
+// 2^shift < d <= 2^(shift + 1), which is exact there (the excess, below n / 2^(32 + shift) < 1 / d, changes no quotient).
+struct DivBy {
+  uint32_t d, mul, shift;
+};
+static DivBy div_by(uint32_t d) {
+  uint32_t l = 0;
+  while ((2u << l) < d) l++;
+  return d < 2 ? DivBy{1, 0, 0} : DivBy{d, (uint32_t)(((uint64_t)1 << (32 + l)) / d + 1), l};
+}
+__device__ __forceinline__ uint32_t div_u31(uint32_t n, const DivBy& d) { return d.d == 1 ? n : __umulhi(n, d.mul) >> d.shift; }
+
+// eight values of a row
+struct Eight {
+  f32x4 lo, hi;
+};
+__device__ __forceinline__ Eight ld8(const float* p) { return {ld4(p), ld4(p + 4)}; }
+__device__ __forceinline__ Eight ld8(const uint16_t* p) {
+  const uint4 u = *(const uint4*)p;
+  const auto two = [](uint32_t a, uint32_t b) {
+    return f32x4{__builtin_bit_cast(float, a << 16), __builtin_bit_cast(float, a & 0xffff0000u), __builtin_bit_cast(float, b << 16),
+                 __builtin_bit_cast(float, b & 0xffff0000u)};
+  };
+  return {two(u.x, u.y), two(u.z, u.w)};
+}
+
+// 16 lanes per block of 128 columns (a lane: eight of them, whose maximum takes four DPP steps), blocks in row
+// order, U of them 16 workgroup threads' blocks apart so that their loads are in flight together.  Bound by the bytes:
+// 8192 x 2048 bf16 rows (50 MB)
+template <class T, int U>
+__global__ __launch_bounds__(256) void quant_rows_f8_kernel(const T* X, int64_t ldx, uint32_t blocks, int K, int64_t M, DivBy KB, uint8_t* Q,
+                                                            float* S) {
+  const int l = threadIdx.x & 15;
+  const uint32_t b0 = (uint32_t)xcd_remap(blockIdx.x, gridDim.x) * (16 * U) + (threadIdx.x >> 4);
+  Eight v[U];
+  uint32_t m[U], kb[U];
+  bool in[U];
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    const uint32_t b = b0 + 16 * u;
+    m[u] = div_u31(b, KB);
+    kb[u] = b - m[u] * KB.d;
+    const int k = (int)kb[u] * 128 + 8 * l;
+    in[u] = b < blocks && k < K;
+    v[u] = in[u] ? ld8(X + (int64_t)m[u] * ldx + k) : Eight{};
+  }
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    uint32_t a = amax4(v[u].hi, amax4(v[u].lo, 0));
+    a = umax(a, dpp<X1>(a));
+    a = umax(a, dpp<X2>(a));
+    a = umax(a, dpp<X4>(a));
+    a = umax(a, dpp<X8>(a));
+    float scale, mul;
+    f8_scale(a, scale, mul);
+    if (in[u]) {
+      *(uint2*)(Q + (int64_t)m[u] * K + kb[u] * 128 + 8 * l) = make_uint2(f8_pack(v[u].lo, mul), f8_pack(v[u].hi, mul));
+      if (l == 0) S[(int64_t)kb[u] * M + m[u]] = scale;
+    }
+  }
 }
 
 // A workgroup per 128 x 128 block: thread t holds columns 4 (t % 32) .. + 3 of rows t / 32 + 8 i.
@@ -183,10 +238,24 @@ struct NormArgs {
   int rows, cols, layer, y_bf16;
 };
 
+// Sum over a wave, in every lane: 16 lanes with DPP, then both halves of 32 and of 64.
+__device__ __forceinline__ float wave_fsum(float v) {
+  const auto bits = [](float f) { return __builtin_bit_cast(uint32_t, f); };
+  const auto val = [](uint32_t u) { return __builtin_bit_cast(float, u); };
+  v += val(dpp<X1>(bits(v)));
+  v += val(dpp<X2>(bits(v)));
+  v += val(dpp<X4>(bits(v)));
+  v += val(dpp<X8>(bits(v)));
+  const auto r = __builtin_amdgcn_permlane16_swap(bits(v), bits(v), false, false);
+  v = val(r[0]) + val(r[1]);
+  const auto q = __builtin_amdgcn_permlane32_swap(bits(v), bits(v), false, false);
+  return val(q[0]) + val(q[1]);
+}
+
 // Sum over the workgroup of T threads; `red` holds T / 64 floats, of its own for each use.
 template <int T>
 __device__ __forceinline__ float group_sum(float v, float* red) {
-  v = wave_sum(v);
+  v = wave_fsum(v);
   if constexpr (T == 64) return v;
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -196,28 +265,55 @@ __device__ __forceinline__ float group_sum(float v, float* red) {
   return v;
 }
 
-// A workgroup per row, the row in registers: thread t holds the four-column groups t + T i, i < NV.
-template <int T, int NV>
-__global__ __launch_bounds__(T) void residual_norm_kernel(NormArgs a) {
+// A workgroup per row, the row in registers: thread t holds the four-column groups t + T i, i < NV.  EARLY: the vectors
+// are asked for together with the row (few rows: one wait for memory instead of three); otherwise where they are
+// needed, other rows' waves covering the wait.
+template <int T, int NV, bool EARLY>
+__global__ __launch_bounds__(T, EARLY ? 1 : 4) void residual_norm_kernel(NormArgs a) {
   __shared__ float red[3][T / 64];
   const int t = threadIdx.x;
-  const int64_t row = blockIdx.x, grp = row / a.group_rows;
+  const uint32_t row32 = xcd_remap(blockIdx.x, gridDim.x);
+  const int64_t row = row32, grp = a.group_rows >= a.rows ? 0 : row32 / (uint32_t)a.group_rows;
   const float inv = 1.0f / (float)a.cols;
-  f32x4 x[NV];
-  float* xr = a.x + row * a.ldx;
+  // every access through a resource of the row's bytes: past its end loads give zeros and stores nothing
+  const __amdgpu_buffer_rsrc_t rx = f8_rsrc(a.x + row * a.ldx, 4 * a.cols);
+  const auto load = [&](__amdgpu_buffer_rsrc_t rs, int i) {
+    return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, 16 * t, 16 * T * i, 0));
+  };
+  const auto vec = [&](const float* p, int i) { return p ? load(f8_rsrc(p, 4 * a.cols), i) : f32x4{}; };
+  const float *gate = a.gate ? a.gate + grp * a.gate_ld : nullptr, *scale = a.scale ? a.scale + grp * a.mod_ld : nullptr,
+              *shift = a.scale ? a.shift + grp * a.mod_ld : nullptr;
+  f32x4 x[NV], y[NV];
 #pragma unroll
-  for (int i = 0; i < NV; i++) {
-    const int c = 4 * (t + T * i);
-    x[i] = c < a.cols ? ld4(xr + c) : f32x4{};
-  }
+  for (int i = 0; i < NV; i++) x[i] = load(rx, i);
   if (a.y) {
-    f32x4 y[NV];
+    if (a.y_bf16) {
+      const __amdgpu_buffer_rsrc_t ry = f8_rsrc((const uint16_t*)a.y + row * a.ldy, 2 * a.cols);
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        const auto u = __builtin_amdgcn_raw_buffer_load_b64(ry, 8 * t, 8 * T * i, 0);
+        y[i] = f32x4{__builtin_bit_cast(float, u[0] << 16), __builtin_bit_cast(float, u[0] & 0xffff0000u), __builtin_bit_cast(float, u[1] << 16),
+                     __builtin_bit_cast(float, u[1] & 0xffff0000u)};
+      }
+    } else {
+      const __amdgpu_buffer_rsrc_t ry = f8_rsrc((const float*)a.y + row * a.ldy, 4 * a.cols);
+#pragma unroll
+      for (int i = 0; i < NV; i++) y[i] = load(ry, i);
+    }
+  }
+  constexpr int E = EARLY ? NV : 1;
+  f32x4 pe[E], ge[E], we[E], ce[E], se[E];
+  if constexpr (EARLY) {
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const int c = 4 * (t + T * i);
-      y[i] = f32x4{};
-      if (c < a.cols) y[i] = a.y_bf16 ? ld4((const uint16_t*)a.y + row * a.ldy + c) : ld4((const float*)a.y + row * a.ldy + c);
+      pe[i] = vec(a.post_w, i);
+      ge[i] = vec(gate, i);
+      we[i] = vec(a.norm_w, i);
+      ce[i] = vec(scale, i);
+      se[i] = vec(shift, i);
     }
+  }
+  if (a.y) {
     if (a.post_w) {
       float ss = 0.0f;
 #pragma unroll
@@ -226,63 +322,64 @@ __global__ __launch_bounds__(T) void residual_norm_kernel(NormArgs a) {
         for (int e = 0; e < 4; e++) ss = __builtin_fmaf(y[i][e], y[i][e], ss);
       const float r = 1.0f / sqrtf(group_sum<T>(ss, red[0]) * inv + a.eps);
 #pragma unroll
-      for (int i = 0; i < NV; i++) {
-        const int c = 4 * (t + T * i);
-        if (c < a.cols) y[i] = y[i] * r * ld4(a.post_w + c);
-      }
+      for (int i = 0; i < NV; i++) y[i] = y[i] * r * (EARLY ? pe[i % E] : vec(a.post_w, i));
+    }
+    if (gate) {
+#pragma unroll
+      for (int i = 0; i < NV; i++) y[i] = y[i] * (EARLY ? ge[i % E] : vec(gate, i));
     }
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const int c = 4 * (t + T * i);
-      if (c < a.cols) {
-        if (a.gate) y[i] = y[i] * ld4(a.gate + grp * a.gate_ld + c);
 #pragma unroll
-        for (int e = 0; e < 4; e++) x[i][e] = __builtin_fmaf(a.res_scale, y[i][e], x[i][e]);
-        *(f32x4*)(xr + c) = x[i];
-      }
+      for (int e = 0; e < 4; e++) x[i][e] = __builtin_fmaf(a.res_scale, y[i][e], x[i][e]);
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x[i]), rx, 16 * t, 16 * T * i, 0);
     }
   }
-  float mean = 0.0f;
   if (a.layer) {
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; i++) s += (x[i][0] + x[i][1]) + (x[i][2] + x[i][3]);
-    mean = group_sum<T>(s, red[1]) * inv;
+    const float mean = group_sum<T>(s, red[1]) * inv;
+    const bool whole = a.cols == 4 * T * NV;  // (past the row x stays zero)
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[i][e] -= whole || 4 * (t + T * i) < a.cols ? mean : 0.0f;
   }
   float ss = 0.0f;
 #pragma unroll
-  for (int i = 0; i < NV; i++) {
-    const int c = 4 * (t + T * i);
-    if (c < a.cols) {
+  for (int i = 0; i < NV; i++)
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        x[i][e] -= mean;
-        ss = __builtin_fmaf(x[i][e], x[i][e], ss);
-      }
-    }
-  }
+    for (int e = 0; e < 4; e++) ss = __builtin_fmaf(x[i][e], x[i][e], ss);
   const float r = 1.0f / sqrtf(group_sum<T>(ss, red[2]) * inv + a.eps);
 #pragma unroll
-  for (int i = 0; i < NV; i++) {
-    const int c = 4 * (t + T * i);
-    const bool in = c < a.cols;
-    f32x4 h = x[i] * r;
-    if (in) {
-      if (a.norm_w) h = h * ld4(a.norm_w + c);
-      if (a.scale) {
-        const f32x4 sc = ld4(a.scale + grp * a.mod_ld + c), sh = ld4(a.shift + grp * a.mod_ld + c);
+  for (int i = 0; i < NV; i++) x[i] = x[i] * r;
+  if (a.norm_w) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) h[e] = __builtin_fmaf(h[e], 1.0f + sc[e], sh[e]);
-      }
-      if (a.h) *(f32x4*)(a.h + row * a.ldh + c) = h;
+    for (int i = 0; i < NV; i++) x[i] = x[i] * (EARLY ? we[i % E] : vec(a.norm_w, i));
+  }
+  if (scale) {
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const f32x4 sc = EARLY ? ce[i % E] : vec(scale, i), sh = EARLY ? se[i % E] : vec(shift, i);
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[i][e] = __builtin_fmaf(x[i][e], 1.0f + sc[e], sh[e]);
     }
-    if (a.q) {  // 32 lanes hold one block of 128 columns (zeros past the row)
-      float scale, mul;
-      f8_scale(half_umax(amax4(in ? h : f32x4{}, 0)), scale, mul);
-      if (in) {
-        *(uint32_t*)(a.q + row * a.cols + c) = f8_pack(h, mul);
-        if ((t & 31) == 0) a.s[(int64_t)(c >> 7) * a.rows + row] = scale;
-      }
+  }
+  if (a.h) {
+    const __amdgpu_buffer_rsrc_t rh = f8_rsrc(a.h + row * a.ldh, 4 * a.cols);
+#pragma unroll
+    for (int i = 0; i < NV; i++) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x[i]), rh, 16 * t, 16 * T * i, 0);
+  }
+  if (a.q) {  // 32 lanes hold one block of 128 columns (zeros past the row)
+    const __amdgpu_buffer_rsrc_t rq = f8_rsrc(a.q + row * a.cols, a.cols);
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      float sc, mul;
+      f8_scale(half_umax(amax4(x[i], 0)), sc, mul);
+      __builtin_amdgcn_raw_buffer_store_b32(f8_pack(x[i], mul), rq, 4 * t, 4 * T * i, 0);
+      const int c = 4 * (t + T * i);
+      if ((t & 31) == 0 && c < a.cols) a.s[(int64_t)(c >> 7) * a.rows + row] = sc;
     }
   }
 }
@@ -421,10 +518,6 @@ __device__ __forceinline__ void f8_glu_store(const F8Args& a, int m, int n, f32x
 // next block's weight before this one's products.
 constexpr int SKW = 16;
 constexpr uint32_t F8_PAST = 0x80000000u;  // an offset past every resource's end: reads as zero
-
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t f8_rsrc(const void* p, int64_t bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc((void*)p, (short)0, (int)bytes, 0x00020000);
-}
 
 // 32 bytes at k of a row that starts at `row`, zeros past K
 __device__ __forceinline__ i32x8 f8_frag(__amdgpu_buffer_rsrc_t rs, uint32_t row, int k, int K) {
@@ -934,14 +1027,26 @@ int quant_rows_f8_launch(anima_ctx* c, const void* x, int x_bf16, int64_t M, int
   if (M == 0) return ANIMA_OK;
   OnDevice on(c);
   const int KB = (K + 127) / 128;
-  const int64_t groups = (M * KB + 7) / 8, ld = ldx ? ldx : K;
-  if (groups > 0x7fffffff) return fail(c, ANIMA_E_UNSUPPORTED, "anima_quant_rows_f8: %lld blocks", (long long)(M * KB));
+  const int64_t ld = ldx ? ldx : K;
+  const DivBy div = div_by((uint32_t)KB);
   Launch L(c, x_bf16 ? "quant.f8.bf16" : "quant.f8", 0.0, (double)M * K * (x_bf16 ? 3 : 5));
-  if (x_bf16)
-    hipLaunchKernelGGL(quant_rows_f8_kernel<uint16_t>, dim3((unsigned)groups), dim3(256), 0, c->stream, (const uint16_t*)x, ld, (int)M, K,
-                       KB, q, s);
-  else
-    hipLaunchKernelGGL(quant_rows_f8_kernel<float>, dim3((unsigned)groups), dim3(256), 0, c->stream, (const float*)x, ld, (int)M, K, KB, q, s);
+  const int64_t part = (1 << 30) / KB;  // rows of a launch: their blocks are counted in 31 bits
+  for (int64_t m = 0; m < M; m += part) {
+    const uint32_t blocks = (uint32_t)((M - m < part ? M - m : part) * KB);
+    const bool many = blocks >= 65536;  // (two blocks in flight per thread once the workgroups fill the chip)
+    const dim3 grid((blocks + (many ? 31 : 15)) / (many ? 32 : 16)), block(256);
+#define QR(T, U)                                                                                                                   \
+  hipLaunchKernelGGL((quant_rows_f8_kernel<T, U>), grid, block, 0, c->stream, (const T*)x + m * ld, ld, blocks, K, M, div, q + m * K, \
+                     s + m)
+    if (x_bf16) {
+      if (many) QR(uint16_t, 2);
+      else QR(uint16_t, 1);
+    } else {
+      if (many) QR(float, 2);
+      else QR(float, 1);
+    }
+#undef QR
+  }
   return L.end();
 }
 
@@ -992,14 +1097,24 @@ int residual_norm_launch(anima_ctx* c, const anima_resnorm_desc* d) {
                    d->y_bf16};
   const dim3 grid((unsigned)d->rows);
   Launch L(c, "residual_norm", 0.0, (double)d->rows * C * ((d->y ? d->y_bf16 ? 10.0 : 12.0 : 4.0) + (d->h ? 4 : 0) + (d->q ? 1 : 0)));
-#define RN(T, NV) hipLaunchKernelGGL((residual_norm_kernel<T, NV>), grid, dim3(T), 0, c->stream, a)
-  if (C <= 256) RN(64, 1);
-  else if (C <= 512) RN(64, 2);
-  else if (C <= 1024) RN(64, 4);
-  else if (C <= 2048) RN(128, 4);
-  else if (C <= 4096) RN(256, 4);
-  else if (C <= 8192) RN(512, 4);
-  else RN(1024, 4);
+#define RN(T, NV, EARLY) hipLaunchKernelGGL((residual_norm_kernel<T, NV, EARLY>), grid, dim3(T), 0, c->stream, a)
+  if (d->rows <= 4 * c->num_cus) {
+    if (C <= 256) RN(64, 1, true);
+    else if (C <= 512) RN(128, 1, true);
+    else if (C <= 1024) RN(256, 1, true);
+    else if (C <= 2048) RN(256, 2, true);
+    else if (C <= 4096) RN(512, 2, true);
+    else if (C <= 8192) RN(1024, 2, true);
+    else RN(1024, 4, true);
+  } else {
+    if (C <= 256) RN(64, 1, false);
+    else if (C <= 512) RN(64, 2, false);
+    else if (C <= 1024) RN(64, 4, false);
+    else if (C <= 2048) RN(64, 8, false);
+    else if (C <= 4096) RN(128, 8, false);
+    else if (C <= 8192) RN(256, 8, false);
+    else RN(512, 8, false);
+  }
 #undef RN
   return L.end();
 }
