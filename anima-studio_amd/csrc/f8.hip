@@ -1152,8 +1152,8 @@ static int f8_choose(anima_ctx* c, bool glu, bool f8_out, int64_t M, int64_t N, 
   static const Fit fit[2][2][F8_COUNT] = {
       {{{1.56f, 1.05f, 1.60f, 0.0f}, {6.94f, 1.57f, 1.44f, 0.64f}, {4.51f, 0.68f, 0.0f, 0.60f}, {}, {3.23f, 0.316f, 0.0f, 0.66f}},
        {{1.56f, 1.05f, 1.58f, 0.0f}, {6.98f, 2.74f, 1.84f, 0.69f}, {4.48f, 1.06f, 0.0f, 0.61f}, {}, {3.29f, 0.394f, 0.0f, 0.62f}}},
-      {{{1.15f, 1.84f, 2.74f, 0.08f}, {7.69f, 1.65f, 5.87f, 0.93f}, {4.77f, 0.68f, 0.0f, 1.02f}, {5.10f, 1.06f, 2.90f, 1.0f}, {4.80f, 0.512f, 0.2f, 1.15f}},
-       {{1.15f, 1.84f, 2.74f, 0.08f}, {7.76f, 2.77f, 5.30f, 0.96f}, {4.79f, 1.05f, 0.0f, 1.05f}, {5.10f, 1.49f, 2.80f, 1.10f}, {4.85f, 0.747f, 0.2f, 1.05f}}}};
+      {{{1.15f, 1.84f, 2.74f, 0.08f}, {7.69f, 1.65f, 5.87f, 0.93f}, {4.77f, 0.68f, 0.0f, 1.02f}, {4.80f, 0.80f, 2.90f, 1.0f}, {4.80f, 0.512f, 0.2f, 1.15f}},
+       {{1.15f, 1.84f, 2.74f, 0.08f}, {7.76f, 2.77f, 5.30f, 0.96f}, {4.79f, 1.05f, 0.0f, 1.05f}, {4.80f, 1.15f, 2.90f, 1.02f}, {4.85f, 0.747f, 0.2f, 1.05f}}}};
   const int KB = (K + 127) / 128;
   int best = F8_256;
   float bt = 0.0f;
@@ -1224,7 +1224,7 @@ static int f8_product(anima_ctx* c, F8Args a, int kind, int precision) {
   } else if (kind == F8_128) {
     f8_tile_launch<128, 128, 64, 64, 2, GLU>(c, a, precision);
   } else if (GLU && kind == F8_64x256) {
-    if constexpr (GLU) f8_tile_launch<64, 256, 64, 64, 2, GLU>(c, a, precision);
+    if constexpr (GLU) f8_tile_launch<64, 256, 32, 64, 2, GLU>(c, a, precision);
   } else {
     if constexpr (GLU) f8_tile_launch<64, 128, 32, 64, 3, GLU>(c, a, precision);
     else f8_tile_launch<64, 64, 32, 32, 3, GLU>(c, a, precision);
