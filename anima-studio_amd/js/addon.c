@@ -723,7 +723,8 @@ static napi_value js_fill_random(napi_env env, napi_callback_info info) {
 }
 
 /* linear(ctx, W, desc): W = {kind, N, K, w, scale, srel, codebook, bias}, desc mirrors
- * anima_linear_desc (x, ldx, xRotated, xq, xs, out, ldc, alpha, act, epilogue, gate, gOff, accOut) */
+ * anima_linear_desc (x, ldx, xRotated, xq, xs, out, ldc, alpha, act, epilogue, gate, gOff, accOut,
+ * precision, outBf16) */
 /* the weight object {kindId, N, K, buf, scale, srel, codebook, bias} of ops.mjs weightArg */
 static void read_weight(napi_env env, napi_value wo, anima_weight* w) {
   memset(w, 0, sizeof *w);
@@ -779,7 +780,93 @@ static napi_value js_linear(napi_env env, napi_callback_info info) {
   d.lora_b = (const uint16_t*)pptr(env, o, "loraB");
   d.lora_r = (int)pnum(env, o, "loraR");
   d.lora_cols = (int)pnum(env, o, "loraCols");
+  d.precision = (int)pnum(env, o, "precision");
+  d.out_bf16 = (int)pnum(env, o, "outBf16");
   CHECK_RC(env, c, anima_linear(c, &d));
+  return NULL;
+}
+
+/* quantRowsF8(ctx, x, bf16, M, K, ldx, q, s): anima_quant_rows_f8 */
+static napi_value js_quant_rows_f8(napi_env env, napi_callback_info info) {
+  napi_value a[8];
+  get_args(env, info, 8, a);
+  anima_ctx* c = ctx_of(env, a[0]);
+  CHECK_RC(env, c, anima_quant_rows_f8(c, ptr(env, a[1]), (int)num(env, a[2]), i64(env, a[3]), (int)num(env, a[4]),
+                                       i64(env, a[5]), (uint8_t*)ptr(env, a[6]), (float*)ptr(env, a[7])));
+  return NULL;
+}
+
+/* weightQuantF8(ctx, w, bf16, N, K, q, scale): anima_weight_quant_f8 */
+static napi_value js_weight_quant_f8(napi_env env, napi_callback_info info) {
+  napi_value a[7];
+  get_args(env, info, 7, a);
+  anima_ctx* c = ctx_of(env, a[0]);
+  CHECK_RC(env, c, anima_weight_quant_f8(c, ptr(env, a[1]), (int)num(env, a[2]), (int)num(env, a[3]), (int)num(env, a[4]),
+                                         (uint8_t*)ptr(env, a[5]), (float*)ptr(env, a[6])));
+  return NULL;
+}
+
+/* linearGlu(ctx, gate, up, desc): desc mirrors anima_glu_desc (M, x, xq, xs, ldx, act, out, ldc,
+ * outQ, outS, precision) */
+static napi_value js_linear_glu(napi_env env, napi_callback_info info) {
+  napi_value a[4];
+  get_args(env, info, 4, a);
+  anima_ctx* c = ctx_of(env, a[0]);
+  napi_value o = a[3];
+  anima_weight g, u;
+  read_weight(env, a[1], &g);
+  read_weight(env, a[2], &u);
+  anima_glu_desc d;
+  memset(&d, 0, sizeof d);
+  d.M = (int64_t)pnum(env, o, "M");
+  d.gate = &g;
+  d.up = &u;
+  d.x = (const float*)pptr(env, o, "x");
+  d.xq = (const int8_t*)pptr(env, o, "xq");
+  d.xs = (const float*)pptr(env, o, "xs");
+  d.ldx = (int64_t)pnum(env, o, "ldx");
+  d.act = (int)pnum(env, o, "act");
+  d.out = (float*)pptr(env, o, "out");
+  d.ldc = (int64_t)pnum(env, o, "ldc");
+  d.out_q = (uint8_t*)pptr(env, o, "outQ");
+  d.out_s = (float*)pptr(env, o, "outS");
+  d.precision = (int)pnum(env, o, "precision");
+  CHECK_RC(env, c, anima_linear_glu(c, &d));
+  return NULL;
+}
+
+/* residualNorm(ctx, desc): desc mirrors anima_resnorm_desc (rows, cols, x, ldx, y, ldy, yBf16, postW,
+ * gate, gateLd, resScale, norm, normW, shift, scale, modLd, groupRows, eps, h, ldh, q, s) */
+static napi_value js_residual_norm(napi_env env, napi_callback_info info) {
+  napi_value a[2];
+  get_args(env, info, 2, a);
+  anima_ctx* c = ctx_of(env, a[0]);
+  napi_value o = a[1];
+  anima_resnorm_desc d;
+  memset(&d, 0, sizeof d);
+  d.rows = (int64_t)pnum(env, o, "rows");
+  d.cols = (int)pnum(env, o, "cols");
+  d.x = (float*)pptr(env, o, "x");
+  d.ldx = (int64_t)pnum(env, o, "ldx");
+  d.y = pptr(env, o, "y");
+  d.ldy = (int64_t)pnum(env, o, "ldy");
+  d.y_bf16 = (int)pnum(env, o, "yBf16");
+  d.post_w = (const float*)pptr(env, o, "postW");
+  d.gate = (const float*)pptr(env, o, "gate");
+  d.gate_ld = (int64_t)pnum(env, o, "gateLd");
+  d.res_scale = (float)pnum(env, o, "resScale");
+  d.norm = (int)pnum(env, o, "norm");
+  d.norm_w = (const float*)pptr(env, o, "normW");
+  d.shift = (const float*)pptr(env, o, "shift");
+  d.scale = (const float*)pptr(env, o, "scale");
+  d.mod_ld = (int64_t)pnum(env, o, "modLd");
+  d.group_rows = (int64_t)pnum(env, o, "groupRows");
+  d.eps = (float)pnum(env, o, "eps");
+  d.h = (float*)pptr(env, o, "h");
+  d.ldh = (int64_t)pnum(env, o, "ldh");
+  d.q = (uint8_t*)pptr(env, o, "q");
+  d.s = (float*)pptr(env, o, "s");
+  CHECK_RC(env, c, anima_residual_norm(c, &d));
   return NULL;
 }
 
@@ -971,7 +1058,8 @@ static napi_value Init(napi_env env, napi_value exports) {
       FN("qkNormRope", js_qk_norm_rope), FN("rmsnorm", js_rmsnorm), FN("rope", js_rope),
       FN("hadamard", js_hadamard), FN("quantRows", js_quant_rows), FN("quantRowsBf16", js_quant_rows_bf16), FN("layernormMod", js_layernorm_mod),
       FN("elementwise", js_elementwise), FN("zero", js_zero), FN("patchify", js_patchify), FN("linearGroupedBf16", js_linear_grouped_bf16), FN("gemvGroupedF32", js_gemv_grouped_f32), FN("unpatchify", js_unpatchify), FN("fillRandom", js_fill_random),
-      FN("linear", js_linear), FN("linearQkv", js_linear_qkv), FN("samplerStep", js_sampler_step), FN("attentionKvBytes", js_attention_kv_bytes), FN("split3", js_split3), FN("lastError", js_last_error),
+      FN("linear", js_linear), FN("quantRowsF8", js_quant_rows_f8), FN("weightQuantF8", js_weight_quant_f8),
+      FN("linearGlu", js_linear_glu), FN("residualNorm", js_residual_norm), FN("linearQkv", js_linear_qkv), FN("samplerStep", js_sampler_step), FN("attentionKvBytes", js_attention_kv_bytes), FN("split3", js_split3), FN("lastError", js_last_error),
       FN("graphBegin", js_graph_begin), FN("graphEnd", js_graph_end), FN("graphLaunch", js_graph_launch),
       FN("graphDestroy", js_graph_destroy), FN("conv3x3", js_conv3x3), FN("channelNorm", js_channel_norm), FN("toRgba", js_to_rgba),
       FN("weightUnpackW4", js_weight_unpack_w4),

@@ -26,9 +26,13 @@ function releaseAll(xs) {
 // reads the int8 rows unless ops.setLoraInput("fp32"))
 const wantsXr = (W) => !!(W.lora && W.lora.length) && !ops.loraReadsInt8(W);
 
-// LayerNorm + adaLN for inputs that feed W: int8 { xq } when W is quantized (W8A8), else the
-// fp32 modulated rows (normFor of app/models/dit.js:34-38).
+// whether W reads e4m3 rows (a LoRA on it needs the fp32 rows, which ops.linear then quantizes)
+const f8In = (W) => W.kind === "f8" && !(W.lora && W.lora.length);
+
+// LayerNorm + adaLN for inputs that feed W: int8 { xq } when W is quantized (W8A8), e4m3 { xq } when
+// it is an e4m3 weight, else the fp32 modulated rows (normFor of app/models/dit.js:34-38).
 function normFor(gpu, x, mod, W) {
+  if (f8In(W)) return { xq: ops.residualNorm(gpu, x, D, { norm: "layer", mod, shiftOff: 0, scaleOff: D, f8: true }) };
   if (ops.needsRotation(W)) return { xq: ops.layernormModQ(gpu, x, mod, 0, D, D, wantsXr(W)) };
   return { n: ops.layernormMod(gpu, x, mod, 0, D, D, false) };
 }
@@ -43,10 +47,14 @@ function project(gpu, nf, W, M, opts) {
 }
 
 // The attention output projection with its gated residual into x: a bf16 output (attention's
-// oBf16) is quantized here, the form the int8 / W4 GEMM reads, otherwise ops.linear quantizes the
+// oBf16) is quantized here, the form the int8 / W4 / e4m3 GEMM reads, otherwise ops.linear quantizes the
 // fp32 rows itself.
 function outProject(gpu, a, W, M, x, mod) {
-  if (a.dtype === "bf16") {
+  if (W.kind === "f8" && a.dtype === "bf16") {
+    const aq = ops.quantRowsF8(gpu, a, D);
+    ops.linear(gpu, null, W, { M, xq: aq, out: x, resid: true, gate: mod, gOff: 2 * D, precision: "bf16" });
+    aq.release();
+  } else if (a.dtype === "bf16") {
     const aq = ops.quantRows(gpu, a, D, true);
     ops.linear(gpu, null, W, { M, xq: aq, out: x, resid: true, gate: mod, gOff: 2 * D });
     aq.release();
@@ -56,8 +64,8 @@ function outProject(gpu, a, W, M, x, mod) {
 }
 
 // whether an attention may write bf16 O for the output projection W (quantized, and its LoRA if
-// any reads the int8 rows)
-const bf16Out = (W, precision) => precision === "bf16" && ops.needsRotation(W) && !wantsXr(W);
+// any reads the int8 rows; e4m3 without a LoRA)
+const bf16Out = (W, precision) => precision === "bf16" && (f8In(W) || (ops.needsRotation(W) && !wantsXr(W)));
 
 function releaseNorm(nf) {
   if (nf.xq) nf.xq.release();
@@ -202,6 +210,17 @@ export class AnimaDiT {
           n++;
         }
       }
+    }
+    return n;
+  }
+
+  // Converts the blocks' bf16 linears to e4m3 with one scale per 128 x 128 block (ops.quantizeF8; as
+  // Qwen3.quantizeF8), before any ForwardGraph is recorded.  Returns the number of linears converted.
+  quantizeF8() {
+    let n = 0;
+    for (const b of this.blocks) {
+      const Ws = [b.self.qkv, b.self.q, b.self.k, b.self.v, b.self.o, b.cross.q, b.cross.k, b.cross.v, b.cross.o, b.l1, b.l2];
+      for (const W of Ws) if (W && W.kind !== "f8" && ops.quantizeF8(this.gpu, W).kind === "f8") n++;
     }
     return n;
   }
@@ -492,7 +511,7 @@ export class AnimaDiT {
         let qkv;
         if (b.self.qkv) {
           nf = normFor(gpu, x, m.self, b.self.qkv);
-          qkv = project(gpu, nf, b.self.qkv, M, { name: "dit.self.qkv" });
+          qkv = project(gpu, nf, b.self.qkv, M, { name: "dit.self.qkv", precision: this.precision });
           releaseNorm(nf);
         } else {
           qkv = projectParts(gpu, x, m.self, [b.self.q, b.self.k, b.self.v], M);
@@ -518,7 +537,7 @@ export class AnimaDiT {
           precision: "bf16", oBf16: bf16Out(b.cross.o, "bf16") });
         f.qPrep.release();
       } else {
-        const q = project(gpu, nf, b.cross.q, M);
+        const q = project(gpu, nf, b.cross.q, M, { precision: this.precision });
         releaseNorm(nf);
         a = ops.attention(gpu, { q, kvPrep: kv.prep, B, Lq: L, Lk: cond.Lk, H: HEADS, D: HD, ldq: D, qNorm: b.cross.qn,
           precision: cond.precision, oBf16: bf16Out(b.cross.o, cond.precision) });
@@ -537,6 +556,14 @@ export class AnimaDiT {
         const hq = ops.quantRows(gpu, pre, MLP, true, "gelu");
         pre.release();
         ops.linear(gpu, null, b.l2, { M, xq: hq, out: x, resid: true, gate: m.mlp, gOff: 2 * D });
+        hq.release();
+      } else if (f8In(b.l1) && f8In(b.l2)) {
+        const bf16 = this.precision === "bf16";
+        const act = project(gpu, nf, b.l1, M, { act: "gelu", precision: this.precision, outBf16: bf16 });
+        releaseNorm(nf);
+        const hq = ops.quantRowsF8(gpu, act, MLP);
+        act.release();
+        ops.linear(gpu, null, b.l2, { M, xq: hq, out: x, resid: true, gate: m.mlp, gOff: 2 * D, precision: this.precision });
         hq.release();
       } else {
         const hdn = project(gpu, nf, b.l1, M, { act: "gelu" });

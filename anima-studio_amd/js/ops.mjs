@@ -6,12 +6,17 @@
 //              qNorm / kNorm / cs (q/k RMSNorm + RoPE fused into the attention loads), precision.
 //   linear:    opts.xq = { q, s } per-token int8 activations (layernormModQ / quantRows); a LoRA
 //              on a quantized weight reads them too (setLoraInput), or the fp32 input opts.xr / x.
+//   linear on an e4m3 weight (kind "f8"): opts.xq = { q, s } of quantRowsF8 / linearGlu / residualNorm,
+//              opts.precision and opts.outBf16.
+//   linearGlu, residualNorm: a gated feed-forward's first half, and the residual addition with the
+//              next block's norm, each one kernel, with e4m3 rows out.
 //   layernormModQ: LayerNorm + adaLN + ConvRot + per-token int8 in one pass.
 
 import { native } from "./gpu.mjs";
 
-const KIND = { bf16: 0, i8: 1, w4: 2, f32: 3, f32s3: 4 };
+const KIND = { bf16: 0, i8: 1, w4: 2, f32: 3, f32s3: 4, f8: 5 };
 const ACT = { none: 0, gelu: 1, silu: 2 };
+const NORM = { rms: 0, layer: 1 };
 const EW = { silu_mul: 0, add: 1, silu: 2, copy: 3 };
 const ptr = (t) => (t ? (typeof t === "number" ? t : t.buf) : 0);
 
@@ -72,6 +77,43 @@ export function unpackW4(gpu, W) {
   return W;
 }
 
+// Rows [M, K] (f32 or bf16) as e4m3 values with one scale per 128 columns, s [ceil(K / 128), M]: the
+// input of a linear on an "f8" weight.
+export function quantRowsF8(gpu, x, K) {
+  const M = x.size / K;
+  const r = f8Rows(gpu, M, K);
+  native.quantRowsF8(gpu.ctx, x.buf, x.dtype === "bf16" ? 1 : 0, M, K, 0, r.q.buf, r.s.buf);
+  return r;
+}
+
+function f8Rows(gpu, M, K) {
+  const q = gpu.empty([M, K], "u8");
+  const s = gpu.empty([Math.ceil(K / 128), M]);
+  return { q, s, release() { q.release(); s.release(); } };
+}
+
+// A bf16 or f32 weight turned into the e4m3 weight with one scale per 128 x 128 block, in place (as
+// unpackW4: LoRA attachments stay).  Half the bytes of bf16; a weight is off by at most 2^-4 of its
+// value.  Other kinds, and input widths that are no multiple of 16, stay as they are.
+export function quantizeF8(gpu, W) {
+  if ((W.kind !== "bf16" && W.kind !== "f32") || W.K % 16) return W;
+  const q = gpu.empty([W.N * W.K], "u8");
+  const scale = gpu.empty([Math.ceil(W.N / 128) * Math.ceil(W.K / 128)]);
+  native.weightQuantF8(gpu.ctx, ptr(W.buf), W.kind === "bf16" ? 1 : 0, W.N, W.K, q.buf, scale.buf);
+  if (W.buf.release) W.buf.release();
+  W.kind = "f8";
+  W.buf = q;
+  W.scale = scale;
+  return W;
+}
+
+// opts.xq of a linear on W: the row form that W's kind reads (int8 rows and e4m3 rows are both bytes)
+function checkRows(W, xq) {
+  const f8 = xq.q.dtype === "u8";
+  if (f8 !== (W.kind === "f8"))
+    throw new Error(`${W.name || "linear"}: ${f8 ? "e4m3" : "int8"} rows for a ${W.kind} weight`);
+}
+
 function weightArg(W) {
   if (!(W.kind in KIND)) throw new Error(`unsupported weight kind ${W.kind}`);
   return { kindId: KIND[W.kind], N: W.N, K: W.K, buf: ptr(W.buf), scale: ptr(W.scale), srel: ptr(W.srel),
@@ -81,9 +123,13 @@ function weightArg(W) {
 // y = x @ W^T (+ bias) (act) (ops.js:48-66).  Quantized weights take the ConvRot-rotated input
 // `xr` when given, else rotate x here; the activations are quantized per token (W8A8).
 // opts.out + opts.resid: out += (gate[gOff + n] *) y in place.
+// On an "f8" weight, opts.precision: "fp32" (default: products added in 32 bits) or "bf16" (by the
+// 8-bit matrix instructions, about 1.5e-5 of the result, twice the rate), and opts.outBf16: a bf16
+// result (no residual).
 export function linear(gpu, x, W, opts) {
   const o = opts || {};
-  const M = o.M !== undefined ? o.M : (o.xq ? o.xq.s.size : x.size / W.K);
+  if (o.xq) checkRows(W, o.xq);
+  const M = o.M !== undefined ? o.M : (o.xq ? o.xq.q.size / W.K : x.size / W.K);
   // LoRAs: y += sum_i scale_i B_i (A_i x), after the bias and before act / gate (ops.js:55-62).
   // The reference feeds ConvRot layers' LoRAs the rotated input and a rotated A; since
   // (x H)(A H)^T = x A^T, the unrotated x and A are used when x is at hand (no rotation pass), and
@@ -105,13 +151,15 @@ export function linear(gpu, x, W, opts) {
     : linear(gpu, xin, { kind: "f32s3", N: F.R, K: W.K, buf: rot ? F.Ars : F.As }, { M });
   const late = lora && !F && !o.resid && ACT[o.act || "none"] === 0;
   const delta = lora && !F && !late ? loraDelta(gpu, xin, W, M, rot) : null;
-  const out = o.out || gpu.empty([M, W.N]);
+  if (o.outBf16 && W.kind !== "f8") throw new Error(`${W.name || "linear"}: bf16 results are for f8 weights`);
+  if (o.outBf16 && late) throw new Error(`${W.name || "linear"}: no bf16 result with a LoRA`);
+  const out = o.out || gpu.empty([M, W.N], o.outBf16 ? "bf16" : "f32");
   const d = { M, out: out.buf, ldc: o.ldc || 0, alpha: o.alpha || 0, act: ACT[o.act || "none"],
     epilogue: o.resid ? (o.gate ? 2 : 1) : 0, gate: ptr(o.gate), gOff: o.gOff || 0, accOut: ptr(o.accOut),
     add: delta ? delta.buf : 0, ldAdd: delta ? W.N : 0,
     loraXa: down ? down.buf : 0, ldLoraXa: down ? F.R : 0, loraB: F ? F.Bs.buf : 0, loraR: F ? F.Rb : 0,
-    loraCols: F ? F.cols : 0 };
-  if ((needsRotation(W) || W.kind === "f32s3") && o.xq) {
+    loraCols: F ? F.cols : 0, precision: W.kind === "f8" ? precisionId(o) : 0, outBf16: o.outBf16 ? 1 : 0 };
+  if ((needsRotation(W) || W.kind === "f32s3" || W.kind === "f8") && o.xq) {
     d.xq = o.xq.q.buf;
     d.xs = o.xq.s.buf;
   } else if (needsRotation(W)) {
@@ -327,6 +375,46 @@ export function splitPlanes(gpu, t, n) {
   const p = gpu.empty([3 * n], "u16");
   native.split3(gpu.ctx, t.buf || t, p.buf, n);
   return p;
+}
+
+// The first half of a gated feed-forward block on e4m3 weights of one shape: act(x Wg^T + bg) *
+// (x Wu^T + bu) (act "silu" by default, the linears and silu_mul of app/models/qwen3.js:66-72).
+// opts: xq (e4m3 rows, else x is quantized), M, act, precision as linear's; opts.f8: the result as
+// e4m3 rows { q, s }, else a [M, N] tensor (opts.out).  No LoRA.
+export function linearGlu(gpu, x, Wg, Wu, opts) {
+  const o = opts || {};
+  for (const W of [Wg, Wu]) {
+    if (W.kind !== "f8") throw new Error(`linearGlu: ${W.name || "weight"} is ${W.kind}, expected f8`);
+    if (W.lora && W.lora.length) throw new Error(`linearGlu: ${W.name || "weight"} has a LoRA`);
+    if (o.xq) checkRows(W, o.xq);
+  }
+  const M = o.M !== undefined ? o.M : (o.xq ? o.xq.q.size / Wg.K : x.size / Wg.K);
+  const rows = o.f8 ? f8Rows(gpu, M, Wg.N) : null;
+  const out = rows ? null : o.out || gpu.empty([M, Wg.N]);
+  native.linearGlu(gpu.ctx, weightArg(Wg), weightArg(Wu), { M, x: o.xq ? 0 : x.buf, xq: o.xq ? o.xq.q.buf : 0,
+    xs: o.xq ? o.xq.s.buf : 0, ldx: o.xq ? 0 : o.ldx || 0, act: ACT[o.act || "silu"], out: ptr(out), ldc: o.ldc || 0,
+    outQ: rows ? rows.q.buf : 0, outS: rows ? rows.s.buf : 0, precision: precisionId(o) });
+  return rows || out;
+}
+
+// The seam between two blocks in one pass over x [rows, cols]: x += resScale * gate * post(y) in place
+// (opts.y, f32 or bf16; optional), then h = norm(x) * weight * (1 + scale) + shift.
+// opts: postWeight (RMSNorm of y first), gate + gOff, resScale, norm ("rms" | "layer"), weight,
+// mod + shiftOff + scaleOff, eps; opts.h: fp32 rows (default when f8 is not set), opts.f8: e4m3 rows.
+// Returns { h, q, s, release }: an { q, s } of linear / linearGlu when f8.
+export function residualNorm(gpu, x, cols, opts) {
+  const o = opts || {};
+  if (o.norm !== undefined && !(o.norm in NORM)) throw new Error(`residualNorm: unknown norm ${o.norm}`);
+  const rows = x.size / cols;
+  if (o.y && o.y.size !== x.size) throw new Error(`residualNorm: y of ${o.y.size} values for x of ${x.size}`);
+  const r = o.f8 ? f8Rows(gpu, rows, cols) : null;
+  const h = o.h || !r ? gpu.empty([rows, cols]) : null;
+  const at = (t, off) => (t ? ptr(t) + 4 * (off || 0) : 0);
+  native.residualNorm(gpu.ctx, { rows, cols, x: x.buf, y: ptr(o.y), yBf16: o.y && o.y.dtype === "bf16" ? 1 : 0,
+    postW: ptr(o.postWeight), gate: at(o.gate, o.gOff), resScale: o.resScale || 0, norm: NORM[o.norm || "rms"],
+    normW: ptr(o.weight), shift: at(o.mod, o.shiftOff), scale: at(o.mod, o.scaleOff),
+    eps: o.eps === undefined ? 1e-6 : o.eps, h: ptr(h), q: r ? r.q.buf : 0, s: r ? r.s.buf : 0 });
+  return { h, q: r ? r.q : null, s: r ? r.s : null, release() { for (const t of [h, r]) if (t) t.release(); } };
 }
 
 export function zero(gpu, t) {

@@ -9,6 +9,8 @@ import { ropeTable } from "./common.mjs";
 import { concatLinears } from "./weights.mjs";
 import { native } from "./gpu.mjs";
 
+const LINEARS = ["qkv", "q", "k", "v", "o", "gate", "up", "down"];
+
 function releaseGraph(gpu, g) {
   native.graphDestroy(gpu.ctx, g.graph);
   for (const t of [g.out, g.x, g.cs]) t.release();
@@ -25,6 +27,11 @@ function stackQKV(gpu, l) {
   delete l.k;
   delete l.v;
 }
+
+const hasLora = (l) => LINEARS.some((k) => l[k] && l[k].lora && l[k].lora.length > 0);
+// whether a layer runs on e4m3 rows from norm to norm (layersF8)
+const isF8 = (l) => !!l.qkv && ["qkv", "o", "gate", "up", "down"].every((k) => l[k].kind === "f8") &&
+  l.gate.K === l.up.K && l.gate.N === l.up.N && !hasLora(l);
 
 export const QWEN3 = { layers: 28, hidden: 1024, heads: 16, kvHeads: 8, headDim: 128, mlp: 3072, theta: 1e6, vocab: 151936 };
 
@@ -108,7 +115,7 @@ export class Qwen3 {
     const Lt = ids.length;
     const rows = await this.embedRows(ids);
     // LoRA side paths (attachLoras) run eagerly: a graph recorded before an attach would not hold them
-    const lora = this.layers.some((l) => ["qkv", "q", "k", "v", "o", "gate", "up", "down"].some((k) => l[k] && l[k].lora && l[k].lora.length));
+    const lora = this.layers.some(hasLora);
     if (!this.graphs || lora) {
       const x = gpu.fromArray(rows, [Lt, D]);
       const cs = ropeTable(gpu, Lt, HD, this.cfg.theta);
@@ -164,11 +171,61 @@ export class Qwen3 {
     return { x, cs, out, graph };
   }
 
+  // Converts the layers' bf16 linears to e4m3 with one scale per 128 x 128 block (ops.quantizeF8): half
+  // the bytes, and the layers then run on e4m3 rows (layersF8).  An option for a caller who accepts
+  // 8-bit weights and activations; the checkpoint's form is the default.
+  // Returns the number of linears converted.
+  quantizeF8() {
+    let n = 0;
+    for (const l of this.layers)
+      for (const k of LINEARS)
+        if (l[k] && l[k].kind !== "f8" && ops.quantizeF8(this.gpu, l[k]).kind === "f8") n++;
+    for (const g of this.graphCache.values()) releaseGraph(this.gpu, g);
+    this.graphCache.clear();
+    return n;
+  }
+
+  // The layers on e4m3 weights: every product reads e4m3 rows that the kernel before it wrote.  A
+  // layer is seven launches: seam (residual addition + norm), qkv, attention, its rows to e4m3, o,
+  // seam, gate / up / SiLU, down; the last seam is the final norm.
+  layersF8(x, cs, Lt) {
+    const gpu = this.gpu;
+    const { hidden: D, heads: H, kvHeads: KH, headDim: HD } = this.cfg;
+    const ld = (H + 2 * KH) * HD, precision = this.precision, bf16 = precision === "bf16";
+    let y = null;
+    const seam = (weight, f8) => {
+      const r = ops.residualNorm(gpu, x, D, { y, weight, f8 });
+      if (y) y.release();
+      y = null;
+      return r;
+    };
+    for (const l of this.layers) {
+      const h = seam(l.ln1, true);
+      const qkv = ops.linear(gpu, null, l.qkv, { xq: h, precision });
+      h.release();
+      const a = ops.attention(gpu, { q: qkv, k: qkv, v: qkv, Lq: Lt, Lk: Lt, H, D: HD, ldq: ld, ldk: ld, ldv: ld, qOff: 0,
+        kOff: H * HD, vOff: (H + KH) * HD, group: H / KH, causal: true, qNorm: l.qn, kNorm: l.kn, cs, precision,
+        oBf16: bf16 });
+      qkv.release();
+      const aq = ops.quantRowsF8(gpu, a, H * HD);
+      a.release();
+      y = ops.linear(gpu, null, l.o, { xq: aq, precision, outBf16: bf16 });
+      aq.release();
+      const h2 = seam(l.ln2, true);
+      const gu = ops.linearGlu(gpu, null, l.gate, l.up, { xq: h2, precision, f8: true });
+      h2.release();
+      y = ops.linear(gpu, null, l.down, { xq: gu, precision, outBf16: bf16 });
+      gu.release();
+    }
+    return seam(this.norm, false).h;
+  }
+
   // The decoder layers and the final RMSNorm on the residual stream x [Lt, D] (updated in place);
   // returns the normed hidden states (a new tensor).
   layersDevice(x, cs, Lt) {
     const gpu = this.gpu;
     const { hidden: D, heads: H, kvHeads: KH, headDim: HD } = this.cfg;
+    if (this.layers.length && this.layers.every(isF8)) return this.layersF8(x, cs, Lt);
     for (const l of this.layers) {
       const h = ops.rmsnorm(gpu, x, l.ln1, D);
       const hr = ops.needsRotation(l.qkv || l.q) ? ops.rotate(gpu, h) : null;

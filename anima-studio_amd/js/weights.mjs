@@ -127,7 +127,7 @@ export class SafeTensors {
     return W;
   }
 
-  // comfy_quant -> { kind: i8 | w4 }, else bf16 (app/weights.js:118-147)
+  // comfy_quant -> { kind: i8 | w4 }, block-scaled e4m3 -> f8, else bf16 (app/weights.js:118-147)
   linearWeights(gpu, base) {
     const w = this.info(base + "weight");
     const bias = this.has(base + "bias") ? this.vector(gpu, base + "bias") : null;
@@ -153,6 +153,15 @@ export class SafeTensors {
       }
       throw new Error(`unsupported quant format ${meta.format}`);
     }
+    // e4m3 with one scale per 128 x 128 block, [ceil(N / 128), ceil(K / 128)]
+    if (w.dtype === "F8_E4M3" && this.has(base + "weight_scale_inv")) {
+      const N = w.shape[0], K = w.shape[1], nb = Math.ceil(N / 128), kb = Math.ceil(K / 128);
+      const s = this.info(base + "weight_scale_inv").shape;
+      if (w.shape.length !== 2 || s.length !== 2 || s[0] !== nb || s[1] !== kb)
+        throw new Error(`${base}: scales [${s}] of an e4m3 weight [${w.shape}], expected [${nb}, ${kb}]`);
+      return { kind: "f8", N, K, buf: gpu.upload(this.bytes(base + "weight").slice()),
+        scale: this.vector(gpu, base + "weight_scale_inv"), bias };
+    }
     if (w.dtype !== "BF16") throw new Error(`expected bf16 weight for ${base}, got ${w.dtype}`);
     const N = w.shape[0];
     const K = w.shape.slice(1).reduce((a, b) => a * b, 1);
@@ -161,7 +170,8 @@ export class SafeTensors {
 }
 
 // Stack linears sharing an input into one [sum N, K] weight (app/weights.js:152-189): rows and
-// per-row scales concatenate; w4 also needs one shared codebook.  Returns null otherwise.
+// per-row scales concatenate; w4 also needs one shared codebook, and f8 parts before the last whole
+// blocks of 128 rows.  Returns null otherwise.
 export function concatLinears(gpu, Ws) {
   const kind = Ws[0].kind, K = Ws[0].K;
   if (!Ws.every((w) => w.kind === kind && w.K === K && !w.bias)) return null;
@@ -169,13 +179,14 @@ export function concatLinears(gpu, Ws) {
     const cb = Ws[0].codebookData;
     if (!Ws.every((w) => w.codebookData.every((v, i) => v === cb[i]))) return null;
   }
+  if (kind === "f8" && !Ws.every((w, i) => w.N % 128 === 0 || i === Ws.length - 1)) return null;
   const bytes = {
-    buf: (n) => (kind === "bf16" ? n * K * 2 : kind === "i8" ? n * K : (n * K) / 2),
-    scale: (n) => n * 4,
+    buf: (n) => (kind === "bf16" ? n * K * 2 : kind === "w4" ? (n * K) / 2 : n * K),
+    scale: (n) => (kind === "f8" ? Math.ceil(n / 128) * Math.ceil(K / 128) : n) * 4,
     srel: (n) => (n * K) / 16,
   };
   const dtype = { buf: kind === "bf16" ? "u16" : kind === "i8" ? "i8" : "u8", scale: "f32", srel: "u8" };
-  const fields = kind === "bf16" ? ["buf"] : kind === "i8" ? ["buf", "scale"] : ["buf", "scale", "srel"];
+  const fields = kind === "bf16" ? ["buf"] : kind === "i8" || kind === "f8" ? ["buf", "scale"] : ["buf", "scale", "srel"];
   const N = Ws.reduce((a, w) => a + w.N, 0);
   const out = { kind, K, N, parts: [] };
   let colOff = 0;

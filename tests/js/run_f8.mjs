@@ -1,0 +1,147 @@
+// Runs one case of the e4m3 operators through the JS op layer (ops.mjs -> N-API -> libanima.so) for
+// the parity tests: reads a JSON spec whose inputs are raw little-endian files, writes the outputs
+// the same way.  node run_f8.mjs case.json
+//
+// Cases:
+//   block   residualNorm -> linear -> quantRowsF8 -> linear (bf16) -> residualNorm -> linearGlu ->
+//           linear, on bf16 weights converted by quantizeF8 or on an e4m3 safetensors file
+//   qwen3   Qwen3.encode of a synthetic text encoder after quantizeF8 (both precisions; recorded,
+//           replayed and eager) and its weights; an encoding with a LoRA of zeros attached
+//   dit     a synthetic DiT's velocities: bf16 weights, after quantizeF8, and with LoRAs of zeros
+
+import fs from "fs";
+import { GPU } from "../../anima-studio_amd/js/gpu.mjs";
+import * as ops from "../../anima-studio_amd/js/ops.mjs";
+import { SafeTensors, SyntheticWeights, concatLinears } from "../../anima-studio_amd/js/weights.mjs";
+import { ropeTable } from "../../anima-studio_amd/js/common.mjs";
+import { AnimaDiT } from "../../anima-studio_amd/js/dit.mjs";
+import { Qwen3 } from "../../anima-studio_amd/js/qwen3.mjs";
+
+const ARR = { f32: Float32Array, u8: Uint8Array, u16: Uint16Array };
+
+function load(path, dtype) {
+  const b = fs.readFileSync(path);
+  return new ARR[dtype || "f32"](b.buffer.slice(b.byteOffset, b.byteOffset + b.length));
+}
+
+function save(path, arr) {
+  fs.writeFileSync(path, Buffer.from(arr.buffer, arr.byteOffset, arr.byteLength));
+}
+
+// a LoRA entry of zeros on W: its linears then take the fp32 input
+function zeroLora(gpu, W) {
+  const A = gpu.upload(new Float32Array(8 * W.K)), B = gpu.upload(new Float32Array(W.N * 8));
+  W.lora = [{ A, B, r: 8, scale: 1, off: 0, n: W.N }];
+}
+
+async function block(gpu, c) {
+  const st = c.file ? SafeTensors.open(c.file) : null;
+  const weight = (name, N, K) => {
+    if (st) return st.linear(gpu, name + ".");
+    return ops.quantizeF8(gpu, { kind: "bf16", N, K, name, buf: gpu.upload(load(c.w[name], "u16")) });
+  };
+  const { M, C, F } = c;
+  const Wa = weight("a", C, C), Wb = weight("b", C, C), Wg = weight("gate", F, C), Wu = weight("up", F, C), Wd = weight("down", C, F);
+  const two = concatLinears(gpu, [Object.assign({}, weight("gate", F, C)), weight("up", F, C)]);
+  const x = gpu.fromArray(load(c.x), [M, C]);
+  const mod = gpu.upload(load(c.mod));
+  const h = ops.residualNorm(gpu, x, C, { norm: "layer", mod, shiftOff: 0, scaleOff: C, f8: true });
+  const y = ops.linear(gpu, null, Wa, { xq: h, act: "gelu" });
+  const yq = ops.quantRowsF8(gpu, y, C);
+  const z = ops.linear(gpu, null, Wb, { xq: yq, precision: "bf16", outBf16: true });
+  const h2 = ops.residualNorm(gpu, x, C, { y: z, gate: mod, gOff: 2 * C, weight: gpu.upload(load(c.norm)), h: true, f8: true });
+  const g = ops.linearGlu(gpu, null, Wg, Wu, { xq: h2, f8: true });
+  const gf = ops.linearGlu(gpu, h2.h, Wg, Wu, {});
+  const both = two ? ops.linear(gpu, null, two, { xq: h2 }) : null;
+  const x1 = await gpu.read(x);
+  ops.linear(gpu, null, Wd, { xq: g, out: x, resid: true, gate: mod, gOff: 2 * C });
+  const out = { x: await gpu.read(x), x1, y: await gpu.read(y), z: await gpu.read(z), h2: await gpu.read(h2.h), gf: await gpu.read(gf) };
+  for (const [n, r] of [["h", h], ["yq", yq], ["h2", h2], ["g", g]]) {
+    out[n + ".q"] = await gpu.read(r.q);
+    out[n + ".s"] = await gpu.read(r.s);
+  }
+  for (const [n, W] of [["a", Wa], ["b", Wb], ["gate", Wg], ["up", Wu], ["down", Wd]]) {
+    out[`w.${n}.q`] = await gpu.read(W.buf);
+    out[`w.${n}.s`] = await gpu.read(W.scale);
+  }
+  if (both) out.both = await gpu.read(both);
+  for (const k of Object.keys(out)) save(`${c.out}.${k}`, out[k]);
+}
+
+// the encoder's layers in fp32 precision, op by op on fp32 rows
+function encoderSteps(gpu, te, rows, L) {
+  const { hidden: D, heads: H, kvHeads: KH, headDim: HD } = te.cfg;
+  const x = gpu.fromArray(rows, [L, D]), cs = ropeTable(gpu, L, HD, te.cfg.theta), ld = (H + 2 * KH) * HD;
+  for (const l of te.layers) {
+    const h = ops.residualNorm(gpu, x, D, { weight: l.ln1 }).h;
+    const qkv = ops.linear(gpu, h, l.qkv, {});
+    const a = ops.attention(gpu, { q: qkv, k: qkv, v: qkv, Lq: L, Lk: L, H, D: HD, ldq: ld, ldk: ld, ldv: ld, qOff: 0,
+      kOff: H * HD, vOff: (H + KH) * HD, group: H / KH, causal: true, qNorm: l.qn, kNorm: l.kn, cs, precision: "fp32" });
+    ops.linear(gpu, a, l.o, { out: x, resid: true });
+    const h2 = ops.residualNorm(gpu, x, D, { weight: l.ln2 }).h;
+    ops.linear(gpu, ops.linearGlu(gpu, h2, l.gate, l.up, {}), l.down, { out: x, resid: true });
+  }
+  return ops.residualNorm(gpu, x, D, { weight: te.norm }).h;
+}
+
+async function qwen3(gpu, c) {
+  const te = Qwen3.synthetic(gpu, new SyntheticWeights(gpu, 17), { layers: c.layers, vocab: c.vocab });
+  (await te.encode(c.ids)).release(); // a graph over the bf16 weights, dropped by quantizeF8
+  console.log(JSON.stringify({ converted: te.quantizeF8(), again: te.quantizeF8() }));
+  for (const prec of ["fp32", "bf16"]) {
+    te.precision = prec;
+    for (const tag of ["", ".replay", ".replay2"]) save(`${c.out}.${prec}${tag}`, await gpu.read(await te.encode(c.ids)));
+    te.graphs = false;
+    save(`${c.out}.${prec}.eager`, await gpu.read(await te.encode(c.ids)));
+    te.graphs = true;
+  }
+  for (let i = 0; i < te.layers.length; i++) {
+    const l = te.layers[i];
+    for (const k of ["ln1", "ln2", "qn", "kn"]) save(`${c.out}.w.${i}.${k}`, await gpu.read(l[k]));
+    for (const k of ["qkv", "o", "gate", "up", "down"]) {
+      save(`${c.out}.w.${i}.${k}`, await gpu.read(l[k].buf));
+      save(`${c.out}.w.${i}.${k}.s`, await gpu.read(l[k].scale));
+    }
+  }
+  save(`${c.out}.w.norm`, await gpu.read(te.norm));
+  save(`${c.out}.w.embed`, await gpu.read(te.table));
+  te.precision = "fp32";
+  save(`${c.out}.steps`, await gpu.read(encoderSteps(gpu, te, await te.embedRows(c.ids), c.ids.length)));
+  zeroLora(gpu, te.layers[0].o);
+  save(`${c.out}.lora`, await gpu.read(await te.encode(c.ids)));
+  te.release();
+}
+
+async function dit(gpu, c) {
+  const model = AnimaDiT.synthetic(gpu, new SyntheticWeights(gpu, c.seed, { mode: "bf16", blocks: c.blocks }));
+  const lat = c.latents.map((p) => load(p));
+  const forward = async (tag) => {
+    const tc = model.timeCond(c.sigma);
+    const cond = model.prepareContext(c.ctx.map((p) => gpu.fromArray(load(p), [c.Lk, 1024])));
+    const v = await model.forward(lat, c.h, c.w, cond, tc);
+    v.forEach((vb, b) => save(`${c.out}.${tag}.${b}`, vb));
+    tc.release();
+    cond.release();
+  };
+  model.precision = "fp32";
+  await forward("bf16w");
+  console.log(JSON.stringify({ converted: model.quantizeF8() }));
+  await forward("f8");
+  model.precision = "bf16";
+  await forward("f8bf16");
+  model.precision = "fp32";
+  for (const b of model.blocks)
+    for (const W of [b.self.qkv, b.self.o, b.cross.q, b.cross.o, b.l1, b.l2]) if (W) zeroLora(gpu, W);
+  await forward("f8lora");
+}
+
+const c = JSON.parse(fs.readFileSync(process.argv[2], "utf8"));
+GPU.create({})
+  .then(async (gpu) => {
+    await { block, qwen3, dit }[c.case](gpu, c);
+    gpu.destroy();
+  })
+  .catch((e) => {
+    console.error(e);
+    process.exit(1);
+  });
