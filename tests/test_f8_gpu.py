@@ -698,3 +698,84 @@ def test_refusals_leave_the_context_usable(ctx):
     ctx.residual_norm(0, 64, 0x10000, h=0x10000)
     ctx.quant_rows_f8(0x10000, 0, 64, 0x10000, 0x10000)
     ctx.sync()
+
+
+# ------------------------------------------------------------------ every kernel, as chosen
+
+
+def sampled(M, seed):
+    """Rows of the first, a middle and the last tile."""
+    return np.unique(np.concatenate([np.arange(min(M, 20)), np.random.default_rng(seed).integers(0, M, 24), np.arange(max(M - 20, 0), M)]))
+
+
+@pytest.mark.parametrize("fast", [True, False])
+def test_linear_kernels(ctx, fast):
+    """The four kernels of anima_linear, at sizes past their tiles' ends, into bf16 and gated fp32 rows; fp32 x
+    quantized inside the product and before it."""
+    m = amd()
+    prec = m.PREC_BF16 if fast else m.PREC_FP32
+    seen = set()
+    for M, N, K in [(3, 514, 1040), (50, 1030, 2064), (517, 1316, 1424), (1501, 2004, 528), (3901, 4100, 400), (3333, 4104, 4112)]:
+        case(f"linear f8 kernels M={M} N={N} K={K} fast={fast}")
+        w, scale = f8_weight(N, N, K)
+        W = m.weight(m.W_F8, N, K, ctx.upload(w), scale=ctx.upload(scale))
+        w64, idx = weight64(w, scale), sampled(M, N)
+        gate = randn(30, N).astype(np.float32)
+        for kind in ("f8", "f32"):
+            args, x64 = inputs(ctx, M, M, K, kind)
+            y, dy = product64(x64[idx], w64, fast)
+            out = Guarded(ctx, (M, N), np.float32, np.ones((M, N), np.float32))
+            ran_f = ran(ctx, lambda: ctx.linear(W, M, out.ptr, epilogue=m.EPI_GATED, gate=ctx.upload(gate), precision=prec, **args))
+            got, r = out.numpy()[idx], y * gate
+            assert np.all(np.abs(got - (1 + r)) <= dy * np.abs(gate) + 2 * U * (1 + 2 * np.abs(r)))
+            out = Guarded(ctx, (M, N), np.uint16)
+            ctx.linear(W, M, out.ptr, out_bf16=True, precision=prec, **args)
+            gb = torch.from_numpy(out.numpy()[idx].view(np.int16)).view(torch.bfloat16).double().numpy()
+            assert np.all(np.abs(gb - y) <= dy * (1 + 2.0 ** -8) + 2.0 ** -8 * np.abs(y))
+            seen.add(tuple(sorted(ran_f)))
+    names = {n for t in seen for n in t}
+    assert {"gemm.f8.skinny", "gemm.f8.64x64", "gemm.f8.128x128", "gemm.f8.256x256", "quant.f8"} <= names
+    assert ("gemm.f8.skinny",) in seen and ("gemm.f8.skinny", "quant.f8") in seen
+
+
+@pytest.mark.parametrize("fast", [True, False])
+def test_glu_kernels(ctx, fast):
+    """The five kernels of anima_linear_glu, into fp32 and e4m3 rows (from the tile, or by a pass)."""
+    m = amd()
+    prec = m.PREC_BF16 if fast else m.PREC_FP32
+    names = set()
+    for M, F, K in [(3, 272, 1040), (517, 1040, 1040), (900, 4112, 272), (2101, 1296, 272), (1300, 8208, 528), (3333, 4112, 1040)]:
+        (wg, sg), (wu, su) = f8_weight(F, F, K), f8_weight(F + 1, F, K)
+        G, Up = m.weight(m.W_F8, F, K, ctx.upload(wg), scale=ctx.upload(sg)), m.weight(m.W_F8, F, K, ctx.upload(wu), scale=ctx.upload(su))
+        args, x64 = inputs(ctx, M, M, K, "f8")
+        idx = sampled(M, F)
+        g, dg = product64(x64[idx], weight64(wg, sg), fast)
+        u, du = product64(x64[idx], weight64(wu, su), fast)
+        a, da = act64(g, "silu"), act_error(g, "silu", dg)
+        h = a * u
+        dh = da * (np.abs(u) + du) + np.abs(a) * du + 2 * U * np.abs(h)
+        out = Guarded(ctx, (M, F), np.float32)
+        q, s = Guarded(ctx, (M, F), np.uint8), Guarded(ctx, (-(-F // 128), M), np.float32)
+        case(f"linear_glu kernels M={M} F={F} K={K} fast={fast}")
+        n1 = ran(ctx, lambda: ctx.linear_glu(G, Up, M, act="silu", out=out.ptr, precision=prec, **args))
+        n2 = ran(ctx, lambda: ctx.linear_glu(G, Up, M, act="silu", out_q=q.ptr, out_s=s.ptr, precision=prec, **args))
+        print(n1, n2, flush=True)
+        names |= n1 | n2
+        assert np.all(np.abs(out.numpy()[idx] - h) <= dh)
+        check_f8_rows(q.numpy()[idx], s.numpy()[:, idx], h, dh)
+    assert names == {"glu.f8.skinny", "glu.f8.64x128", "glu.f8.128x128", "glu.f8.64x256", "glu.f8.256x256", "quant.f8"}
+
+
+def test_quant_many_rows(ctx):
+    """More blocks than one launch's whole waves of workgroups, an odd row count, both types."""
+    m = amd()
+    M, K = 70001, 272
+    x = randn(31, 4096 * K).reshape(4096, K).astype(np.float32)
+    x = np.tile(x, (-(-M // 4096), 1))[:M] * np.linspace(0.5, 2, M, dtype=np.float32)[:, None]
+    for wide in (False, True):
+        case(f"quant f8 many rows bf16={wide}")
+        bits, val = bf16(x) if wide else (x, x)
+        q, s = Guarded(ctx, (M, K), np.uint8), Guarded(ctx, (3, M), np.float32)
+        ctx.quant_rows_f8(ctx.upload(bits), M, K, q.ptr, s.ptr, bf16=wide)
+        rq, rs = quant_ref(val)
+        assert np.array_equal(q.numpy(), rq) and np.array_equal(s.numpy(), rs)
