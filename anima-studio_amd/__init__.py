@@ -461,10 +461,10 @@ class Context:
     def linear(self, W, M, out, *, x=None, ldx=0, x_rotated=True, xq=None, xs=None, ldc=0, alpha=0.0, act="none",
                epilogue=EPI_STORE, gate=None, gate_off=0, acc_out=None, add=None, ld_add=0, lora_xa=None,
                ld_lora_xa=0, lora_b=None, lora_r=0, lora_cols=0, precision=PREC_BF16, out_bf16=False):
-        """anima_linear; precision, out_bf16: of f8 weights (sums in 32 bits; bf16 rows out); lora_xa / lora_b / lora_r: the LoRA delta's factors for the quantized
+        """anima_linear; lora_xa / lora_b / lora_r: the LoRA delta's factors for the quantized
         GEMM's epilogue (A products [M][ld_lora_xa] fp32, B as three bf16 planes [3][N][lora_r]);
         lora_cols > 0: block-diagonal ranks, column n reading xa columns (n // lora_cols) * lora_r
-        + k."""
+        + k.  f8 weights: precision (PREC_FP32: sums in 32 bits), out_bf16 (bf16 rows out)."""
         # (the fields in order, absent pointers as they are: half the time of keywords, on every short call)
         d = LinearDesc(M, ctypes.pointer(W), x and _ptr(x), ldx, int(x_rotated), xq and _ptr(xq), xs and _ptr(xs),
                        _ptr(out), ldc, alpha, ACT[act] if isinstance(act, str) else act, epilogue, gate and _ptr(gate),

@@ -637,9 +637,9 @@ __global__ __launch_bounds__(64 * SKW) void f8_skinny(F8Args a) {
 
 // f8_tile: one BM x BN output tile per workgroup (GLU: BN / 2 columns of each projection), waves of WM x WN.
 // A stage is one block of 128 k: BM rows of x, BN of the weight (128 bytes each) and BM scales, filled NST - 1
-// stages ahead by buffer_load ... lds.  LDS row r holds eight 16-byte units, unit u at slot u ^ (r % 8): a copy
-// (eight whole rows, 1 KiB) is contiguous in LDS as the instruction needs it, and eight consecutive rows' reads
-// of one unit touch every bank once.  Rows past M (N) lie past their resource's end and units past K are sent
+// stages ahead by buffer_load ... lds.  LDS row r holds eight 16-byte units, unit u at slot u ^ (r / 2 % 8): a copy
+// (eight whole rows, 1 KiB) is contiguous in LDS as the instruction needs it, and sixteen consecutive rows' reads
+// of one unit touch each of the 64 banks once (229 bytes per cycle and CU; 120 with r % 8).  Rows past M (N) lie past their resource's end and units past K are sent
 // there: they read as zero.  GLU: each 64 rows of the weight tile are 32 of the gate and the same 32 of the up
 // projection, so that a lane holds both values of an output.
 typedef __attribute__((address_space(3))) void f8_lds_t;
@@ -712,20 +712,31 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void f8_tile(F8Args 
   // The lanes' parts of the addresses are formed again for every stage (the asm keeps them there): registers are
   // what the sums leave, and a spilled one waits for all copies in flight.
   int ikb = 0;  // the next block to copy (into buffer p = ikb % NST)
-  const auto issue = [&](int p) __attribute__((always_inline)) {
+  uint32_t lx[2], lw[2], soff;
+  const auto lanes = [&]() __attribute__((always_inline)) {
     int l;
     asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
-    const int unit = (l & 7) ^ (l >> 3), k = ikb * 128;
-    const uint32_t kl = k + 16 * unit < K ? (uint32_t)(k + 16 * unit) : F8_PAST;
-    const uint32_t lx = (uint32_t)(l >> 3) * (uint32_t)a.ldx + kl, lw = (uint32_t)(l >> 3) * (uint32_t)K + kl;
-    const uint32_t soff = wave < SPW ? 4 * (64 * wave + l) : 4 * ((l & 1) * KB);
+    const int unit = (l & 7) ^ (l >> 4), k = ikb * 128;  // (rows of an odd eight: unit ^ 4)
 #pragma unroll
-    for (int c = 0; c < CPW; c++)
+    for (int o = 0; o < 2; o++) {
+      const int kl = k + 16 * (unit ^ 4 * o);
+      lx[o] = (uint32_t)(l >> 3) * (uint32_t)a.ldx + (kl < K ? (uint32_t)kl : F8_PAST);
+      lw[o] = (uint32_t)(l >> 3) * (uint32_t)K + (kl < K ? (uint32_t)kl : F8_PAST);
+    }
+    soff = wave < SPW ? 4 * (64 * wave + l) : 4 * ((l & 1) * KB);
+  };
+  const auto copies = [&](int p, int c0, int c1) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = c0; c < c1 && c < CPW; c++) {
+      const uint32_t even = src[c] ? lw[c & 1] : lx[c & 1], odd = src[c] ? lw[~c & 1] : lx[~c & 1];
       f8_copy16(src[c] == 0 ? rx : src[c] == 1 ? rw : rw2, smem + (wave * CPW + c) * 1024 + (src[c] ? WO - XB + p * WB : p * XB),
-                (src[c] ? lw : lx) + roff[c]);
-    const int kbc = min(ikb, KB - 1);  // (past the last block its scales again, unused)
-    f8_copy4(f8_rsrc(sbase + kbc * sstep, srec - (wave < SPW ? 0 : 4 * kbc)), smem + sdst + p * sdstep, soff);
-    ikb++;
+                (CPW % 2 && wave & 1 ? odd : even) + roff[c]);
+    }
+    if (c1 == CPW + 1) {
+      const int kbc = min(ikb, KB - 1);  // (past the last block its scales again, unused)
+      f8_copy4(f8_rsrc(sbase + kbc * sstep, srec - (wave < SPW ? 0 : 4 * kbc)), smem + sdst + p * sdstep, soff);
+      ikb++;
+    }
   };
   f32x16 acc[MT][NT];
 #pragma unroll
@@ -736,7 +747,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void f8_tile(F8Args 
   int xa[4], wa[4];
 #pragma unroll
   for (int c = 0; c < 4; c++) {
-    const int f = r * 128 + 16 * ((2 * c + hf) ^ (r & 7));
+    const int f = r * 128 + 16 * ((2 * c + hf) ^ (r >> 1 & 7));
     xa[c] = f + wm * 128;
     wa[c] = f + wn * 128 + WO;
   }
@@ -752,9 +763,23 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void f8_tile(F8Args 
   const auto wunit = [&](int p, int j, int c) __attribute__((always_inline)) { return *(const i32x4*)(smem + wa[c] + p * WB + 4096 * j); };
 
   // The order of a stage is written out (sched_barrier): a tile's sums are scaled and added between the products of
-  // the tiles after it.
+  // the tiles after it.  A stage's copies are issued one by one between the products of the last tiles of one stage
+  // and of the first ones of the next (slots): all at once, they would wait for each other at the CU's one address
+  // unit (72 of 16 cycles each) and the products behind them (a stage of 256 x 256 3700 cycles, spread 2850, without
+  // copies 2650; with 32-bit sums 6500, 6050 and 5600).
+  constexpr int T = MT * NT;
+  constexpr bool SPREAD = WIDE ? T >= 4 : MT >= 2;
+  constexpr int SLOTS = WIDE ? 16 : 4 * NT;
+  static_assert(!SPREAD || NST == 2, "the wait counts");
+  const auto slot = [&](int p, int n) __attribute__((always_inline)) {
+    if constexpr (SPREAD) copies(p, (CPW + 1) * n / SLOTS, (CPW + 1) * (n + 1) / SLOTS);
+  };
+  constexpr int FIRST = SPREAD ? (CPW + 1) / 2 : CPW + 1;  // of the last stage before the loop
 #pragma unroll
-  for (int p = 0; p < NST; p++) issue(p);
+  for (int p = 0; p < NST; p++) {
+    lanes();
+    copies(p, 0, p + 1 < NST ? CPW + 1 : FIRST);
+  }
   const auto stages = [&](const auto& stage) __attribute__((always_inline)) {  // the buffer as a constant
     int kb = 0;
     for (; kb + NST <= KB; kb += NST) {
@@ -773,11 +798,11 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void f8_tile(F8Args 
     __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
     F8_WAIT_VM((NST - 2) * (CPW + 1));
     f8_barrier();
-    issue(p);
+    lanes();
+    if constexpr (!SPREAD) copies(p, 0, CPW + 1);
   };
-  F8_WAIT_VM((NST - 1) * (CPW + 1));
+  F8_WAIT_VM((NST - 2) * (CPW + 1) + FIRST);
   f8_barrier();
-  constexpr int T = MT * NT;
   static_assert((MT == 1 || MT % 2 == 0) && (T == 1 || T % 2 == 0), "fragments and sums alternate");
   f32x16 d[2];
   float sp = 0.0f;  // the scale of the tile in the other d
@@ -809,6 +834,8 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void f8_tile(F8Args 
             if (i + 1 == MT) wr[q / 2] = wunit(last ? pn : p, (j + 1) % NT, q / 2);
           }
           d[t & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[q], xq, q ? d[t & 1] : f32x16{}, 0, 0, 0);
+          if (t == 0) slot((p + NST - 1) % NST, 8 + q);
+          if (last) slot(p, q);
           if constexpr (T > 1) axpy(sp, d[(t + 1) & 1], acc[pt % MT][pt / MT], 2 * q, 2 * q + 2);
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -845,6 +872,8 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void f8_tile(F8Args 
 #pragma unroll
         for (int h = 0; h < 2; h++) {
           d[t & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[j][h], xf[i & 1][h], h ? d[t & 1] : f32x16{}, 0, 0, 0, 0, 0, 0);
+          if (i == 0) slot((p + NST - 1) % NST, 2 * NT + 2 * j + h);
+          if (i + 1 == MT) slot(p, 2 * j + h);
           if constexpr (T > 1) axpy(sp, d[(t + 1) & 1], acc[pt / NT][pt % NT], 8 * h, 8 * h + 8);
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -1140,20 +1169,20 @@ static int64_t f8_tiles(int kind, bool glu, int64_t M, int64_t N) {
 
 // Microseconds of a product (f8_skinny: base + step for each block of k of a wave + work for each 4096 blocks that all
 // its workgroups read; tiles: base + for each tile per CU step for each block of k, round for each tile after the first)
-// + out for a million outputs.  Fitted to 4000 products of M = 1 .. 8192, N and K = 64 .. 8192: the choice takes
-// 0.2 to 0.7% longer than the best kernel in the mean.  Small products are bound by the depth of one
+// + out for a million outputs.  Fitted to 1100 products of M = 1 .. 8192, N and K = 64 .. 8192: the choice takes
+// 0.1 to 0.9% longer than the best kernel in the mean.  Small products are bound by the depth of one
 // workgroup's k loop, so they take the waves of f8_skinny or small tiles; large ones by the bytes that a tile's
-// operands move per product (43 x 2048 x 1024: 4.6, 64x64 8.6, 256x256 33 us; 8192 x 2048 x 8192: 64x64 219, 256x256 124).
+// operands move per product (43 x 2048 x 1024: 4.6, 64x64 8.6, 256x256 33 us; 8192 x 2048 x 8192: 64x64 220, 256x256 116).
 // The gated form leaves e4m3 rows from the tiles of 128 columns; from the others they cost a pass.
 static int f8_choose(anima_ctx* c, bool glu, bool f8_out, int64_t M, int64_t N, int K, int precision) {
   struct Fit {
     float base, step, round, out;
   };
   static const Fit fit[2][2][F8_COUNT] = {
-      {{{1.56f, 1.05f, 1.60f, 0.0f}, {6.94f, 1.57f, 1.44f, 0.64f}, {4.51f, 0.68f, 0.0f, 0.60f}, {}, {3.23f, 0.316f, 0.0f, 0.66f}},
-       {{1.56f, 1.05f, 1.58f, 0.0f}, {6.98f, 2.74f, 1.84f, 0.69f}, {4.48f, 1.06f, 0.0f, 0.61f}, {}, {3.29f, 0.394f, 0.0f, 0.62f}}},
-      {{{1.15f, 1.84f, 2.74f, 0.08f}, {7.69f, 1.65f, 5.87f, 0.93f}, {4.77f, 0.68f, 0.0f, 1.02f}, {4.80f, 0.80f, 2.90f, 1.0f}, {4.80f, 0.512f, 0.2f, 1.15f}},
-       {{1.15f, 1.84f, 2.74f, 0.08f}, {7.76f, 2.77f, 5.30f, 0.96f}, {4.79f, 1.05f, 0.0f, 1.05f}, {4.80f, 1.15f, 2.90f, 1.02f}, {4.85f, 0.747f, 0.2f, 1.05f}}}};
+      {{{1.50f, 1.10f, 1.55f, 0.0f}, {6.92f, 1.23f, 1.58f, 0.69f}, {4.30f, 0.68f, 0.0f, 0.62f}, {}, {3.24f, 0.31f, 0.0f, 0.66f}},
+       {{1.50f, 1.12f, 1.58f, 0.0f}, {6.75f, 2.59f, 0.0f, 0.62f}, {4.30f, 1.00f, 0.0f, 0.59f}, {}, {3.33f, 0.40f, 0.0f, 0.63f}}},
+      {{{1.15f, 1.80f, 2.75f, 0.08f}, {7.80f, 1.34f, 5.96f, 0.92f}, {4.66f, 0.73f, 0.0f, 0.97f}, {4.82f, 0.78f, 3.04f, 1.25f}, {4.84f, 0.535f, 0.2f, 1.05f}},
+       {{1.15f, 1.80f, 2.75f, 0.08f}, {7.50f, 2.61f, 6.00f, 0.90f}, {4.59f, 0.99f, 0.0f, 1.08f}, {4.80f, 1.17f, 2.60f, 1.25f}, {4.87f, 0.76f, 0.2f, 1.10f}}}};
   const int KB = (K + 127) / 128;
   int best = F8_256;
   float bt = 0.0f;
