@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import json
 import os
+import struct
 
 import numpy as np
 
@@ -117,6 +118,19 @@ class ResNormDesc(ctypes.Structure):
                 ("y_bf16", ctypes.c_int)]
 
 
+def _packer(cls):
+    """Packs values of a descriptor's fields, in order, into the bytes of its C struct: less than half the time of
+    building the ctypes object, on every call (pointers: 0 for none)."""
+    codes = {ctypes.c_int: "i", _i64: "q", ctypes.c_float: "f"}
+    s = struct.Struct("@" + "".join(codes.get(t, "P") for _, t in cls._fields_) + "0P")
+    if s.size != ctypes.sizeof(cls):
+        raise RuntimeError(f"{cls.__name__}: {s.size} bytes packed, {ctypes.sizeof(cls)} in the library")
+    return s.pack
+
+
+_linear_desc, _glu_desc, _resnorm_desc = _packer(LinearDesc), _packer(GluDesc), _packer(ResNormDesc)
+
+
 ABI_STRUCTS = {"anima_attn_desc": AttnDesc, "anima_linear_desc": LinearDesc, "anima_weight": Weight,
                "anima_sampler_desc": SamplerDesc, "anima_conv_desc": ConvDesc, "anima_limits": Limits,
                "anima_qkv_desc": QkvDesc, "anima_glu_desc": GluDesc, "anima_resnorm_desc": ResNormDesc}
@@ -195,7 +209,7 @@ def lib():
                                              _i64, ctypes.c_float, ctypes.c_int]
         L.anima_patchify.argtypes = [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp]
         L.anima_unpatchify.argtypes = [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp]
-        L.anima_linear.argtypes = [_vp, ctypes.POINTER(LinearDesc)]
+        L.anima_linear.argtypes = [_vp, _vp]  # (packed descriptors: bytes)
         L.anima_weight_unpack_w4.argtypes = [_vp, ctypes.POINTER(Weight), _vp]
         L.anima_sampler_step.argtypes = [_vp, ctypes.POINTER(SamplerDesc)]
         L.anima_split3_bf16.argtypes = [_vp, _vp, _vp, _i64]
@@ -207,8 +221,8 @@ def lib():
         L.anima_fill_random.argtypes = [_vp, _vp, _i64, ctypes.c_int, ctypes.c_uint64, ctypes.c_float, ctypes.c_float]
         L.anima_quant_rows_f8.argtypes = [_vp, _vp, ctypes.c_int, _i64, ctypes.c_int, _i64, _vp, _vp]
         L.anima_weight_quant_f8.argtypes = [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp]
-        L.anima_linear_glu.argtypes = [_vp, P(GluDesc)]
-        L.anima_residual_norm.argtypes = [_vp, P(ResNormDesc)]
+        L.anima_linear_glu.argtypes = [_vp, _vp]
+        L.anima_residual_norm.argtypes = [_vp, _vp]
         L.anima_graph_begin.argtypes = [_vp]
         L.anima_graph_end.argtypes = [_vp, P(_vp)]
         L.anima_graph_launch.argtypes = [_vp, _vp]
@@ -465,12 +479,10 @@ class Context:
         GEMM's epilogue (A products [M][ld_lora_xa] fp32, B as three bf16 planes [3][N][lora_r]);
         lora_cols > 0: block-diagonal ranks, column n reading xa columns (n // lora_cols) * lora_r
         + k.  f8 weights: precision (PREC_FP32: sums in 32 bits), out_bf16 (bf16 rows out)."""
-        # (the fields in order, absent pointers as they are: half the time of keywords, on every short call)
-        d = LinearDesc(M, ctypes.pointer(W), x and _ptr(x), ldx, int(x_rotated), xq and _ptr(xq), xs and _ptr(xs),
-                       _ptr(out), ldc, alpha, ACT[act] if isinstance(act, str) else act, epilogue, gate and _ptr(gate),
-                       gate_off, acc_out and _ptr(acc_out), add and _ptr(add), ld_add, lora_xa and _ptr(lora_xa),
-                       ld_lora_xa, lora_b and _ptr(lora_b), lora_r, lora_cols, precision, int(out_bf16))
-        return self._check(lib().anima_linear(self.h, ctypes.byref(d)))
+        d = _linear_desc(M, ctypes.addressof(W), _adr(x), ldx, x_rotated, _adr(xq), _adr(xs), _adr(out), ldc, alpha,
+                         ACT[act] if isinstance(act, str) else act, epilogue, _adr(gate), gate_off, _adr(acc_out), _adr(add), ld_add,
+                         _adr(lora_xa), ld_lora_xa, _adr(lora_b), lora_r, lora_cols, precision, out_bf16)
+        return self._check(lib().anima_linear(self.h, d))
 
     def linear_qkv(self, W, M, out, *, B, L, H, k_norm=None, rope_cs=None, rope_sin_off=0, kv_prep=None, eps=1e-6,
                    x=None, ldx=0, x_rotated=True, xq=None, xs=None, ldc=0, alpha=0.0, lora_xa=None, ld_lora_xa=0,
@@ -505,21 +517,19 @@ class Context:
                    out_s=None, precision=PREC_BF16):
         """anima_linear_glu: act(x W_gate^T) * (x W_up^T) of two W_F8 weights, from fp32 rows x or e4m3 rows
         xq, xs, into fp32 rows out or e4m3 rows out_q, out_s."""
-        d = GluDesc(M, ctypes.pointer(gate), ctypes.pointer(up), x and _ptr(x), xq and _ptr(xq), xs and _ptr(xs), ldx,
-                    ACT[act] if isinstance(act, str) else act, out and _ptr(out), ldc, out_q and _ptr(out_q),
-                    out_s and _ptr(out_s), precision)
-        return self._check(lib().anima_linear_glu(self.h, ctypes.byref(d)))
+        d = _glu_desc(M, ctypes.addressof(gate), ctypes.addressof(up), _adr(x), _adr(xq), _adr(xs), ldx,
+                      ACT[act] if isinstance(act, str) else act, _adr(out), ldc, _adr(out_q), _adr(out_s), precision)
+        return self._check(lib().anima_linear_glu(self.h, d))
 
     def residual_norm(self, rows, cols, x, *, ldx=0, y=None, ldy=0, y_bf16=False, post_w=None, gate=None, gate_ld=0, res_scale=0.0,
                       norm="rms", norm_w=None, shift=None, scale=None, mod_ld=0, group_rows=0, eps=1e-6, h=None, ldh=0,
                       q=None, s=None):
         """anima_residual_norm: x += res_scale * gate * post(y) in place, then the norm of x (norm "rms" /
         "layer", norm_w, shift / scale) as fp32 rows h and / or e4m3 rows q, s."""
-        d = ResNormDesc(rows, cols, _ptr(x), ldx, y and _ptr(y), ldy, post_w and _ptr(post_w), gate and _ptr(gate), gate_ld,
-                        res_scale, NORM[norm] if isinstance(norm, str) else norm, norm_w and _ptr(norm_w),
-                        shift and _ptr(shift), scale and _ptr(scale), mod_ld, group_rows, eps, h and _ptr(h), ldh,
-                        q and _ptr(q), s and _ptr(s), int(y_bf16))
-        return self._check(lib().anima_residual_norm(self.h, ctypes.byref(d)))
+        d = _resnorm_desc(rows, cols, _adr(x), ldx, _adr(y), ldy, _adr(post_w), _adr(gate), gate_ld, res_scale,
+                          NORM[norm] if isinstance(norm, str) else norm, _adr(norm_w), _adr(shift), _adr(scale), mod_ld, group_rows,
+                          eps, _adr(h), ldh, _adr(q), _adr(s), y_bf16)
+        return self._check(lib().anima_residual_norm(self.h, d))
 
     def split3_bf16(self, src, dst, n):
         return self._check(lib().anima_split3_bf16(self.h, _ptr(src), _ptr(dst), n))
@@ -573,6 +583,10 @@ def rope_table(angles: np.ndarray) -> np.ndarray:
 
 def dit_rope_table(Hp: int, Wp: int) -> np.ndarray:
     return rope_table(dit_rope_angles(Hp, Wp))
+
+
+def _adr(b):
+    return b if type(b) is int else 0 if b is None else b.ptr if isinstance(b, DeviceBuffer) else int(b)
 
 
 def _ptr(b):

@@ -136,3 +136,18 @@ def test_null_context():
     assert L.anima_weight_quant_f8(None, None, 0, 1, 16, None, None) == -1
     assert L.anima_linear_glu(None, None) == -1
     assert L.anima_residual_norm(None, None) == -1
+
+
+@pytest.mark.parametrize("name", ["LinearDesc", "GluDesc", "ResNormDesc"])
+def test_packed_descriptors(name):
+    """The binding's packed descriptors are the bytes of the ctypes structs (whose offsets the library confirms)."""
+    m = amd()
+    cls = getattr(m, name)
+    pack = {"LinearDesc": m._linear_desc, "GluDesc": m._glu_desc, "ResNormDesc": m._resnorm_desc}[name]
+    values = [i + 0.25 if t is ctypes.c_float else i + 1 for i, (_, t) in enumerate(cls._fields_)]
+    d = cls.from_buffer_copy(pack(*values))
+    for (f, t), v in zip(cls._fields_, values):
+        got = getattr(d, f)
+        if issubclass(t, ctypes._Pointer):
+            got = ctypes.cast(got, ctypes.c_void_p).value
+        assert got == v, f
