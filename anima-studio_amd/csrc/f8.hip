@@ -768,7 +768,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void f8_tile(F8Args 
   // unit (72 of 16 cycles each) and the products behind them (a stage of 256 x 256 3700 cycles, spread 2850, without
   // copies 2650; with 32-bit sums 6500, 6050 and 5600).
   constexpr int T = MT * NT;
-  constexpr bool SPREAD = WIDE ? T >= 4 : MT >= 2;
+  constexpr bool SPREAD = T >= 4;
   constexpr int SLOTS = WIDE ? 16 : 4 * NT;
   static_assert(!SPREAD || NST == 2, "the wait counts");
   const auto slot = [&](int p, int n) __attribute__((always_inline)) {
@@ -1160,40 +1160,42 @@ static void f8_input(F8Args& a, const anima_weight* W, const float* x, int64_t l
 }
 
 // The kernel for a product's sizes.
-enum { F8_SKINNY, F8_256, F8_128, F8_64x256, F8_64, F8_COUNT };
+enum { F8_SKINNY, F8_256, F8_128, F8_MID, F8_64, F8_COUNT };  // (F8_MID: 128 x 64, gated 64 x 256)
 
 static int64_t f8_tiles(int kind, bool glu, int64_t M, int64_t N) {
-  static const int bm[F8_COUNT] = {16, 256, 128, 64, 64}, bn[2][F8_COUNT] = {{16, 256, 128, 256, 64}, {16, 128, 64, 128, 64}};
-  return (M + bm[kind] - 1) / bm[kind] * ((N + bn[glu][kind] - 1) / bn[glu][kind]);
+  static const int bm[2][F8_COUNT] = {{16, 256, 128, 128, 64}, {16, 256, 128, 64, 64}};
+  static const int bn[2][F8_COUNT] = {{16, 256, 128, 64, 64}, {16, 128, 64, 128, 64}};  // (gated: columns of each projection)
+  return (M + bm[glu][kind] - 1) / bm[glu][kind] * ((N + bn[glu][kind] - 1) / bn[glu][kind]);
 }
 
 // Microseconds of a product (f8_skinny: base + step for each block of k of a wave + work for each 4096 blocks that all
 // its workgroups read; tiles: base + for each tile per CU step for each block of k, round for each tile after the first)
-// + out for a million outputs.  Fitted to 1100 products of M = 1 .. 8192, N and K = 64 .. 8192: the choice takes
-// 0.1 to 0.9% longer than the best kernel in the mean.  Small products are bound by the depth of one
+// + out for a million outputs.  Fitted to 3000 products of M = 1 .. 8192, N and K = 64 .. 8192: the choice takes
+// 0.1 to 1.0% longer than the best kernel in the mean.  Small products are bound by the depth of one
 // workgroup's k loop, so they take the waves of f8_skinny or small tiles; large ones by the bytes that a tile's
-// operands move per product (43 x 2048 x 1024: 4.6, 64x64 8.6, 256x256 33 us; 8192 x 2048 x 8192: 64x64 220, 256x256 116).
+// operands move per product (43 x 2048 x 1024: 4.6, 64x64 8.6, 256x256
+// 33 us; 3013 x 1316 x 1424 gated with 32-bit sums: 64x64 26.2, 128x64 23.3, 128x128 31.6; 8192 x 2048 x 8192: 64x64 220,
+// 256x256 116).
 // The gated form leaves e4m3 rows from the tiles of 128 columns; from the others they cost a pass.
 static int f8_choose(anima_ctx* c, bool glu, bool f8_out, int64_t M, int64_t N, int K, int precision) {
   struct Fit {
     float base, step, round, out;
   };
   static const Fit fit[2][2][F8_COUNT] = {
-      {{{1.50f, 1.10f, 1.55f, 0.0f}, {6.92f, 1.23f, 1.58f, 0.69f}, {4.30f, 0.68f, 0.0f, 0.62f}, {}, {3.24f, 0.31f, 0.0f, 0.66f}},
-       {{1.50f, 1.12f, 1.58f, 0.0f}, {6.75f, 2.59f, 0.0f, 0.62f}, {4.30f, 1.00f, 0.0f, 0.59f}, {}, {3.33f, 0.40f, 0.0f, 0.63f}}},
+      {{{1.55f, 1.05f, 1.58f, 0.0f}, {6.95f, 1.20f, 1.40f, 0.66f}, {4.20f, 0.68f, 0.0f, 0.61f}, {3.59f, 0.40f, 0.1f, 0.76f}, {3.24f, 0.312f, 0.0f, 0.67f}},
+       {{1.55f, 1.05f, 1.60f, 0.0f}, {6.72f, 2.58f, 0.5f, 0.69f}, {4.31f, 0.99f, 0.0f, 0.62f}, {3.51f, 0.625f, 0.0f, 0.53f}, {3.30f, 0.408f, 0.0f, 0.61f}}},
       {{{1.15f, 1.80f, 2.75f, 0.08f}, {7.80f, 1.34f, 5.96f, 0.92f}, {4.66f, 0.73f, 0.0f, 0.97f}, {4.82f, 0.78f, 3.04f, 1.25f}, {4.84f, 0.535f, 0.2f, 1.05f}},
        {{1.15f, 1.80f, 2.75f, 0.08f}, {7.50f, 2.61f, 6.00f, 0.90f}, {4.59f, 0.99f, 0.0f, 1.08f}, {4.80f, 1.17f, 2.60f, 1.25f}, {4.87f, 0.76f, 0.2f, 1.10f}}}};
   const int KB = (K + 127) / 128;
   int best = F8_256;
   float bt = 0.0f;
   for (int k = F8_COUNT - 1; k >= 0; k--) {
-    if (k == F8_64x256 && !glu) continue;
     if (k == F8_SKINNY && M > 16 * 65535) continue;  // (the grid's second dimension)
     const int64_t tiles = f8_tiles(k, glu, M, N);
     if (tiles > 0x7fffffff) continue;
     const Fit& f = fit[glu][precision][k];
     const float rounds = (float)((tiles + c->num_cus - 1) / c->num_cus), mn = 1e-6f * (float)M * (float)N;
-    const bool fused = k == F8_256 || k == F8_64x256;
+    const bool fused = k == F8_256 || k == F8_MID;
     float us = f.base + f.out * mn * (f8_out && fused ? 0.6f : 1.0f);
     if (k == F8_SKINNY) us += f.step * (float)((KB + SKW - 1) / SKW) + f.round * (float)tiles * (float)KB / 4096.0f;
     else us += f.step * (float)KB * rounds + f.round * (rounds - 1.0f);
@@ -1216,18 +1218,18 @@ static bool f8_quantizes(const F8Args& a, int kind) {
   return work <= 240 && work * f8_tiles(F8_SKINNY, false, a.M, a.N) <= 50000;
 }
 
-template <int BM, int BN, int WM, int WN, int NST, bool GLU>
+template <int BM, int BN, int WM, int WN, int NST, bool GLU, int WIDE_NST = NST>
 static void f8_tile_launch(anima_ctx* c, const F8Args& a, int precision) {
   constexpr int FN = GLU ? BN / 2 : BN;
   const dim3 grid((unsigned)((int64_t)((a.N + FN - 1) / FN) * ((a.M + BM - 1) / BM))), block(64 * (BM / WM) * (BN / WN));
-  if (precision == ANIMA_PREC_FP32) hipLaunchKernelGGL((f8_tile<BM, BN, WM, WN, NST, true, GLU>), grid, block, 0, c->stream, a);
+  if (precision == ANIMA_PREC_FP32) hipLaunchKernelGGL((f8_tile<BM, BN, WM, WN, WIDE_NST, true, GLU>), grid, block, 0, c->stream, a);
   else hipLaunchKernelGGL((f8_tile<BM, BN, WM, WN, NST, false, GLU>), grid, block, 0, c->stream, a);
 }
 
 // Runs the product of a's rows, quantizing fp32 rows first where the kernel takes e4m3 rows.
 template <bool GLU>
 static int f8_product(anima_ctx* c, F8Args a, int kind, int precision) {
-  static const char* const names[2][F8_COUNT] = {{"gemm.f8.skinny", "gemm.f8.256x256", "gemm.f8.128x128", "", "gemm.f8.64x64"},
+  static const char* const names[2][F8_COUNT] = {{"gemm.f8.skinny", "gemm.f8.256x256", "gemm.f8.128x128", "gemm.f8.128x64", "gemm.f8.64x64"},
                                                  {"glu.f8.skinny", "glu.f8.256x256", "glu.f8.128x128", "glu.f8.64x256", "glu.f8.64x128"}};
   void* scratch = nullptr;
   if (a.x && !f8_quantizes(a, kind)) {
@@ -1252,8 +1254,9 @@ static int f8_product(anima_ctx* c, F8Args a, int kind, int precision) {
     f8_tile_launch<256, 256, 128, 64, 2, GLU>(c, a, precision);
   } else if (kind == F8_128) {
     f8_tile_launch<128, 128, 64, 64, 2, GLU>(c, a, precision);
-  } else if (GLU && kind == F8_64x256) {
+  } else if (kind == F8_MID) {
     if constexpr (GLU) f8_tile_launch<64, 256, 32, 64, 2, GLU>(c, a, precision);
+    else f8_tile_launch<128, 64, 64, 32, 3, GLU, 2>(c, a, precision);  // (1024 x 2048 x 2048 with 2 stages 15.1 us, 3 12.4; 32-bit sums 16.6, 16.8)
   } else {
     if constexpr (GLU) f8_tile_launch<64, 128, 32, 64, 3, GLU>(c, a, precision);
     else f8_tile_launch<64, 64, 32, 32, 3, GLU>(c, a, precision);
@@ -1308,7 +1311,7 @@ int linear_glu_launch(anima_ctx* c, const anima_glu_desc* d) {
   a.ldc = d->ldc ? d->ldc : a.N;
   void* tmp = nullptr;
   const int kind = f8_choose(c, true, d->out_q != nullptr, a.M, a.N, a.K, d->precision);
-  if (d->out_q && (kind == F8_256 || kind == F8_64x256)) {  // a tile is one block of 128 columns
+  if (d->out_q && (kind == F8_256 || kind == F8_MID)) {  // a tile is one block of 128 columns
     a.oq = d->out_q;
     a.os = d->out_s;
     a.out = nullptr;

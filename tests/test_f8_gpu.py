@@ -710,12 +710,12 @@ def sampled(M, seed):
 
 @pytest.mark.parametrize("fast", [True, False])
 def test_linear_kernels(ctx, fast):
-    """The four kernels of anima_linear, at sizes past their tiles' ends, into bf16 and gated fp32 rows; fp32 x
+    """The five kernels of anima_linear, at sizes past their tiles' ends, into bf16 and gated fp32 rows; fp32 x
     quantized inside the product and before it."""
     m = amd()
     prec = m.PREC_BF16 if fast else m.PREC_FP32
     seen = set()
-    for M, N, K in [(3, 514, 1040), (50, 1030, 2064), (517, 1316, 1424), (1501, 2004, 528), (3901, 4100, 400), (3333, 4104, 4112)]:
+    for M, N, K in [(3, 514, 1040), (50, 1030, 2064), (517, 1316, 1424), (1499, 900, 528), (1501, 2004, 528), (3901, 4100, 400), (3333, 4104, 4112)]:
         case(f"linear f8 kernels M={M} N={N} K={K} fast={fast}")
         w, scale = f8_weight(N, N, K)
         W = m.weight(m.W_F8, N, K, ctx.upload(w), scale=ctx.upload(scale))
@@ -734,7 +734,7 @@ def test_linear_kernels(ctx, fast):
             assert np.all(np.abs(gb - y) <= dy * (1 + 2.0 ** -8) + 2.0 ** -8 * np.abs(y))
             seen.add(tuple(sorted(ran_f)))
     names = {n for t in seen for n in t}
-    assert {"gemm.f8.skinny", "gemm.f8.64x64", "gemm.f8.128x128", "gemm.f8.256x256", "quant.f8"} <= names
+    assert {"gemm.f8.skinny", "gemm.f8.64x64", "gemm.f8.128x64", "gemm.f8.128x128", "gemm.f8.256x256", "quant.f8"} <= names
     assert ("gemm.f8.skinny",) in seen and ("gemm.f8.skinny", "quant.f8") in seen
 
 
