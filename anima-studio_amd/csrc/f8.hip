@@ -277,10 +277,11 @@ __global__ __launch_bounds__(T, EARLY ? 1 : 4) void residual_norm_kernel(NormArg
   const uint32_t row32 = xcd_remap(blockIdx.x, gridDim.x);
   const int64_t row = row32, grp = a.group_rows >= a.rows ? 0 : row32 / (uint32_t)a.group_rows;
   const float inv = 1.0f / (float)a.cols;
-  // every access through a resource of the row's bytes: past its end loads give zeros and stores nothing
+  // every access through a resource of the row's bytes: past its end loads give zeros and stores nothing (the whole
+  // offset in the lanes' part: the bound is of that part alone)
   const __amdgpu_buffer_rsrc_t rx = f8_rsrc(a.x + row * a.ldx, 4 * a.cols);
   const auto load = [&](__amdgpu_buffer_rsrc_t rs, int i) {
-    return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, 16 * t, 16 * T * i, 0));
+    return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, 16 * t + 16 * T * i, 0, 0));
   };
   const auto vec = [&](const float* p, int i) { return p ? load(f8_rsrc(p, 4 * a.cols), i) : f32x4{}; };
   const float *gate = a.gate ? a.gate + grp * a.gate_ld : nullptr, *scale = a.scale ? a.scale + grp * a.mod_ld : nullptr,
@@ -293,7 +294,7 @@ __global__ __launch_bounds__(T, EARLY ? 1 : 4) void residual_norm_kernel(NormArg
       const __amdgpu_buffer_rsrc_t ry = f8_rsrc((const uint16_t*)a.y + row * a.ldy, 2 * a.cols);
 #pragma unroll
       for (int i = 0; i < NV; i++) {
-        const auto u = __builtin_amdgcn_raw_buffer_load_b64(ry, 8 * t, 8 * T * i, 0);
+        const auto u = __builtin_amdgcn_raw_buffer_load_b64(ry, 8 * t + 8 * T * i, 0, 0);
         y[i] = f32x4{__builtin_bit_cast(float, u[0] << 16), __builtin_bit_cast(float, u[0] & 0xffff0000u), __builtin_bit_cast(float, u[1] << 16),
                      __builtin_bit_cast(float, u[1] & 0xffff0000u)};
       }
@@ -334,7 +335,7 @@ __global__ __launch_bounds__(T, EARLY ? 1 : 4) void residual_norm_kernel(NormArg
     for (int i = 0; i < NV; i++) {
 #pragma unroll
       for (int e = 0; e < 4; e++) x[i][e] = __builtin_fmaf(a.res_scale, y[i][e], x[i][e]);
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x[i]), rx, 16 * t, 16 * T * i, 0);
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x[i]), rx, 16 * t + 16 * T * i, 0, 0);
     }
   }
   if (a.layer) {
@@ -371,7 +372,7 @@ __global__ __launch_bounds__(T, EARLY ? 1 : 4) void residual_norm_kernel(NormArg
   if (a.h) {
     const __amdgpu_buffer_rsrc_t rh = f8_rsrc(a.h + row * a.ldh, 4 * a.cols);
 #pragma unroll
-    for (int i = 0; i < NV; i++) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x[i]), rh, 16 * t, 16 * T * i, 0);
+    for (int i = 0; i < NV; i++) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x[i]), rh, 16 * t + 16 * T * i, 0, 0);
   }
   if (a.q) {  // 32 lanes hold one block of 128 columns (zeros past the row)
     const __amdgpu_buffer_rsrc_t rq = f8_rsrc(a.q + row * a.cols, a.cols);
@@ -379,7 +380,7 @@ __global__ __launch_bounds__(T, EARLY ? 1 : 4) void residual_norm_kernel(NormArg
     for (int i = 0; i < NV; i++) {
       float sc, mul;
       f8_scale(half_umax(amax4(x[i], 0)), sc, mul);
-      __builtin_amdgcn_raw_buffer_store_b32(f8_pack(x[i], mul), rq, 4 * t, 4 * T * i, 0);
+      __builtin_amdgcn_raw_buffer_store_b32(f8_pack(x[i], mul), rq, 4 * t + 4 * T * i, 0, 0);
       const int c = 4 * (t + T * i);
       if ((t & 31) == 0 && c < a.cols) a.s[(int64_t)(c >> 7) * a.rows + row] = sc;
     }

@@ -57,12 +57,13 @@ inline int check_f8_operands(const char* who, const anima_weight* W, const float
   if (W->N < 1 || W->K < 1 || W->K % 16 || W->K > F8_MAX_K)
     return fail(ANIMA_E_ARG, "%s: an f8 weight needs K %% 16 == 0 and K <= %d (N=%d K=%d)", who, F8_MAX_K, W->N, W->K);
   if (!W->w || !W->scale) return fail(ANIMA_E_ARG, "%s: an f8 weight needs its data and block scales", who);
-  if (!f8_al(W->w, 16)) return fail(ANIMA_E_ARG, "%s: the f8 weight's data on 16 bytes", who);
+  if (!f8_al(W->w, 16) || !f8_al(W->scale, 4) || !f8_al(W->bias, 4))
+    return fail(ANIMA_E_ARG, "%s: the f8 weight's data on 16 bytes, its scales and bias on 4", who);
   const int64_t ld = ldx ? ldx : W->K;
   if (ld < W->K) return fail(ANIMA_E_ARG, "%s: ldx=%lld < K=%d", who, (long long)ld, W->K);
   if (xq) {
     if (!xs) return fail(ANIMA_E_ARG, "%s: e4m3 rows need their scales xs", who);
-    if (ld % 16 || !f8_al(xq, 16)) return fail(ANIMA_E_ARG, "%s: e4m3 rows on 16 bytes (ldx=%lld)", who, (long long)ld);
+    if (ld % 16 || !f8_al(xq, 16) || !f8_al(xs, 4)) return fail(ANIMA_E_ARG, "%s: e4m3 rows on 16 bytes (ldx=%lld)", who, (long long)ld);
     if (ld > F8_MAX_LDX) return fail(ANIMA_E_UNSUPPORTED, "%s: ldx=%lld above %lld", who, (long long)ld, (long long)F8_MAX_LDX);
   } else {
     if (!x) return fail(ANIMA_E_ARG, "%s: needs fp32 rows x or e4m3 rows xq", who);
@@ -79,7 +80,8 @@ inline int check_linear_f8(const anima_linear_desc* d, F8Msg fail) {
   if (d->out_bf16 != 0 && d->out_bf16 != 1) return fail(ANIMA_E_ARG, "anima_linear: out_bf16=%d", d->out_bf16);
   if (d->out_bf16 && d->epilogue != ANIMA_EPI_STORE)
     return fail(ANIMA_E_UNSUPPORTED, "anima_linear: bf16 rows with the store epilogue only (%d)", d->epilogue);
-  if (!f8_al(d->out, d->out_bf16 ? 2 : 4)) return fail(ANIMA_E_ARG, "anima_linear: out off its element size");
+  if (!f8_al(d->out, d->out_bf16 ? 2 : 4) || !f8_al(d->gate, 4) || !f8_al(d->add, 4))
+    return fail(ANIMA_E_ARG, "anima_linear: out, gate or add off its element size");
   return check_f8_operands("anima_linear", d->W, d->x, d->ldx, d->xq, d->xs, fail);
 }
 
@@ -101,11 +103,11 @@ inline int check_linear_glu(const anima_glu_desc* d, F8Msg fail) {
   if (rc != ANIMA_OK) return rc;
   if (d->out_q) {
     if (d->out) return fail(ANIMA_E_ARG, "anima_linear_glu: fp32 rows or e4m3 rows, not both");
-    if (!d->out_s) return fail(ANIMA_E_ARG, "anima_linear_glu: e4m3 rows need out_s");
+    if (!d->out_s || !f8_al(d->out_s, 4)) return fail(ANIMA_E_ARG, "anima_linear_glu: e4m3 rows need out_s");
     if (G->N % 16 || !f8_al(d->out_q, 16))
       return fail(ANIMA_E_ARG, "anima_linear_glu: e4m3 rows on 16 bytes need N %% 16 == 0 (N=%d)", G->N);
   } else {
-    if (!d->out) return fail(ANIMA_E_ARG, "anima_linear_glu: null out");
+    if (!d->out || !f8_al(d->out, 4)) return fail(ANIMA_E_ARG, "anima_linear_glu: null out, or off 4 bytes");
     if (d->out_s) return fail(ANIMA_E_ARG, "anima_linear_glu: out_s without out_q");
     if (d->ldc && d->ldc < G->N) return fail(ANIMA_E_ARG, "anima_linear_glu: ldc=%lld < N=%d", (long long)d->ldc, G->N);
   }
@@ -133,6 +135,7 @@ inline int check_residual_norm(const anima_resnorm_desc* d, F8Msg fail) {
   if (ldx < C || ldx % 4 || ldy < C || ldy % 4 || ldh < C || ldh % 4 || ldm < C || ldm % 4 || ldg < C || ldg % 4)
     return fail(ANIMA_E_ARG, "anima_residual_norm: row strides of at least cols=%d, multiples of 4", d->cols);
   if (!f8_al(d->y, d->y_bf16 ? 8 : 16)) return fail(ANIMA_E_ARG, "anima_residual_norm: rows of y on four elements");
+  if (!f8_al(d->s, 4)) return fail(ANIMA_E_ARG, "anima_residual_norm: s off 4 bytes");
   const void* const p[] = {d->x, d->post_w, d->gate, d->norm_w, d->shift, d->scale, d->h, d->q};
   for (const void* v : p)
     if (!f8_al(v, 16)) return fail(ANIMA_E_ARG, "anima_residual_norm: rows and vectors on 16 bytes");

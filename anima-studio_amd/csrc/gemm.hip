@@ -2729,6 +2729,8 @@ int linear_launch(anima_ctx* c, const anima_linear_desc* d, int64_t s3_plane) {
                   d->lora_cols, N, (long long)d->ld_lora_xa);
     if (d->add) return fail(c, ANIMA_E_UNSUPPORTED, "anima_linear: the LoRA epilogue and an add term together");
   }
+  if (W->kind != ANIMA_W_F8 && (d->precision || d->out_bf16))
+    return fail(c, ANIMA_E_UNSUPPORTED, "anima_linear: precision and out_bf16 are for f8 weights (kind %d)", W->kind);
   if (M == 0) return ANIMA_OK;
 
   if (W->kind == ANIMA_W_F8) return linear_f8_launch(c, d);
@@ -3033,6 +3035,7 @@ int linear_qkv_launch(anima_ctx* c, const anima_linear_desc* d, const anima_qkv_
   if ((N != 3 * H * HD_K && !qonly) || K % GBK)
     return fail(c, ANIMA_E_ARG, "anima_linear_qkv: N=%d must be 3 * H * 128 = %d (or H * 128 with q_prep), K %% %d == 0", N,
                 3 * H * HD_K, GBK);
+  if (d->precision || d->out_bf16) return fail(c, ANIMA_E_UNSUPPORTED, "anima_linear_qkv: precision and out_bf16 are for anima_linear");
   if (d->epilogue != ANIMA_EPI_STORE || d->act != ANIMA_ACT_NONE || d->add || d->acc_out)
     return fail(c, ANIMA_E_UNSUPPORTED, "anima_linear_qkv: plain store only (no activation, residual, gate, add term or acc_out)");
   const bool lora = d->lora_xa || d->lora_b || d->lora_r;

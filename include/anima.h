@@ -525,7 +525,7 @@ int anima_set_w4_path(anima_ctx* ctx, int path);
 
 /* Rows x[M] (fp32, or bf16 with x_bf16 = 1; ldx elements apart, 0 -> K) to e4m3 rows q[M][K] with a scale for
  * every 128 columns, s[ceil(K/128)][M]: block-major, since a product's k step reads one block of many rows.
- * K % 16 == 0; x and q 16-byte aligned, ldx a multiple of 16 bytes. */
+ * K % 16 == 0; x and q 16-byte aligned, ldx a multiple of 16 bytes.  q and s overlap no input. */
 int anima_quant_rows_f8(anima_ctx* ctx, const void* x, int x_bf16, int64_t M, int K, int64_t ldx, uint8_t* q, float* s);
 /* A weight w[N][K] (fp32, or bf16 with w_bf16 = 1) to the data q[N][K] and scales [ceil(N/128)][ceil(K/128)]
  * of an ANIMA_W_F8 weight, one scale per 128 x 128 block: a loader's conversion of a bf16 checkpoint. */
@@ -535,7 +535,7 @@ int anima_weight_quant_f8(anima_ctx* ctx, const void* w, int w_bf16, int N, int 
  * app/models/qwen3.js:66-72) in one kernel:
  *   h[m][n] = act(x W_gate^T + b_gate) * (x W_up^T + b_up)
  * both products as anima_linear's of f8 weights, h as fp32 rows or as the e4m3 rows that the following
- * product reads.  The two weights have equal N and K and biases of their own. */
+ * product reads.  The two weights have equal N and K and biases of their own.  Outputs overlap no input. */
 typedef struct {
   int64_t M;
   const anima_weight* gate;

@@ -81,7 +81,8 @@ def weight(**kw):
     ({}, {"xq": P + 8, "xs": P}, -1), ({}, {"xq": P, "xs": P, "ldx": 168}, -1),
     ({}, {"xq": P, "xs": P, "ldx": (1 << 22) + 16}, -5), ({}, {"acc_out": P}, -5), ({}, {"precision": 1, "out_bf16": 1}, 0),
     ({}, {"precision": 2}, -1), ({}, {"out_bf16": 2}, -1), ({}, {"out_bf16": 1, "epilogue": 1}, -5), ({}, {"out": P + 2}, -1),
-    ({}, {"out_bf16": 1, "out": P + 2}, 0), ({}, {"out_bf16": 1, "out": P + 1}, -1)])
+    ({}, {"out_bf16": 1, "out": P + 2}, 0), ({}, {"out_bf16": 1, "out": P + 1}, -1), ({"scale": P + 2}, {}, -1),
+    ({"bias": P + 1}, {}, -1), ({}, {"xq": P, "xs": P + 2}, -1), ({}, {"gate": P + 2}, -1), ({}, {"add": P + 2}, -1)])
 def test_linear(checks, w, change, code):
     m = amd()
     W = weight(**w)
@@ -96,7 +97,8 @@ def test_linear(checks, w, change, code):
     ({}, {"w": P + 4}, {}, -1), ({}, {}, {"M": -2}, -1), ({}, {}, {"act": 3}, -1), ({}, {}, {"x": 0}, -1),
     ({}, {}, {"out": 0}, -1), ({}, {}, {"ldc": 99}, -1), ({}, {}, {"out_s": P}, -1), ({}, {}, {"out_q": P, "out_s": P}, -1),
     ({}, {}, {"out": 0, "out_q": P, "out_s": P}, -1),  # N = 100: rows of 100 bytes
-    ({"N": 96}, {"N": 96}, {"out": 0, "out_q": P}, -1), ({"N": 96}, {"N": 96}, {"out": 0, "out_q": P + 8, "out_s": P}, -1)])
+    ({"N": 96}, {"N": 96}, {"out": 0, "out_q": P}, -1), ({"N": 96}, {"N": 96}, {"out": 0, "out_q": P + 8, "out_s": P}, -1),
+    ({}, {"bias": P + 2}, {}, -1), ({}, {}, {"out": P + 2}, -1), ({"N": 96}, {"N": 96}, {"out": 0, "out_q": P, "out_s": P + 2}, -1)])
 def test_glu(checks, g, u, change, code):
     m = amd()
     G, U = weight(**g), weight(**u)
@@ -118,7 +120,7 @@ def test_glu_null(checks):
     ({"eps": -1.0}, -1), ({"eps": float("nan")}, -1), ({"x": 0}, -1), ({"h": 0}, -1), ({"q": P}, -1), ({"s": P}, -1),
     ({"cols": 68, "q": P, "s": P}, -1), ({"post_w": P}, -1), ({"gate": P}, -1), ({"shift": P}, -1), ({"scale": P}, -1),
     ({"group_rows": -1}, -1), ({"ldx": 60}, -1), ({"ldy": 66}, -1), ({"ldh": 2}, -1), ({"mod_ld": 63}, -1), ({"gate_ld": 65}, -1),
-    ({"x": P + 4}, -1), ({"y": P + 8}, -1), ({"y": P + 8, "y_bf16": 1}, 0), ({"y": P + 4, "y_bf16": 1}, -1), ({"y_bf16": 2}, -1), ({"norm_w": P + 4}, -1), ({"h": P + 8}, -1)])
+    ({"x": P + 4}, -1), ({"y": P + 8}, -1), ({"y": P + 8, "y_bf16": 1}, 0), ({"y": P + 4, "y_bf16": 1}, -1), ({"y_bf16": 2}, -1), ({"norm_w": P + 4}, -1), ({"h": P + 8}, -1), ({"q": P, "s": P + 2}, -1)])
 def test_residual_norm(checks, change, code):
     m = amd()
     d = m.ResNormDesc(**dict(dict(rows=3, cols=64, x=P, norm=0, eps=1e-6, h=P), **change))

@@ -9,7 +9,7 @@ matrix instructions drop, of each of eight products but the largest, what lies 2
 7 * 2^-13 of the largest, so 7 * 2^-13 A more; and as the dropped parts have either sign, in the 2-norm 1e-4 (seven
 parts uniform up to 2^-13 of a largest product of about twice the mean square: 2^-13 * 2 * sqrt(7 / 12 / 8) = 6.6e-5).
 Norms are compared with
-64-bit norms: sums of squares are off by at most 2^-24 (log2 of the row's threads + terms per thread <= 32) of
+64-bit norms: sums of squares are off by at most 2^-24 (log2 of the row's threads + terms per thread <= 41) of
 themselves, and every other step rounds once.
 """
 
@@ -779,3 +779,59 @@ def test_quant_many_rows(ctx):
         ctx.quant_rows_f8(ctx.upload(bits), M, K, q.ptr, s.ptr, bf16=wide)
         rq, rs = quant_ref(val)
         assert np.array_equal(q.numpy(), rq) and np.array_equal(s.numpy(), rs)
+
+
+@pytest.mark.parametrize("C", [132, 256, 272, 516, 1028, 1600, 2052, 4112, 8208, 16384])
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+def test_residual_norm_many_rows(ctx, C, norm):
+    """The kernels of more rows than four per CU, rows that end inside a thread's stride, inside wider rows."""
+    case(f"residual_norm many rows C={C} {norm}")
+    m = amd()
+    rows, ld, groups = 1031, C + 12, 5
+    per = -(-rows // groups)
+    x0, y = randn(70, rows * ld).reshape(rows, ld).astype(np.float32), randn(71, rows * C).reshape(rows, C).astype(np.float32)
+    vec = (1 + 0.3 * randn(72, 2 * C)).reshape(2, C).astype(np.float32)
+    mod = (0.5 * randn(73, groups * 3 * C)).reshape(groups, 3 * C).astype(np.float32)
+    d_mod, x = ctx.upload(mod), Guarded(ctx, (rows, ld), np.float32, x0)
+    h = Guarded(ctx, (rows, ld), np.float32, np.full((rows, ld), 7, np.float32))
+    f8 = C % 16 == 0
+    q, s = Guarded(ctx, (rows, C), np.uint8), Guarded(ctx, (-(-C // 128), rows), np.float32)
+    ctx.residual_norm(rows, C, x.ptr, ldx=ld, y=ctx.upload(y), post_w=ctx.upload(vec[0]), gate=d_mod.ptr + 8 * C, gate_ld=3 * C, res_scale=0.5,
+                      norm=norm, norm_w=ctx.upload(vec[1]), shift=d_mod.ptr, scale=d_mod.ptr + 4 * C, mod_ld=3 * C, group_rows=per,
+                      h=h.ptr, ldh=ld, q=q.ptr if f8 else None, s=s.ptr if f8 else None)
+    g64 = mod[np.arange(rows) // per].astype(np.float64)
+    y64 = y.astype(np.float64)
+    post = y64 / np.sqrt((y64 * y64).mean(1, keepdims=True) + 1e-6) * vec[0] * g64[:, 2 * C:]
+    x64 = x0[:, :C] + 0.5 * post
+    gx, gh = x.numpy(), h.numpy()
+    # half of the sum's 44 roundings (41, the mean's two, eps), two of 1 / sqrt, three products; the addition
+    dx = 28 * U * np.abs(post) + U * (np.abs(x64) + np.abs(post))
+    assert np.all(np.abs(gx[:, :C] - x64) <= dx)
+    assert np.array_equal(gx[:, C:], x0[:, C:]) and np.all(gh[:, C:] == 7)
+    v = gx[:, :C].astype(np.float64)  # from here on the rows that the kernel wrote
+    mean = v.mean(1, keepdims=True) if norm == "layer" else 0.0
+    dv = 40 * U * (np.abs(v) + np.abs(v).mean(1, keepdims=True))
+    v = v - mean
+    var = (v * v).mean(1, keepdims=True) + 1e-6
+    dr = (np.abs(v) * dv).mean(1, keepdims=True) / var + 24 * U
+    f, sh = vec[1] * (1 + g64[:, C:2 * C]), g64[:, :C]
+    ref = v / np.sqrt(var) * f + sh
+    dh = (dv + np.abs(v) * (dr + 8 * U)) / np.sqrt(var) * np.abs(f) + 4 * U * (np.abs(ref) + np.abs(sh))
+    assert np.all(np.abs(gh[:, :C] - ref) <= dh)
+    if f8:
+        rq, rs = quant_ref(gh[:, :C])
+        assert np.array_equal(q.numpy(), rq) and np.array_equal(s.numpy(), rs)
+
+
+def test_f8_fields_of_other_kinds(ctx):
+    """precision and out_bf16 with another kind of weight are refused, before anything is written."""
+    case("precision / out_bf16 with a bf16 weight")
+    m = amd()
+    W = m.weight(m.W_BF16, 32, 64, ctx.upload(np.zeros((32, 64), np.uint16)))
+    x, out = ctx.upload(np.ones((4, 64), np.float32)), Guarded(ctx, (4, 32), np.float32, np.full((4, 32), 3, np.float32))
+    for change in (dict(precision=m.PREC_FP32), dict(out_bf16=True)):
+        with pytest.raises(m.AnimaError, match="f8 weights"):
+            ctx.linear(W, 4, out.ptr, x=x, **change)
+        assert np.all(out.numpy() == 3)
+    ctx.linear(W, 4, out.ptr, x=x)
+    assert np.all(out.numpy() == 0)
