@@ -817,10 +817,13 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void f8_tile(F8Args 
   float sp = 0.0f;  // the scale of the tile in the other d
   d[1] = f32x16{};
   if constexpr (WIDE) {
-    // One column of tiles after the other, so that the widened weight is one fragment; x is widened again
-    // for each column, and its registers take the next row's units one by one.
+    // One column of tiles after the other, so that the widened weight is one fragment; x, where its fragments of all
+    // rows find registers, is widened once (KEEP: 128 x 128 tiles 7 to 10% faster), else again for each column, and
+    // the registers of its bytes take the next row's units one by one.
     i32x4 xr[4], wr[4];
     bf16x8 wf[8];
+    constexpr bool KEEP = NT > 1 && MT <= 2;
+    bf16x8 xk[KEEP ? MT : 1][8];
 #pragma unroll
     for (int c = 0; c < 4; c++) {
       xr[c] = xunit(0, 0, c);
@@ -836,10 +839,11 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void f8_tile(F8Args 
         if (last) turn(p);
 #pragma unroll
         for (int q = 0; q < 8; q++) {
-          const bf16x8 xq = widen8(xr[q / 2][q % 2 * 2], xr[q / 2][q % 2 * 2 + 1]);
+          bf16x8& xq = xk[KEEP ? i : 0][q];
+          if (!KEEP || j == 0) xq = widen8(xr[q / 2][q % 2 * 2], xr[q / 2][q % 2 * 2 + 1]);
           if (i == 0) wf[q] = widen8(wr[q / 2][q % 2 * 2], wr[q / 2][q % 2 * 2 + 1]);
           if (q % 2 == 1) {  // the unit is done with
-            xr[q / 2] = xunit(last ? pn : p, (i + 1) % MT, q / 2);
+            if (!KEEP || last || (j == 0 && i + 1 < MT)) xr[q / 2] = xunit(last ? pn : p, (i + 1) % MT, q / 2);
             if (i + 1 == MT) wr[q / 2] = wunit(last ? pn : p, (j + 1) % NT, q / 2);
           }
           d[t & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[q], xq, q ? d[t & 1] : f32x16{}, 0, 0, 0);
@@ -1183,7 +1187,7 @@ static int64_t f8_tiles(int kind, bool glu, int64_t M, int64_t N) {
 // 0.1 to 1.0% longer than the best kernel in the mean.  Small products are bound by the depth of one
 // workgroup's k loop, so they take the waves of f8_skinny or small tiles; large ones by the bytes that a tile's
 // operands move per product (43 x 2048 x 1024: 4.6, 64x64 8.6, 256x256
-// 33 us; 3013 x 1316 x 1424 gated with 32-bit sums: 64x64 26.2, 128x64 23.3, 128x128 31.6; 8192 x 2048 x 8192: 64x64 220,
+// 33 us; 3013 x 1316 x 1424 gated with 32-bit sums: 64x64 26.2, 128x64 23.3; 8192 x 2048 x 8192: 64x64 220,
 // 256x256 116).
 // The gated form leaves e4m3 rows from the tiles of 128 columns; from the others they cost a pass.
 static int f8_choose(anima_ctx* c, bool glu, bool f8_out, int64_t M, int64_t N, int K, int precision) {
@@ -1192,9 +1196,9 @@ static int f8_choose(anima_ctx* c, bool glu, bool f8_out, int64_t M, int64_t N, 
   };
   static const Fit fit[2][2][F8_COUNT] = {
       {{{1.55f, 1.05f, 1.58f, 0.0f}, {6.95f, 1.20f, 1.40f, 0.66f}, {4.20f, 0.68f, 0.0f, 0.61f}, {3.59f, 0.40f, 0.1f, 0.76f}, {3.24f, 0.312f, 0.0f, 0.67f}},
-       {{1.55f, 1.05f, 1.60f, 0.0f}, {6.72f, 2.58f, 0.5f, 0.69f}, {4.31f, 0.99f, 0.0f, 0.62f}, {3.51f, 0.625f, 0.0f, 0.53f}, {3.30f, 0.408f, 0.0f, 0.61f}}},
+       {{1.55f, 1.05f, 1.60f, 0.0f}, {6.75f, 2.58f, 2.0f, 0.72f}, {4.31f, 0.852f, 0.0f, 0.70f}, {3.51f, 0.625f, 0.0f, 0.53f}, {3.30f, 0.408f, 0.0f, 0.61f}}},
       {{{1.15f, 1.80f, 2.75f, 0.08f}, {7.80f, 1.34f, 5.96f, 0.92f}, {4.66f, 0.73f, 0.0f, 0.97f}, {4.82f, 0.78f, 3.04f, 1.25f}, {4.84f, 0.535f, 0.2f, 1.05f}},
-       {{1.15f, 1.80f, 2.75f, 0.08f}, {7.50f, 2.61f, 6.00f, 0.90f}, {4.59f, 0.99f, 0.0f, 1.08f}, {4.80f, 1.17f, 2.60f, 1.25f}, {4.87f, 0.76f, 0.2f, 1.10f}}}};
+       {{1.15f, 1.80f, 2.75f, 0.08f}, {7.50f, 2.61f, 5.70f, 0.85f}, {4.56f, 0.87f, 0.0f, 1.09f}, {4.83f, 1.07f, 2.65f, 1.23f}, {4.85f, 0.723f, 0.2f, 1.15f}}}};
   const int KB = (K + 127) / 128;
   int best = F8_256;
   float bt = 0.0f;
