@@ -479,9 +479,12 @@ class Context:
         GEMM's epilogue (A products [M][ld_lora_xa] fp32, B as three bf16 planes [3][N][lora_r]);
         lora_cols > 0: block-diagonal ranks, column n reading xa columns (n // lora_cols) * lora_r
         + k.  f8 weights: precision (PREC_FP32: sums in 32 bits), out_bf16 (bf16 rows out)."""
-        d = _linear_desc(M, ctypes.addressof(W), _adr(x), ldx, x_rotated, _adr(xq), _adr(xs), _adr(out), ldc, alpha,
-                         ACT[act] if isinstance(act, str) else act, epilogue, _adr(gate), gate_off, _adr(acc_out), _adr(add), ld_add,
-                         _adr(lora_xa), ld_lora_xa, _adr(lora_b), lora_r, lora_cols, precision, out_bf16)
+        # (absent pointers without a call: half a microsecond of every linear)
+        d = _linear_desc(M, ctypes.addressof(W), x and _adr(x) or 0, ldx, x_rotated, xq and _adr(xq) or 0,
+                         xs and _adr(xs) or 0, _adr(out), ldc, alpha, ACT[act] if isinstance(act, str) else act, epilogue,
+                         gate and _adr(gate) or 0, gate_off, acc_out and _adr(acc_out) or 0, add and _adr(add) or 0, ld_add,
+                         lora_xa and _adr(lora_xa) or 0, ld_lora_xa, lora_b and _adr(lora_b) or 0, lora_r, lora_cols,
+                         precision, out_bf16)
         return self._check(lib().anima_linear(self.h, d))
 
     def linear_qkv(self, W, M, out, *, B, L, H, k_norm=None, rope_cs=None, rope_sin_off=0, kv_prep=None, eps=1e-6,
@@ -517,8 +520,9 @@ class Context:
                    out_s=None, precision=PREC_BF16):
         """anima_linear_glu: act(x W_gate^T) * (x W_up^T) of two W_F8 weights, from fp32 rows x or e4m3 rows
         xq, xs, into fp32 rows out or e4m3 rows out_q, out_s."""
-        d = _glu_desc(M, ctypes.addressof(gate), ctypes.addressof(up), _adr(x), _adr(xq), _adr(xs), ldx,
-                      ACT[act] if isinstance(act, str) else act, _adr(out), ldc, _adr(out_q), _adr(out_s), precision)
+        d = _glu_desc(M, ctypes.addressof(gate), ctypes.addressof(up), x and _adr(x) or 0, xq and _adr(xq) or 0,
+                      xs and _adr(xs) or 0, ldx, ACT[act] if isinstance(act, str) else act, out and _adr(out) or 0, ldc,
+                      out_q and _adr(out_q) or 0, out_s and _adr(out_s) or 0, precision)
         return self._check(lib().anima_linear_glu(self.h, d))
 
     def residual_norm(self, rows, cols, x, *, ldx=0, y=None, ldy=0, y_bf16=False, post_w=None, gate=None, gate_ld=0, res_scale=0.0,
@@ -526,9 +530,10 @@ class Context:
                       q=None, s=None):
         """anima_residual_norm: x += res_scale * gate * post(y) in place, then the norm of x (norm "rms" /
         "layer", norm_w, shift / scale) as fp32 rows h and / or e4m3 rows q, s."""
-        d = _resnorm_desc(rows, cols, _adr(x), ldx, _adr(y), ldy, _adr(post_w), _adr(gate), gate_ld, res_scale,
-                          NORM[norm] if isinstance(norm, str) else norm, _adr(norm_w), _adr(shift), _adr(scale), mod_ld, group_rows,
-                          eps, _adr(h), ldh, _adr(q), _adr(s), y_bf16)
+        d = _resnorm_desc(rows, cols, _adr(x), ldx, y and _adr(y) or 0, ldy, post_w and _adr(post_w) or 0,
+                          gate and _adr(gate) or 0, gate_ld, res_scale, NORM[norm] if isinstance(norm, str) else norm,
+                          norm_w and _adr(norm_w) or 0, shift and _adr(shift) or 0, scale and _adr(scale) or 0, mod_ld,
+                          group_rows, eps, h and _adr(h) or 0, ldh, q and _adr(q) or 0, s and _adr(s) or 0, y_bf16)
         return self._check(lib().anima_residual_norm(self.h, d))
 
     def split3_bf16(self, src, dst, n):
