@@ -107,11 +107,17 @@ export function quantizeF8(gpu, W) {
   return W;
 }
 
-// opts.xq of a linear on W: the row form that W's kind reads (int8 rows and e4m3 rows are both bytes)
+// opts.xq of a linear on W: the row form that W's kind reads (int8 rows and e4m3 rows are both bytes),
+// and e4m3 rows of W's width.  Returns their number.
 function checkRows(W, xq) {
   const f8 = xq.q.dtype === "u8";
   if (f8 !== (W.kind === "f8"))
     throw new Error(`${W.name || "linear"}: ${f8 ? "e4m3" : "int8"} rows for a ${W.kind} weight`);
+  if (!f8) return xq.s.size;
+  const [M, K] = xq.q.shape;
+  if (K !== W.K || xq.s.size !== Math.ceil(K / 128) * M)
+    throw new Error(`${W.name || "linear"}: e4m3 rows [${xq.q.shape}] with ${xq.s.size} scales for K = ${W.K}`);
+  return M;
 }
 
 function weightArg(W) {
@@ -128,8 +134,8 @@ function weightArg(W) {
 // result (no residual).
 export function linear(gpu, x, W, opts) {
   const o = opts || {};
-  if (o.xq) checkRows(W, o.xq);
-  const M = o.M !== undefined ? o.M : (o.xq ? o.xq.q.size / W.K : x.size / W.K);
+  const rows = o.xq ? checkRows(W, o.xq) : 0;
+  const M = o.M !== undefined ? o.M : (o.xq ? rows : x.size / W.K);
   // LoRAs: y += sum_i scale_i B_i (A_i x), after the bias and before act / gate (ops.js:55-62).
   // The reference feeds ConvRot layers' LoRAs the rotated input and a rotated A; since
   // (x H)(A H)^T = x A^T, the unrotated x and A are used when x is at hand (no rotation pass), and
@@ -388,7 +394,7 @@ export function linearGlu(gpu, x, Wg, Wu, opts) {
     if (W.lora && W.lora.length) throw new Error(`linearGlu: ${W.name || "weight"} has a LoRA`);
     if (o.xq) checkRows(W, o.xq);
   }
-  const M = o.M !== undefined ? o.M : (o.xq ? o.xq.q.size / Wg.K : x.size / Wg.K);
+  const M = o.M !== undefined ? o.M : (o.xq ? checkRows(Wg, o.xq) : x.size / Wg.K);
   const rows = o.f8 ? f8Rows(gpu, M, Wg.N) : null;
   const out = rows ? null : o.out || gpu.empty([M, Wg.N]);
   native.linearGlu(gpu.ctx, weightArg(Wg), weightArg(Wu), { M, x: o.xq ? 0 : x.buf, xq: o.xq ? o.xq.q.buf : 0,

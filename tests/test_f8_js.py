@@ -90,6 +90,8 @@ def test_refusals():
                "console.log(JSON.stringify({"
                "int8_rows: msg(() => ops.linear(gpu, null, f8, { xq: rows('i8') })),"
                "e4m3_rows: msg(() => ops.linear(gpu, null, i8, { xq: rows('u8') })),"
+               "width: msg(() => ops.linear(gpu, null, f8, { xq: { q: gpu.empty([4, 256], 'u8'), s: gpu.empty([2, 4]) } })),"
+               "scales: msg(() => ops.linearGlu(gpu, null, f8, f8, { xq: { q: gpu.empty([4, 128], 'u8'), s: gpu.empty([1, 3]) } })),"
                "bf16_out: msg(() => ops.linear(gpu, gpu.empty([4, 128]), i8, { outBf16: true })),"
                "lora_rows: msg(() => ops.linear(gpu, null, lora, { xq: rows('u8') })),"
                "lora_bf16: msg(() => ops.linear(gpu, gpu.empty([4, 128]), lora, { outBf16: true })),"
@@ -102,6 +104,7 @@ def test_refusals():
                "}))")
     assert "int8 rows for a f8 weight" in got["int8_rows"]
     assert "e4m3 rows for a i8 weight" in got["e4m3_rows"]
+    assert "rows [4,256] with 8 scales for K = 128" in got["width"] and "rows [4,128] with 3 scales" in got["scales"]
     assert "bf16 results are for f8" in got["bf16_out"]
     assert "needs its input" in got["lora_rows"]
     assert "no bf16 result with a LoRA" in got["lora_bf16"]
