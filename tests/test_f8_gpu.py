@@ -835,3 +835,50 @@ def test_f8_fields_of_other_kinds(ctx):
         assert np.all(out.numpy() == 3)
     ctx.linear(W, 4, out.ptr, x=x)
     assert np.all(out.numpy() == 0)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 1, 16), (2, 3, 32), (1, 5, 144), (4099, 1, 16), (300, 2, 128)])
+@pytest.mark.parametrize("kind", ["f8", "f32"])
+def test_smallest(ctx, M, N, K, kind):
+    case(f"smallest products M={M} N={N} K={K} x={kind}")
+    m = amd()
+    (w, sw), (u, su) = f8_weight(N, N, K), f8_weight(N + 9, N, K)
+    args, x64 = inputs(ctx, M, M, K, kind)
+    W, Up = m.weight(m.W_F8, N, K, ctx.upload(w), scale=ctx.upload(sw)), m.weight(m.W_F8, N, K, ctx.upload(u), scale=ctx.upload(su))
+    y, dy = product64(x64, weight64(w, sw), False)
+    z, dz = product64(x64, weight64(u, su), False)
+    out = Guarded(ctx, (M, N), np.float32)
+    ctx.linear(W, M, out.ptr, precision=m.PREC_FP32, **args)
+    assert np.all(np.abs(out.numpy() - y) <= dy + U * np.abs(y))
+    out = Guarded(ctx, (M, N), np.float32)
+    ctx.linear_glu(W, Up, M, act="none", out=out.ptr, precision=m.PREC_FP32, **args)
+    assert np.all(np.abs(out.numpy() - y * z) <= dy * (np.abs(z) + dz) + np.abs(y) * dz + 3 * U * np.abs(y * z))
+
+
+def test_widest(ctx):
+    """The longest k of a product, and e4m3 rows as far apart as they may be."""
+    m = amd()
+    L = m.lib()
+    M, N, K = 3, 20, 1 << 20
+    case(f"linear f8 M={M} N={N} K={K}")
+    w, scale = f8_weight(80, N, K)
+    args, x64 = inputs(ctx, 81, M, K, "f8")
+    out = Guarded(ctx, (M, N), np.float32)
+    ctx.linear(m.weight(m.W_F8, N, K, ctx.upload(w), scale=ctx.upload(scale)), M, out.ptr, precision=m.PREC_FP32, **args)
+    y, dy = product64(x64, weight64(w, scale), False)
+    assert np.all(np.abs(out.numpy() - y) <= dy + U * np.abs(y))
+    M, N, K, ld = 300, 1500, 272, 1 << 22
+    case(f"linear f8 ldx={ld}")
+    w, scale = f8_weight(82, N, K)
+    q = random_e4m3(83, M, K)
+    s = np.random.default_rng(84).uniform(0.5, 1.5, (3, M)).astype(np.float32) / 100
+    x = ctx.empty(((M - 1) * ld + K,), np.uint8)
+    for r in range(M):
+        ctx._check(L.anima_h2d(ctx.h, x.ptr + r * ld, q[r].ctypes.data, K))
+    W = m.weight(m.W_F8, N, K, ctx.upload(w), scale=ctx.upload(scale))
+    y, dy = product64(rows64(q, s), weight64(w, scale), False)
+    for rows in (5, M):
+        out = Guarded(ctx, (rows, N), np.float32)
+        ctx.linear(W, rows, out.ptr, xq=x, xs=ctx.upload(np.ascontiguousarray(s[:, :rows])), ldx=ld, precision=m.PREC_FP32)
+        assert np.all(np.abs(out.numpy() - y[:rows]) <= dy[:rows] + U * np.abs(y[:rows]))
+    x.release()
