@@ -777,9 +777,8 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void f8_tile(F8Args 
   // unit (72 of 16 cycles each) and the products behind them (a stage of 256 x 256 3700 cycles, spread 2850, without
   // copies 2650; with 32-bit sums 6500, 6050 and 5600).
   constexpr int T = MT * NT;
-  constexpr bool SPREAD = T >= 4;
+  constexpr bool SPREAD = T >= 4 || (WIDE && T == 2 && NST == 3);  // (else the next stage's wait would meet the copies)
   constexpr int SLOTS = WIDE ? 16 : 4 * NT;
-  static_assert(!SPREAD || NST == 2, "the wait counts");
   const auto slot = [&](int p, int n) __attribute__((always_inline)) {
     if constexpr (SPREAD) copies(p, (CPW + 1) * n / SLOTS, (CPW + 1) * (n + 1) / SLOTS);
   };
@@ -1231,11 +1230,11 @@ static bool f8_quantizes(const F8Args& a, int kind) {
   return work <= 240 && work * f8_tiles(F8_SKINNY, false, a.M, a.N) <= 50000;
 }
 
-template <int BM, int BN, int WM, int WN, int NST, bool GLU, int WIDE_NST = NST>
+template <int BM, int BN, int WM, int WN, int NST, bool GLU>
 static void f8_tile_launch(anima_ctx* c, const F8Args& a, int precision) {
   constexpr int FN = GLU ? BN / 2 : BN;
   const dim3 grid((unsigned)((int64_t)((a.N + FN - 1) / FN) * ((a.M + BM - 1) / BM))), block(64 * (BM / WM) * (BN / WN));
-  if (precision == ANIMA_PREC_FP32) hipLaunchKernelGGL((f8_tile<BM, BN, WM, WN, WIDE_NST, true, GLU>), grid, block, 0, c->stream, a);
+  if (precision == ANIMA_PREC_FP32) hipLaunchKernelGGL((f8_tile<BM, BN, WM, WN, NST, true, GLU>), grid, block, 0, c->stream, a);
   else hipLaunchKernelGGL((f8_tile<BM, BN, WM, WN, NST, false, GLU>), grid, block, 0, c->stream, a);
 }
 
@@ -1269,7 +1268,7 @@ static int f8_product(anima_ctx* c, F8Args a, int kind, int precision) {
     f8_tile_launch<128, 128, 64, 64, 2, GLU>(c, a, precision);
   } else if (kind == F8_MID) {
     if constexpr (GLU) f8_tile_launch<64, 256, 32, 64, 2, GLU>(c, a, precision);
-    else f8_tile_launch<128, 64, 64, 32, 3, GLU, 2>(c, a, precision);  // (1024 x 2048 x 2048 with 2 stages 15.1 us, 3 12.4; 32-bit sums 16.6, 16.8)
+    else f8_tile_launch<128, 64, 64, 32, 3, GLU>(c, a, precision);  // (1024 x 2048 x 2048 with 2 stages 15.1 us, 3 12.4)
   } else {
     if constexpr (GLU) f8_tile_launch<64, 128, 32, 64, 3, GLU>(c, a, precision);
     else f8_tile_launch<64, 64, 32, 32, 3, GLU>(c, a, precision);
