@@ -7,14 +7,14 @@
 //           linear, on bf16 weights converted by quantizeF8 or on an e4m3 safetensors file
 //   qwen3   Qwen3.encode of a synthetic text encoder after quantizeF8 (both precisions; recorded,
 //           replayed and eager) and its weights; an encoding with a LoRA of zeros attached
-//   dit     a synthetic DiT's velocities: bf16 weights, after quantizeF8, and with LoRAs of zeros
+//   dit     a synthetic DiT's velocities: bf16 weights, after quantizeF8, and with LoRAs of zeros; graph replays
 
 import fs from "fs";
 import { GPU } from "../../anima-studio_amd/js/gpu.mjs";
 import * as ops from "../../anima-studio_amd/js/ops.mjs";
 import { SafeTensors, SyntheticWeights, concatLinears } from "../../anima-studio_amd/js/weights.mjs";
 import { ropeTable } from "../../anima-studio_amd/js/common.mjs";
-import { AnimaDiT } from "../../anima-studio_amd/js/dit.mjs";
+import { AnimaDiT, ForwardGraph } from "../../anima-studio_amd/js/dit.mjs";
 import { Qwen3 } from "../../anima-studio_amd/js/qwen3.mjs";
 
 const ARR = { f32: Float32Array, u8: Uint8Array, u16: Uint16Array };
@@ -129,6 +129,22 @@ async function dit(gpu, c) {
   await forward("f8");
   model.precision = "bf16";
   await forward("f8bf16");
+  // recorded into a graph and replayed with other latents, an eager forward before each
+  const cond = model.prepareContext(c.ctx.map((p) => gpu.fromArray(load(p), [c.Lk, 1024])));
+  const n = lat.length * lat[0].length;
+  const x = gpu.empty([lat.length, 16, c.h, c.w]), tc = model.timeCond(c.sigma);
+  gpu.write(x, lat[0], 0);
+  gpu.write(x, lat[1], lat[0].length * 4);
+  const fg = await ForwardGraph.capture(model, x, c.h, c.w, cond, tc);
+  const differ = [];
+  for (let i = 0; i < 3; i++) {
+    gpu.write(x, lat[i % 2].map((v) => v * (i + 1)), 0);
+    const e = await gpu.read(await model.forwardDevice(x, c.h, c.w, cond, tc));
+    const g = await gpu.read(fg.run(tc));
+    differ.push(e.reduce((k, v, j) => k + (v !== g[j]), 0));
+  }
+  console.log(JSON.stringify({ differ, n }));
+  fg.release();
   model.precision = "fp32";
   for (const b of model.blocks)
     for (const W of [b.self.qkv, b.self.o, b.cross.q, b.cross.o, b.l1, b.l2]) if (W) zeroLora(gpu, W);

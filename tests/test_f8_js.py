@@ -299,6 +299,7 @@ def test_js_dit_f8(tmp_path):
     log = run_case(tmp_path, spec)
     # qkv (stacked), o, cross q / k / v / o, the two of the feed-forward
     assert json.loads(log.splitlines()[0]) == {"converted": 16}
+    assert json.loads(log.splitlines()[1])["differ"] == [0, 0, 0]  # replays against eager forwards
     bar = ROUNDING * 24 ** 0.5
     for b in range(2):
         v = {t: np.fromfile(f"{out}.{t}.{b}", np.float32) for t in ("bf16w", "f8", "f8bf16", "f8lora")}
