@@ -50,6 +50,7 @@ struct F8Args {
   const float* add;
   int64_t ld_add;
   int M, N, K, KB;
+  int kbs;            // f8_tile: blocks of k of a split (blockIdx.y), whose sums leave as fp32 rows [M][N] of their own
   int vec;            // four columns of out, add, bias and gate at a time
   int obf;            // out is bf16 rows
   uint8_t* oq;        // GLU: e4m3 rows [M][N] instead, and their scales
@@ -695,6 +696,8 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void f8_tile(F8Args 
     tm = row0 + (local - tn * gm);
   }
   const int bm = tm * BM, bn = tn * FN, K = a.K, KB = a.KB;
+  const int kb0 = blockIdx.y * a.kbs, nkb = min(a.kbs, KB - kb0);
+  if (blockIdx.y > 0) a.out += (int64_t)blockIdx.y * a.M * a.N;
   const int wm = (wave % NWM) * WM, wn = (wave / NWM) * WN;
 
   const int mrows = min(BM, a.M - bm), nrows = min(FN, a.N - bn);
@@ -720,7 +723,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void f8_tile(F8Args 
   const int sdst = wave < SPW ? XSO + wave * 256 : WSO + (up ? 256 : 0), sdstep = wave < SPW ? BM * 4 : SB;
   // The lanes' parts of the addresses are formed again for every stage (the asm keeps them there): registers are
   // what the sums leave, and a spilled one waits for all copies in flight.
-  int ikb = 0;  // the next block to copy (into buffer p = ikb % NST)
+  int ikb = kb0;  // the next block to copy (into buffer p = (ikb - kb0) % NST)
   uint32_t lx[2], lw[2], soff;
   const auto lanes = [&]() __attribute__((always_inline)) {
     int l;
@@ -790,14 +793,14 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void f8_tile(F8Args 
   }
   const auto stages = [&](const auto& stage) __attribute__((always_inline)) {  // the buffer as a constant
     int kb = 0;
-    for (; kb + NST <= KB; kb += NST) {
+    for (; kb + NST <= nkb; kb += NST) {
       stage(std::integral_constant<int, 0>{});
       stage(std::integral_constant<int, 1>{});
       if constexpr (NST == 3) stage(std::integral_constant<int, 2>{});
     }
-    if (kb < KB) stage(std::integral_constant<int, 0>{});
+    if (kb < nkb) stage(std::integral_constant<int, 0>{});
     if constexpr (NST == 3)
-      if (kb + 1 < KB) stage(std::integral_constant<int, 1>{});
+      if (kb + 1 < nkb) stage(std::integral_constant<int, 1>{});
   };
   // Stages overlap: before the last tiles of stage kb, whose fragments are in registers by then, a barrier ends every
   // wave's reads of the stage (its buffer is refilled) and publishes stage kb + 1 (arrived once at most the copies of
@@ -1043,6 +1046,27 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void f8_tile(F8Args 
   }
 }
 
+// The sums of a product's splits, added in their order, and its epilogue: a thread holds four columns of a row.
+// Bound by its launch and one trip to memory: 100 x 1300 in six splits (3.6 MB) 3.1 us, 512 x 1024 in four (10.5 MB) 4.1
+// (the loads in turn 4.0 and 4.8).
+constexpr int F8_SPLITS = 8;
+__global__ __launch_bounds__(256) void f8_join(F8Args a, const float* part, int splits) {
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x, quads = (uint32_t)(a.N + 3) / 4, row = i / quads;
+  const int m = (int)row, n = (int)(4 * (i - row * quads));
+  if (m >= a.M) return;
+  const float* p = part + (int64_t)m * a.N;
+  f32x4 v[F8_SPLITS];  // (all asked for before the first is added)
+#pragma unroll
+  for (int s = 0; s < F8_SPLITS; s++) v[s] = s < splits ? f8_ld4(p + (int64_t)s * a.M * a.N, n, a.N, a.vec) : f32x4{};
+  const f32x4 bias = a.bias ? f8_ld4(a.bias, n, a.N, a.vec) : f32x4{};
+  const f32x4 gate = a.epi == ANIMA_EPI_GATED ? f8_ld4(a.gate, n, a.N, a.vec) : f32x4{};
+  const f32x4 c = a.epi != ANIMA_EPI_STORE ? f8_ld_out(a, m, n) : f32x4{};
+  f32x4 r = v[0];
+#pragma unroll
+  for (int s = 1; s < F8_SPLITS; s++) r = r + v[s];
+  f8_store(a, m, n, r, bias, gate, c);
+}
+
 // ------------------------------------------------------------------ host
 
 namespace {
@@ -1189,7 +1213,10 @@ static int64_t f8_tiles(int kind, bool glu, int64_t M, int64_t N) {
 // 33 us; 3013 x 1316 x 1424 gated with 32-bit sums: 64x64 26.2, 128x64 23.3; 8192 x 2048 x 8192: 64x64 220,
 // 256x256 116).
 // The gated form leaves e4m3 rows from the tiles of 128 columns; from the others they cost a pass.
-static int f8_choose(anima_ctx* c, bool glu, bool f8_out, int64_t M, int64_t N, int K, int precision) {
+// Where the tiles leave CUs idle, the k loop of a linear is split (*splits): each split's sums go through memory and
+// f8_join (512 x 1024 x 8192 with 32-bit sums 32.7 us, split 20.0; 64 x 4096 x 4096 20.4, 12.5; 300 x 384 x 4096 10.9,
+// 11.3: not taken).
+static int f8_choose(anima_ctx* c, bool glu, bool f8_out, int64_t M, int64_t N, int K, int precision, int* splits) {
   struct Fit {
     float base, step, round, out;
   };
@@ -1199,8 +1226,8 @@ static int f8_choose(anima_ctx* c, bool glu, bool f8_out, int64_t M, int64_t N, 
       {{{1.15f, 1.80f, 2.75f, 0.08f}, {7.80f, 1.34f, 5.96f, 0.92f}, {4.66f, 0.73f, 0.0f, 0.97f}, {4.82f, 0.78f, 3.04f, 1.25f}, {4.84f, 0.535f, 0.2f, 1.05f}},
        {{1.15f, 1.80f, 2.75f, 0.08f}, {7.50f, 2.61f, 5.70f, 0.85f}, {4.56f, 0.87f, 0.0f, 1.09f}, {4.83f, 1.07f, 2.65f, 1.23f}, {4.85f, 0.723f, 0.2f, 1.15f}}}};
   const int KB = (K + 127) / 128;
-  int best = F8_256;
-  float bt = 0.0f;
+  int best = F8_256, sbest = F8_256, sn = 1;
+  float bt = 0.0f, st = 0.0f;  // of the best kernel, of the best one with its k loop split
   for (int k = F8_COUNT - 1; k >= 0; k--) {
     if (k == F8_SKINNY && M > 16 * 65535) continue;  // (the grid's second dimension)
     const int64_t tiles = f8_tiles(k, glu, M, N);
@@ -1216,8 +1243,22 @@ static int f8_choose(anima_ctx* c, bool glu, bool f8_out, int64_t M, int64_t N, 
       best = k;
       bt = us;
     }
+    if (glu || k == F8_SKINNY || tiles > 2 * c->num_cus || KB < 8) continue;
+    for (int s = 2; s <= F8_SPLITS; s++) {
+      const int kbs = (KB + s - 1) / s, n = (KB + kbs - 1) / kbs;
+      if (kbs < 3 || M * N * n > (1 << 26)) break;
+      const float rs = (float)((tiles * n + c->num_cus - 1) / c->num_cus);
+      us = f.base + f.step * (float)kbs * rs + f.round * (rs - 1.0f) + f.out * mn * (float)n + 2.4f + mn * (1.6f + (float)n);
+      if (st == 0.0f || us < st) {
+        sbest = k;
+        st = us;
+        sn = n;
+      }
+    }
   }
-  return best;
+  const bool split = st > 0.0f && st < 0.9f * bt;  // (what the model is sure of)
+  *splits = split ? sn : 1;
+  return split ? sbest : best;
 }
 
 // Whether fp32 rows are quantized inside f8_skinny (each workgroup quantizes its 16 rows again) instead of by a pass
@@ -1233,14 +1274,14 @@ static bool f8_quantizes(const F8Args& a, int kind) {
 template <int BM, int BN, int WM, int WN, int NST, bool GLU>
 static void f8_tile_launch(anima_ctx* c, const F8Args& a, int precision) {
   constexpr int FN = GLU ? BN / 2 : BN;
-  const dim3 grid((unsigned)((int64_t)((a.N + FN - 1) / FN) * ((a.M + BM - 1) / BM))), block(64 * (BM / WM) * (BN / WN));
+  const dim3 grid((unsigned)((int64_t)((a.N + FN - 1) / FN) * ((a.M + BM - 1) / BM)), (unsigned)((a.KB + a.kbs - 1) / a.kbs)), block(64 * (BM / WM) * (BN / WN));
   if (precision == ANIMA_PREC_FP32) hipLaunchKernelGGL((f8_tile<BM, BN, WM, WN, NST, true, GLU>), grid, block, 0, c->stream, a);
   else hipLaunchKernelGGL((f8_tile<BM, BN, WM, WN, NST, false, GLU>), grid, block, 0, c->stream, a);
 }
 
 // Runs the product of a's rows, quantizing fp32 rows first where the kernel takes e4m3 rows.
 template <bool GLU>
-static int f8_product(anima_ctx* c, F8Args a, int kind, int precision) {
+static int f8_product(anima_ctx* c, F8Args a, int kind, int precision, int splits) {
   static const char* const names[2][F8_COUNT] = {{"gemm.f8.skinny", "gemm.f8.256x256", "gemm.f8.128x128", "gemm.f8.128x64", "gemm.f8.64x64"},
                                                  {"glu.f8.skinny", "glu.f8.256x256", "glu.f8.128x128", "glu.f8.64x256", "glu.f8.64x128"}};
   void* scratch = nullptr;
@@ -1256,6 +1297,23 @@ static int f8_product(anima_ctx* c, F8Args a, int kind, int precision) {
     }
     a.ldx = a.K;
     a.x = nullptr;
+  }
+  const F8Args whole = a;
+  void* part = nullptr;
+  a.kbs = (a.KB + splits - 1) / splits;
+  if (splits > 1) {  // (a linear's tiles) the sums alone, into pooled scratch
+    if (int rc = anima_alloc(c, (size_t)splits * a.M * a.N * 4, &part)) {
+      if (scratch) anima_free(c, scratch);
+      return rc;
+    }
+    a.out = (float*)part;
+    a.ldc = a.N;
+    a.alpha = 1.0f;
+    a.bias = a.add = nullptr;
+    a.act = ANIMA_ACT_NONE;
+    a.epi = ANIMA_EPI_STORE;
+    a.obf = 0;
+    a.vec = a.N % 4 == 0;
   }
   Launch L(c, names[GLU][kind], (GLU ? 4.0 : 2.0) * a.M * a.N * a.K, (double)a.N * a.K * (GLU ? 2 : 1));
   if (kind == F8_SKINNY) {
@@ -1273,7 +1331,16 @@ static int f8_product(anima_ctx* c, F8Args a, int kind, int precision) {
     if constexpr (GLU) f8_tile_launch<64, 128, 32, 64, 3, GLU>(c, a, precision);
     else f8_tile_launch<64, 64, 32, 32, 3, GLU>(c, a, precision);
   }
-  const int rc = L.end();
+  int rc = L.end();
+  if (part) {
+    if (rc == ANIMA_OK) {
+      Launch J(c, "gemm.f8.join", 0.0, (double)a.M * a.N * 4 * (splits + 1));
+      const int64_t quads = (int64_t)a.M * ((a.N + 3) / 4);
+      hipLaunchKernelGGL(f8_join, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, c->stream, whole, (const float*)part, splits);
+      rc = J.end();
+    }
+    anima_free(c, part);
+  }
   if (scratch) anima_free(c, scratch);
   return rc;
 }
@@ -1300,7 +1367,9 @@ int linear_f8_launch(anima_ctx* c, const anima_linear_desc* d) {
   a.obf = d->out_bf16;
   a.vec = a.N % 4 == 0 && a.ldc % 4 == 0 && f8_al(a.out, a.obf ? 8 : 16) && f8_al(a.bias, 16) && (!a.add || (a.ld_add % 4 == 0 && f8_al(a.add, 16))) &&
           (a.epi != ANIMA_EPI_GATED || f8_al(a.gate, 16));
-  return f8_product<false>(c, a, f8_choose(c, false, false, a.M, a.N, a.K, d->precision), d->precision);
+  int splits = 1;
+  const int kind = f8_choose(c, false, false, a.M, a.N, a.K, d->precision, &splits);
+  return f8_product<false>(c, a, kind, d->precision, splits);
 }
 
 int linear_glu_launch(anima_ctx* c, const anima_glu_desc* d) {
@@ -1322,7 +1391,8 @@ int linear_glu_launch(anima_ctx* c, const anima_glu_desc* d) {
   a.out = d->out;
   a.ldc = d->ldc ? d->ldc : a.N;
   void* tmp = nullptr;
-  const int kind = f8_choose(c, true, d->out_q != nullptr, a.M, a.N, a.K, d->precision);
+  int splits = 1;
+  const int kind = f8_choose(c, true, d->out_q != nullptr, a.M, a.N, a.K, d->precision, &splits);
   if (d->out_q && (kind == F8_256 || kind == F8_MID)) {  // a tile is one block of 128 columns
     a.oq = d->out_q;
     a.os = d->out_s;
@@ -1333,7 +1403,7 @@ int linear_glu_launch(anima_ctx* c, const anima_glu_desc* d) {
     a.ldc = a.N;
   }
   a.vec = a.N % 4 == 0 && a.ldc % 4 == 0 && f8_al(a.out, 16);
-  int rc = f8_product<true>(c, a, kind, d->precision);
+  int rc = f8_product<true>(c, a, kind, d->precision, splits);
   if (tmp) {
     if (rc == ANIMA_OK) rc = quant_rows_f8_launch(c, tmp, 0, a.M, a.N, 0, d->out_q, d->out_s);
     anima_free(c, tmp);

@@ -453,7 +453,8 @@ typedef struct {
  * f8: r = alpha * sum_b xs[b][m] scale[n / 128][b] * (sum of xq[m][k] w[n][k] over the 128 k of block b):
  * each block's products summed on the matrix cores (see precision), the blocks added in fp32.  Any M and N;
  * K % 16 == 0, K <= 2^20.  fp32 rows x are quantized as anima_quant_rows_f8 does, few of them inside the
- * product's kernel, more in a pass before it (pooled scratch).  The order in which a result's blocks are
+ * product's kernel, more in a pass before it (pooled scratch); few tiles of a long k are split over k, with the
+ * splits' sums in pooled scratch.  The order in which a result's blocks are
  * added, and so its last bits, depends on the sizes.  No acc_out and no LoRA factors (`add` carries a
  * delta). */
 int anima_linear(anima_ctx* ctx, const anima_linear_desc* desc);

@@ -882,3 +882,44 @@ def test_widest(ctx):
         ctx.linear(W, rows, out.ptr, xq=x, xs=ctx.upload(np.ascontiguousarray(s[:, :rows])), ldx=ld, precision=m.PREC_FP32)
         assert np.all(np.abs(out.numpy() - y[:rows]) <= dy[:rows] + U * np.abs(y[:rows]))
     x.release()
+
+
+@pytest.mark.parametrize("M,N,K", [(100, 1300, 6000), (70, 1301, 8208), (513, 1024, 8192), (64, 4100, 4112)])
+@pytest.mark.parametrize("fast", [True, False])
+def test_linear_split(ctx, M, N, K, fast):
+    """Products whose k loop is split over workgroups: every epilogue, replayed from a graph."""
+    case(f"linear f8 split M={M} N={N} K={K} fast={fast}")
+    m = amd()
+    prec = m.PREC_BF16 if fast else m.PREC_FP32
+    w, scale = f8_weight(N, N, K)
+    bias, gate = randn(91, N).astype(np.float32), randn(92, N).astype(np.float32)
+    add, out0 = randn(93, M * N).reshape(M, N).astype(np.float32), randn(94, M * N).reshape(M, N).astype(np.float32)
+    W = m.weight(m.W_F8, N, K, ctx.upload(w), scale=ctx.upload(scale), bias=ctx.upload(bias))
+    d_gate, d_add = ctx.upload(gate), ctx.upload(add)
+    for kind in ("f8", "f32"):
+        args, x64 = inputs(ctx, M + K, M, K, kind)
+        y, dy = product64(x64, weight64(w, scale), fast)
+        v = 0.75 * y + bias + add
+        dv = 0.75 * dy + 3 * U * (np.abs(0.75 * y) + np.abs(bias) + np.abs(add))
+        a, da = act64(v, "gelu"), act_error(v, "gelu", dv)
+        for epi in (m.EPI_STORE, m.EPI_RESID, m.EPI_GATED):
+            out = Guarded(ctx, (M, N), np.float32, out0)
+            names = ran(ctx, lambda: ctx.linear(W, M, out.ptr, act="gelu", alpha=0.75, epilogue=epi, gate=d_gate, add=d_add, precision=prec, **args))
+            assert "gemm.f8.join" in names, names
+            r, dr = (a * gate, (da + U * np.abs(a)) * np.abs(gate)) if epi == m.EPI_GATED else (a, da)
+            ref = r if epi == m.EPI_STORE else out0 + r
+            assert np.all(np.abs(out.numpy() - ref) <= dr + 2 * U * (np.abs(r) + np.abs(ref)))
+        eager = Guarded(ctx, (M, N), np.uint16)
+        ctx.linear(W, M, eager.ptr, act="gelu", alpha=0.75, add=d_add, out_bf16=True, precision=prec, **args)
+        bits = eager.numpy()
+        gb = torch.from_numpy(bits.view(np.int16)).view(torch.bfloat16).double().numpy()
+        assert np.all(np.abs(gb - a) <= (da + 2 * U * np.abs(a)) * (1 + 2.0 ** -8) + 2.0 ** -8 * np.abs(a))
+        out = Guarded(ctx, (M, N), np.uint16)
+        ctx.graph_begin()
+        ctx.linear(W, M, out.ptr, act="gelu", alpha=0.75, add=d_add, out_bf16=True, precision=prec, **args)
+        g = ctx.graph_end()
+        for _ in range(3):
+            ctx.linear(W, M, eager.ptr, act="gelu", alpha=0.75, add=d_add, out_bf16=True, precision=prec, **args)
+            ctx.graph_launch(g)
+            assert np.array_equal(out.numpy(), bits) and np.array_equal(eager.numpy(), bits)
+        ctx.graph_destroy(g)
