@@ -108,8 +108,9 @@ export function quantizeF8(gpu, W) {
 }
 
 // opts.xq of a linear on W: the row form that W's kind reads (int8 rows and e4m3 rows are both bytes),
-// and e4m3 rows of W's width.  Returns their number.
-function checkRows(W, xq) {
+// and e4m3 rows of W's width.  Their scales lie block by block, [ceil(K / 128), rows], so opts.M, if
+// given, has to be the number of rows: any other M would read other rows' scales.  Returns the number.
+function checkRows(W, xq, want) {
   const f8 = xq.q.dtype === "u8";
   if (f8 !== (W.kind === "f8"))
     throw new Error(`${W.name || "linear"}: ${f8 ? "e4m3" : "int8"} rows for a ${W.kind} weight`);
@@ -117,6 +118,7 @@ function checkRows(W, xq) {
   const [M, K] = xq.q.shape;
   if (K !== W.K || xq.s.size !== Math.ceil(K / 128) * M)
     throw new Error(`${W.name || "linear"}: e4m3 rows [${xq.q.shape}] with ${xq.s.size} scales for K = ${W.K}`);
+  if (want !== undefined && want !== M) throw new Error(`${W.name || "linear"}: M = ${want} for ${M} e4m3 rows`);
   return M;
 }
 
@@ -134,7 +136,7 @@ function weightArg(W) {
 // result (no residual).
 export function linear(gpu, x, W, opts) {
   const o = opts || {};
-  const rows = o.xq ? checkRows(W, o.xq) : 0;
+  const rows = o.xq ? checkRows(W, o.xq, o.M) : 0;
   const M = o.M !== undefined ? o.M : (o.xq ? rows : x.size / W.K);
   // LoRAs: y += sum_i scale_i B_i (A_i x), after the bias and before act / gate (ops.js:55-62).
   // The reference feeds ConvRot layers' LoRAs the rotated input and a rotated A; since
@@ -392,7 +394,7 @@ export function linearGlu(gpu, x, Wg, Wu, opts) {
   for (const W of [Wg, Wu]) {
     if (W.kind !== "f8") throw new Error(`linearGlu: ${W.name || "weight"} is ${W.kind}, expected f8`);
     if (W.lora && W.lora.length) throw new Error(`linearGlu: ${W.name || "weight"} has a LoRA`);
-    if (o.xq) checkRows(W, o.xq);
+    if (o.xq) checkRows(W, o.xq, o.M);
   }
   const M = o.M !== undefined ? o.M : (o.xq ? checkRows(Wg, o.xq) : x.size / Wg.K);
   const rows = o.f8 ? f8Rows(gpu, M, Wg.N) : null;

@@ -113,6 +113,28 @@ def test_refusals():
     assert "unknown norm batch" in got["norm"] and "y of 384" in got["y"]
 
 
+def test_m_of_e4m3_rows():
+    """opts.M beside e4m3 rows: their scales lie [blocks][rows], so a prefix or more rows than there are is refused
+    (the kernels take M as the scales' stride); int8 rows, with one scale each, can be cut."""
+    got = node("import * as ops from './ops.mjs';" + FAKE +
+               "const f8 = { kind: 'f8', N: 32, K: 384, buf: 0, scale: 0, name: 'w' };"
+               "const f8rows = () => ({ q: gpu.empty([8, 384], 'u8'), s: gpu.empty([3, 8]) });"
+               "const i8rows = () => ({ q: gpu.empty([8, 384], 'i8'), s: gpu.empty([8]) });"
+               "const tries = {};"
+               "for (const M of [4, 7, 8, 9, 16, undefined]) {"
+               "  tries['linear ' + M] = msg(() => ops.linear(gpu, null, f8, { M, xq: f8rows() }));"
+               "  tries['glu ' + M] = msg(() => ops.linearGlu(gpu, null, f8, f8, { M, xq: f8rows() }));"
+               "}"
+               "tries.int8 = msg(() => ops.linear(gpu, null, Object.assign({}, f8, { kind: 'i8' }), { M: 4, xq: i8rows() }));"
+               "console.log(JSON.stringify(tries))")
+    for op in ("linear", "glu"):
+        for M in (4, 7, 9, 16):
+            assert f"M = {M} for 8 e4m3 rows" in got[f"{op} {M}"], (op, M)
+        # what passes reaches the library, which has no context here
+        assert got[f"{op} 8"] == got[f"{op} undefined"] == got["int8"]
+    assert "rows" not in got["int8"]
+
+
 def test_checkpoint_and_stacking(tmp_path):
     """SafeTensors.linear on block-scaled e4m3, and concatLinears of whole blocks only."""
     rng = np.random.default_rng(3)
