@@ -402,12 +402,14 @@ export class AnimaDiT {
     });
     const quant = this.blocks.some((b) => ops.needsRotation(b.cross.k));
     const xq = quant ? ops.quantRows(gpu, ctx, CTX_DIM, true) : null;
+    // (the int8 rows for the weights that read them only: a model may mix kinds)
+    const project = (W) => ops.linear(gpu, ctx, W, xq && ops.needsRotation(W) ? { xq, M: B * Lk } : { M: B * Lk });
     // per block: k = RMSNorm(ctx Wk), v = ctx Wv, then converted once to the attention operand
     // layout (bf16 K rows, bf16 V^T) and kept; the fp32 k / v are released
     const kv = this.blocks.map((b) => {
-      const k = ops.linear(gpu, ctx, b.cross.k, xq ? { xq, M: B * Lk } : { M: B * Lk });
+      const k = project(b.cross.k);
       ops.rmsnorm(gpu, k, b.cross.kn, HD, 1e-6, k);
-      const v = ops.linear(gpu, ctx, b.cross.v, xq ? { xq, M: B * Lk } : { M: B * Lk });
+      const v = project(b.cross.v);
       const prep = ops.attentionPrepareKV(gpu, { q: k, k, v, B, Lq: Lk, Lk, H: HEADS, D: HD, ldq: D, ldk: D, ldv: D,
         precision: this.precision });
       releaseAll([k, v]);

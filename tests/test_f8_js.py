@@ -135,6 +135,27 @@ def test_m_of_e4m3_rows():
     assert "rows" not in got["int8"]
 
 
+# the native calls recorded instead of made: [name, arguments], buffers numbered from 1
+RECORD = ("import Module from 'module'; const calls = [];"
+          "Module._extensions['.node'] = (m) => { m.exports = new Proxy({}, { get: (t, k) => (...a) => { calls.push([k, ...a]); return 64; } }); };"
+          "let last = 0; const tensor = (s, d) => ({ buf: ++last, shape: s, dtype: d || 'f32', bytes: 0,"
+          " get size() { return this.shape.reduce((a, b) => a * b, 1); }, at() { return this.buf; }, release() {} });"
+          "const gpu = { ctx: 1, empty: tensor, copy() {} };")
+
+
+def test_context_of_mixed_kinds():
+    """Cross-attention k / v of several kinds in one model: each linear gets the rows that its weight reads."""
+    kinds = [("i8", "i8"), ("f8", "f8"), ("bf16", "bf16"), ("w4", "f8"), ("f8", "i8")]
+    got = node(RECORD + "import('./dit.mjs').then(({ AnimaDiT }) => {"
+               "const W = (kind) => ({ kind, N: 2048, K: 1024, buf: ++last, scale: ++last, name: kind });"
+               f"const m = new AnimaDiT(gpu); m.blocks = {json.dumps(kinds)}.map(([k, v]) => ({{ cross: {{ k: W(k), v: W(v), kn: tensor([128]) }} }}));"
+               "m.prepareContext([tensor([40, 1024]), tensor([40, 1024])]);"
+               "console.log(JSON.stringify(calls.filter((c) => c[0] === 'linear').map((c) => [c[2].kindId, !!c[3].xq, !!c[3].x, c[3].M])));"
+               "})")
+    ids = {"bf16": 0, "i8": 1, "w4": 2, "f8": 5}
+    assert got == [[ids[k], k in ("i8", "w4"), k not in ("i8", "w4"), 80] for pair in kinds for k in pair]
+
+
 def test_checkpoint_and_stacking(tmp_path):
     """SafeTensors.linear on block-scaled e4m3, and concatLinears of whole blocks only."""
     rng = np.random.default_rng(3)
