@@ -238,6 +238,7 @@ struct NormArgs {
   int64_t ldx, ldy, ldh, gate_ld, mod_ld, group_rows;
   float res_scale, eps;
   int rows, cols, layer, y_bf16;
+  uint32_t row0;  // of the launch
 };
 
 // Sum over a wave, in every lane: 16 lanes with DPP, then both halves of 32 and of 64.
@@ -275,7 +276,7 @@ template <int T, int NV, bool EARLY>
 __global__ __launch_bounds__(T, EARLY ? 1 : 4) void residual_norm_kernel(NormArgs a) {
   __shared__ float red[3][T / 64];
   const int t = threadIdx.x;
-  const uint32_t row32 = xcd_remap(blockIdx.x, gridDim.x);
+  const uint32_t row32 = a.row0 + (uint32_t)xcd_remap(blockIdx.x, gridDim.x);
   const int64_t row = row32, grp = a.group_rows >= a.rows ? 0 : row32 / (uint32_t)a.group_rows;
   const float inv = 1.0f / (float)a.cols;
   // every access through a resource of the row's bytes: past its end loads give zeros and stores nothing (the whole
@@ -1091,11 +1092,11 @@ int quant_rows_f8_launch(anima_ctx* c, const void* x, int x_bf16, int64_t M, int
   if (int rc = check_quant_rows_f8(x, x_bf16, M, K, ldx, q, s, F8Msg{msg, sizeof msg})) return refused(c, rc, msg);
   if (M == 0) return ANIMA_OK;
   OnDevice on(c);
-  const int KB = (K + 127) / 128;
+  const int KB = (K - 1) / 128 + 1;
   const int64_t ld = ldx ? ldx : K;
   const DivBy div = div_by((uint32_t)KB);
   Launch L(c, x_bf16 ? "quant.f8.bf16" : "quant.f8", 0.0, (double)M * K * (x_bf16 ? 3 : 5));
-  const int64_t part = (1 << 30) / KB;  // rows of a launch: their blocks are counted in 31 bits
+  const int64_t part = f8_quant_part(K);
   for (int64_t m = 0; m < M; m += part) {
     const uint32_t blocks = (uint32_t)((M - m < part ? M - m : part) * KB);
     const bool many = blocks >= 65536;  // (two blocks in flight per thread once the workgroups fill the chip)
@@ -1119,9 +1120,8 @@ int weight_quant_f8_launch(anima_ctx* c, const void* w, int w_bf16, int N, int K
   char msg[256];
   if (int rc = check_weight_quant_f8(w, w_bf16, N, K, q, scale, F8Msg{msg, sizeof msg})) return refused(c, rc, msg);
   OnDevice on(c);
-  const int KB = (K + 127) / 128;
-  const int64_t blocks = (int64_t)((N + 127) / 128) * KB;
-  if (blocks > 0x7fffffff) return fail(c, ANIMA_E_UNSUPPORTED, "anima_weight_quant_f8: %lld blocks", (long long)blocks);
+  const int KB = (K - 1) / 128 + 1;
+  const int64_t blocks = (int64_t)((N - 1) / 128 + 1) * KB;
   Launch L(c, "weight_quant.f8", 0.0, (double)N * K * (w_bf16 ? 3 : 5));
   if (w_bf16)
     hipLaunchKernelGGL(weight_quant_f8_kernel<uint16_t>, dim3((unsigned)blocks), dim3(256), 0, c->stream, (const uint16_t*)w, N, K, KB, q,
@@ -1138,47 +1138,52 @@ int residual_norm_launch(anima_ctx* c, const anima_resnorm_desc* d) {
   OnDevice on(c);
   const int64_t C = d->cols;
   const auto ld = [&](int64_t v) { return v ? v : C; };
-  const NormArgs a{d->x,
-                   d->y,
-                   d->post_w,
-                   d->gate,
-                   d->norm_w,
-                   d->shift,
-                   d->scale,
-                   d->h,
-                   d->q,
-                   d->s,
-                   ld(d->ldx),
-                   ld(d->ldy),
-                   ld(d->ldh),
-                   ld(d->gate_ld),
-                   ld(d->mod_ld),
-                   d->group_rows ? d->group_rows : d->rows,
-                   d->res_scale != 0.0f ? d->res_scale : 1.0f,
-                   d->eps,
-                   (int)d->rows,
-                   d->cols,
-                   d->norm == ANIMA_NORM_LAYER,
-                   d->y_bf16};
-  const dim3 grid((unsigned)d->rows);
+  NormArgs a{d->x,
+             d->y,
+             d->post_w,
+             d->gate,
+             d->norm_w,
+             d->shift,
+             d->scale,
+             d->h,
+             d->q,
+             d->s,
+             ld(d->ldx),
+             ld(d->ldy),
+             ld(d->ldh),
+             ld(d->gate_ld),
+             ld(d->mod_ld),
+             d->group_rows ? d->group_rows : d->rows,
+             d->res_scale != 0.0f ? d->res_scale : 1.0f,
+             d->eps,
+             (int)d->rows,
+             d->cols,
+             d->norm == ANIMA_NORM_LAYER,
+             d->y_bf16,
+             0};
   Launch L(c, "residual_norm", 0.0, (double)d->rows * C * ((d->y ? d->y_bf16 ? 10.0 : 12.0 : 4.0) + (d->h ? 4 : 0) + (d->q ? 1 : 0)));
-#define RN(T, NV, EARLY) hipLaunchKernelGGL((residual_norm_kernel<T, NV, EARLY>), grid, dim3(T), 0, c->stream, a)
+#define RN(T, NV, EARLY)                                                                                                     \
+  for (int64_t r = 0, part = f8_norm_part(T); r < d->rows; r += part) {                                                      \
+    a.row0 = (uint32_t)r;                                                                                                    \
+    hipLaunchKernelGGL((residual_norm_kernel<T, NV, EARLY>), dim3((unsigned)(d->rows - r < part ? d->rows - r : part)), dim3(T), 0, \
+                       c->stream, a);                                                                                        \
+  }
   if (d->rows <= 4 * c->num_cus) {
-    if (C <= 256) RN(64, 1, true);
-    else if (C <= 512) RN(128, 1, true);
-    else if (C <= 1024) RN(256, 1, true);
-    else if (C <= 2048) RN(256, 2, true);
-    else if (C <= 4096) RN(512, 2, true);
-    else if (C <= 8192) RN(1024, 2, true);
-    else RN(1024, 4, true);
+    if (C <= 256) RN(64, 1, true)
+    else if (C <= 512) RN(128, 1, true)
+    else if (C <= 1024) RN(256, 1, true)
+    else if (C <= 2048) RN(256, 2, true)
+    else if (C <= 4096) RN(512, 2, true)
+    else if (C <= 8192) RN(1024, 2, true)
+    else RN(1024, 4, true)
   } else {
-    if (C <= 256) RN(64, 1, false);
-    else if (C <= 512) RN(64, 2, false);
-    else if (C <= 1024) RN(64, 4, false);
-    else if (C <= 2048) RN(64, 8, false);
-    else if (C <= 4096) RN(128, 8, false);
-    else if (C <= 8192) RN(256, 8, false);
-    else RN(512, 8, false);
+    if (C <= 256) RN(64, 1, false)
+    else if (C <= 512) RN(64, 2, false)
+    else if (C <= 1024) RN(64, 4, false)
+    else if (C <= 2048) RN(64, 8, false)
+    else if (C <= 4096) RN(128, 8, false)
+    else if (C <= 8192) RN(256, 8, false)
+    else RN(512, 8, false)
   }
 #undef RN
   return L.end();
@@ -1229,9 +1234,10 @@ static int f8_choose(anima_ctx* c, bool glu, bool f8_out, int64_t M, int64_t N, 
   int best = F8_256, sbest = F8_256, sn = 1;
   float bt = 0.0f, st = 0.0f;  // of the best kernel, of the best one with its k loop split
   for (int k = F8_COUNT - 1; k >= 0; k--) {
-    if (k == F8_SKINNY && M > 16 * 65535) continue;  // (the grid's second dimension)
     const int64_t tiles = f8_tiles(k, glu, M, N);
-    if (tiles > 0x7fffffff) continue;
+    // the grid's second dimension, and its threads (512 a tile at the most); 256 x 256 tiles have room for every product
+    // whose output finds memory
+    if (k == F8_SKINNY ? M > 16 * 65535 || (N + 15) / 16 * 64 * SKW > F8_MAX_THREADS : tiles > F8_MAX_THREADS / 512) continue;
     const Fit& f = fit[glu][precision][k];
     const float rounds = (float)((tiles + c->num_cus - 1) / c->num_cus), mn = 1e-6f * (float)M * (float)N;
     const bool fused = k == F8_256 || k == F8_MID;

@@ -13,6 +13,15 @@ namespace anima {
 constexpr int F8_MAX_K = 1 << 20;         // of a product: 256 rows of a tile stay below 2^31 bytes
 constexpr int64_t F8_MAX_LDX = 1 << 22;   // bytes between e4m3 rows of a product's input, likewise
 constexpr int F8_NORM_MAX_COLS = 16384;   // a row in one workgroup's registers
+constexpr int F8_MAX_SIDE = 1 << 30;      // rows and outputs of a product: 256 x 256 tiles of either stay below 2^32 threads
+
+// A launch has fewer than 2^32 threads a dimension, so large calls are cut into several.
+constexpr int64_t F8_MAX_THREADS = 0xffffffff;
+// Rows of a launch of quant_rows_f8_kernel: up to 16 threads to a block of 128 columns, 2^27 blocks (which are counted
+// in 31 bits).
+inline int64_t f8_quant_part(int K) { return ((int64_t)1 << 27) / ((K - 1) / 128 + 1); }
+// Rows of a launch of residual_norm_kernel, whose workgroups of `threads` take one each.
+constexpr int64_t f8_norm_part(int threads) { return ((int64_t)1 << 31) / threads; }
 
 struct F8Msg {
   char* buf;
@@ -48,14 +57,18 @@ inline int check_weight_quant_f8(const void* w, int w_bf16, int N, int K, const 
   if (w_bf16 != 0 && w_bf16 != 1) return fail(ANIMA_E_ARG, "anima_weight_quant_f8: w_bf16=%d", w_bf16);
   if (!w || !q || !scale) return fail(ANIMA_E_ARG, "anima_weight_quant_f8: null pointer");
   if (!f8_al(w, 16) || !f8_al(q, 16) || !f8_al(scale, 4)) return fail(ANIMA_E_ARG, "anima_weight_quant_f8: w and q on 16 bytes");
+  if ((int64_t)((N - 1) / 128 + 1) * ((K - 1) / 128 + 1) > F8_MAX_THREADS / 256)
+    return fail(ANIMA_E_UNSUPPORTED, "anima_weight_quant_f8: N=%d K=%d, 2^24 blocks and more", N, K);
   return ANIMA_OK;
 }
 
 // The weight and the input rows of a product: e4m3 rows xq, else fp32 rows x.
-inline int check_f8_operands(const char* who, const anima_weight* W, const float* x, int64_t ldx, const void* xq, const float* xs,
+inline int check_f8_operands(const char* who, const anima_weight* W, int64_t M, const float* x, int64_t ldx, const void* xq, const float* xs,
                              F8Msg fail) {
   if (W->N < 1 || W->K < 1 || W->K % 16 || W->K > F8_MAX_K)
     return fail(ANIMA_E_ARG, "%s: an f8 weight needs K %% 16 == 0 and K <= %d (N=%d K=%d)", who, F8_MAX_K, W->N, W->K);
+  if (M > F8_MAX_SIDE || W->N > F8_MAX_SIDE)
+    return fail(ANIMA_E_UNSUPPORTED, "%s: M=%lld N=%d, more than %d rows or outputs", who, (long long)M, W->N, F8_MAX_SIDE);
   if (!W->w || !W->scale) return fail(ANIMA_E_ARG, "%s: an f8 weight needs its data and block scales", who);
   if (!f8_al(W->w, 16) || !f8_al(W->scale, 4) || !f8_al(W->bias, 4))
     return fail(ANIMA_E_ARG, "%s: the f8 weight's data on 16 bytes, its scales and bias on 4", who);
@@ -82,7 +95,7 @@ inline int check_linear_f8(const anima_linear_desc* d, F8Msg fail) {
     return fail(ANIMA_E_UNSUPPORTED, "anima_linear: bf16 rows with the store epilogue only (%d)", d->epilogue);
   if (!f8_al(d->out, d->out_bf16 ? 2 : 4) || !f8_al(d->gate, 4) || !f8_al(d->add, 4))
     return fail(ANIMA_E_ARG, "anima_linear: out, gate or add off its element size");
-  return check_f8_operands("anima_linear", d->W, d->x, d->ldx, d->xq, d->xs, fail);
+  return check_f8_operands("anima_linear", d->W, d->M, d->x, d->ldx, d->xq, d->xs, fail);
 }
 
 inline int check_linear_glu(const anima_glu_desc* d, F8Msg fail) {
@@ -98,8 +111,8 @@ inline int check_linear_glu(const anima_glu_desc* d, F8Msg fail) {
   if (d->precision != ANIMA_PREC_BF16 && d->precision != ANIMA_PREC_FP32)
     return fail(ANIMA_E_ARG, "anima_linear_glu: unknown precision %d", d->precision);
   if (d->M == 0) return ANIMA_OK;
-  int rc = check_f8_operands("anima_linear_glu", G, d->x, d->ldx, d->xq, d->xs, fail);
-  if (rc == ANIMA_OK) rc = check_f8_operands("anima_linear_glu", U, d->x, d->ldx, d->xq, d->xs, fail);
+  int rc = check_f8_operands("anima_linear_glu", G, d->M, d->x, d->ldx, d->xq, d->xs, fail);
+  if (rc == ANIMA_OK) rc = check_f8_operands("anima_linear_glu", U, d->M, d->x, d->ldx, d->xq, d->xs, fail);
   if (rc != ANIMA_OK) return rc;
   if (d->out_q) {
     if (d->out) return fail(ANIMA_E_ARG, "anima_linear_glu: fp32 rows or e4m3 rows, not both");
