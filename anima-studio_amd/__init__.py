@@ -209,7 +209,7 @@ def lib():
                                              _i64, ctypes.c_float, ctypes.c_int]
         L.anima_patchify.argtypes = [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp]
         L.anima_unpatchify.argtypes = [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp]
-        L.anima_linear.argtypes = [_vp, _vp]  # (packed descriptors: bytes)
+        L.anima_linear.argtypes = [_vp, P(LinearDesc)]
         L.anima_weight_unpack_w4.argtypes = [_vp, ctypes.POINTER(Weight), _vp]
         L.anima_sampler_step.argtypes = [_vp, ctypes.POINTER(SamplerDesc)]
         L.anima_split3_bf16.argtypes = [_vp, _vp, _vp, _i64]
@@ -221,8 +221,12 @@ def lib():
         L.anima_fill_random.argtypes = [_vp, _vp, _i64, ctypes.c_int, ctypes.c_uint64, ctypes.c_float, ctypes.c_float]
         L.anima_quant_rows_f8.argtypes = [_vp, _vp, ctypes.c_int, _i64, ctypes.c_int, _i64, _vp, _vp]
         L.anima_weight_quant_f8.argtypes = [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp]
-        L.anima_linear_glu.argtypes = [_vp, _vp]
-        L.anima_residual_norm.argtypes = [_vp, _vp]
+        L.anima_linear_glu.argtypes = [_vp, P(GluDesc)]
+        L.anima_residual_norm.argtypes = [_vp, P(ResNormDesc)]
+        for n in ("anima_linear", "anima_linear_glu", "anima_residual_norm"):  # with a packed descriptor (bytes)
+            packed = L[n]
+            packed.argtypes = [_vp, _vp]
+            setattr(L, n + "_packed", packed)
         L.anima_graph_begin.argtypes = [_vp]
         L.anima_graph_end.argtypes = [_vp, P(_vp)]
         L.anima_graph_launch.argtypes = [_vp, _vp]
@@ -480,12 +484,12 @@ class Context:
         lora_cols > 0: block-diagonal ranks, column n reading xa columns (n // lora_cols) * lora_r
         + k.  f8 weights: precision (PREC_FP32: sums in 32 bits), out_bf16 (bf16 rows out)."""
         # (absent pointers without a call: half a microsecond of every linear)
-        d = _linear_desc(M, ctypes.addressof(W), x and _adr(x) or 0, ldx, x_rotated, xq and _adr(xq) or 0,
+        d = _linear_desc(M, _weight_adr(W), x and _adr(x) or 0, ldx, int(x_rotated), xq and _adr(xq) or 0,
                          xs and _adr(xs) or 0, _adr(out), ldc, alpha, ACT[act] if isinstance(act, str) else act, epilogue,
                          gate and _adr(gate) or 0, gate_off, acc_out and _adr(acc_out) or 0, add and _adr(add) or 0, ld_add,
                          lora_xa and _adr(lora_xa) or 0, ld_lora_xa, lora_b and _adr(lora_b) or 0, lora_r, lora_cols,
-                         precision, out_bf16)
-        return self._check(lib().anima_linear(self.h, d))
+                         precision, int(out_bf16))
+        return self._check(lib().anima_linear_packed(self.h, d))
 
     def linear_qkv(self, W, M, out, *, B, L, H, k_norm=None, rope_cs=None, rope_sin_off=0, kv_prep=None, eps=1e-6,
                    x=None, ldx=0, x_rotated=True, xq=None, xs=None, ldc=0, alpha=0.0, lora_xa=None, ld_lora_xa=0,
@@ -520,10 +524,10 @@ class Context:
                    out_s=None, precision=PREC_BF16):
         """anima_linear_glu: act(x W_gate^T) * (x W_up^T) of two W_F8 weights, from fp32 rows x or e4m3 rows
         xq, xs, into fp32 rows out or e4m3 rows out_q, out_s."""
-        d = _glu_desc(M, ctypes.addressof(gate), ctypes.addressof(up), x and _adr(x) or 0, xq and _adr(xq) or 0,
+        d = _glu_desc(M, _weight_adr(gate), _weight_adr(up), x and _adr(x) or 0, xq and _adr(xq) or 0,
                       xs and _adr(xs) or 0, ldx, ACT[act] if isinstance(act, str) else act, out and _adr(out) or 0, ldc,
                       out_q and _adr(out_q) or 0, out_s and _adr(out_s) or 0, precision)
-        return self._check(lib().anima_linear_glu(self.h, d))
+        return self._check(lib().anima_linear_glu_packed(self.h, d))
 
     def residual_norm(self, rows, cols, x, *, ldx=0, y=None, ldy=0, y_bf16=False, post_w=None, gate=None, gate_ld=0, res_scale=0.0,
                       norm="rms", norm_w=None, shift=None, scale=None, mod_ld=0, group_rows=0, eps=1e-6, h=None, ldh=0,
@@ -533,8 +537,8 @@ class Context:
         d = _resnorm_desc(rows, cols, _adr(x), ldx, y and _adr(y) or 0, ldy, post_w and _adr(post_w) or 0,
                           gate and _adr(gate) or 0, gate_ld, res_scale, NORM[norm] if isinstance(norm, str) else norm,
                           norm_w and _adr(norm_w) or 0, shift and _adr(shift) or 0, scale and _adr(scale) or 0, mod_ld,
-                          group_rows, eps, h and _adr(h) or 0, ldh, q and _adr(q) or 0, s and _adr(s) or 0, y_bf16)
-        return self._check(lib().anima_residual_norm(self.h, d))
+                          group_rows, eps, h and _adr(h) or 0, ldh, q and _adr(q) or 0, s and _adr(s) or 0, int(y_bf16))
+        return self._check(lib().anima_residual_norm_packed(self.h, d))
 
     def split3_bf16(self, src, dst, n):
         return self._check(lib().anima_split3_bf16(self.h, _ptr(src), _ptr(dst), n))
@@ -591,7 +595,13 @@ def dit_rope_table(Hp: int, Wp: int) -> np.ndarray:
 
 
 def _adr(b):
-    return b if type(b) is int else 0 if b is None else b.ptr if isinstance(b, DeviceBuffer) else int(b)
+    return b if type(b) is int else 0 if b is None else b.ptr or 0 if isinstance(b, DeviceBuffer) else int(b)
+
+
+def _weight_adr(W):
+    if not isinstance(W, Weight):
+        raise TypeError(f"expected a Weight (weight()), got {type(W).__name__}")
+    return ctypes.addressof(W)
 
 
 def _ptr(b):
