@@ -147,6 +147,9 @@ inline int check_residual_norm(const anima_resnorm_desc* d, F8Msg fail) {
                 ldg = d->gate_ld ? d->gate_ld : C;
   if (ldx < C || ldx % 4 || ldy < C || ldy % 4 || ldh < C || ldh % 4 || ldm < C || ldm % 4 || ldg < C || ldg % 4)
     return fail(ANIMA_E_ARG, "anima_residual_norm: row strides of at least cols=%d, multiples of 4", d->cols);
+  // (a row's h is written when its own y has been read, other rows' y not yet)
+  if (d->h && (const void*)d->h == d->y && (d->y_bf16 || (d->rows > 1 && ldh != ldy)))
+    return fail(ANIMA_E_ARG, "anima_residual_norm: h may be an fp32 y of its own stride (ldh=%lld ldy=%lld)", (long long)ldh, (long long)ldy);
   if (!f8_al(d->y, d->y_bf16 ? 8 : 16)) return fail(ANIMA_E_ARG, "anima_residual_norm: rows of y on four elements");
   if (!f8_al(d->s, 4)) return fail(ANIMA_E_ARG, "anima_residual_norm: s off 4 bytes");
   const void* const p[] = {d->x, d->post_w, d->gate, d->norm_w, d->shift, d->scale, d->h, d->q};

@@ -563,7 +563,7 @@ int anima_linear_glu(anima_ctx* ctx, const anima_glu_desc* desc);
  * e4m3 rows q, s (as anima_quant_rows_f8 of those fp32 rows: the same values).  In the reference these are
  * the residual epilogues of ops.linear, ops.rmsnorm and ops.layernormMod (app/gpu/ops.js:48-66, 111-137).
  * cols % 4 == 0 (q: % 16), cols <= 16384; rows and vectors 16-byte aligned (bf16 y: 8), strides multiples of 4.
- * h may be an fp32 y; other outputs overlap no input. */
+ * h may be an fp32 y (the same rows: ldh == ldy); other outputs overlap no input. */
 #define ANIMA_NORM_RMS 0
 #define ANIMA_NORM_LAYER 1
 typedef struct {

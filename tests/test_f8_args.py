@@ -128,6 +128,17 @@ def test_residual_norm(checks, change, code):
     assert rc == code and (code == 0 or "anima_residual_norm" in msg)
 
 
+@pytest.mark.parametrize("change,code", [
+    ({}, 0), ({"ldy": 80, "ldh": 80}, 0), ({"ldy": 64}, 0), ({"ldh": 80}, -1), ({"ldy": 80}, -1), ({"y_bf16": 1}, -1),
+    ({"rows": 1, "ldy": 80}, 0), ({"h": 0, "ldh": 80, "q": P, "s": P}, 0), ({"y": P + 64, "ldy": 80}, 0)])
+def test_residual_norm_in_place(checks, change, code):
+    """h may be y: the same fp32 rows; with other strides a row's h would be another row's y."""
+    m = amd()
+    d = m.ResNormDesc(**dict(dict(rows=3, cols=64, x=2 * P, y=P, norm=0, eps=1e-6, h=P), **change))
+    rc, msg = call(checks.t_norm, ctypes.byref(d))
+    assert rc == code and (code == 0 or "h may be" in msg)
+
+
 def test_residual_norm_null(checks):
     assert call(checks.t_norm, v(0))[0] == -1
 
