@@ -111,6 +111,7 @@ export function quantizeF8(gpu, W) {
 // and e4m3 rows of W's width.  Their scales lie block by block, [ceil(K / 128), rows], so opts.M, if
 // given, has to be the number of rows: any other M would read other rows' scales.  Returns the number.
 function checkRows(W, xq, want) {
+  if (!xq.q || !xq.s) throw new Error(`${W.name || "linear"}: opts.xq without rows q and scales s (residualNorm gives them with f8)`);
   const f8 = xq.q.dtype === "u8";
   if (f8 !== (W.kind === "f8"))
     throw new Error(`${W.name || "linear"}: ${f8 ? "e4m3" : "int8"} rows for a ${W.kind} weight`);
@@ -407,19 +408,30 @@ export function linearGlu(gpu, x, Wg, Wu, opts) {
 
 // The seam between two blocks in one pass over x [rows, cols]: x += resScale * gate * post(y) in place
 // (opts.y, f32 or bf16; optional), then h = norm(x) * weight * (1 + scale) + shift.
-// opts: postWeight (RMSNorm of y first), gate + gOff, resScale, norm ("rms" | "layer"), weight,
+// opts: postWeight (RMSNorm of y first), gate + gOff, resScale (0: 1), norm ("rms" | "layer"), weight,
 // mod + shiftOff + scaleOff, eps; opts.h: fp32 rows (default when f8 is not set), opts.f8: e4m3 rows.
+// opts.groupRows: row r takes the gate and modulation of group r / groupRows, whose vectors lie
+// gateLd and modLd values apart (cols by default), e.g. one group per image of a batch.
 // Returns { h, q, s, release }: an { q, s } of linear / linearGlu when f8.
 export function residualNorm(gpu, x, cols, opts) {
   const o = opts || {};
   if (o.norm !== undefined && !(o.norm in NORM)) throw new Error(`residualNorm: unknown norm ${o.norm}`);
   const rows = x.size / cols;
   if (o.y && o.y.size !== x.size) throw new Error(`residualNorm: y of ${o.y.size} values for x of ${x.size}`);
+  const groups = o.groupRows ? Math.ceil(rows / o.groupRows) : 1;
+  const vectors = (name, t, off, ld) => {
+    const end = (off || 0) + (groups - 1) * (ld || cols) + cols;
+    if (t && t.size < end) throw new Error(`residualNorm: ${name} of ${t.size} values, ${end} for ${groups} groups`);
+  };
+  vectors("gate", o.gate, o.gOff, o.gateLd);
+  vectors("mod", o.mod, o.shiftOff, o.modLd);
+  vectors("mod", o.mod, o.scaleOff, o.modLd);
   const r = o.f8 ? f8Rows(gpu, rows, cols) : null;
   const h = o.h || !r ? gpu.empty([rows, cols]) : null;
   const at = (t, off) => (t ? ptr(t) + 4 * (off || 0) : 0);
   native.residualNorm(gpu.ctx, { rows, cols, x: x.buf, y: ptr(o.y), yBf16: o.y && o.y.dtype === "bf16" ? 1 : 0,
-    postW: ptr(o.postWeight), gate: at(o.gate, o.gOff), resScale: o.resScale || 0, norm: NORM[o.norm || "rms"],
+    postW: ptr(o.postWeight), gate: at(o.gate, o.gOff), gateLd: o.gateLd || 0, groupRows: o.groupRows || 0,
+    modLd: o.modLd || 0, resScale: o.resScale || 0, norm: NORM[o.norm || "rms"],
     normW: ptr(o.weight), shift: at(o.mod, o.shiftOff), scale: at(o.mod, o.scaleOff),
     eps: o.eps === undefined ? 1e-6 : o.eps, h: ptr(h), q: r ? r.q.buf : 0, s: r ? r.s.buf : 0 });
   return { h, q: r ? r.q : null, s: r ? r.s : null, release() { for (const t of [h, r]) if (t) t.release(); } };

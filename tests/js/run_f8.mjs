@@ -5,6 +5,7 @@
 // Cases:
 //   block   residualNorm -> linear -> quantRowsF8 -> linear (bf16) -> residualNorm -> linearGlu ->
 //           linear, on bf16 weights converted by quantizeF8 or on an e4m3 safetensors file
+//   groups  residualNorm of rows in groups with gates and modulations of their own, and of each group by itself
 //   qwen3   Qwen3.encode of a synthetic text encoder after quantizeF8 (both precisions; recorded,
 //           replayed and eager) and its weights; an encoding with a LoRA of zeros attached
 //   dit     a synthetic DiT's velocities: bf16 weights, after quantizeF8, and with LoRAs of zeros; graph replays
@@ -66,6 +67,21 @@ async function block(gpu, c) {
   }
   if (both) out.both = await gpu.read(both);
   for (const k of Object.keys(out)) save(`${c.out}.${k}`, out[k]);
+}
+
+async function groups(gpu, c) {
+  const { M, C, per, ld } = c;
+  const gate = gpu.upload(load(c.gate)), mod = gpu.upload(load(c.mod)), y = gpu.fromArray(load(c.y), [M, C]);
+  const run = async (tag, x, opts) => {
+    const r = ops.residualNorm(gpu, x, C, Object.assign({ gate, mod, norm: "layer", h: true, f8: true }, opts));
+    for (const [n, t] of [["x", x], ["h", r.h], ["q", r.q], ["s", r.s]]) save(`${c.out}.${tag}.${n}`, await gpu.read(t));
+  };
+  await run("all", gpu.fromArray(load(c.x), [M, C]), { y, groupRows: per, gateLd: ld, modLd: 2 * ld, gOff: 4, shiftOff: 0, scaleOff: ld });
+  const x = gpu.fromArray(load(c.x), [M, C]);
+  for (let g = 0, m = 0; m < M; g++, m += per) {
+    const n = Math.min(per, M - m);
+    await run(g, x.view(m * C, [n, C]), { y: y.view(m * C, [n, C]), gOff: g * ld + 4, shiftOff: 2 * g * ld, scaleOff: 2 * g * ld + ld });
+  }
 }
 
 // the encoder's layers in fp32 precision, op by op on fp32 rows
@@ -154,7 +170,7 @@ async function dit(gpu, c) {
 const c = JSON.parse(fs.readFileSync(process.argv[2], "utf8"));
 GPU.create({})
   .then(async (gpu) => {
-    await { block, qwen3, dit }[c.case](gpu, c);
+    await { block, groups, qwen3, dit }[c.case](gpu, c);
     gpu.destroy();
   })
   .catch((e) => {

@@ -80,6 +80,7 @@ def test_exports():
 FAKE = ("const gpu = { ctx: null, empty: (s, d) => ({ buf: 0, shape: s, dtype: d || 'f32', size: s.reduce((a, b) => a * b, 1), "
         "release() {} }), upload: (a) => ({ buf: 0, data: Array.from(a), release() {} }), copy() {} };"
         "const msg = (f) => { try { f(); return ''; } catch (e) { return e.message; } };")
+MSG = "const msg = (f) => { try { f(); return ''; } catch (e) { return e.message; } };"
 
 
 def test_refusals():
@@ -141,6 +142,29 @@ RECORD = ("import Module from 'module'; const calls = [];"
           "let last = 0; const tensor = (s, d) => ({ buf: ++last, shape: s, dtype: d || 'f32', bytes: 0,"
           " get size() { return this.shape.reduce((a, b) => a * b, 1); }, at() { return this.buf; }, release() {} });"
           "const gpu = { ctx: 1, empty: tensor, copy() {} };")
+
+
+def test_residual_norm_groups():
+    """groupRows, gateLd and modLd reach the library; vectors too short for the groups, and a result without e4m3 rows
+    in a linear's place, are refused."""
+    got = node(RECORD + MSG + "import('./ops.mjs').then((ops) => {"
+               "const x = tensor([6, 128]), norm = (o) => ops.residualNorm(gpu, x, 128, o);"
+               "norm({ gate: tensor([3, 128]), gOff: 0, mod: tensor([3, 256]), scaleOff: 128, groupRows: 2, modLd: 256 });"
+               "norm({ gate: tensor([1152]), gOff: 512, gateLd: 256, groupRows: 2 });"
+               "norm({ gate: tensor([128]) });"
+               "const none = norm({});"
+               "const d = calls.filter((c) => c[0] === 'residualNorm').map((c) => [c[2].groupRows, c[2].gateLd, c[2].modLd]);"
+               "console.log(JSON.stringify({ d,"
+               " gate: msg(() => norm({ gate: tensor([2, 128]), groupRows: 2 })),"
+               " off: msg(() => norm({ gate: tensor([3, 128]), gOff: 4, groupRows: 2 })),"
+               " mod: msg(() => norm({ mod: tensor([3, 256]), scaleOff: 128, groupRows: 2, modLd: 260 })),"
+               " one: msg(() => norm({ gate: tensor([100]) })),"
+               " rows: msg(() => ops.linear(gpu, null, { kind: 'f8', N: 32, K: 128, name: 'w' }, { xq: none })),"
+               " glu: msg(() => ops.linearGlu(gpu, null, { kind: 'f8', N: 32, K: 128 }, { kind: 'f8', N: 32, K: 128 }, { xq: none })) })); })")
+    assert got["d"] == [[2, 0, 256], [2, 256, 0], [0, 0, 0], [0, 0, 0]]
+    assert "gate of 256 values, 384 for 3 groups" in got["gate"] and "gate of 384 values, 388" in got["off"]
+    assert "mod of 768 values, 776" in got["mod"] and "gate of 100 values, 128" in got["one"]
+    assert "without rows q and scales s" in got["rows"] and "without rows q and scales s" in got["glu"]
 
 
 def test_context_of_mixed_kinds():
@@ -262,6 +286,28 @@ def test_js_block(tmp_path, file):
     d, dd = ref.product64(rows("g", F), W["down"], False)
     gate = mod[2 * C:].astype(np.float64)
     check("x", get("x").reshape(M, C), g1 + gate * d, np.abs(gate) * dd + 3 * ref.U * (np.abs(g1) + np.abs(gate * d)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,per", [(20, 10), (21, 8)])
+def test_js_groups(tmp_path, M, per):
+    """Rows in groups (the last one short) with gates and modulations of their own: the same bits as each group alone."""
+    C, ld, out = 272, 288, str(tmp_path / "g")
+    rng = np.random.default_rng(M)
+    n = -(-M // per)
+    spec = {"case": "groups", "M": M, "C": C, "per": per, "ld": ld, "out": out}
+    for k, size in (("x", M * C), ("y", M * C), ("gate", n * ld), ("mod", 2 * n * ld)):
+        spec[k] = write(tmp_path, k, rng.normal(size=size).astype(np.float32))
+    run_case(tmp_path, spec)
+
+    def get(tag, name, dtype=np.float32):
+        return np.fromfile(f"{out}.{tag}.{name}", dtype)
+
+    for name, dtype, rows in (("x", np.float32, True), ("h", np.float32, True), ("q", np.uint8, True), ("s", np.float32, False)):
+        whole = get("all", name, dtype)
+        parts = [get(g, name, dtype).reshape(min(per, M - g * per), C) if rows else
+                 get(g, name, dtype).reshape(-1, min(per, M - g * per)) for g in range(n)]
+        assert np.array_equal(whole.reshape(M, C) if rows else whole.reshape(-1, M), np.concatenate(parts, 0 if rows else 1)), name
 
 
 def encode_ref(W, ids, layers):
