@@ -8,6 +8,7 @@
 //   groups  residualNorm of rows in groups with gates and modulations of their own, and of each group by itself
 //   qwen3   Qwen3.encode of a synthetic text encoder after quantizeF8 (both precisions; recorded,
 //           replayed and eager) and its weights; an encoding with a LoRA of zeros attached
+//   ditsteps  a synthetic DiT's residual stream after each block, and after the e4m3 blocks op by op
 //   dit     a synthetic DiT's velocities: bf16 weights, after quantizeF8, and with LoRAs of zeros; graph replays
 
 import fs from "fs";
@@ -167,10 +168,59 @@ async function dit(gpu, c) {
   await forward("f8lora");
 }
 
+// A DiT block on e4m3 weights op by op: fp32 rows between the ops (bf16 rows widened on the host), which each product
+// quantizes itself.  x: [B * L, 2048], updated in place.
+async function blockSteps(gpu, model, i, x, cond, tc, B, L, cs) {
+  const D = 2048, H = 16, HD = 128, M = B * L, precision = model.precision;
+  const b = model.blocks[i], m = tc.blocks[i];
+  const wide = async (t) => {
+    if (t.dtype !== "bf16") return t;
+    const u = await gpu.read(t), f = new Float32Array(u.length), bits = new Uint32Array(f.buffer);
+    u.forEach((v, j) => { bits[j] = v * 65536; });
+    return gpu.fromArray(f, t.shape);
+  };
+  const norm = (mod) => ops.residualNorm(gpu, x, D, { norm: "layer", mod, shiftOff: 0, scaleOff: D }).h;
+  const into = (y, W, mod) => ops.linear(gpu, y, W, { M, out: x, resid: true, gate: mod, gOff: 2 * D, precision });
+  const qkv = ops.linear(gpu, norm(m.self), b.self.qkv, { precision });
+  const a = ops.attention(gpu, { q: qkv, k: qkv, v: qkv, B, Lq: L, Lk: L, H, D: HD, ldq: 3 * D, ldk: 3 * D, ldv: 3 * D, qOff: 0,
+    kOff: D, vOff: 2 * D, qNorm: b.self.qn, kNorm: b.self.kn, cs, precision, oBf16: precision === "bf16" });
+  into(await wide(a), b.self.o, m.self);
+  const q = ops.linear(gpu, norm(m.cross), b.cross.q, { precision });
+  const k = ops.linear(gpu, cond.ctx, b.cross.k, {}), v = ops.linear(gpu, cond.ctx, b.cross.v, {});
+  ops.rmsnorm(gpu, k, b.cross.kn, HD, 1e-6, k);
+  const c = ops.attention(gpu, { q, k, v, B, Lq: L, Lk: cond.Lk, H, D: HD, ldq: D, ldk: D, ldv: D, qNorm: b.cross.qn, precision,
+    oBf16: precision === "bf16" });
+  into(await wide(c), b.cross.o, m.cross);
+  const h = ops.linear(gpu, norm(m.mlp), b.l1, { act: "gelu", precision, outBf16: precision === "bf16" });
+  into(await wide(h), b.l2, m.mlp);
+}
+
+async function ditsteps(gpu, c) {
+  const src = new SyntheticWeights(gpu, c.seed, { blocks: c.kinds.length });
+  src.quantKind = (i) => c.kinds[i];
+  const model = AnimaDiT.synthetic(gpu, src);
+  console.log(JSON.stringify({ converted: model.quantizeF8() }));
+  const B = c.latents.length, L = (c.h / 2) * (c.w / 2), tc = model.timeCond(c.sigma);
+  for (const precision of ["fp32", "bf16"]) {
+    model.precision = precision;
+    const cond = model.prepareContext(c.ctx.map((p) => gpu.fromArray(load(p), [c.Lk, 1024])));
+    const xs = [];
+    await model.forward(c.latents.map((p) => load(p)), c.h, c.w, cond, tc, async (i, x) => xs.push(await gpu.read(x)));
+    for (let i = 1; i < xs.length; i++) {
+      if (c.kinds[i] !== "bf16") continue;
+      const x = gpu.fromArray(xs[i - 1], [B * L, 2048]);
+      await blockSteps(gpu, model, i, x, cond, tc, B, L, model.ropeTable(c.h / 2, c.w / 2));
+      save(`${c.out}.${precision}.${i}`, xs[i]);
+      save(`${c.out}.${precision}.${i}.steps`, await gpu.read(x));
+    }
+    cond.release();
+  }
+}
+
 const c = JSON.parse(fs.readFileSync(process.argv[2], "utf8"));
 GPU.create({})
   .then(async (gpu) => {
-    await { block, groups, qwen3, dit }[c.case](gpu, c);
+    await { block, groups, qwen3, dit, ditsteps }[c.case](gpu, c);
     gpu.destroy();
   })
   .catch((e) => {

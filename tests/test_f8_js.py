@@ -396,3 +396,25 @@ def test_js_dit_f8(tmp_path):
         assert report("dit f8 rows from norms vs from fp32 rows", v["f8"], v["f8lora"])[0] <= bar
         assert report("dit f8 bf16 vs fp32", v["f8bf16"], v["f8"])[0] <= bar
         assert 1e-3 < report("dit f8 vs bf16 weights", v["f8"], v["bf16w"])[0] <= bar
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kinds", [["bf16", "bf16", "bf16"], ["i8", "bf16"], ["w4", "bf16", "i8", "bf16"]])
+def test_js_dit_f8_steps(tmp_path, kinds):
+    """The DiT's e4m3 blocks (of bf16 ones converted) between others, in both precisions: the residual stream bit for bit
+    as the block's ops one by one give it, on fp32 rows that every product quantizes itself."""
+    out = str(tmp_path / "s")
+    h, w, Lk = 16, 24, 40
+    spec = {"case": "ditsteps", "seed": 11, "kinds": kinds, "sigma": 0.6, "h": h, "w": w, "Lk": Lk, "out": out,
+            "latents": [write(tmp_path, f"l{b}", orc.randn(80 + b, 16 * h * w)) for b in range(2)],
+            "ctx": [write(tmp_path, f"c{b}", orc.randn(90 + b, Lk * 1024)) for b in range(2)]}
+    log = run_case(tmp_path, spec)
+    assert json.loads(log.splitlines()[0]) == {"converted": 8 * kinds.count("bf16")}
+    n = 0
+    for prec in ("fp32", "bf16"):
+        for i in range(1, len(kinds)):
+            if kinds[i] == "bf16":
+                got, want = (np.fromfile(f"{out}.{prec}.{i}{t}", np.float32) for t in ("", ".steps"))
+                assert np.isfinite(got).all() and np.array_equal(got, want), (prec, i, np.abs(got - want).max())
+                n += 1
+    assert n == 2 * kinds[1:].count("bf16")
