@@ -923,3 +923,30 @@ def test_linear_split(ctx, M, N, K, fast):
             ctx.graph_launch(g)
             assert np.array_equal(out.numpy(), bits) and np.array_equal(eager.numpy(), bits)
         ctx.graph_destroy(g)
+
+
+@pytest.mark.parametrize("tile,fast,M,N,K", [
+    ("64x64", True, 372, 328, 4112), ("64x64", False, 502, 504, 2976), ("128x64", True, 786, 274, 5104), ("128x64", False, 326, 648, 4384),
+    ("128x128", True, 131, 2097, 7792), ("128x128", False, 520, 775, 7056), ("256x256", True, 2400, 1707, 7136),
+    ("256x256", False, 1233, 3316, 8000)])
+def test_linear_split_tiles(ctx, tile, fast, M, N, K):
+    """The k loop of every tile split over workgroups, in both precisions; the same bits on every call."""
+    case(f"linear f8 split tile={tile} M={M} N={N} K={K} fast={fast}")
+    m = amd()
+    prec = m.PREC_BF16 if fast else m.PREC_FP32
+    w, scale = f8_weight(N + K, N, K)
+    bias, gate = randn(95, N).astype(np.float32), randn(96, N).astype(np.float32)
+    out0 = randn(97, M * N).reshape(M, N).astype(np.float32)
+    W = m.weight(m.W_F8, N, K, ctx.upload(w), scale=ctx.upload(scale), bias=ctx.upload(bias))
+    args, x64 = inputs(ctx, M + K, M, K, "f8")
+    y, dy = product64(x64, weight64(w, scale), fast)
+    r, dr = (y + bias) * gate, (dy + U * np.abs(y + bias)) * np.abs(gate)
+    d_gate, bits = ctx.upload(gate), None
+    for _ in range(3):
+        out = Guarded(ctx, (M, N), np.float32, out0)
+        names = ran(ctx, lambda: ctx.linear(W, M, out.ptr, epilogue=m.EPI_GATED, gate=d_gate, precision=prec, **args))
+        assert f"gemm.f8.{tile}" in names and "gemm.f8.join" in names, names
+        got = out.numpy()
+        assert np.all(np.abs(got - (out0 + r)) <= dr + 2 * U * (np.abs(r) + np.abs(out0 + r)))
+        assert bits is None or np.array_equal(bits, got)
+        bits = got
