@@ -112,9 +112,11 @@ __device__ __forceinline__ uint32_t cross_umax(uint32_t v) {
   return umax(q[0], q[1]);
 }
 
-// SiLU as r * rcp(1 + 2^(-r log2 e)) on v_exp_f32 and v_rcp_f32 (1 ulp each): within 2^-22 (1 + |r| / 2) of itself for
-// negative r (the rounding of the exponent), 2^-22 for others; 5 instructions, where silu_f's expf and quotient take 40
-// (of a 256 x 256 tile's epilogue 25000 cycles, and 9000).
+// SiLU as r * rcp(1 + 2^(-r log2 e)) on v_exp_f32 and v_rcp_f32 (1 ulp each): the exponent is off by 1.22 roundings of
+// itself, the power, the sum, the reciprocal and the product by 2, 1, 2 and 1, so within 2^-22 (3/2 + |r| / 3) of itself for
+// r from -87 to 0 and 1.3 2^-22 for others; below -87, where the power or its reciprocal leaves the range, it may be -0
+// (within 1.5e-36).  5 instructions, where silu_f's expf and quotient take 40 (of a 256 x 256 tile's epilogue 25000 cycles,
+// and 9000).
 __device__ __forceinline__ float f8_silu(float r) {
   return r * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(r * -1.4426950408889634f));
 }

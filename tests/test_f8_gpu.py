@@ -950,3 +950,31 @@ def test_linear_split_tiles(ctx, tile, fast, M, N, K):
         assert np.all(np.abs(got - (out0 + r)) <= dr + 2 * U * (np.abs(r) + np.abs(out0 + r)))
         assert bits is None or np.array_equal(bits, got)
         bits = got
+
+
+@pytest.mark.parametrize("M", [1, 300])
+def test_silu_range(ctx, M):
+    """The activation by itself: rows of zeros, so that a result is silu(bias).  Within 2^-22 (3/2 + |r| / 3) of itself from
+    -87 to 0 and 1.3 2^-22 above (the roundings of its exponent, power, sum, reciprocal and product); below -87 within
+    1.5e-36; an infinity stays, NaN too."""
+    case(f"silu f8 M={M}")
+    m = amd()
+    N, K = 16384, 128
+    r = np.concatenate([np.linspace(-120, 40, N - 1024), np.random.default_rng(6).normal(size=1020) * 3,
+                        [np.inf, np.nan, 3e38, -3e38]]).astype(np.float32)
+    zero = ctx.upload(np.zeros((M, K), np.float32))
+    w, scale = f8_weight(1, N, K)
+    weights = [m.weight(m.W_F8, N, K, ctx.upload(w), scale=ctx.upload(scale), bias=ctx.upload(b)) for b in (r, np.ones(N, np.float32))]
+    lin, glu = Guarded(ctx, (M, N), np.float32), Guarded(ctx, (M, N), np.float32)
+    ctx.linear(weights[0], M, lin.ptr, x=zero, act="silu", precision=m.PREC_FP32)
+    ctx.linear_glu(weights[0], weights[1], M, x=zero, act="silu", out=glu.ptr, precision=m.PREC_FP32)
+    r64 = r.astype(np.float64)
+    fin, low = np.isfinite(r64), r64 < -87
+    with np.errstate(all="ignore"):
+        want = np.where(low, r64 * np.exp(np.maximum(r64, -700)), r64 / (1 + np.exp(-r64)))
+        bound = np.where(low, 1.5e-36, 2.0 ** -22 * np.where(r64 < 0, 1.5 + np.abs(r64) / 3, 1.3) * np.abs(want))
+    for got in (lin.numpy(), glu.numpy()):
+        assert np.array_equal(got, np.broadcast_to(got[0], got.shape), equal_nan=True)
+        off = np.abs(got[0][fin] - want[fin])
+        assert (off <= bound[fin]).all(), r[fin][off > bound[fin]]
+        assert got[0][-4] == np.inf and np.isnan(got[0][-3])
