@@ -451,8 +451,8 @@ typedef struct {
  * and the store / residual / gated-residual epilogue of gemm.js:186-192.
  * i8/w4 need K % 64 == 0 (and K <= 8192 when x is quantized here).
  * f8: r = alpha * sum_b xs[b][m] scale[n / 128][b] * (sum of xq[m][k] w[n][k] over the 128 k of block b):
- * each block's products summed on the matrix cores (see precision), the blocks added in fp32.  Any M and N;
- * K % 16 == 0, K <= 2^20.  fp32 rows x are quantized as anima_quant_rows_f8 does, few of them inside the
+ * each block's products summed on the matrix cores (see precision), the blocks added in fp32.  M and N up to
+ * 2^30; K % 16 == 0, K <= 2^20.  fp32 rows x are quantized as anima_quant_rows_f8 does, few of them inside the
  * product's kernel, more in a pass before it (pooled scratch); few tiles of a long k are split over k, with the
  * splits' sums in pooled scratch.  The order in which a result's blocks are
  * added, and so its last bits, depends on the sizes.  No acc_out and no LoRA factors (`add` carries a
@@ -529,7 +529,8 @@ int anima_set_w4_path(anima_ctx* ctx, int path);
  * K % 16 == 0; x and q 16-byte aligned, ldx a multiple of 16 bytes.  q and s overlap no input. */
 int anima_quant_rows_f8(anima_ctx* ctx, const void* x, int x_bf16, int64_t M, int K, int64_t ldx, uint8_t* q, float* s);
 /* A weight w[N][K] (fp32, or bf16 with w_bf16 = 1) to the data q[N][K] and scales [ceil(N/128)][ceil(K/128)]
- * of an ANIMA_W_F8 weight, one scale per 128 x 128 block: a loader's conversion of a bf16 checkpoint. */
+ * of an ANIMA_W_F8 weight, one scale per 128 x 128 block (fewer than 2^24 blocks): a loader's conversion of a
+ * bf16 checkpoint. */
 int anima_weight_quant_f8(anima_ctx* ctx, const void* w, int w_bf16, int N, int K, uint8_t* q, float* scale);
 
 /* The first half of a gated feed-forward block (the gate / up linears and the silu_mul of
