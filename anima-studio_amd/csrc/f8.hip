@@ -199,7 +199,8 @@ __global__ __launch_bounds__(256) void quant_rows_f8_kernel(const T* X, int64_t 
   }
 }
 
-// A workgroup per 128 x 128 block (a checkpoint's conversion, once per weight): thread t holds columns 4 (t % 32) .. + 3 of rows t / 32 + 8 i.
+// A workgroup per 128 x 128 block (a checkpoint's conversion, once per weight): thread t holds columns 4 (t % 32) .. + 3 of
+// rows t / 32 + 8 i.  Bound by the bytes: 8192 x 2048 from bf16 (50 MB) 10.4 us, 4.8 TB/s, from fp32 (84 MB) 14.6, 5.7.
 template <class T>
 __global__ __launch_bounds__(256) void weight_quant_f8_kernel(const T* W, int N, int K, int KB, uint8_t* Q, float* S) {
   __shared__ uint32_t red[8];
@@ -1214,7 +1215,8 @@ static int64_t f8_tiles(int kind, bool glu, int64_t M, int64_t N) {
 // Microseconds of a product (f8_skinny: base + step for each block of k of a wave + work for each 4096 blocks that all
 // its workgroups read; tiles: base + for each tile per CU step for each block of k, round for each tile after the first)
 // + out for a million outputs.  Fitted to 3000 products of M = 1 .. 8192, N and K = 64 .. 8192: the choice takes
-// 0.1 to 1.0% longer than the best kernel in the mean.  Small products are bound by the depth of one
+// 0.1 to 1.0% longer than the best kernel in the mean (the linear's 128 x 64 tiles with 32-bit sums as they were with
+// two stages; their third took 4 to 5% off where the choice takes 128 x 128: 4096 x 1024 x 2048, 2048 x 2048 x 4096).  Small products are bound by the depth of one
 // workgroup's k loop, so they take the waves of f8_skinny or small tiles; large ones by the bytes that a tile's
 // operands move per product (43 x 2048 x 1024: 4.6, 64x64 8.6, 256x256
 // 33 us; 3013 x 1316 x 1424 gated with 32-bit sums: 64x64 26.2, 128x64 23.3; 8192 x 2048 x 8192: 64x64 220,
