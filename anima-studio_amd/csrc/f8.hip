@@ -1216,11 +1216,10 @@ static int64_t f8_tiles(int kind, bool glu, int64_t M, int64_t N) {
 // its workgroups read; tiles: base + for each tile per CU step for each block of k, round for each tile after the first)
 // + out for a million outputs.  Fitted to 3000 products of M = 1 .. 8192, N and K = 64 .. 8192: the choice takes
 // 0.1 to 1.0% longer than the best kernel in the mean (the linear's 128 x 64 tiles with 32-bit sums as they were with
-// two stages; their third took 4 to 5% off where the choice takes 128 x 128: 4096 x 1024 x 2048, 2048 x 2048 x 4096).  Small products are bound by the depth of one
-// workgroup's k loop, so they take the waves of f8_skinny or small tiles; large ones by the bytes that a tile's
-// operands move per product (43 x 2048 x 1024: 4.6, 64x64 8.6, 256x256
-// 33 us; 3013 x 1316 x 1424 gated with 32-bit sums: 64x64 26.2, 128x64 23.3; 8192 x 2048 x 8192: 64x64 220,
-// 256x256 116).
+// two stages; their third took 4 to 5% off where the choice takes 128 x 128: 4096 x 1024 x 2048, 2048 x 2048 x 4096).
+// Small products are bound by the depth of one workgroup's k loop, so they take the waves of f8_skinny or small tiles;
+// large ones by the bytes that a tile's operands move per product (43 x 2048 x 1024: 4.6, 64x64 8.6, 256x256 33 us;
+// 3013 x 1316 x 1424 gated with 32-bit sums: 64x64 26.2, 128x64 23.3; 8192 x 2048 x 8192: 64x64 220, 256x256 116).
 // The gated form leaves e4m3 rows from the tiles of 128 columns; from the others they cost a pass.
 // Where the tiles leave CUs idle, the k loop of a linear is split (*splits): each split's sums go through memory and
 // f8_join (512 x 1024 x 8192 with 32-bit sums 32.7 us, split 20.0; 64 x 4096 x 4096 20.4, 12.5; 300 x 384 x 4096 10.9,

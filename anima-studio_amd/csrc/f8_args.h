@@ -13,7 +13,7 @@ namespace anima {
 constexpr int F8_MAX_K = 1 << 20;         // of a product: 256 rows of a tile stay below 2^31 bytes
 constexpr int64_t F8_MAX_LDX = 1 << 22;   // bytes between e4m3 rows of a product's input, likewise
 constexpr int F8_NORM_MAX_COLS = 16384;   // a row in one workgroup's registers
-constexpr int F8_MAX_SIDE = 1 << 30;      // rows and outputs of a product: 256 x 256 tiles of either stay below 2^32 threads
+constexpr int F8_MAX_SIDE = 1 << 29;      // rows and outputs of a product: tiles of 256 x 128 stay below 2^32 threads
 
 // A launch has fewer than 2^32 threads a dimension, so large calls are cut into several.
 constexpr int64_t F8_MAX_THREADS = 0xffffffff;

@@ -95,7 +95,8 @@ function f8Rows(gpu, M, K) {
 // A bf16 or f32 weight turned into the e4m3 weight with one scale per 128 x 128 block, in place (as
 // unpackW4: LoRA attachments stay).  Half the bytes of bf16; a weight is off by at most 2^-4 of its
 // value, or, below 2^-6 of its block's scale, by 2^-10 of the scale (1/448 of the block's largest
-// weight: small weights beside large ones become 0).  Other kinds, and input widths that are no multiple of 16, stay as they are.
+// weight: small weights beside large ones become 0).  Other kinds, and input widths that are no
+// multiple of 16, stay as they are.
 export function quantizeF8(gpu, W) {
   if ((W.kind !== "bf16" && W.kind !== "f32") || W.K % 16) return W;
   const q = gpu.empty([W.N * W.K], "u8");

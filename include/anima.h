@@ -452,7 +452,7 @@ typedef struct {
  * i8/w4 need K % 64 == 0 (and K <= 8192 when x is quantized here).
  * f8: r = alpha * sum_b xs[b][m] scale[n / 128][b] * (sum of xq[m][k] w[n][k] over the 128 k of block b):
  * each block's products summed on the matrix cores (see precision), the blocks added in fp32.  M and N up to
- * 2^30; K % 16 == 0, K <= 2^20.  fp32 rows x are quantized as anima_quant_rows_f8 does, few of them inside the
+ * 2^29; K % 16 == 0, K <= 2^20.  fp32 rows x are quantized as anima_quant_rows_f8 does, few of them inside the
  * product's kernel, more in a pass before it (pooled scratch); few tiles of a long k are split over k, with the
  * splits' sums in pooled scratch.  The order in which a result's blocks are
  * added, and so its last bits, depends on the sizes.  No acc_out and no LoRA factors (`add` carries a

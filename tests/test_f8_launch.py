@@ -60,10 +60,12 @@ def test_weight_quant(parts, N, K, code):
     assert rc == code and (code == 0 or "anima_weight_quant_f8" in msg)
 
 
-@pytest.mark.parametrize("M,N,code", [(1, 1 << 30, 0), (1, (1 << 30) + 1, -5), (1, (1 << 31) - 1, -5), (1 << 30, 1, 0),
-                                      ((1 << 30) + 1, 1, -5), ((1 << 31) - 1, 1, -5)])
+@pytest.mark.parametrize("M,N,code", [(1, 1 << 29, 0), (1, (1 << 29) + 1, -5), (1, (1 << 31) - 1, -5), (1 << 29, 1, 0),
+                                      ((1 << 29) + 1, 1, -5), ((1 << 31) - 1, 1, -5)])
 def test_products(parts, M, N, code):
-    """Sides of a product: at 2^30 the largest tiles still fit a launch, and sizes rounded up to a tile fit 31 bits."""
+    """Sides of a product: at 2^29 the largest tiles (256 x 256, gated 256 x 128, of 512 threads) fit a launch, and sizes
+    rounded up to a tile fit 31 bits."""
+    assert code != 0 or max(-(-M // 256) * -(-N // 128), -(-M // 128) * -(-N // 256)) * 512 < 1 << 32
     m = amd()
     W = weight(N=N, K=16)
     rc, msg = call(parts.t_linear, ctypes.byref(m.LinearDesc(M=M, W=ctypes.pointer(W), x=P, out=P)))
