@@ -125,6 +125,11 @@ function checkRows(W, xq, want) {
   return M;
 }
 
+// a tensor that the kernel reads or writes as fp32 (bf16: its other form), of twice the bytes
+function checkDtype(name, t, dtype) {
+  if (t && t.dtype && t.dtype !== dtype) throw new Error(`${name}: a ${t.dtype} tensor, expected ${dtype}`);
+}
+
 function weightArg(W) {
   if (!(W.kind in KIND)) throw new Error(`unsupported weight kind ${W.kind}`);
   return { kindId: KIND[W.kind], N: W.N, K: W.K, buf: ptr(W.buf), scale: ptr(W.scale), srel: ptr(W.srel),
@@ -164,6 +169,10 @@ export function linear(gpu, x, W, opts) {
   const delta = lora && !F && !late ? loraDelta(gpu, xin, W, M, rot) : null;
   if (o.outBf16 && W.kind !== "f8") throw new Error(`${W.name || "linear"}: bf16 results are for f8 weights`);
   if (o.outBf16 && late) throw new Error(`${W.name || "linear"}: no bf16 result with a LoRA`);
+  if (W.kind === "f8") {
+    if (!o.xq) checkDtype(`${W.name || "linear"}: x`, x, "f32");
+    checkDtype(`${W.name || "linear"}: out`, o.out, o.outBf16 ? "bf16" : "f32");
+  }
   const out = o.out || gpu.empty([M, W.N], o.outBf16 ? "bf16" : "f32");
   const d = { M, out: out.buf, ldc: o.ldc || 0, alpha: o.alpha || 0, act: ACT[o.act || "none"],
     epilogue: o.resid ? (o.gate ? 2 : 1) : 0, gate: ptr(o.gate), gOff: o.gOff || 0, accOut: ptr(o.accOut),
@@ -399,6 +408,8 @@ export function linearGlu(gpu, x, Wg, Wu, opts) {
     if (W.lora && W.lora.length) throw new Error(`linearGlu: ${W.name || "weight"} has a LoRA`);
     if (o.xq) checkRows(W, o.xq, o.M);
   }
+  if (!o.xq) checkDtype("linearGlu: x", x, "f32");
+  checkDtype("linearGlu: out", o.out, "f32");
   const M = o.M !== undefined ? o.M : (o.xq ? checkRows(Wg, o.xq) : x.size / Wg.K);
   const rows = o.f8 ? f8Rows(gpu, M, Wg.N) : null;
   const out = rows ? null : o.out || gpu.empty([M, Wg.N]);
@@ -419,6 +430,7 @@ export function residualNorm(gpu, x, cols, opts) {
   const o = opts || {};
   if (o.norm !== undefined && !(o.norm in NORM)) throw new Error(`residualNorm: unknown norm ${o.norm}`);
   const rows = x.size / cols;
+  checkDtype("residualNorm: x", x, "f32");
   if (o.y && o.y.size !== x.size) throw new Error(`residualNorm: y of ${o.y.size} values for x of ${x.size}`);
   const groups = o.groupRows ? Math.ceil(rows / o.groupRows) : 1;
   const vectors = (name, t, off, ld) => {

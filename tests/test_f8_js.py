@@ -167,6 +167,25 @@ def test_residual_norm_groups():
     assert "without rows q and scales s" in got["rows"] and "without rows q and scales s" in got["glu"]
 
 
+def test_types_of_tensors():
+    """bf16 tensors where the kernels read or write fp32 rows, twice the bytes, and the other way round."""
+    got = node(RECORD + MSG + "import('./ops.mjs').then((ops) => {"
+               "const W = { kind: 'f8', N: 32, K: 128, name: 'w' }, f = () => tensor([4, 128]), b = () => tensor([4, 128], 'bf16');"
+               "console.log(JSON.stringify({"
+               " x: msg(() => ops.linear(gpu, b(), W, {})), glu: msg(() => ops.linearGlu(gpu, b(), W, W, {})),"
+               " norm: msg(() => ops.residualNorm(gpu, b(), 128, {})),"
+               " out: msg(() => ops.linear(gpu, f(), W, { out: tensor([4, 32], 'bf16') })),"
+               " bf16_out: msg(() => ops.linear(gpu, f(), W, { out: tensor([4, 32]), outBf16: true })),"
+               " glu_out: msg(() => ops.linearGlu(gpu, f(), W, W, { out: tensor([4, 32], 'bf16') })),"
+               " fine: [msg(() => ops.linear(gpu, f(), W, { out: tensor([4, 32]) })),"
+               "  msg(() => ops.linear(gpu, f(), W, { out: tensor([4, 32], 'bf16'), outBf16: true })),"
+               "  msg(() => ops.linearGlu(gpu, f(), W, W, { out: tensor([4, 32]) })),"
+               "  msg(() => ops.residualNorm(gpu, f(), 128, { y: b() }))] })); })")
+    assert got.pop("fine") == [""] * 4
+    for name, m in got.items():
+        assert "a bf16 tensor, expected f32" in m if name != "bf16_out" else "a f32 tensor, expected bf16" in m, (name, m)
+
+
 def test_context_of_mixed_kinds():
     """Cross-attention k / v of several kinds in one model: each linear gets the rows that its weight reads."""
     kinds = [("i8", "i8"), ("f8", "f8"), ("bf16", "bf16"), ("w4", "f8"), ("f8", "i8")]
