@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import json
+import operator
 import os
 import struct
 
@@ -21,7 +22,7 @@ HEADER = os.path.join(os.path.dirname(HERE), "include", "anima.h")
 ANIMA_OK = 0
 PREC_BF16 = 0
 PREC_FP32 = 1
-W_BF16, W_I8, W_W4, W_F32, W_F32S3, W_F8 = 0, 1, 2, 3, 4, 5
+W_BF16, W_I8, W_W4, W_F32, W_F32S3, W_F8, W_Q4 = 0, 1, 2, 3, 4, 5, 6
 W4_GRID_SCRATCH, W4_IN_GEMM = 0, 1
 ACT = {"none": 0, "gelu": 1, "silu": 2}
 EPI_STORE, EPI_RESID, EPI_GATED = 0, 1, 2
@@ -60,6 +61,15 @@ class AttnDesc(ctypes.Structure):
     ]
 
 
+class PrefixAttnDesc(ctypes.Structure):
+    _fields_ = [("B", ctypes.c_int), ("len", _vp), ("P", ctypes.c_int), ("H", ctypes.c_int), ("D", ctypes.c_int),
+                ("group", ctypes.c_int), ("q", _vp), ("ldq", _i64), ("q_off", _i64), ("k", _vp), ("ldk", _i64),
+                ("k_off", _i64), ("v", _vp), ("ldv", _i64), ("v_off", _i64), ("o", _vp), ("ldo", _i64), ("o_off", _i64),
+                ("prefix_kv", _vp), ("prefix_kv_bytes", _i64), ("scale", ctypes.c_float), ("causal", ctypes.c_int),
+                ("precision", ctypes.c_int), ("q_norm", _vp), ("k_norm", _vp), ("rope_cs", _vp), ("rope_sin_off", _i64),
+                ("eps", ctypes.c_float), ("o_bf16", ctypes.c_int)]
+
+
 class ConvDesc(ctypes.Structure):
     _fields_ = [("B", ctypes.c_int), ("H", ctypes.c_int), ("W", ctypes.c_int), ("cin", ctypes.c_int),
                 ("cout", ctypes.c_int), ("up", ctypes.c_int), ("x", _vp), ("w", _vp), ("bias", _vp), ("out", _vp),
@@ -68,7 +78,8 @@ class ConvDesc(ctypes.Structure):
 
 class Weight(ctypes.Structure):
     _fields_ = [("kind", ctypes.c_int), ("N", ctypes.c_int), ("K", ctypes.c_int), ("w", _vp), ("scale", _vp),
-                ("srel", _vp), ("codebook", _vp), ("bias", _vp)]
+                ("srel", _vp), ("codebook", _vp), ("bias", _vp), ("group", ctypes.c_int), ("group_scale", _vp),
+                ("group_mid", _vp)]
 
 
 class LinearDesc(ctypes.Structure):
@@ -129,11 +140,13 @@ def _packer(cls):
 
 
 _linear_desc, _glu_desc, _resnorm_desc = _packer(LinearDesc), _packer(GluDesc), _packer(ResNormDesc)
+_prefix_attn_desc = _packer(PrefixAttnDesc)
 
 
 ABI_STRUCTS = {"anima_attn_desc": AttnDesc, "anima_linear_desc": LinearDesc, "anima_weight": Weight,
                "anima_sampler_desc": SamplerDesc, "anima_conv_desc": ConvDesc, "anima_limits": Limits,
-               "anima_qkv_desc": QkvDesc, "anima_glu_desc": GluDesc, "anima_resnorm_desc": ResNormDesc}
+               "anima_qkv_desc": QkvDesc, "anima_glu_desc": GluDesc, "anima_resnorm_desc": ResNormDesc,
+               "anima_prefix_attn_desc": PrefixAttnDesc}
 
 
 def abi_mismatches(L):
@@ -221,9 +234,12 @@ def lib():
         L.anima_fill_random.argtypes = [_vp, _vp, _i64, ctypes.c_int, ctypes.c_uint64, ctypes.c_float, ctypes.c_float]
         L.anima_quant_rows_f8.argtypes = [_vp, _vp, ctypes.c_int, _i64, ctypes.c_int, _i64, _vp, _vp]
         L.anima_weight_quant_f8.argtypes = [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp]
+        L.anima_weight_quant_q4.argtypes = [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp, _vp]
+        L.anima_embed_rows.argtypes = [_vp, _vp, _vp, _i64, _vp, ctypes.c_float, _vp, _i64]
+        L.anima_attention_prefix.argtypes = [_vp, P(PrefixAttnDesc)]
         L.anima_linear_glu.argtypes = [_vp, P(GluDesc)]
         L.anima_residual_norm.argtypes = [_vp, P(ResNormDesc)]
-        for n in ("anima_linear", "anima_linear_glu", "anima_residual_norm"):  # with a packed descriptor (bytes)
+        for n in ("anima_linear", "anima_linear_glu", "anima_residual_norm", "anima_attention_prefix"):  # with a packed descriptor (bytes)
             packed = L[n]
             packed.argtypes = [_vp, _vp]
             setattr(L, n + "_packed", packed)
@@ -482,7 +498,8 @@ class Context:
         """anima_linear; lora_xa / lora_b / lora_r: the LoRA delta's factors for the quantized
         GEMM's epilogue (A products [M][ld_lora_xa] fp32, B as three bf16 planes [3][N][lora_r]);
         lora_cols > 0: block-diagonal ranks, column n reading xa columns (n // lora_cols) * lora_r
-        + k.  f8 weights: precision (PREC_FP32: sums in 32 bits), out_bf16 (bf16 rows out)."""
+        + k.  f8 and q4 weights: precision (PREC_FP32: sums in 32 bits, q4: of x as it is), out_bf16 (bf16
+        rows out)."""
         # (absent pointers without a call: half a microsecond of every linear)
         d = _linear_desc(M, _weight_adr(W), x and _adr(x) or 0, ldx, int(x_rotated), xq and _adr(xq) or 0,
                          xs and _adr(xs) or 0, _adr(out), ldc, alpha, ACT[act] if isinstance(act, str) else act, epilogue,
@@ -519,6 +536,34 @@ class Context:
     def weight_quant_f8(self, w, N, K, q, scale, *, bf16=True):
         """anima_weight_quant_f8: a bf16 (fp32) weight to the data and block scales of a W_F8 weight."""
         return self._check(lib().anima_weight_quant_f8(self.h, _ptr(w), int(bf16), N, K, _ptr(q), _ptr(scale)))
+
+    def weight_quant_q4(self, w, N, K, group, q, scale, mid=None, *, bf16=True):
+        """anima_weight_quant_q4: a bf16 (fp32) weight to the codes, group scales and (mid) middles of a W_Q4
+        weight."""
+        return self._check(lib().anima_weight_quant_q4(self.h, _ptr(w), int(bf16), N, K, group, _ptr(q), _ptr(scale),
+                                                       _ptr(mid)))
+
+    def embed_rows(self, table, ids, T, out, *, weights=None, scale=0.0, ldo=0):
+        """anima_embed_rows: out[t] = scale * weights[t] * table[ids[t]] of a table (weight()) of kind W_F32, W_BF16
+        or W_Q4; ids (int32, on the device) outside it give rows of zeros."""
+        return self._check(lib().anima_embed_rows(self.h, _weight_adr(table), _ptr(ids), T, _ptr(weights), scale, _ptr(out),
+                                                  ldo))
+
+    def attention_prefix(self, *, q, k, v, o, lens, H, D=128, ldq, ldk, ldv, ldo=None, q_off=0, k_off=0, v_off=0, o_off=0,
+                         group=1, P=0, prefix_kv=None, prefix_kv_bytes=None, scale=0.0, causal=1, precision=PREC_BF16,
+                         q_norm=None, k_norm=None, rope_cs=None, rope_sin_off=0, eps=1e-6, o_bf16=False):
+        """anima_attention_prefix: packed sequences of lens[b] rows, each behind the same P keys, which
+        attention(B=1, Lk=P, prepare_into=prefix_kv) has prepared.  prefix_kv_bytes defaults to the size that P,
+        the heads and the precision take."""
+        if not (isinstance(lens, np.ndarray) and lens.dtype == np.int32 and lens.ndim == 1 and lens.flags.c_contiguous):
+            lens = np.array([operator.index(n) for n in lens], np.int32)
+        if prefix_kv_bytes is None:
+            prefix_kv_bytes = self.attention_kv_bytes(1, H // max(group, 1), P, precision) if P > 0 else 0
+        d = _prefix_attn_desc(lens.size, lens.ctypes.data, P, H, D, group, _adr(q), ldq, q_off, _adr(k), ldk, k_off, _adr(v),
+                              ldv, v_off, _adr(o), ldo if ldo is not None else H * D, o_off, _adr(prefix_kv), prefix_kv_bytes,
+                              scale, causal, precision, _adr(q_norm), _adr(k_norm), _adr(rope_cs), rope_sin_off, eps,
+                              int(o_bf16))
+        return self._check(lib().anima_attention_prefix_packed(self.h, d))
 
     def linear_glu(self, gate, up, M, *, x=None, xq=None, xs=None, ldx=0, act="silu", out=None, ldc=0, out_q=None,
                    out_s=None, precision=PREC_BF16):
@@ -562,10 +607,10 @@ class Context:
                                             row_stride if row_stride is not None else H * D, col_off))
 
 
-def weight(kind, N, K, w, scale=None, srel=None, codebook=None, bias=None):
+def weight(kind, N, K, w, scale=None, srel=None, codebook=None, bias=None, group=0, group_scale=None, group_mid=None):
     """Linear weight object of app/weights.js:1-4 (device buffers)."""
     return Weight(kind=kind, N=N, K=K, w=_ptr(w), scale=_ptr(scale), srel=_ptr(srel), codebook=_ptr(codebook),
-                  bias=_ptr(bias))
+                  bias=_ptr(bias), group=group, group_scale=_ptr(group_scale), group_mid=_ptr(group_mid))
 
 
 def dit_rope_angles(Hp: int, Wp: int) -> np.ndarray:

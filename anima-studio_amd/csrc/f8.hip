@@ -1075,17 +1075,6 @@ __global__ __launch_bounds__(256) void f8_join(F8Args a, const float* part, int 
 
 namespace {
 
-// Makes the context's device the current one for a call's launches.
-struct OnDevice {
-  int before = -1;
-  explicit OnDevice(const anima_ctx* c) {
-    if (hipGetDevice(&before) != hipSuccess || before == c->device || hipSetDevice(c->device) != hipSuccess) before = -1;
-  }
-  ~OnDevice() {
-    if (before >= 0) (void)hipSetDevice(before);
-  }
-};
-
 int refused(anima_ctx* c, int rc, const char* msg) { return fail(c, rc, "%s", msg); }
 
 }  // namespace

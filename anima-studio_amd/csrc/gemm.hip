@@ -2729,11 +2729,12 @@ int linear_launch(anima_ctx* c, const anima_linear_desc* d, int64_t s3_plane) {
                   d->lora_cols, N, (long long)d->ld_lora_xa);
     if (d->add) return fail(c, ANIMA_E_UNSUPPORTED, "anima_linear: the LoRA epilogue and an add term together");
   }
-  if (W->kind != ANIMA_W_F8 && (d->precision || d->out_bf16))
-    return fail(c, ANIMA_E_UNSUPPORTED, "anima_linear: precision and out_bf16 are for f8 weights (kind %d)", W->kind);
+  if (W->kind != ANIMA_W_F8 && W->kind != ANIMA_W_Q4 && (d->precision || d->out_bf16))
+    return fail(c, ANIMA_E_UNSUPPORTED, "anima_linear: precision and out_bf16 are for f8 and q4 weights (kind %d)", W->kind);
   if (M == 0) return ANIMA_OK;
 
   if (W->kind == ANIMA_W_F8) return linear_f8_launch(c, d);
+  if (W->kind == ANIMA_W_Q4) return linear_q4_launch(c, d);
   if (W->kind == ANIMA_W_F32S3) {
     // x: fp32 rows, or per-token int8 rows xq with their scales xs (y = xs[m] * (q W^T)[m])
     const bool q8 = d->xq != nullptr;

@@ -87,6 +87,17 @@ int hip_fail(anima_ctx* c, hipError_t e, const char* what);
 // Workspace of at least `bytes` (grows by synchronizing and reallocating).
 int workspace(anima_ctx* c, size_t bytes, void** out);
 
+// Makes the context's device the current one for a call's launches.
+struct OnDevice {
+  int before = -1;
+  explicit OnDevice(const anima_ctx* c) {
+    if (hipGetDevice(&before) != hipSuccess || before == c->device || hipSetDevice(c->device) != hipSuccess) before = -1;
+  }
+  ~OnDevice() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
+
 // Launch bracket for the profiler: begin() before a kernel launch, end() after it.
 struct Launch {
   anima_ctx* c;
@@ -157,5 +168,15 @@ int weight_quant_f8_launch(anima_ctx* c, const void* w, int w_bf16, int N, int K
 int linear_f8_launch(anima_ctx* c, const anima_linear_desc* d);
 int linear_glu_launch(anima_ctx* c, const anima_glu_desc* d);
 int residual_norm_launch(anima_ctx* c, const anima_resnorm_desc* d);
+
+// ---- kernel launchers (q4.hip)
+int weight_quant_q4_launch(anima_ctx* c, const void* w, int w_bf16, int N, int K, int group, uint8_t* q, uint16_t* scale, uint16_t* mid);
+int embed_rows_launch(anima_ctx* c, const anima_weight* table, const int32_t* ids, int64_t T, const float* weights, float scale,
+                      float* out, int64_t ldo);
+// (linear_launch has made the checks that every kind of weight shares)
+int linear_q4_launch(anima_ctx* c, const anima_linear_desc* d);
+
+// ---- kernel launchers (prefix.hip)
+int attention_prefix_launch(anima_ctx* c, const anima_prefix_attn_desc* d);
 
 }  // namespace anima

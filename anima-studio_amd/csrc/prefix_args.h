@@ -1,0 +1,89 @@
+// Argument checks of anima_attention_prefix (prefix.hip).  Plain host code: no HIP call and no context, so every
+// refusal can be reached without a device.
+#pragma once
+
+#include <cstdint>
+#include <cstdio>
+
+#include "../../include/anima.h"
+
+namespace anima {
+
+constexpr int64_t PREFIX_MAX_KEYS = 1 << 22;  // of the prefix and of a sequence, as anima_attention's Lk
+constexpr int64_t PREFIX_MAX_ROWS = 1 << 28;  // of all sequences
+constexpr int64_t PREFIX_MAX_LD = 1 << 20;    // floats between rows: 256 rows of a tile stay below 2^31 bytes
+constexpr int PREFIX_MAX_HEADS = 1 << 12;
+
+struct PrefixMsg {
+  char* buf;
+  size_t len;
+  template <class... A>
+  int operator()(int code, const char* fmt, A... args) const {
+    snprintf(buf, len, fmt, args...);
+    return code;
+  }
+  int operator()(int code, const char* text) const {
+    snprintf(buf, len, "%s", text);
+    return code;
+  }
+};
+
+// Bytes of a prefix's prepared K and V: rows in blocks of 64 (attention_kv_bytes of one batch element).
+inline int64_t prefix_kv_bytes(int Hkv, int P, int precision) {
+  return P < 1 ? 0 : 2 * (int64_t)Hkv * (((int64_t)P + 63) / 64 * 64) * 128 * (precision == ANIMA_PREC_BF16 ? 2 : 4);
+}
+
+// rows: the sum of the lengths; longest: the largest.
+inline int check_attention_prefix(const anima_prefix_attn_desc* d, int64_t* rows, int* longest, PrefixMsg fail) {
+  const char* const who = "anima_attention_prefix";
+  const auto al = [](const void* p, int b) { return ((uintptr_t)p & (uintptr_t)(b - 1)) == 0; };
+  *rows = 0;
+  *longest = 0;
+  if (!d) return fail(ANIMA_E_ARG, "%s: null descriptor", who);
+  const int group = d->group == 0 ? 1 : d->group;
+  if (d->D != 128) return fail(ANIMA_E_UNSUPPORTED, "%s: head dim %d (128)", who, d->D);
+  if (d->B < 0 || (d->B > 0 && !d->len)) return fail(ANIMA_E_ARG, "%s: B=%d, or null len", who, d->B);
+  if (d->H < 1 || group < 1 || d->H % group || d->H > PREFIX_MAX_HEADS)
+    return fail(ANIMA_E_ARG, "%s: H=%d heads in groups of %d (at most %d heads)", who, d->H, d->group, PREFIX_MAX_HEADS);
+  if (d->P < 0 || d->P > PREFIX_MAX_KEYS) return fail(ANIMA_E_ARG, "%s: P=%d outside [0, %lld]", who, d->P, (long long)PREFIX_MAX_KEYS);
+  if (d->precision != ANIMA_PREC_BF16 && d->precision != ANIMA_PREC_FP32) return fail(ANIMA_E_ARG, "%s: unknown precision %d", who, d->precision);
+  if (d->causal != 0 && d->causal != 1) return fail(ANIMA_E_ARG, "%s: causal=%d", who, d->causal);
+  if (d->o_bf16 != 0 && d->o_bf16 != 1) return fail(ANIMA_E_ARG, "%s: o_bf16=%d", who, d->o_bf16);
+  if (d->o_bf16 && d->precision != ANIMA_PREC_BF16) return fail(ANIMA_E_ARG, "%s: a bf16 O needs bf16 precision", who);
+  for (int b = 0; b < d->B; b++) {
+    if (d->len[b] < 0 || d->len[b] > PREFIX_MAX_KEYS)
+      return fail(ANIMA_E_ARG, "%s: len[%d]=%d outside [0, %lld]", who, b, d->len[b], (long long)PREFIX_MAX_KEYS);
+    *rows += d->len[b];
+    if (d->len[b] > *longest) *longest = d->len[b];
+    if (*rows > PREFIX_MAX_ROWS) return fail(ANIMA_E_UNSUPPORTED, "%s: more than %lld rows", who, (long long)PREFIX_MAX_ROWS);
+  }
+  if (*rows == 0) return ANIMA_OK;
+  if (!d->q || !d->k || !d->v || !d->o) return fail(ANIMA_E_ARG, "%s: null q/k/v/o", who);
+  const int64_t ld[4] = {d->ldq, d->ldk, d->ldv, d->ldo}, off[4] = {d->q_off, d->k_off, d->v_off, d->o_off};
+  const int heads[4] = {d->H, d->H / group, d->H / group, d->H};
+  const char* const nm[4] = {"q", "k", "v", "o"};
+  for (int i = 0; i < 4; i++) {
+    if (ld[i] % 4 || off[i] % 4 || off[i] < 0 || ld[i] < off[i] + (int64_t)heads[i] * 128)
+      return fail(ANIMA_E_ARG, "%s: %s rows of %lld elements (a multiple of 4) cannot hold off %lld + %d heads x 128", who, nm[i],
+                  (long long)ld[i], (long long)off[i], heads[i]);
+    if (ld[i] > PREFIX_MAX_LD) return fail(ANIMA_E_UNSUPPORTED, "%s: %s rows %lld apart (at most %lld)", who, nm[i], (long long)ld[i], (long long)PREFIX_MAX_LD);
+  }
+  if (!al(d->q, 16) || !al(d->k, 16) || !al(d->v, 16) || !al(d->o, d->o_bf16 ? 8 : 16) || !al(d->q_norm, 16) || !al(d->k_norm, 16) ||
+      !al(d->rope_cs, 16) || !al(d->prefix_kv, 16))
+    return fail(ANIMA_E_ARG, "%s: q/k/v/o, prefix_kv, norms and rope_cs on 16 bytes (a bf16 o on 8)", who);
+  if ((d->P > 0) != (d->prefix_kv != nullptr)) return fail(ANIMA_E_ARG, "%s: prefix_kv goes with P > 0 (P=%d)", who, d->P);
+  const int64_t want = prefix_kv_bytes(d->H / group, d->P, d->precision);
+  if (d->prefix_kv_bytes != want)
+    return fail(ANIMA_E_ARG, "%s: prefix_kv_bytes=%lld, but %d kv heads and P=%d at this precision take %lld", who,
+                (long long)d->prefix_kv_bytes, d->H / group, d->P, (long long)want);
+  if (d->rope_cs) {
+    const int64_t table = d->rope_sin_off / 64;
+    if (d->rope_sin_off <= 0 || d->rope_sin_off % 64 || table < (int64_t)d->P + *longest)
+      return fail(ANIMA_E_ARG, "%s: rope_sin_off=%lld must be rows*64 with rows >= P + longest = %lld", who, (long long)d->rope_sin_off,
+                  (long long)d->P + *longest);
+  }
+  if (!(d->eps >= 0.0f)) return fail(ANIMA_E_ARG, "%s: eps=%g", who, (double)d->eps);
+  return ANIMA_OK;
+}
+
+}  // namespace anima

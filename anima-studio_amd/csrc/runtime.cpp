@@ -672,6 +672,23 @@ int anima_weight_quant_f8(anima_ctx* c, const void* w, int w_bf16, int N, int K,
   return weight_quant_f8_launch(c, w, w_bf16, N, K, q, scale);
 }
 
+int anima_weight_quant_q4(anima_ctx* c, const void* w, int w_bf16, int N, int K, int group, uint8_t* q, uint16_t* scale,
+                          uint16_t* mid) {
+  CHECK_CTX(c);
+  return weight_quant_q4_launch(c, w, w_bf16, N, K, group, q, scale, mid);
+}
+
+int anima_embed_rows(anima_ctx* c, const anima_weight* table, const int32_t* ids, int64_t T, const float* weights, float scale,
+                     float* out, int64_t ldo) {
+  CHECK_CTX(c);
+  return embed_rows_launch(c, table, ids, T, weights, scale, out, ldo);
+}
+
+int anima_attention_prefix(anima_ctx* c, const anima_prefix_attn_desc* d) {
+  CHECK_CTX(c);
+  return attention_prefix_launch(c, d);
+}
+
 int anima_linear_glu(anima_ctx* c, const anima_glu_desc* d) {
   CHECK_CTX(c);
   return linear_glu_launch(c, d);
@@ -717,7 +734,8 @@ static const struct {
     ABI_FIELD(anima_attn_desc, kv_prep_bytes), ABI_FIELD(anima_attn_desc, q_prep), ABI_FIELD(anima_attn_desc, o_bf16),
     ABI_SIZE(anima_weight), ABI_FIELD(anima_weight, kind), ABI_FIELD(anima_weight, N), ABI_FIELD(anima_weight, K),
     ABI_FIELD(anima_weight, w), ABI_FIELD(anima_weight, scale), ABI_FIELD(anima_weight, srel),
-    ABI_FIELD(anima_weight, codebook), ABI_FIELD(anima_weight, bias),
+    ABI_FIELD(anima_weight, codebook), ABI_FIELD(anima_weight, bias), ABI_FIELD(anima_weight, group),
+    ABI_FIELD(anima_weight, group_scale), ABI_FIELD(anima_weight, group_mid),
     ABI_SIZE(anima_linear_desc), ABI_FIELD(anima_linear_desc, M), ABI_FIELD(anima_linear_desc, W),
     ABI_FIELD(anima_linear_desc, x), ABI_FIELD(anima_linear_desc, ldx), ABI_FIELD(anima_linear_desc, x_rotated),
     ABI_FIELD(anima_linear_desc, xq), ABI_FIELD(anima_linear_desc, xs), ABI_FIELD(anima_linear_desc, out),
@@ -758,6 +776,20 @@ static const struct {
     ABI_FIELD(anima_resnorm_desc, scale), ABI_FIELD(anima_resnorm_desc, mod_ld),
     ABI_FIELD(anima_resnorm_desc, group_rows), ABI_FIELD(anima_resnorm_desc, eps), ABI_FIELD(anima_resnorm_desc, h),
     ABI_FIELD(anima_resnorm_desc, ldh), ABI_FIELD(anima_resnorm_desc, q), ABI_FIELD(anima_resnorm_desc, s), ABI_FIELD(anima_resnorm_desc, y_bf16),
+    ABI_SIZE(anima_prefix_attn_desc), ABI_FIELD(anima_prefix_attn_desc, B), ABI_FIELD(anima_prefix_attn_desc, len),
+    ABI_FIELD(anima_prefix_attn_desc, P), ABI_FIELD(anima_prefix_attn_desc, H), ABI_FIELD(anima_prefix_attn_desc, D),
+    ABI_FIELD(anima_prefix_attn_desc, group), ABI_FIELD(anima_prefix_attn_desc, q),
+    ABI_FIELD(anima_prefix_attn_desc, ldq), ABI_FIELD(anima_prefix_attn_desc, q_off),
+    ABI_FIELD(anima_prefix_attn_desc, k), ABI_FIELD(anima_prefix_attn_desc, ldk),
+    ABI_FIELD(anima_prefix_attn_desc, k_off), ABI_FIELD(anima_prefix_attn_desc, v),
+    ABI_FIELD(anima_prefix_attn_desc, ldv), ABI_FIELD(anima_prefix_attn_desc, v_off),
+    ABI_FIELD(anima_prefix_attn_desc, o), ABI_FIELD(anima_prefix_attn_desc, ldo),
+    ABI_FIELD(anima_prefix_attn_desc, o_off), ABI_FIELD(anima_prefix_attn_desc, prefix_kv),
+    ABI_FIELD(anima_prefix_attn_desc, prefix_kv_bytes), ABI_FIELD(anima_prefix_attn_desc, scale),
+    ABI_FIELD(anima_prefix_attn_desc, causal), ABI_FIELD(anima_prefix_attn_desc, precision),
+    ABI_FIELD(anima_prefix_attn_desc, q_norm), ABI_FIELD(anima_prefix_attn_desc, k_norm),
+    ABI_FIELD(anima_prefix_attn_desc, rope_cs), ABI_FIELD(anima_prefix_attn_desc, rope_sin_off),
+    ABI_FIELD(anima_prefix_attn_desc, eps), ABI_FIELD(anima_prefix_attn_desc, o_bf16),
 };
 #undef ABI_FIELD
 #undef ABI_SIZE

@@ -106,7 +106,7 @@ int anima_timer_stop(anima_ctx* ctx, float* ms);
 /* ABI self-description, for bindings that restate the descriptor structs below (ctypes, FFI):
  * the byte offset of `field` in the struct named `type` -- "anima_attn_desc", "anima_linear_desc",
  * "anima_weight", "anima_sampler_desc", "anima_conv_desc", "anima_limits", "anima_qkv_desc",
- * "anima_glu_desc", "anima_resnorm_desc" -- or the struct's size when `field` is
+ * "anima_glu_desc", "anima_resnorm_desc", "anima_prefix_attn_desc" -- or the struct's size when `field` is
  * NULL; -1 for a name this library does not know.  No counterpart in the reference (its op layer
  * has no C ABI); it lets a binding refuse to load when its layout differs from the library's. */
 int64_t anima_abi_offset(const char* type, const char* field);
@@ -210,6 +210,46 @@ int64_t anima_attention_kv_bytes(int B, int Hkv, int Lk, int precision);
  * on different contexts / streams of the same GPU that overlap in time race on it (serialize them). */
 int anima_attention_noalloc(anima_ctx* ctx, const anima_attn_desc* desc);
 int64_t anima_attention_noalloc_scratch_bytes(void);
+
+/* Causal (or full) attention of B sequences behind one shared prefix: a batch of prompts whose leading
+ * tokens are the same, where those tokens' keys and values are computed once for all (under a causal mask
+ * they do not depend on what follows).  The sequences' rows are packed one behind the other, len[0] rows, then
+ * len[1] rows, ...; row i of a sequence stands at position P + i and sees the P prefix keys and the keys of its
+ * own sequence up to itself (causal = 0: all of them):
+ *   o[row] = softmax_j(scale * q[row] . k_j) v_j       j: prefix keys, own keys
+ * q, k, v, o as anima_attn_desc's, with the packed row for the row (no batch strides).  q / k RMSNorm and RoPE
+ * are fused as there, RoPE at the position.  The prefix's K and V come as anima_attention_prepare_kv
+ * (B = 1, Lk = P, the same precision) writes them, normed and rotated at 0 .. P - 1.  The reference encodes
+ * one prompt at a time (app/pipeline.js:192-211, the causal attention of app/models/qwen3.js:60).
+ * D = 128 (ANIMA_E_UNSUPPORTED otherwise).  A sequence of no rows is left out; P = 0: no prefix.  A key of a
+ * sequence with a NaN or an infinity in k or v makes the rows that see it NaN, and no others.  The scratch (the
+ * packed K and V, and partial sums) is the context's workspace. */
+typedef struct {
+  int B;
+  const int* len;        /* host array [B] of row counts >= 0 (read by the call) */
+  int P;
+  int H, D, group;       /* q heads, head dim (128), q heads per kv head (0 -> 1) */
+  const float* q;
+  int64_t ldq, q_off;
+  const float* k;
+  int64_t ldk, k_off;
+  const float* v;
+  int64_t ldv, v_off;
+  float* o;
+  int64_t ldo, o_off;
+  const void* prefix_kv; /* NULL with P = 0; 16-byte aligned */
+  int64_t prefix_kv_bytes; /* anima_attention_kv_bytes(1, H / group, P, precision) */
+  float scale;           /* 0 -> 1/sqrt(D) */
+  int causal;
+  int precision;         /* ANIMA_PREC_* */
+  const float* q_norm;   /* [128] or NULL */
+  const float* k_norm;
+  const float* rope_cs;  /* cos block [rows][64] then sin block at rope_sin_off, rows >= P + longest, or NULL */
+  int64_t rope_sin_off;
+  float eps;
+  int o_bf16;            /* 1: O as bf16 rows (bf16 precision only; as anima_attn_desc) */
+} anima_prefix_attn_desc;
+int anima_attention_prefix(anima_ctx* ctx, const anima_prefix_attn_desc* desc);
 
 /* ---------------------------------------------------------------- row ops */
 
@@ -376,6 +416,10 @@ int anima_to_rgba(anima_ctx* ctx, const float* x, int64_t n, uint8_t* out);
 #define ANIMA_W_F8 5 /* e4m3 [N][K] + scale [ceil(N/128)][ceil(K/128)], one for each 128 x 128 block; the
                         activations are e4m3 rows with one scale per 128 columns (anima_quant_rows_f8).
                         K % 16 == 0.  No reference counterpart (its loader knows comfy_quant formats only) */
+#define ANIMA_W_Q4 6 /* 4-bit codes [N][K/2] (low nibble = even k) in groups of `group` along k (32, 64 or
+                        128; K % group == 0), each with a bf16 scale and, optionally, a bf16 middle value:
+                        w[n][k] = group_scale[n][k/group] * (code - 8) (+ group_mid[n][k/group]).  fp32
+                        activations.  No reference counterpart (anima_weight_quant_q4 converts bf16 weights) */
 #define ANIMA_ACT_NONE 0
 #define ANIMA_ACT_GELU 1 /* erf GELU (kernels.js:9-20) */
 #define ANIMA_ACT_SILU 2
@@ -391,6 +435,9 @@ typedef struct {
   const uint8_t* srel;     /* w4: [N][K/16] fp8 e4m3 */
   const float* codebook;   /* w4: [16] */
   const float* bias;       /* [N] or NULL */
+  int group;                   /* q4: 32, 64 or 128 (the q4 fields are not read for other kinds) */
+  const uint16_t* group_scale; /* q4: bf16 [N][K/group] */
+  const uint16_t* group_mid;   /* q4: bf16 [N][K/group] or NULL (0) */
 } anima_weight;
 
 typedef struct {
@@ -437,10 +484,11 @@ typedef struct {
   const uint16_t* lora_b;
   int lora_r;
   int lora_cols;
-  /* f8 weights only (0 otherwise).  precision: ANIMA_PREC_BF16 lets the 8-bit matrix instructions add the
-   * products, which keep 2^-13 of the largest of each eight (about 1.5e-5 of the result, far below a bf16
-   * rounding); ANIMA_PREC_FP32 adds them in 32 bits, at the rate of bf16 products.  out_bf16 = 1: out is
-   * bf16 rows (round to nearest even; out and ldc then address uint16 elements), store epilogue only. */
+  /* f8 and q4 weights only (0 otherwise).  precision, f8: ANIMA_PREC_BF16 lets the 8-bit matrix instructions
+   * add the products, which keep 2^-13 of the largest of each eight (about 1.5e-5 of the result, far below a
+   * bf16 rounding); ANIMA_PREC_FP32 adds them in 32 bits, at the rate of bf16 products.  q4: ANIMA_PREC_BF16
+   * may round the activations to 11 bits (2^-12 of each) first, ANIMA_PREC_FP32 keeps them.  out_bf16 = 1: out
+   * is bf16 rows (round to nearest even; out and ldc then address uint16 elements), store epilogue only. */
   int precision;
   int out_bf16;
 } anima_linear_desc;
@@ -456,7 +504,11 @@ typedef struct {
  * product's kernel, more in a pass before it (pooled scratch); few tiles of a long k are split over k, with the
  * splits' sums in pooled scratch.  The order in which a result's blocks are
  * added, and so its last bits, depends on the sizes.  No acc_out and no LoRA factors (`add` carries a
- * delta). */
+ * delta).
+ * q4: r = alpha * sum_k x[m][k] w[n][k] of fp32 rows x (16-byte aligned, ldx % 4 == 0), with the products of
+ * 32-bit accuracy or, on more than a few rows and with ANIMA_PREC_BF16, of x rounded to 11 bits.  A row of x
+ * with an infinity or a NaN gives a row of NaN.  M and N up to 2^29, K up to 2^20; as f8 in the rest (pooled
+ * scratch, the order of sums by the sizes, no acc_out and no LoRA factors). */
 int anima_linear(anima_ctx* ctx, const anima_linear_desc* desc);
 
 /* The stacked QKV projection of a DiT block with the attention's operand preparation in its
@@ -532,6 +584,29 @@ int anima_quant_rows_f8(anima_ctx* ctx, const void* x, int x_bf16, int64_t M, in
  * of an ANIMA_W_F8 weight, one scale per 128 x 128 block (fewer than 2^24 blocks): a loader's conversion of a
  * bf16 checkpoint. */
 int anima_weight_quant_f8(anima_ctx* ctx, const void* w, int w_bf16, int N, int K, uint8_t* q, float* scale);
+
+/* ---------------------------------------------------------------- 4-bit weights, embedding rows
+ * No reference counterpart. */
+
+/* A weight w[N][K] (fp32, or bf16 with w_bf16 = 1) to the codes q[N][K/2], scales and, where mid is given,
+ * middle values [N][K/group] of an ANIMA_W_Q4 weight: a loader's conversion of a bf16 checkpoint.  For each
+ * group, in fp32 with every step rounded to nearest even:
+ *   without mid  s = bf16(max|w| / 7)
+ *   with mid     s = bf16((max - min) / 15),  z = bf16(fma(8, s, min))
+ *   code = clamp(rint((w - z) / s), -8, 7) + 8     (s = 0: 8)
+ * A NaN or an infinity in a group makes its scale (and middle) no number or infinite.  w and q on 16 bytes;
+ * fewer than 2^34 weights. */
+int anima_weight_quant_q4(anima_ctx* ctx, const void* w, int w_bf16, int N, int K, int group, uint8_t* q, uint16_t* scale,
+                          uint16_t* mid);
+
+/* Rows of an embedding table, scaled: out[t][:] = (scale * weights[t]) * table[ids[t]][:] for t < T, fp32
+ * rows ldo apart (0 -> K); without weights times scale (0 -> 1).  The table is a weight object of kind
+ * ANIMA_W_F32, ANIMA_W_BF16 or ANIMA_W_Q4 with N rows of K values (bias not read).  ids: T indexes on the
+ * device; one outside [0, N) gives a row of zeros (padding: -1).  The encoders read the rows on the host
+ * (app/models/qwen3.js:40-44) and scale prompt weights there (app/models/dit.js:181-188).
+ * K % 4 == 0; out on 16 bytes, the table's rows on 4 elements (Q4: 16 bytes), ldo % 4 == 0. */
+int anima_embed_rows(anima_ctx* ctx, const anima_weight* table, const int32_t* ids, int64_t T, const float* weights,
+                     float scale, float* out, int64_t ldo);
 
 /* The first half of a gated feed-forward block (the gate / up linears and the silu_mul of
  * app/models/qwen3.js:66-72) in one kernel:
