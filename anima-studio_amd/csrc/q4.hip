@@ -5,6 +5,7 @@
 // s (code - 8) has at most 11 significant bits (8 of s, 3 of 1 .. 7, and 8 is a power of two), so it is exact in fp32,
 // and w is one rounding away from it.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "internal.h"
@@ -196,6 +197,374 @@ __global__ __launch_bounds__(256) void q4_rows_kernel(Q4Args a) {
   }
 }
 
+// ------------------------------------------------------------------ products of many rows
+//
+// On the f16 matrix cores.  A row of x, times a power of two that brings its largest value to 2^14 .. 2^15, is the sum of
+// two f16 terms to 2^-23 of each value (or 2^-40 of the largest); ANIMA_PREC_BF16 keeps the first term, 11 bits.
+// s (c - 8), times a power of two for the whole column, is one f16 value: exact where it is above 2^-39 of the column's
+// largest.  Both powers come off the sums at the end, so the k loop has nothing but matrix products and the codes'
+// decode.  The middles' part, sum_g z[n][g] (sum of x over group g), is a small fp32 product of its own.
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// 2^e as a float, e from -126 to 127
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// The exponent that brings a largest magnitude to [2^top, 2^(top + 1)); 0 for zeros, infinities and NaN.
+__device__ __forceinline__ int q4_exp(float amax, int top) {
+  const int b = (int)(__float_as_uint(amax) >> 23);
+  return amax == 0.0f || b == 255 ? 0 : min(top + 127 - b, 120);
+}
+
+struct Q4Prep {
+  const float* x;
+  int64_t ldx;
+  _Float16* xh;   // [M][Kp], each eight values in the order k 0 4 1 5 2 6 3 7 (the decode's), zeros from K on
+  _Float16* xl;   // the second terms, or NULL
+  float* rm;      // [M] what x's power comes off with
+  float* sx;      // [M][K/G] group sums of x, or NULL
+  const uint16_t* gs;
+  float* rn;      // [N] what the column's power comes off with
+  int M, N, K, Kp, G, rows;  // rows: workgroups of x rows (four each), the rest are of columns
+};
+
+// A wave per row of x, or per column's scales.  Two passes over the row, the second from the caches.
+__global__ __launch_bounds__(256) void q4_prep_kernel(Q4Prep a) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if ((int)blockIdx.x >= a.rows) {
+    const int64_t n = (int64_t)(blockIdx.x - a.rows) * 4 + wave;
+    if (n >= a.N) return;
+    const int KG = a.K / a.G;
+    float m = 0.0f;
+    for (int g = lane; g < KG; g += 64) m = fmaxf(m, fabsf(bf16_f(a.gs[n * KG + g])));
+    m = wave_max(m);
+    if (lane == 0) a.rn[n] = pow2f(-q4_exp(m, 11));
+    return;
+  }
+  const int64_t m = (int64_t)blockIdx.x * 4 + wave;
+  if (m >= a.M) return;
+  const float* x = a.x + m * a.ldx;
+  float mx = 0.0f;
+  for (int k = 4 * lane; k < a.K; k += 256) {
+    const f32x4 v = *(const f32x4*)(x + k);
+#pragma unroll
+    for (int j = 0; j < 4; j++) mx = fmaxf(mx, fabsf(v[j]));
+  }
+  mx = wave_max(mx);
+  const int e = q4_exp(mx, 14);
+  const float f = pow2f(e);
+  if (lane == 0) a.rm[m] = pow2f(-e);
+  for (int k = 8 * lane; k < a.Kp; k += 512) {
+    float v[8] = {};
+    if (k < a.K) ld8(x + k, v);
+    if (a.sx) {
+      float t = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+      for (int s = 1; s < a.G / 8; s <<= 1) t += __shfl_xor(t, s);
+      if (k < a.K && k % a.G == 0) a.sx[m * (a.K / a.G) + k / a.G] = t;
+    }
+    f16x8 h, l;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const float y = v[j] * f;
+      const int o = 2 * (j & 3) + (j >> 2);
+      h[o] = (_Float16)y;
+      l[o] = (_Float16)(y - (float)h[o]);
+    }
+    *(f16x8*)(a.xh + m * a.Kp + k) = h;
+    if (a.xl) *(f16x8*)(a.xl + m * a.Kp + k) = l;
+  }
+}
+
+// Eight codes, times the scale pair, in the order 0 4 1 5 2 6 3 7: 1024 + c by its bits, less 1032 (exact), times s.
+__device__ __forceinline__ f16x8 q4_decode(uint32_t c, f16x2 s) {
+  const f16x2 off = {(_Float16)-1032.0f, (_Float16)-1032.0f};
+  f16x8 r;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const f16x2 v = (__builtin_bit_cast(f16x2, ((c >> (4 * i)) & 0x000f000fu) | 0x64006400u) + off) * s;
+    r[2 * i] = v[0];
+    r[2 * i + 1] = v[1];
+  }
+  return r;
+}
+
+typedef __attribute__((address_space(3))) void q4_lds_t;
+#define Q4_WAIT_VM(n) __builtin_amdgcn_s_waitcnt(((n) & 15) | (7 << 4) | (15 << 8) | (((n) >> 4) << 14))
+
+__device__ __forceinline__ void q4_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t q4_rsrc(const void* p, int64_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, (short)0, (int)bytes, 0x00020000);
+}
+
+// a wave's copy of 64 x 16 bytes into LDS
+__device__ __forceinline__ void q4_copy16(__amdgpu_buffer_rsrc_t rs, char* dst, uint32_t off, uint32_t step) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (q4_lds_t*)dst, 16, off, step, 0, 0);
+}
+
+struct Q4Tile {
+  Q4Args a;
+  const _Float16* xh;
+  const _Float16* xl;
+  const float* rm;
+  const float* rn;   // (readable to the next multiple of 256 columns)
+  const float* sx;
+  float* part;       // [splits][M][N] sums of a product split over k, or NULL
+  int Kp, sps;       // k padded; steps of 64 k in a split
+  int vec;           // rows of out, bias, add and gate in quads of 16 bytes
+};
+
+// Four columns of a row: + bias and add, the activation, and out's epilogue.
+__device__ __forceinline__ void q4_store4(const Q4Args& a, int vec, int64_t m, int n, f32x4 r) {
+  if (!vec) {
+    for (int i = 0; i < 4; i++)
+      if (n + i < a.N) q4_store(a, m, n + i, r[i]);
+    return;
+  }
+  r = r * a.alpha;
+  if (a.bias) r = r + *(const f32x4*)(a.bias + n);
+  if (a.add) r = r + *(const f32x4*)(a.add + m * a.ld_add + n);
+  if (a.act != ANIMA_ACT_NONE) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) r[i] = q4_act(r[i], a.act);
+  }
+  if (a.obf) {
+    *(bf16x4*)((bf16*)a.out + m * a.ldc + n) = bf16x4{to_bf16(r[0]), to_bf16(r[1]), to_bf16(r[2]), to_bf16(r[3])};
+    return;
+  }
+  f32x4* c = (f32x4*)((float*)a.out + m * a.ldc + n);
+  if (a.epi == ANIMA_EPI_RESID) {
+    r = *c + r;
+  } else if (a.epi == ANIMA_EPI_GATED) {
+    const f32x4 g = *(const f32x4*)(a.gate + n), o = *c;
+#pragma unroll
+    for (int i = 0; i < 4; i++) r[i] = __builtin_fmaf(g[i], r[i], o[i]);
+  }
+  *c = r;
+}
+
+// One BM x BN tile a workgroup, waves of WM rows x WN columns.  A step is 64 k: BM rows of x (128 bytes, each term) in one of four LDS
+// stages, filled three steps ahead by buffer_load ... lds, units of 16 bytes at slot u ^ (row / 2 % 8) (sixteen rows' reads of one
+// unit touch each bank once).  The codes go straight to registers, four steps ahead: lane (n, half) takes the 16 bytes of
+// column n's 32 k of its half, so that matrix step i of a lane pair covers k 8 i .. 8 i + 7 of both halves; x's units follow.
+constexpr int q4_waves(int BM, int BN, int WM, int WN, int TERMS) {  // waves a SIMD that a tile's LDS leaves room for
+  return (BM / WM) * (BN / WN) < 8 && TERMS * BM * 128 * 4 > 81920 ? 1 : 2;
+}
+template <int BM, int BN, int WM, int WN, int TERMS>
+__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), q4_waves(BM, BN, WM, WN, TERMS)) void q4_tile_kernel(Q4Tile t) {
+  constexpr int NWM = BM / WM, NW = NWM * (BN / WN), MT = WM / 32, NT = WN / 32, NST = 4;
+  constexpr int XB = BM * 128, SB = XB * TERMS, CPW = TERMS * BM / 8 / NW;
+  static_assert(CPW * NW * 8 == TERMS * BM, "whole copies");
+  constexpr int RS = WN + 4, EPL = NW * 32 * RS * 4;
+  constexpr int LDS = NST * SB > EPL ? NST * SB : EPL;
+  __shared__ __attribute__((aligned(1024))) char smem[LDS];
+  const Q4Args& a = t.a;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 31, hf = lane >> 5;
+  const int ntn = (a.N + BN - 1) / BN, ntm = (a.M + BM - 1) / BM;
+  int tm, tn;
+  {
+    // XCD x takes a contiguous range of tiles, in groups of 8 row tiles, column-major inside a group
+    const int total = ntn * ntm, q = total >> 3, rem = total & 7, x = blockIdx.x & 7;
+    const int i = x * q + min(x, rem) + (int)(blockIdx.x >> 3);
+    const int grp = i / (8 * ntn), row0 = 8 * grp, gm = min(8, ntm - row0), local = i - grp * 8 * ntn;
+    tn = local / gm;
+    tm = row0 + (local - tn * gm);
+  }
+  const int bm = tm * BM, bn = tn * BN, K = a.K, KG = K / a.G;
+  const int wm = (wave % NWM) * WM, wn = (wave / NWM) * WN;
+  const int s0 = blockIdx.y * t.sps, steps = min(t.sps, t.Kp / 64 - s0);
+
+  const int mrows = min(BM, a.M - bm);
+  const __amdgpu_buffer_rsrc_t rh = q4_rsrc(t.xh + (int64_t)bm * t.Kp, (int64_t)mrows * t.Kp * 2),
+                               rl = q4_rsrc((TERMS > 1 ? t.xl : t.xh) + (int64_t)bm * t.Kp, (int64_t)mrows * t.Kp * 2);
+  // copy c of this wave: eight rows of a term
+  uint32_t xo[CPW];
+#pragma unroll
+  for (int c = 0; c < CPW; c++) {
+    const int row = (8 * (wave * CPW + c)) % BM + (lane >> 3);
+    xo[c] = (uint32_t)row * (uint32_t)(t.Kp * 2) + 16 * ((lane & 7) ^ ((row >> 1) & 7)) + 128 * s0;
+  }
+  const auto copies = [&](int step, int p) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < CPW; c++)
+      q4_copy16(TERMS > 1 && wave * CPW + c >= BM / 8 ? rl : rh, smem + p * SB + (wave * CPW + c) * 1024, xo[c], 128 * step);
+  };
+  // columns of this wave's tiles (past the last: the last, whose sums are not stored)
+  const uint8_t* wrow[NT];
+  const uint16_t* srow[NT];
+  float fn[NT];
+#pragma unroll
+  for (int j = 0; j < NT; j++) {
+    const int64_t n = min(bn + wn + 32 * j + r, a.N - 1);
+    wrow[j] = a.w + n * (K / 2);
+    srow[j] = a.gs + n * KG;
+    fn[j] = 1.0f / t.rn[n];
+  }
+  u32x4 wr[2][NT];
+  uint16_t sc[2][NT];
+  const int lg = 31 - __builtin_clz(a.G);
+  const auto codes = [&](int step, int u) __attribute__((always_inline)) {
+    const int k = min(64 * (s0 + step) + 32 * hf, K - 32);  // (past the row's end its last 32: they meet zeros of x)
+#pragma unroll
+    for (int j = 0; j < NT; j++) {
+      wr[u][j] = *(const u32x4*)(wrow[j] + k / 2);
+      sc[u][j] = srow[j][k >> lg];
+    }
+  };
+  f32x16 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; i++)
+#pragma unroll
+    for (int j = 0; j < NT; j++) acc[i][j] = f32x16{};
+  int xa[4];  // unit 4 hf + i of row r
+#pragma unroll
+  for (int i = 0; i < 4; i++) xa[i] = (wm + r) * 128 + 16 * ((4 * hf + i) ^ ((r >> 1) & 7));
+
+  // Fragments of matrix step i + 1 are read and decoded under step i's products.  Before the last of a stage's four, whose
+  // fragments are in registers by then, a barrier ends every wave's reads of the stage (its buffer is refilled) and publishes
+  // the next one: this wave's copies of it have arrived when at most the loads of the two turns after it pend.
+  f16x8 xf[2][MT][TERMS], wf[2][NT];
+  f16x2 sv[NT];
+  const auto xread = [&](int u, int p, int i) __attribute__((always_inline)) {
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+      for (int e = 0; e < TERMS; e++) xf[u][m][e] = *(const f16x8*)(smem + p * SB + e * XB + m * 4096 + xa[i]);
+  };
+  const auto decode = [&](int u, int b, int i) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < NT; j++) {
+      if (i == 0) {
+        const _Float16 v = (_Float16)(bf16_f(sc[b][j]) * fn[j]);
+        sv[j] = f16x2{v, v};
+      }
+      wf[u][j] = q4_decode(wr[b][j][i], sv[j]);
+    }
+  };
+#pragma unroll
+  for (int p = 0; p < NST; p++) {
+    copies(p, p);
+    if (p < 2) codes(p, p);
+  }
+  Q4_WAIT_VM((NST - 1) * CPW);
+  q4_barrier();
+  xread(0, 0, 0);
+  decode(0, 0, 0);
+  const auto stage = [&](int step, auto buffer) __attribute__((always_inline)) {
+    constexpr int p = decltype(buffer)::value, pn = (p + 1) % NST, b = p & 1;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int u = i & 1;
+      if (i == 3) {
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+        Q4_WAIT_VM(2 * (CPW + 2 * NT));
+        q4_barrier();
+        copies(step + NST, p);
+        xread(u ^ 1, pn, 0);
+        decode(u ^ 1, b ^ 1, 0);
+        codes(step + 2, b);
+      } else {
+        xread(u ^ 1, p, i + 1);
+        decode(u ^ 1, b, i + 1);
+      }
+#pragma unroll
+      for (int e = TERMS - 1; e >= 0; e--)
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+          for (int j = 0; j < NT; j++) acc[m][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(wf[u][j], xf[u][m][e], acc[m][j], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  int s = 0;
+  for (; s + NST <= steps; s += NST) {
+    stage(s, std::integral_constant<int, 0>{});
+    stage(s + 1, std::integral_constant<int, 1>{});
+    stage(s + 2, std::integral_constant<int, 2>{});
+    stage(s + 3, std::integral_constant<int, 3>{});
+  }
+  if (s < steps) stage(s, std::integral_constant<int, 0>{});
+  if (s + 1 < steps) stage(s + 1, std::integral_constant<int, 1>{});
+  if (s + 2 < steps) stage(s + 2, std::integral_constant<int, 2>{});
+  Q4_WAIT_VM(0);  // no copy into LDS outlives the loop
+  q4_barrier();
+
+  // Rows leave through LDS, 32 rows of a wave at a time, so that neighbouring lanes hold 16 bytes of one row each.
+  float* rows = (float*)smem + wave * 32 * RS;
+  constexpr int LR = WN / 4, PR = 64 / LR;
+  const int n0 = bn + wn;
+  const bool zero = a.gz && blockIdx.y == 0;  // (the middles' part goes with the first split)
+#pragma unroll
+  for (int i = 0; i < MT; i++) {
+    const int m = bm + wm + 32 * i + r, mc = min(m, a.M - 1);
+    const float fm = t.rm[mc];
+#pragma unroll
+    for (int j = 0; j < NT; j++) {
+      f32x16 z = {};
+      if (zero) {
+        const uint16_t* zr = a.gz + (int64_t)min(n0 + 32 * j + r, a.N - 1) * KG;
+        const float* xr = t.sx + (int64_t)mc * KG;
+        for (int g = hf; g < KG + hf; g += 2) {  // (an odd last group: zeros in the other half)
+          const bool in = g < KG;
+          z = __builtin_amdgcn_mfma_f32_32x32x2f32(in ? bf16_f(zr[min(g, KG - 1)]) : 0.0f, in ? xr[min(g, KG - 1)] : 0.0f, z, 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        const f32x4 f = *(const f32x4*)(t.rn + n0 + 32 * j + 8 * q + 4 * hf);
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = acc[i][j][4 * q + e] * f[e] * fm + z[4 * q + e];
+        *(f32x4*)(rows + r * RS + 32 * j + 8 * q + 4 * hf) = v;
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 4
+    for (int q = 0; q < 32; q += PR) {
+      const int row = q + lane / LR, n = n0 + 4 * (lane % LR);
+      const f32x4 v = *(const f32x4*)(rows + row * RS + 4 * (lane % LR));
+      const int64_t mo = bm + wm + 32 * i + row;
+      if (mo < a.M && n < a.N) {
+        if (t.part) {
+          float* o = t.part + ((int64_t)blockIdx.y * a.M + mo) * a.N + n;
+          if (t.vec) *(f32x4*)o = v;
+          else
+            for (int e = 0; e < 4; e++)
+              if (n + e < a.N) o[e] = v[e];
+        } else {
+          q4_store4(a, t.vec, mo, n, v);
+        }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// A split product's sums, added in order, and the epilogue.
+constexpr int Q4_SPLITS = 16;
+__global__ __launch_bounds__(256) void q4_join_kernel(Q4Tile t, int splits) {
+  const Q4Args& a = t.a;
+  const int64_t quads = (a.N + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / quads;
+  if (m >= a.M) return;
+  const int n = (int)(4 * (i - m * quads));
+  const float* p = t.part + m * a.N + n;
+  const int64_t plane = (int64_t)a.M * a.N;
+  f32x4 v = {};
+  for (int s = 0; s < splits; s++) {
+    if (t.vec) v = v + *(const f32x4*)(p + s * plane);
+    else
+      for (int e = 0; e < 4; e++)
+        if (n + e < a.N) v[e] += p[s * plane + e];
+  }
+  q4_store4(a, t.vec, m, n, v);
+}
+
 // ------------------------------------------------------------------ host
 
 namespace {
@@ -238,6 +607,69 @@ int embed_rows_launch(anima_ctx* c, const anima_weight* W, const int32_t* ids, i
   return L.end();
 }
 
+constexpr int Q4_FEW = 8;
+
+template <int BM, int BN, int WM, int WN, int TERMS>
+static void q4_tile_launch(anima_ctx* c, const Q4Tile& t, int splits) {
+  const dim3 grid((unsigned)(((t.a.N + BN - 1) / BN) * ((t.a.M + BM - 1) / BM)), (unsigned)splits), block(64 * (BM / WM) * (BN / WN));
+  hipLaunchKernelGGL((q4_tile_kernel<BM, BN, WM, WN, TERMS>), grid, block, 0, c->stream, t);
+}
+
+// x into f16 terms and both sides' powers, then the tiles, then, where k was split, the sums.
+static int q4_tiles(anima_ctx* c, const Q4Args& a, bool two) {
+  Q4Tile t{};
+  t.a = a;
+  t.Kp = (a.K + 63) / 64 * 64;
+  const int KG = a.K / a.G, steps = t.Kp / 64;
+  const auto tiles = [&](int bm, int bn) { return (int64_t)((a.M + bm - 1) / bm) * ((a.N + bn - 1) / bn); };
+  // the largest tile of which there are enough
+  const int tile = tiles(two ? 128 : 256, 256) >= c->num_cus ? 0 : tiles(128, 128) >= c->num_cus ? 1 : 2;
+  const int64_t nt = tile == 0 ? tiles(two ? 128 : 256, 256) : tile == 1 ? tiles(128, 128) : tiles(64, 64);
+  int splits = 1;
+  while (splits < Q4_SPLITS && nt * splits * 2 <= c->num_cus && steps / (splits * 2) >= 4) splits *= 2;
+  t.sps = (steps + splits - 1) / splits;
+  splits = (steps + t.sps - 1) / t.sps;
+  const auto al = [](const void* p, int b) { return ((uintptr_t)p & (uintptr_t)(b - 1)) == 0; };
+  t.vec = a.N % 4 == 0 && a.ldc % 4 == 0 && al(a.out, a.obf ? 8 : 16) && al(a.bias, 16) && al(a.gate, 16) &&
+          (!a.add || (al(a.add, 16) && a.ld_add % 4 == 0));
+  // scratch: the terms, the powers, the group sums, the splits' sums
+  size_t at = 0;
+  const auto take = [&](size_t bytes) {
+    const size_t o = at;
+    at += (bytes + 255) / 256 * 256;
+    return o;
+  };
+  const size_t plane = (size_t)a.M * t.Kp * 2, oh = take(plane), ol = two ? take(plane) : 0, om = take((size_t)a.M * 4),
+               on = take(((size_t)a.N + 255) / 256 * 1024), os = a.gz ? take((size_t)a.M * KG * 4) : 0,
+               op = splits > 1 ? take((size_t)splits * a.M * a.N * 4) : 0;
+  void* tmp = nullptr;
+  if (int rc = anima_alloc(c, at, &tmp)) return rc;
+  char* const b = (char*)tmp;
+  t.xh = (_Float16*)(b + oh);
+  t.xl = two ? (_Float16*)(b + ol) : nullptr;
+  t.rm = (float*)(b + om);
+  t.rn = (float*)(b + on);
+  t.sx = a.gz ? (float*)(b + os) : nullptr;
+  t.part = splits > 1 ? (float*)(b + op) : nullptr;
+  Q4Prep p{a.x, a.ldx, (_Float16*)t.xh, (_Float16*)t.xl, (float*)t.rm, (float*)t.sx, a.gs, (float*)t.rn, a.M, a.N, a.K, t.Kp, a.G, (a.M + 3) / 4};
+  Launch L(c, tile == 0 ? "gemm.q4.256" : tile == 1 ? "gemm.q4.128" : "gemm.q4.64", 2.0 * a.M * a.N * a.K, 0.0);
+  hipLaunchKernelGGL(q4_prep_kernel, dim3((unsigned)(p.rows + (a.N + 3) / 4)), dim3(256), 0, c->stream, p);
+  if (two) {
+    if (tile == 0) q4_tile_launch<128, 256, 64, 64, 2>(c, t, splits);
+    else if (tile == 1) q4_tile_launch<128, 128, 64, 64, 2>(c, t, splits);
+    else q4_tile_launch<64, 64, 32, 32, 2>(c, t, splits);
+  } else {
+    if (tile == 0) q4_tile_launch<256, 256, 128, 64, 1>(c, t, splits);
+    else if (tile == 1) q4_tile_launch<128, 128, 64, 64, 1>(c, t, splits);
+    else q4_tile_launch<64, 64, 32, 32, 1>(c, t, splits);
+  }
+  if (splits > 1)
+    hipLaunchKernelGGL(q4_join_kernel, dim3((unsigned)(((int64_t)a.M * ((a.N + 3) / 4) + 255) / 256)), dim3(256), 0, c->stream, t, splits);
+  const int rc = L.end();
+  anima_free(c, tmp);
+  return rc;
+}
+
 int linear_q4_launch(anima_ctx* c, const anima_linear_desc* d) {
   char msg[256];
   if (int rc = check_linear_q4(d, Q4Msg{msg, sizeof msg})) return refused(c, rc, msg);
@@ -246,6 +678,7 @@ int linear_q4_launch(anima_ctx* c, const anima_linear_desc* d) {
   Q4Args a{d->x, d->ldx ? d->ldx : W->K, (const uint8_t*)W->w, W->group_scale, W->group_mid, W->bias, d->out, d->ldc ? d->ldc : W->N,
            d->alpha != 0.0f ? d->alpha : 1.0f, d->act, d->epilogue, d->epilogue == ANIMA_EPI_GATED ? d->gate + d->gate_off : nullptr, d->add,
            d->ld_add ? d->ld_add : W->N, (int)d->M, W->N, W->K, W->group, d->out_bf16};
+  if (a.M > Q4_FEW) return q4_tiles(c, a, d->precision == ANIMA_PREC_FP32);
   Launch L(c, "gemv.q4", 2.0 * a.M * a.N * a.K, 0.5 * a.N * a.K);
   constexpr int PART = 65535 * 4;  // (rows of a launch's grid)
   const int M = a.M;
