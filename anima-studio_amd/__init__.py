@@ -237,6 +237,7 @@ def lib():
         L.anima_weight_quant_q4.argtypes = [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp, _vp]
         L.anima_embed_rows.argtypes = [_vp, _vp, _vp, _i64, _vp, ctypes.c_float, _vp, _i64]
         L.anima_attention_prefix.argtypes = [_vp, P(PrefixAttnDesc)]
+        L.anima_attention_prefix_prepare.argtypes = [_vp, _vp, _vp, _i64]
         L.anima_linear_glu.argtypes = [_vp, P(GluDesc)]
         L.anima_residual_norm.argtypes = [_vp, P(ResNormDesc)]
         for n in ("anima_linear", "anima_linear_glu", "anima_residual_norm", "anima_attention_prefix"):  # with a packed descriptor (bytes)
@@ -549,20 +550,24 @@ class Context:
         return self._check(lib().anima_embed_rows(self.h, _weight_adr(table), _ptr(ids), T, _ptr(weights), scale, _ptr(out),
                                                   ldo))
 
-    def attention_prefix(self, *, q, k, v, o, lens, H, D=128, ldq, ldk, ldv, ldo=None, q_off=0, k_off=0, v_off=0, o_off=0,
-                         group=1, P=0, prefix_kv=None, prefix_kv_bytes=None, scale=0.0, causal=1, precision=PREC_BF16,
-                         q_norm=None, k_norm=None, rope_cs=None, rope_sin_off=0, eps=1e-6, o_bf16=False):
-        """anima_attention_prefix: packed sequences of lens[b] rows, each behind the same P keys, which
-        attention(B=1, Lk=P, prepare_into=prefix_kv) has prepared.  prefix_kv_bytes defaults to the size that P,
-        the heads and the precision take."""
+    def attention_prefix(self, *, k, v, lens, H, ldk, ldv, q=None, o=None, D=128, ldq=0, ldo=None, q_off=0, k_off=0, v_off=0,
+                         o_off=0, group=1, P=0, prefix_kv=None, prefix_kv_bytes=None, scale=0.0, causal=1,
+                         precision=PREC_BF16, q_norm=None, k_norm=None, rope_cs=None, rope_sin_off=0, eps=1e-6,
+                         o_bf16=False, prepare_into=None):
+        """anima_attention_prefix: packed sequences of lens[b] rows, each behind the same P keys prefix_kv, which a call
+        with prepare_into has prepared (anima_attention_prefix_prepare, of the one sequence lens[0]; q and o are not
+        read).  prefix_kv_bytes defaults to the size that the keys, the heads and the precision take."""
         if not (isinstance(lens, np.ndarray) and lens.dtype == np.int32 and lens.ndim == 1 and lens.flags.c_contiguous):
             lens = np.array([operator.index(n) for n in lens], np.int32)
+        keys = P if prepare_into is None else int(lens[0]) if lens.size else 0
         if prefix_kv_bytes is None:
-            prefix_kv_bytes = self.attention_kv_bytes(1, H // max(group, 1), P, precision) if P > 0 else 0
+            prefix_kv_bytes = self.attention_kv_bytes(1, H // max(group, 1), keys, precision) if keys > 0 else 0
         d = _prefix_attn_desc(lens.size, lens.ctypes.data, P, H, D, group, _adr(q), ldq, q_off, _adr(k), ldk, k_off, _adr(v),
                               ldv, v_off, _adr(o), ldo if ldo is not None else H * D, o_off, _adr(prefix_kv), prefix_kv_bytes,
                               scale, causal, precision, _adr(q_norm), _adr(k_norm), _adr(rope_cs), rope_sin_off, eps,
                               int(o_bf16))
+        if prepare_into is not None:
+            return self._check(lib().anima_attention_prefix_prepare(self.h, d, _ptr(prepare_into), prefix_kv_bytes))
         return self._check(lib().anima_attention_prefix_packed(self.h, d))
 
     def linear_glu(self, gate, up, M, *, x=None, xq=None, xs=None, ldx=0, act="silu", out=None, ldc=0, out_q=None,

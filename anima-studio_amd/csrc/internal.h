@@ -178,5 +178,6 @@ int linear_q4_launch(anima_ctx* c, const anima_linear_desc* d);
 
 // ---- kernel launchers (prefix.hip)
 int attention_prefix_launch(anima_ctx* c, const anima_prefix_attn_desc* d);
+int attention_prefix_prepare_launch(anima_ctx* c, const anima_prefix_attn_desc* d, void* out, int64_t bytes);
 
 }  // namespace anima

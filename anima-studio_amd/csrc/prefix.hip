@@ -7,6 +7,7 @@
 // blocks whatever sequence the rows belong to, then over the packed keys of their own sequences, masked by each row's
 // range of them.  The packed K (normed, rotated at P + place) and V are laid out as the prefix's are, in one pass.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "internal.h"
@@ -18,6 +19,9 @@ constexpr int PHD = 128;      // head dim
 constexpr int PBK = 64;       // keys per block of the prepared layouts
 constexpr int PSEQ = 256;     // sequences of one launch (their first rows go with the kernel's arguments)
 constexpr float LOG2E = 1.4426950408889634f;
+
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 struct PrefixSeqs {
   int n;                // sequences
@@ -54,6 +58,10 @@ struct PrefixArgs {
   int64_t sin_off;
   float eps, c;     // c = scale * log2(e)
   int T, Tp, P, Pp, H, Hkv, group, causal, obf;
+  // tiles: virtual rows V = T * group of a kv head (row v / group, its head v % group), key blocks in `splits` parts
+  int V, nt, splits;
+  float* po;        // [splits][Hkv][V][128] sums, and
+  float* pml;       // [splits][Hkv][V][2] maximum and sum of weights, of a split call
   PrefixSeqs seq;
 };
 
@@ -73,44 +81,107 @@ __device__ __forceinline__ void row_norm_rope(const PrefixArgs& a, const float* 
   }
 }
 
-// place of key l in a V^T row: the bf16 form keeps each 16 keys as 0-3, 8-11, 4-7, 12-15
-template <class T>
-__device__ __forceinline__ int vt_place(int l) {
-  if (sizeof(T) == 4) return l;
-  const int r = l & 15;
-  return (l & ~15) | (r & 3) | ((r & 4) << 1) | ((r & 8) >> 1);
-}
-
-// A wave per packed row and kv head; rows T .. Tp are zeros.  A key whose K or V is not finite gets a K of NaN and a V of
-// zeros: every row that sees it becomes NaN, and where it is masked its weight of 0 meets no NaN in V.
+// One workgroup per 64 packed rows and kv head; rows T .. Tp are zeros.  K: 16 lanes a row, lane q holding dims 4 q .. + 3 and
+// 64 + the same (both of each rotated pair); V: wave w takes dims 32 w .. + 31 of all rows, lane (q, c) the eight keys of V^T
+// chunk c at dims 4 q .. + 3, so that every load and store moves whole lines.  The bf16 form has K in f16 (its rounding
+// to 8 bits alone would be 0.004 of a result) and keeps each 16 keys of a V^T row as 0-3, 8-11, 4-7, 12-15, as the matrix
+// products take them.
+// A key whose K or V is not finite (in its form) gets a K of NaN and a V of zeros: every row that sees it becomes NaN, and where it
+// is masked its weight of 0 meets no NaN in V.
 template <class T>
 __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a) {
-  const int l = blockIdx.x * 4 + (threadIdx.x >> 6), hk = blockIdx.y, lane = threadIdx.x & 63;
-  if (l >= a.Tp) return;
-  float k0 = 0.0f, k1 = 0.0f, v0 = 0.0f, v1 = 0.0f;
-  if (l < a.T) {
-    const float* k = a.k + (int64_t)l * a.ldk + hk * PHD;
-    const float* v = a.v + (int64_t)l * a.ldv + hk * PHD;
-    k0 = k[lane];
-    k1 = k[lane + 64];
-    v0 = v[lane];
-    v1 = v[lane + 64];
-    row_norm_rope(a, a.kn, a.P + l - a.seq.start[seq_of(a.seq, l)], k0, k1);
+  constexpr bool BF = sizeof(T) == 2;
+  __shared__ int bad[64];
+  const int t = threadIdx.x, w = t >> 6, lane = t & 63, kb0 = blockIdx.x * 64, hk = blockIdx.y;
+  if (t < 64) bad[t] = 0;
+  const int q16 = lane & 15, rsub = lane >> 4, vq = lane & 7, vc = lane >> 3;
+  const auto vkey = [&](int e) { return BF ? kb0 + 16 * (vc >> 1) + 4 * (vc & 1) + (e & 3) + 8 * (e >> 2) : kb0 + 8 * vc + e; };
+  f32x4 klo[4], khi[4], ve[8], cv[4], sv[4], wl{}, wh{};
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int l = min(kb0 + 16 * w + 4 * i + rsub, a.T - 1);
+    const float* src = a.k + (int64_t)l * a.ldk + hk * PHD + 4 * q16;
+    klo[i] = *(const f32x4*)src;
+    khi[i] = *(const f32x4*)(src + 64);
+    if (a.cs) {
+      const float* cr = a.cs + (int64_t)(a.P + l - a.seq.start[seq_of(a.seq, l)]) * 64 + 4 * q16;
+      cv[i] = *(const f32x4*)cr;
+      sv[i] = *(const f32x4*)(cr + a.sin_off);
+    }
   }
-  k0 = (float)(T)k0;
-  k1 = (float)(T)k1;
-  v0 = (float)(T)v0;
-  v1 = (float)(T)v1;
-  if (__builtin_amdgcn_ballot_w64(!(fabsf(k0) < INFINITY && fabsf(k1) < INFINITY && fabsf(v0) < INFINITY && fabsf(v1) < INFINITY))) {
-    k0 = k1 = __builtin_nanf("");
-    v0 = v1 = 0.0f;
+  if (a.kn) {
+    wl = *(const f32x4*)(a.kn + 4 * q16);
+    wh = *(const f32x4*)(a.kn + 64 + 4 * q16);
   }
-  T* kd = (T*)a.ok + ((int64_t)hk * a.Tp + l) * PHD;
-  kd[lane] = (T)k0;
-  kd[lane + 64] = (T)k1;
-  T* vd = (T*)a.ovt + (int64_t)hk * PHD * a.Tp + vt_place<T>(l);
-  vd[(int64_t)lane * a.Tp] = (T)v0;
-  vd[(int64_t)(lane + 64) * a.Tp] = (T)v1;
+#pragma unroll
+  for (int e = 0; e < 8; e++) ve[e] = *(const f32x4*)(a.v + (int64_t)min(vkey(e), a.T - 1) * a.ldv + hk * PHD + 32 * w + 4 * vq);
+  __syncthreads();
+  const auto finite = [](f32x4 v, auto as) {
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; j++) m += (float)(decltype(as))v[j] * 0.0f;  // (0 of finite values, else NaN)
+    return m == 0.0f;
+  };
+  typedef std::conditional_t<BF, _Float16, float> TK;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    f32x4 lo = klo[i], hi = khi[i];
+    if (a.kn) {
+      float ss = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; j++) ss += lo[j] * lo[j] + hi[j] * hi[j];
+#pragma unroll
+      for (int s = 1; s < 16; s <<= 1) ss += __shfl_xor(ss, s);
+      const float rn = 1.0f / sqrtf(ss / 128.0f + a.eps);
+      lo = lo * rn * wl;
+      hi = hi * rn * wh;
+    }
+    if (a.cs) {
+      const f32x4 x = lo;
+      lo = x * cv[i] - hi * sv[i];
+      hi = hi * cv[i] + x * sv[i];
+    }
+    klo[i] = lo;
+    khi[i] = hi;
+    if (!finite(lo, TK()) || !finite(hi, TK())) bad[16 * w + 4 * i + rsub] = 1;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; e++)
+    if (!finite(ve[e], T())) bad[vkey(e) - kb0] = 1;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int r = 16 * w + 4 * i + rsub, l = kb0 + r;
+    const float k = __builtin_nanf("");
+    const f32x4 z = l < a.T ? f32x4{k, k, k, k} : f32x4{};
+    const bool keep = l < a.T && !bad[r];
+    const f32x4 lo = keep ? klo[i] : z, hi = keep ? khi[i] : z;
+    TK* d = (TK*)a.ok + ((int64_t)hk * a.Tp + l) * PHD + 4 * q16;
+    if constexpr (BF) {
+      *(f16x4*)d = f16x4{(_Float16)lo[0], (_Float16)lo[1], (_Float16)lo[2], (_Float16)lo[3]};
+      *(f16x4*)(d + 64) = f16x4{(_Float16)hi[0], (_Float16)hi[1], (_Float16)hi[2], (_Float16)hi[3]};
+    } else {
+      *(f32x4*)d = lo;
+      *(f32x4*)(d + 64) = hi;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; e++)
+    if (vkey(e) >= a.T || bad[vkey(e) - kb0]) ve[e] = f32x4{};
+  T* vd = (T*)a.ovt + ((int64_t)hk * PHD + 32 * w + 4 * vq) * a.Tp + kb0 + 8 * vc;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    T* d = vd + (int64_t)j * a.Tp;
+    if constexpr (BF) {
+      bf16x8 o;
+#pragma unroll
+      for (int e = 0; e < 8; e++) o[e] = to_bf16(ve[e][j]);
+      *(bf16x8*)d = o;
+    } else {
+      *(f32x4*)d = f32x4{ve[0][j], ve[1][j], ve[2][j], ve[3][j]};
+      *(f32x4*)(d + 4) = f32x4{ve[4][j], ve[5][j], ve[6][j], ve[7][j]};
+    }
+  }
 }
 
 // A wave per packed row and head, one key at a time, running maximum and sum.
@@ -139,7 +210,7 @@ __global__ __launch_bounds__(256) void prefix_rows_kernel(PrefixArgs a) {
         m = s;
       }
       const float p = __builtin_amdgcn_exp2f(s - m);
-      const int jp = vt_place<T>(j);
+      const int jp = j;
       sum += p;
       o0 += p * (float)vt[lane * ld + jp];
       o1 += p * (float)vt[(lane + 64) * ld + jp];
@@ -159,24 +230,450 @@ __global__ __launch_bounds__(256) void prefix_rows_kernel(PrefixArgs a) {
   }
 }
 
+// ------------------------------------------------------------------ bf16 tiles
+//
+// A workgroup takes 32 NW virtual rows of one kv head (a wave 32 of them) and a part of their key blocks of 64: first the
+// blocks that every row sees whole (the prefix's, then own ones before all of the tile's rows), then the prefix's last
+// part and the own blocks that the rows' ranges cut.  Keys in any order give the same softmax, so both kinds are one loop each.
+//
+// Scores transposed, S^T = K Q^T: lane (r, hf) of a 32 x 32 product owns row r, and each of its maxima and sums is a register.  q and k
+// are in f16, 11 bits (in bf16 they would be 0.005 of a result off: more than its own rounding), the weights and V in bf16.
+// p = 2^(s - m) with an integer m that only rises (a power of two, so no rounding depends on when it rose): in blocks that
+// are seen whole without looking, as long as the weights' sum stays below 2^64, from -m in the scores' accumulators.
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) void prefix_lds_t;
+constexpr float P_LIMIT = 18446744073709551616.0f;  // 2^64
+constexpr float M_NONE = -1e30f;                    // no key so far
+constexpr int PKT = 64 * PHD * 2;                   // bytes of a block's K; its V^T follows
+constexpr int PST = 2 * PKT;                        // of a stage
+constexpr int PNST = 4;
+
+#define P_WAIT_VM(n) __builtin_amdgcn_s_waitcnt(((n) & 15) | (7 << 4) | (15 << 8) | (((n) >> 4) << 14))
+#define P_SB() __builtin_amdgcn_sched_barrier(0)
+
+__device__ __forceinline__ void p_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t p_rsrc(const void* p, int64_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, (short)0, (int)bytes, 0x00020000);
+}
+__device__ __forceinline__ void p_copy16(__amdgpu_buffer_rsrc_t rs, char* dst, uint32_t off, uint32_t base) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (prefix_lds_t*)dst, 16, off, base, 0, 0);
+}
+// of a value over the lane pair (l, l ^ 32)
+__device__ __forceinline__ float p_pair_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float p_pair_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// The key blocks of a tile: `full` whole ones (nP of the prefix, then own ones from of0), then the cut ones (the
+// prefix's last, then own ones from ob0 up to of0 and from of1 up to ob1).
+struct PrefixBlocks {
+  int nP, of0, full, tail, ob0, cut0, of1, total;
+  __device__ __forceinline__ PrefixBlocks(const PrefixArgs& a, int row0, int row1) {  // rows row0 .. row1
+    const int b0 = seq_of(a.seq, row0), b1 = seq_of(a.seq, row1), s0 = a.seq.start[b0];
+    const int end = a.causal ? row1 + 1 : a.seq.start[b1 + 1];
+    const int hi = b0 != b1 ? 0 : a.causal ? row0 + 1 : end;  // keys s0 .. hi are seen by all
+    nP = a.P / PBK;
+    tail = a.P % PBK ? 1 : 0;
+    ob0 = s0 / PBK;
+    const int ob1 = (end + PBK - 1) / PBK;
+    of0 = (s0 + PBK - 1) / PBK;
+    of1 = hi / PBK;
+    if (of1 <= of0) of0 = of1 = ob0;
+    full = nP + of1 - of0;
+    cut0 = of0 - ob0;
+    total = full + tail + cut0 + ob1 - of1;
+  }
+  // block i: its number, and whether it is of the prefix
+  __device__ __forceinline__ int at(int i, bool& prefix) const {
+    if (i < full) {
+      prefix = i < nP;
+      return prefix ? i : of0 + i - nP;
+    }
+    i -= full;
+    prefix = i < tail;
+    if (prefix) return nP;
+    i -= tail;
+    return i < cut0 ? ob0 + i : of1 + i - cut0;
+  }
+};
+
+// q of virtual row v: the lane's dims 16 ks + 8 hf + j in x[8 ks + j], normed, rotated at pos.
+__device__ __forceinline__ void p_load_q(const PrefixArgs& a, const float* src, int pos, int hf, float (&x)[64]) {
+#pragma unroll
+  for (int ks = 0; ks < 8; ks++) {
+    const f32x4 lo = *(const f32x4*)(src + 16 * ks + 8 * hf), hi = *(const f32x4*)(src + 16 * ks + 8 * hf + 4);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      x[8 * ks + j] = lo[j];
+      x[8 * ks + 4 + j] = hi[j];
+    }
+  }
+  if (a.qn) {
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 64; i++) ss = __builtin_fmaf(x[i], x[i], ss);
+    const float rn = 1.0f / sqrtf(p_pair_sum(ss) / 128.0f + a.eps);
+#pragma unroll
+    for (int ks = 0; ks < 8; ks++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[8 * ks + j] = x[8 * ks + j] * rn * a.qn[16 * ks + 8 * hf + j];
+  }
+  if (a.cs) {
+    const float* cr = a.cs + (int64_t)pos * 64 + 8 * hf;
+#pragma unroll
+    for (int ks = 0; ks < 4; ks++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float c = cr[16 * ks + j], s = cr[a.sin_off + 16 * ks + j], x1 = x[8 * ks + j], x2 = x[8 * ks + 32 + j];
+        x[8 * ks + j] = x1 * c - x2 * s;
+        x[8 * ks + 32 + j] = x2 * c + x1 * s;
+      }
+  }
+}
+
+template <int NW>
+__global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_bf16(PrefixArgs a) {
+  constexpr int CPW = 16 / NW;  // copies of K, and of V^T, a wave and block
+  __shared__ __attribute__((aligned(1024))) char smem[PNST * PST];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 31, hf = lane >> 5;
+  // tiles of a head and split follow each other (on one XCD: they read the same blocks)
+  const int id = xcd_remap(blockIdx.x, gridDim.x), hs = id / a.nt, tile = id - hs * a.nt, hk = hs / a.splits, sp = hs - hk * a.splits;
+  const int v0 = tile * 32 * NW, v = v0 + 32 * wave + r;
+  const PrefixBlocks B(a, v0 / a.group, (min(v0 + 32 * NW, a.V) - 1) / a.group);
+  const int i0 = (int)((int64_t)B.total * sp / a.splits), i1 = (int)((int64_t)B.total * (sp + 1) / a.splits), nb = i1 - i0;
+  const bool live = v0 + 32 * wave < a.V;  // the wave has rows
+
+  const int64_t pb = (int64_t)a.Pp * PHD * 2, ob = (int64_t)a.Tp * PHD * 2;
+  const __amdgpu_buffer_rsrc_t rpk = p_rsrc((const char*)a.pk + hk * pb, a.P ? pb : 0), rpv = p_rsrc((const char*)a.pvt + hk * pb, a.P ? pb : 0),
+                               rok = p_rsrc((const char*)a.ok + hk * ob, ob), rov = p_rsrc((const char*)a.ovt + hk * ob, ob);
+  uint32_t ko[CPW], vd[CPW], vu[CPW];
+#pragma unroll
+  for (int c = 0; c < CPW; c++) {
+    const int row = 4 * (wave * CPW + c) + (lane >> 4), d = 8 * (wave * CPW + c) + (lane >> 3);
+    ko[c] = row * 256 + 16 * ((lane & 15) ^ (row & 15));
+    vd[c] = d;
+    vu[c] = 16 * ((lane & 7) ^ ((d >> 1) & 7));
+  }
+  const auto load = [&](int j) __attribute__((always_inline)) {  // block j of the part (past the last: that one again, unused)
+    bool pre;
+    const int blk = B.at(i0 + min(j, nb - 1), pre);
+    char* st = smem + (j & 3) * PST;
+    const uint32_t ld = 2 * (pre ? a.Pp : a.Tp);
+#pragma unroll
+    for (int c = 0; c < CPW; c++) p_copy16(pre ? rpk : rok, st + (wave * CPW + c) * 1024, ko[c], blk * (64 * 256));
+#pragma unroll
+    for (int c = 0; c < CPW; c++) p_copy16(pre ? rpv : rov, st + PKT + (wave * CPW + c) * 1024, vd[c] * ld + vu[c], blk * 128);
+  };
+  if (nb > 0) {
+    load(0);
+    load(1);
+    load(2);
+  }
+
+  // the lane's row
+  const int vc = min(v, a.V - 1), row = vc / a.group, h = hk * a.group + vc - row * a.group, sq = seq_of(a.seq, row);
+  const int klo = a.seq.start[sq], khi = a.causal ? row + 1 : a.seq.start[sq + 1];
+  f16x8 qf[8];
+  {
+    float x[64];
+    p_load_q(a, a.q + (int64_t)row * a.ldq + h * PHD, a.P + row - klo, hf, x);
+#pragma unroll
+    for (int ks = 0; ks < 8; ks++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) qf[ks][j] = (_Float16)(x[8 * ks + j] * a.c);
+  }
+  f32x16 o[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) o[i] = f32x16{};
+  float m = M_NONE, l = 0.0f;
+  int kof[8], vof[4];
+#pragma unroll
+  for (int ks = 0; ks < 8; ks++) kof[ks] = r * 256 + 16 * ((2 * ks + hf) ^ (r & 15));
+#pragma unroll
+  for (int j = 0; j < 4; j++) vof[j] = PKT + r * 128 + 16 * ((2 * j + hf) ^ ((r >> 1) & 7));
+  const bf16x2 ones = {(bf16)1.0f, (bf16)1.0f};
+
+  // sets p (eight weights) and adds their sum
+  const auto weights = [&](const f32x16& s, int u, bf16x8& p, float& sum) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) p[e] = to_bf16(__builtin_amdgcn_exp2f(s[8 * u + e]));
+#pragma unroll
+    for (int e = 0; e < 4; e++) sum = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{p[2 * e], p[2 * e + 1]}, ones, sum, false);
+  };
+  // A block with its maximum looked at.  Keys k0 + ... outside [lo, hi) are masked.
+  const auto block = [&](const char* st, auto masked, int k0, int lo, int hi) __attribute__((always_inline)) {
+    f32x16 s[2];
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      s[t] = f32x16{};
+#pragma unroll
+      for (int ks = 0; ks < 8; ks++) {
+        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const f16x8*)(st + kof[ks] + t * 8192), qf[ks], s[t], 0, 0, 0);
+      }
+    }
+    if constexpr (decltype(masked)::value) {
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          const int k = k0 + 32 * t + 8 * (e >> 2) + 4 * hf + (e & 3);
+          if (k < lo || k >= hi) s[t][e] = -INFINITY;
+        }
+    }
+    float bm = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+    for (int e = 1; e < 16; e++) bm = fmaxf(bm, fmaxf(s[0][e], s[1][e]));
+    const float mn = fmaxf(m, ceilf(p_pair_max(bm)));
+    if (__builtin_amdgcn_ballot_w64(mn > m)) {
+      const float f = __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < 4; i++) o[i] *= f;
+    }
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      s[t] -= m;
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        bf16x8 p;
+        weights(s[t], u, p, l);
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(st + vof[2 * t + u] + i * 4096), p, o[i], 0, 0, 0);
+      }
+    }
+  };
+  // A block that every row sees whole, after another: the written order is kept (each product's fragment was read four
+  // reads before it, one half's exponentials run beside the next products).
+  f32x16 negm;
+  const auto whole = [&](const char* st) __attribute__((always_inline)) {
+    const auto frag = [&](int i) __attribute__((always_inline)) {
+      return i < 16 ? *(const bf16x8*)(st + kof[i & 7] + (i >> 3) * 8192)
+                    : *(const bf16x8*)(st + vof[(i - 16) >> 3 << 1 | (i & 1)] + (((i - 16) & 7) >> 1) * 4096);
+    };
+    bf16x8 f[4] = {frag(0), frag(1), frag(2), frag(3)};
+    f32x16 s[2];
+    bf16x8 p[4];
+    float la = 0.0f, lb = 0.0f;
+    const auto prob2 = [&](int t, int k) __attribute__((always_inline)) {
+      bf16x8& q = p[2 * t + (k >> 2)];
+      q[2 * (k & 3)] = to_bf16(__builtin_amdgcn_exp2f(s[t][2 * k]));
+      q[2 * (k & 3) + 1] = to_bf16(__builtin_amdgcn_exp2f(s[t][2 * k + 1]));
+      float& acc = k & 1 ? lb : la;
+      acc = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{q[2 * (k & 3)], q[2 * (k & 3) + 1]}, ones, acc, false);
+    };
+    // the rare case of a sum above 2^64: m rises to the half's largest score
+    const auto settle = [&](int t) __attribute__((always_inline)) {
+      float sum = la + lb;
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(sum <= P_LIMIT)) != 0, 0)) {
+        float bm = s[t][0];
+#pragma unroll
+        for (int e = 1; e < 16; e++) bm = fmaxf(bm, s[t][e]);
+        const float d = fmaxf(ceilf(p_pair_max(bm)), 0.0f), g = __builtin_amdgcn_exp2f(-d);
+        m += d;
+        negm -= d;
+        l *= g;
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] *= g;
+#pragma unroll
+        for (int u = t; u < 2; u++) s[u] -= d;
+        la = lb = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) prob2(t, k);
+        sum = la + lb;
+      }
+      l += sum;
+      la = lb = 0.0f;
+    };
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      f32x16& d = s[i >> 3];
+      d = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, f[i & 3]), qf[i & 7], (i & 7) == 0 ? negm : d, 0, 0, 0);
+      f[i & 3] = frag(i + 4);
+      if (i >= 8) prob2(0, i - 8);
+      P_SB();
+    }
+    settle(0);
+    P_SB();
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+      if (j == 8) {
+        settle(1);
+        P_SB();
+      }
+      o[(j & 7) >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[j & 3], p[j >> 3 << 1 | (j & 1)], o[(j & 7) >> 1], 0, 0, 0);
+      if (j < 12) f[j & 3] = frag(j + 20);
+      if (j < 8) prob2(1, j);
+      P_SB();
+    }
+  };
+
+  // Block j in stage j % 4.  At the top of its turn this wave's copies of it have arrived (those of the two blocks after it may
+  // pend); behind the barrier everyone's have, and the stage of block j - 1 is refilled.
+  const auto turn = [&](int j) __attribute__((always_inline)) {
+    P_WAIT_VM(2 * 2 * CPW);
+    p_barrier();
+    load(j + 3);
+    return (const char*)smem + (j & 3) * PST;
+  };
+  const int nf = max(min(B.full, i1) - i0, 0);
+  int j = 0;
+  if (nf > 0) {
+    const char* st = turn(0);
+    if (live) block(st, std::false_type{}, 0, 0, 0);
+    negm = f32x16{} - m;
+    for (j = 1; j < nf; j++) {
+      st = turn(j);
+      if (live) whole(st);
+    }
+  }
+  for (; j < nb; j++) {
+    const char* st = turn(j);
+    bool pre;
+    const int blk = B.at(i0 + j, pre);
+    if (live) block(st, std::true_type{}, blk * PBK, pre ? 0 : klo, pre ? a.P : khi);
+  }
+  P_WAIT_VM(0);  // no copy into LDS outlives the loop
+  p_barrier();
+
+  // Rows leave through LDS in halves of 64 columns, so that every store writes 256 bytes of a row.
+  l = p_pair_sum(l);
+  const bool part = a.splits > 1;
+  const float inv = part ? 1.0f : 1.0f / l;
+  const int64_t plane = ((int64_t)sp * a.Hkv + hk) * a.V;
+  if (part && v < a.V && hf == 0) *(float2*)(a.pml + (plane + v) * 2) = make_float2(m, l);
+  constexpr int RS = 64 + 4;
+  float* ow = (float*)smem + wave * 32 * RS;
+  const int rr = lane >> 4, cc = 4 * (lane & 15);
+#pragma unroll
+  for (int half = 0; half < 2; half++) {
+#pragma unroll
+    for (int d2 = 0; d2 < 2; d2++)
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const f32x16& w = o[2 * half + d2];
+        *(f32x4*)(ow + r * RS + 32 * d2 + 8 * g + 4 * hf) = f32x4{w[4 * g] * inv, w[4 * g + 1] * inv, w[4 * g + 2] * inv, w[4 * g + 3] * inv};
+      }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const int q = 4 * k + rr, vo = v0 + 32 * wave + q;
+      const f32x4 w = *(const f32x4*)(ow + q * RS + cc);
+      if (vo < a.V) {
+        if (part) {
+          *(f32x4*)(a.po + (plane + vo) * PHD + 64 * half + cc) = w;
+        } else {
+          const int64_t ro = vo / a.group, off = ro * a.ldo + (hk * a.group + vo - ro * a.group) * PHD + 64 * half + cc;
+          if (a.obf) *(bf16x4*)((bf16*)a.o + off) = bf16x4{to_bf16(w[0]), to_bf16(w[1]), to_bf16(w[2]), to_bf16(w[3])};
+          else *(f32x4*)((float*)a.o + off) = w;
+        }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// The parts of a split call, a half wave per virtual row: o = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s.
+__global__ __launch_bounds__(256) void prefix_join_kernel(PrefixArgs a) {
+  const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), n = (int64_t)a.Hkv * a.V;
+  if (i >= n) return;
+  const int d = 4 * (threadIdx.x & 31);
+  float m = M_NONE;
+  for (int s = 0; s < a.splits; s++) m = fmaxf(m, a.pml[(s * n + i) * 2]);
+  float l = 0.0f;
+  f32x4 o = {};
+  for (int s = 0; s < a.splits; s++) {
+    const float2 ml = *(const float2*)(a.pml + (s * n + i) * 2);
+    const float f = __builtin_amdgcn_exp2f(ml.x - m);
+    const f32x4 w = *(const f32x4*)(a.po + (s * n + i) * PHD + d);
+    l += f * ml.y;
+    o += f * w;
+  }
+  o *= 1.0f / l;
+  const int hk = (int)(i / a.V), v = (int)(i - (int64_t)hk * a.V);
+  const int64_t row = v / a.group, off = row * a.ldo + (hk * a.group + v - row * a.group) * PHD + d;
+  if (a.obf) *(bf16x4*)((bf16*)a.o + off) = bf16x4{to_bf16(o[0]), to_bf16(o[1]), to_bf16(o[2]), to_bf16(o[3])};
+  else *(f32x4*)((float*)a.o + off) = o;
+}
+
 // ------------------------------------------------------------------ host
+
+template <class T>
+static int prefix_prep_launch(anima_ctx* c, const PrefixArgs& a) {
+  Launch L(c, sizeof(T) == 2 ? "attn.prefix_prep_bf16" : "attn.prefix_prep_fp32", 0.0, (double)a.Hkv * a.T * PHD * (8.0 + 2 * sizeof(T)));
+  hipLaunchKernelGGL(prefix_prep_kernel<T>, dim3((unsigned)(a.Tp / 64), (unsigned)a.Hkv), dim3(256), 0, c->stream, a);
+  return L.end();
+}
 
 // The sequences of one launch, which the arguments describe: their keys and values into the workspace, then the rows.
 template <class T>
 static int prefix_part(anima_ctx* c, PrefixArgs& a) {
+  constexpr bool BF = sizeof(T) == 2;
+  a.V = a.T * a.group;
+  const int blocks = a.Pp / PBK + a.Tp / PBK;
+  bool eight = false;
+  a.splits = 1;
+  if (BF) {
+    eight = (int64_t)((a.V + 255) / 256) * a.Hkv >= c->num_cus;
+    const int rows = eight ? 256 : 128;
+    a.nt = (a.V + rows - 1) / rows;
+    const int64_t wgs = (int64_t)a.nt * a.Hkv;
+    a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({c->num_cus / wgs, blocks / 2, 64}));
+  }
+  const size_t plane = (size_t)a.Hkv * a.Tp * PHD * sizeof(T), n = a.splits > 1 ? (size_t)a.splits * a.Hkv * a.V : 0;
   void* ws = nullptr;
-  const size_t plane = (size_t)a.Hkv * a.Tp * PHD * sizeof(T);
-  if (int rc = workspace(c, 2 * plane, &ws)) return rc;
+  if (int rc = workspace(c, 2 * plane + n * (PHD + 2) * 4, &ws)) return rc;
   a.ok = ws;
   a.ovt = (char*)ws + plane;
-  {
-    Launch L(c, "attn.prefix_prep", 0.0, (double)a.Hkv * a.T * PHD * (8.0 + 2 * sizeof(T)));
-    hipLaunchKernelGGL(prefix_prep_kernel<T>, dim3((unsigned)(a.Tp / 4), (unsigned)a.Hkv), dim3(256), 0, c->stream, a);
-    if (int rc = L.end()) return rc;
+  a.po = (float*)((char*)ws + 2 * plane);
+  a.pml = a.po + n * PHD;
+  if (int rc = prefix_prep_launch<T>(c, a)) return rc;
+  Launch L(c, BF ? "attn.prefix_bf16" : "attn.prefix_fp32", 4.0 * a.T * a.H * PHD * a.P, 0.0);
+  if constexpr (BF) {
+    const dim3 grid((unsigned)((int64_t)a.nt * a.Hkv * a.splits));
+    if (eight) hipLaunchKernelGGL(prefix_flash_bf16<8>, grid, dim3(512), 0, c->stream, a);
+    else hipLaunchKernelGGL(prefix_flash_bf16<4>, grid, dim3(256), 0, c->stream, a);
+    if (a.splits > 1)
+      hipLaunchKernelGGL(prefix_join_kernel, dim3((unsigned)(((int64_t)a.Hkv * a.V + 7) / 8)), dim3(256), 0, c->stream, a);
+  } else {
+    hipLaunchKernelGGL(prefix_rows_kernel<T>, dim3((unsigned)(((int64_t)a.T * a.H + 3) / 4)), dim3(256), 0, c->stream, a);
   }
-  Launch L(c, "attn.prefix", 4.0 * a.T * a.H * PHD * a.P, 0.0);
-  hipLaunchKernelGGL(prefix_rows_kernel<T>, dim3((unsigned)(((int64_t)a.T * a.H + 3) / 4)), dim3(256), 0, c->stream, a);
   return L.end();
+}
+
+int attention_prefix_prepare_launch(anima_ctx* c, const anima_prefix_attn_desc* d, void* out, int64_t bytes) {
+  char msg[256];
+  if (int rc = check_attention_prefix_prepare(d, out, bytes, PrefixMsg{msg, sizeof msg})) return fail(c, rc, "%s", msg);
+  OnDevice on(c);
+  const bool bf = d->precision == ANIMA_PREC_BF16;
+  PrefixArgs a{};
+  a.group = d->group == 0 ? 1 : d->group;
+  a.H = d->H;
+  a.Hkv = d->H / a.group;
+  a.T = d->len[0];
+  a.Tp = (a.T + PBK - 1) / PBK * PBK;
+  a.k = d->k + d->k_off;
+  a.ldk = d->ldk;
+  a.v = d->v + d->v_off;
+  a.ldv = d->ldv;
+  a.kn = d->k_norm;
+  a.cs = d->rope_cs;
+  a.sin_off = d->rope_sin_off;
+  a.eps = d->eps;
+  a.ok = out;
+  a.ovt = (char*)out + bytes / 2;
+  a.seq.n = 1;
+  a.seq.start[1] = a.T;
+  return bf ? prefix_prep_launch<bf16>(c, a) : prefix_prep_launch<float>(c, a);
 }
 
 int attention_prefix_launch(anima_ctx* c, const anima_prefix_attn_desc* d) {
@@ -209,10 +706,10 @@ int attention_prefix_launch(anima_ctx* c, const anima_prefix_attn_desc* d) {
   a.obf = d->o_bf16;
   int64_t row = 0;
   for (int b = 0; b < d->B;) {
-    // the next sequences, as many as one launch describes and 2^22 rows hold
+    // the next sequences, as many as one launch describes, 2^22 keys and 2^30 rows of all heads hold
     a.seq.n = 0;
     int64_t t = 0;
-    while (b < d->B && a.seq.n < PSEQ && t + d->len[b] <= PREFIX_MAX_KEYS) {
+    while (b < d->B && a.seq.n < PSEQ && t + d->len[b] <= PREFIX_MAX_KEYS && (t + d->len[b]) * d->H <= PREFIX_MAX_VROWS) {
       if (d->len[b] > 0) {
         a.seq.start[a.seq.n++] = (int)t;
         t += d->len[b];

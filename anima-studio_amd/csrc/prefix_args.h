@@ -13,6 +13,7 @@ constexpr int64_t PREFIX_MAX_KEYS = 1 << 22;  // of the prefix and of a sequence
 constexpr int64_t PREFIX_MAX_ROWS = 1 << 28;  // of all sequences
 constexpr int64_t PREFIX_MAX_LD = 1 << 20;    // floats between rows: 256 rows of a tile stay below 2^31 bytes
 constexpr int PREFIX_MAX_HEADS = 1 << 12;
+constexpr int64_t PREFIX_MAX_VROWS = 1 << 30;  // rows times heads of a launch: 256 threads to 128 of them stay below 2^32
 
 struct PrefixMsg {
   char* buf;
@@ -53,6 +54,8 @@ inline int check_attention_prefix(const anima_prefix_attn_desc* d, int64_t* rows
   for (int b = 0; b < d->B; b++) {
     if (d->len[b] < 0 || d->len[b] > PREFIX_MAX_KEYS)
       return fail(ANIMA_E_ARG, "%s: len[%d]=%d outside [0, %lld]", who, b, d->len[b], (long long)PREFIX_MAX_KEYS);
+    if ((int64_t)d->len[b] * d->H > PREFIX_MAX_VROWS)
+      return fail(ANIMA_E_UNSUPPORTED, "%s: len[%d]=%d rows of %d heads (at most 2^30 together)", who, b, d->len[b], d->H);
     *rows += d->len[b];
     if (d->len[b] > *longest) *longest = d->len[b];
     if (*rows > PREFIX_MAX_ROWS) return fail(ANIMA_E_UNSUPPORTED, "%s: more than %lld rows", who, (long long)PREFIX_MAX_ROWS);
@@ -83,6 +86,33 @@ inline int check_attention_prefix(const anima_prefix_attn_desc* d, int64_t* rows
                   (long long)d->P + *longest);
   }
   if (!(d->eps >= 0.0f)) return fail(ANIMA_E_ARG, "%s: eps=%g", who, (double)d->eps);
+  return ANIMA_OK;
+}
+
+// One sequence's keys and values as a prefix: what anima_attention_prefix asks of them, at positions 0 ...
+inline int check_attention_prefix_prepare(const anima_prefix_attn_desc* d, const void* out, int64_t bytes, PrefixMsg fail) {
+  const char* const who = "anima_attention_prefix_prepare";
+  if (!d || !out) return fail(ANIMA_E_ARG, "%s: null descriptor or output", who);
+  if (d->B != 1 || !d->len || d->len[0] < 1) return fail(ANIMA_E_ARG, "%s: one sequence of rows (B=%d)", who, d->B);
+  if (d->P || d->prefix_kv) return fail(ANIMA_E_ARG, "%s: P=%d, a prefix starts at 0 and has none before it", who, d->P);
+  anima_prefix_attn_desc k = *d;  // (q and o take no part)
+  k.q = d->k;
+  k.ldq = (int64_t)d->H * 128;
+  k.q_off = 0;
+  k.q_norm = nullptr;
+  k.o = (float*)out;
+  k.ldo = k.ldq;
+  k.o_off = 0;
+  k.o_bf16 = 0;
+  k.prefix_kv_bytes = 0;
+  int64_t rows;
+  int longest;
+  if (int rc = check_attention_prefix(&k, &rows, &longest, fail)) return rc;
+  const int Hkv = d->H / (d->group == 0 ? 1 : d->group);
+  const int64_t want = prefix_kv_bytes(Hkv, d->len[0], d->precision);
+  if (bytes != want)
+    return fail(ANIMA_E_ARG, "%s: %lld bytes, but %d kv heads and %d rows at this precision take %lld", who, (long long)bytes, Hkv, d->len[0],
+                (long long)want);
   return ANIMA_OK;
 }
 

@@ -689,6 +689,11 @@ int anima_attention_prefix(anima_ctx* c, const anima_prefix_attn_desc* d) {
   return attention_prefix_launch(c, d);
 }
 
+int anima_attention_prefix_prepare(anima_ctx* c, const anima_prefix_attn_desc* d, void* prefix_kv, int64_t bytes) {
+  CHECK_CTX(c);
+  return attention_prefix_prepare_launch(c, d, prefix_kv, bytes);
+}
+
 int anima_linear_glu(anima_ctx* c, const anima_glu_desc* d) {
   CHECK_CTX(c);
   return linear_glu_launch(c, d);

@@ -218,12 +218,14 @@ int64_t anima_attention_noalloc_scratch_bytes(void);
  * own sequence up to itself (causal = 0: all of them):
  *   o[row] = softmax_j(scale * q[row] . k_j) v_j       j: prefix keys, own keys
  * q, k, v, o as anima_attn_desc's, with the packed row for the row (no batch strides).  q / k RMSNorm and RoPE
- * are fused as there, RoPE at the position.  The prefix's K and V come as anima_attention_prepare_kv
- * (B = 1, Lk = P, the same precision) writes them, normed and rotated at 0 .. P - 1.  The reference encodes
- * one prompt at a time (app/pipeline.js:192-211, the causal attention of app/models/qwen3.js:60).
- * D = 128 (ANIMA_E_UNSUPPORTED otherwise).  A sequence of no rows is left out; P = 0: no prefix.  A key of a
- * sequence with a NaN or an infinity in k or v makes the rows that see it NaN, and no others.  The scratch (the
- * packed K and V, and partial sums) is the context's workspace. */
+ * are fused as there, RoPE at the position.  The prefix's K and V come as anima_attention_prefix_prepare
+ * (at the same precision) writes them.  The reference encodes one prompt at a time (app/pipeline.js:192-211,
+ * the causal attention of app/models/qwen3.js:60).
+ * ANIMA_PREC_BF16 rounds q (times scale log2 e) and k to 11 bits (f16: values from 65520 on count as not
+ * finite), the weights and v to bf16; ANIMA_PREC_FP32 rounds nothing.
+ * D = 128 (ANIMA_E_UNSUPPORTED otherwise).  A sequence of no rows is left out; P = 0: no prefix.  A key with
+ * a NaN or an infinity in k or v makes the rows that see it NaN, and no others.  The scratch (the packed K and
+ * V, and partial sums) is the context's workspace. */
 typedef struct {
   int B;
   const int* len;        /* host array [B] of row counts >= 0 (read by the call) */
@@ -237,7 +239,7 @@ typedef struct {
   int64_t ldv, v_off;
   float* o;
   int64_t ldo, o_off;
-  const void* prefix_kv; /* NULL with P = 0; 16-byte aligned */
+  const void* prefix_kv; /* anima_attention_prefix_prepare's, NULL with P = 0; 16-byte aligned */
   int64_t prefix_kv_bytes; /* anima_attention_kv_bytes(1, H / group, P, precision) */
   float scale;           /* 0 -> 1/sqrt(D) */
   int causal;
@@ -250,6 +252,11 @@ typedef struct {
   int o_bf16;            /* 1: O as bf16 rows (bf16 precision only; as anima_attn_desc) */
 } anima_prefix_attn_desc;
 int anima_attention_prefix(anima_ctx* ctx, const anima_prefix_attn_desc* desc);
+/* The keys and values of one sequence (B = 1, len[0] rows at positions 0 ..., P = 0; q, o and the query's side
+ * are not read) as a prefix for later calls, normed and rotated, in the form that the precision multiplies:
+ * prefix_kv[bytes], bytes = anima_attention_kv_bytes(1, H / group, len[0], precision), 16-byte aligned.  (Not
+ * the form of anima_attention_prepare_kv, whose K has 8 bits in bf16.) */
+int anima_attention_prefix_prepare(anima_ctx* ctx, const anima_prefix_attn_desc* desc, void* prefix_kv, int64_t bytes);
 
 /* ---------------------------------------------------------------- row ops */
 

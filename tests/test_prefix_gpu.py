@@ -3,10 +3,10 @@
 Tolerances.  fp32: a score is off by the roundings of the norms, the rotations and the products: at most 40 2^-24 |q| |k| scale;
 a weight by twice that of itself, the sums by 2^-24 (32 + keys / 16); so an output element is off by at most
 (80 |q| |k| scale + 32 + keys / 16) 2^-24 of the largest value of v that the row sees.
-bf16: q, k, the weights and v are rounded to 8 bits, each value off by 2^-8 of itself at the most, by 2^-9.3 in the root mean
-square.  A score is then off by sqrt(2) 2^-9.3 sqrt(sum (q_d k_d)^2) scale, which is 0.005 where q and k have normed rows of
-1.4; an output row, a mean of many independent values, by sqrt(0.005^2 + 2 2^-18.6) = 0.006 of the root of sum (p v)^2.  The tests
-ask for five times that, 0.03, of every row of 128 values.  A bf16 result adds 2^-8 of itself."""
+bf16: q and k are rounded to 11 bits, the weights and v to 8, each value off by 2^-11 and 2^-8 of itself at the most, by 2^-12.3 and
+2^-9.3 in the root mean square.  A score is off by sqrt(2) 2^-12.3 sqrt(sum (q_d k_d)^2) scale, which is 0.0006 where q and k have
+normed rows of 1.4; an output row, a mean of many independent values, by sqrt(0.0006^2 + 2 2^-18.6) = 0.0023 of the root of sum
+(p v)^2.  The tests ask for five times that, 0.012, of every row of 128 values.  A bf16 result adds 2^-8 of itself."""
 
 import numpy as np
 import pytest
@@ -57,10 +57,10 @@ class Case:
         if P:
             up = [ctx.upload(self.pk), ctx.upload(self.pv)]
             self.prefix = ctx.empty((ctx.attention_kv_bytes(1, Hkv, P, precision),), np.uint8)
-            ctx.attention(q=up[0], k=up[0], v=up[1], o=up[0], B=1, Lq=P, Lk=P, H=Hkv, D=128, ldq=Hkv * 128, ldk=Hkv * 128,
-                          ldv=Hkv * 128, precision=precision, prepare_into=self.prefix, k_norm=self.put("kn", self.kn),
-                          rope_cs=self.put("cs", np.concatenate([t.reshape(-1) for t in self.cs]) if roped else None),
-                          rope_sin_off=self.cs[0].size if roped else 0)
+            ctx.attention_prefix(k=up[0], v=up[1], lens=[P], H=H, group=H // Hkv, ldk=Hkv * 128, ldv=Hkv * 128, precision=precision,
+                                 prepare_into=self.prefix, k_norm=self.put("kn", self.kn),
+                                 rope_cs=self.put("cs", np.concatenate([t.reshape(-1) for t in self.cs]) if roped else None),
+                                 rope_sin_off=self.cs[0].size if roped else 0)
         else:
             self.prefix = None
 
@@ -117,7 +117,7 @@ class Case:
                 tol = (80 * size + 32 + (P + n) / 16) * 2.0 ** -24 * np.abs(v).max((0, 2))[None, :, None] + 0 * o
             else:
                 spread = np.sqrt(np.einsum("hij,jhd->ihd", p * p, v * v).sum(2, keepdims=True))  # of a whole row
-                tol = 0.03 * spread + 0 * o
+                tol = 0.012 * spread + 0 * o
             outs.append(o)
             tols.append(tol)
         return np.concatenate(outs), np.concatenate(tols)
@@ -275,7 +275,8 @@ def test_replayed_from_a_graph(ctx, lens, P, precision):
 @pytest.mark.parametrize("precision", [0, 1], ids=["bf16", "fp32"])
 def test_against_the_attention_of_each_sequence(ctx, precision):
     """The framework's own causal attention of the whole prompt, prefix and rows in one sequence: the same rows within both
-    sides' tolerance."""
+    sides' tolerance.  Its bf16 form rounds q and k to 8 bits: a score is off by eight times 0.0006, so a row by
+    sqrt(0.005^2 + 2 2^-18.6) = 0.006 in the root mean square, 0.03 at five times that, beside this side's 0.012."""
     m = amd()
     c = Case(ctx, [37, 5, 90], 150, 4, 2, precision)
     got = c.get().reshape(c.T, 4, 128)
@@ -292,5 +293,5 @@ def test_against_the_attention_of_each_sequence(ctx, precision):
                       precision=precision, q_norm=c.put("qn", c.qn), k_norm=c.put("kn", c.kn), rope_cs=ctx.upload(cs), rope_sin_off=L * 64)
         d = got[at: at + n] - o.numpy()[150:].reshape(n, 4, 128)
         err = np.abs(d) if precision == m.PREC_FP32 else np.sqrt((d * d).sum(2, keepdims=True))
-        assert np.all(err <= 2 * tol[at: at + n])
+        assert np.all(err <= (2 if precision == m.PREC_FP32 else 3.5) * tol[at: at + n])
         at += n

@@ -26,6 +26,8 @@ int t_embed(const anima_weight* w, const int32_t* ids, int64_t T, const float* f
   return check_embed_rows(w, ids, T, f, out, ldo, Q4Msg{m, n}); }
 int t_prefix(const anima_prefix_attn_desc* d, int64_t* rows, int* longest, char* m, size_t n) {
   return check_attention_prefix(d, rows, longest, PrefixMsg{m, n}); }
+int t_prepare(const anima_prefix_attn_desc* d, const void* out, int64_t bytes, char* m, size_t n) {
+  return check_attention_prefix_prepare(d, out, bytes, PrefixMsg{m, n}); }
 int64_t t_bytes(int h, int p, int prec) { return prefix_kv_bytes(h, p, prec); }
 }
 """
@@ -124,7 +126,7 @@ NONE = {"P": 0, "prefix_kv": 0, "prefix_kv_bytes": 0}
     ([3], {"o_bf16": 1, "o": P + 8}, 0), ([3], {"rope_cs": P, "rope_sin_off": 103 * 64}, 0), ([3], {"group": 0, "H": 2,
      "prefix_kv_bytes": 2 * 2 * 128 * 128 * 2}, 0), ([3], {"precision": 1, "prefix_kv_bytes": 2 * 2 * 128 * 128 * 4}, 0),
     ([3], {"D": 64}, -5), ([3], {"B": -1}, -1), ([3], {"len": 0}, -1), ([3, -1], {}, -1), ([(1 << 22) + 1], {}, -1),
-    ([1 << 22] * 65, {}, -5), ([3], {"H": 0}, -1), ([3], {"group": 4}, -1), ([3], {"group": -1}, -1), ([3], {"H": 1 << 13, "group": 1}, -1),
+    ([1 << 22] * 65, {}, -5), ([1 << 22], {"H": 257, "group": 1, "ldq": 1 << 18}, -5), ([3], {"H": 0}, -1), ([3], {"group": 4}, -1), ([3], {"group": -1}, -1), ([3], {"H": 1 << 13, "group": 1}, -1),
     ([3], {"P": -1}, -1), ([3], {"P": (1 << 22) + 1}, -1), ([3], {"precision": 2}, -1), ([3], {"causal": 2}, -1), ([3], {"o_bf16": 2}, -1),
     ([3], {"precision": 1, "o_bf16": 1}, -1), ([3], {"q": 0}, -1), ([3], {"k": 0}, -1), ([3], {"v": 0}, -1), ([3], {"o": 0}, -1),
     ([3], {"ldq": 764}, -1), ([3], {"ldk": 1020}, -1), ([3], {"ldv": 1276}, -1), ([3], {"ldo": 764}, -1), ([3], {"ldq": 1282}, -1),
@@ -146,10 +148,27 @@ def test_prefix_without_a_descriptor(checks):
     assert call(checks.t_prefix, None, ctypes.byref(rows), ctypes.byref(longest))[0] == -1
 
 
+PREP = dict(NONE, q=0, ldq=0, o=0, ldo=0)
+BYTES = 2 * 2 * 128 * 128 * 2
+
+
+@pytest.mark.parametrize("lens,change,out,size,code", [
+    ([100], {}, P, BYTES, 0), ([100], {"q_off": 3, "q_norm": 4, "o_bf16": 1}, P, BYTES, 0), ([100], {"precision": 1}, P, 2 * BYTES, 0),
+    ([100], {"rope_cs": P, "rope_sin_off": 100 * 64}, P, BYTES, 0), ([129], {}, P, 3 * BYTES // 2, 0), ([100], {}, 0, BYTES, -1),
+    ([100], {}, P + 8, BYTES, -1), ([100], {}, P, BYTES - 1, -1), ([100], {}, P, 0, -1), ([129], {}, P, BYTES, -1), ([0], {}, P, 0, -1),
+    ([], {"len": 0}, P, 0, -1), ([50, 50], {}, P, BYTES, -1), ([100], {"P": 4}, P, BYTES, -1), ([100], {"prefix_kv": P}, P, BYTES, -1),
+    ([100], {"k": 0}, P, BYTES, -1), ([100], {"v": 0}, P, BYTES, -1), ([100], {"ldk": 1020}, P, BYTES, -1), ([100], {"v": P + 4}, P, BYTES, -1),
+    ([100], {"k_norm": P + 4}, P, BYTES, -1), ([100], {"rope_cs": P, "rope_sin_off": 99 * 64}, P, BYTES, -1),
+    ([100], {"D": 64}, P, BYTES, -5), ([100], {"group": 4}, P, BYTES, -1), ([100], {"precision": 2}, P, BYTES, -1)])
+def test_prepare(checks, lens, change, out, size, code):
+    rc, msg = call(checks.t_prepare, ctypes.byref(prefix_desc(lens, **dict(PREP, **change))), v(out), I64(size))
+    assert rc == code and (code == 0 or "anima_attention_prefix" in msg)
+
+
 @pytest.mark.parametrize("p", [0, 1, 63, 64, 65, 1000, 1 << 22])
 @pytest.mark.parametrize("prec", [0, 1])
 def test_prefix_bytes(checks, p, prec):
-    """The size the check asks for is the one anima_attention_prepare_kv's buffer has."""
+    """The size the check asks for is anima_attention_kv_bytes'."""
     assert checks.t_bytes(5, p, prec) == (amd().Context.attention_kv_bytes(1, 5, p, prec) if p else 0)
 
 
