@@ -332,8 +332,8 @@ def _keep(s):
     if case["p"]:
         p, hkv = case["p"], case["hkv"]
         s.prefix = torch.empty(ctx.attention_kv_bytes(1, hkv, p, s.precision), dtype=torch.uint8, device="cuda")
-        ctx.attention(q=_ptr(t["pk"]), k=_ptr(t["pk"]), v=_ptr(t["pv"]), o=_ptr(t["pk"]), B=1, Lq=p, Lk=p, H=hkv, D=HD, ldq=hkv * HD,
-                      ldk=hkv * HD, ldv=hkv * HD, precision=s.precision, prepare_into=_ptr(s.prefix))
+        ctx.attention_prefix(k=_ptr(t["pk"]), v=_ptr(t["pv"]), lens=[p], H=hkv, ldk=hkv * HD, ldv=hkv * HD, precision=s.precision,
+                             prepare_into=_ptr(s.prefix))
         ctx.sync()
 
 
