@@ -28,16 +28,23 @@ struct PrefixSeqs {
   int start[PSEQ + 1];  // first packed row of each, then the number of rows
 };
 
-// The sequence of packed row l (rows past the last count to the last one).
-__device__ __forceinline__ int seq_of(const PrefixSeqs& s, int l) {
-  int lo = 0, hi = s.n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (s.start[mid] <= l) lo = mid;
-    else hi = mid - 1;
+// The sequences' first rows in LDS: a search there is a few LDS reads, in the arguments as many trips to memory.
+struct SeqStarts {
+  int at[PSEQ + 1];
+  __device__ __forceinline__ void fill(const PrefixSeqs& s) {  // (a barrier follows)
+    for (int i = threadIdx.x; i <= s.n; i += blockDim.x) at[i] = s.start[i];
   }
-  return lo;
-}
+  // the sequence of packed row l
+  __device__ __forceinline__ int of(int n, int l) const {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (at[mid] <= l) lo = mid;
+      else hi = mid - 1;
+    }
+    return lo;
+  }
+};
 
 struct PrefixArgs {
   const float* q;
@@ -92,8 +99,11 @@ template <class T>
 __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a) {
   constexpr bool BF = sizeof(T) == 2;
   __shared__ int bad[64];
+  __shared__ SeqStarts seq;
   const int t = threadIdx.x, w = t >> 6, lane = t & 63, kb0 = blockIdx.x * 64, hk = blockIdx.y;
   if (t < 64) bad[t] = 0;
+  seq.fill(a.seq);
+  __syncthreads();
   const int q16 = lane & 15, rsub = lane >> 4, vq = lane & 7, vc = lane >> 3;
   const auto vkey = [&](int e) { return BF ? kb0 + 16 * (vc >> 1) + 4 * (vc & 1) + (e & 3) + 8 * (e >> 2) : kb0 + 8 * vc + e; };
   f32x4 klo[4], khi[4], ve[8], cv[4], sv[4], wl{}, wh{};
@@ -104,7 +114,7 @@ __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a) {
     klo[i] = *(const f32x4*)src;
     khi[i] = *(const f32x4*)(src + 64);
     if (a.cs) {
-      const float* cr = a.cs + (int64_t)(a.P + l - a.seq.start[seq_of(a.seq, l)]) * 64 + 4 * q16;
+      const float* cr = a.cs + (int64_t)(a.P + l - seq.at[seq.of(a.seq.n, l)]) * 64 + 4 * q16;
       cv[i] = *(const f32x4*)cr;
       sv[i] = *(const f32x4*)(cr + a.sin_off);
     }
@@ -115,7 +125,6 @@ __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a) {
   }
 #pragma unroll
   for (int e = 0; e < 8; e++) ve[e] = *(const f32x4*)(a.v + (int64_t)min(vkey(e), a.T - 1) * a.ldv + hk * PHD + 32 * w + 4 * vq);
-  __syncthreads();
   const auto finite = [](f32x4 v, auto as) {
     float m = 0.0f;
 #pragma unroll
@@ -190,8 +199,11 @@ __global__ __launch_bounds__(256) void prefix_rows_kernel(PrefixArgs a) {
   const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int l = (int)(i / a.H), h = (int)(i - (int64_t)l * a.H), hk = h / a.group;
+  __shared__ SeqStarts seq;
+  seq.fill(a.seq);
+  __syncthreads();
   if (l >= a.T) return;
-  const int b = seq_of(a.seq, l), lo = a.seq.start[b], hi = a.causal ? l + 1 : a.seq.start[b + 1];
+  const int b = seq.of(a.seq.n, l), lo = seq.at[b], hi = a.causal ? l + 1 : seq.at[b + 1];
   float q0 = a.q[(int64_t)l * a.ldq + h * PHD + lane], q1 = a.q[(int64_t)l * a.ldq + h * PHD + lane + 64];
   row_norm_rope(a, a.qn, a.P + l - lo, q0, q1);
   q0 = (float)(T)(q0 * a.c);
@@ -273,13 +285,16 @@ __device__ __forceinline__ float p_pair_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// a value that is the same in all lanes, in a scalar register (quotients are formed in vector ones)
+__device__ __forceinline__ int p_same(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // The key blocks of a tile: `full` whole ones (nP of the prefix, then own ones from of0), then the cut ones (the
 // prefix's last, then own ones from ob0 up to of0 and from of1 up to ob1).
 struct PrefixBlocks {
   int nP, of0, full, tail, ob0, cut0, of1, total;
-  __device__ __forceinline__ PrefixBlocks(const PrefixArgs& a, int row0, int row1) {  // rows row0 .. row1
-    const int b0 = seq_of(a.seq, row0), b1 = seq_of(a.seq, row1), s0 = a.seq.start[b0];
-    const int end = a.causal ? row1 + 1 : a.seq.start[b1 + 1];
+  __device__ __forceinline__ PrefixBlocks(const PrefixArgs& a, const SeqStarts& seq, int row0, int row1) {  // rows row0 .. row1
+    const int b0 = p_same(seq.of(a.seq.n, row0)), b1 = p_same(seq.of(a.seq.n, row1)), s0 = p_same(seq.at[b0]);
+    const int end = a.causal ? row1 + 1 : p_same(seq.at[b1 + 1]);
     const int hi = b0 != b1 ? 0 : a.causal ? row0 + 1 : end;  // keys s0 .. hi are seen by all
     nP = a.P / PBK;
     tail = a.P % PBK ? 1 : 0;
@@ -343,35 +358,40 @@ __device__ __forceinline__ void p_load_q(const PrefixArgs& a, const float* src, 
 template <int NW>
 __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_bf16(PrefixArgs a) {
   constexpr int CPW = 16 / NW;  // copies of K, and of V^T, a wave and block
-  __shared__ __attribute__((aligned(1024))) char smem[PNST * PST];
+  // (one LDS object: beside a second one the compiler has every read of the stages wait for all copies in flight)
+  __shared__ __attribute__((aligned(1024))) char smem[PNST * PST + sizeof(SeqStarts)];
+  SeqStarts& seq = *(SeqStarts*)(smem + PNST * PST);
+  seq.fill(a.seq);
+  __syncthreads();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 31, hf = lane >> 5;
   // tiles of a head and split follow each other (on one XCD: they read the same blocks)
-  const int id = xcd_remap(blockIdx.x, gridDim.x), hs = id / a.nt, tile = id - hs * a.nt, hk = hs / a.splits, sp = hs - hk * a.splits;
+  const int id = xcd_remap(blockIdx.x, gridDim.x), hs = p_same(id / a.nt), tile = id - hs * a.nt, hk = p_same(hs / a.splits),
+            sp = hs - hk * a.splits;
   const int v0 = tile * 32 * NW, v = v0 + 32 * wave + r;
-  const PrefixBlocks B(a, v0 / a.group, (min(v0 + 32 * NW, a.V) - 1) / a.group);
-  const int i0 = (int)((int64_t)B.total * sp / a.splits), i1 = (int)((int64_t)B.total * (sp + 1) / a.splits), nb = i1 - i0;
+  const PrefixBlocks B(a, seq, p_same(v0 / a.group), p_same((min(v0 + 32 * NW, a.V) - 1) / a.group));
+  const int each = p_same(B.total / a.splits), more = B.total - each * a.splits;  // (blocks of a part: each, and one more of the first)
+  const int i0 = sp * each + min(sp, more), nb = each + (sp < more ? 1 : 0), i1 = i0 + nb;
   const bool live = v0 + 32 * wave < a.V;  // the wave has rows
 
   const int64_t pb = (int64_t)a.Pp * PHD * 2, ob = (int64_t)a.Tp * PHD * 2;
   const __amdgpu_buffer_rsrc_t rpk = p_rsrc((const char*)a.pk + hk * pb, a.P ? pb : 0), rpv = p_rsrc((const char*)a.pvt + hk * pb, a.P ? pb : 0),
                                rok = p_rsrc((const char*)a.ok + hk * ob, ob), rov = p_rsrc((const char*)a.ovt + hk * ob, ob);
-  uint32_t ko[CPW], vd[CPW], vu[CPW];
+  uint32_t ko[CPW], vp[CPW], vo[CPW];
 #pragma unroll
   for (int c = 0; c < CPW; c++) {
     const int row = 4 * (wave * CPW + c) + (lane >> 4), d = 8 * (wave * CPW + c) + (lane >> 3);
     ko[c] = row * 256 + 16 * ((lane & 15) ^ (row & 15));
-    vd[c] = d;
-    vu[c] = 16 * ((lane & 7) ^ ((d >> 1) & 7));
+    vp[c] = d * a.Pp * 2 + 16 * ((lane & 7) ^ ((d >> 1) & 7));
+    vo[c] = d * a.Tp * 2 + 16 * ((lane & 7) ^ ((d >> 1) & 7));
   }
   const auto load = [&](int j) __attribute__((always_inline)) {  // block j of the part (past the last: that one again, unused)
     bool pre;
     const int blk = B.at(i0 + min(j, nb - 1), pre);
     char* st = smem + (j & 3) * PST;
-    const uint32_t ld = 2 * (pre ? a.Pp : a.Tp);
 #pragma unroll
     for (int c = 0; c < CPW; c++) p_copy16(pre ? rpk : rok, st + (wave * CPW + c) * 1024, ko[c], blk * (64 * 256));
 #pragma unroll
-    for (int c = 0; c < CPW; c++) p_copy16(pre ? rpv : rov, st + PKT + (wave * CPW + c) * 1024, vd[c] * ld + vu[c], blk * 128);
+    for (int c = 0; c < CPW; c++) p_copy16(pre ? rpv : rov, st + PKT + (wave * CPW + c) * 1024, pre ? vp[c] : vo[c], blk * 128);
   };
   if (nb > 0) {
     load(0);
@@ -380,8 +400,8 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_bf16(PrefixArgs 
   }
 
   // the lane's row
-  const int vc = min(v, a.V - 1), row = vc / a.group, h = hk * a.group + vc - row * a.group, sq = seq_of(a.seq, row);
-  const int klo = a.seq.start[sq], khi = a.causal ? row + 1 : a.seq.start[sq + 1];
+  const int vc = min(v, a.V - 1), row = vc / a.group, h = hk * a.group + vc - row * a.group, sq = seq.of(a.seq.n, row);
+  const int klo = seq.at[sq], khi = a.causal ? row + 1 : seq.at[sq + 1];
   f16x8 qf[8];
   {
     float x[64];
@@ -455,12 +475,12 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_bf16(PrefixArgs 
   // A block that every row sees whole, after another: the written order is kept (each product's fragment was read four
   // reads before it, one half's exponentials run beside the next products).
   f32x16 negm;
-  const auto whole = [&](const char* st) __attribute__((always_inline)) {
+  bf16x8 f[4];  // the block's first fragments; at its end the next one's (st: the block, nx: the next)
+  const auto whole = [&](const char* st, const char* nx) __attribute__((always_inline)) {
     const auto frag = [&](int i) __attribute__((always_inline)) {
       return i < 16 ? *(const bf16x8*)(st + kof[i & 7] + (i >> 3) * 8192)
                     : *(const bf16x8*)(st + vof[(i - 16) >> 3 << 1 | (i & 1)] + (((i - 16) & 7) >> 1) * 4096);
     };
-    bf16x8 f[4] = {frag(0), frag(1), frag(2), frag(3)};
     f32x16 s[2];
     bf16x8 p[4];
     float la = 0.0f, lb = 0.0f;
@@ -511,29 +531,35 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_bf16(PrefixArgs 
         P_SB();
       }
       o[(j & 7) >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[j & 3], p[j >> 3 << 1 | (j & 1)], o[(j & 7) >> 1], 0, 0, 0);
-      if (j < 12) f[j & 3] = frag(j + 20);
+      f[j & 3] = j < 12 ? frag(j + 20) : *(const bf16x8*)(nx + kof[j - 12]);
       if (j < 8) prob2(1, j);
       P_SB();
     }
   };
 
-  // Block j in stage j % 4.  At the top of its turn this wave's copies of it have arrived (those of the two blocks after it may
-  // pend); behind the barrier everyone's have, and the stage of block j - 1 is refilled.
+  // Block j in stage j % 4.  At the top of its turn this wave's copies of block j + 1 have arrived (those of the block after it
+  // may pend); behind the barrier everyone's have, so that its first fragments are read under block j's last products, and the
+  // stage of block j - 1 is refilled.
   const auto turn = [&](int j) __attribute__((always_inline)) {
-    P_WAIT_VM(2 * 2 * CPW);
+    P_WAIT_VM(2 * CPW);
     p_barrier();
     load(j + 3);
     return (const char*)smem + (j & 3) * PST;
   };
+  const auto after = [&](int j) __attribute__((always_inline)) { return (const char*)smem + ((j + 1) & 3) * PST; };
   const int nf = max(min(B.full, i1) - i0, 0);
   int j = 0;
   if (nf > 0) {
     const char* st = turn(0);
-    if (live) block(st, std::false_type{}, 0, 0, 0);
+    if (live) {
+      block(st, std::false_type{}, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < 4; i++) f[i] = *(const bf16x8*)(after(0) + kof[i]);
+    }
     negm = f32x16{} - m;
     for (j = 1; j < nf; j++) {
       st = turn(j);
-      if (live) whole(st);
+      if (live) whole(st, after(j));
     }
   }
   for (; j < nb; j++) {
@@ -582,21 +608,36 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_bf16(PrefixArgs 
   }
 }
 
-// The parts of a split call, a half wave per virtual row: o = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s.
+// The parts of a split call, a half wave per virtual row: o = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s, eight parts asked for
+// at a time.
 __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixArgs a) {
   const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), n = (int64_t)a.Hkv * a.V;
   if (i >= n) return;
   const int d = 4 * (threadIdx.x & 31);
-  float m = M_NONE;
-  for (int s = 0; s < a.splits; s++) m = fmaxf(m, a.pml[(s * n + i) * 2]);
-  float l = 0.0f;
+  float m = M_NONE, l = 0.0f;
   f32x4 o = {};
-  for (int s = 0; s < a.splits; s++) {
-    const float2 ml = *(const float2*)(a.pml + (s * n + i) * 2);
-    const float f = __builtin_amdgcn_exp2f(ml.x - m);
-    const f32x4 w = *(const f32x4*)(a.po + (s * n + i) * PHD + d);
-    l += f * ml.y;
-    o += f * w;
+  for (int s0 = 0; s0 < a.splits; s0 += 8) {
+    float2 ml[8];
+    f32x4 w[8];
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+      const int64_t p = min(s0 + u, a.splits - 1) * n + i;
+      ml[u] = *(const float2*)(a.pml + p * 2);
+      w[u] = *(const f32x4*)(a.po + p * PHD + d);
+    }
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < 8; u++) mn = fmaxf(mn, ml[u].x);
+    const float g = __builtin_amdgcn_exp2f(m - mn);
+    l *= g;
+    o *= g;
+    m = mn;
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+      const float f = s0 + u < a.splits ? __builtin_amdgcn_exp2f(ml[u].x - m) : 0.0f;
+      l += f * ml[u].y;
+      if (f != 0.0f) o += f * w[u];
+    }
   }
   o *= 1.0f / l;
   const int hk = (int)(i / a.V), v = (int)(i - (int64_t)hk * a.V);
