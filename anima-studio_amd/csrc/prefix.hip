@@ -72,20 +72,11 @@ struct PrefixArgs {
   PrefixSeqs seq;
 };
 
-// One packed row of q or k in a wave, lane l holding dims l and l + 64: RMS norm, then the rotation.
-__device__ __forceinline__ void row_norm_rope(const PrefixArgs& a, const float* w, int pos, float& x0, float& x1) {
-  const int lane = threadIdx.x & 63;
-  if (w) {
-    const float rn = 1.0f / sqrtf(wave_sum(x0 * x0 + x1 * x1) / 128.0f + a.eps);
-    x0 = x0 * rn * w[lane];
-    x1 = x1 * rn * w[lane + 64];
-  }
-  if (a.cs) {
-    const float c = a.cs[(int64_t)pos * 64 + lane], s = a.cs[a.sin_off + (int64_t)pos * 64 + lane];
-    const float y0 = x0 * c - x1 * s;
-    x1 = x1 * c + x0 * s;
-    x0 = y0;
-  }
+// A workgroup barrier that waits for nothing: what it publishes has been waited for before it.
+__device__ __forceinline__ void p_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
 // One workgroup per 64 packed rows and kv head; rows T .. Tp are zeros.  K: 16 lanes a row, lane q holding dims 4 q .. + 3 and
@@ -101,9 +92,6 @@ __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a) {
   __shared__ int bad[64];
   __shared__ SeqStarts seq;
   const int t = threadIdx.x, w = t >> 6, lane = t & 63, kb0 = blockIdx.x * 64, hk = blockIdx.y;
-  if (t < 64) bad[t] = 0;
-  seq.fill(a.seq);
-  __syncthreads();
   const int q16 = lane & 15, rsub = lane >> 4, vq = lane & 7, vc = lane >> 3;
   const auto vkey = [&](int e) { return BF ? kb0 + 16 * (vc >> 1) + 4 * (vc & 1) + (e & 3) + 8 * (e >> 2) : kb0 + 8 * vc + e; };
   f32x4 klo[4], khi[4], ve[8], cv[4], sv[4], wl{}, wh{};
@@ -113,6 +101,16 @@ __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a) {
     const float* src = a.k + (int64_t)l * a.ldk + hk * PHD + 4 * q16;
     klo[i] = *(const f32x4*)src;
     khi[i] = *(const f32x4*)(src + 64);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; e++) ve[e] = *(const f32x4*)(a.v + (int64_t)min(vkey(e), a.T - 1) * a.ldv + hk * PHD + 32 * w + 4 * vq);
+  if (t < 64) bad[t] = 0;
+  seq.fill(a.seq);
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // (LDS alone: the loads above go on)
+  p_barrier();
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int l = min(kb0 + 16 * w + 4 * i + rsub, a.T - 1);
     if (a.cs) {
       const float* cr = a.cs + (int64_t)(a.P + l - seq.at[seq.of(a.seq.n, l)]) * 64 + 4 * q16;
       cv[i] = *(const f32x4*)cr;
@@ -123,8 +121,6 @@ __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a) {
     wl = *(const f32x4*)(a.kn + 4 * q16);
     wh = *(const f32x4*)(a.kn + 64 + 4 * q16);
   }
-#pragma unroll
-  for (int e = 0; e < 8; e++) ve[e] = *(const f32x4*)(a.v + (int64_t)min(vkey(e), a.T - 1) * a.ldv + hk * PHD + 32 * w + 4 * vq);
   const auto finite = [](f32x4 v, auto as) {
     float m = 0.0f;
 #pragma unroll
@@ -193,55 +189,6 @@ __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a) {
   }
 }
 
-// A wave per packed row and head, one key at a time, running maximum and sum.
-template <class T>
-__global__ __launch_bounds__(256) void prefix_rows_kernel(PrefixArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  const int l = (int)(i / a.H), h = (int)(i - (int64_t)l * a.H), hk = h / a.group;
-  __shared__ SeqStarts seq;
-  seq.fill(a.seq);
-  __syncthreads();
-  if (l >= a.T) return;
-  const int b = seq.of(a.seq.n, l), lo = seq.at[b], hi = a.causal ? l + 1 : seq.at[b + 1];
-  float q0 = a.q[(int64_t)l * a.ldq + h * PHD + lane], q1 = a.q[(int64_t)l * a.ldq + h * PHD + lane + 64];
-  row_norm_rope(a, a.qn, a.P + l - lo, q0, q1);
-  q0 = (float)(T)(q0 * a.c);
-  q1 = (float)(T)(q1 * a.c);
-  float m = -INFINITY, sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
-  auto keys = [&](const T* k, const T* vt, int64_t ld, int j0, int j1) {
-    k += (int64_t)hk * ld * PHD;
-    vt += (int64_t)hk * ld * PHD;
-    for (int j = j0; j < j1; j++) {
-      const float s = wave_sum(q0 * (float)k[(int64_t)j * PHD + lane] + q1 * (float)k[(int64_t)j * PHD + lane + 64]);
-      if (s > m) {
-        const float r = __builtin_amdgcn_exp2f(m - s);  // (0 at the first key)
-        sum *= r;
-        o0 *= r;
-        o1 *= r;
-        m = s;
-      }
-      const float p = __builtin_amdgcn_exp2f(s - m);
-      const int jp = j;
-      sum += p;
-      o0 += p * (float)vt[lane * ld + jp];
-      o1 += p * (float)vt[(lane + 64) * ld + jp];
-    }
-  };
-  keys((const T*)a.pk, (const T*)a.pvt, a.Pp, 0, a.P);
-  keys((const T*)a.ok, (const T*)a.ovt, a.Tp, lo, hi);
-  const float inv = 1.0f / sum;
-  if (a.obf) {
-    bf16* o = (bf16*)a.o + (int64_t)l * a.ldo + h * PHD;
-    o[lane] = to_bf16(o0 * inv);
-    o[lane + 64] = to_bf16(o1 * inv);
-  } else {
-    float* o = (float*)a.o + (int64_t)l * a.ldo + h * PHD;
-    o[lane] = o0 * inv;
-    o[lane + 64] = o1 * inv;
-  }
-}
-
 // ------------------------------------------------------------------ bf16 tiles
 //
 // A workgroup takes 32 NW virtual rows of one kv head (a wave 32 of them) and a part of their key blocks of 64: first the
@@ -264,11 +211,6 @@ constexpr int PNST = 4;
 #define P_WAIT_VM(n) __builtin_amdgcn_s_waitcnt(((n) & 15) | (7 << 4) | (15 << 8) | (((n) >> 4) << 14))
 #define P_SB() __builtin_amdgcn_sched_barrier(0)
 
-__device__ __forceinline__ void p_barrier() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t p_rsrc(const void* p, int64_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)p, (short)0, (int)bytes, 0x00020000);
 }
@@ -321,37 +263,37 @@ struct PrefixBlocks {
   }
 };
 
-// q of virtual row v: the lane's dims 16 ks + 8 hf + j in x[8 ks + j], normed, rotated at pos.
-__device__ __forceinline__ void p_load_q(const PrefixArgs& a, const float* src, int pos, int hf, float (&x)[64]) {
+// A row's lane part: dims 16 ks + 8 hf + j in x[8 ks + j] (NK of the eight ks).
+template <int NK>
+__device__ __forceinline__ void p_load(const float* src, int hf, float (&x)[8 * NK]) {
 #pragma unroll
-  for (int ks = 0; ks < 8; ks++) {
-    const f32x4 lo = *(const f32x4*)(src + 16 * ks + 8 * hf), hi = *(const f32x4*)(src + 16 * ks + 8 * hf + 4);
+  for (int ks = 0; ks < NK; ks++)
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      x[8 * ks + j] = lo[j];
-      x[8 * ks + 4 + j] = hi[j];
+    for (int q = 0; q < 2; q++) {
+      const f32x4 w = *(const f32x4*)(src + 16 * ks + 8 * hf + 4 * q);
+#pragma unroll
+      for (int j = 0; j < 4; j++) x[8 * ks + 4 * q + j] = w[j];
     }
-  }
+}
+
+// The row's RMS norm (qw: its weights) and rotation (cs, sn), x, qw, cs and sn as p_load leaves them.
+__device__ __forceinline__ void p_norm_rope(const PrefixArgs& a, const float (&qw)[64], const float (&cs)[32], const float (&sn)[32],
+                                            float (&x)[64]) {
   if (a.qn) {
     float ss = 0.0f;
 #pragma unroll
     for (int i = 0; i < 64; i++) ss = __builtin_fmaf(x[i], x[i], ss);
-    const float rn = 1.0f / sqrtf(p_pair_sum(ss) / 128.0f + a.eps);
+    const float f = 1.0f / sqrtf(p_pair_sum(ss) / 128.0f + a.eps);
 #pragma unroll
-    for (int ks = 0; ks < 8; ks++)
-#pragma unroll
-      for (int j = 0; j < 8; j++) x[8 * ks + j] = x[8 * ks + j] * rn * a.qn[16 * ks + 8 * hf + j];
+    for (int i = 0; i < 64; i++) x[i] = x[i] * f * qw[i];
   }
   if (a.cs) {
-    const float* cr = a.cs + (int64_t)pos * 64 + 8 * hf;
 #pragma unroll
-    for (int ks = 0; ks < 4; ks++)
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const float c = cr[16 * ks + j], s = cr[a.sin_off + 16 * ks + j], x1 = x[8 * ks + j], x2 = x[8 * ks + 32 + j];
-        x[8 * ks + j] = x1 * c - x2 * s;
-        x[8 * ks + 32 + j] = x2 * c + x1 * s;
-      }
+    for (int i = 0; i < 32; i++) {
+      const float x1 = x[i], x2 = x[32 + i];
+      x[i] = x1 * cs[i] - x2 * sn[i];
+      x[32 + i] = x2 * cs[i] + x1 * sn[i];
+    }
   }
 }
 
@@ -361,13 +303,19 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_bf16(PrefixArgs 
   // (one LDS object: beside a second one the compiler has every read of the stages wait for all copies in flight)
   __shared__ __attribute__((aligned(1024))) char smem[PNST * PST + sizeof(SeqStarts)];
   SeqStarts& seq = *(SeqStarts*)(smem + PNST * PST);
-  seq.fill(a.seq);
-  __syncthreads();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 31, hf = lane >> 5;
   // tiles of a head and split follow each other (on one XCD: they read the same blocks)
   const int id = xcd_remap(blockIdx.x, gridDim.x), hs = p_same(id / a.nt), tile = id - hs * a.nt, hk = p_same(hs / a.splits),
             sp = hs - hk * a.splits;
   const int v0 = tile * 32 * NW, v = v0 + 32 * wave + r;
+  // the lane's row, asked for before anything that takes a search (the barrier waits for LDS alone)
+  const int vc = min(v, a.V - 1), row = vc / a.group, h = hk * a.group + vc - row * a.group;
+  float x[64], qw[64];
+  p_load<8>(a.q + (int64_t)row * a.ldq + h * PHD, hf, x);
+  if (a.qn) p_load<8>(a.qn, hf, qw);
+  seq.fill(a.seq);
+  __builtin_amdgcn_s_waitcnt(0xc07f);
+  p_barrier();
   const PrefixBlocks B(a, seq, p_same(v0 / a.group), p_same((min(v0 + 32 * NW, a.V) - 1) / a.group));
   const int each = p_same(B.total / a.splits), more = B.total - each * a.splits;  // (blocks of a part: each, and one more of the first)
   const int i0 = sp * each + min(sp, more), nb = each + (sp < more ? 1 : 0), i1 = i0 + nb;
@@ -399,13 +347,16 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_bf16(PrefixArgs 
     load(2);
   }
 
-  // the lane's row
-  const int vc = min(v, a.V - 1), row = vc / a.group, h = hk * a.group + vc - row * a.group, sq = seq.of(a.seq.n, row);
-  const int klo = seq.at[sq], khi = a.causal ? row + 1 : seq.at[sq + 1];
+  const int sq = seq.of(a.seq.n, row), klo = seq.at[sq], khi = a.causal ? row + 1 : seq.at[sq + 1];
+  float cs[32], sn[32];
+  if (a.cs) {
+    const float* cr = a.cs + (int64_t)(a.P + row - klo) * 64;
+    p_load<4>(cr, hf, cs);
+    p_load<4>(cr + a.sin_off, hf, sn);
+  }
+  p_norm_rope(a, qw, cs, sn, x);
   f16x8 qf[8];
   {
-    float x[64];
-    p_load_q(a, a.q + (int64_t)row * a.ldq + h * PHD, a.P + row - klo, hf, x);
 #pragma unroll
     for (int ks = 0; ks < 8; ks++)
 #pragma unroll
@@ -608,6 +559,147 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_bf16(PrefixArgs 
   }
 }
 
+// ------------------------------------------------------------------ fp32 tiles
+//
+// The same parts on the fp32 matrix cores (64 cycles an instruction, which bound it): 128 virtual rows a workgroup, two
+// workgroups a CU, which cover each other's loads.  p = 2^(s - m) with m raised where a block's maximum passes it by more than 8.
+// A block's products of V are added by themselves first: chains of one step a block across blocks.
+constexpr int PKS = PHD + 4, PVS = 64 + 4;  // floats between rows of K and of V^T in LDS
+
+__global__ __launch_bounds__(256, 2) void prefix_flash_fp32(PrefixArgs a) {
+  __shared__ __attribute__((aligned(16))) float smem[64 * PKS + PHD * PVS + sizeof(SeqStarts) / 4];
+  float* const Ks = smem;
+  float* const Vs = smem + 64 * PKS;
+  SeqStarts& seq = *(SeqStarts*)(smem + 64 * PKS + PHD * PVS);
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 31, hf = lane >> 5;
+  const int id = xcd_remap(blockIdx.x, gridDim.x), hs = p_same(id / a.nt), tile = id - hs * a.nt, hk = p_same(hs / a.splits),
+            sp = hs - hk * a.splits;
+  const int v0 = tile * 128, v = v0 + 32 * wave + r;
+  const int vc = min(v, a.V - 1), row = vc / a.group, h = hk * a.group + vc - row * a.group;
+  seq.fill(a.seq);
+  __syncthreads();
+  const PrefixBlocks B(a, seq, p_same(v0 / a.group), p_same((min(v0 + 128, a.V) - 1) / a.group));
+  const int each = p_same(B.total / a.splits), more = B.total - each * a.splits;
+  const int i0 = sp * each + min(sp, more), nb = each + (sp < more ? 1 : 0);
+  const int sq = seq.of(a.seq.n, row), klo = seq.at[sq], khi = a.causal ? row + 1 : seq.at[sq + 1];
+
+  // k-step 4 g + e of the scores: dim 8 g + e in lane half 0, 8 g + 4 + e in half 1, so that a lane reads its K values
+  // four steps at a time; lane keeps q's dim 8 g + 4 hf + e as qv[4 g + e]
+  float qv[64];
+  {
+    float x[64], qw[64], cs[32], sn[32];
+    p_load<8>(a.q + (int64_t)row * a.ldq + h * PHD, hf, x);
+    if (a.qn) p_load<8>(a.qn, hf, qw);
+    if (a.cs) {
+      const float* cr = a.cs + (int64_t)(a.P + row - klo) * 64;
+      p_load<4>(cr, hf, cs);
+      p_load<4>(cr + a.sin_off, hf, sn);
+    }
+    p_norm_rope(a, qw, cs, sn, x);
+#pragma unroll
+    for (int k8 = 0; k8 < 8; k8++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float lo = x[8 * k8 + e] * a.c, hi = x[8 * k8 + 4 + e] * a.c;
+        const float other = __shfl_xor(hf ? lo : hi, 32);  // half 0's dim 16 k8 + 4 + e, half 1's 16 k8 + 8 + e
+        qv[8 * k8 + e] = hf ? other : lo;
+        qv[8 * k8 + 4 + e] = hf ? hi : other;
+      }
+  }
+  f32x16 o[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) o[i] = f32x16{};
+  float m = M_NONE, l = 0.0f;
+  for (int j = 0; j < nb; j++) {
+    bool pre;
+    const int blk = B.at(i0 + j, pre), ld = pre ? a.Pp : a.Tp;
+    const float* kg = (const float*)(pre ? a.pk : a.ok) + ((int64_t)hk * ld + blk * 64) * PHD;
+    const float* vg = (const float*)(pre ? a.pvt : a.ovt) + (int64_t)hk * PHD * ld + blk * 64;
+    // K tile 64 x 128 floats, V^T tile 128 x 64: eight pieces of 4 floats of each per thread, consecutive threads
+    // consecutive pieces
+    f32x4 kr[8], vr[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int u = 256 * i + tid;
+      kr[i] = *(const f32x4*)(kg + 4 * u);
+      vr[i] = *(const f32x4*)(vg + (int64_t)(u >> 4) * ld + 4 * (u & 15));
+    }
+    if (j) __syncthreads();  // every wave is done with the previous block's tiles
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int u = 256 * i + tid;
+      *(f32x4*)(Ks + (u >> 5) * PKS + 4 * (u & 31)) = kr[i];
+      *(f32x4*)(Vs + (u >> 4) * PVS + 4 * (u & 15)) = vr[i];
+    }
+    __syncthreads();
+    f32x16 s0 = {}, s1 = {};
+    const float* kp = Ks + r * PKS + 4 * hf;
+#pragma unroll
+    for (int g = 0; g < 16; g++) {
+      const f32x4 k0 = *(const f32x4*)(kp + 8 * g), k1 = *(const f32x4*)(kp + 32 * PKS + 8 * g);
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        s0 = __builtin_amdgcn_mfma_f32_32x32x2f32(k0[e], qv[4 * g + e], s0, 0, 0, 0);
+        s1 = __builtin_amdgcn_mfma_f32_32x32x2f32(k1[e], qv[4 * g + e], s1, 0, 0, 0);
+      }
+    }
+    if (i0 + j >= B.full) {
+      const int lo = pre ? 0 : klo, hi = pre ? a.P : khi;
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        const int k = blk * 64 + 8 * (e >> 2) + 4 * hf + (e & 3);
+        if (k < lo || k >= hi) s0[e] = -INFINITY;
+        if (k + 32 < lo || k + 32 >= hi) s1[e] = -INFINITY;
+      }
+    }
+    float bm = fmaxf(s0[0], s1[0]);
+#pragma unroll
+    for (int e = 1; e < 16; e++) bm = fmaxf(bm, fmaxf(s0[e], s1[e]));
+    bm = p_pair_max(bm);
+    const bool need = bm > m + 8.0f;
+    if (__builtin_amdgcn_ballot_w64(need)) {
+      const float mn = need ? ceilf(bm) : m, f = __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < 4; i++) o[i] *= f;
+    }
+    float bl = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+      s0[e] = __builtin_amdgcn_exp2f(s0[e] - m);
+      s1[e] = __builtin_amdgcn_exp2f(s1[e] - m);
+      bl += s0[e] + s1[e];
+    }
+    l += bl;
+    // k-step (tile t, register e): keys 32 t + 8 (e / 4) + 4 hf + e % 4
+#pragma unroll
+    for (int dt = 0; dt < 4; dt++) {
+      const float* vrow = Vs + (32 * dt + r) * PVS;
+      f32x16 p = {};
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        const int key = 8 * (e >> 2) + 4 * hf + (e & 3);
+        p = __builtin_amdgcn_mfma_f32_32x32x2f32(vrow[key], s0[e], p, 0, 0, 0);
+        p = __builtin_amdgcn_mfma_f32_32x32x2f32(vrow[32 + key], s1[e], p, 0, 0, 0);
+      }
+      o[dt] += p;
+    }
+  }
+  l = p_pair_sum(l);
+  if (v >= a.V) return;
+  const bool part = a.splits > 1;
+  const float inv = part ? 1.0f : 1.0f / l;
+  const int64_t at = ((int64_t)sp * a.Hkv + hk) * a.V + v;
+  if (part && hf == 0) *(float2*)(a.pml + at * 2) = make_float2(m, l);
+  float* d = (part ? a.po + at * PHD : (float*)a.o + (int64_t)row * a.ldo + h * PHD) + 4 * hf;
+#pragma unroll
+  for (int dt = 0; dt < 4; dt++)
+#pragma unroll
+    for (int g = 0; g < 4; g++)
+      *(f32x4*)(d + 32 * dt + 8 * g) = f32x4{o[dt][4 * g] * inv, o[dt][4 * g + 1] * inv, o[dt][4 * g + 2] * inv, o[dt][4 * g + 3] * inv};
+}
+
 // The parts of a split call, a half wave per virtual row: o = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s, eight parts asked for
 // at a time.
 __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixArgs a) {
@@ -661,15 +753,10 @@ static int prefix_part(anima_ctx* c, PrefixArgs& a) {
   constexpr bool BF = sizeof(T) == 2;
   a.V = a.T * a.group;
   const int blocks = a.Pp / PBK + a.Tp / PBK;
-  bool eight = false;
-  a.splits = 1;
-  if (BF) {
-    eight = (int64_t)((a.V + 255) / 256) * a.Hkv >= c->num_cus;
-    const int rows = eight ? 256 : 128;
-    a.nt = (a.V + rows - 1) / rows;
-    const int64_t wgs = (int64_t)a.nt * a.Hkv;
-    a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({c->num_cus / wgs, blocks / 2, 64}));
-  }
+  const bool eight = BF && (int64_t)((a.V + 255) / 256) * a.Hkv >= c->num_cus;
+  const int rows = eight ? 256 : 128, fill = BF ? c->num_cus : 2 * c->num_cus;  // (two fp32 workgroups to a CU)
+  a.nt = (a.V + rows - 1) / rows;
+  a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({fill / ((int64_t)a.nt * a.Hkv), blocks / 2, 64}));
   const size_t plane = (size_t)a.Hkv * a.Tp * PHD * sizeof(T), n = a.splits > 1 ? (size_t)a.splits * a.Hkv * a.V : 0;
   void* ws = nullptr;
   if (int rc = workspace(c, 2 * plane + n * (PHD + 2) * 4, &ws)) return rc;
@@ -679,15 +766,12 @@ static int prefix_part(anima_ctx* c, PrefixArgs& a) {
   a.pml = a.po + n * PHD;
   if (int rc = prefix_prep_launch<T>(c, a)) return rc;
   Launch L(c, BF ? "attn.prefix_bf16" : "attn.prefix_fp32", 4.0 * a.T * a.H * PHD * a.P, 0.0);
-  if constexpr (BF) {
-    const dim3 grid((unsigned)((int64_t)a.nt * a.Hkv * a.splits));
-    if (eight) hipLaunchKernelGGL(prefix_flash_bf16<8>, grid, dim3(512), 0, c->stream, a);
-    else hipLaunchKernelGGL(prefix_flash_bf16<4>, grid, dim3(256), 0, c->stream, a);
-    if (a.splits > 1)
-      hipLaunchKernelGGL(prefix_join_kernel, dim3((unsigned)(((int64_t)a.Hkv * a.V + 7) / 8)), dim3(256), 0, c->stream, a);
-  } else {
-    hipLaunchKernelGGL(prefix_rows_kernel<T>, dim3((unsigned)(((int64_t)a.T * a.H + 3) / 4)), dim3(256), 0, c->stream, a);
-  }
+  const dim3 grid((unsigned)((int64_t)a.nt * a.Hkv * a.splits));
+  if (!BF) hipLaunchKernelGGL(prefix_flash_fp32, grid, dim3(256), 0, c->stream, a);
+  else if (eight) hipLaunchKernelGGL(prefix_flash_bf16<8>, grid, dim3(512), 0, c->stream, a);
+  else hipLaunchKernelGGL(prefix_flash_bf16<4>, grid, dim3(256), 0, c->stream, a);
+  if (a.splits > 1)
+    hipLaunchKernelGGL(prefix_join_kernel, dim3((unsigned)(((int64_t)a.Hkv * a.V + 7) / 8)), dim3(256), 0, c->stream, a);
   return L.end();
 }
 
