@@ -167,33 +167,86 @@ __device__ __forceinline__ void q4_store(const Q4Args& a, int64_t m, int n, floa
   else *c = __builtin_fmaf(a.gate[n], r, *c);
 }
 
-// One wave per output column and four rows, lanes striding k in pieces of eight, sums in fp32.
-__global__ __launch_bounds__(256) void q4_rows_kernel(Q4Args a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), m0 = (int64_t)blockIdx.y * 4;
-  if (n >= a.N) return;
-  const int live = min(4, a.M - (int)m0);
-  float acc[4] = {};
-  for (int k = 8 * lane; k < a.K; k += 512) {
-    const uint32_t c = *(const uint32_t*)(a.w + (n * a.K + k) / 2);
-    const int64_t g = n * (a.K / a.G) + k / a.G;
-    const float s = bf16_f(a.gs[g]), z = a.gz ? bf16_f(a.gz[g]) : 0.0f;
-    float w[8];
+// One to four rows on the vector units, in fp32: a wave takes U columns, a lane 16 consecutive k of each 1024 (eight bytes of
+// codes, one group).  x goes through LDS, quad j of lane l's 16 at [j][l], so that the reads touch every bank once.  A code with its
+// highest bit turned is c - 8 in two's complement: in a byte's upper half 16 (c - 8), one conversion away from a
+// float, and s takes the 16.
+// Bound by its launch and one trip to memory for the codes.
+template <int MR, int U>
+__global__ __launch_bounds__(256) void q4_gemv_kernel(Q4Args a) {
+  __shared__ f32x4 xs[2][MR][256];
+  const int tid = threadIdx.x, lane = tid & 63, n0 = (blockIdx.x * 4 + (tid >> 6)) * U, KG = a.K / a.G, lg = 31 - __builtin_clz(a.G);
+  float acc[MR][U] = {};
+  const uint8_t* w[U];
+  const uint16_t *gs[U], *gz[U];
 #pragma unroll
-    for (int j = 0; j < 8; j++) w[j] = __builtin_fmaf((float)((int)((c >> (4 * j)) & 15) - 8), s, z);
-#pragma unroll
-    for (int r = 0; r < 4; r++)
-      if (r < live) {
-        float x[8];
-        ld8(a.x + (m0 + r) * a.ldx + k, x);
-#pragma unroll
-        for (int j = 0; j < 8; j++) acc[r] = __builtin_fmaf(x[j], w[j], acc[r]);
-      }
+  for (int u = 0; u < U; u++) {
+    const int64_t n = min(n0 + u, a.N - 1);
+    w[u] = a.w + n * (a.K / 2);
+    gs[u] = a.gs + n * KG;
+    gz[u] = a.gz ? a.gz + n * KG : gs[u];
   }
+  for (int k0 = 0, p = 0; k0 < a.K; k0 += 1024, p ^= 1) {
+    const int k = min(k0 + 16 * lane, a.K - 16);  // (past the row's end its last 16: they meet zeros of x)
+    uint2 c[U];
+    uint16_t s[U], z[U];
 #pragma unroll
-  for (int r = 0; r < 4; r++) {
-    const float t = wave_sum(acc[r]);
-    if (lane == 0 && r < live) q4_store(a, m0 + r, (int)n, t);
+    for (int u = 0; u < U; u++) {
+      c[u] = *(const uint2*)(w[u] + k / 2);
+      s[u] = gs[u][k >> lg];
+      z[u] = gz[u][k >> lg];
+    }
+#pragma unroll
+    for (int m = 0; m < MR; m++) {
+      const int kq = k0 + 4 * tid;
+      const f32x4 v = *(const f32x4*)(a.x + min(m, a.M - 1) * a.ldx + min(kq, a.K - 4));
+      xs[p][m][(tid & 3) * 64 + (tid >> 2)] = kq < a.K ? v : f32x4{};
+    }
+    __syncthreads();  // (one a turn: the other buffer's readers are past it by the next)
+#pragma unroll
+    for (int m = 0; m < MR; m++) {
+      float t[U] = {}, sx = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {  // quad j: half a word of codes
+        const f32x4 x = xs[p][m][j * 64 + lane];
+        sx += (x[0] + x[1]) + (x[2] + x[3]);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          const uint32_t v = (j < 2 ? c[u].x : c[u].y) ^ 0x88888888u;
+          const uint32_t half[2] = {(v << 4) & 0xf0f0f0f0u, v & 0xf0f0f0f0u};  // (even and odd k)
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            t[u] = __builtin_fmaf(x[e], (float)(int8_t)(half[e & 1] >> (16 * (j & 1) + 8 * (e >> 1))), t[u]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        acc[m][u] = __builtin_fmaf(bf16_f(s[u]) * 0.0625f, t[u], acc[m][u]);
+        if (a.gz) acc[m][u] = __builtin_fmaf(bf16_f(z[u]), sx, acc[m][u]);
+      }
+    }
+  }
+  // The sums over the lanes: while a lane holds several outputs, the two of a pair keep half of them each.
+#pragma unroll
+  for (int m = 0; m < MR; m++) {
+    int cnt = U, first = 0;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+      if (cnt > 1) {
+        cnt >>= 1;
+        const bool hi = lane & d;
+#pragma unroll
+        for (int u = 0; u < U / 2; u++)
+          if (u < cnt) {
+            const float send = hi ? acc[m][u] : acc[m][u + cnt], keep = hi ? acc[m][u + cnt] : acc[m][u];
+            acc[m][u] = keep + __shfl_xor(send, d);
+          }
+        if (hi) first += cnt;
+      } else {
+        acc[m][0] += __shfl_xor(acc[m][0], d);
+      }
+    }
+    if ((lane & (64 / U - 1)) == 0 && m < a.M && n0 + first < a.N) q4_store(a, m, n0 + first, acc[m][0]);
   }
 }
 
@@ -230,7 +283,9 @@ struct Q4Prep {
   int M, N, K, Kp, G, rows;  // rows: workgroups of x rows (four each), the rest are of columns
 };
 
-// A wave per row of x, or per column's scales.  Two passes over the row, the second from the caches.
+// A wave per row of x (NV: pieces of 512 k that a wave holds; 0: two passes over the row, the second from the caches), or per
+// column's scales.
+template <int NV>
 __global__ __launch_bounds__(256) void q4_prep_kernel(Q4Prep a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if ((int)blockIdx.x >= a.rows) {
@@ -246,19 +301,19 @@ __global__ __launch_bounds__(256) void q4_prep_kernel(Q4Prep a) {
   const int64_t m = (int64_t)blockIdx.x * 4 + wave;
   if (m >= a.M) return;
   const float* x = a.x + m * a.ldx;
-  float mx = 0.0f;
-  for (int k = 4 * lane; k < a.K; k += 256) {
-    const f32x4 v = *(const f32x4*)(x + k);
+  const auto piece = [&](int k, float (&v)[8]) __attribute__((always_inline)) {  // (past K: zeros)
+    const bool in = k < a.K;
+    ld8(x + (in ? k : 0), v);
+    if (!in)
 #pragma unroll
-    for (int j = 0; j < 4; j++) mx = fmaxf(mx, fabsf(v[j]));
-  }
-  mx = wave_max(mx);
-  const int e = q4_exp(mx, 14);
-  const float f = pow2f(e);
-  if (lane == 0) a.rm[m] = pow2f(-e);
-  for (int k = 8 * lane; k < a.Kp; k += 512) {
-    float v[8] = {};
-    if (k < a.K) ld8(x + k, v);
+      for (int j = 0; j < 8; j++) v[j] = 0.0f;
+  };
+  const auto largest = [](const float (&v)[8], float mx) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(v[j]));
+    return mx;
+  };
+  const auto leave = [&](int k, const float (&v)[8], float f) __attribute__((always_inline)) {
     if (a.sx) {
       float t = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
       for (int s = 1; s < a.G / 8; s <<= 1) t += __shfl_xor(t, s);
@@ -272,8 +327,34 @@ __global__ __launch_bounds__(256) void q4_prep_kernel(Q4Prep a) {
       h[o] = (_Float16)y;
       l[o] = (_Float16)(y - (float)h[o]);
     }
-    *(f16x8*)(a.xh + m * a.Kp + k) = h;
-    if (a.xl) *(f16x8*)(a.xl + m * a.Kp + k) = l;
+    if (k < a.Kp) {
+      *(f16x8*)(a.xh + m * a.Kp + k) = h;
+      if (a.xl) *(f16x8*)(a.xl + m * a.Kp + k) = l;
+    }
+  };
+  float mx = 0.0f;
+  if constexpr (NV > 0) {
+    float v[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; i++) piece(8 * lane + 512 * i, v[i]);
+#pragma unroll
+    for (int i = 0; i < NV; i++) mx = largest(v[i], mx);
+    const int e = q4_exp(wave_max(mx), 14);
+    if (lane == 0) a.rm[m] = pow2f(-e);
+#pragma unroll
+    for (int i = 0; i < NV; i++) leave(8 * lane + 512 * i, v[i], pow2f(e));
+  } else {
+    float v[8];
+    for (int k = 8 * lane; k < a.K; k += 512) {
+      piece(k, v);
+      mx = largest(v, mx);
+    }
+    const int e = q4_exp(wave_max(mx), 14);
+    if (lane == 0) a.rm[m] = pow2f(-e);
+    for (int k = 8 * lane; k < (a.Kp + 511) / 512 * 512; k += 512) {
+      piece(k, v);
+      leave(k, v, pow2f(e));
+    }
   }
 }
 
@@ -348,6 +429,118 @@ __device__ __forceinline__ void q4_store4(const Q4Args& a, int vec, int64_t m, i
   }
   *c = r;
 }
+
+// ------------------------------------------------------------------ products of a few rows
+//
+// A workgroup takes 32 columns and 32 rows, its eight waves every eighth step of 64 k each, their sums joined in order
+// through LDS.  The codes stay whole numbers (exact in f16), and each group's sums meet their scale in fp32; scales and
+// middles lie in LDS as [group][column].  x comes as q4_prep_kernel leaves it (split here, again for each 32 columns, it took
+// 20 us of 43 x 1024 x 2048).
+constexpr int QF_WAVES = 8;
+
+template <int TERMS, bool G32>
+__global__ __launch_bounds__(64 * QF_WAVES, 2) void q4_few_kernel(Q4Tile q) {
+  constexpr int NG = G32 ? 2 : 1;  // groups in a step (of 64 k; groups of 128 meet it in two)
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const Q4Args& a = q.a;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 31, hf = lane >> 5;
+  const int n0 = blockIdx.x * 32, m0 = blockIdx.y * 32, KG = a.K / a.G, steps = q.Kp / 64;
+  float* const ss = (float*)smem;  // [KG][32]
+  float* const zs = ss + KG * 32;  // the middles, where there are
+  // a step's operands: codes 32 hf .. + 31 of column r; x's 16 i + 8 hf .. + 7 of row r; the groups' sums of x
+  struct Step {
+    u32x4 w;
+    f16x8 x[TERMS][4];
+    float sx[NG];
+  } st[2];
+  const uint8_t* wr = a.w + (int64_t)min(n0 + r, a.N - 1) * (a.K / 2);
+  const int64_t mr = min(m0 + r, a.M - 1), xo = mr * q.Kp + 8 * hf, so = mr * KG;
+  const auto load = [&](Step& v, int step) __attribute__((always_inline)) {  // (past the last step: that one again, unused)
+    const int k = 64 * min(step, steps - 1);
+    v.w = *(const u32x4*)(wr + min(k + 32 * hf, a.K - 32) / 2);  // (past the row's end its last 32: they meet zeros of x)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      v.x[0][i] = *(const f16x8*)(q.xh + xo + k + 16 * i);
+      if (TERMS > 1) v.x[TERMS - 1][i] = *(const f16x8*)(q.xl + xo + k + 16 * i);
+    }
+    if (a.gz)
+#pragma unroll
+      for (int g = 0; g < NG; g++) v.sx[g] = q.sx[so + min((k + 32 * g) / a.G, KG - 1)];
+  };
+  load(st[0], wave);
+  load(st[1], wave + QF_WAVES);
+  for (int i = tid; i < KG * 32; i += 64 * QF_WAVES) {
+    const int64_t at = (int64_t)min(n0 + (i & 31), a.N - 1) * KG + (i >> 5);
+    ss[i] = bf16_f(a.gs[at]);
+    if (a.gz) zs[i] = bf16_f(a.gz[at]);
+  }
+  const float rm = q.rm[mr], up = 1.0f / rm;  // (powers of two)
+  __builtin_amdgcn_s_waitcnt(0xc07f);
+  q4_barrier();
+  f32x16 acc = {};
+  const f16x2 one = {(_Float16)1.0f, (_Float16)1.0f};
+  const auto product = [&](const Step& v, int step) __attribute__((always_inline)) {
+    // the halves' words exchanged, so that matrix step i covers k 16 i .. 16 i + 15: lane half hf word 2 i + hf of 8
+    u32x4 w = v.w;
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      const auto e = __builtin_amdgcn_permlane32_swap(w[i], w[i + 1], false, false);
+      w[i] = e[0];      // k 8 i .. 8 i + 15
+      w[i + 1] = e[1];  // k 32 + 8 i ..
+    }
+    f32x16 part[NG];
+#pragma unroll
+    for (int g = 0; g < NG; g++) part[g] = f32x16{};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      f32x16& p = part[G32 ? i >> 1 : 0];
+      const f16x8 wf = q4_decode(w[i < 2 ? 2 * i : 2 * i - 3], one);
+#pragma unroll
+      for (int e = TERMS - 1; e >= 0; e--) p = __builtin_amdgcn_mfma_f32_32x32x16_f16(wf, v.x[e][i], p, 0, 0, 0);
+    }
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+      const int at = min((64 * step + 32 * g) / a.G, KG - 1) * 32 + 4 * hf;
+      // (a group of 128 meets its middle once; past K there is none)
+      const float sx = (G32 ? 64 * step + 32 * g < a.K : (64 * step) % a.G == 0) ? v.sx[g] * up : 0.0f;
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        const f32x4 s = *(const f32x4*)(ss + at + 8 * c);
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[4 * c + e] = __builtin_fmaf(part[g][4 * c + e], s[e], acc[4 * c + e]);
+        if (a.gz) {
+          const f32x4 z = *(const f32x4*)(zs + at + 8 * c);
+#pragma unroll
+          for (int e = 0; e < 4; e++) acc[4 * c + e] = __builtin_fmaf(z[e], sx, acc[4 * c + e]);
+        }
+      }
+    }
+  };
+  for (int s = wave; s < steps; s += 2 * QF_WAVES) {
+    product(st[0], s);
+    load(st[0], s + 2 * QF_WAVES);
+    if (s + QF_WAVES < steps) product(st[1], s + QF_WAVES);
+    load(st[1], s + 3 * QF_WAVES);
+  }
+  __syncthreads();  // (the scales' place becomes the sums')
+  f32x4* const sum = (f32x4*)smem;  // [wave][quad][lane]
+#pragma unroll
+  for (int c = 0; c < 4; c++) {
+    f32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = acc[4 * c + e] * rm;
+    sum[(wave * 4 + c) * 64 + lane] = v;
+  }
+  __syncthreads();
+  if (tid >= 256) return;
+  f32x4 v = sum[tid];
+#pragma unroll
+  for (int w = 1; w < QF_WAVES; w++) v = v + sum[w * 256 + tid];
+  const int c = tid >> 6, m = m0 + (lane & 31), n = n0 + 8 * c + 4 * (lane >> 5);
+  if (m < a.M && n < a.N) q4_store4(a, q.vec, m, n, v);
+}
+
+// ------------------------------------------------------------------ tiles
 
 // One BM x BN tile a workgroup, waves of WM rows x WN columns.  A step is 64 k: BM rows of x (128 bytes, each term) in one of four LDS
 // stages, filled three steps ahead by buffer_load ... lds, units of 16 bytes at slot u ^ (row / 2 % 8) (sixteen rows' reads of one
@@ -556,9 +749,14 @@ __global__ __launch_bounds__(256) void q4_join_kernel(Q4Tile t, int splits) {
   const float* p = t.part + m * a.N + n;
   const int64_t plane = (int64_t)a.M * a.N;
   f32x4 v = {};
-  for (int s = 0; s < splits; s++) {
-    if (t.vec) v = v + *(const f32x4*)(p + s * plane);
-    else
+  if (t.vec) {
+    f32x4 w[Q4_SPLITS];  // (all asked for before the first is added)
+#pragma unroll
+    for (int s = 0; s < Q4_SPLITS; s++) w[s] = s < splits ? *(const f32x4*)(p + s * plane) : f32x4{};
+#pragma unroll
+    for (int s = 0; s < Q4_SPLITS; s++) v = v + w[s];
+  } else {
+    for (int s = 0; s < splits; s++)
       for (int e = 0; e < 4; e++)
         if (n + e < a.N) v[e] += p[s * plane + e];
   }
@@ -607,7 +805,34 @@ int embed_rows_launch(anima_ctx* c, const anima_weight* W, const int32_t* ids, i
   return L.end();
 }
 
-constexpr int Q4_FEW = 8;
+constexpr int Q4_ROWS = 4;             // rows of the vector kernel
+constexpr int Q4_FEW_LDS = 65536;
+
+static void q4_gemv(anima_ctx* c, const Q4Args& a) {
+#define GEMV(MR, U) hipLaunchKernelGGL((q4_gemv_kernel<MR, U>), dim3((unsigned)((a.N + 4 * U - 1) / (4 * U))), dim3(256), 0, c->stream, a)
+#define GEMV_U(MR)                    \
+  do {                                \
+    if (a.N >= 4096) GEMV(MR, 4);     \
+    else if (a.N >= 2048) GEMV(MR, 2); \
+    else GEMV(MR, 1);                 \
+  } while (0)
+  if (a.M == 1) GEMV_U(1);
+  else if (a.M == 2) GEMV_U(2);
+  else GEMV_U(4);
+#undef GEMV_U
+#undef GEMV
+}
+
+// whether rows of out, bias, add and gate come in quads of 16 bytes (8 of bf16 rows)
+static int q4_vec(const Q4Args& a) {
+  return a.N % 4 == 0 && a.ldc % 4 == 0 && q4_al(a.out, a.obf ? 8 : 16) && q4_al(a.bias, 16) && q4_al(a.gate, 16) &&
+         (!a.add || (q4_al(a.add, 16) && a.ld_add % 4 == 0));
+}
+
+// LDS of the kernel for few rows: the scales and middles, then the waves' sums
+static int64_t q4_few_lds(const Q4Args& a) {
+  return std::max<int64_t>((int64_t)(a.K / a.G) * 128 * (a.gz ? 2 : 1), QF_WAVES * 4096);
+}
 
 template <int BM, int BN, int WM, int WN, int TERMS>
 static void q4_tile_launch(anima_ctx* c, const Q4Tile& t, int splits) {
@@ -615,23 +840,22 @@ static void q4_tile_launch(anima_ctx* c, const Q4Tile& t, int splits) {
   hipLaunchKernelGGL((q4_tile_kernel<BM, BN, WM, WN, TERMS>), grid, block, 0, c->stream, t);
 }
 
-// x into f16 terms and both sides' powers, then the tiles, then, where k was split, the sums.
-static int q4_tiles(anima_ctx* c, const Q4Args& a, bool two) {
+// x into f16 terms (and the columns' powers), then the products, then, where k was split, the sums.
+static int q4_matrix(anima_ctx* c, const Q4Args& a, bool two) {
   Q4Tile t{};
   t.a = a;
   t.Kp = (a.K + 63) / 64 * 64;
+  t.vec = q4_vec(a);
   const int KG = a.K / a.G, steps = t.Kp / 64;
+  const bool few = a.M <= 64 && q4_few_lds(a) <= Q4_FEW_LDS;
   const auto tiles = [&](int bm, int bn) { return (int64_t)((a.M + bm - 1) / bm) * ((a.N + bn - 1) / bn); };
   // the largest tile of which there are enough
   const int tile = tiles(two ? 128 : 256, 256) >= c->num_cus ? 0 : tiles(128, 128) >= c->num_cus ? 1 : 2;
   const int64_t nt = tile == 0 ? tiles(two ? 128 : 256, 256) : tile == 1 ? tiles(128, 128) : tiles(64, 64);
   int splits = 1;
-  while (splits < Q4_SPLITS && nt * splits * 2 <= c->num_cus && steps / (splits * 2) >= 4) splits *= 2;
+  while (!few && splits < Q4_SPLITS && nt * splits * 2 <= c->num_cus && steps / (splits * 2) >= 4) splits *= 2;
   t.sps = (steps + splits - 1) / splits;
   splits = (steps + t.sps - 1) / t.sps;
-  const auto al = [](const void* p, int b) { return ((uintptr_t)p & (uintptr_t)(b - 1)) == 0; };
-  t.vec = a.N % 4 == 0 && a.ldc % 4 == 0 && al(a.out, a.obf ? 8 : 16) && al(a.bias, 16) && al(a.gate, 16) &&
-          (!a.add || (al(a.add, 16) && a.ld_add % 4 == 0));
   // scratch: the terms, the powers, the group sums, the splits' sums
   size_t at = 0;
   const auto take = [&](size_t bytes) {
@@ -640,21 +864,35 @@ static int q4_tiles(anima_ctx* c, const Q4Args& a, bool two) {
     return o;
   };
   const size_t plane = (size_t)a.M * t.Kp * 2, oh = take(plane), ol = two ? take(plane) : 0, om = take((size_t)a.M * 4),
-               on = take(((size_t)a.N + 255) / 256 * 1024), os = a.gz ? take((size_t)a.M * KG * 4) : 0,
+               on = few ? 0 : take(((size_t)a.N + 255) / 256 * 1024), os = a.gz ? take((size_t)a.M * KG * 4) : 0,
                op = splits > 1 ? take((size_t)splits * a.M * a.N * 4) : 0;
   void* tmp = nullptr;
   if (int rc = anima_alloc(c, at, &tmp)) return rc;
   char* const b = (char*)tmp;
-  t.xh = (_Float16*)(b + oh);
-  t.xl = two ? (_Float16*)(b + ol) : nullptr;
-  t.rm = (float*)(b + om);
-  t.rn = (float*)(b + on);
-  t.sx = a.gz ? (float*)(b + os) : nullptr;
+  Q4Prep p{a.x, a.ldx, (_Float16*)(b + oh), two ? (_Float16*)(b + ol) : nullptr, (float*)(b + om), a.gz ? (float*)(b + os) : nullptr, a.gs,
+           (float*)(b + on), a.M, a.N, a.K, t.Kp, a.G, (a.M + 3) / 4};
+  t.xh = p.xh;
+  t.xl = p.xl;
+  t.rm = p.rm;
+  t.rn = p.rn;
+  t.sx = p.sx;
   t.part = splits > 1 ? (float*)(b + op) : nullptr;
-  Q4Prep p{a.x, a.ldx, (_Float16*)t.xh, (_Float16*)t.xl, (float*)t.rm, (float*)t.sx, a.gs, (float*)t.rn, a.M, a.N, a.K, t.Kp, a.G, (a.M + 3) / 4};
-  Launch L(c, tile == 0 ? "gemm.q4.256" : tile == 1 ? "gemm.q4.128" : "gemm.q4.64", 2.0 * a.M * a.N * a.K, 0.0);
-  hipLaunchKernelGGL(q4_prep_kernel, dim3((unsigned)(p.rows + (a.N + 3) / 4)), dim3(256), 0, c->stream, p);
-  if (two) {
+  Launch L(c, few ? "gemm.q4.few" : tile == 0 ? "gemm.q4.256" : tile == 1 ? "gemm.q4.128" : "gemm.q4.64", 2.0 * a.M * a.N * a.K, 0.0);
+  {
+    const dim3 grid((unsigned)(p.rows + (few ? 0 : (a.N + 3) / 4))), block(256);
+    if (a.K <= 1024) hipLaunchKernelGGL(q4_prep_kernel<2>, grid, block, 0, c->stream, p);
+    else if (a.K <= 2048) hipLaunchKernelGGL(q4_prep_kernel<4>, grid, block, 0, c->stream, p);
+    else if (a.K <= 8192) hipLaunchKernelGGL(q4_prep_kernel<16>, grid, block, 0, c->stream, p);
+    else hipLaunchKernelGGL(q4_prep_kernel<0>, grid, block, 0, c->stream, p);
+  }
+  if (few) {
+    const dim3 grid((unsigned)((a.N + 31) / 32), (unsigned)((a.M + 31) / 32)), block(64 * QF_WAVES);
+    const int lds = (int)q4_few_lds(a);
+    if (two && a.G == 32) hipLaunchKernelGGL((q4_few_kernel<2, true>), grid, block, lds, c->stream, t);
+    else if (two) hipLaunchKernelGGL((q4_few_kernel<2, false>), grid, block, lds, c->stream, t);
+    else if (a.G == 32) hipLaunchKernelGGL((q4_few_kernel<1, true>), grid, block, lds, c->stream, t);
+    else hipLaunchKernelGGL((q4_few_kernel<1, false>), grid, block, lds, c->stream, t);
+  } else if (two) {
     if (tile == 0) q4_tile_launch<128, 256, 64, 64, 2>(c, t, splits);
     else if (tile == 1) q4_tile_launch<128, 128, 64, 64, 2>(c, t, splits);
     else q4_tile_launch<64, 64, 32, 32, 2>(c, t, splits);
@@ -678,18 +916,12 @@ int linear_q4_launch(anima_ctx* c, const anima_linear_desc* d) {
   Q4Args a{d->x, d->ldx ? d->ldx : W->K, (const uint8_t*)W->w, W->group_scale, W->group_mid, W->bias, d->out, d->ldc ? d->ldc : W->N,
            d->alpha != 0.0f ? d->alpha : 1.0f, d->act, d->epilogue, d->epilogue == ANIMA_EPI_GATED ? d->gate + d->gate_off : nullptr, d->add,
            d->ld_add ? d->ld_add : W->N, (int)d->M, W->N, W->K, W->group, d->out_bf16};
-  if (a.M > Q4_FEW) return q4_tiles(c, a, d->precision == ANIMA_PREC_FP32);
-  Launch L(c, "gemv.q4", 2.0 * a.M * a.N * a.K, 0.5 * a.N * a.K);
-  constexpr int PART = 65535 * 4;  // (rows of a launch's grid)
-  const int M = a.M;
-  for (int m = 0; m < M; m += PART) {
-    a.M = std::min(PART, M - m);
-    hipLaunchKernelGGL(q4_rows_kernel, dim3((unsigned)((a.N + 3) / 4), (unsigned)((a.M + 3) / 4)), dim3(256), 0, c->stream, a);
-    a.x += (int64_t)PART * a.ldx;
-    if (a.add) a.add += (int64_t)PART * a.ld_add;
-    a.out = (char*)a.out + (int64_t)PART * a.ldc * (a.obf ? 2 : 4);
+  if (a.M <= Q4_ROWS) {
+    Launch L(c, "gemv.q4", 2.0 * a.M * a.N * a.K, 0.5 * a.N * a.K);
+    q4_gemv(c, a);
+    return L.end();
   }
-  return L.end();
+  return q4_matrix(c, a, d->precision == ANIMA_PREC_FP32);
 }
 
 }  // namespace anima
