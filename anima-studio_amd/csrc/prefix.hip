@@ -55,9 +55,9 @@ struct PrefixArgs {
   int64_t ldv;
   void* o;
   int64_t ldo;
-  const void* pk;   // prefix: K [Hkv][Pp][128], V^T [Hkv][128][Pp]
-  const void* pvt;
-  void* ok;         // own: K [Hkv][Tp][128], V^T [Hkv][128][Tp]
+  const void* pk;   // prefix: K [Hkv][Pp][128], V^T [Hkv][Pp/64][128][64] (a block's rows in one piece: rows of all keys would
+  const void* pvt;  // lie a power of two apart, in one memory channel)
+  void* ok;         // own: the same of Tp keys
   void* ovt;
   const float* qn;
   const float* kn;
@@ -173,10 +173,10 @@ __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a) {
 #pragma unroll
   for (int e = 0; e < 8; e++)
     if (vkey(e) >= a.T || bad[vkey(e) - kb0]) ve[e] = f32x4{};
-  T* vd = (T*)a.ovt + ((int64_t)hk * PHD + 32 * w + 4 * vq) * a.Tp + kb0 + 8 * vc;
+  T* vd = (T*)a.ovt + ((int64_t)hk * a.Tp + kb0) * PHD + (32 * w + 4 * vq) * 64 + 8 * vc;
 #pragma unroll
   for (int j = 0; j < 4; j++) {
-    T* d = vd + (int64_t)j * a.Tp;
+    T* d = vd + j * 64;
     if constexpr (BF) {
       bf16x8 o;
 #pragma unroll
@@ -324,13 +324,12 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_bf16(PrefixArgs 
   const int64_t pb = (int64_t)a.Pp * PHD * 2, ob = (int64_t)a.Tp * PHD * 2;
   const __amdgpu_buffer_rsrc_t rpk = p_rsrc((const char*)a.pk + hk * pb, a.P ? pb : 0), rpv = p_rsrc((const char*)a.pvt + hk * pb, a.P ? pb : 0),
                                rok = p_rsrc((const char*)a.ok + hk * ob, ob), rov = p_rsrc((const char*)a.ovt + hk * ob, ob);
-  uint32_t ko[CPW], vp[CPW], vo[CPW];
+  uint32_t ko[CPW], vo[CPW];
 #pragma unroll
   for (int c = 0; c < CPW; c++) {
     const int row = 4 * (wave * CPW + c) + (lane >> 4), d = 8 * (wave * CPW + c) + (lane >> 3);
     ko[c] = row * 256 + 16 * ((lane & 15) ^ (row & 15));
-    vp[c] = d * a.Pp * 2 + 16 * ((lane & 7) ^ ((d >> 1) & 7));
-    vo[c] = d * a.Tp * 2 + 16 * ((lane & 7) ^ ((d >> 1) & 7));
+    vo[c] = d * 128 + 16 * ((lane & 7) ^ ((d >> 1) & 7));
   }
   const auto load = [&](int j) __attribute__((always_inline)) {  // block j of the part (past the last: that one again, unused)
     bool pre;
@@ -339,7 +338,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_bf16(PrefixArgs 
 #pragma unroll
     for (int c = 0; c < CPW; c++) p_copy16(pre ? rpk : rok, st + (wave * CPW + c) * 1024, ko[c], blk * (64 * 256));
 #pragma unroll
-    for (int c = 0; c < CPW; c++) p_copy16(pre ? rpv : rov, st + PKT + (wave * CPW + c) * 1024, pre ? vp[c] : vo[c], blk * 128);
+    for (int c = 0; c < CPW; c++) p_copy16(pre ? rpv : rov, st + PKT + (wave * CPW + c) * 1024, vo[c], blk * (64 * 256));
   };
   if (nb > 0) {
     load(0);
@@ -614,7 +613,7 @@ __global__ __launch_bounds__(256, 2) void prefix_flash_fp32(PrefixArgs a) {
     bool pre;
     const int blk = B.at(i0 + j, pre), ld = pre ? a.Pp : a.Tp;
     const float* kg = (const float*)(pre ? a.pk : a.ok) + ((int64_t)hk * ld + blk * 64) * PHD;
-    const float* vg = (const float*)(pre ? a.pvt : a.ovt) + (int64_t)hk * PHD * ld + blk * 64;
+    const float* vg = (const float*)(pre ? a.pvt : a.ovt) + ((int64_t)hk * ld + blk * 64) * PHD;
     // K tile 64 x 128 floats, V^T tile 128 x 64: eight pieces of 4 floats of each per thread, consecutive threads
     // consecutive pieces
     f32x4 kr[8], vr[8];
@@ -622,7 +621,7 @@ __global__ __launch_bounds__(256, 2) void prefix_flash_fp32(PrefixArgs a) {
     for (int i = 0; i < 8; i++) {
       const int u = 256 * i + tid;
       kr[i] = *(const f32x4*)(kg + 4 * u);
-      vr[i] = *(const f32x4*)(vg + (int64_t)(u >> 4) * ld + 4 * (u & 15));
+      vr[i] = *(const f32x4*)(vg + 4 * u);
     }
     if (j) __syncthreads();  // every wave is done with the previous block's tiles
 #pragma unroll

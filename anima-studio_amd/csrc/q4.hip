@@ -152,19 +152,67 @@ __device__ __forceinline__ float q4_act(float r, int act) {
   return r;
 }
 
-__device__ __forceinline__ void q4_store(const Q4Args& a, int64_t m, int n, float r) {
-  r = r * a.alpha;
-  if (a.bias) r = r + a.bias[n];
-  if (a.add) r = r + a.add[m * a.ld_add + n];
-  r = q4_act(r, a.act);
+// What an output's epilogue reads, asked for before its sum is there.
+template <class V>
+struct Q4Ends {
+  V bias, add, gate, c;
+};
+
+__device__ __forceinline__ Q4Ends<float> q4_ask(const Q4Args& a, int64_t m, int n) {
+  Q4Ends<float> e{};
+  if (a.bias) e.bias = a.bias[n];
+  if (a.add) e.add = a.add[m * a.ld_add + n];
+  if (a.epi == ANIMA_EPI_GATED) e.gate = a.gate[n];
+  if (a.epi != ANIMA_EPI_STORE) e.c = ((const float*)a.out)[m * a.ldc + n];
+  return e;
+}
+
+__device__ __forceinline__ void q4_leave(const Q4Args& a, int64_t m, int n, float r, const Q4Ends<float>& e) {
+  r = q4_act(r * a.alpha + e.bias + e.add, a.act);
   if (a.obf) {
     ((bf16*)a.out)[m * a.ldc + n] = to_bf16(r);
     return;
   }
-  float* c = (float*)a.out + m * a.ldc + n;
-  if (a.epi == ANIMA_EPI_STORE) *c = r;
-  else if (a.epi == ANIMA_EPI_RESID) *c = *c + r;
-  else *c = __builtin_fmaf(a.gate[n], r, *c);
+  ((float*)a.out)[m * a.ldc + n] = a.epi == ANIMA_EPI_GATED ? __builtin_fmaf(e.gate, r, e.c) : r + e.c;
+}
+
+// The same for four columns (vec: rows of out, bias, add and gate in quads of 16 bytes; else one by one, when they leave).
+__device__ __forceinline__ Q4Ends<f32x4> q4_ask4(const Q4Args& a, int vec, int64_t m, int n) {
+  Q4Ends<f32x4> e{};
+  if (!vec) return e;
+  if (a.bias) e.bias = *(const f32x4*)(a.bias + n);
+  if (a.add) e.add = *(const f32x4*)(a.add + m * a.ld_add + n);
+  if (a.epi == ANIMA_EPI_GATED) e.gate = *(const f32x4*)(a.gate + n);
+  if (a.epi != ANIMA_EPI_STORE) e.c = *(const f32x4*)((const float*)a.out + m * a.ldc + n);
+  return e;
+}
+
+__device__ __forceinline__ void q4_leave4(const Q4Args& a, int vec, int64_t m, int n, f32x4 r, const Q4Ends<f32x4>& e) {
+  if (!vec) {
+#pragma unroll 1
+    for (int i = 0; i < 4; i++)
+      if (n + i < a.N) q4_leave(a, m, n + i, i == 0 ? r[0] : i == 1 ? r[1] : i == 2 ? r[2] : r[3], q4_ask(a, m, n + i));
+    return;
+  }
+  r = r * a.alpha + e.bias + e.add;
+  if (a.act == ANIMA_ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) r[i] = gelu_erf(r[i]);
+  } else if (a.act == ANIMA_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) r[i] = silu_f(r[i]);
+  }
+  if (a.obf) {
+    *(bf16x4*)((bf16*)a.out + m * a.ldc + n) = bf16x4{to_bf16(r[0]), to_bf16(r[1]), to_bf16(r[2]), to_bf16(r[3])};
+    return;
+  }
+  if (a.epi == ANIMA_EPI_GATED) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) r[i] = __builtin_fmaf(e.gate[i], r[i], e.c[i]);
+  } else {
+    r = r + e.c;
+  }
+  *(f32x4*)((float*)a.out + m * a.ldc + n) = r;
 }
 
 // One to four rows on the vector units, in fp32: a wave takes U columns, a lane 16 consecutive k of each 1024 (eight bytes of
@@ -177,6 +225,20 @@ __global__ __launch_bounds__(256) void q4_gemv_kernel(Q4Args a) {
   __shared__ f32x4 xs[2][MR][256];
   const int tid = threadIdx.x, lane = tid & 63, n0 = (blockIdx.x * 4 + (tid >> 6)) * U, KG = a.K / a.G, lg = 31 - __builtin_clz(a.G);
   float acc[MR][U] = {};
+  // the output that this lane ends with, if it has any
+  int first = 0;
+#pragma unroll
+  for (int d = 32, cnt = U; cnt > 1; d >>= 1) {
+    cnt >>= 1;
+    if (lane & d) first += cnt;
+  }
+  const int no = n0 + first;
+  const bool ends = (lane & (64 / U - 1)) == 0 && no < a.N;
+  Q4Ends<float> ask[MR] = {};
+  if (ends)
+#pragma unroll
+    for (int m = 0; m < MR; m++)
+      if (m < a.M) ask[m] = q4_ask(a, m, no);
   const uint8_t* w[U];
   const uint16_t *gs[U], *gz[U];
 #pragma unroll
@@ -229,7 +291,7 @@ __global__ __launch_bounds__(256) void q4_gemv_kernel(Q4Args a) {
   // The sums over the lanes: while a lane holds several outputs, the two of a pair keep half of them each.
 #pragma unroll
   for (int m = 0; m < MR; m++) {
-    int cnt = U, first = 0;
+    int cnt = U;
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) {
       if (cnt > 1) {
@@ -241,12 +303,11 @@ __global__ __launch_bounds__(256) void q4_gemv_kernel(Q4Args a) {
             const float send = hi ? acc[m][u] : acc[m][u + cnt], keep = hi ? acc[m][u + cnt] : acc[m][u];
             acc[m][u] = keep + __shfl_xor(send, d);
           }
-        if (hi) first += cnt;
       } else {
         acc[m][0] += __shfl_xor(acc[m][0], d);
       }
     }
-    if ((lane & (64 / U - 1)) == 0 && m < a.M && n0 + first < a.N) q4_store(a, m, n0 + first, acc[m][0]);
+    if (ends && m < a.M) q4_leave(a, m, no, acc[m][0], ask[m]);
   }
 }
 
@@ -280,6 +341,7 @@ struct Q4Prep {
   float* sx;      // [M][K/G] group sums of x, or NULL
   const uint16_t* gs;
   float* rn;      // [N] what the column's power comes off with
+  int64_t ldp;    // values between the terms' rows
   int M, N, K, Kp, G, rows;  // rows: workgroups of x rows (four each), the rest are of columns
 };
 
@@ -328,8 +390,8 @@ __global__ __launch_bounds__(256) void q4_prep_kernel(Q4Prep a) {
       l[o] = (_Float16)(y - (float)h[o]);
     }
     if (k < a.Kp) {
-      *(f16x8*)(a.xh + m * a.Kp + k) = h;
-      if (a.xl) *(f16x8*)(a.xl + m * a.Kp + k) = l;
+      *(f16x8*)(a.xh + m * a.ldp + k) = h;
+      if (a.xl) *(f16x8*)(a.xl + m * a.ldp + k) = l;
     }
   };
   float mx = 0.0f;
@@ -398,37 +460,9 @@ struct Q4Tile {
   const float* sx;
   float* part;       // [splits][M][N] sums of a product split over k, or NULL
   int Kp, sps;       // k padded; steps of 64 k in a split
+  int ldp;           // values between the terms' rows
   int vec;           // rows of out, bias, add and gate in quads of 16 bytes
 };
-
-// Four columns of a row: + bias and add, the activation, and out's epilogue.
-__device__ __forceinline__ void q4_store4(const Q4Args& a, int vec, int64_t m, int n, f32x4 r) {
-  if (!vec) {
-    for (int i = 0; i < 4; i++)
-      if (n + i < a.N) q4_store(a, m, n + i, r[i]);
-    return;
-  }
-  r = r * a.alpha;
-  if (a.bias) r = r + *(const f32x4*)(a.bias + n);
-  if (a.add) r = r + *(const f32x4*)(a.add + m * a.ld_add + n);
-  if (a.act != ANIMA_ACT_NONE) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) r[i] = q4_act(r[i], a.act);
-  }
-  if (a.obf) {
-    *(bf16x4*)((bf16*)a.out + m * a.ldc + n) = bf16x4{to_bf16(r[0]), to_bf16(r[1]), to_bf16(r[2]), to_bf16(r[3])};
-    return;
-  }
-  f32x4* c = (f32x4*)((float*)a.out + m * a.ldc + n);
-  if (a.epi == ANIMA_EPI_RESID) {
-    r = *c + r;
-  } else if (a.epi == ANIMA_EPI_GATED) {
-    const f32x4 g = *(const f32x4*)(a.gate + n), o = *c;
-#pragma unroll
-    for (int i = 0; i < 4; i++) r[i] = __builtin_fmaf(g[i], r[i], o[i]);
-  }
-  *c = r;
-}
 
 // ------------------------------------------------------------------ products of a few rows
 //
@@ -454,7 +488,7 @@ __global__ __launch_bounds__(64 * QF_WAVES, 2) void q4_few_kernel(Q4Tile q) {
     float sx[NG];
   } st[2];
   const uint8_t* wr = a.w + (int64_t)min(n0 + r, a.N - 1) * (a.K / 2);
-  const int64_t mr = min(m0 + r, a.M - 1), xo = mr * q.Kp + 8 * hf, so = mr * KG;
+  const int64_t mr = min(m0 + r, a.M - 1), xo = mr * q.ldp + 8 * hf, so = mr * KG;
   const auto load = [&](Step& v, int step) __attribute__((always_inline)) {  // (past the last step: that one again, unused)
     const int k = 64 * min(step, steps - 1);
     v.w = *(const u32x4*)(wr + min(k + 32 * hf, a.K - 32) / 2);  // (past the row's end its last 32: they meet zeros of x)
@@ -469,12 +503,30 @@ __global__ __launch_bounds__(64 * QF_WAVES, 2) void q4_few_kernel(Q4Tile q) {
   };
   load(st[0], wave);
   load(st[1], wave + QF_WAVES);
-  for (int i = tid; i < KG * 32; i += 64 * QF_WAVES) {
-    const int64_t at = (int64_t)min(n0 + (i & 31), a.N - 1) * KG + (i >> 5);
-    ss[i] = bf16_f(a.gs[at]);
-    if (a.gz) zs[i] = bf16_f(a.gz[at]);
-  }
   const float rm = q.rm[mr], up = 1.0f / rm;  // (powers of two)
+  // what this thread's output reads at the end
+  const int om = m0 + (lane & 31), on = n0 + 8 * wave + 4 * (lane >> 5);
+  const bool out = wave < 4 && om < a.M && on < a.N;
+  Q4Ends<f32x4> ask{};
+  if (out) ask = q4_ask4(a, q.vec, om, on);
+  {
+    const int64_t col = (int64_t)min(n0 + (tid >> 4), a.N - 1) * KG;
+    for (int g0 = tid & 15; g0 < KG; g0 += 64) {
+      uint16_t s[4], z[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int64_t at = col + min(g0 + 16 * i, KG - 1);
+        s[i] = a.gs[at];
+        z[i] = a.gz ? a.gz[at] : 0;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (g0 + 16 * i < KG) {
+          ss[(g0 + 16 * i) * 32 + (tid >> 4)] = bf16_f(s[i]);
+          if (a.gz) zs[(g0 + 16 * i) * 32 + (tid >> 4)] = bf16_f(z[i]);
+        }
+    }
+  }
   __builtin_amdgcn_s_waitcnt(0xc07f);
   q4_barrier();
   f32x16 acc = {};
@@ -532,12 +584,11 @@ __global__ __launch_bounds__(64 * QF_WAVES, 2) void q4_few_kernel(Q4Tile q) {
     sum[(wave * 4 + c) * 64 + lane] = v;
   }
   __syncthreads();
-  if (tid >= 256) return;
+  if (!out) return;
   f32x4 v = sum[tid];
 #pragma unroll
   for (int w = 1; w < QF_WAVES; w++) v = v + sum[w * 256 + tid];
-  const int c = tid >> 6, m = m0 + (lane & 31), n = n0 + 8 * c + 4 * (lane >> 5);
-  if (m < a.M && n < a.N) q4_store4(a, q.vec, m, n, v);
+  q4_leave4(a, q.vec, om, on, v, ask);
 }
 
 // ------------------------------------------------------------------ tiles
@@ -574,14 +625,14 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), q4_waves(BM, BN, WM, WN
   const int s0 = blockIdx.y * t.sps, steps = min(t.sps, t.Kp / 64 - s0);
 
   const int mrows = min(BM, a.M - bm);
-  const __amdgpu_buffer_rsrc_t rh = q4_rsrc(t.xh + (int64_t)bm * t.Kp, (int64_t)mrows * t.Kp * 2),
-                               rl = q4_rsrc((TERMS > 1 ? t.xl : t.xh) + (int64_t)bm * t.Kp, (int64_t)mrows * t.Kp * 2);
+  const __amdgpu_buffer_rsrc_t rh = q4_rsrc(t.xh + (int64_t)bm * t.ldp, (int64_t)mrows * t.ldp * 2),
+                               rl = q4_rsrc((TERMS > 1 ? t.xl : t.xh) + (int64_t)bm * t.ldp, (int64_t)mrows * t.ldp * 2);
   // copy c of this wave: eight rows of a term
   uint32_t xo[CPW];
 #pragma unroll
   for (int c = 0; c < CPW; c++) {
     const int row = (8 * (wave * CPW + c)) % BM + (lane >> 3);
-    xo[c] = (uint32_t)row * (uint32_t)(t.Kp * 2) + 16 * ((lane & 7) ^ ((row >> 1) & 7)) + 128 * s0;
+    xo[c] = (uint32_t)row * (uint32_t)(t.ldp * 2) + 16 * ((lane & 7) ^ ((row >> 1) & 7)) + 128 * s0;
   }
   const auto copies = [&](int step, int p) __attribute__((always_inline)) {
 #pragma unroll
@@ -718,21 +769,31 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), q4_waves(BM, BN, WM, WN
       }
     }
     __builtin_amdgcn_wave_barrier();
-#pragma unroll 4
-    for (int q = 0; q < 32; q += PR) {
-      const int row = q + lane / LR, n = n0 + 4 * (lane % LR);
-      const f32x4 v = *(const f32x4*)(rows + row * RS + 4 * (lane % LR));
-      const int64_t mo = bm + wm + 32 * i + row;
-      if (mo < a.M && n < a.N) {
-        if (t.part) {
-          float* o = t.part + ((int64_t)blockIdx.y * a.M + mo) * a.N + n;
-          if (t.vec) *(f32x4*)o = v;
-          else
-            for (int e = 0; e < 4; e++)
-              if (n + e < a.N) o[e] = v[e];
-        } else {
-          q4_store4(a, t.vec, mo, n, v);
+    const int n = n0 + 4 * (lane % LR);
+    // (a loop with one body: unrolled, the epilogue is more code than the instruction cache holds beside the k loop)
+#pragma unroll 1
+    for (int q = 0; q < 32; q += 4 * PR) {
+      const int64_t mo = bm + wm + 32 * i + q + lane / LR;
+      f32x4 v[4];
+      Q4Ends<f32x4> ask[4];
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        v[u] = *(const f32x4*)(rows + (q + u * PR + lane / LR) * RS + 4 * (lane % LR));
+        if (!t.part && mo + u * PR < a.M && n < a.N) ask[u] = q4_ask4(a, t.vec, mo + u * PR, n);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const int64_t m = mo + u * PR;
+        if (m >= a.M || n >= a.N) continue;
+        if (!t.part) {
+          q4_leave4(a, t.vec, m, n, v[u], ask[u]);
+          continue;
         }
+        float* o = t.part + ((int64_t)blockIdx.y * a.M + m) * a.N + n;
+        if (t.vec) *(f32x4*)o = v[u];
+        else
+          for (int e = 0; e < 4; e++)
+            if (n + e < a.N) o[e] = v[u][e];
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -748,6 +809,7 @@ __global__ __launch_bounds__(256) void q4_join_kernel(Q4Tile t, int splits) {
   const int n = (int)(4 * (i - m * quads));
   const float* p = t.part + m * a.N + n;
   const int64_t plane = (int64_t)a.M * a.N;
+  const Q4Ends<f32x4> ask = q4_ask4(a, t.vec, m, n);
   f32x4 v = {};
   if (t.vec) {
     f32x4 w[Q4_SPLITS];  // (all asked for before the first is added)
@@ -760,7 +822,7 @@ __global__ __launch_bounds__(256) void q4_join_kernel(Q4Tile t, int splits) {
       for (int e = 0; e < 4; e++)
         if (n + e < a.N) v[e] += p[s * plane + e];
   }
-  q4_store4(a, t.vec, m, n, v);
+  q4_leave4(a, t.vec, m, n, v, ask);
 }
 
 // ------------------------------------------------------------------ host
@@ -845,6 +907,8 @@ static int q4_matrix(anima_ctx* c, const Q4Args& a, bool two) {
   Q4Tile t{};
   t.a = a;
   t.Kp = (a.K + 63) / 64 * 64;
+  // rows of the terms an odd number of lines of 128 bytes apart: at a power of two one step's rows meet in one memory channel
+  t.ldp = t.Kp / 64 % 2 ? t.Kp : t.Kp + 64;
   t.vec = q4_vec(a);
   const int KG = a.K / a.G, steps = t.Kp / 64;
   const bool few = a.M <= 64 && q4_few_lds(a) <= Q4_FEW_LDS;
@@ -863,14 +927,14 @@ static int q4_matrix(anima_ctx* c, const Q4Args& a, bool two) {
     at += (bytes + 255) / 256 * 256;
     return o;
   };
-  const size_t plane = (size_t)a.M * t.Kp * 2, oh = take(plane), ol = two ? take(plane) : 0, om = take((size_t)a.M * 4),
+  const size_t plane = (size_t)a.M * t.ldp * 2, oh = take(plane), ol = two ? take(plane) : 0, om = take((size_t)a.M * 4),
                on = few ? 0 : take(((size_t)a.N + 255) / 256 * 1024), os = a.gz ? take((size_t)a.M * KG * 4) : 0,
                op = splits > 1 ? take((size_t)splits * a.M * a.N * 4) : 0;
   void* tmp = nullptr;
   if (int rc = anima_alloc(c, at, &tmp)) return rc;
   char* const b = (char*)tmp;
   Q4Prep p{a.x, a.ldx, (_Float16*)(b + oh), two ? (_Float16*)(b + ol) : nullptr, (float*)(b + om), a.gz ? (float*)(b + os) : nullptr, a.gs,
-           (float*)(b + on), a.M, a.N, a.K, t.Kp, a.G, (a.M + 3) / 4};
+           (float*)(b + on), t.ldp, a.M, a.N, a.K, t.Kp, a.G, (a.M + 3) / 4};
   t.xh = p.xh;
   t.xl = p.xl;
   t.rm = p.rm;
