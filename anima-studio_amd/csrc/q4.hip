@@ -335,7 +335,8 @@ __device__ __forceinline__ int q4_exp(float amax, int top) {
 struct Q4Prep {
   const float* x;
   int64_t ldx;
-  _Float16* xh;   // [M][Kp], each eight values in the order k 0 4 1 5 2 6 3 7 (the decode's), zeros from K on
+  _Float16* xh;   // rows of Kp, ldp apart, each eight values in the order k 0 4 1 5 2 6 3 7 (the decode's), zeros from K on;
+                  // or (frag) as the 32 x 32 x 16 products take them: [rows / 32][Kp / 16][k / 8 % 2][row % 32][8]
   _Float16* xl;   // the second terms, or NULL
   float* rm;      // [M] what x's power comes off with
   float* sx;      // [M][K/G] group sums of x, or NULL
@@ -343,6 +344,7 @@ struct Q4Prep {
   float* rn;      // [N] what the column's power comes off with
   int64_t ldp;    // values between the terms' rows
   int M, N, K, Kp, G, rows;  // rows: workgroups of x rows (four each), the rest are of columns
+  int frag;
 };
 
 // A wave per row of x (NV: pieces of 512 k that a wave holds; 0: two passes over the row, the second from the caches), or per
@@ -390,8 +392,9 @@ __global__ __launch_bounds__(256) void q4_prep_kernel(Q4Prep a) {
       l[o] = (_Float16)(y - (float)h[o]);
     }
     if (k < a.Kp) {
-      *(f16x8*)(a.xh + m * a.ldp + k) = h;
-      if (a.xl) *(f16x8*)(a.xl + m * a.ldp + k) = l;
+      const int64_t at = a.frag ? (((m >> 5) * (a.Kp >> 4) + (k >> 4)) * 2 + (k >> 3 & 1)) * 256 + (m & 31) * 8 : m * a.ldp + k;
+      *(f16x8*)(a.xh + at) = h;
+      if (a.xl) *(f16x8*)(a.xl + at) = l;
     }
   };
   float mx = 0.0f;
@@ -462,14 +465,15 @@ struct Q4Tile {
   int Kp, sps;       // k padded; steps of 64 k in a split
   int ldp;           // values between the terms' rows
   int vec;           // rows of out, bias, add and gate in quads of 16 bytes
+  int svec;          // four steps' scales are one aligned piece of a row
 };
 
 // ------------------------------------------------------------------ products of a few rows
 //
 // A workgroup takes 32 columns and 32 rows, its eight waves every eighth step of 64 k each, their sums joined in order
 // through LDS.  The codes stay whole numbers (exact in f16), and each group's sums meet their scale in fp32; scales and
-// middles lie in LDS as [group][column].  x comes as q4_prep_kernel leaves it (split here, again for each 32 columns, it took
-// 20 us of 43 x 1024 x 2048).
+// middles lie in LDS as [group][column].  x comes from q4_prep_kernel in the order of the lanes (as rows, a load meets 32 lines
+// and takes the address unit four times as long).
 constexpr int QF_WAVES = 8;
 
 template <int TERMS, bool G32>
@@ -488,14 +492,16 @@ __global__ __launch_bounds__(64 * QF_WAVES, 2) void q4_few_kernel(Q4Tile q) {
     float sx[NG];
   } st[2];
   const uint8_t* wr = a.w + (int64_t)min(n0 + r, a.N - 1) * (a.K / 2);
-  const int64_t mr = min(m0 + r, a.M - 1), xo = mr * q.ldp + 8 * hf, so = mr * KG;
+  const int64_t mr = min(m0 + r, a.M - 1), so = mr * KG;
+  const float rm = q.rm[mr];  // (a power of two)
+  const int64_t xo = (int64_t)blockIdx.y * 32 * q.Kp + lane * 8;
   const auto load = [&](Step& v, int step) __attribute__((always_inline)) {  // (past the last step: that one again, unused)
     const int k = 64 * min(step, steps - 1);
     v.w = *(const u32x4*)(wr + min(k + 32 * hf, a.K - 32) / 2);  // (past the row's end its last 32: they meet zeros of x)
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      v.x[0][i] = *(const f16x8*)(q.xh + xo + k + 16 * i);
-      if (TERMS > 1) v.x[TERMS - 1][i] = *(const f16x8*)(q.xl + xo + k + 16 * i);
+      v.x[0][i] = *(const f16x8*)(q.xh + xo + (k + 16 * i) * 32);
+      if (TERMS > 1) v.x[TERMS - 1][i] = *(const f16x8*)(q.xl + xo + (k + 16 * i) * 32);
     }
     if (a.gz)
 #pragma unroll
@@ -503,7 +509,6 @@ __global__ __launch_bounds__(64 * QF_WAVES, 2) void q4_few_kernel(Q4Tile q) {
   };
   load(st[0], wave);
   load(st[1], wave + QF_WAVES);
-  const float rm = q.rm[mr], up = 1.0f / rm;  // (powers of two)
   // what this thread's output reads at the end
   const int om = m0 + (lane & 31), on = n0 + 8 * wave + 4 * (lane >> 5);
   const bool out = wave < 4 && om < a.M && on < a.N;
@@ -530,6 +535,7 @@ __global__ __launch_bounds__(64 * QF_WAVES, 2) void q4_few_kernel(Q4Tile q) {
   __builtin_amdgcn_s_waitcnt(0xc07f);
   q4_barrier();
   f32x16 acc = {};
+  const float up = 1.0f / rm;
   const f16x2 one = {(_Float16)1.0f, (_Float16)1.0f};
   const auto product = [&](const Step& v, int step) __attribute__((always_inline)) {
     // the halves' words exchanged, so that matrix step i covers k 16 i .. 16 i + 15: lane half hf word 2 i + hf of 8
@@ -593,18 +599,20 @@ __global__ __launch_bounds__(64 * QF_WAVES, 2) void q4_few_kernel(Q4Tile q) {
 
 // ------------------------------------------------------------------ tiles
 
-// One BM x BN tile a workgroup, waves of WM rows x WN columns.  A step is 64 k: BM rows of x (128 bytes, each term) in one of four LDS
-// stages, filled three steps ahead by buffer_load ... lds, units of 16 bytes at slot u ^ (row / 2 % 8) (sixteen rows' reads of one
-// unit touch each bank once).  The codes go straight to registers, four steps ahead: lane (n, half) takes the 16 bytes of
-// column n's 32 k of its half, so that matrix step i of a lane pair covers k 8 i .. 8 i + 7 of both halves; x's units follow.
+// One BM x BN tile a workgroup, waves of WM rows x WN columns.  A step is 64 k: BM rows of x (128 bytes, each term) and BN columns'
+// codes (32 bytes) in one of four LDS stages, filled three steps ahead by buffer_load ... lds.  x's units of 16 bytes lie at slot
+// u ^ (row / 2 % 8) (sixteen rows' reads of one unit touch each bank once).  Lane (n, half) takes the 16 bytes of column n's 32 k of
+// its half, so that matrix step i of a lane pair covers k 8 i .. 8 i + 7 of both halves; x's units follow.  The scales of four
+// steps come in one load where rows of them allow it: each of a lane's own addresses costs the address unit as
+// much as 64 neighbouring bytes.
 constexpr int q4_waves(int BM, int BN, int WM, int WN, int TERMS) {  // waves a SIMD that a tile's LDS leaves room for
-  return (BM / WM) * (BN / WN) < 8 && TERMS * BM * 128 * 4 > 81920 ? 1 : 2;
+  return (BM / WM) * (BN / WN) < 8 && (TERMS * BM * 128 + BN * 32) * 4 > 81920 ? 1 : 2;
 }
 template <int BM, int BN, int WM, int WN, int TERMS>
 __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), q4_waves(BM, BN, WM, WN, TERMS)) void q4_tile_kernel(Q4Tile t) {
   constexpr int NWM = BM / WM, NW = NWM * (BN / WN), MT = WM / 32, NT = WN / 32, NST = 4;
-  constexpr int XB = BM * 128, SB = XB * TERMS, CPW = TERMS * BM / 8 / NW;
-  static_assert(CPW * NW * 8 == TERMS * BM, "whole copies");
+  constexpr int XB = BM * 128, WO = XB * TERMS, SB = WO + BN * 32, CX = TERMS * BM / 8 / NW, CW = (BN / 32 + NW - 1) / NW, CPW = CX + CW;
+  static_assert(CX * NW * 8 == TERMS * BM, "whole copies");
   constexpr int RS = WN + 4, EPL = NW * 32 * RS * 4;
   constexpr int LDS = NST * SB > EPL ? NST * SB : EPL;
   __shared__ __attribute__((aligned(1024))) char smem[LDS];
@@ -617,48 +625,87 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), q4_waves(BM, BN, WM, WN
     const int total = ntn * ntm, q = total >> 3, rem = total & 7, x = blockIdx.x & 7;
     const int i = x * q + min(x, rem) + (int)(blockIdx.x >> 3);
     const int grp = i / (8 * ntn), row0 = 8 * grp, gm = min(8, ntm - row0), local = i - grp * 8 * ntn;
-    tn = local / gm;
-    tm = row0 + (local - tn * gm);
+    tn = __builtin_amdgcn_readfirstlane(local / gm);
+    tm = __builtin_amdgcn_readfirstlane(row0 + (local - tn * gm));
   }
-  const int bm = tm * BM, bn = tn * BN, K = a.K, KG = K / a.G;
+  const int bm = tm * BM, bn = tn * BN, K = a.K, KG = __builtin_amdgcn_readfirstlane(K / a.G);
   const int wm = (wave % NWM) * WM, wn = (wave / NWM) * WN;
   const int s0 = blockIdx.y * t.sps, steps = min(t.sps, t.Kp / 64 - s0);
 
-  const int mrows = min(BM, a.M - bm);
+  const int mrows = min(BM, a.M - bm), ncols = min(BN, a.N - bn);
   const __amdgpu_buffer_rsrc_t rh = q4_rsrc(t.xh + (int64_t)bm * t.ldp, (int64_t)mrows * t.ldp * 2),
-                               rl = q4_rsrc((TERMS > 1 ? t.xl : t.xh) + (int64_t)bm * t.ldp, (int64_t)mrows * t.ldp * 2);
-  // copy c of this wave: eight rows of a term
-  uint32_t xo[CPW];
+                               rl = q4_rsrc((TERMS > 1 ? t.xl : t.xh) + (int64_t)bm * t.ldp, (int64_t)mrows * t.ldp * 2),
+                               rw = q4_rsrc(a.w + (int64_t)bn * (K / 2), (int64_t)ncols * (K / 2));
+  // copies of this wave: eight rows of a term, or 32 columns' codes (past the tile's last: that one again)
+  uint32_t xo[CX], wo[CW];
 #pragma unroll
-  for (int c = 0; c < CPW; c++) {
-    const int row = (8 * (wave * CPW + c)) % BM + (lane >> 3);
+  for (int c = 0; c < CX; c++) {
+    const int row = (8 * (wave * CX + c)) % BM + (lane >> 3);
     xo[c] = (uint32_t)row * (uint32_t)(t.ldp * 2) + 16 * ((lane & 7) ^ ((row >> 1) & 7)) + 128 * s0;
   }
+#pragma unroll
+  for (int c = 0; c < CW; c++) wo[c] = (uint32_t)(32 * min(wave * CW + c, BN / 32 - 1) + (lane >> 1)) * (uint32_t)(K / 2) + 16 * (lane & 1);
   const auto copies = [&](int step, int p) __attribute__((always_inline)) {
 #pragma unroll
-    for (int c = 0; c < CPW; c++)
-      q4_copy16(TERMS > 1 && wave * CPW + c >= BM / 8 ? rl : rh, smem + p * SB + (wave * CPW + c) * 1024, xo[c], 128 * step);
+    for (int c = 0; c < CX; c++)
+      q4_copy16(TERMS > 1 && wave * CX + c >= BM / 8 ? rl : rh, smem + p * SB + (wave * CX + c) * 1024, xo[c], 128 * step);
+    // (K of an odd number of 32: the last half is the next column's or past the end, and meets zeros of x)
+#pragma unroll
+    for (int c = 0; c < CW; c++) q4_copy16(rw, smem + p * SB + WO + min(wave * CW + c, BN / 32 - 1) * 1024, wo[c], 32 * (s0 + step));
   };
-  // columns of this wave's tiles (past the last: the last, whose sums are not stored)
-  const uint8_t* wrow[NT];
+  // The scales of steps s .. s + 3 (s % 4 == 0): as they lie, if four steps' are one aligned piece of the row, else one by one; then
+  // each step's as a pair for the decode.
   const uint16_t* srow[NT];
   float fn[NT];
 #pragma unroll
   for (int j = 0; j < NT; j++) {
     const int64_t n = min(bn + wn + 32 * j + r, a.N - 1);
-    wrow[j] = a.w + n * (K / 2);
     srow[j] = a.gs + n * KG;
     fn[j] = 1.0f / t.rn[n];
   }
-  u32x4 wr[2][NT];
-  uint16_t sc[2][NT];
   const int lg = 31 - __builtin_clz(a.G);
-  const auto codes = [&](int step, int u) __attribute__((always_inline)) {
-    const int k = min(64 * (s0 + step) + 32 * hf, K - 32);  // (past the row's end its last 32: they meet zeros of x)
+  u32x4 sc[NT];
+  f16x2 sv[NST][NT];
+  const auto scales = [&](int step) __attribute__((always_inline)) {
+    const int g = (s0 + step) * 64 >> lg;
 #pragma unroll
     for (int j = 0; j < NT; j++) {
-      wr[u][j] = *(const u32x4*)(wrow[j] + k / 2);
-      sc[u][j] = srow[j][k >> lg];
+      if (t.svec) {
+        const int at = min(g, KG - (256 >> lg));
+        if (a.G == 32) {
+          sc[j] = *(const u32x4*)(srow[j] + at);
+        } else if (a.G == 64) {
+          const uint2 v = *(const uint2*)(srow[j] + at);
+          sc[j][0] = v.x;
+          sc[j][1] = v.y;
+        } else {
+          sc[j][0] = *(const uint32_t*)(srow[j] + at);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) sc[j][i] = srow[j][min(64 * (s0 + step + i) + 32 * hf, K - 32) >> lg];
+      }
+    }
+  };
+  const auto pairs = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < NT; j++) {
+      u32x4 v = sc[j];
+      if (t.svec) {
+        if (a.G == 32) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) v[i] = v[i] >> (16 * hf);
+        } else if (a.G == 64) {
+          v = u32x4{v[0], v[0] >> 16, v[1], v[1] >> 16};
+        } else {
+          v = u32x4{v[0], v[0], v[0] >> 16, v[0] >> 16};
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const _Float16 f = (_Float16)(__uint_as_float(v[i] << 16) * fn[j]);
+        sv[i][j] = f16x2{f, f};
+      }
     }
   };
   f32x16 acc[MT][NT];
@@ -669,53 +716,57 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), q4_waves(BM, BN, WM, WN
   int xa[4];  // unit 4 hf + i of row r
 #pragma unroll
   for (int i = 0; i < 4; i++) xa[i] = (wm + r) * 128 + 16 * ((4 * hf + i) ^ ((r >> 1) & 7));
+  const int wa = WO + (wn + r) * 32 + 16 * hf;
 
   // Fragments of matrix step i + 1 are read and decoded under step i's products.  Before the last of a stage's four, whose
   // fragments are in registers by then, a barrier ends every wave's reads of the stage (its buffer is refilled) and publishes
-  // the next one: this wave's copies of it have arrived when at most the loads of the two turns after it pend.
+  // the next one: this wave's copies of it have arrived when at most those of the two stages after it pend.
   f16x8 xf[2][MT][TERMS], wf[2][NT];
-  f16x2 sv[NT];
+  u32x4 wr[NT];
   const auto xread = [&](int u, int p, int i) __attribute__((always_inline)) {
 #pragma unroll
     for (int m = 0; m < MT; m++)
 #pragma unroll
       for (int e = 0; e < TERMS; e++) xf[u][m][e] = *(const f16x8*)(smem + p * SB + e * XB + m * 4096 + xa[i]);
   };
-  const auto decode = [&](int u, int b, int i) __attribute__((always_inline)) {
+  const auto wread = [&](int p) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < NT; j++) {
-      if (i == 0) {
-        const _Float16 v = (_Float16)(bf16_f(sc[b][j]) * fn[j]);
-        sv[j] = f16x2{v, v};
-      }
-      wf[u][j] = q4_decode(wr[b][j][i], sv[j]);
-    }
+    for (int j = 0; j < NT; j++) wr[j] = *(const u32x4*)(smem + p * SB + wa + j * 1024);
   };
+  const auto decode = [&](int u, int p, int i) __attribute__((always_inline)) {
 #pragma unroll
-  for (int p = 0; p < NST; p++) {
-    copies(p, p);
-    if (p < 2) codes(p, p);
-  }
+    for (int j = 0; j < NT; j++) wf[u][j] = q4_decode(wr[j][i], sv[p][j]);
+  };
+  scales(0);
+#pragma unroll
+  for (int p = 0; p < NST; p++) copies(p, p);
+  pairs();
   Q4_WAIT_VM((NST - 1) * CPW);
   q4_barrier();
+  scales(NST);
+  wread(0);
   xread(0, 0, 0);
   decode(0, 0, 0);
   const auto stage = [&](int step, auto buffer) __attribute__((always_inline)) {
-    constexpr int p = decltype(buffer)::value, pn = (p + 1) % NST, b = p & 1;
+    constexpr int p = decltype(buffer)::value, pn = (p + 1) % NST;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       const int u = i & 1;
       if (i == 3) {
         __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
-        Q4_WAIT_VM(2 * (CPW + 2 * NT));
+        Q4_WAIT_VM(2 * CPW);
         q4_barrier();
         copies(step + NST, p);
+        wread(pn);
         xread(u ^ 1, pn, 0);
-        decode(u ^ 1, b ^ 1, 0);
-        codes(step + 2, b);
+        if (p == NST - 1) {
+          pairs();
+          scales(step + 1 + NST);
+        }
+        decode(u ^ 1, pn, 0);
       } else {
         xread(u ^ 1, p, i + 1);
-        decode(u ^ 1, b, i + 1);
+        decode(u ^ 1, p, i + 1);
       }
 #pragma unroll
       for (int e = TERMS - 1; e >= 0; e--)
@@ -919,6 +970,8 @@ static int q4_matrix(anima_ctx* c, const Q4Args& a, bool two) {
   int splits = 1;
   while (!few && splits < Q4_SPLITS && nt * splits * 2 <= c->num_cus && steps / (splits * 2) >= 4) splits *= 2;
   t.sps = (steps + splits - 1) / splits;
+  if (splits > 1) t.sps = (t.sps + 3) / 4 * 4;
+  t.svec = a.K % 256 == 0 && q4_al(a.gs, 16);
   splits = (steps + t.sps - 1) / t.sps;
   // scratch: the terms, the powers, the group sums, the splits' sums
   size_t at = 0;
@@ -927,14 +980,14 @@ static int q4_matrix(anima_ctx* c, const Q4Args& a, bool two) {
     at += (bytes + 255) / 256 * 256;
     return o;
   };
-  const size_t plane = (size_t)a.M * t.ldp * 2, oh = take(plane), ol = two ? take(plane) : 0, om = take((size_t)a.M * 4),
+  const size_t plane = (few ? (size_t)(a.M + 31) / 32 * 32 * t.Kp : (size_t)a.M * t.ldp) * 2, oh = take(plane), ol = two ? take(plane) : 0, om = take((size_t)a.M * 4),
                on = few ? 0 : take(((size_t)a.N + 255) / 256 * 1024), os = a.gz ? take((size_t)a.M * KG * 4) : 0,
                op = splits > 1 ? take((size_t)splits * a.M * a.N * 4) : 0;
   void* tmp = nullptr;
   if (int rc = anima_alloc(c, at, &tmp)) return rc;
   char* const b = (char*)tmp;
   Q4Prep p{a.x, a.ldx, (_Float16*)(b + oh), two ? (_Float16*)(b + ol) : nullptr, (float*)(b + om), a.gz ? (float*)(b + os) : nullptr, a.gs,
-           (float*)(b + on), t.ldp, a.M, a.N, a.K, t.Kp, a.G, (a.M + 3) / 4};
+           (float*)(b + on), t.ldp, a.M, a.N, a.K, t.Kp, a.G, (a.M + 3) / 4, few};
   t.xh = p.xh;
   t.xl = p.xl;
   t.rm = p.rm;
