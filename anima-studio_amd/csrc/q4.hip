@@ -600,17 +600,14 @@ __global__ __launch_bounds__(64 * QF_WAVES, 2) void q4_few_kernel(Q4Tile q) {
 // ------------------------------------------------------------------ tiles
 
 // One BM x BN tile a workgroup, waves of WM rows x WN columns.  A step is 64 k: BM rows of x (128 bytes, each term) and BN columns'
-// codes (32 bytes) in one of four LDS stages, filled three steps ahead by buffer_load ... lds.  x's units of 16 bytes lie at slot
+// codes (32 bytes) in one of NST LDS stages, filled ahead by buffer_load ... lds.  x's units of 16 bytes lie at slot
 // u ^ (row / 2 % 8) (sixteen rows' reads of one unit touch each bank once).  Lane (n, half) takes the 16 bytes of column n's 32 k of
 // its half, so that matrix step i of a lane pair covers k 8 i .. 8 i + 7 of both halves; x's units follow.  The scales of four
 // steps come in one load where rows of them allow it: each of a lane's own addresses costs the address unit as
 // much as 64 neighbouring bytes.
-constexpr int q4_waves(int BM, int BN, int WM, int WN, int TERMS) {  // waves a SIMD that a tile's LDS leaves room for
-  return (BM / WM) * (BN / WN) < 8 && (TERMS * BM * 128 + BN * 32) * 4 > 81920 ? 1 : 2;
-}
-template <int BM, int BN, int WM, int WN, int TERMS>
-__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), q4_waves(BM, BN, WM, WN, TERMS)) void q4_tile_kernel(Q4Tile t) {
-  constexpr int NWM = BM / WM, NW = NWM * (BN / WN), MT = WM / 32, NT = WN / 32, NST = 4;
+template <int BM, int BN, int WM, int WN, int TERMS, int NST>
+__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void q4_tile_kernel(Q4Tile t) {
+  constexpr int NWM = BM / WM, NW = NWM * (BN / WN), MT = WM / 32, NT = WN / 32;
   constexpr int XB = BM * 128, WO = XB * TERMS, SB = WO + BN * 32, CX = TERMS * BM / 8 / NW, CW = (BN / 32 + NW - 1) / NW, CPW = CX + CW;
   static_assert(CX * NW * 8 == TERMS * BM, "whole copies");
   constexpr int RS = WN + 4, EPL = NW * 32 * RS * 4;
@@ -645,14 +642,15 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), q4_waves(BM, BN, WM, WN
   }
 #pragma unroll
   for (int c = 0; c < CW; c++) wo[c] = (uint32_t)(32 * min(wave * CW + c, BN / 32 - 1) + (lane >> 1)) * (uint32_t)(K / 2) + 16 * (lane & 1);
-  const auto copies = [&](int step, int p) __attribute__((always_inline)) {
+  const auto copies = [&](int step, int po) __attribute__((always_inline)) {  // into the stage at po
 #pragma unroll
     for (int c = 0; c < CX; c++)
-      q4_copy16(TERMS > 1 && wave * CX + c >= BM / 8 ? rl : rh, smem + p * SB + (wave * CX + c) * 1024, xo[c], 128 * step);
+      q4_copy16(TERMS > 1 && wave * CX + c >= BM / 8 ? rl : rh, smem + po + (wave * CX + c) * 1024, xo[c], 128 * step);
     // (K of an odd number of 32: the last half is the next column's or past the end, and meets zeros of x)
 #pragma unroll
-    for (int c = 0; c < CW; c++) q4_copy16(rw, smem + p * SB + WO + min(wave * CW + c, BN / 32 - 1) * 1024, wo[c], 32 * (s0 + step));
+    for (int c = 0; c < CW; c++) q4_copy16(rw, smem + po + WO + min(wave * CW + c, BN / 32 - 1) * 1024, wo[c], 32 * (s0 + step));
   };
+  copies(0, 0);
   // The scales of steps s .. s + 3 (s % 4 == 0): as they lie, if four steps' are one aligned piece of the row, else one by one; then
   // each step's as a pair for the decode.
   const uint16_t* srow[NT];
@@ -665,7 +663,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), q4_waves(BM, BN, WM, WN
   }
   const int lg = 31 - __builtin_clz(a.G);
   u32x4 sc[NT];
-  f16x2 sv[NST][NT];
+  f16x2 sv[4][NT];
   const auto scales = [&](int step) __attribute__((always_inline)) {
     const int g = (s0 + step) * 64 >> lg;
 #pragma unroll
@@ -713,6 +711,48 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), q4_waves(BM, BN, WM, WN
   for (int i = 0; i < MT; i++)
 #pragma unroll
     for (int j = 0; j < NT; j++) acc[i][j] = f32x16{};
+  scales(0);
+#pragma unroll
+  for (int p = 1; p < NST; p++) copies(p, p * SB);
+  // The middles' part (with the first split): z in bf16 as it is, the groups' sums of x as three bf16 terms, sixteen groups a
+  // matrix step, both with the powers that the sums to come have.
+  if (a.gz && blockIdx.y == 0) {
+    for (int g0 = 0; g0 < KG; g0 += 16) {
+      bf16x8 zf[NT], xs[MT][3];
+#pragma unroll
+      for (int j = 0; j < NT; j++) {
+        const uint16_t* zr = a.gz + (int64_t)min(bn + wn + 32 * j + r, a.N - 1) * KG;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const int g = g0 + 8 * hf + e;
+          const float z = bf16_f(zr[min(g, KG - 1)]);
+          zf[j][e] = to_bf16(g < KG ? z * fn[j] : 0.0f);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < MT; i++) {
+        const int m = min(bm + wm + 32 * i + r, a.M - 1);
+        const float up = 1.0f / t.rm[m];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const int g = g0 + 8 * hf + e;
+          float v = t.sx[(int64_t)m * KG + min(g, KG - 1)] * up;
+          v = g < KG ? v : 0.0f;
+#pragma unroll
+          for (int c = 0; c < 3; c++) {
+            xs[i][c][e] = to_bf16(v);
+            v -= (float)xs[i][c][e];
+          }
+        }
+      }
+#pragma unroll
+      for (int c = 2; c >= 0; c--)
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+          for (int j = 0; j < NT; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(zf[j], xs[i][c], acc[i][j], 0, 0, 0);
+    }
+  }
   int xa[4];  // unit 4 hf + i of row r
 #pragma unroll
   for (int i = 0; i < 4; i++) xa[i] = (wm + r) * 128 + 16 * ((4 * hf + i) ^ ((r >> 1) & 7));
@@ -720,53 +760,52 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), q4_waves(BM, BN, WM, WN
 
   // Fragments of matrix step i + 1 are read and decoded under step i's products.  Before the last of a stage's four, whose
   // fragments are in registers by then, a barrier ends every wave's reads of the stage (its buffer is refilled) and publishes
-  // the next one: this wave's copies of it have arrived when at most those of the two stages after it pend.
+  // the next one: this wave's copies of it have arrived when at most those of the stages after it pend.
   f16x8 xf[2][MT][TERMS], wf[2][NT];
   u32x4 wr[NT];
-  const auto xread = [&](int u, int p, int i) __attribute__((always_inline)) {
+  const auto xread = [&](int u, int po, int i) __attribute__((always_inline)) {
 #pragma unroll
     for (int m = 0; m < MT; m++)
 #pragma unroll
-      for (int e = 0; e < TERMS; e++) xf[u][m][e] = *(const f16x8*)(smem + p * SB + e * XB + m * 4096 + xa[i]);
+      for (int e = 0; e < TERMS; e++) xf[u][m][e] = *(const f16x8*)(smem + po + xa[i] + e * XB + m * 4096);
   };
-  const auto wread = [&](int p) __attribute__((always_inline)) {
+  const auto wread = [&](int po) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < NT; j++) wr[j] = *(const u32x4*)(smem + p * SB + wa + j * 1024);
+    for (int j = 0; j < NT; j++) wr[j] = *(const u32x4*)(smem + po + wa + j * 1024);
   };
-  const auto decode = [&](int u, int p, int i) __attribute__((always_inline)) {
+  const auto decode = [&](int u, int q, int i) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < NT; j++) wf[u][j] = q4_decode(wr[j][i], sv[p][j]);
+    for (int j = 0; j < NT; j++) wf[u][j] = q4_decode(wr[j][i], sv[q][j]);
   };
-  scales(0);
-#pragma unroll
-  for (int p = 0; p < NST; p++) copies(p, p);
   pairs();
   Q4_WAIT_VM((NST - 1) * CPW);
   q4_barrier();
-  scales(NST);
+  scales(4);
   wread(0);
   xread(0, 0, 0);
   decode(0, 0, 0);
-  const auto stage = [&](int step, auto buffer) __attribute__((always_inline)) {
-    constexpr int p = decltype(buffer)::value, pn = (p + 1) % NST;
+  int po = 0;  // the stage's place
+  const auto stage = [&](int step, auto quarter) __attribute__((always_inline)) {
+    constexpr int q = decltype(quarter)::value, qn = (q + 1) % 4;  // of its four
+    const int pn = po + SB == NST * SB ? 0 : po + SB;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       const int u = i & 1;
       if (i == 3) {
         __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
-        Q4_WAIT_VM(2 * CPW);
+        Q4_WAIT_VM((NST - 2) * CPW);
         q4_barrier();
-        copies(step + NST, p);
+        copies(step + NST, po);
         wread(pn);
         xread(u ^ 1, pn, 0);
-        if (p == NST - 1) {
+        if (q == 3) {
           pairs();
-          scales(step + 1 + NST);
+          scales(step + 5);
         }
-        decode(u ^ 1, pn, 0);
+        decode(u ^ 1, qn, 0);
       } else {
-        xread(u ^ 1, p, i + 1);
-        decode(u ^ 1, p, i + 1);
+        xread(u ^ 1, po, i + 1);
+        decode(u ^ 1, q, i + 1);
       }
 #pragma unroll
       for (int e = TERMS - 1; e >= 0; e--)
@@ -776,9 +815,10 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), q4_waves(BM, BN, WM, WN
           for (int j = 0; j < NT; j++) acc[m][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(wf[u][j], xf[u][m][e], acc[m][j], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
     }
+    po = pn;
   };
   int s = 0;
-  for (; s + NST <= steps; s += NST) {
+  for (; s + 4 <= steps; s += 4) {
     stage(s, std::integral_constant<int, 0>{});
     stage(s + 1, std::integral_constant<int, 1>{});
     stage(s + 2, std::integral_constant<int, 2>{});
@@ -794,28 +834,18 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), q4_waves(BM, BN, WM, WN
   float* rows = (float*)smem + wave * 32 * RS;
   constexpr int LR = WN / 4, PR = 64 / LR;
   const int n0 = bn + wn;
-  const bool zero = a.gz && blockIdx.y == 0;  // (the middles' part goes with the first split)
 #pragma unroll
   for (int i = 0; i < MT; i++) {
     const int m = bm + wm + 32 * i + r, mc = min(m, a.M - 1);
     const float fm = t.rm[mc];
 #pragma unroll
     for (int j = 0; j < NT; j++) {
-      f32x16 z = {};
-      if (zero) {
-        const uint16_t* zr = a.gz + (int64_t)min(n0 + 32 * j + r, a.N - 1) * KG;
-        const float* xr = t.sx + (int64_t)mc * KG;
-        for (int g = hf; g < KG + hf; g += 2) {  // (an odd last group: zeros in the other half)
-          const bool in = g < KG;
-          z = __builtin_amdgcn_mfma_f32_32x32x2f32(in ? bf16_f(zr[min(g, KG - 1)]) : 0.0f, in ? xr[min(g, KG - 1)] : 0.0f, z, 0, 0, 0);
-        }
-      }
 #pragma unroll
       for (int q = 0; q < 4; q++) {
         const f32x4 f = *(const f32x4*)(t.rn + n0 + 32 * j + 8 * q + 4 * hf);
         f32x4 v;
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = acc[i][j][4 * q + e] * f[e] * fm + z[4 * q + e];
+        for (int e = 0; e < 4; e++) v[e] = acc[i][j][4 * q + e] * f[e] * fm;
         *(f32x4*)(rows + r * RS + 32 * j + 8 * q + 4 * hf) = v;
       }
     }
@@ -947,10 +977,10 @@ static int64_t q4_few_lds(const Q4Args& a) {
   return std::max<int64_t>((int64_t)(a.K / a.G) * 128 * (a.gz ? 2 : 1), QF_WAVES * 4096);
 }
 
-template <int BM, int BN, int WM, int WN, int TERMS>
+template <int BM, int BN, int WM, int WN, int TERMS, int NST>
 static void q4_tile_launch(anima_ctx* c, const Q4Tile& t, int splits) {
   const dim3 grid((unsigned)(((t.a.N + BN - 1) / BN) * ((t.a.M + BM - 1) / BM)), (unsigned)splits), block(64 * (BM / WM) * (BN / WN));
-  hipLaunchKernelGGL((q4_tile_kernel<BM, BN, WM, WN, TERMS>), grid, block, 0, c->stream, t);
+  hipLaunchKernelGGL((q4_tile_kernel<BM, BN, WM, WN, TERMS, NST>), grid, block, 0, c->stream, t);
 }
 
 // x into f16 terms (and the columns' powers), then the products, then, where k was split, the sums.
@@ -965,8 +995,9 @@ static int q4_matrix(anima_ctx* c, const Q4Args& a, bool two) {
   const bool few = a.M <= 64 && q4_few_lds(a) <= Q4_FEW_LDS;
   const auto tiles = [&](int bm, int bn) { return (int64_t)((a.M + bm - 1) / bm) * ((a.N + bn - 1) / bn); };
   // the largest tile of which there are enough
-  const int tile = tiles(two ? 128 : 256, 256) >= c->num_cus ? 0 : tiles(128, 128) >= c->num_cus ? 1 : 2;
-  const int64_t nt = tile == 0 ? tiles(two ? 128 : 256, 256) : tile == 1 ? tiles(128, 128) : tiles(64, 64);
+  const int rows = two ? 64 : 128;  // of the larger tiles
+  const int tile = tiles(rows, 256) >= c->num_cus ? 0 : tiles(rows, 128) >= c->num_cus ? 1 : 2;
+  const int64_t nt = tile == 0 ? tiles(rows, 256) : tile == 1 ? tiles(rows, 128) : tiles(64, 64);
   int splits = 1;
   while (!few && splits < Q4_SPLITS && nt * splits * 2 <= c->num_cus && steps / (splits * 2) >= 4) splits *= 2;
   t.sps = (steps + splits - 1) / splits;
@@ -1010,13 +1041,13 @@ static int q4_matrix(anima_ctx* c, const Q4Args& a, bool two) {
     else if (a.G == 32) hipLaunchKernelGGL((q4_few_kernel<1, true>), grid, block, lds, c->stream, t);
     else hipLaunchKernelGGL((q4_few_kernel<1, false>), grid, block, lds, c->stream, t);
   } else if (two) {
-    if (tile == 0) q4_tile_launch<128, 256, 64, 64, 2>(c, t, splits);
-    else if (tile == 1) q4_tile_launch<128, 128, 64, 64, 2>(c, t, splits);
-    else q4_tile_launch<64, 64, 32, 32, 2>(c, t, splits);
+    if (tile == 0) q4_tile_launch<64, 256, 64, 64, 2, 3>(c, t, splits);
+    else if (tile == 1) q4_tile_launch<64, 128, 64, 32, 2, 4>(c, t, splits);
+    else q4_tile_launch<64, 64, 32, 32, 2, 4>(c, t, splits);
   } else {
-    if (tile == 0) q4_tile_launch<256, 256, 128, 64, 1>(c, t, splits);
-    else if (tile == 1) q4_tile_launch<128, 128, 64, 64, 1>(c, t, splits);
-    else q4_tile_launch<64, 64, 32, 32, 1>(c, t, splits);
+    if (tile == 0) q4_tile_launch<128, 256, 128, 64, 1, 3>(c, t, splits);
+    else if (tile == 1) q4_tile_launch<128, 128, 64, 64, 1, 4>(c, t, splits);
+    else q4_tile_launch<64, 64, 32, 32, 1, 4>(c, t, splits);
   }
   if (splits > 1)
     hipLaunchKernelGGL(q4_join_kernel, dim3((unsigned)(((int64_t)a.M * ((a.N + 3) / 4) + 255) / 256)), dim3(256), 0, c->stream, t, splits);
