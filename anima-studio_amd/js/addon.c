@@ -562,6 +562,58 @@ static napi_value js_attention(napi_env env, napi_callback_info info) {
   return NULL;
 }
 
+/* attentionPrefix(ctx, desc) -- desc mirrors anima_prefix_attn_desc (pointers as Numbers, lens an Int32Array); with
+ * prepareInto (and prepareBytes) it runs anima_attention_prefix_prepare into that buffer */
+static napi_value js_attention_prefix(napi_env env, napi_callback_info info) {
+  napi_value argv[2];
+  get_args(env, info, 2, argv);
+  anima_ctx* c = ctx_of(env, argv[0]);
+  napi_value o = argv[1], lens = prop(env, o, "lens"), ab;
+  napi_typedarray_type type;
+  size_t n = 0, off;
+  void* data = NULL;
+  if (napi_get_typedarray_info(env, lens, &type, &n, &data, &ab, &off) != napi_ok || type != napi_int32_array || n > INT32_MAX) {
+    napi_throw_type_error(env, NULL, "attentionPrefix: lens must be an Int32Array");
+    return NULL;
+  }
+  anima_prefix_attn_desc d;
+  memset(&d, 0, sizeof d);
+  d.B = (int)n;
+  d.len = (const int*)data;
+  d.P = (int)pnum(env, o, "P");
+  d.H = (int)pnum(env, o, "H");
+  d.D = (int)pnum(env, o, "D");
+  d.group = (int)pnum(env, o, "group");
+  d.q = (const float*)pptr(env, o, "q");
+  d.k = (const float*)pptr(env, o, "k");
+  d.v = (const float*)pptr(env, o, "v");
+  d.o = (float*)pptr(env, o, "o");
+  d.ldq = (int64_t)pnum(env, o, "ldq");
+  d.ldk = (int64_t)pnum(env, o, "ldk");
+  d.ldv = (int64_t)pnum(env, o, "ldv");
+  d.ldo = (int64_t)pnum(env, o, "ldo");
+  d.q_off = (int64_t)pnum(env, o, "qOff");
+  d.k_off = (int64_t)pnum(env, o, "kOff");
+  d.v_off = (int64_t)pnum(env, o, "vOff");
+  d.o_off = (int64_t)pnum(env, o, "oOff");
+  d.prefix_kv = pptr(env, o, "prefixKv");
+  d.prefix_kv_bytes = (int64_t)pnum(env, o, "prefixKvBytes");
+  d.scale = (float)pnum(env, o, "scale");
+  d.causal = (int)pnum(env, o, "causal");
+  d.precision = (int)pnum(env, o, "precision");
+  d.q_norm = (const float*)pptr(env, o, "qNorm");
+  d.k_norm = (const float*)pptr(env, o, "kNorm");
+  d.rope_cs = (const float*)pptr(env, o, "cs");
+  d.rope_sin_off = (int64_t)pnum(env, o, "sinOff");
+  d.eps = (float)pnum(env, o, "eps");
+  d.o_bf16 = (int)pnum(env, o, "oBf16");
+  void* into = pptr(env, o, "prepareInto");
+  int64_t bytes = (int64_t)pnum(env, o, "prepareBytes");
+  if (into) CHECK_RC(env, c, anima_attention_prefix_prepare(c, &d, into, bytes));
+  else CHECK_RC(env, c, anima_attention_prefix(c, &d));
+  return NULL;
+}
+
 /* attentionKvBytes(B, Hkv, Lk, precision) */
 static napi_value js_attention_kv_bytes(napi_env env, napi_callback_info info) {
   napi_value a[4];
@@ -736,6 +788,9 @@ static void read_weight(napi_env env, napi_value wo, anima_weight* w) {
   w->srel = (const uint8_t*)pptr(env, wo, "srel");
   w->codebook = (const float*)pptr(env, wo, "codebook");
   w->bias = (const float*)pptr(env, wo, "bias");
+  w->group = (int)pnum(env, wo, "group");
+  w->group_scale = (const uint16_t*)pptr(env, wo, "groupScale");
+  w->group_mid = (const uint16_t*)pptr(env, wo, "groupMid");
 }
 
 /* weightUnpackW4(ctx, weight, grid) */
@@ -803,6 +858,29 @@ static napi_value js_weight_quant_f8(napi_env env, napi_callback_info info) {
   anima_ctx* c = ctx_of(env, a[0]);
   CHECK_RC(env, c, anima_weight_quant_f8(c, ptr(env, a[1]), (int)num(env, a[2]), (int)num(env, a[3]), (int)num(env, a[4]),
                                          (uint8_t*)ptr(env, a[5]), (float*)ptr(env, a[6])));
+  return NULL;
+}
+
+/* weightQuantQ4(ctx, w, bf16, N, K, group, q, scale, mid): anima_weight_quant_q4 */
+static napi_value js_weight_quant_q4(napi_env env, napi_callback_info info) {
+  napi_value a[9];
+  get_args(env, info, 9, a);
+  anima_ctx* c = ctx_of(env, a[0]);
+  CHECK_RC(env, c, anima_weight_quant_q4(c, ptr(env, a[1]), (int)num(env, a[2]), (int)num(env, a[3]), (int)num(env, a[4]),
+                                         (int)num(env, a[5]), (uint8_t*)ptr(env, a[6]), (uint16_t*)ptr(env, a[7]),
+                                         (uint16_t*)ptr(env, a[8])));
+  return NULL;
+}
+
+/* embedRows(ctx, table, ids, T, weights, scale, out, ldo): anima_embed_rows */
+static napi_value js_embed_rows(napi_env env, napi_callback_info info) {
+  napi_value a[8];
+  get_args(env, info, 8, a);
+  anima_ctx* c = ctx_of(env, a[0]);
+  anima_weight w;
+  read_weight(env, a[1], &w);
+  CHECK_RC(env, c, anima_embed_rows(c, &w, (const int32_t*)ptr(env, a[2]), i64(env, a[3]), (const float*)ptr(env, a[4]),
+                                    (float)num(env, a[5]), (float*)ptr(env, a[6]), i64(env, a[7])));
   return NULL;
 }
 
@@ -1063,6 +1141,7 @@ static napi_value Init(napi_env env, napi_value exports) {
       FN("graphBegin", js_graph_begin), FN("graphEnd", js_graph_end), FN("graphLaunch", js_graph_launch),
       FN("graphDestroy", js_graph_destroy), FN("conv3x3", js_conv3x3), FN("channelNorm", js_channel_norm), FN("toRgba", js_to_rgba),
       FN("weightUnpackW4", js_weight_unpack_w4),
+      FN("weightQuantQ4", js_weight_quant_q4), FN("embedRows", js_embed_rows), FN("attentionPrefix", js_attention_prefix),
   };
 #undef FN
   if (napi_define_properties(env, exports, sizeof desc / sizeof desc[0], desc) != napi_ok) return NULL;

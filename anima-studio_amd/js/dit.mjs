@@ -754,13 +754,20 @@ export async function adapt(gpu, A, hidden, t5Ids, t5Weights, precision) {
   x.release();
   const on = ops.rmsnorm(gpu, o, A.norm, D);
   o.release();
-  // prompt weights and zero rows up to 512 (on the host, as the reference: tiny)
+  // prompt weights and zero rows up to 512
+  const rows = Math.max(ADAPTER.ctxLen, Lt);
+  const weights = Array.from({ length: Lt }, (_, i) => (t5Weights ? t5Weights[i] : 1));
+  if (weights.every((w) => Math.fround(w) === w)) {
+    // on the device: one rounding of the product, as on the host
+    const out = ops.embedRows(gpu, { kind: "f32", N: Lt, K: D, buf: on.buf }, Array.from({ length: rows }, (_, i) => (i < Lt ? i : -1)),
+      { weights: weights.concat(new Array(rows - Lt).fill(0)) });
+    on.release();
+    return out;
+  }
+  // weights of more than 24 bits (on the host, as the reference: tiny)
   const vals = await gpu.read(on);
   on.release();
-  const ctx = new Float32Array(Math.max(ADAPTER.ctxLen, Lt) * D);
-  for (let i = 0; i < Lt; i++) {
-    const w = t5Weights ? t5Weights[i] : 1;
-    for (let j = 0; j < D; j++) ctx[i * D + j] = vals[i * D + j] * w;
-  }
-  return gpu.fromArray(ctx, [ctx.length / D, D]);
+  const ctx = new Float32Array(rows * D);
+  for (let i = 0; i < Lt; i++) for (let j = 0; j < D; j++) ctx[i * D + j] = vals[i * D + j] * weights[i];
+  return gpu.fromArray(ctx, [rows, D]);
 }

@@ -8,13 +8,17 @@
 //              on a quantized weight reads them too (setLoraInput), or the fp32 input opts.xr / x.
 //   linear on an e4m3 weight (kind "f8"): opts.xq = { q, s } of quantRowsF8 / linearGlu / residualNorm,
 //              opts.precision and opts.outBf16.
+//   linear on a 4-bit weight with group scales (kind "q4", quantizeQ4): fp32 rows, opts.precision and
+//              opts.outBf16.
+//   embedRows: rows of an embedding table that lies on the device, with a weight a row.
+//   attentionPrefix, attentionPrefixPrepare: sequences of different lengths, packed, behind one shared prefix.
 //   linearGlu, residualNorm: a gated feed-forward's first half, and the residual addition with the
 //              next block's norm, each one kernel, with e4m3 rows out.
 //   layernormModQ: LayerNorm + adaLN + ConvRot + per-token int8 in one pass.
 
 import { native } from "./gpu.mjs";
 
-const KIND = { bf16: 0, i8: 1, w4: 2, f32: 3, f32s3: 4, f8: 5 };
+const KIND = { bf16: 0, i8: 1, w4: 2, f32: 3, f32s3: 4, f8: 5, q4: 6 };
 const ACT = { none: 0, gelu: 1, silu: 2 };
 const NORM = { rms: 0, layer: 1 };
 const EW = { silu_mul: 0, add: 1, silu: 2, copy: 3 };
@@ -109,6 +113,51 @@ export function quantizeF8(gpu, W) {
   return W;
 }
 
+// A bf16 or f32 weight turned into the 4-bit weight with a bf16 scale per `group` values along K (32, 64
+// or 128; default 64), in place (as quantizeF8).  opts.mid: a bf16 middle value per group as well, so that the
+// codes span the group's range and not twice its largest magnitude.  A weight is off by half a step, a 14th of
+// the group's largest magnitude or a 30th of its range.  Other kinds, and input widths that are no multiple of
+// the group, stay as they are.
+export function quantizeQ4(gpu, W, opts) {
+  const o = opts || {}, group = o.group || 64;
+  if (group !== 32 && group !== 64 && group !== 128) throw new Error(`${W.name || "weight"}: groups of ${group} (32, 64 or 128)`);
+  if ((W.kind !== "bf16" && W.kind !== "f32") || W.K % group) return W;
+  const q = gpu.empty([(W.N * W.K) / 2], "u8");
+  const scale = gpu.empty([W.N, W.K / group], "bf16"), mid = o.mid ? gpu.empty([W.N, W.K / group], "bf16") : null;
+  native.weightQuantQ4(gpu.ctx, ptr(W.buf), W.kind === "bf16" ? 1 : 0, W.N, W.K, group, q.buf, scale.buf, ptr(mid));
+  if (W.buf.release) W.buf.release();
+  W.kind = "q4";
+  W.buf = q;
+  W.group = group;
+  W.groupScale = scale;
+  W.groupMid = mid;
+  return W;
+}
+
+// Rows ids of an embedding table on the device ({ kind: "f32" | "bf16" | "q4", N, K, buf }): a tensor
+// [ids.length, K], each row times opts.weights[t] and opts.scale (default 1).  ids: an array or a Tensor
+// (i32); an id outside [0, N) gives a row of zeros.  opts.weights: an array or a Tensor; opts.out: the tensor
+// to write.
+export function embedRows(gpu, table, ids, opts) {
+  const o = opts || {};
+  if (table.kind !== "f32" && table.kind !== "bf16" && table.kind !== "q4") throw new Error(`embedRows: a ${table.kind} table (f32, bf16 or q4)`);
+  const onDevice = (t, T) => (t && t.buf !== undefined ? t : T.from(t));
+  const id = onDevice(ids, Int32Array), T = id.buf !== undefined ? id.size : id.length;
+  checkDtype("embedRows: ids", id, "i32");
+  const w = o.weights ? onDevice(o.weights, Float32Array) : null;
+  checkDtype("embedRows: weights", w, "f32");
+  if (w && (w.buf !== undefined ? w.size : w.length) !== T) throw new Error(`embedRows: ${w.buf !== undefined ? w.size : w.length} weights for ${T} rows`);
+  checkDtype("embedRows: out", o.out, "f32");
+  if (o.out && o.out.size < T * table.K) throw new Error(`embedRows: ${T} rows of ${table.K} do not fit into ${o.out.size} values`);
+  const idT = id.buf !== undefined ? id : gpu.fromArray(id, [T]);
+  const wT = !w || w.buf !== undefined ? w : gpu.fromArray(w, [T]);
+  const out = o.out || gpu.empty([T, table.K]);
+  native.embedRows(gpu.ctx, weightArg(table), idT.buf, T, ptr(wT), o.scale || 0, out.buf, 0);
+  if (idT !== ids) idT.release();
+  if (wT && wT !== o.weights) wT.release();
+  return out;
+}
+
 // opts.xq of a linear on W: the row form that W's kind reads (int8 rows and e4m3 rows are both bytes),
 // and e4m3 rows of W's width.  Their scales lie block by block, [ceil(K / 128), rows], so opts.M, if
 // given, has to be the number of rows: any other M would read other rows' scales.  Returns the number.
@@ -133,7 +182,7 @@ function checkDtype(name, t, dtype) {
 function weightArg(W) {
   if (!(W.kind in KIND)) throw new Error(`unsupported weight kind ${W.kind}`);
   return { kindId: KIND[W.kind], N: W.N, K: W.K, buf: ptr(W.buf), scale: ptr(W.scale), srel: ptr(W.srel),
-    codebook: ptr(W.codebook), bias: ptr(W.bias) };
+    codebook: ptr(W.codebook), bias: ptr(W.bias), group: W.group || 0, groupScale: ptr(W.groupScale), groupMid: ptr(W.groupMid) };
 }
 
 // y = x @ W^T (+ bias) (act) (ops.js:48-66).  Quantized weights take the ConvRot-rotated input
@@ -141,9 +190,11 @@ function weightArg(W) {
 // opts.out + opts.resid: out += (gate[gOff + n] *) y in place.
 // On an "f8" weight, opts.precision: "fp32" (default: products added in 32 bits) or "bf16" (by the
 // 8-bit matrix instructions, about 1.5e-5 of the result, twice the rate), and opts.outBf16: a bf16
-// result (no residual).
+// result (no residual).  On a "q4" weight likewise: "bf16" may round x to 11 bits.
 export function linear(gpu, x, W, opts) {
   const o = opts || {};
+  const own = W.kind === "f8" || W.kind === "q4"; // with a precision and a bf16 result of its own
+  if (o.xq && W.kind === "q4") throw new Error(`${W.name || "linear"}: quantized rows for a q4 weight`);
   const rows = o.xq ? checkRows(W, o.xq, o.M) : 0;
   const M = o.M !== undefined ? o.M : (o.xq ? rows : x.size / W.K);
   // LoRAs: y += sum_i scale_i B_i (A_i x), after the bias and before act / gate (ops.js:55-62).
@@ -167,9 +218,9 @@ export function linear(gpu, x, W, opts) {
     : linear(gpu, xin, { kind: "f32s3", N: F.R, K: W.K, buf: rot ? F.Ars : F.As }, { M });
   const late = lora && !F && !o.resid && ACT[o.act || "none"] === 0;
   const delta = lora && !F && !late ? loraDelta(gpu, xin, W, M, rot) : null;
-  if (o.outBf16 && W.kind !== "f8") throw new Error(`${W.name || "linear"}: bf16 results are for f8 weights`);
+  if (o.outBf16 && !own) throw new Error(`${W.name || "linear"}: bf16 results are for f8 and q4 weights`);
   if (o.outBf16 && late) throw new Error(`${W.name || "linear"}: no bf16 result with a LoRA`);
-  if (W.kind === "f8") {
+  if (own) {
     if (!o.xq) checkDtype(`${W.name || "linear"}: x`, x, "f32");
     checkDtype(`${W.name || "linear"}: out`, o.out, o.outBf16 ? "bf16" : "f32");
   }
@@ -178,7 +229,7 @@ export function linear(gpu, x, W, opts) {
     epilogue: o.resid ? (o.gate ? 2 : 1) : 0, gate: ptr(o.gate), gOff: o.gOff || 0, accOut: ptr(o.accOut),
     add: delta ? delta.buf : 0, ldAdd: delta ? W.N : 0,
     loraXa: down ? down.buf : 0, ldLoraXa: down ? F.R : 0, loraB: F ? F.Bs.buf : 0, loraR: F ? F.Rb : 0,
-    loraCols: F ? F.cols : 0, precision: W.kind === "f8" ? precisionId(o) : 0, outBf16: o.outBf16 ? 1 : 0 };
+    loraCols: F ? F.cols : 0, precision: own ? precisionId(o) : 0, outBf16: o.outBf16 ? 1 : 0 };
   if ((needsRotation(W) || W.kind === "f32s3" || W.kind === "f8") && o.xq) {
     d.xq = o.xq.q.buf;
     d.xs = o.xq.s.buf;
@@ -526,6 +577,52 @@ export function attentionPrepareKV(gpu, a) {
   const o = a.out || { buf: a.q.buf };
   native.attention(gpu.ctx, attnDesc(a, B, H, D, o, { prepareInto: prep.buf, kvPrepBytes: bytes }));
   return prep;
+}
+
+// Attention of packed sequences behind one shared prefix (anima_attention_prefix): a.lens[b] rows of each
+// sequence, one behind the other in a.q / a.k / a.v (strides and offsets as attention's), row i of a sequence at
+// position P + i.  a.prefix: the prefix's keys and values of attentionPrefixPrepare, P their number (absent: 0); at
+// the same precision.  Causal unless a.causal is false.  Returns [sum of lens, H * D] (a.out, or a new tensor).
+export function attentionPrefix(gpu, a) {
+  const lens = Int32Array.from(a.lens), T = lens.reduce((s, n) => s + n, 0);
+  const o = a.out || gpu.empty([T, a.H * a.D], a.oBf16 ? "bf16" : "f32");
+  checkDtype("attentionPrefix: out", o, a.oBf16 ? "bf16" : "f32");
+  if (a.prefix && (a.prefix.precision !== precisionId(a) || a.prefix.heads !== a.H / (a.group || 1)))
+    throw new Error("attentionPrefix: a prefix of another precision or of other heads");
+  const d = prefixDesc(a, lens, T, a.prefix ? a.prefix.keys : 0);
+  const ldo = a.ldo || a.H * a.D;
+  prefixRows("out", o, T, ldo, a.oOff || 0, a.H * a.D);
+  prefixRows("q", a.q, T, a.ldq, a.qOff || 0, a.H * a.D);
+  native.attentionPrefix(gpu.ctx, Object.assign(d, { q: a.q.buf, ldq: a.ldq, qOff: a.qOff || 0, o: o.buf, ldo, oOff: a.oOff || 0,
+    prefixKv: ptr(a.prefix), prefixKvBytes: a.prefix ? a.prefix.bytes : 0, qNorm: ptr(a.qNorm), oBf16: a.oBf16 ? 1 : 0 }));
+  return o;
+}
+
+// The keys and values of a.len rows at positions 0 ... as a prefix for attentionPrefix: a new buffer, normed,
+// rotated and in the form that the precision multiplies.
+export function attentionPrefixPrepare(gpu, a) {
+  const heads = a.H / (a.group || 1), d = prefixDesc(a, Int32Array.of(a.len), a.len, 0);
+  const bytes = native.attentionKvBytes(1, heads, a.len, precisionId(a));
+  const prep = gpu.empty([bytes], "u8");
+  native.attentionPrefix(gpu.ctx, Object.assign(d, { prepareInto: prep.buf, prepareBytes: bytes }));
+  return Object.assign(prep, { keys: a.len, precision: precisionId(a), heads });
+}
+
+// the fields that both read
+function prefixDesc(a, lens, T, P) {
+  const kv = (a.H / (a.group || 1)) * a.D;
+  prefixRows("k", a.k, T, a.ldk, a.kOff || 0, kv);
+  prefixRows("v", a.v, T, a.ldv, a.vOff || 0, kv);
+  return { lens, P, H: a.H, D: a.D, group: a.group || 1, k: a.k.buf, ldk: a.ldk, kOff: a.kOff || 0, v: a.v.buf, ldv: a.ldv,
+    vOff: a.vOff || 0, scale: a.scale || 0, causal: a.causal === false ? 0 : 1, precision: precisionId(a), kNorm: ptr(a.kNorm),
+    cs: ptr(a.cs), sinOff: a.cs ? a.cs.sinOff : 0, eps: 1e-6 };
+}
+
+// T rows of `cols` values at `off`, ld apart, have to lie in t
+function prefixRows(name, t, T, ld, off, cols) {
+  if (name !== "out") checkDtype(`attentionPrefix: ${name}`, t, "f32");
+  if (T > 0 && t.size < (T - 1) * ld + off + cols)
+    throw new Error(`attentionPrefix: ${name} of ${t.size} values does not hold ${T} rows ${ld} apart`);
 }
 
 function precisionId(a) {

@@ -71,6 +71,33 @@ export class LatentPipeline {
     return cond;
   }
 
+  // Several prompts (as encode's) at once -> their conditionings, in order: those not cached pass the text
+  // encoder together (Qwen3.encodeBatch: the tokens that they all begin with once).  They alone stay cached.
+  async encodeBatch(prompts) {
+    if (!this.te || !this.adapter) throw new Error("encodeBatch: the pipeline was built without opts.te / opts.adapter");
+    const byKey = new Map(prompts.map((p) => [promptKey(p), p]));
+    if (this.ctxGeneration !== loraGeneration()) {
+      this.clearContexts();
+      this.ctxGeneration = loraGeneration();
+    }
+    for (const [k, t] of this.ctxCache)
+      if (!byKey.has(k)) {
+        t.release();
+        this.ctxCache.delete(k);
+      }
+    const missing = Array.from(byKey.keys()).filter((k) => !this.ctxCache.has(k));
+    this.stats.encodeMisses += missing.length;
+    this.stats.encodeHits += prompts.length - missing.length;
+    const hidden = await this.te.encodeBatch(missing.map((k) => byKey.get(k).qwenIds));
+    for (let i = 0; i < missing.length; i++) {
+      const p = byKey.get(missing[i]);
+      const ctx = await adapt(this.gpu, this.adapter, hidden[i], p.t5Ids, p.t5Weights);
+      hidden[i].release();
+      this.ctxCache.set(missing[i], this.dit.prepareContext([ctx]));
+    }
+    return prompts.map((p) => this.ctxCache.get(promptKey(p)));
+  }
+
   clearContexts() {
     for (const t of this.ctxCache.values()) t.release();
     this.ctxCache.clear();

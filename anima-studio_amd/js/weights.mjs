@@ -121,6 +121,24 @@ export class SafeTensors {
     return out;
   }
 
+  // The whole table on the device, a table of ops.embedRows: bf16 as it is, F32 / F16 and per-row
+  // int8 tables as the f32 values that rows() gives.
+  async table(gpu, name) {
+    const t = this.info(name), N = t.shape[0], K = t.shape[1], bf16 = t.dtype === "BF16";
+    const buf = gpu.empty([N, K], bf16 ? "bf16" : "f32"), step = 4096; // (rows in host memory at a time)
+    for (let i = 0; i < N; i += step) {
+      const n = Math.min(step, N - i), rows = await this.rows(name, Array.from({ length: n }, (_, j) => i + j));
+      if (!bf16) {
+        gpu.write(buf, rows, i * K * 4);
+        continue;
+      }
+      const bits = new Uint32Array(rows.buffer), half = new Uint16Array(n * K);
+      for (let j = 0; j < half.length; j++) half[j] = bits[j] >>> 16;
+      gpu.write(buf, half, i * K * 2);
+    }
+    return { kind: bf16 ? "bf16" : "f32", N, K, buf };
+  }
+
   linear(gpu, base) {
     const W = this.linearWeights(gpu, base);
     W.name = base.replace(/\.$/, "");
