@@ -42,11 +42,14 @@ const hasLora = (l) => LINEARS.some((k) => l[k] && l[k].lora && l[k].lora.length
 const isF8 = (l) => !!l.qkv && ["qkv", "o", "gate", "up", "down"].every((k) => l[k].kind === "f8") &&
   l.gate.K === l.up.K && l.gate.N === l.up.N && !hasLora(l);
 
-// the number of ids that all prompts begin with
+// The number of ids that all prompts begin with, or 0 where sharing them saves fewer than SHARE_ROWS rows: the
+// prefix costs two more calls a layer.  The 28 layers of 8 prompts with 77 shared ids and 40 of their own
+// (539 rows saved) take 4.6 ms shared and 5.4 apart, of 2 with 77 and 77 (77 rows) 4.1 and 3.6.
+const SHARE_ROWS = 256;
 function commonPrefix(prompts) {
   let n = 0;
-  while (prompts.length && n < prompts[0].length && prompts.every((p) => p[n] === prompts[0][n])) n++;
-  return n;
+  while (n < prompts[0].length && prompts.every((p) => p[n] === prompts[0][n])) n++;
+  return (prompts.length - 1) * n < SHARE_ROWS ? 0 : n;
 }
 
 export const QWEN3 = { layers: 28, hidden: 1024, heads: 16, kvHeads: 8, headDim: 128, mlp: 3072, theta: 1e6, vocab: 151936 };
@@ -267,8 +270,8 @@ export class Qwen3 {
   }
 
   // Several prompts (arrays of ids) at once -> one Tensor [length, D] each, as encode gives it.  The tokens that
-  // they all begin with (or opts.prefix of keepPrefix, which all have to begin with) pass the layers once, and the
-  // rest of all prompts in one pass behind them: every weight is read once for the whole batch.
+  // they all begin with, where they are enough (or opts.prefix of keepPrefix, which all have to begin with), pass
+  // the layers once, and the rest of all prompts in one pass behind them: every weight is read once for the batch.
   async encodeBatch(prompts, opts) {
     const gpu = this.gpu, D = this.cfg.hidden;
     const kept = (opts && opts.prefix) || null;

@@ -150,9 +150,11 @@ def test_batch_calls():
                "const trace = () => calls.splice(0).filter((c) => /^attention(Prefix)?$/.test(c[0])).map((c) => [c[0], c[2].Lq || Array.from(c[2].lens),"
                "  c[2].P || 0, c[2].prepareInto ? 1 : 0, c[2].ldq || 0, c[2].sinOff]);"
                "const out = {}, err = async (f) => { try { await f(); return ''; } catch (e) { return e.message; } };"
-               "const shapes = (await te.encodeBatch([[1, 2, 3, 4], [1, 2, 7], [1, 2]])).map((t) => t.shape); out.shapes = shapes; out.shared = trace();"
+               "const long = new Array(128).fill(5);"
+               "const shapes = (await te.encodeBatch([long.concat([3, 4]), long.concat([7]), long])).map((t) => t.shape); out.shapes = shapes; out.shared = trace();"
                "await te.encodeBatch([[1, 2], [3]]); out.none = trace();"
-               "await te.encodeBatch([[1, 2], [1, 2]]); out.same = trace();"
+               "await te.encodeBatch([[1, 2], [1, 2]]); out.few = trace();"
+               "await te.encodeBatch([long.concat(long), long.concat(long)]); out.same = trace();"
                "const prefix = await te.keepPrefix([1, 2]); out.keep = trace();"
                "await te.encodeBatch([[1, 2, 3], [1, 2, 4, 5]], { prefix }); out.kept = trace();"
                "await te.encodeBatch([[1, 2]], { prefix }); out.whole = trace();"
@@ -161,9 +163,9 @@ def test_batch_calls():
                "te.conversions++; out.e.push(await err(() => te.encodeBatch([[1, 2]], { prefix })));"
                "te.deviceTable = { kind: 'f32', N: 8, K: 256, buf: 1 }; out.e.push(await err(() => te.encodeBatch([[1, 8]])));"
                "console.log(JSON.stringify(out)); })")
-    assert got["shapes"] == [[4, 256], [3, 256], [2, 256]] and got["empty"] == 0
+    assert got["shapes"] == [[130, 256], [129, 256], [128, 256]] and got["empty"] == 0
 
-    def calls(n, P, lens, cs, own, keep=False):
+    def calls(n, P, lens, cs, keep=False):
         r = []
         for ld in (512, 256):
             if n:
@@ -174,11 +176,12 @@ def test_batch_calls():
                 r.append(["attentionPrefix", lens, P, 0, ld, cs * 64])
         return r
 
-    assert got["shared"] == calls(2, 2, [2, 1, 0], 4, 3)
-    assert got["none"] == calls(0, 0, [2, 1], 2, 3)
-    assert got["same"] == calls(2, 2, [], 2, 0)
-    assert got["keep"] == calls(2, 2, [], 2, 0, True)
-    assert got["kept"] == calls(0, 2, [1, 2], 4, 3)
+    assert got["shared"] == calls(128, 128, [2, 1, 0], 130)
+    assert got["none"] == calls(0, 0, [2, 1], 2)
+    assert got["few"] == calls(0, 0, [2, 2], 2)
+    assert got["same"] == calls(256, 256, [], 256)
+    assert got["keep"] == calls(2, 2, [], 2, True)
+    assert got["kept"] == calls(0, 2, [1, 2], 4)
     assert got["whole"] == []
     for e, w in zip(got["e"], ("prompt 1 has no tokens", "does not begin with opts.prefix", "no tokens", "other weights", "token id 8 outside")):
         assert w in e, got["e"]
@@ -255,7 +258,7 @@ def test_js_encode_batch(tmp_path, q4):
 
     V, L = 97, 2
     rng = np.random.default_rng(11)
-    head = [int(v) for v in rng.integers(0, V - 1, size=70)]
+    head = [int(v) for v in rng.integers(0, V - 1, size=90)]
     prompts = [head + [int(v) for v in rng.integers(0, V - 1, size=n)] for n in (9, 0, 130, 1)]
     out = str(tmp_path / "e")
     log = run_case(tmp_path, {"case": "encode", "layers": L, "vocab": V, "prompts": prompts, "keep": 66, "q4": q4, "out": out})
@@ -292,9 +295,9 @@ def test_js_encode_batch(tmp_path, q4):
                 got = get(f"{prec}.{name}.{i}").reshape(r.shape)
                 assert report(f"{prec} {name} {i}", got, r)[0] <= bar
         # the rows of the prefix are computed once
-        first = get(f"{prec}.batch.0").reshape(-1, D)[:70]
+        first = get(f"{prec}.batch.0").reshape(-1, D)[:90]
         for i in range(1, 4):
-            assert np.array_equal(first, get(f"{prec}.batch.{i}").reshape(-1, D)[:70])
+            assert np.array_equal(first, get(f"{prec}.batch.{i}").reshape(-1, D)[:90])
 
 
 @pytest.mark.gpu
