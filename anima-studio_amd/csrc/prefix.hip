@@ -5,7 +5,8 @@
 //
 // The sequences' rows are packed, so the prefix is one product for all of them: tiles of rows run over the prefix's key
 // blocks whatever sequence the rows belong to, then over the packed keys of their own sequences, masked by each row's
-// range of them.  The packed K (normed, rotated at P + place) and V are laid out as the prefix's are, in one pass.
+// range of them.  One pass before it norms and rotates q and the packed K (at P + place), and lays K and V out as the
+// prefix's are.
 #include <algorithm>
 #include <type_traits>
 
@@ -59,6 +60,8 @@ struct PrefixArgs {
   const void* pvt;  // lie a power of two apart, in one memory channel)
   void* ok;         // own: the same of Tp keys
   void* ovt;
+  void* pq;         // q [Hkv][V][128], ready to be multiplied: normed, rotated, times c
+  int2* range;      // [T] own keys that a row sees: from, to
   const float* qn;
   const float* kn;
   const float* cs;
@@ -79,47 +82,59 @@ __device__ __forceinline__ void p_barrier() {
   asm volatile("" ::: "memory");
 }
 
-// One workgroup per 64 packed rows and kv head; rows T .. Tp are zeros.  K: 16 lanes a row, lane q holding dims 4 q .. + 3 and
-// 64 + the same (both of each rotated pair); V: wave w takes dims 32 w .. + 31 of all rows, lane (q, c) the eight keys of V^T
-// chunk c at dims 4 q .. + 3, so that every load and store moves whole lines.  The bf16 form has K in f16 (its rounding
-// to 8 bits alone would be 0.004 of a result) and keeps each 16 keys of a V^T row as 0-3, 8-11, 4-7, 12-15, as the matrix
-// products take them.
+// One workgroup per 64 packed rows and kv head (then, with a.pq, per q head); rows T .. Tp are zeros.  K: 16 lanes a row, lane q
+// holding dims 4 q .. + 3 and 64 + the same (both of each rotated pair); V: wave w takes dims 32 w .. + 31 of all rows, lane
+// (q, c) the eight keys of V^T chunk c at dims 4 q .. + 3, so that every load and store moves whole lines.  The bf16 form has K
+// and q in f16 (their rounding to 8 bits alone would be 0.005 of a result) and keeps each 16 keys of a V^T row as 0-3, 8-11,
+// 4-7, 12-15, as the matrix products take them.
 // A key whose K or V is not finite (in its form) gets a K of NaN and a V of zeros: every row that sees it becomes NaN, and where it
 // is masked its weight of 0 meets no NaN in V.
 template <class T>
 __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a) {
   constexpr bool BF = sizeof(T) == 2;
+  typedef std::conditional_t<BF, _Float16, float> TK;
   __shared__ int bad[64];
   __shared__ SeqStarts seq;
-  const int t = threadIdx.x, w = t >> 6, lane = t & 63, kb0 = blockIdx.x * 64, hk = blockIdx.y;
+  const int t = threadIdx.x, w = t >> 6, lane = t & 63, kb0 = blockIdx.x * 64;
+  const bool query = (int)blockIdx.y >= a.Hkv;
+  const int hk = query ? blockIdx.y - a.Hkv : blockIdx.y;  // (its q head)
   const int q16 = lane & 15, rsub = lane >> 4, vq = lane & 7, vc = lane >> 3;
   const auto vkey = [&](int e) { return BF ? kb0 + 16 * (vc >> 1) + 4 * (vc & 1) + (e & 3) + 8 * (e >> 2) : kb0 + 8 * vc + e; };
   f32x4 klo[4], khi[4], ve[8], cv[4], sv[4], wl{}, wh{};
+  const float* const x = query ? a.q : a.k;
+  const int64_t ldx = query ? a.ldq : a.ldk;
+  const float* const norm = query ? a.qn : a.kn;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     const int l = min(kb0 + 16 * w + 4 * i + rsub, a.T - 1);
-    const float* src = a.k + (int64_t)l * a.ldk + hk * PHD + 4 * q16;
+    const float* src = x + (int64_t)l * ldx + hk * PHD + 4 * q16;
     klo[i] = *(const f32x4*)src;
     khi[i] = *(const f32x4*)(src + 64);
   }
+  if (!query) {
 #pragma unroll
-  for (int e = 0; e < 8; e++) ve[e] = *(const f32x4*)(a.v + (int64_t)min(vkey(e), a.T - 1) * a.ldv + hk * PHD + 32 * w + 4 * vq);
+    for (int e = 0; e < 8; e++) ve[e] = *(const f32x4*)(a.v + (int64_t)min(vkey(e), a.T - 1) * a.ldv + hk * PHD + 32 * w + 4 * vq);
+  }
+  if (norm) {
+    wl = *(const f32x4*)(norm + 4 * q16);
+    wh = *(const f32x4*)(norm + 64 + 4 * q16);
+  }
   if (t < 64) bad[t] = 0;
   seq.fill(a.seq);
   __builtin_amdgcn_s_waitcnt(0xc07f);  // (LDS alone: the loads above go on)
   p_barrier();
+  if (a.cs) {
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const int l = min(kb0 + 16 * w + 4 * i + rsub, a.T - 1);
-    if (a.cs) {
+    for (int i = 0; i < 4; i++) {
+      const int l = min(kb0 + 16 * w + 4 * i + rsub, a.T - 1);
       const float* cr = a.cs + (int64_t)(a.P + l - seq.at[seq.of(a.seq.n, l)]) * 64 + 4 * q16;
       cv[i] = *(const f32x4*)cr;
       sv[i] = *(const f32x4*)(cr + a.sin_off);
     }
   }
-  if (a.kn) {
-    wl = *(const f32x4*)(a.kn + 4 * q16);
-    wh = *(const f32x4*)(a.kn + 64 + 4 * q16);
+  if (a.range && blockIdx.y == 0 && t < 64 && kb0 + t < a.T) {
+    const int b = seq.of(a.seq.n, kb0 + t);
+    a.range[kb0 + t] = make_int2(seq.at[b], a.causal ? kb0 + t + 1 : seq.at[b + 1]);
   }
   const auto finite = [](f32x4 v, auto as) {
     float m = 0.0f;
@@ -127,11 +142,19 @@ __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a) {
     for (int j = 0; j < 4; j++) m += (float)(decltype(as))v[j] * 0.0f;  // (0 of finite values, else NaN)
     return m == 0.0f;
   };
-  typedef std::conditional_t<BF, _Float16, float> TK;
+  const auto put = [](TK* d, f32x4 lo, f32x4 hi) {
+    if constexpr (BF) {
+      *(f16x4*)d = f16x4{(_Float16)lo[0], (_Float16)lo[1], (_Float16)lo[2], (_Float16)lo[3]};
+      *(f16x4*)(d + 64) = f16x4{(_Float16)hi[0], (_Float16)hi[1], (_Float16)hi[2], (_Float16)hi[3]};
+    } else {
+      *(f32x4*)d = lo;
+      *(f32x4*)(d + 64) = hi;
+    }
+  };
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     f32x4 lo = klo[i], hi = khi[i];
-    if (a.kn) {
+    if (norm) {
       float ss = 0.0f;
 #pragma unroll
       for (int j = 0; j < 4; j++) ss += lo[j] * lo[j] + hi[j] * hi[j];
@@ -148,7 +171,15 @@ __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a) {
     }
     klo[i] = lo;
     khi[i] = hi;
-    if (!finite(lo, TK()) || !finite(hi, TK())) bad[16 * w + 4 * i + rsub] = 1;
+    if (!query && (!finite(lo, TK()) || !finite(hi, TK()))) bad[16 * w + 4 * i + rsub] = 1;
+  }
+  if (query) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int l = kb0 + 16 * w + 4 * i + rsub;
+      if (l < a.T) put((TK*)a.pq + ((int64_t)(hk / a.group) * a.V + (int64_t)l * a.group + hk % a.group) * PHD + 4 * q16, klo[i] * a.c, khi[i] * a.c);
+    }
+    return;
   }
 #pragma unroll
   for (int e = 0; e < 8; e++)
@@ -160,15 +191,7 @@ __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a) {
     const float k = __builtin_nanf("");
     const f32x4 z = l < a.T ? f32x4{k, k, k, k} : f32x4{};
     const bool keep = l < a.T && !bad[r];
-    const f32x4 lo = keep ? klo[i] : z, hi = keep ? khi[i] : z;
-    TK* d = (TK*)a.ok + ((int64_t)hk * a.Tp + l) * PHD + 4 * q16;
-    if constexpr (BF) {
-      *(f16x4*)d = f16x4{(_Float16)lo[0], (_Float16)lo[1], (_Float16)lo[2], (_Float16)lo[3]};
-      *(f16x4*)(d + 64) = f16x4{(_Float16)hi[0], (_Float16)hi[1], (_Float16)hi[2], (_Float16)hi[3]};
-    } else {
-      *(f32x4*)d = lo;
-      *(f32x4*)(d + 64) = hi;
-    }
+    put((TK*)a.ok + ((int64_t)hk * a.Tp + l) * PHD + 4 * q16, keep ? klo[i] : z, keep ? khi[i] : z);
   }
 #pragma unroll
   for (int e = 0; e < 8; e++)
@@ -234,10 +257,9 @@ __device__ __forceinline__ int p_same(int x) { return __builtin_amdgcn_readfirst
 // prefix's last, then own ones from ob0 up to of0 and from of1 up to ob1).
 struct PrefixBlocks {
   int nP, of0, full, tail, ob0, cut0, of1, total;
-  __device__ __forceinline__ PrefixBlocks(const PrefixArgs& a, const SeqStarts& seq, int row0, int row1) {  // rows row0 .. row1
-    const int b0 = p_same(seq.of(a.seq.n, row0)), b1 = p_same(seq.of(a.seq.n, row1)), s0 = p_same(seq.at[b0]);
-    const int end = a.causal ? row1 + 1 : p_same(seq.at[b1 + 1]);
-    const int hi = b0 != b1 ? 0 : a.causal ? row0 + 1 : end;  // keys s0 .. hi are seen by all
+  __device__ __forceinline__ PrefixBlocks(const PrefixArgs& a, int row0, int row1) {  // rows row0 .. row1
+    const int2 r0 = a.range[row0], r1 = a.range[row1];
+    const int s0 = p_same(r0.x), end = p_same(r1.y), hi = p_same(r0.x == r1.x ? r0.y : 0);  // own keys s0 .. end, s0 .. hi of them seen by all
     nP = a.P / PBK;
     tail = a.P % PBK ? 1 : 0;
     ob0 = s0 / PBK;
@@ -263,63 +285,26 @@ struct PrefixBlocks {
   }
 };
 
-// A row's lane part: dims 16 ks + 8 hf + j in x[8 ks + j] (NK of the eight ks).
-template <int NK>
-__device__ __forceinline__ void p_load(const float* src, int hf, float (&x)[8 * NK]) {
-#pragma unroll
-  for (int ks = 0; ks < NK; ks++)
-#pragma unroll
-    for (int q = 0; q < 2; q++) {
-      const f32x4 w = *(const f32x4*)(src + 16 * ks + 8 * hf + 4 * q);
-#pragma unroll
-      for (int j = 0; j < 4; j++) x[8 * ks + 4 * q + j] = w[j];
-    }
-}
-
-// The row's RMS norm (qw: its weights) and rotation (cs, sn), x, qw, cs and sn as p_load leaves them.
-__device__ __forceinline__ void p_norm_rope(const PrefixArgs& a, const float (&qw)[64], const float (&cs)[32], const float (&sn)[32],
-                                            float (&x)[64]) {
-  if (a.qn) {
-    float ss = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 64; i++) ss = __builtin_fmaf(x[i], x[i], ss);
-    const float f = 1.0f / sqrtf(p_pair_sum(ss) / 128.0f + a.eps);
-#pragma unroll
-    for (int i = 0; i < 64; i++) x[i] = x[i] * f * qw[i];
-  }
-  if (a.cs) {
-#pragma unroll
-    for (int i = 0; i < 32; i++) {
-      const float x1 = x[i], x2 = x[32 + i];
-      x[i] = x1 * cs[i] - x2 * sn[i];
-      x[32 + i] = x2 * cs[i] + x1 * sn[i];
-    }
-  }
-}
-
 template <int NW>
 __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_bf16(PrefixArgs a) {
   constexpr int CPW = 16 / NW;  // copies of K, and of V^T, a wave and block
   // (one LDS object: beside a second one the compiler has every read of the stages wait for all copies in flight)
-  __shared__ __attribute__((aligned(1024))) char smem[PNST * PST + sizeof(SeqStarts)];
-  SeqStarts& seq = *(SeqStarts*)(smem + PNST * PST);
+  __shared__ __attribute__((aligned(1024))) char smem[PNST * PST];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 31, hf = lane >> 5;
   // tiles of a head and split follow each other (on one XCD: they read the same blocks)
   const int id = xcd_remap(blockIdx.x, gridDim.x), hs = p_same(id / a.nt), tile = id - hs * a.nt, hk = p_same(hs / a.splits),
             sp = hs - hk * a.splits;
-  const int v0 = tile * 32 * NW, v = v0 + 32 * wave + r;
-  // the lane's row, asked for before anything that takes a search (the barrier waits for LDS alone)
-  const int vc = min(v, a.V - 1), row = vc / a.group, h = hk * a.group + vc - row * a.group;
-  float x[64], qw[64];
-  p_load<8>(a.q + (int64_t)row * a.ldq + h * PHD, hf, x);
-  if (a.qn) p_load<8>(a.qn, hf, qw);
-  seq.fill(a.seq);
-  __builtin_amdgcn_s_waitcnt(0xc07f);
-  p_barrier();
-  const PrefixBlocks B(a, seq, p_same(v0 / a.group), p_same((min(v0 + 32 * NW, a.V) - 1) / a.group));
+  const int v0 = tile * 32 * NW, v = v0 + 32 * wave + r, vc = min(v, a.V - 1);
+  f16x8 qf[8];
+#pragma unroll
+  for (int ks = 0; ks < 8; ks++) qf[ks] = *(const f16x8*)((const _Float16*)a.pq + ((int64_t)hk * a.V + vc) * PHD + 16 * ks + 8 * hf);
+  const int2 range = a.range[vc / a.group];
+  const PrefixBlocks B(a, p_same(v0 / a.group), p_same((min(v0 + 32 * NW, a.V) - 1) / a.group));
   const int each = p_same(B.total / a.splits), more = B.total - each * a.splits;  // (blocks of a part: each, and one more of the first)
   const int i0 = sp * each + min(sp, more), nb = each + (sp < more ? 1 : 0), i1 = i0 + nb;
-  const bool live = v0 + 32 * wave < a.V;  // the wave has rows
+  // own keys that a row of the wave sees (its rows ascend; none without rows)
+  const int wlo = __builtin_amdgcn_readfirstlane(range.x), whi = __builtin_amdgcn_readlane(range.y, 31);
+  const bool live = v0 + 32 * wave < a.V;
 
   const int64_t pb = (int64_t)a.Pp * PHD * 2, ob = (int64_t)a.Tp * PHD * 2;
   const __amdgpu_buffer_rsrc_t rpk = p_rsrc((const char*)a.pk + hk * pb, a.P ? pb : 0), rpv = p_rsrc((const char*)a.pvt + hk * pb, a.P ? pb : 0),
@@ -331,36 +316,20 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_bf16(PrefixArgs 
     ko[c] = row * 256 + 16 * ((lane & 15) ^ (row & 15));
     vo[c] = d * 128 + 16 * ((lane & 7) ^ ((d >> 1) & 7));
   }
-  const auto load = [&](int j) __attribute__((always_inline)) {  // block j of the part (past the last: that one again, unused)
+  const auto load = [&](int j) __attribute__((always_inline)) {  // block j of the part, if there is one
+    if (j >= nb) return;
     bool pre;
-    const int blk = B.at(i0 + min(j, nb - 1), pre);
+    const int blk = B.at(i0 + j, pre);
     char* st = smem + (j & 3) * PST;
 #pragma unroll
     for (int c = 0; c < CPW; c++) p_copy16(pre ? rpk : rok, st + (wave * CPW + c) * 1024, ko[c], blk * (64 * 256));
 #pragma unroll
     for (int c = 0; c < CPW; c++) p_copy16(pre ? rpv : rov, st + PKT + (wave * CPW + c) * 1024, vo[c], blk * (64 * 256));
   };
-  if (nb > 0) {
-    load(0);
-    load(1);
-    load(2);
-  }
+  load(0);
+  load(1);
+  load(2);
 
-  const int sq = seq.of(a.seq.n, row), klo = seq.at[sq], khi = a.causal ? row + 1 : seq.at[sq + 1];
-  float cs[32], sn[32];
-  if (a.cs) {
-    const float* cr = a.cs + (int64_t)(a.P + row - klo) * 64;
-    p_load<4>(cr, hf, cs);
-    p_load<4>(cr + a.sin_off, hf, sn);
-  }
-  p_norm_rope(a, qw, cs, sn, x);
-  f16x8 qf[8];
-  {
-#pragma unroll
-    for (int ks = 0; ks < 8; ks++)
-#pragma unroll
-      for (int j = 0; j < 8; j++) qf[ks][j] = (_Float16)(x[8 * ks + j] * a.c);
-  }
   f32x16 o[4];
 #pragma unroll
   for (int i = 0; i < 4; i++) o[i] = f32x16{};
@@ -491,7 +460,8 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_bf16(PrefixArgs 
   // may pend); behind the barrier everyone's have, so that its first fragments are read under block j's last products, and the
   // stage of block j - 1 is refilled.
   const auto turn = [&](int j) __attribute__((always_inline)) {
-    P_WAIT_VM(2 * CPW);
+    if (j + 2 < nb) P_WAIT_VM(2 * CPW);
+    else P_WAIT_VM(0);
     p_barrier();
     load(j + 3);
     return (const char*)smem + (j & 3) * PST;
@@ -516,10 +486,10 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_bf16(PrefixArgs 
     const char* st = turn(j);
     bool pre;
     const int blk = B.at(i0 + j, pre);
-    if (live) block(st, std::true_type{}, blk * PBK, pre ? 0 : klo, pre ? a.P : khi);
+    if (live && (pre || (blk * PBK < whi && blk * PBK + PBK > wlo)))
+      block(st, std::true_type{}, blk * PBK, pre ? 0 : range.x, pre ? a.P : range.y);
   }
-  P_WAIT_VM(0);  // no copy into LDS outlives the loop
-  p_barrier();
+  p_barrier();  // (the stages become the rows')
 
   // Rows leave through LDS in halves of 64 columns, so that every store writes 256 bytes of a row.
   l = p_pair_sum(l);
@@ -566,45 +536,25 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_bf16(PrefixArgs 
 constexpr int PKS = PHD + 4, PVS = 64 + 4;  // floats between rows of K and of V^T in LDS
 
 __global__ __launch_bounds__(256, 2) void prefix_flash_fp32(PrefixArgs a) {
-  __shared__ __attribute__((aligned(16))) float smem[64 * PKS + PHD * PVS + sizeof(SeqStarts) / 4];
-  float* const Ks = smem;
-  float* const Vs = smem + 64 * PKS;
-  SeqStarts& seq = *(SeqStarts*)(smem + 64 * PKS + PHD * PVS);
+  __shared__ __attribute__((aligned(16))) float Ks[64 * PKS], Vs[PHD * PVS];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 31, hf = lane >> 5;
   const int id = xcd_remap(blockIdx.x, gridDim.x), hs = p_same(id / a.nt), tile = id - hs * a.nt, hk = p_same(hs / a.splits),
             sp = hs - hk * a.splits;
   const int v0 = tile * 128, v = v0 + 32 * wave + r;
   const int vc = min(v, a.V - 1), row = vc / a.group, h = hk * a.group + vc - row * a.group;
-  seq.fill(a.seq);
-  __syncthreads();
-  const PrefixBlocks B(a, seq, p_same(v0 / a.group), p_same((min(v0 + 128, a.V) - 1) / a.group));
-  const int each = p_same(B.total / a.splits), more = B.total - each * a.splits;
-  const int i0 = sp * each + min(sp, more), nb = each + (sp < more ? 1 : 0);
-  const int sq = seq.of(a.seq.n, row), klo = seq.at[sq], khi = a.causal ? row + 1 : seq.at[sq + 1];
-
   // k-step 4 g + e of the scores: dim 8 g + e in lane half 0, 8 g + 4 + e in half 1, so that a lane reads its K values
   // four steps at a time; lane keeps q's dim 8 g + 4 hf + e as qv[4 g + e]
   float qv[64];
-  {
-    float x[64], qw[64], cs[32], sn[32];
-    p_load<8>(a.q + (int64_t)row * a.ldq + h * PHD, hf, x);
-    if (a.qn) p_load<8>(a.qn, hf, qw);
-    if (a.cs) {
-      const float* cr = a.cs + (int64_t)(a.P + row - klo) * 64;
-      p_load<4>(cr, hf, cs);
-      p_load<4>(cr + a.sin_off, hf, sn);
-    }
-    p_norm_rope(a, qw, cs, sn, x);
 #pragma unroll
-    for (int k8 = 0; k8 < 8; k8++)
+  for (int g = 0; g < 16; g++) {
+    const f32x4 x = *(const f32x4*)((const float*)a.pq + ((int64_t)hk * a.V + vc) * PHD + 8 * g + 4 * hf);
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const float lo = x[8 * k8 + e] * a.c, hi = x[8 * k8 + 4 + e] * a.c;
-        const float other = __shfl_xor(hf ? lo : hi, 32);  // half 0's dim 16 k8 + 4 + e, half 1's 16 k8 + 8 + e
-        qv[8 * k8 + e] = hf ? other : lo;
-        qv[8 * k8 + 4 + e] = hf ? hi : other;
-      }
+    for (int e = 0; e < 4; e++) qv[4 * g + e] = x[e];
   }
+  const int2 range = a.range[row];
+  const PrefixBlocks B(a, p_same(v0 / a.group), p_same((min(v0 + 128, a.V) - 1) / a.group));
+  const int each = p_same(B.total / a.splits), more = B.total - each * a.splits;
+  const int i0 = sp * each + min(sp, more), nb = each + (sp < more ? 1 : 0);
   f32x16 o[4];
 #pragma unroll
   for (int i = 0; i < 4; i++) o[i] = f32x16{};
@@ -643,7 +593,7 @@ __global__ __launch_bounds__(256, 2) void prefix_flash_fp32(PrefixArgs a) {
       }
     }
     if (i0 + j >= B.full) {
-      const int lo = pre ? 0 : klo, hi = pre ? a.P : khi;
+      const int lo = pre ? 0 : range.x, hi = pre ? a.P : range.y;
 #pragma unroll
       for (int e = 0; e < 16; e++) {
         const int k = blk * 64 + 8 * (e >> 2) + 4 * hf + (e & 3);
@@ -741,8 +691,8 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixArgs a) {
 
 template <class T>
 static int prefix_prep_launch(anima_ctx* c, const PrefixArgs& a) {
-  Launch L(c, sizeof(T) == 2 ? "attn.prefix_prep_bf16" : "attn.prefix_prep_fp32", 0.0, (double)a.Hkv * a.T * PHD * (8.0 + 2 * sizeof(T)));
-  hipLaunchKernelGGL(prefix_prep_kernel<T>, dim3((unsigned)(a.Tp / 64), (unsigned)a.Hkv), dim3(256), 0, c->stream, a);
+  Launch L(c, sizeof(T) == 2 ? "attn.prefix_prep_bf16" : "attn.prefix_prep_fp32", 0.0, (double)a.T * PHD * (a.Hkv * (8.0 + 2 * sizeof(T)) + (a.pq ? a.H * (4.0 + sizeof(T)) : 0.0)));
+  hipLaunchKernelGGL(prefix_prep_kernel<T>, dim3((unsigned)(a.Tp / 64), (unsigned)(a.Hkv + (a.pq ? a.H : 0))), dim3(256), 0, c->stream, a);
   return L.end();
 }
 
@@ -756,13 +706,16 @@ static int prefix_part(anima_ctx* c, PrefixArgs& a) {
   const int rows = eight ? 256 : 128, fill = BF ? c->num_cus : 2 * c->num_cus;  // (two fp32 workgroups to a CU)
   a.nt = (a.V + rows - 1) / rows;
   a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({fill / ((int64_t)a.nt * a.Hkv), blocks / 2, 64}));
-  const size_t plane = (size_t)a.Hkv * a.Tp * PHD * sizeof(T), n = a.splits > 1 ? (size_t)a.splits * a.Hkv * a.V : 0;
+  const size_t plane = (size_t)a.Hkv * a.Tp * PHD * sizeof(T), q = (size_t)a.Hkv * a.V * PHD * sizeof(T),
+               n = a.splits > 1 ? (size_t)a.splits * a.Hkv * a.V : 0;
   void* ws = nullptr;
-  if (int rc = workspace(c, 2 * plane + n * (PHD + 2) * 4, &ws)) return rc;
+  if (int rc = workspace(c, 2 * plane + q + n * (PHD + 2) * 4 + (size_t)a.T * 8, &ws)) return rc;
   a.ok = ws;
   a.ovt = (char*)ws + plane;
-  a.po = (float*)((char*)ws + 2 * plane);
+  a.pq = (char*)ws + 2 * plane;
+  a.po = (float*)((char*)a.pq + q);
   a.pml = a.po + n * PHD;
+  a.range = (int2*)(a.pml + 2 * n);
   if (int rc = prefix_prep_launch<T>(c, a)) return rc;
   Launch L(c, BF ? "attn.prefix_bf16" : "attn.prefix_fp32", 4.0 * a.T * a.H * PHD * a.P, 0.0);
   const dim3 grid((unsigned)((int64_t)a.nt * a.Hkv * a.splits));
