@@ -285,6 +285,47 @@ struct PrefixBlocks {
   }
 };
 
+// A wave's rows v0 ... (o of lane (r, hf) is row r's, register 4 g + e of o[i] its dim 32 i + 8 g + 4 hf + e; m, l: exponent and
+// this lane's sum of the weights), divided, or as a part of a split call.  They leave through LDS in halves of 64 columns, so that
+// every store writes 256 bytes of a row.
+__device__ __forceinline__ void p_leave(const PrefixArgs& a, char* smem, int sp, int hk, int v0, int wave, int lane, f32x16 (&o)[4], float m, float l) {
+  const int r = lane & 31, hf = lane >> 5, v = v0 + r;
+  l = p_pair_sum(l);
+  const bool part = a.splits > 1;
+  const float inv = part ? 1.0f : 1.0f / l;
+  const int64_t plane = ((int64_t)sp * a.Hkv + hk) * a.V;
+  if (part && v < a.V && hf == 0) *(float2*)(a.pml + (plane + v) * 2) = make_float2(m, l);
+  constexpr int RS = 64 + 4;
+  float* ow = (float*)smem + wave * 32 * RS;
+  const int rr = lane >> 4, cc = 4 * (lane & 15);
+#pragma unroll
+  for (int half = 0; half < 2; half++) {
+#pragma unroll
+    for (int d2 = 0; d2 < 2; d2++)
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const f32x16& w = o[2 * half + d2];
+        *(f32x4*)(ow + r * RS + 32 * d2 + 8 * g + 4 * hf) = f32x4{w[4 * g] * inv, w[4 * g + 1] * inv, w[4 * g + 2] * inv, w[4 * g + 3] * inv};
+      }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const int q = 4 * k + rr, vo = v0 + q;
+      const f32x4 w = *(const f32x4*)(ow + q * RS + cc);
+      if (vo < a.V) {
+        if (part) {
+          *(f32x4*)(a.po + (plane + vo) * PHD + 64 * half + cc) = w;
+        } else {
+          const int64_t ro = vo / a.group, off = ro * a.ldo + (hk * a.group + vo - ro * a.group) * PHD + 64 * half + cc;
+          if (a.obf) *(bf16x4*)((bf16*)a.o + off) = bf16x4{to_bf16(w[0]), to_bf16(w[1]), to_bf16(w[2]), to_bf16(w[3])};
+          else *(f32x4*)((float*)a.o + off) = w;
+        }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
 template <int NW>
 __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_bf16(PrefixArgs a) {
   constexpr int CPW = 16 / NW;  // copies of K, and of V^T, a wave and block
@@ -491,119 +532,167 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_bf16(PrefixArgs 
   }
   p_barrier();  // (the stages become the rows')
 
-  // Rows leave through LDS in halves of 64 columns, so that every store writes 256 bytes of a row.
-  l = p_pair_sum(l);
-  const bool part = a.splits > 1;
-  const float inv = part ? 1.0f : 1.0f / l;
-  const int64_t plane = ((int64_t)sp * a.Hkv + hk) * a.V;
-  if (part && v < a.V && hf == 0) *(float2*)(a.pml + (plane + v) * 2) = make_float2(m, l);
-  constexpr int RS = 64 + 4;
-  float* ow = (float*)smem + wave * 32 * RS;
-  const int rr = lane >> 4, cc = 4 * (lane & 15);
-#pragma unroll
-  for (int half = 0; half < 2; half++) {
-#pragma unroll
-    for (int d2 = 0; d2 < 2; d2++)
-#pragma unroll
-      for (int g = 0; g < 4; g++) {
-        const f32x16& w = o[2 * half + d2];
-        *(f32x4*)(ow + r * RS + 32 * d2 + 8 * g + 4 * hf) = f32x4{w[4 * g] * inv, w[4 * g + 1] * inv, w[4 * g + 2] * inv, w[4 * g + 3] * inv};
-      }
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int k = 0; k < 8; k++) {
-      const int q = 4 * k + rr, vo = v0 + 32 * wave + q;
-      const f32x4 w = *(const f32x4*)(ow + q * RS + cc);
-      if (vo < a.V) {
-        if (part) {
-          *(f32x4*)(a.po + (plane + vo) * PHD + 64 * half + cc) = w;
-        } else {
-          const int64_t ro = vo / a.group, off = ro * a.ldo + (hk * a.group + vo - ro * a.group) * PHD + 64 * half + cc;
-          if (a.obf) *(bf16x4*)((bf16*)a.o + off) = bf16x4{to_bf16(w[0]), to_bf16(w[1]), to_bf16(w[2]), to_bf16(w[3])};
-          else *(f32x4*)((float*)a.o + off) = w;
-        }
-      }
-    }
-    __builtin_amdgcn_wave_barrier();
-  }
+  p_leave(a, smem, sp, hk, v0 + 32 * wave, wave, lane, o, m, l);
 }
 
 // ------------------------------------------------------------------ fp32 tiles
 //
-// The same parts on the fp32 matrix cores (64 cycles an instruction, which bound it): 128 virtual rows a workgroup, two
-// workgroups a CU, which cover each other's loads.  p = 2^(s - m) with m raised where a block's maximum passes it by more than 8.
-// A block's products of V are added by themselves first: chains of one step a block across blocks.
-constexpr int PKS = PHD + 4, PVS = 64 + 4;  // floats between rows of K and of V^T in LDS
+// The same parts in fp32 precision.  A value is three bf16 ones, x = x1 + x2 + x3 exactly (8 bits each, cut off and not rounded), and
+// a product six on the bf16 matrix cores, x1 y1 + x1 y2 + x2 y1 + x2 y2 + x1 y3 + x3 y1, without what is below 2^-22 of it: five
+// times the rate of the fp32 matrix cores.
+// A step is 32 keys.  They come as fp32 by buffer_load ... lds into one of two stages, a step ahead are cut into their planes (once
+// for all waves, under the products of the step before), and a step later are multiplied: one barrier a step.
+// p = 2^(s - m) with m raised where a step's maximum passes it by more than 8.  A step's products of V are added by themselves first:
+// chains of one step a sum across steps.
+constexpr int FRAW = 2 * 32 * PHD * 4;   // bytes of a step's K, then V^T, as they come
+constexpr int FPL = 32 * PHD * 2;        // of one plane of its K or V^T
+constexpr int FST = 6 * FPL;             // of its planes: three of K, three of V^T
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-__global__ __launch_bounds__(256, 2) void prefix_flash_fp32(PrefixArgs a) {
-  __shared__ __attribute__((aligned(16))) float Ks[64 * PKS], Vs[PHD * PVS];
+// Two values' terms, packed: bf16 is the upper half of an fp32.
+__device__ __forceinline__ void p_terms(float x, float y, uint32_t (&t)[3]) {
+#pragma unroll
+  for (int i = 0; i < 3; i++) {
+    const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+    t[i] = __builtin_amdgcn_perm(b, a, 0x07060302);
+    x -= __uint_as_float(a & 0xffff0000u);
+    y -= __uint_as_float(b & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void p_terms8(const float* x, bf16x8 (&t)[3]) {
+  uint32_t w[4][3];
+#pragma unroll
+  for (int i = 0; i < 4; i++) p_terms(x[2 * i], x[2 * i + 1], w[i]);
+#pragma unroll
+  for (int c = 0; c < 3; c++) t[c] = __builtin_bit_cast(bf16x8, u32x4{w[0][c], w[1][c], w[2][c], w[3][c]});
+}
+// c + x y of six terms, the smallest first
+__device__ __forceinline__ f32x16 p_mfma6(const bf16x8 (&x)[3], const bf16x8 (&y)[3], f32x16 c) {
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[2], y[0], c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], y[2], c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[1], y[1], c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[1], y[0], c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], y[1], c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], y[0], c, 0, 0, 0);
+}
+
+template <int NW>
+__global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_fp32(PrefixArgs a) {
+  constexpr int CP = 16 / NW;  // pieces of 16 bytes of a step's K, and of its V^T, a thread
+  __shared__ __attribute__((aligned(1024))) char smem[2 * FRAW + 2 * FST];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 31, hf = lane >> 5;
   const int id = xcd_remap(blockIdx.x, gridDim.x), hs = p_same(id / a.nt), tile = id - hs * a.nt, hk = p_same(hs / a.splits),
             sp = hs - hk * a.splits;
-  const int v0 = tile * 128, v = v0 + 32 * wave + r;
-  const int vc = min(v, a.V - 1), row = vc / a.group, h = hk * a.group + vc - row * a.group;
-  // k-step 4 g + e of the scores: dim 8 g + e in lane half 0, 8 g + 4 + e in half 1, so that a lane reads its K values
-  // four steps at a time; lane keeps q's dim 8 g + 4 hf + e as qv[4 g + e]
-  float qv[64];
+  const int v0 = tile * 32 * NW, v = v0 + 32 * wave + r, vc = min(v, a.V - 1);
+  float x[64];
 #pragma unroll
   for (int g = 0; g < 16; g++) {
-    const f32x4 x = *(const f32x4*)((const float*)a.pq + ((int64_t)hk * a.V + vc) * PHD + 8 * g + 4 * hf);
+    const f32x4 w = *(const f32x4*)((const float*)a.pq + ((int64_t)hk * a.V + vc) * PHD + 16 * (g >> 1) + 8 * hf + 4 * (g & 1));
 #pragma unroll
-    for (int e = 0; e < 4; e++) qv[4 * g + e] = x[e];
+    for (int e = 0; e < 4; e++) x[4 * g + e] = w[e];
   }
-  const int2 range = a.range[row];
-  const PrefixBlocks B(a, p_same(v0 / a.group), p_same((min(v0 + 128, a.V) - 1) / a.group));
+  const int2 range = a.range[vc / a.group];
+  const PrefixBlocks B(a, p_same(v0 / a.group), p_same((min(v0 + 32 * NW, a.V) - 1) / a.group));
   const int each = p_same(B.total / a.splits), more = B.total - each * a.splits;
-  const int i0 = sp * each + min(sp, more), nb = each + (sp < more ? 1 : 0);
+  const int i0 = sp * each + min(sp, more), ns = 2 * (each + (sp < more ? 1 : 0));  // steps: halves of blocks
+  const int wlo = __builtin_amdgcn_readfirstlane(range.x), whi = __builtin_amdgcn_readlane(range.y, 31);
+  const bool live = v0 + 32 * wave < a.V;
+
+  const int64_t pb = (int64_t)a.Pp * PHD * 4, ob = (int64_t)a.Tp * PHD * 4;
+  const __amdgpu_buffer_rsrc_t rpk = p_rsrc((const char*)a.pk + hk * pb, a.P ? pb : 0), rpv = p_rsrc((const char*)a.pvt + hk * pb, a.P ? pb : 0),
+                               rok = p_rsrc((const char*)a.ok + hk * ob, ob), rov = p_rsrc((const char*)a.ovt + hk * ob, ob);
+  // piece u = 64 (wave CP + c) + lane: K row u / 32, V^T row u / 8 (its 32 keys are 128 bytes of 256)
+  uint32_t vo[CP];
+#pragma unroll
+  for (int c = 0; c < CP; c++) {
+    const int u = 64 * (wave * CP + c) + lane;
+    vo[c] = (u >> 3) * 256 + (u & 7) * 16;
+  }
+  const auto load = [&](int j) __attribute__((always_inline)) {  // step j of the part, if there is one
+    if (j >= ns) return;
+    bool pre;
+    const uint32_t blk = B.at(i0 + (j >> 1), pre), half = j & 1;
+    char* st = smem + half * FRAW;
+#pragma unroll
+    for (int c = 0; c < CP; c++) p_copy16(pre ? rpk : rok, st + (wave * CP + c) * 1024, lane * 16, blk * 32768 + half * 16384 + (wave * CP + c) * 1024);
+#pragma unroll
+    for (int c = 0; c < CP; c++) p_copy16(pre ? rpv : rov, st + FRAW / 2 + (wave * CP + c) * 1024, vo[c], blk * 32768 + half * 128);
+  };
+  // this thread's own pieces of step j (those of its own wave's copies) into planes
+  const auto cut = [&](int j) __attribute__((always_inline)) {
+    const char* st = smem + (j & 1) * FRAW;
+    char* pl = smem + 2 * FRAW + (j & 1) * FST;
+#pragma unroll
+    for (int c = 0; c < 2 * CP; c++) {
+      const bool key = c < CP;
+      const int u = 64 * (wave * CP + (key ? c : c - CP)) + lane;
+      const f32x4 w = *(const f32x4*)(st + (key ? 0 : FRAW / 2) + u * 16);
+      uint32_t t0[3], t1[3];
+      p_terms(w[0], w[1], t0);
+      p_terms(w[2], w[3], t1);
+      // K: dims 4 (u % 32) .. of row u / 32.  V^T: keys 4 q .. of row u / 8, each 16 of them kept as 0-3, 8-11, 4-7, 12-15
+      const int row = key ? u >> 5 : u >> 3, q = key ? u & 31 : u & 7;
+      const int at = key ? row * 256 + 16 * ((q >> 1) ^ (row & 15)) + 8 * (q & 1)
+                         : 3 * FPL + row * 64 + 16 * ((2 * (q >> 2) + (q & 1)) ^ ((row >> 1) & 3)) + 8 * ((q >> 1) & 1);
+#pragma unroll
+      for (int p = 0; p < 3; p++) *(u32x2*)(pl + at + p * FPL) = u32x2{t0[p], t1[p]};
+    }
+  };
+  load(0);
+  load(1);
+  bf16x8 qf[8][3];
+#pragma unroll
+  for (int ks = 0; ks < 8; ks++) p_terms8(x + 8 * ks, qf[ks]);
   f32x16 o[4];
 #pragma unroll
   for (int i = 0; i < 4; i++) o[i] = f32x16{};
   float m = M_NONE, l = 0.0f;
-  for (int j = 0; j < nb; j++) {
+  int kof[8], vof[2];
+#pragma unroll
+  for (int ks = 0; ks < 8; ks++) kof[ks] = r * 256 + 16 * ((2 * ks + hf) ^ (r & 15));
+#pragma unroll
+  for (int u = 0; u < 2; u++) vof[u] = 3 * FPL + r * 64 + 16 * ((2 * u + hf) ^ ((r >> 1) & 3));
+  if (ns > 0) {
+    if (ns > 1) P_WAIT_VM(2 * CP);
+    else P_WAIT_VM(0);
+    cut(0);
+  }
+  for (int j = 0; j < ns; j++) {
+    // This wave's copies of step j + 1 have arrived and its planes of step j are written; behind the barrier everyone's are, and the
+    // planes of step j - 1 and this wave's copies of step j are done with.
+    P_WAIT_VM(0);
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    p_barrier();
+    load(j + 2);
     bool pre;
-    const int blk = B.at(i0 + j, pre), ld = pre ? a.Pp : a.Tp;
-    const float* kg = (const float*)(pre ? a.pk : a.ok) + ((int64_t)hk * ld + blk * 64) * PHD;
-    const float* vg = (const float*)(pre ? a.pvt : a.ovt) + ((int64_t)hk * ld + blk * 64) * PHD;
-    // K tile 64 x 128 floats, V^T tile 128 x 64: eight pieces of 4 floats of each per thread, consecutive threads
-    // consecutive pieces
-    f32x4 kr[8], vr[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const int u = 256 * i + tid;
-      kr[i] = *(const f32x4*)(kg + 4 * u);
-      vr[i] = *(const f32x4*)(vg + 4 * u);
+    const int blk = B.at(i0 + (j >> 1), pre), k0 = blk * PBK + 32 * (j & 1);
+    const bool cutting = j + 1 < ns;
+    if (!live || (i0 + (j >> 1) >= B.full && !pre && (k0 >= whi || k0 + 32 <= wlo))) {
+      if (cutting) cut(j + 1);
+      continue;
     }
-    if (j) __syncthreads();  // every wave is done with the previous block's tiles
+    const char* st = smem + 2 * FRAW + (j & 1) * FST;
+    f32x16 s = {};
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const int u = 256 * i + tid;
-      *(f32x4*)(Ks + (u >> 5) * PKS + 4 * (u & 31)) = kr[i];
-      *(f32x4*)(Vs + (u >> 4) * PVS + 4 * (u & 15)) = vr[i];
+    for (int ks = 0; ks < 8; ks++) {
+      bf16x8 kf[3];
+#pragma unroll
+      for (int p = 0; p < 3; p++) kf[p] = *(const bf16x8*)(st + kof[ks] + p * FPL);
+      s = p_mfma6(kf, qf[ks], s);
     }
-    __syncthreads();
-    f32x16 s0 = {}, s1 = {};
-    const float* kp = Ks + r * PKS + 4 * hf;
-#pragma unroll
-    for (int g = 0; g < 16; g++) {
-      const f32x4 k0 = *(const f32x4*)(kp + 8 * g), k1 = *(const f32x4*)(kp + 32 * PKS + 8 * g);
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        s0 = __builtin_amdgcn_mfma_f32_32x32x2f32(k0[e], qv[4 * g + e], s0, 0, 0, 0);
-        s1 = __builtin_amdgcn_mfma_f32_32x32x2f32(k1[e], qv[4 * g + e], s1, 0, 0, 0);
-      }
-    }
-    if (i0 + j >= B.full) {
+    if (cutting) cut(j + 1);
+    if (i0 + (j >> 1) >= B.full) {
       const int lo = pre ? 0 : range.x, hi = pre ? a.P : range.y;
 #pragma unroll
       for (int e = 0; e < 16; e++) {
-        const int k = blk * 64 + 8 * (e >> 2) + 4 * hf + (e & 3);
-        if (k < lo || k >= hi) s0[e] = -INFINITY;
-        if (k + 32 < lo || k + 32 >= hi) s1[e] = -INFINITY;
+        const int k = k0 + 8 * (e >> 2) + 4 * hf + (e & 3);
+        if (k < lo || k >= hi) s[e] = -INFINITY;
       }
     }
-    float bm = fmaxf(s0[0], s1[0]);
+    float bm = s[0];
 #pragma unroll
-    for (int e = 1; e < 16; e++) bm = fmaxf(bm, fmaxf(s0[e], s1[e]));
+    for (int e = 1; e < 16; e++) bm = fmaxf(bm, s[e]);
     bm = p_pair_max(bm);
     const bool need = bm > m + 8.0f;
     if (__builtin_amdgcn_ballot_w64(need)) {
@@ -613,40 +702,31 @@ __global__ __launch_bounds__(256, 2) void prefix_flash_fp32(PrefixArgs a) {
 #pragma unroll
       for (int i = 0; i < 4; i++) o[i] *= f;
     }
-    float bl = 0.0f;
+    float w[16], bl = 0.0f;
 #pragma unroll
     for (int e = 0; e < 16; e++) {
-      s0[e] = __builtin_amdgcn_exp2f(s0[e] - m);
-      s1[e] = __builtin_amdgcn_exp2f(s1[e] - m);
-      bl += s0[e] + s1[e];
+      w[e] = __builtin_amdgcn_exp2f(s[e] - m);
+      bl += w[e];
     }
     l += bl;
-    // k-step (tile t, register e): keys 32 t + 8 (e / 4) + 4 hf + e % 4
+    bf16x8 pf[2][3];
+#pragma unroll
+    for (int u = 0; u < 2; u++) p_terms8(w + 8 * u, pf[u]);
 #pragma unroll
     for (int dt = 0; dt < 4; dt++) {
-      const float* vrow = Vs + (32 * dt + r) * PVS;
-      f32x16 p = {};
+      f32x16 sum = {};
 #pragma unroll
-      for (int e = 0; e < 16; e++) {
-        const int key = 8 * (e >> 2) + 4 * hf + (e & 3);
-        p = __builtin_amdgcn_mfma_f32_32x32x2f32(vrow[key], s0[e], p, 0, 0, 0);
-        p = __builtin_amdgcn_mfma_f32_32x32x2f32(vrow[32 + key], s1[e], p, 0, 0, 0);
+      for (int u = 0; u < 2; u++) {
+        bf16x8 vf[3];
+#pragma unroll
+        for (int p = 0; p < 3; p++) vf[p] = *(const bf16x8*)(st + vof[u] + dt * 2048 + p * FPL);
+        sum = p_mfma6(vf, pf[u], sum);
       }
-      o[dt] += p;
+      o[dt] += sum;
     }
   }
-  l = p_pair_sum(l);
-  if (v >= a.V) return;
-  const bool part = a.splits > 1;
-  const float inv = part ? 1.0f : 1.0f / l;
-  const int64_t at = ((int64_t)sp * a.Hkv + hk) * a.V + v;
-  if (part && hf == 0) *(float2*)(a.pml + at * 2) = make_float2(m, l);
-  float* d = (part ? a.po + at * PHD : (float*)a.o + (int64_t)row * a.ldo + h * PHD) + 4 * hf;
-#pragma unroll
-  for (int dt = 0; dt < 4; dt++)
-#pragma unroll
-    for (int g = 0; g < 4; g++)
-      *(f32x4*)(d + 32 * dt + 8 * g) = f32x4{o[dt][4 * g] * inv, o[dt][4 * g + 1] * inv, o[dt][4 * g + 2] * inv, o[dt][4 * g + 3] * inv};
+  p_barrier();  // (the planes become the rows')
+  p_leave(a, smem, sp, hk, v0 + 32 * wave, wave, lane, o, m, l);
 }
 
 // The parts of a split call, a half wave per virtual row: o = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s, eight parts asked for
@@ -702,10 +782,10 @@ static int prefix_part(anima_ctx* c, PrefixArgs& a) {
   constexpr bool BF = sizeof(T) == 2;
   a.V = a.T * a.group;
   const int blocks = a.Pp / PBK + a.Tp / PBK;
-  const bool eight = BF && (int64_t)((a.V + 255) / 256) * a.Hkv >= c->num_cus;
-  const int rows = eight ? 256 : 128, fill = BF ? c->num_cus : 2 * c->num_cus;  // (two fp32 workgroups to a CU)
+  const bool eight = BF ? (int64_t)((a.V + 255) / 256) * a.Hkv >= c->num_cus : a.V > 128;
+  const int rows = eight ? 256 : 128;
   a.nt = (a.V + rows - 1) / rows;
-  a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({fill / ((int64_t)a.nt * a.Hkv), blocks / 2, 64}));
+  a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({c->num_cus / ((int64_t)a.nt * a.Hkv), blocks / 2, 64}));
   const size_t plane = (size_t)a.Hkv * a.Tp * PHD * sizeof(T), q = (size_t)a.Hkv * a.V * PHD * sizeof(T),
                n = a.splits > 1 ? (size_t)a.splits * a.Hkv * a.V : 0;
   void* ws = nullptr;
@@ -719,7 +799,8 @@ static int prefix_part(anima_ctx* c, PrefixArgs& a) {
   if (int rc = prefix_prep_launch<T>(c, a)) return rc;
   Launch L(c, BF ? "attn.prefix_bf16" : "attn.prefix_fp32", 4.0 * a.T * a.H * PHD * a.P, 0.0);
   const dim3 grid((unsigned)((int64_t)a.nt * a.Hkv * a.splits));
-  if (!BF) hipLaunchKernelGGL(prefix_flash_fp32, grid, dim3(256), 0, c->stream, a);
+  if (!BF && eight) hipLaunchKernelGGL(prefix_flash_fp32<8>, grid, dim3(512), 0, c->stream, a);
+  else if (!BF) hipLaunchKernelGGL(prefix_flash_fp32<4>, grid, dim3(256), 0, c->stream, a);
   else if (eight) hipLaunchKernelGGL(prefix_flash_bf16<8>, grid, dim3(512), 0, c->stream, a);
   else hipLaunchKernelGGL(prefix_flash_bf16<4>, grid, dim3(256), 0, c->stream, a);
   if (a.splits > 1)
