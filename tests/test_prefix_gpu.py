@@ -178,6 +178,54 @@ def test_long(ctx, lens, P, precision):
 
 
 @pytest.mark.parametrize("precision", [0, 1], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("lens,P", [([64] * 32, 70), ([65, 1, 30] * 24 + [77], 130)])
+def test_many_tiles(ctx, lens, P, precision):
+    """Tiles of 256 rows enough for every compute unit (32 heads, a kv head each): several sequences to a tile, not split."""
+    Case(ctx, lens, P, 32, 32, precision).check()
+
+
+@pytest.mark.parametrize("precision", [0, 1], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("lens,P,H,Hkv", [([3, 1], 640, 2, 1), ([64] * 32, 640, 32, 32), ([200], 0, 2, 2), ([300, 90], 200, 2, 1)])
+@pytest.mark.parametrize("falling", [False, True])
+def test_scores_that_rise(ctx, lens, P, H, Hkv, precision, falling):
+    """Scores of 2^90 times the weight every 64 keys (or a 2^90th): a row is the mean of the values at its last (first) such
+    keys, whose scores are the same.  q and k are powers of two times signs, so that only the common factor scale rounds."""
+    c = Case(ctx, lens, P, H, Hkv, precision, normed=False, roped=False)
+    sign = np.where(np.random.default_rng(1).random(128) < 0.5, -1.0, 1.0).astype(np.float32)
+    level = lambda j: (-1.0 if falling else 1.0) * (j // 64).astype(np.float32)[:, None, None] * 0.5
+    c.pk = (level(np.arange(P)) * sign * np.ones((1, Hkv, 1))).astype(np.float32)
+    if P:
+        up = [ctx.upload(c.pk), ctx.upload(c.pv)]
+        ctx.attention_prefix(k=up[0], v=up[1], lens=[P], H=H, group=H // Hkv, ldk=Hkv * 128, ldv=Hkv * 128, precision=precision,
+                             prepare_into=c.prefix)
+    at = 0
+    c.qkv[:, : H * 128] = np.tile(sign, H)
+    for n in lens:
+        c.qkv[at: at + n, H * 128: (H + Hkv) * 128] = (level(P + np.arange(n)) * sign * np.ones((1, Hkv, 1))).reshape(n, -1)
+        at += n
+    c.scale = float(90 / 64 * np.log(2.0))  # a level is 128 * 0.5 * scale
+    got = c.get().reshape(c.T, H, 128)
+    ref, _ = c.ref()
+    v = max(np.abs(c.pv).max() if P else 0, np.abs(c.qkv[:, (H + Hkv) * 128:]).max())
+    # equal weights at one level, rounded alike and divided by the sum of what they were rounded to: a value of v is off by half a
+    # bf16 step (8 significant bits: 2^-8 of a value just above a power of two), a sum of up to 64 by 64 2^-24
+    assert np.abs(got - ref).max() <= (2.0 ** -8 if precision == 0 else 0.0) * v + 128 * 2.0 ** -24 * v
+
+
+@pytest.mark.parametrize("precision", [0, 1], ids=["bf16", "fp32"])
+def test_two_contexts(ctx, precision):
+    """Calls of two contexts at once, each on its stream with scratch of its own."""
+    with amd().Context(0) as other:
+        a, b = Case(ctx, [40, 1, 17], 200, 4, 2, precision), Case(other, [40, 1, 17], 200, 4, 2, precision)
+        ra, rb = a.get(), b.get()
+        outs = [(a.call(), b.call()) for _ in range(4)]
+        for x, y in outs:
+            np.testing.assert_array_equal(x.numpy(), ra)
+            np.testing.assert_array_equal(y.numpy(), rb)
+        np.testing.assert_array_equal(ra, rb)
+
+
+@pytest.mark.parametrize("precision", [0, 1], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("lens,P", [([5, 70, 1], 100), ([5, 70, 1], 0), ([1] * 70, 64), ([300, 200], 130)])
 @pytest.mark.parametrize("std", [30.0, 1e-3])
 def test_large_and_small_scores(ctx, lens, P, precision, std):

@@ -100,6 +100,25 @@ def test_products(ctx, M, N, K, g, mid, precision):
     assert np.all(err <= tol), (err / tol).max()
 
 
+@pytest.mark.parametrize("precision,M,N,K,g,mid,name", [
+    (1, 1025, 4092, 288, 32, True, "gemm.q4.256"), (1, 515, 3700, 1312, 32, True, "gemm.q4.128"), (0, 2050, 3900, 320, 64, True, "gemm.q4.256"),
+    (0, 1030, 3600, 1152, 128, False, "gemm.q4.128"), (1, 70, 260, 256, 64, True, "gemm.q4.64"), (0, 300, 64, 4160, 64, True, "gemm.q4.64"),
+    (1, 20, 40, 16416, 32, True, "gemm.q4.64"), (1, 20, 40, 8224, 32, False, "gemm.q4.few"), (0, 64, 300, 1024, 64, True, "gemm.q4.few"),
+    (1, 4, 300, 1024, 64, True, "gemv.q4")])
+def test_variants(ctx, precision, M, N, K, g, mid, name):
+    """Each kernel by its profiler name, at ragged sizes, with an activation and bf16 rows."""
+    rng = np.random.default_rng(M + K)
+    W = Q4(ctx, rng, N, K, g, mid)
+    x = rng.normal(0, 1, (M, K)).astype(np.float32)
+    dx, out = ctx.upload(x), ctx.empty((M, N), np.uint16)
+    assert ran(ctx, lambda: ctx.linear(W.w, M, out, x=dx, act="gelu", precision=precision, out_bf16=True)) == {name}
+    r0 = x.astype(np.float64) @ W.values.T
+    ref = act64(r0, "gelu")
+    err = np.abs(widen(out.numpy()) - ref)
+    tol = bound(x.astype(np.float64), W.values, K, precision, True, ref, r0)
+    assert np.all(err <= tol), (err / tol).max()
+
+
 @pytest.mark.parametrize("M", [1, 3, 20, 150])
 @pytest.mark.parametrize("epi,act,add,alpha,out_bf16", [
     (0, "none", False, 0.0, True), (0, "gelu", False, 0.0, True), (0, "silu", True, 0.5, False), (0, "gelu", True, 0.0, False),
