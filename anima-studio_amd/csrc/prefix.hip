@@ -93,7 +93,7 @@ template <class T>
 __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a) {
   constexpr bool BF = sizeof(T) == 2;
   typedef std::conditional_t<BF, _Float16, float> TK;
-  __shared__ int bad[64];
+  __shared__ int bad[64], start[64];  // of the rows: whether they are not finite, their sequences' first rows
   __shared__ SeqStarts seq;
   const int t = threadIdx.x, w = t >> 6, lane = t & 63, kb0 = blockIdx.x * 64;
   const bool query = (int)blockIdx.y >= a.Hkv;
@@ -123,18 +123,21 @@ __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a) {
   seq.fill(a.seq);
   __builtin_amdgcn_s_waitcnt(0xc07f);  // (LDS alone: the loads above go on)
   p_barrier();
+  if (t < 64) {
+    const int l = min(kb0 + t, a.T - 1), b = seq.of(a.seq.n, l);
+    start[t] = seq.at[b];
+    if (a.range && blockIdx.y == 0 && kb0 + t < a.T) a.range[l] = make_int2(seq.at[b], a.causal ? l + 1 : seq.at[b + 1]);
+  }
+  __builtin_amdgcn_s_waitcnt(0xc07f);
+  p_barrier();
   if (a.cs) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const int l = min(kb0 + 16 * w + 4 * i + rsub, a.T - 1);
-      const float* cr = a.cs + (int64_t)(a.P + l - seq.at[seq.of(a.seq.n, l)]) * 64 + 4 * q16;
+      const int rl = 16 * w + 4 * i + rsub, l = min(kb0 + rl, a.T - 1);
+      const float* cr = a.cs + (int64_t)(a.P + l - start[rl]) * 64 + 4 * q16;
       cv[i] = *(const f32x4*)cr;
       sv[i] = *(const f32x4*)(cr + a.sin_off);
     }
-  }
-  if (a.range && blockIdx.y == 0 && t < 64 && kb0 + t < a.T) {
-    const int b = seq.of(a.seq.n, kb0 + t);
-    a.range[kb0 + t] = make_int2(seq.at[b], a.causal ? kb0 + t + 1 : seq.at[b + 1]);
   }
   const auto finite = [](f32x4 v, auto as) {
     float m = 0.0f;
