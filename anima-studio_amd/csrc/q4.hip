@@ -176,22 +176,26 @@ __device__ __forceinline__ void q4_leave(const Q4Args& a, int64_t m, int n, floa
   ((float*)a.out)[m * a.ldc + n] = a.epi == ANIMA_EPI_GATED ? __builtin_fmaf(e.gate, r, e.c) : r + e.c;
 }
 
-// The same for four columns (vec: rows of out, bias, add and gate in quads of 16 bytes; else one by one, when they leave).
-__device__ __forceinline__ Q4Ends<f32x4> q4_ask4(const Q4Args& a, int vec, int64_t m, int n) {
+// The same for four columns from n (a multiple of 4) on, fewer at the row's end.  Rows may start anywhere: the memory takes 16 bytes
+// of any four columns at once (2770 x 6019 x 256 in one term: 94 us with aligned
+// quads alone, a column at a time elsewhere, 59 so).
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef __bf16 bf16x4_any __attribute__((ext_vector_type(4), aligned(2)));
+
+__device__ __forceinline__ Q4Ends<f32x4> q4_ask4(const Q4Args& a, int64_t m, int n) {
   Q4Ends<f32x4> e{};
-  if (!vec) return e;
-  if (a.bias) e.bias = *(const f32x4*)(a.bias + n);
-  if (a.add) e.add = *(const f32x4*)(a.add + m * a.ld_add + n);
-  if (a.epi == ANIMA_EPI_GATED) e.gate = *(const f32x4*)(a.gate + n);
-  if (a.epi != ANIMA_EPI_STORE) e.c = *(const f32x4*)((const float*)a.out + m * a.ldc + n);
+  if (n + 4 > a.N) return e;
+  if (a.bias) e.bias = *(const f32x4_any*)(a.bias + n);
+  if (a.add) e.add = *(const f32x4_any*)(a.add + m * a.ld_add + n);
+  if (a.epi == ANIMA_EPI_GATED) e.gate = *(const f32x4_any*)(a.gate + n);
+  if (a.epi != ANIMA_EPI_STORE) e.c = *(const f32x4_any*)((const float*)a.out + m * a.ldc + n);
   return e;
 }
 
-__device__ __forceinline__ void q4_leave4(const Q4Args& a, int vec, int64_t m, int n, f32x4 r, const Q4Ends<f32x4>& e) {
-  if (!vec) {
+__device__ __forceinline__ void q4_leave4(const Q4Args& a, int64_t m, int n, f32x4 r, const Q4Ends<f32x4>& e) {
+  if (n + 4 > a.N) {
 #pragma unroll 1
-    for (int i = 0; i < 4; i++)
-      if (n + i < a.N) q4_leave(a, m, n + i, i == 0 ? r[0] : i == 1 ? r[1] : i == 2 ? r[2] : r[3], q4_ask(a, m, n + i));
+    for (int i = 0; n + i < a.N; i++) q4_leave(a, m, n + i, i == 0 ? r[0] : i == 1 ? r[1] : r[2], q4_ask(a, m, n + i));
     return;
   }
   r = r * a.alpha + e.bias + e.add;
@@ -203,7 +207,7 @@ __device__ __forceinline__ void q4_leave4(const Q4Args& a, int vec, int64_t m, i
     for (int i = 0; i < 4; i++) r[i] = silu_f(r[i]);
   }
   if (a.obf) {
-    *(bf16x4*)((bf16*)a.out + m * a.ldc + n) = bf16x4{to_bf16(r[0]), to_bf16(r[1]), to_bf16(r[2]), to_bf16(r[3])};
+    *(bf16x4_any*)((bf16*)a.out + m * a.ldc + n) = bf16x4_any{to_bf16(r[0]), to_bf16(r[1]), to_bf16(r[2]), to_bf16(r[3])};
     return;
   }
   if (a.epi == ANIMA_EPI_GATED) {
@@ -212,7 +216,7 @@ __device__ __forceinline__ void q4_leave4(const Q4Args& a, int vec, int64_t m, i
   } else {
     r = r + e.c;
   }
-  *(f32x4*)((float*)a.out + m * a.ldc + n) = r;
+  *(f32x4_any*)((float*)a.out + m * a.ldc + n) = r;
 }
 
 // One to four rows on the vector units, in fp32: a wave takes U columns, a lane 16 consecutive k of each 1024 (eight bytes of
@@ -461,10 +465,10 @@ struct Q4Tile {
   const float* rm;
   const float* rn;   // (readable to the next multiple of 256 columns)
   const float* sx;
-  float* part;       // [splits][M][N] sums of a product split over k, or NULL
+  float* part;       // [splits][M][ldn] sums of a product split over k, or NULL
   int Kp, sps;       // k padded; steps of 64 k in a split
   int ldp;           // values between the terms' rows
-  int vec;           // rows of out, bias, add and gate in quads of 16 bytes
+  int ldn;           // N to the next multiple of 4
   int svec;          // four steps' scales are one aligned piece of a row
 };
 
@@ -513,7 +517,7 @@ __global__ __launch_bounds__(64 * QF_WAVES, 2) void q4_few_kernel(Q4Tile q) {
   const int om = m0 + (lane & 31), on = n0 + 8 * wave + 4 * (lane >> 5);
   const bool out = wave < 4 && om < a.M && on < a.N;
   Q4Ends<f32x4> ask{};
-  if (out) ask = q4_ask4(a, q.vec, om, on);
+  if (out) ask = q4_ask4(a, om, on);
   {
     const int64_t col = (int64_t)min(n0 + (tid >> 4), a.N - 1) * KG;
     for (int g0 = tid & 15; g0 < KG; g0 += 64) {
@@ -594,7 +598,7 @@ __global__ __launch_bounds__(64 * QF_WAVES, 2) void q4_few_kernel(Q4Tile q) {
   f32x4 v = sum[tid];
 #pragma unroll
   for (int w = 1; w < QF_WAVES; w++) v = v + sum[w * 256 + tid];
-  q4_leave4(a, q.vec, om, on, v, ask);
+  q4_leave4(a, om, on, v, ask);
 }
 
 // ------------------------------------------------------------------ tiles
@@ -860,21 +864,14 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void q4_tile_kernel(
 #pragma unroll
       for (int u = 0; u < 4; u++) {
         v[u] = *(const f32x4*)(rows + (q + u * PR + lane / LR) * RS + 4 * (lane % LR));
-        if (!t.part && mo + u * PR < a.M && n < a.N) ask[u] = q4_ask4(a, t.vec, mo + u * PR, n);
+        if (!t.part && mo + u * PR < a.M && n < a.N) ask[u] = q4_ask4(a, mo + u * PR, n);
       }
 #pragma unroll
       for (int u = 0; u < 4; u++) {
         const int64_t m = mo + u * PR;
         if (m >= a.M || n >= a.N) continue;
-        if (!t.part) {
-          q4_leave4(a, t.vec, m, n, v[u], ask[u]);
-          continue;
-        }
-        float* o = t.part + ((int64_t)blockIdx.y * a.M + m) * a.N + n;
-        if (t.vec) *(f32x4*)o = v[u];
-        else
-          for (int e = 0; e < 4; e++)
-            if (n + e < a.N) o[e] = v[u][e];
+        if (t.part) *(f32x4*)(t.part + ((int64_t)blockIdx.y * a.M + m) * t.ldn + n) = v[u];
+        else q4_leave4(a, m, n, v[u], ask[u]);
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -885,25 +882,16 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void q4_tile_kernel(
 constexpr int Q4_SPLITS = 16;
 __global__ __launch_bounds__(256) void q4_join_kernel(Q4Tile t, int splits) {
   const Q4Args& a = t.a;
-  const int64_t quads = (a.N + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / quads;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / (t.ldn / 4), plane = (int64_t)a.M * t.ldn;
   if (m >= a.M) return;
-  const int n = (int)(4 * (i - m * quads));
-  const float* p = t.part + m * a.N + n;
-  const int64_t plane = (int64_t)a.M * a.N;
-  const Q4Ends<f32x4> ask = q4_ask4(a, t.vec, m, n);
-  f32x4 v = {};
-  if (t.vec) {
-    f32x4 w[Q4_SPLITS];  // (all asked for before the first is added)
+  const int n = (int)(4 * i - m * t.ldn);
+  const Q4Ends<f32x4> ask = q4_ask4(a, m, n);
+  f32x4 w[Q4_SPLITS], v = {};  // (all asked for before the first is added)
 #pragma unroll
-    for (int s = 0; s < Q4_SPLITS; s++) w[s] = s < splits ? *(const f32x4*)(p + s * plane) : f32x4{};
+  for (int s = 0; s < Q4_SPLITS; s++) w[s] = s < splits ? *(const f32x4*)(t.part + s * plane + 4 * i) : f32x4{};
 #pragma unroll
-    for (int s = 0; s < Q4_SPLITS; s++) v = v + w[s];
-  } else {
-    for (int s = 0; s < splits; s++)
-      for (int e = 0; e < 4; e++)
-        if (n + e < a.N) v[e] += p[s * plane + e];
-  }
-  q4_leave4(a, t.vec, m, n, v, ask);
+  for (int s = 0; s < Q4_SPLITS; s++) v = v + w[s];
+  q4_leave4(a, m, n, v, ask);
 }
 
 // ------------------------------------------------------------------ host
@@ -967,11 +955,6 @@ static void q4_gemv(anima_ctx* c, const Q4Args& a) {
 }
 
 // whether rows of out, bias, add and gate come in quads of 16 bytes (8 of bf16 rows)
-static int q4_vec(const Q4Args& a) {
-  return a.N % 4 == 0 && a.ldc % 4 == 0 && q4_al(a.out, a.obf ? 8 : 16) && q4_al(a.bias, 16) && q4_al(a.gate, 16) &&
-         (!a.add || (q4_al(a.add, 16) && a.ld_add % 4 == 0));
-}
-
 // LDS of the kernel for few rows: the scales and middles, then the waves' sums
 static int64_t q4_few_lds(const Q4Args& a) {
   return std::max<int64_t>((int64_t)(a.K / a.G) * 128 * (a.gz ? 2 : 1), QF_WAVES * 4096);
@@ -990,17 +973,33 @@ static int q4_matrix(anima_ctx* c, const Q4Args& a, bool two) {
   t.Kp = (a.K + 63) / 64 * 64;
   // rows of the terms an odd number of lines of 128 bytes apart: at a power of two one step's rows meet in one memory channel
   t.ldp = t.Kp / 64 % 2 ? t.Kp : t.Kp + 64;
-  t.vec = q4_vec(a);
+  t.ldn = (a.N + 3) / 4 * 4;
   const int KG = a.K / a.G, steps = t.Kp / 64;
   const bool few = a.M <= 64 && q4_few_lds(a) <= Q4_FEW_LDS;
   const auto tiles = [&](int bm, int bn) { return (int64_t)((a.M + bm - 1) / bm) * ((a.N + bn - 1) / bn); };
-  // the largest tile of which there are enough
+  // The largest tile of which there are enough; the smallest ends soonest (K = 256 in one term, 2770 x 6019: 39 us, 59 by the largest),
+  // the largest read x least (8192 x 8192 x 2048: two terms 587, 636, 888 us from the largest down, one term 337, 392, 513).
+  // Where there are too few, parts of k: of 16 steps and more on the CUs' second places (two terms, 644 x 1695 x 6912:
+  // 82 us whole, 62 in parts), of three and more while CUs are idle (202 x 122 x 1792: 24 and 14; a join takes 3 us and more).
   const int rows = two ? 64 : 128;  // of the larger tiles
-  const int tile = tiles(rows, 256) >= c->num_cus ? 0 : tiles(rows, 128) >= c->num_cus ? 1 : 2;
-  const int64_t nt = tile == 0 ? tiles(rows, 256) : tile == 1 ? tiles(rows, 128) : tiles(64, 64);
-  // k is split until the tiles fill half of the CUs (a split of 515 x 1316 x 1440, 189 tiles, takes 14.6 us and 4.1 for its join: 16 whole)
-  int splits = 1;
-  while (!few && splits < Q4_SPLITS && nt * splits * 2 <= c->num_cus && steps / (splits * 2) >= 4) splits *= 2;
+  const int64_t cus = c->num_cus, t0 = tiles(rows, 256), t1 = tiles(rows, 128), t2 = tiles(64, 64);
+  int tile = 2, splits = 1;
+  if (few) {
+  } else if (t0 >= 2 * cus && (two ? steps >= 16 || t0 >= 4 * cus : steps >= 8)) {
+    tile = 0;
+  } else if (two ? t1 >= cus : t1 >= 2 * cus && steps >= 8) {
+    tile = 1;
+  } else {
+    if (two) {
+      while (t1 * splits < cus && splits < Q4_SPLITS) splits *= 2;
+      if (t1 * splits >= cus && steps / splits >= 16) tile = 1;
+      else splits = 1;
+    } else {
+      while (t2 * splits < 2 * cus && splits < Q4_SPLITS && steps / (2 * splits) >= 16) splits *= 2;
+    }
+    if (tile == 2 && steps >= 16)
+      while (splits < Q4_SPLITS && t2 * splits * 2 <= cus && steps / (2 * splits) >= 3) splits *= 2;
+  }
   t.sps = (steps + splits - 1) / splits;
   if (splits > 1) t.sps = (t.sps + 3) / 4 * 4;
   t.svec = a.K % 256 == 0 && q4_al(a.gs, 16);
@@ -1014,7 +1013,7 @@ static int q4_matrix(anima_ctx* c, const Q4Args& a, bool two) {
   };
   const size_t plane = (few ? (size_t)(a.M + 31) / 32 * 32 * t.Kp : (size_t)a.M * t.ldp) * 2, oh = take(plane), ol = two ? take(plane) : 0, om = take((size_t)a.M * 4),
                on = few ? 0 : take(((size_t)a.N + 255) / 256 * 1024), os = a.gz ? take((size_t)a.M * KG * 4) : 0,
-               op = splits > 1 ? take((size_t)splits * a.M * a.N * 4) : 0;
+               op = splits > 1 ? take((size_t)splits * a.M * t.ldn * 4) : 0;
   void* tmp = nullptr;
   if (int rc = anima_alloc(c, at, &tmp)) return rc;
   char* const b = (char*)tmp;
@@ -1051,7 +1050,7 @@ static int q4_matrix(anima_ctx* c, const Q4Args& a, bool two) {
     else q4_tile_launch<64, 64, 32, 32, 1, 4>(c, t, splits);
   }
   if (splits > 1)
-    hipLaunchKernelGGL(q4_join_kernel, dim3((unsigned)(((int64_t)a.M * ((a.N + 3) / 4) + 255) / 256)), dim3(256), 0, c->stream, t, splits);
+    hipLaunchKernelGGL(q4_join_kernel, dim3((unsigned)(((int64_t)a.M * (t.ldn / 4) + 255) / 256)), dim3(256), 0, c->stream, t, splits);
   const int rc = L.end();
   anima_free(c, tmp);
   return rc;
