@@ -975,7 +975,10 @@ static int q4_matrix(anima_ctx* c, const Q4Args& a, bool two) {
   t.ldp = t.Kp / 64 % 2 ? t.Kp : t.Kp + 64;
   t.ldn = (a.N + 3) / 4 * 4;
   const int KG = a.K / a.G, steps = t.Kp / 64;
-  const bool few = a.M <= 64 && q4_few_lds(a) <= Q4_FEW_LDS;
+  // Up to 64 rows by 32 x 32 tiles, but two terms of more than 32 rows with many steps, where x is read once more for every 32 rows
+  // (33 x 8192 x 4096: 29 us, 23 by the tiles; 64 x 4096 x 4096: 19 and 23).
+  const bool many = two && a.M > 32 && (a.K >= 8192 || (int64_t)a.N * a.K >= (int64_t)1 << 25);
+  const bool few = a.M <= 64 && !many && q4_few_lds(a) <= Q4_FEW_LDS;
   const auto tiles = [&](int bm, int bn) { return (int64_t)((a.M + bm - 1) / bm) * ((a.N + bn - 1) / bn); };
   // The largest tile of which there are enough; the smallest ends soonest (K = 256 in one term, 2770 x 6019: 39 us, 59 by the largest),
   // the largest read x least (8192 x 8192 x 2048: two terms 587, 636, 888 us from the largest down, one term 337, 392, 513).
