@@ -213,6 +213,49 @@ def test_scores_that_rise(ctx, lens, P, H, Hkv, precision, falling):
 
 
 @pytest.mark.parametrize("precision", [0, 1], ids=["bf16", "fp32"])
+def test_longest_prefix(ctx, precision):
+    """2^22 keys: 2 GiB of k in fp32, prepared planes of 1 and 2 GiB.  Values of 1 plus noise, so that a result is 1 but for the
+    mean of the noise: the sums of 4 million weights, in chains of at most 65536 keys a part and 64 parts, are off by 2^-24 a step of
+    16 keys (fp32: of half of one) in the worst case, a bf16 value by 2^-8 of itself, and the errors of q, k and the weights meet the noise
+    alone."""
+    m = amd()
+    P, T = 1 << 22, 3
+    k, v = ctx.empty((P, 128)), ctx.empty((P, 128))
+    ctx.fill_random(k, P * 128, "f32", 1, -1.0, 1.0)
+    ctx.fill_random(v, P * 128, "f32", 2, 0.75, 1.25)
+    prefix = ctx.empty((ctx.attention_kv_bytes(1, 1, P, precision),), np.uint8)
+    ctx.attention_prefix(k=k, v=v, lens=[P], H=2, group=2, ldk=128, ldv=128, precision=precision, prepare_into=prefix)
+    hk, hv = k.numpy(), v.numpy()
+    k.release()
+    v.release()
+    rng = np.random.default_rng(0)
+    x = rng.normal(0, 1, (T, 4 * 128)).astype(np.float32)
+    x[:, :256] *= np.float32(0.5)
+    # the last block of the prefix counts: row 0 of head 0 looks for its last key
+    x[0, :128] = 40.0 * hk[-1]
+    dx, out = ctx.upload(x), ctx.empty((T, 256))
+    ctx.attention_prefix(q=dx, k=dx, v=dx, o=out, lens=[2, 1], H=2, group=2, ldq=512, ldk=512, ldv=512, k_off=256, v_off=384, P=P,
+                         prefix_kv=prefix, precision=precision)
+    got = out.numpy().reshape(T, 2, 128)
+    prefix.release()
+    ctx.trim()
+    s = np.concatenate([(x[:, h * 128: h * 128 + 128].astype(np.float64) @ hk[i: i + (1 << 19)].T.astype(np.float64))
+                        for h in range(2) for i in range(0, P, 1 << 19)], 1).reshape(T, 2, P) / np.sqrt(128.0)
+    for t in range(T):
+        own = [0] if t == 0 else [0, 1] if t == 1 else [2]
+        ko, vo = x[own, 256:384].astype(np.float64), x[own, 384:].astype(np.float64)
+        for h in range(2):
+            so = ko @ x[t, h * 128: h * 128 + 128].astype(np.float64) / np.sqrt(128.0)
+            top = max(s[t, h].max(), so.max())
+            p, po = np.exp(s[t, h] - top), np.exp(so - top)
+            l = p.sum() + po.sum()
+            ref = (sum(p[i: i + (1 << 19)] @ hv[i: i + (1 << 19)].astype(np.float64) for i in range(0, P, 1 << 19)) + po @ vo) / l
+            # 65536 keys in steps of 16 (fp32: 32), then 64 parts
+            tol = 1.25 * 2.0 ** -24 * (65536 / (16 if precision == m.PREC_BF16 else 32) + 64) + (2.0 ** -8 if precision == m.PREC_BF16 else 1e-5)
+            assert np.abs(got[t, h] - ref).max() <= tol * max(1.0, np.abs(ref).max()), (t, h, np.abs(got[t, h] - ref).max())
+
+
+@pytest.mark.parametrize("precision", [0, 1], ids=["bf16", "fp32"])
 def test_two_contexts(ctx, precision):
     """Calls of two contexts at once, each on its stream with scratch of its own."""
     with amd().Context(0) as other:
