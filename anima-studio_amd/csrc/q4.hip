@@ -427,13 +427,19 @@ __global__ __launch_bounds__(256) void q4_prep_kernel(Q4Prep a) {
   }
 }
 
-// Eight codes, times the scale pair, in the order 0 4 1 5 2 6 3 7: 1024 + c by its bits, less 1032 (exact), times s.
-__device__ __forceinline__ f16x8 q4_decode(uint32_t c, f16x2 s) {
-  const f16x2 off = {(_Float16)-1032.0f, (_Float16)-1032.0f};
+// Eight codes, times the scale pair s (s16: a 16th of it), in the order 0 4 1 5 2 6 3 7.  A code's bits in the mantissa of 1024 are 1024 +
+// c, four places further up 1024 + 16 c: less 1032, or 1152, (exact), times s, or s16.
+struct Q4Bits {  // (in registers: an instruction takes one constant of its own, and v_and_or two)
+  uint32_t even = 0x000f000fu, odd = 0x00f000f0u, big = 0x64006400u;
+  __device__ __forceinline__ Q4Bits() { asm("" : "+s"(even), "+s"(odd), "+v"(big)); }
+};
+__device__ __forceinline__ f16x8 q4_decode(const Q4Bits& b, uint32_t c, f16x2 s, f16x2 s16) {
+  const f16x2 off = {(_Float16)-1032.0f, (_Float16)-1032.0f}, off16 = {(_Float16)-1152.0f, (_Float16)-1152.0f};
   f16x8 r;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    const f16x2 v = (__builtin_bit_cast(f16x2, ((c >> (4 * i)) & 0x000f000fu) | 0x64006400u) + off) * s;
+    const f16x2 k = __builtin_bit_cast(f16x2, ((i < 2 ? c : c >> 8) & (i & 1 ? b.odd : b.even)) | b.big);
+    const f16x2 v = i & 1 ? (k + off16) * s16 : (k + off) * s;
     r[2 * i] = v[0];
     r[2 * i + 1] = v[1];
   }
@@ -540,7 +546,8 @@ __global__ __launch_bounds__(64 * QF_WAVES, 2) void q4_few_kernel(Q4Tile q) {
   q4_barrier();
   f32x16 acc = {};
   const float up = 1.0f / rm;
-  const f16x2 one = {(_Float16)1.0f, (_Float16)1.0f};
+  const f16x2 one = {(_Float16)1.0f, (_Float16)1.0f}, one16 = {(_Float16)0.0625f, (_Float16)0.0625f};
+  const Q4Bits bits;
   const auto product = [&](const Step& v, int step) __attribute__((always_inline)) {
     // the halves' words exchanged, so that matrix step i covers k 16 i .. 16 i + 15: lane half hf word 2 i + hf of 8
     u32x4 w = v.w;
@@ -556,7 +563,7 @@ __global__ __launch_bounds__(64 * QF_WAVES, 2) void q4_few_kernel(Q4Tile q) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       f32x16& p = part[G32 ? i >> 1 : 0];
-      const f16x8 wf = q4_decode(w[i < 2 ? 2 * i : 2 * i - 3], one);
+      const f16x8 wf = q4_decode(bits, w[i < 2 ? 2 * i : 2 * i - 3], one, one16);
 #pragma unroll
       for (int e = TERMS - 1; e >= 0; e--) p = __builtin_amdgcn_mfma_f32_32x32x16_f16(wf, v.x[e][i], p, 0, 0, 0);
     }
@@ -767,6 +774,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void q4_tile_kernel(
   // the next one: this wave's copies of it have arrived when at most those of the stages after it pend.
   f16x8 xf[2][MT][TERMS], wf[2][NT];
   u32x4 wr[NT];
+  const Q4Bits bits;
   const auto xread = [&](int u, int po, int i) __attribute__((always_inline)) {
 #pragma unroll
     for (int m = 0; m < MT; m++)
@@ -779,7 +787,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void q4_tile_kernel(
   };
   const auto decode = [&](int u, int q, int i) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < NT; j++) wf[u][j] = q4_decode(wr[j][i], sv[q][j]);
+    for (int j = 0; j < NT; j++) wf[u][j] = q4_decode(bits, wr[j][i], sv[q][j], sv[q][j] * (_Float16)0.0625f);
   };
   pairs();
   Q4_WAIT_VM((NST - 1) * CPW);
