@@ -86,7 +86,9 @@ __device__ __forceinline__ void p_barrier() {
 // holding dims 4 q .. + 3 and 64 + the same (both of each rotated pair); V: wave w takes dims 32 w .. + 31 of all rows, lane
 // (q, c) the eight keys of V^T chunk c at dims 4 q .. + 3, so that every load and store moves whole lines.  The bf16 form has K
 // and q in f16 (their rounding to 8 bits alone would be 0.005 of a result) and keeps each 16 keys of a V^T row as 0-3, 8-11,
-// 4-7, 12-15, as the matrix products take them.
+// 4-7, 12-15, as the matrix products take them.  Every part of a split call would norm and rotate q again: once here (64 rows behind
+// 8192 keys 36 us with it in the tiles, 31 so).  Bound by memory (7741 rows of 16 and 8 heads: 190 MB, 36 us, 5.2 TB/s), few
+// rows by a launch and three trips to memory, one behind the other (7 us).
 // A key whose K or V is not finite (in its form) gets a K of NaN and a V of zeros: every row that sees it becomes NaN, and where it
 // is masked its weight of 0 meets no NaN in V.
 template <class T>
@@ -225,6 +227,10 @@ __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a) {
 // are in f16, 11 bits (in bf16 they would be 0.005 of a result off: more than its own rounding), the weights and V in bf16.
 // p = 2^(s - m) with an integer m that only rises (a power of two, so no rounding depends on when it rose): in blocks that
 // are seen whole without looking, as long as the weights' sum stays below 2^64, from -m in the scores' accumulators.
+// Blocks are copied by buffer_load ... lds three ahead into four stages of LDS, so a barrier a block is all that waves share.
+// 7741 rows of 16 heads behind 4096 keys: 264 GFLOP in 273 us, 967 TFLOP/s; the matrix cores are busy 56 % of the cycles at the 1.67
+// GHz that the power limit leaves (a library product of 8192 x 8192 x 8192: 1150).  64 rows of 32 heads behind 8192: 33.6 MB of keys
+// in 19 us, a start of 2, twelve until the last block is there, and the sums' way out.
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) void prefix_lds_t;
@@ -547,6 +553,8 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_bf16(PrefixArgs 
 // for all waves, under the products of the step before), and a step later are multiplied: one barrier a step.
 // p = 2^(s - m) with m raised where a step's maximum passes it by more than 8.  A step's products of V are added by themselves first:
 // chains of one step a sum across steps.
+// 1265 rows of 15 heads behind 1000 keys: 78 us (131 by the fp32 matrix cores), 1000 TFLOP/s of bf16 products with the tiles' unseen
+// keys, the matrix cores busy 54 % of the cycles at 1.5 GHz; LDS is full (raw keys and planes, two stages each).
 constexpr int FRAW = 2 * 32 * PHD * 4;   // bytes of a step's K, then V^T, as they come
 constexpr int FPL = 32 * PHD * 2;        // of one plane of its K or V^T
 constexpr int FST = 6 * FPL;             // of its planes: three of K, three of V^T
@@ -733,7 +741,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_fp32(PrefixArgs 
 }
 
 // The parts of a split call, a half wave per virtual row: o = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s, eight parts asked for
-// at a time.
+// at a time.  Bound by the parts' bytes (1265 rows of 15 heads in three parts: 39 MB, 8.6 us), few rows by a launch (2.5 us).
 __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixArgs a) {
   const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), n = (int64_t)a.Hkv * a.V;
   if (i >= n) return;
@@ -795,7 +803,8 @@ static int prefix_plan(const anima_ctx* c, bool bf, int longest, PrefixArgs& a) 
       const double block = !bf ? 6.0 : nw == 4 ? 1.2 : 1.4, start = bf ? 5.0 : 4.0, join = 2.0 + (double)s * a.Hkv * a.V * 1056 / 5e6;
       const double blocks = 0.5 * ((total + s - 1) / s) + 0.5 * total / s;  // (the longest part and the mean one)
       const double t = (double)rounds * (start + blocks * block) + (s > 1 ? join : 0.0);
-      if (best_nw && t >= best) continue;
+      // (one wave of rows whose blocks are all copied at its start: 2 rows behind 77 keys 15.1 us whole, 16.7 in three parts)
+      if (best_nw && (t >= best || (s > 1 && a.V <= 32 && total <= 3))) continue;
       best = t;
       best_nw = nw;
       a.nt = nt;

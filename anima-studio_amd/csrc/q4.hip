@@ -34,8 +34,8 @@ __device__ __forceinline__ void ld8(const T* p, float (&v)[8]) {
   }
 }
 
-// Eight weights a thread; the G / 8 neighbouring lanes of a group share its extremes.  One pass over the weight
-// (a load-time conversion, bound by its bytes).
+// Eight weights a thread; the G / 8 neighbouring lanes of a group share its extremes.  One pass over the weight, a load-time
+// conversion (151936 x 1024 from bf16: 132 us, 3.0 TB/s: the divisions, which the definition rounds, beside the bytes).
 template <class T>
 __global__ __launch_bounds__(256) void weight_quant_q4_kernel(const T* w, int64_t n8, int lanes, uint32_t* q, uint16_t* scale,
                                                               uint16_t* mid) {
@@ -112,7 +112,8 @@ __device__ __forceinline__ f32x4 embed4(const EmbedArgs& a, int64_t row, int k) 
   }
 }
 
-// A workgroup of 256 threads per row, four columns a thread at a time.
+// A workgroup of 256 threads per row, four columns a thread at a time.  Bound by the rows' bytes: 8191 rows of 2048 from 4 bits 13.5
+// us, 77 MB at 5.7 TB/s; one row of 1024 1.3 us.
 template <int KIND>
 __global__ __launch_bounds__(256) void embed_rows_kernel(EmbedArgs a) {
   const int64_t t = blockIdx.x;
@@ -223,7 +224,9 @@ __device__ __forceinline__ void q4_leave4(const Q4Args& a, int64_t m, int n, f32
 // codes, one group).  x goes through LDS, quad j of lane l's 16 at [j][l], so that the reads touch every bank once.  A code with its
 // highest bit turned is c - 8 in two's complement: in a byte's upper half 16 (c - 8), one conversion away from a
 // float, and s takes the 16.
-// Bound by its launch and one trip to memory for the codes.
+// Bound by its launch and one trip to memory for the codes: 1 x 4096 x 1024 3.6 us, 1 x 8192 x 2048 in groups of 32 5.2 us (10.6 MB).
+// More columns a wave share x's way through LDS, fewer fill more CUs: four from N = 4096 on, two from 2048 (four rows of 8192 x 2048:
+// 8.2 us, 13.7 a column a wave; one of 1024 x 8192: 5.7 a column a wave, 9.1 four).
 template <int MR, int U>
 __global__ __launch_bounds__(256) void q4_gemv_kernel(Q4Args a) {
   __shared__ f32x4 xs[2][MR][256];
@@ -352,7 +355,7 @@ struct Q4Prep {
 };
 
 // A wave per row of x (NV: pieces of 512 k that a wave holds; 0: two passes over the row, the second from the caches), or per
-// column's scales.
+// column's scales.  Bound by memory (8192 x 2048 into one term: 101 MB, 16 us), few rows by a launch and a trip (4 us).
 template <int NV>
 __global__ __launch_bounds__(256) void q4_prep_kernel(Q4Prep a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -483,7 +486,8 @@ struct Q4Tile {
 // A workgroup takes 32 columns and 32 rows, its eight waves every eighth step of 64 k each, their sums joined in order
 // through LDS.  The codes stay whole numbers (exact in f16), and each group's sums meet their scale in fp32; scales and
 // middles lie in LDS as [group][column].  x comes from q4_prep_kernel in the order of the lanes (as rows, a load meets 32 lines
-// and takes the address unit four times as long).
+// and takes the address unit four times as long).  Bound by trips to memory, of which each wave has two steps' under way (four:
+// no faster): 43 x 1024 x 2048 10 us, behind 4.3 for x.
 constexpr int QF_WAVES = 8;
 
 template <int TERMS, bool G32>
@@ -886,7 +890,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void q4_tile_kernel(
   }
 }
 
-// A split product's sums, added in order, and the epilogue.
+// A split product's sums, added in order, and the epilogue.  Bound by a launch and a trip to memory (3 to 5 us).
 constexpr int Q4_SPLITS = 16;
 __global__ __launch_bounds__(256) void q4_join_kernel(Q4Tile t, int splits) {
   const Q4Args& a = t.a;
@@ -944,8 +948,8 @@ int embed_rows_launch(anima_ctx* c, const anima_weight* W, const int32_t* ids, i
   return L.end();
 }
 
-constexpr int Q4_ROWS = 4;             // rows of the vector kernel
-constexpr int Q4_FEW_LDS = 65536;
+constexpr int Q4_ROWS = 4;         // rows of the vector kernel (four of 500 x 1024: 4.8 us, 9.2 by 32 x 32 tiles; of 8192 x 2048: 8.2 and 11.2)
+constexpr int Q4_FEW_LDS = 65536;  // that a launch may ask for
 
 static void q4_gemv(anima_ctx* c, const Q4Args& a) {
 #define GEMV(MR, U) hipLaunchKernelGGL((q4_gemv_kernel<MR, U>), dim3((unsigned)((a.N + 4 * U - 1) / (4 * U))), dim3(256), 0, c->stream, a)
@@ -962,7 +966,6 @@ static void q4_gemv(anima_ctx* c, const Q4Args& a) {
 #undef GEMV
 }
 
-// whether rows of out, bias, add and gate come in quads of 16 bytes (8 of bf16 rows)
 // LDS of the kernel for few rows: the scales and middles, then the waves' sums
 static int64_t q4_few_lds(const Q4Args& a) {
   return std::max<int64_t>((int64_t)(a.K / a.G) * 128 * (a.gz ? 2 : 1), QF_WAVES * 4096);
