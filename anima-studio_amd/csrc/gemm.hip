@@ -2730,7 +2730,7 @@ int linear_launch(anima_ctx* c, const anima_linear_desc* d, int64_t s3_plane) {
     if (d->add) return fail(c, ANIMA_E_UNSUPPORTED, "anima_linear: the LoRA epilogue and an add term together");
   }
   if (W->kind != ANIMA_W_F8 && W->kind != ANIMA_W_Q4 && (d->precision || d->out_bf16))
-    return fail(c, ANIMA_E_UNSUPPORTED, "anima_linear: precision and out_bf16 are for f8 and q4 weights (kind %d)", W->kind);
+    return fail(c, ANIMA_E_UNSUPPORTED, "anima_linear: precision and out_bf16 are for q4 and f8 weights (kind %d)", W->kind);
   if (M == 0) return ANIMA_OK;
 
   if (W->kind == ANIMA_W_F8) return linear_f8_launch(c, d);
