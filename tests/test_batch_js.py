@@ -187,6 +187,32 @@ def test_batch_calls():
         assert w in e, got["e"]
 
 
+def test_table(tmp_path):
+    """SafeTensors.table: the values that rows() reads one by one, whatever the file's type; more rows than one piece holds."""
+    from test_f8_js import safetensors
+
+    rng = np.random.default_rng(2)
+    v = rng.normal(0, 1, (5000, 8)).astype(np.float32)
+    v[0] = [0.0, -0.0, np.inf, -np.inf, np.nan, 1e-42, 3e38, -1.5]
+    q, sc = rng.integers(-128, 128, (4097, 8)).astype(np.int8), rng.normal(0, 1, 4097).astype(np.float32)
+    half = v.astype(np.float16)
+    path = safetensors(tmp_path / "t.safetensors", {
+        "a.weight": ("BF16", v.shape, bf16(v).tobytes()), "b.weight": ("F32", v.shape, v.tobytes()), "c.weight": ("F16", half.shape, half.tobytes()),
+        "d.weight": ("I8", q.shape, q.tobytes()), "d.weight_scale": ("F32", sc.shape, sc.tobytes()), "d.comfy_quant": ("U8", (2,), b"{}")})
+    got = node("import { SafeTensors } from './weights.mjs'; import fs from 'fs';"
+               "const gpu = { empty: (s, d) => ({ bytes: Buffer.alloc(s[0] * s[1] * (d === 'bf16' ? 2 : 4)), dtype: d, release() {} }),"
+               " write(t, a, off) { Buffer.from(a.buffer, a.byteOffset, a.byteLength).copy(t.bytes, off || 0); } };"
+               f"const st = SafeTensors.open({json.dumps(path)});"
+               "(async () => { const r = {}; for (const n of ['a', 'b', 'c', 'd']) { const t = await st.table(gpu, n + '.weight');"
+               f" fs.writeFileSync({json.dumps(str(tmp_path))} + '/' + n, t.buf.bytes); r[n] = [t.kind, t.N, t.K, t.buf.dtype]; }}"
+               " console.log(JSON.stringify(r)); })();")
+    assert got == {"a": ["bf16", 5000, 8, "bf16"], "b": ["f32", 5000, 8, "f32"], "c": ["f32", 5000, 8, "f32"], "d": ["f32", 4097, 8, "f32"]}
+    np.testing.assert_array_equal(np.fromfile(tmp_path / "a", np.uint16).reshape(v.shape), bf16(v))
+    np.testing.assert_array_equal(np.fromfile(tmp_path / "b", np.uint32), v.view(np.uint32).reshape(-1))
+    np.testing.assert_array_equal(np.fromfile(tmp_path / "c", np.float32).reshape(v.shape), half.astype(np.float32))
+    np.testing.assert_array_equal(np.fromfile(tmp_path / "d", np.float32).reshape(q.shape), (q.astype(np.float64) * sc[:, None]).astype(np.float32))
+
+
 # ------------------------------------------------------------------ on the device
 
 
