@@ -220,7 +220,7 @@ __device__ __forceinline__ void q4_leave4(const Q4Args& a, int64_t m, int n, f32
   *(f32x4_any*)((float*)a.out + m * a.ldc + n) = r;
 }
 
-// One to four rows on the vector units, in fp32: a wave takes U columns, a lane 16 consecutive k of each 1024 (eight bytes of
+// One to four rows (a group of blockIdx.y) on the vector units, in fp32: a wave takes U columns, a lane 16 consecutive k of each 1024 (eight bytes of
 // codes, one group).  x goes through LDS, quad j of lane l's 16 at [j][l], so that the reads touch every bank once.  A code with its
 // highest bit turned is c - 8 in two's complement: in a byte's upper half 16 (c - 8), one conversion away from a
 // float, and s takes the 16.
@@ -231,6 +231,12 @@ template <int MR, int U>
 __global__ __launch_bounds__(256) void q4_gemv_kernel(Q4Args a) {
   __shared__ f32x4 xs[2][MR][256];
   const int tid = threadIdx.x, lane = tid & 63, n0 = (blockIdx.x * 4 + (tid >> 6)) * U, KG = a.K / a.G, lg = 31 - __builtin_clz(a.G);
+  if (const int64_t m0 = (int64_t)blockIdx.y * MR) {  // this group's rows
+    a.x += m0 * a.ldx;
+    a.out = (char*)a.out + m0 * a.ldc * (a.obf ? 2 : 4);
+    if (a.add) a.add += m0 * a.ld_add;
+    a.M -= (int)m0;
+  }
   float acc[MR][U] = {};
   // the output that this lane ends with, if it has any
   int first = 0;
@@ -948,15 +954,16 @@ int embed_rows_launch(anima_ctx* c, const anima_weight* W, const int32_t* ids, i
   return L.end();
 }
 
-constexpr int Q4_ROWS = 4;         // rows of the vector kernel (four of 500 x 1024: 4.8 us, 9.2 by 32 x 32 tiles; of 8192 x 2048: 8.2 and 11.2)
 constexpr int Q4_FEW_LDS = 65536;  // that a launch may ask for
 
+static int q4_columns(const Q4Args& a) { return a.N >= 4096 ? 4 : a.N >= 2048 ? 2 : 1; }  // of a wave of the vector kernel
+
 static void q4_gemv(anima_ctx* c, const Q4Args& a) {
-#define GEMV(MR, U) hipLaunchKernelGGL((q4_gemv_kernel<MR, U>), dim3((unsigned)((a.N + 4 * U - 1) / (4 * U))), dim3(256), 0, c->stream, a)
+#define GEMV(MR, U) hipLaunchKernelGGL((q4_gemv_kernel<MR, U>), dim3((unsigned)((a.N + 4 * U - 1) / (4 * U)), (unsigned)((a.M + MR - 1) / MR)), dim3(256), 0, c->stream, a)
 #define GEMV_U(MR)                    \
   do {                                \
-    if (a.N >= 4096) GEMV(MR, 4);     \
-    else if (a.N >= 2048) GEMV(MR, 2); \
+    if (q4_columns(a) == 4) GEMV(MR, 4);     \
+    else if (q4_columns(a) == 2) GEMV(MR, 2); \
     else GEMV(MR, 1);                 \
   } while (0)
   if (a.M == 1) GEMV_U(1);
@@ -977,6 +984,26 @@ static void q4_tile_launch(anima_ctx* c, const Q4Tile& t, int splits) {
   hipLaunchKernelGGL((q4_tile_kernel<BM, BN, WM, WN, TERMS, NST>), grid, block, 0, c->stream, t);
 }
 
+// Up to 64 rows by 32 x 32 tiles, but two terms of more than 32 rows with many steps, where x is read once more for every 32 rows
+// (33 x 8192 x 4096: 29 us, 23 by the larger tiles; 64 x 4096 x 4096: 19 and 23).
+static bool q4_few(const Q4Args& a, bool two) {
+  const bool many = two && a.M > 32 && (a.K >= 8192 || (int64_t)a.N * a.K >= (int64_t)1 << 25);
+  return a.M <= 64 && !many && q4_few_lds(a) <= Q4_FEW_LDS;
+}
+
+// Whether the vector kernel, four rows a group, ends before the matrix kernels, by times in us that were fitted to 54 sizes: it takes a
+// launch, then a trip to memory for each 1024 of k or its share of the codes' conversions, once for every group; they take a
+// launch more, and k's steps one behind the other.  8 x 2048 x 1024: 5.8 us, 9.5 by 32 x 32 tiles (8 x 8192 x 2048: 13.2 and 11.2);
+// 1093 x 65 x 64: 5.0, 9.0 by tiles of 64 x 64.
+static bool q4_rows(const Q4Args& a, bool two) {
+  if (a.M <= 4) return true;
+  const int64_t groups = (a.M + 3) / 4;
+  if (groups > 65535) return false;
+  const int u = q4_columns(a);
+  const double k = a.K / 1024.0, work = (u == 4 ? 0.28 : u == 2 ? 0.42 : 0.55) * 1e-6 * (double)(groups * a.N) * a.K;
+  return 4.5 + std::max(1.24 * k, work) < (!q4_few(a, two) ? 8.5 : two ? 7.0 + 2.0 * k : 6.6 + 1.4 * k);
+}
+
 // x into f16 terms (and the columns' powers), then the products, then, where k was split, the sums.
 static int q4_matrix(anima_ctx* c, const Q4Args& a, bool two) {
   Q4Tile t{};
@@ -986,12 +1013,9 @@ static int q4_matrix(anima_ctx* c, const Q4Args& a, bool two) {
   t.ldp = t.Kp / 64 % 2 ? t.Kp : t.Kp + 64;
   t.ldn = (a.N + 3) / 4 * 4;
   const int KG = a.K / a.G, steps = t.Kp / 64;
-  // Up to 64 rows by 32 x 32 tiles, but two terms of more than 32 rows with many steps, where x is read once more for every 32 rows
-  // (33 x 8192 x 4096: 29 us, 23 by the tiles; 64 x 4096 x 4096: 19 and 23).
-  const bool many = two && a.M > 32 && (a.K >= 8192 || (int64_t)a.N * a.K >= (int64_t)1 << 25);
-  const bool few = a.M <= 64 && !many && q4_few_lds(a) <= Q4_FEW_LDS;
+  const bool few = q4_few(a, two);
   const auto tiles = [&](int bm, int bn) { return (int64_t)((a.M + bm - 1) / bm) * ((a.N + bn - 1) / bn); };
-  // The largest tile of which there are enough; the smallest ends soonest (K = 256 in one term, 2770 x 6019: 39 us, 59 by the largest),
+  // The largest tile of which there are enough and that the columns fill by more than half; the smallest ends soonest (K = 256 in one term, 2770 x 6019: 39 us, 59 by the largest),
   // the largest read x least (8192 x 8192 x 2048: two terms 587, 636, 888 us from the largest down, one term 337, 392, 513).
   // Where there are too few, parts of k: of 16 steps and more on the CUs' second places (two terms, 644 x 1695 x 6912:
   // 82 us whole, 62 in parts), of three and more while CUs are idle (202 x 122 x 1792: 24 and 14; a join takes 3 us and more).
@@ -999,9 +1023,9 @@ static int q4_matrix(anima_ctx* c, const Q4Args& a, bool two) {
   const int64_t cus = c->num_cus, t0 = tiles(rows, 256), t1 = tiles(rows, 128), t2 = tiles(64, 64);
   int tile = 2, splits = 1;
   if (few) {
-  } else if (t0 >= 2 * cus && (two ? steps >= 16 || t0 >= 4 * cus : steps >= 8)) {
+  } else if (a.N > 128 && t0 >= 2 * cus && (two ? steps >= 16 || t0 >= 4 * cus : steps >= 8)) {
     tile = 0;
-  } else if (two ? t1 >= cus : t1 >= 2 * cus && steps >= 8) {
+  } else if (a.N > 64 && (two ? t1 >= cus : t1 >= 2 * cus && steps >= 8)) {
     tile = 1;
   } else {
     if (two) {
@@ -1078,12 +1102,13 @@ int linear_q4_launch(anima_ctx* c, const anima_linear_desc* d) {
   Q4Args a{d->x, d->ldx ? d->ldx : W->K, (const uint8_t*)W->w, W->group_scale, W->group_mid, W->bias, d->out, d->ldc ? d->ldc : W->N,
            d->alpha != 0.0f ? d->alpha : 1.0f, d->act, d->epilogue, d->epilogue == ANIMA_EPI_GATED ? d->gate + d->gate_off : nullptr, d->add,
            d->ld_add ? d->ld_add : W->N, (int)d->M, W->N, W->K, W->group, d->out_bf16};
-  if (a.M <= Q4_ROWS) {
+  const bool two = d->precision == ANIMA_PREC_FP32;
+  if (q4_rows(a, two)) {
     Launch L(c, "gemv.q4", 2.0 * a.M * a.N * a.K, 0.5 * a.N * a.K);
     q4_gemv(c, a);
     return L.end();
   }
-  return q4_matrix(c, a, d->precision == ANIMA_PREC_FP32);
+  return q4_matrix(c, a, two);
 }
 
 }  // namespace anima

@@ -82,7 +82,10 @@ SHAPES = [(1, 1, 32, 32), (1, 5, 64, 64), (1, 1000, 1024, 64), (1, 4096, 256, 12
           (4, 129, 1440, 32), (5, 64, 128, 64), (7, 333, 4096, 64), (8, 100, 1184, 32), (9, 65, 320, 64), (15, 1024, 512, 128),
           (16, 48, 32, 32), (17, 70, 64, 64), (31, 257, 1056, 32), (33, 127, 384, 128), (43, 1024, 2048, 64), (64, 96, 8192, 128),
           (65, 514, 96, 32), (100, 300, 640, 64), (127, 129, 1088, 64), (128, 128, 256, 32), (129, 260, 160, 32), (200, 1000, 512, 128),
-          (257, 513, 288, 32), (300, 64, 4160, 64), (515, 516, 1440, 32), (1024, 384, 128, 128)]
+          (257, 513, 288, 32), (300, 64, 4160, 64), (515, 516, 1440, 32), (1024, 384, 128, 128),
+          # (products that the matrix kernels take: the smaller ones above are the vector kernel's)
+          (14, 2668, 4032, 32), (31, 2101, 1056, 32), (64, 1025, 1184, 32), (48, 1500, 2176, 128), (20, 2050, 2112, 64), (129, 2260, 160, 32),
+          (257, 1513, 288, 32), (66, 1031, 2048, 128), (130, 700, 1056, 32)]
 
 
 @pytest.mark.parametrize("precision", [0, 1], ids=["bf16", "fp32"])
@@ -103,8 +106,9 @@ def test_products(ctx, M, N, K, g, mid, precision):
 @pytest.mark.parametrize("precision,M,N,K,g,mid,name", [
     (1, 1025, 4092, 288, 32, True, "gemm.q4.128"), (1, 515, 3700, 1312, 32, True, "gemm.q4.128"), (0, 2050, 3900, 320, 64, True, "gemm.q4.64"),
     (0, 1030, 3600, 1152, 128, False, "gemm.q4.64"), (1, 2049, 4092, 1056, 32, True, "gemm.q4.256"), (0, 4100, 3901, 544, 32, True, "gemm.q4.256"),
-    (0, 2050, 3901, 576, 64, False, "gemm.q4.128"), (1, 640, 1701, 4160, 64, True, "gemm.q4.128"), (0, 640, 1701, 4160, 64, True, "gemm.q4.64"), (1, 70, 260, 256, 64, True, "gemm.q4.64"), (0, 300, 64, 4160, 64, True, "gemm.q4.64"),
-    (1, 20, 40, 16416, 32, True, "gemm.q4.64"), (1, 20, 40, 8224, 32, False, "gemm.q4.few"), (0, 64, 300, 1024, 64, True, "gemm.q4.few"), (1, 40, 100, 8192, 128, True, "gemm.q4.64"),
+    (0, 2050, 3901, 576, 64, False, "gemm.q4.128"), (1, 640, 1701, 4160, 64, True, "gemm.q4.128"), (0, 640, 1701, 4160, 64, True, "gemm.q4.64"), (1, 70, 260, 256, 64, True, "gemv.q4"), (1, 70, 2600, 256, 64, True, "gemm.q4.64"), (0, 300, 64, 4160, 64, True, "gemm.q4.64"),
+    (1, 20, 40, 16416, 32, True, "gemm.q4.64"), (1, 20, 40, 8224, 32, False, "gemv.q4"), (0, 64, 300, 1024, 64, True, "gemv.q4"), (1, 20, 2700, 8224, 32, False, "gemm.q4.few"),
+    (0, 64, 1300, 1024, 64, True, "gemm.q4.few"), (0, 5000, 65, 64, 32, True, "gemv.q4"), (1, 300000, 3, 32, 32, False, "gemm.q4.64"), (1, 40, 100, 8192, 128, True, "gemm.q4.64"),
     (1, 4, 300, 1024, 64, True, "gemv.q4")])
 def test_variants(ctx, precision, M, N, K, g, mid, name):
     """Each kernel by its profiler name, at ragged sizes, with an activation and bf16 rows."""
@@ -124,11 +128,11 @@ def test_variants(ctx, precision, M, N, K, g, mid, name):
 @pytest.mark.parametrize("epi,act,add,alpha,out_bf16", [
     (0, "none", False, 0.0, True), (0, "gelu", False, 0.0, True), (0, "silu", True, 0.5, False), (0, "gelu", True, 0.0, False),
     (1, "none", False, 0.0, False), (1, "silu", True, -2.0, False), (2, "none", False, 0.0, False), (2, "gelu", True, 0.25, False)])
-@pytest.mark.parametrize("N,ragged", [(132, False), (67, True), (256, True)])
-def test_epilogues(ctx, M, epi, act, add, alpha, out_bf16, N, ragged):
+@pytest.mark.parametrize("N,ragged,K", [(132, False, 224), (67, True, 224), (256, True, 224), (2668, False, 1056), (2667, True, 1056)])
+def test_epilogues(ctx, M, epi, act, add, alpha, out_bf16, N, ragged, K):
     """Every epilogue, with rows of out, add and x further apart than they are wide, and gate and buffers at odd offsets."""
     m = amd()
-    K, g = 224, 32
+    g = 32
     rng = np.random.default_rng(M + N)
     W = Q4(ctx, rng, N, K, g, True, bias=rng.normal(0, 1, N).astype(np.float32))
     ldx, ldc, lda, goff = (K + 8, N + 3, N + 1, 5) if ragged else (K, N, N, 0)
@@ -158,7 +162,7 @@ def test_epilogues(ctx, M, epi, act, add, alpha, out_bf16, N, ragged):
         np.testing.assert_array_equal(got[:, N:], widen(bf16(before))[:, N:] if out_bf16 else before[:, N:])
 
 
-@pytest.mark.parametrize("M,N,K", [(1, 200, 512), (12, 200, 512), (80, 200, 512), (300, 520, 512)])
+@pytest.mark.parametrize("M,N,K", [(1, 200, 512), (12, 200, 512), (80, 200, 512), (300, 520, 512), (12, 2700, 2048), (80, 900, 2048)])
 @pytest.mark.parametrize("g", [32, 64, 128])
 @pytest.mark.parametrize("rows", ["tiny", "huge", "one", "zero", "mixed"])
 def test_ranges_of_rows(ctx, M, N, K, g, rows):
@@ -182,7 +186,7 @@ def test_ranges_of_rows(ctx, M, N, K, g, rows):
     assert np.all(err <= tol), (err / np.maximum(tol, 1e-300)).max()
 
 
-@pytest.mark.parametrize("M,N,K", [(1, 70, 256), (12, 70, 256), (80, 200, 256), (300, 300, 256)])
+@pytest.mark.parametrize("M,N,K", [(1, 70, 256), (12, 70, 256), (80, 200, 256), (300, 300, 256), (24, 2100, 1024), (80, 900, 1024)])
 def test_outliers_and_small_scales(ctx, M, N, K):
     """One activation 10^4 times the rest, and groups whose scales are 2^20 apart within a column: the parts beside the large
     ones count with 2^-24 of the row's largest magnitude times the column's."""
@@ -203,11 +207,10 @@ def test_outliers_and_small_scales(ctx, M, N, K):
     assert np.all(err <= tol), (err / tol).max()
 
 
-@pytest.mark.parametrize("M", [1, 6, 40, 200])
+@pytest.mark.parametrize("M,N,K", [(1, 150, 192), (6, 150, 192), (40, 150, 192), (200, 150, 192), (24, 2100, 1024), (200, 900, 1024)])
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
-def test_rows_that_are_not_finite(ctx, M, bad):
+def test_rows_that_are_not_finite(ctx, M, N, K, bad):
     """A row of x with a NaN or an infinity gives NaN or infinities; no other row changes."""
-    N, K = 150, 192
     rng = np.random.default_rng(9)
     W = Q4(ctx, rng, N, K, 64, True)
     x = rng.normal(0, 1, (M, K)).astype(np.float32)
@@ -224,10 +227,9 @@ def test_rows_that_are_not_finite(ctx, M, bad):
     np.testing.assert_array_equal(got[keep], good[keep])
 
 
-@pytest.mark.parametrize("M", [1, 5, 50, 300])
-def test_rows_do_not_depend_on_their_neighbours(ctx, M):
+@pytest.mark.parametrize("M,N,K", [(1, 260, 512), (5, 260, 512), (50, 260, 512), (300, 260, 512), (50, 2100, 1024), (17, 4100, 2048)])
+def test_rows_do_not_depend_on_their_neighbours(ctx, M, N, K):
     """The same row twice in a batch gives the same bits, and a batch gives the same bits twice."""
-    N, K = 260, 512
     rng = np.random.default_rng(4)
     W = Q4(ctx, rng, N, K, 64, True)
     x = rng.normal(0, 1, (M, K)).astype(np.float32)
@@ -247,10 +249,9 @@ def test_no_rows(ctx):
     assert (out.numpy() == 7.0).all()
 
 
-@pytest.mark.parametrize("M", [1, 24, 160, 300])
-def test_replayed_from_a_graph(ctx, M):
+@pytest.mark.parametrize("M,N,K", [(1, 384, 1024), (24, 384, 1024), (160, 384, 1024), (300, 384, 1024), (24, 2100, 1024), (200, 300, 4096)])
+def test_replayed_from_a_graph(ctx, M, N, K):
     """A captured product, replayed several times with other work and other inputs between the replays."""
-    N, K = 384, 1024
     rng = np.random.default_rng(2)
     W = Q4(ctx, rng, N, K, 64, True)
     xs = [rng.normal(0, 1, (M, K)).astype(np.float32) for _ in range(3)]
