@@ -991,17 +991,16 @@ static bool q4_few(const Q4Args& a, bool two) {
   return a.M <= 64 && !many && q4_few_lds(a) <= Q4_FEW_LDS;
 }
 
-// Whether the vector kernel, four rows a group, ends before the matrix kernels, by times in us that were fitted to 54 sizes: it takes a
-// launch, then a trip to memory for each 1024 of k or its share of the codes' conversions, once for every group; they take a
-// launch more, and k's steps one behind the other.  8 x 2048 x 1024: 5.8 us, 9.5 by 32 x 32 tiles (8 x 8192 x 2048: 13.2 and 11.2);
-// 1093 x 65 x 64: 5.0, 9.0 by tiles of 64 x 64.
+// Whether the vector kernel, four rows a group, ends before the matrix kernels, by times in us that were fitted to 70 sizes: it takes a
+// launch, then a trip to memory for each 1024 of k, or its workgroups' shares (a start, and for each 1024 of k the rows of x and the
+// columns' codes); they take a launch more, and k's steps one behind the other.  8 x 2048 x 1024: 5.8 us, 9.5 by 32 x 32 tiles
+// (8 x 8192 x 2048: 13.2 and 11.2); 100 x 100 x 512: 5.5, 10.4 by tiles of 64 x 64 (1093 x 65 x 64: 20.8 and 8.6).
 static bool q4_rows(const Q4Args& a, bool two) {
   if (a.M <= 4) return true;
-  const int64_t groups = (a.M + 3) / 4;
+  const int64_t groups = (a.M + 3) / 4, u = q4_columns(a), wgs = (a.N + 4 * u - 1) / (4 * u) * groups;
   if (groups > 65535) return false;
-  const int u = q4_columns(a);
-  const double k = a.K / 1024.0, work = (u == 4 ? 0.28 : u == 2 ? 0.42 : 0.55) * 1e-6 * (double)(groups * a.N) * a.K;
-  return 4.5 + std::max(1.24 * k, work) < (!q4_few(a, two) ? 8.5 : two ? 7.0 + 2.0 * k : 6.6 + 1.4 * k);
+  const double k = a.K / 1024.0, turns = (a.K + 1023) / 1024, work = 1e-3 * (double)wgs * (1.6 + turns * (1.27 + 0.63 * (double)u));
+  return 4.0 + std::max(1.24 * turns, work) < (!q4_few(a, two) ? 8.5 : two ? 7.0 + 2.0 * k : 6.6 + 1.4 * k);
 }
 
 // x into f16 terms (and the columns' powers), then the products, then, where k was split, the sums.

@@ -107,8 +107,8 @@ def test_products(ctx, M, N, K, g, mid, precision):
     (1, 1025, 4092, 288, 32, True, "gemm.q4.128"), (1, 515, 3700, 1312, 32, True, "gemm.q4.128"), (0, 2050, 3900, 320, 64, True, "gemm.q4.64"),
     (0, 1030, 3600, 1152, 128, False, "gemm.q4.64"), (1, 2049, 4092, 1056, 32, True, "gemm.q4.256"), (0, 4100, 3901, 544, 32, True, "gemm.q4.256"),
     (0, 2050, 3901, 576, 64, False, "gemm.q4.128"), (1, 640, 1701, 4160, 64, True, "gemm.q4.128"), (0, 640, 1701, 4160, 64, True, "gemm.q4.64"), (1, 70, 260, 256, 64, True, "gemv.q4"), (1, 70, 2600, 256, 64, True, "gemm.q4.64"), (0, 300, 64, 4160, 64, True, "gemm.q4.64"),
-    (1, 20, 40, 16416, 32, True, "gemm.q4.64"), (1, 20, 40, 8224, 32, False, "gemv.q4"), (0, 64, 300, 1024, 64, True, "gemv.q4"), (1, 20, 2700, 8224, 32, False, "gemm.q4.few"),
-    (0, 64, 1300, 1024, 64, True, "gemm.q4.few"), (0, 5000, 65, 64, 32, True, "gemv.q4"), (1, 300000, 3, 32, 32, False, "gemm.q4.64"), (1, 40, 100, 8192, 128, True, "gemm.q4.64"),
+    (1, 20, 40, 16416, 32, True, "gemm.q4.64"), (1, 20, 40, 8224, 32, False, "gemv.q4"), (0, 64, 300, 1024, 64, True, "gemm.q4.few"), (1, 20, 2700, 8224, 32, False, "gemm.q4.few"),
+    (0, 64, 1300, 1024, 64, True, "gemm.q4.few"), (0, 5000, 65, 64, 32, True, "gemm.q4.64"), (0, 100, 101, 512, 32, True, "gemv.q4"), (1, 300000, 3, 32, 32, False, "gemm.q4.64"), (1, 40, 100, 8192, 128, True, "gemm.q4.64"),
     (1, 4, 300, 1024, 64, True, "gemv.q4")])
 def test_variants(ctx, precision, M, N, K, g, mid, name):
     """Each kernel by its profiler name, at ragged sizes, with an activation and bf16 rows."""
