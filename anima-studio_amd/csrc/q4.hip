@@ -352,11 +352,13 @@ struct Q4Prep {
                   // or (frag) as the 32 x 32 x 16 products take them: [rows / 32][Kp / 16][k / 8 % 2][row % 32][8]
   _Float16* xl;   // the second terms, or NULL
   float* rm;      // [M] what x's power comes off with
-  float* sx;      // [M][K/G] group sums of x, or NULL
+  bf16* sx;       // [3][M][KGp] group sums of x with x's power, three terms each, or NULL
+  bf16* zp;       // [N][KGp] the middles with the column's power, zeros from K / G on
   const uint16_t* gs;
+  const uint16_t* gz;
   float* rn;      // [N] what the column's power comes off with
   int64_t ldp;    // values between the terms' rows
-  int M, N, K, Kp, G, rows;  // rows: workgroups of x rows (four each), the rest are of columns
+  int M, N, K, Kp, G, KGp, rows;  // rows: workgroups of x rows (four each), the rest are of columns
   int frag;
 };
 
@@ -372,7 +374,15 @@ __global__ __launch_bounds__(256) void q4_prep_kernel(Q4Prep a) {
     float m = 0.0f;
     for (int g = lane; g < KG; g += 64) m = fmaxf(m, fabsf(bf16_f(a.gs[n * KG + g])));
     m = wave_max(m);
-    if (lane == 0) a.rn[n] = pow2f(-q4_exp(m, 11));
+    int e = a.rn ? q4_exp(m, 11) : 0;
+    if (a.zp) {
+      float mz = 0.0f;
+      for (int g = lane; g < KG; g += 64) mz = fmaxf(mz, fabsf(bf16_f(a.gz[n * KG + g])));
+      mz = wave_max(mz);
+      if (a.rn && mz != 0.0f) e = min(e, q4_exp(mz, 100));  // (middles of 2^107 scales: these have nothing to add)
+      for (int g = lane; g < a.KGp; g += 64) a.zp[n * a.KGp + g] = to_bf16(g < KG ? bf16_f(a.gz[n * KG + g]) * pow2f(e) : 0.0f);
+    }
+    if (a.rn && lane == 0) a.rn[n] = pow2f(-e);
     return;
   }
   const int64_t m = (int64_t)blockIdx.x * 4 + wave;
@@ -394,7 +404,15 @@ __global__ __launch_bounds__(256) void q4_prep_kernel(Q4Prep a) {
     if (a.sx) {
       float t = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
       for (int s = 1; s < a.G / 8; s <<= 1) t += __shfl_xor(t, s);
-      if (k < a.K && k % a.G == 0) a.sx[m * (a.K / a.G) + k / a.G] = t;
+      if (k < a.K && k % a.G == 0) {
+        t *= f;
+#pragma unroll
+        for (int c = 0; c < 3; c++) {
+          const bf16 b = to_bf16(t);
+          a.sx[((int64_t)c * a.M + m) * a.KGp + k / a.G] = b;
+          t -= (float)b;
+        }
+      }
     }
     f16x8 h, l;
 #pragma unroll
@@ -410,6 +428,9 @@ __global__ __launch_bounds__(256) void q4_prep_kernel(Q4Prep a) {
       if (a.xl) *(f16x8*)(a.xl + at) = l;
     }
   };
+  if (a.sx && a.K / a.G + lane < a.KGp)
+#pragma unroll
+    for (int c = 0; c < 3; c++) a.sx[((int64_t)c * a.M + m) * a.KGp + a.K / a.G + lane] = (bf16)0.0f;
   float mx = 0.0f;
   if constexpr (NV > 0) {
     float v[NV][8];
@@ -479,9 +500,10 @@ struct Q4Tile {
   const _Float16* xl;
   const float* rm;
   const float* rn;   // (readable to the next multiple of 256 columns)
-  const float* sx;
+  const bf16* sx;    // (as q4_prep_kernel leaves them)
+  const bf16* zp;
   float* part;       // [splits][M][ldn] sums of a product split over k, or NULL
-  int Kp, sps;       // k padded; steps of 64 k in a split
+  int Kp, KGp, sps;  // k padded, groups padded to 16; steps of 64 k in a split
   int ldp;           // values between the terms' rows
   int ldn;           // N to the next multiple of 4
   int svec;          // four steps' scales are one aligned piece of a row
@@ -504,15 +526,13 @@ __global__ __launch_bounds__(64 * QF_WAVES, 2) void q4_few_kernel(Q4Tile q) {
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 31, hf = lane >> 5;
   const int n0 = blockIdx.x * 32, m0 = blockIdx.y * 32, KG = a.K / a.G, steps = q.Kp / 64;
   float* const ss = (float*)smem;  // [KG][32]
-  float* const zs = ss + KG * 32;  // the middles, where there are
-  // a step's operands: codes 32 hf .. + 31 of column r; x's 16 i + 8 hf .. + 7 of row r; the groups' sums of x
+  // a step's operands: codes 32 hf .. + 31 of column r; x's 16 i + 8 hf .. + 7 of row r
   struct Step {
     u32x4 w;
     f16x8 x[TERMS][4];
-    float sx[NG];
   } st[2];
   const uint8_t* wr = a.w + (int64_t)min(n0 + r, a.N - 1) * (a.K / 2);
-  const int64_t mr = min(m0 + r, a.M - 1), so = mr * KG;
+  const int64_t mr = min(m0 + r, a.M - 1);
   const float rm = q.rm[mr];  // (a power of two)
   const int64_t xo = (int64_t)blockIdx.y * 32 * q.Kp + lane * 8;
   const auto load = [&](Step& v, int step) __attribute__((always_inline)) {  // (past the last step: that one again, unused)
@@ -523,9 +543,6 @@ __global__ __launch_bounds__(64 * QF_WAVES, 2) void q4_few_kernel(Q4Tile q) {
       v.x[0][i] = *(const f16x8*)(q.xh + xo + (k + 16 * i) * 32);
       if (TERMS > 1) v.x[TERMS - 1][i] = *(const f16x8*)(q.xl + xo + (k + 16 * i) * 32);
     }
-    if (a.gz)
-#pragma unroll
-      for (int g = 0; g < NG; g++) v.sx[g] = q.sx[so + min((k + 32 * g) / a.G, KG - 1)];
   };
   load(st[0], wave);
   load(st[1], wave + QF_WAVES);
@@ -537,25 +554,17 @@ __global__ __launch_bounds__(64 * QF_WAVES, 2) void q4_few_kernel(Q4Tile q) {
   {
     const int64_t col = (int64_t)min(n0 + (tid >> 4), a.N - 1) * KG;
     for (int g0 = tid & 15; g0 < KG; g0 += 64) {
-      uint16_t s[4], z[4];
+      uint16_t s[4];
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int64_t at = col + min(g0 + 16 * i, KG - 1);
-        s[i] = a.gs[at];
-        z[i] = a.gz ? a.gz[at] : 0;
-      }
+      for (int i = 0; i < 4; i++) s[i] = a.gs[col + min(g0 + 16 * i, KG - 1)];
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        if (g0 + 16 * i < KG) {
-          ss[(g0 + 16 * i) * 32 + (tid >> 4)] = bf16_f(s[i]);
-          if (a.gz) zs[(g0 + 16 * i) * 32 + (tid >> 4)] = bf16_f(z[i]);
-        }
+        if (g0 + 16 * i < KG) ss[(g0 + 16 * i) * 32 + (tid >> 4)] = bf16_f(s[i]);
     }
   }
   __builtin_amdgcn_s_waitcnt(0xc07f);
   q4_barrier();
   f32x16 acc = {};
-  const float up = 1.0f / rm;
   const f16x2 one = {(_Float16)1.0f, (_Float16)1.0f}, one16 = {(_Float16)0.0625f, (_Float16)0.0625f};
   const Q4Bits bits;
   const auto product = [&](const Step& v, int step) __attribute__((always_inline)) {
@@ -580,21 +589,24 @@ __global__ __launch_bounds__(64 * QF_WAVES, 2) void q4_few_kernel(Q4Tile q) {
 #pragma unroll
     for (int g = 0; g < NG; g++) {
       const int at = min((64 * step + 32 * g) / a.G, KG - 1) * 32 + 4 * hf;
-      // (a group of 128 meets its middle once; past K there is none)
-      const float sx = (G32 ? 64 * step + 32 * g < a.K : (64 * step) % a.G == 0) ? v.sx[g] * up : 0.0f;
 #pragma unroll
       for (int c = 0; c < 4; c++) {
         const f32x4 s = *(const f32x4*)(ss + at + 8 * c);
 #pragma unroll
         for (int e = 0; e < 4; e++) acc[4 * c + e] = __builtin_fmaf(part[g][4 * c + e], s[e], acc[4 * c + e]);
-        if (a.gz) {
-          const f32x4 z = *(const f32x4*)(zs + at + 8 * c);
-#pragma unroll
-          for (int e = 0; e < 4; e++) acc[4 * c + e] = __builtin_fmaf(z[e], sx, acc[4 * c + e]);
-        }
       }
     }
   };
+  // the middles' part: sixteen groups a wave
+  if (a.gz)
+    for (int g = 16 * wave; g < q.KGp; g += 16 * QF_WAVES) {
+      bf16x8 xs[3];
+      const bf16x8 z = *(const bf16x8*)(q.zp + (int64_t)min(n0 + r, a.N - 1) * q.KGp + g + 8 * hf);
+#pragma unroll
+      for (int c = 0; c < 3; c++) xs[c] = *(const bf16x8*)(q.sx + ((int64_t)c * a.M + mr) * q.KGp + g + 8 * hf);
+#pragma unroll
+      for (int c = 2; c >= 0; c--) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(z, xs[c], acc, 0, 0, 0);
+    }
   for (int s = wave; s < steps; s += 2 * QF_WAVES) {
     product(st[0], s);
     load(st[0], s + 2 * QF_WAVES);
@@ -733,46 +745,33 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void q4_tile_kernel(
 #pragma unroll
     for (int j = 0; j < NT; j++) acc[i][j] = f32x16{};
   scales(0);
+  // The middles' part: z in bf16, the groups' sums of x as three bf16 terms, sixteen groups a matrix step, dealt to the parts of k.  The
+  // first are asked for before the copies that the loop waits for.  (515 x 1316 x 1440 in groups of 32: 20.2 us without middles, 22.5
+  // with them, 25.0 where every tile cut its rows' sums into terms and took all of them in the first part.)
+  const int mids = a.gz ? t.KGp / 16 : 0;
+  int mid = blockIdx.y;
+  bf16x8 zf[NT], xs[MT][3];
+  const auto ask_mids = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < NT; j++) zf[j] = *(const bf16x8*)(t.zp + (int64_t)min(bn + wn + 32 * j + r, a.N - 1) * t.KGp + 16 * mid + 8 * hf);
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+      for (int c = 0; c < 3; c++)
+        xs[i][c] = *(const bf16x8*)(t.sx + ((int64_t)c * a.M + min(bm + wm + 32 * i + r, a.M - 1)) * t.KGp + 16 * mid + 8 * hf);
+  };
+  if (mid < mids) ask_mids();
 #pragma unroll
   for (int p = 1; p < NST; p++) copies(p, p * SB);
-  // The middles' part (with the first split): z in bf16 as it is, the groups' sums of x as three bf16 terms, sixteen groups a
-  // matrix step, both with the powers that the sums to come have.
-  if (a.gz && blockIdx.y == 0) {
-    for (int g0 = 0; g0 < KG; g0 += 16) {
-      bf16x8 zf[NT], xs[MT][3];
+  while (mid < mids) {
 #pragma unroll
-      for (int j = 0; j < NT; j++) {
-        const uint16_t* zr = a.gz + (int64_t)min(bn + wn + 32 * j + r, a.N - 1) * KG;
+    for (int c = 2; c >= 0; c--)
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const int g = g0 + 8 * hf + e;
-          const float z = bf16_f(zr[min(g, KG - 1)]);
-          zf[j][e] = to_bf16(g < KG ? z * fn[j] : 0.0f);
-        }
-      }
+      for (int i = 0; i < MT; i++)
 #pragma unroll
-      for (int i = 0; i < MT; i++) {
-        const int m = min(bm + wm + 32 * i + r, a.M - 1);
-        const float up = 1.0f / t.rm[m];
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const int g = g0 + 8 * hf + e;
-          float v = t.sx[(int64_t)m * KG + min(g, KG - 1)] * up;
-          v = g < KG ? v : 0.0f;
-#pragma unroll
-          for (int c = 0; c < 3; c++) {
-            xs[i][c][e] = to_bf16(v);
-            v -= (float)xs[i][c][e];
-          }
-        }
-      }
-#pragma unroll
-      for (int c = 2; c >= 0; c--)
-#pragma unroll
-        for (int i = 0; i < MT; i++)
-#pragma unroll
-          for (int j = 0; j < NT; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(zf[j], xs[i][c], acc[i][j], 0, 0, 0);
-    }
+        for (int j = 0; j < NT; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(zf[j], xs[i][c], acc[i][j], 0, 0, 0);
+    mid += gridDim.y;
+    if (mid < mids) ask_mids();
   }
   int xa[4];  // unit 4 hf + i of row r
 #pragma unroll
@@ -973,9 +972,9 @@ static void q4_gemv(anima_ctx* c, const Q4Args& a) {
 #undef GEMV
 }
 
-// LDS of the kernel for few rows: the scales and middles, then the waves' sums
+// LDS of the kernel for few rows: the scales, then the waves' sums
 static int64_t q4_few_lds(const Q4Args& a) {
-  return std::max<int64_t>((int64_t)(a.K / a.G) * 128 * (a.gz ? 2 : 1), QF_WAVES * 4096);
+  return std::max<int64_t>((int64_t)(a.K / a.G) * 128, QF_WAVES * 4096);
 }
 
 template <int BM, int BN, int WM, int WN, int TERMS, int NST>
@@ -1011,7 +1010,8 @@ static int q4_matrix(anima_ctx* c, const Q4Args& a, bool two) {
   // rows of the terms an odd number of lines of 128 bytes apart: at a power of two one step's rows meet in one memory channel
   t.ldp = t.Kp / 64 % 2 ? t.Kp : t.Kp + 64;
   t.ldn = (a.N + 3) / 4 * 4;
-  const int KG = a.K / a.G, steps = t.Kp / 64;
+  const int steps = t.Kp / 64;
+  t.KGp = (a.K / a.G + 15) / 16 * 16;
   const bool few = q4_few(a, two);
   const auto tiles = [&](int bm, int bn) { return (int64_t)((a.M + bm - 1) / bm) * ((a.N + bn - 1) / bn); };
   // The largest tile of which there are enough and that the columns fill by more than half; the smallest ends soonest (K = 256 in one term, 2770 x 6019: 39 us, 59 by the largest),
@@ -1049,22 +1049,23 @@ static int q4_matrix(anima_ctx* c, const Q4Args& a, bool two) {
     return o;
   };
   const size_t plane = (few ? (size_t)(a.M + 31) / 32 * 32 * t.Kp : (size_t)a.M * t.ldp) * 2, oh = take(plane), ol = two ? take(plane) : 0, om = take((size_t)a.M * 4),
-               on = few ? 0 : take(((size_t)a.N + 255) / 256 * 1024), os = a.gz ? take((size_t)a.M * KG * 4) : 0,
+               on = few ? 0 : take(((size_t)a.N + 255) / 256 * 1024), os = a.gz ? take((size_t)a.M * t.KGp * 6) : 0, oz = a.gz ? take((size_t)a.N * t.KGp * 2) : 0,
                op = splits > 1 ? take((size_t)splits * a.M * t.ldn * 4) : 0;
   void* tmp = nullptr;
   if (int rc = anima_alloc(c, at, &tmp)) return rc;
   char* const b = (char*)tmp;
-  Q4Prep p{a.x, a.ldx, (_Float16*)(b + oh), two ? (_Float16*)(b + ol) : nullptr, (float*)(b + om), a.gz ? (float*)(b + os) : nullptr, a.gs,
-           (float*)(b + on), t.ldp, a.M, a.N, a.K, t.Kp, a.G, (a.M + 3) / 4, few};
+  Q4Prep p{a.x, a.ldx, (_Float16*)(b + oh), two ? (_Float16*)(b + ol) : nullptr, (float*)(b + om), a.gz ? (bf16*)(b + os) : nullptr,
+           a.gz ? (bf16*)(b + oz) : nullptr, a.gs, a.gz, few ? nullptr : (float*)(b + on), t.ldp, a.M, a.N, a.K, t.Kp, a.G, t.KGp, (a.M + 3) / 4, few};
   t.xh = p.xh;
   t.xl = p.xl;
   t.rm = p.rm;
   t.rn = p.rn;
   t.sx = p.sx;
+  t.zp = p.zp;
   t.part = splits > 1 ? (float*)(b + op) : nullptr;
   Launch L(c, few ? "gemm.q4.few" : tile == 0 ? "gemm.q4.256" : tile == 1 ? "gemm.q4.128" : "gemm.q4.64", 2.0 * a.M * a.N * a.K, 0.0);
   {
-    const dim3 grid((unsigned)(p.rows + (few ? 0 : (a.N + 3) / 4))), block(256);
+    const dim3 grid((unsigned)(p.rows + (few && !a.gz ? 0 : (a.N + 3) / 4))), block(256);
     if (a.K <= 1024) hipLaunchKernelGGL(q4_prep_kernel<2>, grid, block, 0, c->stream, p);
     else if (a.K <= 2048) hipLaunchKernelGGL(q4_prep_kernel<4>, grid, block, 0, c->stream, p);
     else if (a.K <= 8192) hipLaunchKernelGGL(q4_prep_kernel<16>, grid, block, 0, c->stream, p);
