@@ -330,7 +330,7 @@ __global__ __launch_bounds__(256) void q4_gemv_kernel(Q4Args a) {
 // two f16 terms to 2^-23 of each value (or 2^-40 of the largest); ANIMA_PREC_BF16 keeps the first term, 11 bits.
 // s (c - 8), times a power of two for the whole column, is one f16 value: exact where it is above 2^-39 of the column's
 // largest.  Both powers come off the sums at the end, so the k loop has nothing but matrix products and the codes'
-// decode.  The middles' part, sum_g z[n][g] (sum of x over group g), is a small fp32 product of its own.
+// decode.  The middles' part, sum_g z[n][g] (sum of x over group g), is a small product of bf16 terms.
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -515,7 +515,7 @@ struct Q4Tile {
 // through LDS.  The codes stay whole numbers (exact in f16), and each group's sums meet their scale in fp32; scales and
 // middles lie in LDS as [group][column].  x comes from q4_prep_kernel in the order of the lanes (as rows, a load meets 32 lines
 // and takes the address unit four times as long).  Bound by trips to memory, of which each wave has two steps' under way (four:
-// no faster): 43 x 1024 x 2048 10 us, behind 4.3 for x.
+// no faster): 43 x 1024 x 2048 7.7 us, behind 4.8 for x.
 constexpr int QF_WAVES = 8;
 
 template <int TERMS, bool G32>
@@ -637,7 +637,11 @@ __global__ __launch_bounds__(64 * QF_WAVES, 2) void q4_few_kernel(Q4Tile q) {
 // u ^ (row / 2 % 8) (sixteen rows' reads of one unit touch each bank once).  Lane (n, half) takes the 16 bytes of column n's 32 k of
 // its half, so that matrix step i of a lane pair covers k 8 i .. 8 i + 7 of both halves; x's units follow.  The scales of four
 // steps come in one load where rows of them allow it: each of a lane's own addresses costs the address unit as
-// much as 64 neighbouring bytes.
+// much as 64 neighbouring bytes.  The LDS is held to half of a CU's (three stages for the largest tiles), so that one workgroup's
+// first copies and its epilogue pass under another's products: 8192 x 8192 x 2048, one term, gelu, 354 us by 256 x 256 tiles alone on
+// their CU and 336 by two of 128 x 256 (820 TFLOP/s; a library product of f16 matrices reaches 1110).  The matrix cores are busy 42 %
+// of the cycles at 1.8 GHz, the vector instructions (decode and gelu) take nearly as many.  2048 x 4096 x 1024 in two terms: 48 us,
+// one round of tiles, of whose time the k loop takes 30 and the start and the epilogue the rest.
 template <int BM, int BN, int WM, int WN, int TERMS, int NST>
 __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void q4_tile_kernel(Q4Tile t) {
   constexpr int NWM = BM / WM, NW = NWM * (BN / WN), MT = WM / 32, NT = WN / 32;
