@@ -410,13 +410,14 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_bf16(PrefixArgs 
       }
     }
     if constexpr (decltype(masked)::value) {
+      if (__builtin_amdgcn_ballot_w64(lo > k0 || hi < k0 + PBK)) {
+        const uint32_t at = k0 + 4 * hf - lo, n = hi - lo;  // (below lo: a large number)
 #pragma unroll
-      for (int t = 0; t < 2; t++)
+        for (int t = 0; t < 2; t++)
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-          const int k = k0 + 32 * t + 8 * (e >> 2) + 4 * hf + (e & 3);
-          if (k < lo || k >= hi) s[t][e] = -INFINITY;
-        }
+          for (int e = 0; e < 16; e++)
+            if (at + (32 * t + 8 * (e >> 2) + (e & 3)) >= n) s[t][e] = -INFINITY;
+      }
     }
     float bm = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
@@ -695,10 +696,11 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_fp32(PrefixArgs 
     if (cutting) cut(j + 1);
     if (i0 + (j >> 1) >= B.full) {
       const int lo = pre ? 0 : range.x, hi = pre ? a.P : range.y;
+      if (__builtin_amdgcn_ballot_w64(lo > k0 || hi < k0 + 32)) {
+        const uint32_t at = k0 + 4 * hf - lo, n = hi - lo;
 #pragma unroll
-      for (int e = 0; e < 16; e++) {
-        const int k = k0 + 8 * (e >> 2) + 4 * hf + (e & 3);
-        if (k < lo || k >= hi) s[e] = -INFINITY;
+        for (int e = 0; e < 16; e++)
+          if (at + (8 * (e >> 2) + (e & 3)) >= n) s[e] = -INFINITY;
       }
     }
     float bm = s[0];
@@ -803,8 +805,8 @@ static int prefix_plan(const anima_ctx* c, bool bf, int longest, PrefixArgs& a) 
       const double block = !bf ? 6.0 : nw == 4 ? 1.2 : 1.4, start = bf ? 5.0 : 4.0, join = 2.0 + (double)s * a.Hkv * a.V * 1056 / 5e6;
       const double blocks = 0.5 * ((total + s - 1) / s) + 0.5 * total / s;  // (the longest part and the mean one)
       const double t = (double)rounds * (start + blocks * block) + (s > 1 ? join : 0.0);
-      // (one wave of rows whose blocks are all copied at its start: 2 rows behind 77 keys 15.1 us whole, 16.7 in three parts)
-      if (best_nw && (t >= best || (s > 1 && a.V <= 32 && total <= 3))) continue;
+      // (bf16, one wave of rows whose blocks are all copied at its start: 2 rows behind 77 keys 15.1 us whole, 16.7 in three parts)
+      if (best_nw && (t >= best || (bf && s > 1 && a.V <= 32 && total <= 3))) continue;
       best = t;
       best_nw = nw;
       a.nt = nt;
