@@ -230,7 +230,7 @@ __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a) {
 // Blocks are copied by buffer_load ... lds three ahead into four stages of LDS, so a barrier a block is all that waves share.
 // 7741 rows of 16 heads behind 4096 keys: 264 GFLOP in 273 us, 967 TFLOP/s; the matrix cores are busy 56 % of the cycles at the 1.67
 // GHz that the power limit leaves (a library product of 8192 x 8192 x 8192: 1150).  64 rows of 32 heads behind 8192: 33.6 MB of keys
-// in 19 us, a start of 2, twelve until the last block is there, and the sums' way out.
+// in 18 us, a start of 2, eleven until the last block is there, and the sums' way out.
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) void prefix_lds_t;
