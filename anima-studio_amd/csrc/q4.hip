@@ -178,8 +178,8 @@ __device__ __forceinline__ void q4_leave(const Q4Args& a, int64_t m, int n, floa
 }
 
 // The same for four columns from n (a multiple of 4) on, fewer at the row's end.  Rows may start anywhere: the memory takes 16 bytes
-// of any four columns at once (2770 x 6019 x 256 in one term: 94 us with aligned quads alone, a column at a time elsewhere,
-// 59 so by the same tiles).
+// of any four columns at once (2770 x 6019 x 256 in one term, a column at a time against so: 95 and 59 us by the largest tile,
+// 52 and 39 by the smallest).
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef __bf16 bf16x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
@@ -513,9 +513,9 @@ struct Q4Tile {
 //
 // A workgroup takes 32 columns and 32 rows, its eight waves every eighth step of 64 k each, their sums joined in order
 // through LDS.  The codes stay whole numbers (exact in f16), and each group's sums meet their scale in fp32; the scales lie
-// in LDS as [group][column].  x comes from q4_prep_kernel in the order of the lanes (as rows, a load meets 32 lines
-// and takes the address unit four times as long).  Bound by trips to memory, of which each wave has two steps' under way (four:
-// no faster): 43 x 1024 x 2048 7.7 us, behind 4.8 for x.
+// in LDS as [group][column], and the middles' part is a small product of its own.  x comes from q4_prep_kernel in the order of
+// the lanes (as rows, a load meets 32 lines and takes the address unit four times as long).  Bound by trips to memory, of which
+// each wave has two steps' under way (four: no faster): 43 x 1024 x 2048 7.7 us, behind 4.8 for x.
 constexpr int QF_WAVES = 8;
 
 template <int TERMS, bool G32>
