@@ -1075,6 +1075,11 @@ static int q4_matrix(anima_ctx* c, const Q4Args& a, bool two) {
     else if (a.K <= 8192) hipLaunchKernelGGL(q4_prep_kernel<16>, grid, block, 0, c->stream, p);
     else hipLaunchKernelGGL(q4_prep_kernel<0>, grid, block, 0, c->stream, p);
   }
+  if (hipPeekAtLastError() != hipSuccess) {  // (no product of terms that were not written)
+    const int rc = L.end();
+    anima_free(c, tmp);
+    return rc;
+  }
   if (few) {
     const dim3 grid((unsigned)((a.N + 31) / 32), (unsigned)((a.M + 31) / 32)), block(64 * QF_WAVES);
     const int lds = (int)q4_few_lds(a);
@@ -1098,6 +1103,13 @@ static int q4_matrix(anima_ctx* c, const Q4Args& a, bool two) {
   return rc;
 }
 
+static int q4_linear_part(anima_ctx* c, const Q4Args& a, bool two) {
+  if (!q4_rows(a, two)) return q4_matrix(c, a, two);
+  Launch L(c, "gemv.q4", 2.0 * a.M * a.N * a.K, 0.5 * a.N * a.K);
+  q4_gemv(c, a);
+  return L.end();
+}
+
 int linear_q4_launch(anima_ctx* c, const anima_linear_desc* d) {
   char msg[256];
   if (int rc = check_linear_q4(d, Q4Msg{msg, sizeof msg})) return refused(c, rc, msg);
@@ -1107,12 +1119,23 @@ int linear_q4_launch(anima_ctx* c, const anima_linear_desc* d) {
            d->alpha != 0.0f ? d->alpha : 1.0f, d->act, d->epilogue, d->epilogue == ANIMA_EPI_GATED ? d->gate + d->gate_off : nullptr, d->add,
            d->ld_add ? d->ld_add : W->N, (int)d->M, W->N, W->K, W->group, d->out_bf16};
   const bool two = d->precision == ANIMA_PREC_FP32;
-  if (q4_rows(a, two)) {
-    Launch L(c, "gemv.q4", 2.0 * a.M * a.N * a.K, 0.5 * a.N * a.K);
-    q4_gemv(c, a);
-    return L.end();
-  }
-  return q4_matrix(c, a, two);
+  const Q4Part part = q4_part(d->M, W->N);
+  for (int64_t n = 0; n < W->N; n += part.cols)
+    for (int64_t m = 0; m < d->M; m += part.rows) {
+      Q4Args p = a;
+      p.M = (int)std::min(part.rows, d->M - m);
+      p.N = (int)std::min(part.cols, W->N - n);
+      p.x += m * a.ldx;
+      p.w += n * (a.K / 2);
+      p.gs += n * (a.K / a.G);
+      if (a.gz) p.gz += n * (a.K / a.G);
+      if (a.bias) p.bias += n;
+      if (a.gate) p.gate += n;
+      if (a.add) p.add += m * a.ld_add + n;
+      p.out = (char*)a.out + (m * a.ldc + n) * (a.obf ? 2 : 4);
+      if (int rc = q4_linear_part(c, p, two)) return rc;
+    }
+  return ANIMA_OK;
 }
 
 }  // namespace anima

@@ -3,6 +3,7 @@
 // ANIMA_OK, writes the message.
 #pragma once
 
+#include <algorithm>
 #include <cstdint>
 #include <cstdio>
 
@@ -11,7 +12,7 @@
 namespace anima {
 
 constexpr int Q4_MAX_K = 1 << 20;         // of a product
-constexpr int Q4_MAX_SIDE = 1 << 29;      // rows and outputs of a product: a launch has fewer than 2^32 threads a dimension
+constexpr int Q4_MAX_SIDE = 1 << 29;      // rows and outputs of a product (cut into launches by q4_part)
 constexpr int64_t Q4_MAX_LDX = 1 << 22;   // floats between rows of a product's input: 64 rows of a tile stay below 2^31 bytes
 constexpr int64_t Q4_MAX_QUANT = (int64_t)1 << 34;  // weights of one conversion
 
@@ -28,6 +29,17 @@ struct Q4Msg {
     return code;
   }
 };
+
+// The largest part of a product of M rows and N columns that its kernels are launched for: a launch has fewer than 2^32 threads a
+// dimension, and the pass before takes 64 a row and a column, the kernels for few rows 16 a column, tiles of 64 x 64 one for 16
+// outputs.  Columns in whole pieces of 2^24, so that the parts' codes and scales are aligned as the whole's.
+struct Q4Part {
+  int64_t rows, cols;
+};
+inline Q4Part q4_part(int64_t M, int64_t N) {
+  const int64_t side = (int64_t)1 << 24, cols = std::min(N, side);
+  return {std::min(std::min(M, side), ((int64_t)1 << 35) / cols), cols};
+}
 
 inline bool q4_al(const void* p, int b) { return ((uintptr_t)p & (uintptr_t)(b - 1)) == 0; }
 inline bool q4_group(int g) { return g == 32 || g == 64 || g == 128; }
