@@ -327,10 +327,11 @@ __global__ __launch_bounds__(256) void q4_gemv_kernel(Q4Args a) {
 // ------------------------------------------------------------------ products of many rows
 //
 // On the f16 matrix cores.  A row of x, times a power of two that brings its largest value to 2^14 .. 2^15, is the sum of
-// two f16 terms to 2^-23 of each value (or 2^-40 of the largest); ANIMA_PREC_BF16 keeps the first term, 11 bits.
-// s (c - 8), times a power of two for the whole column, is one f16 value: exact where it is above 2^-39 of the column's
-// largest.  Both powers come off the sums at the end, so the k loop has nothing but matrix products and the codes'
-// decode.  The middles' part, sum_g z[n][g] (sum of x over group g), is a small product of bf16 terms.
+// two f16 terms to 2^-23 of each value (or 2^-39 of the largest); ANIMA_PREC_BF16 keeps the first term, 11 bits (or 2^-39).
+// s (c - 8), times a power of two for the whole column that brings its largest scale to 2^11 .. 2^12, is one f16 value: exact
+// for scales from 2^-28 of the largest on; a smaller one is off by at most 2^-36 of the largest.  Both powers come off the sums at
+// the end, so the k loop has nothing but matrix products and the codes' decode.  The middles' part, sum_g z[n][g] (sum of x
+// over group g), is a small product of bf16 terms.
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -457,19 +458,20 @@ __global__ __launch_bounds__(256) void q4_prep_kernel(Q4Prep a) {
   }
 }
 
-// Eight codes, times the scale pair s (s16: a 16th of it), in the order 0 4 1 5 2 6 3 7.  A code's bits in the mantissa of 1024 are 1024 +
-// c, four places further up 1024 + 16 c: less 1032, or 1152, (exact), times s, or s16.
+// Eight codes, times the scale pair s, in the order 0 4 1 5 2 6 3 7.  A code's bits in the mantissa of 1024 are 1024 + c, four places
+// further up 1024 + 16 c: less 1032, or a 16th of it less 72 in one instruction, is c - 8 exactly, and both meet the same s.
 struct Q4Bits {  // (in registers: an instruction takes one constant of its own, and v_and_or two)
   uint32_t even = 0x000f000fu, odd = 0x00f000f0u, big = 0x64006400u;
   __device__ __forceinline__ Q4Bits() { asm("" : "+s"(even), "+s"(odd), "+v"(big)); }
 };
-__device__ __forceinline__ f16x8 q4_decode(const Q4Bits& b, uint32_t c, f16x2 s, f16x2 s16) {
-  const f16x2 off = {(_Float16)-1032.0f, (_Float16)-1032.0f}, off16 = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+__device__ __forceinline__ f16x8 q4_decode(const Q4Bits& b, uint32_t c, f16x2 s) {
+  const f16x2 off = {(_Float16)-1032.0f, (_Float16)-1032.0f}, off16 = {(_Float16)-72.0f, (_Float16)-72.0f},
+              part = {(_Float16)0.0625f, (_Float16)0.0625f};
   f16x8 r;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     const f16x2 k = __builtin_bit_cast(f16x2, ((i < 2 ? c : c >> 8) & (i & 1 ? b.odd : b.even)) | b.big);
-    const f16x2 v = i & 1 ? (k + off16) * s16 : (k + off) * s;
+    const f16x2 v = (i & 1 ? __builtin_elementwise_fma(k, part, off16) : k + off) * s;
     r[2 * i] = v[0];
     r[2 * i + 1] = v[1];
   }
@@ -565,7 +567,7 @@ __global__ __launch_bounds__(64 * QF_WAVES, 2) void q4_few_kernel(Q4Tile q) {
   __builtin_amdgcn_s_waitcnt(0xc07f);
   q4_barrier();
   f32x16 acc = {};
-  const f16x2 one = {(_Float16)1.0f, (_Float16)1.0f}, one16 = {(_Float16)0.0625f, (_Float16)0.0625f};
+  const f16x2 one = {(_Float16)1.0f, (_Float16)1.0f};
   const Q4Bits bits;
   const auto product = [&](const Step& v, int step) __attribute__((always_inline)) {
     // the halves' words exchanged, so that matrix step i covers k 16 i .. 16 i + 15: lane half hf word 2 i + hf of 8
@@ -582,7 +584,7 @@ __global__ __launch_bounds__(64 * QF_WAVES, 2) void q4_few_kernel(Q4Tile q) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       f32x16& p = part[G32 ? i >> 1 : 0];
-      const f16x8 wf = q4_decode(bits, w[i < 2 ? 2 * i : 2 * i - 3], one, one16);
+      const f16x8 wf = q4_decode(bits, w[i < 2 ? 2 * i : 2 * i - 3], one);
 #pragma unroll
       for (int e = TERMS - 1; e >= 0; e--) p = __builtin_amdgcn_mfma_f32_32x32x16_f16(wf, v.x[e][i], p, 0, 0, 0);
     }
@@ -800,7 +802,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void q4_tile_kernel(
   };
   const auto decode = [&](int u, int q, int i) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < NT; j++) wf[u][j] = q4_decode(bits, wr[j][i], sv[q][j], sv[q][j] * (_Float16)0.0625f);
+    for (int j = 0; j < NT; j++) wf[u][j] = q4_decode(bits, wr[j][i], sv[q][j]);
   };
   pairs();
   Q4_WAIT_VM((NST - 1) * CPW);

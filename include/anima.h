@@ -513,7 +513,8 @@ typedef struct {
  * added, and so its last bits, depends on the sizes.  No acc_out and no LoRA factors (`add` carries a
  * delta).
  * q4: r = alpha * sum_k x[m][k] w[n][k] of fp32 rows x (16-byte aligned, ldx % 4 == 0), with the products of
- * 32-bit accuracy or, on more than a few rows and with ANIMA_PREC_BF16, of x rounded to 11 bits.  A row of x
+ * 32-bit accuracy or, on more than a few rows and with ANIMA_PREC_BF16, of x rounded to 11 bits.  A group_scale
+ * below 2^-28 of the largest of its output n may be off by 2^-36 of that largest.  A row of x
  * with an infinity or a NaN gives no finite value.  M and N up to 2^29, K up to 2^20; as f8 in the rest (pooled
  * scratch, the order of sums by the sizes, no acc_out and no LoRA factors). */
 int anima_linear(anima_ctx* ctx, const anima_linear_desc* desc);
