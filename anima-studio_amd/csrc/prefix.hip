@@ -226,7 +226,8 @@ __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a) {
 // Scores transposed, S^T = K Q^T: lane (r, hf) of a 32 x 32 product owns row r, and each of its maxima and sums is a register.  q and k
 // are in f16, 11 bits (in bf16 they would be 0.005 of a result off: more than its own rounding), the weights and V in bf16.
 // p = 2^(s - m) with an integer m that only rises (a power of two, so no rounding depends on when it rose): in blocks that
-// are seen whole without looking, as long as the weights' sum stays below 2^64, from -m in the scores' accumulators.
+// are seen whole without looking, as long as the weights' sum stays below 2^8, from -m in the scores' accumulators.  No key's weight is
+// above 2^8, so n of them with values below 2^119 / n have finite sums.
 // Blocks are copied by buffer_load ... lds three ahead into four stages of LDS, so a barrier a block is all that waves share.
 // 7741 rows of 16 heads behind 4096 keys: 264 GFLOP in 273 us, 967 TFLOP/s; the matrix cores are busy 56 % of the cycles at the 1.67
 // GHz that the power limit leaves (a library product of 8192 x 8192 x 8192: 1150).  64 rows of 32 heads behind 8192: 33.6 MB of keys
@@ -234,7 +235,7 @@ __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a) {
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) void prefix_lds_t;
-constexpr float P_LIMIT = 18446744073709551616.0f;  // 2^64
+constexpr float P_LIMIT = 256.0f;
 constexpr float M_NONE = -1e30f;                    // no key so far
 constexpr int PKT = 64 * PHD * 2;                   // bytes of a block's K; its V^T follows
 constexpr int PST = 2 * PKT;                        // of a stage
@@ -461,7 +462,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_bf16(PrefixArgs 
       float& acc = k & 1 ? lb : la;
       acc = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{q[2 * (k & 3)], q[2 * (k & 3) + 1]}, ones, acc, false);
     };
-    // the rare case of a sum above 2^64: m rises to the half's largest score
+    // the rare case of a sum above 2^8: m rises to the half's largest score
     const auto settle = [&](int t) __attribute__((always_inline)) {
       float sum = la + lb;
       if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(sum <= P_LIMIT)) != 0, 0)) {

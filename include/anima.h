@@ -224,7 +224,8 @@ int64_t anima_attention_noalloc_scratch_bytes(void);
  * ANIMA_PREC_BF16 rounds q (times scale log2 e) and k to 11 bits (f16: values from 65520 on count as not
  * finite), the weights and v to bf16; ANIMA_PREC_FP32 rounds nothing.
  * D = 128 (ANIMA_E_UNSUPPORTED otherwise).  A sequence of no rows is left out; P = 0: no prefix.  A key with
- * a NaN or an infinity in k or v makes the rows that see it NaN, and no others.  The scratch (the packed K and
+ * a NaN or an infinity in k or v makes the rows that see it NaN, and no others; a row of n keys is finite for
+ * values of v below 2^119 / n in magnitude.  The scratch (the packed K and
  * V, and partial sums) is the context's workspace. */
 typedef struct {
   int B;
