@@ -236,7 +236,7 @@ __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a) {
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) void prefix_lds_t;
 constexpr float P_LIMIT = 256.0f;
-constexpr float M_NONE = -1e30f;                    // no key so far
+constexpr float M_NONE = -3e38f;      // no key so far (below every score)
 constexpr int PKT = 64 * PHD * 2;                   // bytes of a block's K; its V^T follows
 constexpr int PST = 2 * PKT;                        // of a stage
 constexpr int PNST = 4;
