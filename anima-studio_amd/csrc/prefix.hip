@@ -227,7 +227,8 @@ __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a) {
 // are in f16, 11 bits (in bf16 they would be 0.005 of a result off: more than its own rounding), the weights and V in bf16.
 // p = 2^(s - m) with an integer m that only rises (a power of two, so no rounding depends on when it rose): in blocks that
 // are seen whole without looking, as long as the weights' sum stays below 2^8, from -m in the scores' accumulators.  No key's weight is
-// above 2^8, so n of them with values below 2^119 / n have finite sums.
+// above 2^8, so n of them with values below 2^119 / n have finite sums.  Where m rises, it rises to 2^24 times the largest weight, so that
+// it seldom does again (7741 rows of 16 heads behind 4096 keys, scores of a standard deviation of 8: 318 us without that, 296 so).
 // Blocks are copied by buffer_load ... lds three ahead into four stages of LDS, so a barrier a block is all that waves share.
 // 7741 rows of 16 heads behind 4096 keys: 264 GFLOP in 273 us, 967 TFLOP/s; the matrix cores are busy 56 % of the cycles at the 1.67
 // GHz that the power limit leaves (a library product of 8192 x 8192 x 8192: 1150).  64 rows of 32 heads behind 8192: 33.6 MB of keys
@@ -235,8 +236,8 @@ __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a) {
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) void prefix_lds_t;
-constexpr float P_LIMIT = 256.0f;
-constexpr float M_NONE = -3e38f;      // no key so far (below every score)
+constexpr float P_LIMIT = 256.0f, P_HEAD = 24.0f;
+constexpr float M_NONE = -3e38f;                    // no key so far (below every score)
 constexpr int PKT = 64 * PHD * 2;                   // bytes of a block's K; its V^T follows
 constexpr int PST = 2 * PKT;                        // of a stage
 constexpr int PNST = 4;
@@ -423,9 +424,9 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_bf16(PrefixArgs 
     float bm = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
     for (int e = 1; e < 16; e++) bm = fmaxf(bm, fmaxf(s[0][e], s[1][e]));
-    const float mn = fmaxf(m, ceilf(p_pair_max(bm)));
-    if (__builtin_amdgcn_ballot_w64(mn > m)) {
-      const float f = __builtin_amdgcn_exp2f(m - mn);
+    const float top = ceilf(p_pair_max(bm));
+    if (__builtin_amdgcn_ballot_w64(top > m)) {
+      const float mn = top > m ? top + P_HEAD : m, f = __builtin_amdgcn_exp2f(m - mn);
       m = mn;
       l *= f;
 #pragma unroll
@@ -469,7 +470,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_bf16(PrefixArgs 
         float bm = s[t][0];
 #pragma unroll
         for (int e = 1; e < 16; e++) bm = fmaxf(bm, s[t][e]);
-        const float d = fmaxf(ceilf(p_pair_max(bm)), 0.0f), g = __builtin_amdgcn_exp2f(-d);
+        const float top = ceilf(p_pair_max(bm)), d = top > 0.0f ? top + P_HEAD : 0.0f, g = __builtin_amdgcn_exp2f(-d);
         m += d;
         negm -= d;
         l *= g;
