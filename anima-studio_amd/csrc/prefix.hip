@@ -17,7 +17,7 @@
 namespace anima {
 
 constexpr int PHD = 128;      // head dim
-constexpr int PBK = 64;       // keys per block of the prepared layouts
+constexpr int PBK = PREFIX_BLOCK;
 constexpr int PSEQ = 256;     // sequences of one launch (their first rows go with the kernel's arguments)
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -791,39 +791,15 @@ static int prefix_prep_launch(anima_ctx* c, const PrefixArgs& a) {
   return L.end();
 }
 
-// Tiles of 128 or 256 rows, and the parts that their key blocks are split into: what ends first by the times that a block of 64
-// keys, a workgroup's start and a join take, in us (fitted to 46 calls timed at all their plans: 1 to 17390 rows of 3 to 32
-// heads behind 0 to 8192 keys; this picks a plan within 2 % of the best on average).
-// 266 rows of 32 heads behind 49 keys, bf16: 22.9 whole, 27.0 in three parts; 365 rows of 8 behind 467, fp32: 86 whole, 33 in 12.
-static int prefix_plan(const anima_ctx* c, bool bf, int longest, PrefixArgs& a) {  // -> waves of a tile; sets nt and splits
-  int best_nw = 0;
-  double best = 0.0;
-  for (int nw = 4; nw <= 8; nw += 4) {
-    const int nt = (a.V + 32 * nw - 1) / (32 * nw);
-    const int64_t span = std::min(a.T, (32 * nw + a.group - 1) / a.group + 1) + (int64_t)longest;  // own keys that a tile's rows see
-    const int total = a.Pp / PBK + (int)std::min<int64_t>(a.Tp / PBK, (span + PBK - 1) / PBK + 1);
-    for (int s = 1; s <= std::min(total, 64); s++) {
-      const int64_t rounds = ((int64_t)nt * a.Hkv * s + c->num_cus - 1) / c->num_cus;
-      const double block = !bf ? 6.0 : nw == 4 ? 1.2 : 1.4, start = bf ? 5.0 : 4.0, join = 2.0 + (double)s * a.Hkv * a.V * 1056 / 5e6;
-      const double blocks = 0.5 * ((total + s - 1) / s) + 0.5 * total / s;  // (the longest part and the mean one)
-      const double t = (double)rounds * (start + blocks * block) + (s > 1 ? join : 0.0);
-      // (bf16, one wave of rows whose blocks are all copied at its start: 2 rows behind 77 keys 15.1 us whole, 16.7 in three parts)
-      if (best_nw && (t >= best || (bf && s > 1 && a.V <= 32 && total <= 3))) continue;
-      best = t;
-      best_nw = nw;
-      a.nt = nt;
-      a.splits = s;
-    }
-  }
-  return best_nw;
-}
-
 // The sequences of one launch, which the arguments describe: their keys and values into the workspace, then the rows.
 template <class T>
 static int prefix_part(anima_ctx* c, PrefixArgs& a, int longest) {
   constexpr bool BF = sizeof(T) == 2;
   a.V = a.T * a.group;
-  const bool eight = prefix_plan(c, BF, longest, a) == 8;
+  const PrefixPlan plan = prefix_plan(c->num_cus, BF, a.V, a.group, a.Hkv, a.T, a.P, longest);
+  const bool eight = plan.waves == 8;
+  a.nt = plan.nt;
+  a.splits = plan.splits;
   const size_t plane = (size_t)a.Hkv * a.Tp * PHD * sizeof(T), q = (size_t)a.Hkv * a.V * PHD * sizeof(T),
                n = a.splits > 1 ? (size_t)a.splits * a.Hkv * a.V : 0;
   void* ws = nullptr;

@@ -2,6 +2,7 @@
 // refusal can be reached without a device.
 #pragma once
 
+#include <algorithm>
 #include <cstdint>
 #include <cstdio>
 
@@ -14,6 +15,9 @@ constexpr int64_t PREFIX_MAX_ROWS = 1 << 28;  // of all sequences
 constexpr int64_t PREFIX_MAX_LD = 1 << 20;    // floats between rows: 256 rows of a tile stay below 2^31 bytes
 constexpr int PREFIX_MAX_HEADS = 1 << 12;
 constexpr int64_t PREFIX_MAX_VROWS = 1 << 30;  // rows times heads of a launch: 256 threads to 128 of them stay below 2^32
+
+constexpr int PREFIX_BLOCK = 64;               // keys per block of the prepared layouts
+constexpr int64_t PREFIX_MAX_PARTS = 1 << 26;  // rows of the parts of a split call: 32 threads each in the join
 
 struct PrefixMsg {
   char* buf;
@@ -32,6 +36,38 @@ struct PrefixMsg {
 // Bytes of a prefix's prepared K and V: rows in blocks of 64 (attention_kv_bytes of one batch element).
 inline int64_t prefix_kv_bytes(int Hkv, int P, int precision) {
   return P < 1 ? 0 : 2 * (int64_t)Hkv * (((int64_t)P + 63) / 64 * 64) * 128 * (precision == ANIMA_PREC_BF16 ? 2 : 4);
+}
+
+// Tiles of 128 or 256 virtual rows (V = T * group of a kv head), and the parts that their key blocks are split into: what ends first
+// by the times that a block of 64 keys, a workgroup's start and a join take, in us (fitted to 46 calls timed at all their plans: 1 to
+// 17390 rows of 3 to 32 heads behind 0 to 8192 keys; this picks a plan within 2 % of the best on average).
+// 266 rows of 32 heads behind 49 keys, bf16: 22.9 whole, 27.0 in three parts; 365 rows of 8 behind 467, fp32: 86 whole, 33 in 12.
+struct PrefixPlan {
+  int waves, nt, splits;  // of a tile; tiles of a kv head; parts
+};
+inline PrefixPlan prefix_plan(int num_cus, bool bf, int V, int group, int Hkv, int T, int P, int longest) {
+  PrefixPlan plan{};
+  double best = 0.0;
+  const int64_t rows = (int64_t)Hkv * V;
+  for (int nw = 4; nw <= 8; nw += 4) {
+    const int nt = (int)(((int64_t)V + 32 * nw - 1) / (32 * nw));
+    const int64_t span = std::min(T, (32 * nw + group - 1) / group + 1) + (int64_t)longest;  // own keys that a tile's rows see
+    const int total = (P + PREFIX_BLOCK - 1) / PREFIX_BLOCK +
+                      (int)std::min<int64_t>((T + PREFIX_BLOCK - 1) / PREFIX_BLOCK, (span + PREFIX_BLOCK - 1) / PREFIX_BLOCK + 1);
+    for (int s = 1; s <= std::min(total, 64); s++) {
+      if (s > 1 && s * rows > PREFIX_MAX_PARTS) break;
+      const int64_t rounds = ((int64_t)nt * Hkv * s + num_cus - 1) / num_cus;
+      const double block = !bf ? 6.0 : nw == 4 ? 1.2 : 1.4, start = bf ? 5.0 : 4.0, join = 2.0 + (double)s * rows * 1056 / 5e6;
+      const double blocks = 0.5 * ((total + s - 1) / s) + 0.5 * total / s;  // (the longest part and the mean one)
+      const double t = (double)rounds * (start + blocks * block) + (s > 1 ? join : 0.0);
+      // (bf16, one wave of rows whose blocks are all copied at its start: whole.  1 to 30 rows behind 70 to 128 keys, at eight sizes of 3
+      // to 32 heads: 14.4 to 16.4 us whole, 15.7 to 16.9 in two or three parts)
+      if (plan.waves && (t >= best || (bf && s > 1 && V <= 32 && total <= 3))) continue;
+      best = t;
+      plan = {nw, nt, s};
+    }
+  }
+  return plan;
 }
 
 // rows: the sum of the lengths; longest: the largest.
