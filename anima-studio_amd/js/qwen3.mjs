@@ -254,19 +254,20 @@ export class Qwen3 {
 
   checkPrefix(kept) {
     if (!kept) return;
+    if (kept.owner !== this) throw new Error("encodeBatch: opts.prefix is of another encoder");
     if (!kept.hidden.buf) throw new Error("encodeBatch: opts.prefix has been released");
     if (kept.key !== this.stateKey()) throw new Error("encodeBatch: opts.prefix is of another precision, other weights or other LoRAs");
   }
 
   // The tokens that a series of prompts begins with (a template), encoded once for encodeBatch's opts.prefix:
   // each layer's keys and values as ops.attentionPrefixPrepare lays them out, and the tokens' hidden states (under
-  // the causal mask neither depends on what follows).  Belongs to the caller (release()); it is of no use after
-  // a change of the precision, the weights or the LoRAs, and encodeBatch then refuses it.
+  // the causal mask neither depends on what follows).  Belongs to the caller (release()); it is of no use to
+  // another encoder, or after a change of the precision, the weights or the LoRAs, and encodeBatch then refuses it.
   async keepPrefix(ids) {
     if (!ids.length) throw new Error("keepPrefix: no tokens");
     const kv = [], key = this.stateKey();
     const hidden = await this.runBatch(ids, { P: ids.length, lens: [], keep: kv });
-    return { ids: Array.from(ids), kv, hidden, key, release() { for (const t of kv.concat([hidden])) t.release(); } };
+    return { owner: this, ids: Array.from(ids), kv, hidden, key, release() { for (const t of kv.concat([hidden])) t.release(); } };
   }
 
   // Several prompts (arrays of ids) at once -> one Tensor [length, D] each, as encode gives it.  The tokens that
