@@ -34,6 +34,7 @@ export class LatentPipeline {
     this.timeCache = new Map(); // key -> timeCond result (device tensors), in insertion (LRU) order
     this.ctxCache = new Map(); // prompt key -> prepared conditioning (B = 1)
     this.ctxGeneration = loraGeneration();
+    this.ctxHeld = new Map(); // conditionings that an encodeBatch under way will return -> how many of them hold it
     this.stats = { timeCondHits: 0, timeCondMisses: 0, encodeHits: 0, encodeMisses: 0 };
   }
 
@@ -49,15 +50,7 @@ export class LatentPipeline {
     if (!this.te || !this.adapter) throw new Error("encode: the pipeline was built without opts.te / opts.adapter");
     const key = promptKey(prompt);
     const keys = (keep || [prompt]).map((k) => (typeof k === "string" ? k : promptKey(k)));
-    if (this.ctxGeneration !== loraGeneration()) {
-      this.clearContexts();
-      this.ctxGeneration = loraGeneration();
-    }
-    for (const [k, t] of this.ctxCache)
-      if (!keys.includes(k)) {
-        t.release();
-        this.ctxCache.delete(k);
-      }
+    this.keepContexts((k) => keys.includes(k));
     if (this.ctxCache.has(key)) {
       this.stats.encodeHits++;
       return this.ctxCache.get(key);
@@ -66,6 +59,10 @@ export class LatentPipeline {
     const hidden = await this.te.encode(prompt.qwenIds);
     const ctx = await adapt(this.gpu, this.adapter, hidden, prompt.t5Ids, prompt.t5Weights);
     hidden.release();
+    if (this.ctxCache.has(key)) { // (another call has put it there meanwhile)
+      ctx.release();
+      return this.ctxCache.get(key);
+    }
     const cond = this.dit.prepareContext([ctx]);
     this.ctxCache.set(key, cond);
     return cond;
@@ -73,33 +70,67 @@ export class LatentPipeline {
 
   // Several prompts (as encode's) at once -> their conditionings, in order: those not cached pass the text
   // encoder together (Qwen3.encodeBatch: the tokens that they all begin with once).  They alone stay cached.
+  // A call that starts meanwhile
+  // leaves this one's conditionings alone; LoRAs attached meanwhile end it with an error.
   async encodeBatch(prompts) {
     if (!this.te || !this.adapter) throw new Error("encodeBatch: the pipeline was built without opts.te / opts.adapter");
     const byKey = new Map(prompts.map((p) => [promptKey(p), p]));
+    this.keepContexts((k) => byKey.has(k));
+    const generation = this.ctxGeneration, conds = new Map(); // key -> this call's conditioning
+    const hold = (k, t) => {
+      conds.set(k, t);
+      this.ctxHeld.set(t, (this.ctxHeld.get(t) || 0) + 1);
+    };
+    const check = () => {
+      if (loraGeneration() !== generation) throw new Error("encodeBatch: LoRAs were attached while it ran");
+    };
+    const missing = [];
+    for (const k of byKey.keys()) {
+      if (this.ctxCache.has(k)) hold(k, this.ctxCache.get(k));
+      else missing.push(k);
+    }
+    this.stats.encodeMisses += missing.length;
+    this.stats.encodeHits += prompts.length - missing.length;
+    let hidden = [];
+    try {
+      hidden = await this.te.encodeBatch(missing.map((k) => byKey.get(k).qwenIds));
+      for (const k of missing) {
+        check();
+        const p = byKey.get(k);
+        const ctx = await adapt(this.gpu, this.adapter, hidden[0], p.t5Ids, p.t5Weights);
+        hidden.shift().release();
+        check();
+        const there = this.ctxCache.get(k); // (another call may have put it there meanwhile)
+        if (there) ctx.release();
+        hold(k, there || this.dit.prepareContext([ctx]));
+        this.ctxCache.set(k, conds.get(k));
+      }
+      return prompts.map((p) => conds.get(promptKey(p)));
+    } finally {
+      for (const t of hidden) t.release();
+      for (const t of conds.values()) {
+        const n = this.ctxHeld.get(t);
+        if (n > 1) this.ctxHeld.set(t, n - 1);
+        else this.ctxHeld.delete(t);
+      }
+    }
+  }
+
+  // Empties the cache after a change of the LoRAs, and drops the entries that are not wanted any more.
+  keepContexts(wanted) {
     if (this.ctxGeneration !== loraGeneration()) {
       this.clearContexts();
       this.ctxGeneration = loraGeneration();
     }
     for (const [k, t] of this.ctxCache)
-      if (!byKey.has(k)) {
+      if (!wanted(k) && !this.ctxHeld.has(t)) {
         t.release();
         this.ctxCache.delete(k);
       }
-    const missing = Array.from(byKey.keys()).filter((k) => !this.ctxCache.has(k));
-    this.stats.encodeMisses += missing.length;
-    this.stats.encodeHits += prompts.length - missing.length;
-    const hidden = await this.te.encodeBatch(missing.map((k) => byKey.get(k).qwenIds));
-    for (let i = 0; i < missing.length; i++) {
-      const p = byKey.get(missing[i]);
-      const ctx = await adapt(this.gpu, this.adapter, hidden[i], p.t5Ids, p.t5Weights);
-      hidden[i].release();
-      this.ctxCache.set(missing[i], this.dit.prepareContext([ctx]));
-    }
-    return prompts.map((p) => this.ctxCache.get(promptKey(p)));
   }
 
   clearContexts() {
-    for (const t of this.ctxCache.values()) t.release();
+    for (const t of this.ctxCache.values()) if (!this.ctxHeld.has(t)) t.release();
     this.ctxCache.clear();
   }
 

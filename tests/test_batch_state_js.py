@@ -23,3 +23,58 @@ def test_prefix_of_another_encoder():
                "const go = (te) => err(() => te.encodeBatch([[1, 2, 3]], { prefix }));"
                "console.log(JSON.stringify([await go(a), await go(b), await go(c)])); })")
     assert got[0] == "" and all("another encoder" in e for e in got[1:]), got
+
+
+# a pipeline whose text encoder and adapter wait until they are told to go on; conditionings count their releases
+PIPELINE = (RECORD + "import('./pipeline.mjs').then(async ({ LatentPipeline }) => { const lora = await import('./lora.mjs');"
+            "const conds = [], hidden = [], waits = []; let ready = [];"
+            "const dit = { prepareContext: ([c]) => { c.release(); const t = { n: conds.length, freed: 0, release() { this.freed++; } }; conds.push(t); return t; } };"
+            "const h = () => { const t = tensor([3, 1024]); hidden.push(t); return t; };"
+            "const gate = () => new Promise((ok, no) => waits.push({ ok, no }));"
+            "const te = { encode: async () => { await gate(); return h(); }, encodeBatch: async (p) => { await gate(); return p.map(h); } };"
+            "const A = { blocks: [], outProj: { kind: 'bf16', N: 1024, K: 1024, buf: 1 }, norm: tensor([1024]), embedRows: async (ids) => { await gate(); return new Float32Array(ids.length * 1024); } };"
+            "gpu.read = async (t) => new Float32Array(t.size);"
+            "const p = new LatentPipeline(gpu, dit, { te, adapter: A });"
+            "const prompt = (key) => ({ key, qwenIds: [1, 2], t5Ids: [3], t5Weights: null });"
+            "const tick = () => new Promise((r) => setTimeout(r, 1));"
+            "const go = async (n) => { for (let i = 0; i < n; i++) { await tick(); const w = waits.shift(); if (w) w.ok(); } await tick(); };"
+            "const done = async (q) => { let r; q.then((v) => { r = { v }; }, (e) => { r = { e: e.message }; }); for (let i = 0; i < 40 && !r; i++) await go(1); return r; };"
+            "const out = {};")
+
+
+def test_overlapping_calls():
+    """encodeBatch beside calls that want other prompts: what it returns is whole, in order, and not released."""
+    got = node(PIPELINE +
+               "const a = (await done(p.encode(prompt('a')))).v;"
+               "const batch = p.encodeBatch([prompt('b'), prompt('a'), prompt('c'), prompt('b')]);"
+               "await go(2);"  # b is there, c under way
+               "const d = p.encode(prompt('d'));"
+               "const r = (await done(batch)).v, dd = (await done(d)).v;"
+               "out.whole = r.map((t) => t && t.freed); out.order = [r[1] === a, r[0] === r[3], new Set(r.concat([dd])).size];"
+               "out.hidden = hidden.every((t) => t.released === 1); out.held = p.ctxHeld.size;"
+               # the next call drops what it does not want, once
+               "const e = (await done(p.encode(prompt('d')))).v; out.next = [e === dd, conds.map((t) => t.freed), p.ctxCache.size];"
+               # the same prompt twice at once: one conditioning in the end
+               "const two = [p.encodeBatch([prompt('e')]), p.encodeBatch([prompt('e')]), p.encode(prompt('e'))];"
+               "const n = conds.length, x = []; for (const q of two) x.push(...[].concat((await done(q)).v));"
+               "out.same = [new Set(x).size, conds.length - n, p.ctxCache.get('e') === x[0], x[0].freed];"
+               # the cache cleared under a call that returns an entry of it
+               "const hit = p.encodeBatch([prompt('e'), prompt('f')]); await tick(); p.clearContexts(); out.cleared = (await done(hit)).v.map((t) => t.freed);"
+               "console.log(JSON.stringify(out)); });")
+    assert got["whole"] == [0, 0, 0, 0] and got["order"] == [True, True, 4] and got["hidden"] and got["held"] == 0
+    assert got["next"] == [True, [1, 1, 1, 0], 1]
+    assert got["same"] == [1, 1, True, 0] and got["cleared"] == [0, 0]
+
+
+def test_failures_release():
+    """An adapter that fails, and LoRAs attached on the way: an error, every hidden state released once, nothing held, nothing stale."""
+    got = node(PIPELINE +
+               "const fail = p.encodeBatch([prompt('a'), prompt('b'), prompt('c')]); fail.catch(() => {}); await go(2); await tick();"
+               "waits.shift().no(new Error('lost')); out.fail = (await done(fail)).e; out.hidden = hidden.map((t) => t.released);"
+               "out.held = p.ctxHeld.size; out.keys = Array.from(p.ctxCache.keys());"
+               "const b = p.encodeBatch([prompt('a'), prompt('x'), prompt('y')]); b.catch(() => {}); await go(2); lora.attachLoras({}, []);"
+               "out.lora = (await done(b)).e; const z = (await done(p.encode(prompt('z')))).v;"
+               "out.left = [Array.from(p.ctxCache.keys()), z.freed, p.ctxHeld.size, hidden.every((t) => t.released === 1)];"
+               "console.log(JSON.stringify(out)); });")
+    assert got["fail"] == "lost" and got["hidden"] == [1, 1, 1] and got["held"] == 0 and got["keys"] == ["a"]
+    assert "LoRAs were attached" in got["lora"] and got["left"] == [["z"], 0, 0, True]
