@@ -136,13 +136,14 @@ export function quantizeQ4(gpu, W, opts) {
 
 // Rows ids of an embedding table on the device ({ kind: "f32" | "bf16" | "q4", N, K, buf }): a tensor
 // [ids.length, K], each row times opts.weights[t] and opts.scale (default 1).  ids: an array or a Tensor
-// (i32); an id outside [0, N) gives a row of zeros.  opts.weights: an array or a Tensor; opts.out: the tensor
+// (i32); an id outside [0, N), or no whole number, gives a row of zeros.  opts.weights: an array or a Tensor; opts.out: the tensor
 // to write.
 export function embedRows(gpu, table, ids, opts) {
   const o = opts || {};
   if (table.kind !== "f32" && table.kind !== "bf16" && table.kind !== "q4") throw new Error(`embedRows: a ${table.kind} table (f32, bf16 or q4)`);
-  const onDevice = (t, T) => (t && t.buf !== undefined ? t : T.from(t));
-  const id = onDevice(ids, Int32Array), T = id.buf !== undefined ? id.size : id.length;
+  const onDevice = (t, T, f) => (t && t.buf !== undefined ? t : T.from(t, f));
+  // (what is no row of the table stays none: 2^32 and NaN would become row 0)
+  const id = onDevice(ids, Int32Array, (i) => (Number.isInteger(i) && i >= 0 && i < table.N ? i : -1)), T = id.buf !== undefined ? id.size : id.length;
   checkDtype("embedRows: ids", id, "i32");
   const w = o.weights ? onDevice(o.weights, Float32Array) : null;
   checkDtype("embedRows: weights", w, "f32");

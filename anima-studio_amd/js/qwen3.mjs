@@ -150,7 +150,7 @@ export class Qwen3 {
       const rows = await this.embedRows(ids);
       return (x) => this.gpu.write(x, rows);
     }
-    for (const id of ids) if (!(id >= 0 && id < t.N)) throw new Error(`token id ${id} outside the embedding table [${t.N},${t.K}]`);
+    for (const id of ids) if (!(Number.isInteger(id) && id >= 0 && id < t.N)) throw new Error(`token id ${id} outside the embedding table [${t.N},${t.K}]`);
     return (x) => ops.embedRows(this.gpu, t, ids, { out: x });
   }
 

@@ -78,3 +78,14 @@ def test_failures_release():
                "console.log(JSON.stringify(out)); });")
     assert got["fail"] == "lost" and got["hidden"] == [1, 1, 1] and got["held"] == 0 and got["keys"] == ["a"]
     assert "LoRAs were attached" in got["lora"] and got["left"] == [["z"], 0, 0, True]
+
+
+def test_ids_that_are_no_row():
+    """Ids from the host that no 32-bit index holds: rows of zeros, as any outside the table; the encoder refuses them."""
+    got = node(ENCODER + "import('./ops.mjs').then(async (ops) => { const { Qwen3 } = await import('./qwen3.mjs');"
+               "const sent = []; const from = gpu.fromArray; gpu.fromArray = (a, s) => { sent.push(Array.from(a)); return from(a, s); };"
+               "ops.embedRows(gpu, { kind: 'f32', N: 10, K: 128, buf: 1 }, [0, 9, 10, -1, 4294967296, 4294967299, NaN, undefined, 1.5, -0.5, Infinity]);"
+               "const te = encoder(Qwen3, 1); te.deviceTable = { kind: 'f32', N: 10, K: 256, buf: 1 };"
+               "console.log(JSON.stringify([sent[0], await err(() => te.encodeBatch([[1, 1.5]])), await err(() => te.encodeBatch([[NaN]]))])); })")
+    assert got[0] == [0, 9] + [-1] * 9
+    assert "token id 1.5 outside" in got[1] and "token id NaN outside" in got[2]
