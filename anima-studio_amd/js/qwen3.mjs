@@ -151,7 +151,7 @@ export class Qwen3 {
       return (x) => this.gpu.write(x, rows);
     }
     for (const id of ids) if (!(Number.isInteger(id) && id >= 0 && id < t.N)) throw new Error(`token id ${id} outside the embedding table [${t.N},${t.K}]`);
-    return (x) => ops.embedRows(this.gpu, t, ids, { out: x });
+    return (x) => ops.embedRows(this.gpu, this.deviceTable, ids, { out: x }); // (the table of that moment: t may have been replaced)
   }
 
   // ids -> Tensor [L, 1024] (qwen3.js:38-78).  With this.graphs (the default) the 28 layers run as a

@@ -89,3 +89,14 @@ def test_ids_that_are_no_row():
                "console.log(JSON.stringify([sent[0], await err(() => te.encodeBatch([[1, 1.5]])), await err(() => te.encodeBatch([[NaN]]))])); })")
     assert got[0] == [0, 9] + [-1] * 9
     assert "token id 1.5 outside" in got[1] and "token id NaN outside" in got[2]
+
+
+def test_table_replaced_under_an_encoding():
+    """embedOnDevice that ends between an encoding's check of its ids and its launches: the rows come from the new table."""
+    got = node(ENCODER + "import('./qwen3.mjs').then(async ({ Qwen3 }) => { const te = encoder(Qwen3, 1);"
+               "const table = () => ({ kind: 'f32', N: 10, K: 256, buf: tensor([10, 256]) }); te.loadTable = async () => table();"
+               "await te.embedOnDevice(); const old = te.deviceTable; calls.splice(0);"
+               "const r = te.embedOnDevice(), e = te.encodeBatch([[1, 2]]); await r; const t = await e; await te.encodeBatch([[3]]);"
+               "const used = calls.filter((c) => c[0] === 'embedRows').map((c) => c[2].buf);"
+               "console.log(JSON.stringify([t.length, old.buf.released, used.map((b) => b === te.deviceTable.buf.buf)])); })")
+    assert got == [1, 1, [True, True]]
