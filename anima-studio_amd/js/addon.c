@@ -277,14 +277,17 @@ static napi_value js_settle(napi_env env, napi_callback_info info) {
   return NULL;
 }
 
-/* process.on("exit", settle) */
-static int settle_at_exit(napi_env env) {
+/* process.on("exit", settle); a process without one (or whose `on` fails) goes without */
+static void settle_at_exit(napi_env env) {
   napi_value global, process, on, args[2], r;
-  return napi_get_global(env, &global) == napi_ok && napi_get_named_property(env, global, "process", &process) == napi_ok &&
-         napi_get_named_property(env, process, "on", &on) == napi_ok &&
-         napi_create_string_utf8(env, "exit", NAPI_AUTO_LENGTH, &args[0]) == napi_ok &&
-         napi_create_function(env, "settle", NAPI_AUTO_LENGTH, js_settle, NULL, &args[1]) == napi_ok &&
-         napi_call_function(env, process, on, 2, args, &r) == napi_ok;
+  bool failed = false;
+  if (!(napi_get_global(env, &global) == napi_ok && napi_get_named_property(env, global, "process", &process) == napi_ok &&
+        napi_get_named_property(env, process, "on", &on) == napi_ok &&
+        napi_create_string_utf8(env, "exit", NAPI_AUTO_LENGTH, &args[0]) == napi_ok &&
+        napi_create_function(env, "settle", NAPI_AUTO_LENGTH, js_settle, NULL, &args[1]) == napi_ok &&
+        napi_call_function(env, process, on, 2, args, &r) == napi_ok) &&
+      napi_is_exception_pending(env, &failed) == napi_ok && failed)
+    napi_get_and_clear_last_exception(env, &r);
 }
 
 /* allocHandle(ctx, bytes) -> handle object (the buffer's owner) */
@@ -1167,7 +1170,7 @@ static napi_value Init(napi_env env, napi_value exports) {
 #undef FN
   if (napi_define_properties(env, exports, sizeof desc / sizeof desc[0], desc) != napi_ok) return NULL;
   if (napi_add_env_cleanup_hook(env, bufs_cleanup, env) != napi_ok) return NULL;
-  if (!settle_at_exit(env)) return NULL;
+  settle_at_exit(env);
   return exports;
 }
 
