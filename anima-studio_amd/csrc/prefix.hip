@@ -549,9 +549,9 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_bf16(PrefixArgs 
 
 // ------------------------------------------------------------------ fp32 tiles
 //
-// The same parts in fp32 precision.  A value is three bf16 ones, x = x1 + x2 + x3 exactly (8 bits each, cut off and not rounded), and
-// a product six on the bf16 matrix cores, x1 y1 + x1 y2 + x2 y1 + x2 y2 + x1 y3 + x3 y1, without what is below 2^-22 of it: five
-// times the rate of the fp32 matrix cores.
+// The same parts in fp32 precision.  A value is three bf16 ones, x = x1 + x2 + x3 exactly (8 bits each, cut off and not rounded: x2 is
+// below 2^-7 of x and x3 below 2^-15), and a product six on the bf16 matrix cores, x1 y1 + x1 y2 + x2 y1 + x2 y2 + x1 y3 + x3 y1.  What
+// is left out, x2 y3 + x3 y2 + x3 y3, has the product's sign and is below 2^-21 of it.
 // A step is 32 keys.  They come as fp32 by buffer_load ... lds into one of two stages, a step ahead are cut into their planes (once
 // for all waves, under the products of the step before), and a step later are multiplied: one barrier a step.
 // p = 2^(s - m) with m raised where a step's maximum passes it by more than 8.  A step's products of V are added by themselves first:

@@ -125,7 +125,8 @@ export class Qwen3 {
   constructor(gpu, cfg) {
     this.gpu = gpu;
     this.cfg = cfg;
-    this.precision = "bf16"; // attention precision ("fp32": the fp32-MFMA kernel)
+    // precision of the attention ("fp32": 32-bit products), and of the products of e4m3 layers and of 4-bit weights
+    this.precision = "bf16";
     this.graphs = true; // replay the layers from a recorded HIP graph (per token count and precision)
     this.graphCache = new Map();
     this.deviceTable = null; // the embedding table, after embedOnDevice
@@ -231,7 +232,8 @@ export class Qwen3 {
   }
 
   // Converts the layers' bf16 linears to 4 bits with one scale per opts.group values (ops.quantizeQ4; opts.mid: and
-  // a middle value): close to a quarter of the bytes.  An option as quantizeF8; the activations stay in fp32.
+  // a middle value): close to a quarter of the bytes.  An option as quantizeF8.  The activations are fp32 rows, which the
+  // products at this.precision "bf16" (the default) round to 11 bits where they run on the matrix cores, and at "fp32" keep.
   // Returns the number of linears converted.
   quantizeQ4(opts) {
     return this.convert((W) => ops.quantizeQ4(this.gpu, W, opts).kind === "q4");

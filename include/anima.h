@@ -222,7 +222,8 @@ int64_t anima_attention_noalloc_scratch_bytes(void);
  * (at the same precision) writes them.  The reference encodes one prompt at a time (app/pipeline.js:192-211,
  * the causal attention of app/models/qwen3.js:60).
  * ANIMA_PREC_BF16 rounds q (times scale log2 e) and k to 11 bits (f16: values from 65520 on count as not
- * finite), the weights and v to bf16; ANIMA_PREC_FP32 rounds nothing.
+ * finite), the weights and v to bf16; ANIMA_PREC_FP32 rounds none of them, and leaves of each product less than
+ * 2^-21 of it out (three bf16 terms a value, the six largest of their nine products).
  * D = 128 (ANIMA_E_UNSUPPORTED otherwise).  A sequence of no rows is left out; P = 0: no prefix.  A key with
  * a NaN or an infinity in k or v makes the rows that see it NaN, and no others; a row of n keys is finite for
  * values of v below 2^119 / n in magnitude.  The scratch (the packed K and
@@ -495,8 +496,9 @@ typedef struct {
   /* f8 and q4 weights only (0 otherwise).  precision, f8: ANIMA_PREC_BF16 lets the 8-bit matrix instructions
    * add the products, which keep 2^-13 of the largest of each eight (about 1.5e-5 of the result, far below a
    * bf16 rounding); ANIMA_PREC_FP32 adds them in 32 bits, at the rate of bf16 products.  q4: ANIMA_PREC_BF16
-   * may round the activations to 11 bits (2^-12 of each) first, ANIMA_PREC_FP32 keeps them.  out_bf16 = 1: out
-   * is bf16 rows (round to nearest even; out and ldc then address uint16 elements), store epilogue only. */
+   * may round the activations to 11 bits first (2^-11 of each, or 2^-39 of the row's largest), ANIMA_PREC_FP32
+   * keeps them to 2^-23 of each (or 2^-39 of the row's largest).  out_bf16 = 1: out is bf16 rows (round to
+   * nearest even; out and ldc then address uint16 elements), store epilogue only. */
   int precision;
   int out_bf16;
 } anima_linear_desc;

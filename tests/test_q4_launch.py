@@ -91,7 +91,8 @@ def test_rows_of_several_launches(ctx, mid, precision):
     for x0, o0, a0, got in zip(xs, os_, ad, out.read()):
         r = x0.astype(np.float64) @ W.values.T + W.bias + a0
         want = o0 + gate * r
-        tol = (ref.bound(x0.astype(np.float64), W.values, K, precision, False, want, r) + 4 * ref.BIT_EPS * (np.abs(W.bias) + np.abs(a0))) * \
+        more = 2.0 ** -12 * (np.abs(x0.astype(np.float64)) @ np.abs(W.values).T) if precision == 0 else 0.0  # (x to 11 bits: 2^-11 in all)
+        tol = (more + ref.bound(x0.astype(np.float64), W.values, K, precision, False, want, r) + 4 * ref.BIT_EPS * (np.abs(W.bias) + np.abs(a0))) * \
             np.maximum(1, np.abs(gate)) + 4 * ref.BIT_EPS * np.abs(o0)
         assert np.all(np.abs(got - want) <= tol), (np.abs(got - want) / tol).max()
 
