@@ -12,7 +12,7 @@ namespace anima {
 
 constexpr int64_t PREFIX_MAX_KEYS = 1 << 22;  // of the prefix and of a sequence, as anima_attention's Lk
 constexpr int64_t PREFIX_MAX_ROWS = 1 << 28;  // of all sequences
-constexpr int64_t PREFIX_MAX_LD = 1 << 20;    // floats between rows: 256 rows of a tile stay below 2^31 bytes
+constexpr int64_t PREFIX_MAX_LD = 1 << 20;    // elements between rows (the interface's bound: offsets have 64 bits)
 constexpr int PREFIX_MAX_HEADS = 1 << 12;
 constexpr int64_t PREFIX_MAX_VROWS = 1 << 30;  // rows times heads of a launch: 256 threads to 128 of them stay below 2^32
 

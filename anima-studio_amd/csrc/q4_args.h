@@ -13,7 +13,7 @@ namespace anima {
 
 constexpr int Q4_MAX_K = 1 << 20;         // of a product
 constexpr int Q4_MAX_SIDE = 1 << 29;      // rows and outputs of a product (cut into launches by q4_part)
-constexpr int64_t Q4_MAX_LDX = 1 << 22;   // floats between rows of a product's input: 64 rows of a tile stay below 2^31 bytes
+constexpr int64_t Q4_MAX_LDX = 1 << 22;   // floats between rows of a product's input (the interface's bound: offsets have 64 bits)
 constexpr int64_t Q4_MAX_QUANT = (int64_t)1 << 34;  // weights of one conversion
 
 struct Q4Msg {

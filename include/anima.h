@@ -224,7 +224,8 @@ int64_t anima_attention_noalloc_scratch_bytes(void);
  * ANIMA_PREC_BF16 rounds q (times scale log2 e) and k to 11 bits (f16: values from 65520 on count as not
  * finite), the weights and v to bf16; ANIMA_PREC_FP32 rounds none of them, and leaves of each product less than
  * 2^-21 of it out (three bf16 terms a value, the six largest of their nine products).
- * D = 128 (ANIMA_E_UNSUPPORTED otherwise).  A sequence of no rows is left out; P = 0: no prefix.  A key with
+ * D = 128 (ANIMA_E_UNSUPPORTED otherwise); P and each len up to 2^22, rows up to 2^20 elements apart, 2^28 rows
+ * in all, H up to 2^12, each len times H up to 2^30.  A sequence of no rows is left out; P = 0: no prefix.  A key with
  * a NaN or an infinity in k or v makes the rows that see it NaN, and no others; a row of n keys is finite for
  * values of v below 2^119 / n in magnitude.  The scratch (the packed K and
  * V, and partial sums) is the context's workspace. */
@@ -517,8 +518,8 @@ typedef struct {
  * delta).
  * q4: r = alpha * sum_k x[m][k] w[n][k] of fp32 rows x (16-byte aligned, ldx % 4 == 0), with the products of
  * 32-bit accuracy or, on more than a few rows and with ANIMA_PREC_BF16, of x rounded to 11 bits.  A group_scale
- * below 2^-28 of the largest of its output n may be off by 2^-36 of that largest.  A row of x
- * with an infinity or a NaN gives no finite value.  M and N up to 2^29, K up to 2^20; as f8 in the rest (pooled
+ * below 2^-28 of the largest of its output n may be off by 2^-36 of that largest.  A row of x with an infinity or
+ * a NaN gives no finite value.  M and N up to 2^29, K up to 2^20, ldx up to 2^22; as f8 in the rest (pooled
  * scratch, the order of sums by the sizes, no acc_out and no LoRA factors). */
 int anima_linear(anima_ctx* ctx, const anima_linear_desc* desc);
 
