@@ -230,9 +230,9 @@ __global__ __launch_bounds__(256) void prefix_prep_kernel(PrefixArgs a) {
 // above 2^8, so n of them with values below 2^119 / n have finite sums.  Where m rises, it rises to 2^24 times the largest weight, so that
 // it seldom does again (7741 rows of 16 heads behind 4096 keys, scores of a standard deviation of 8: 318 us without that, 296 so).
 // Blocks are copied by buffer_load ... lds three ahead into four stages of LDS, so a barrier a block is all that waves share.
-// 7741 rows of 16 heads behind 4096 keys: 264 GFLOP in 273 us, 967 TFLOP/s; the matrix cores are busy 56 % of the cycles at the 1.67
+// 7741 rows of 16 heads behind 4096 keys: 264 GFLOP in 267 us, 990 TFLOP/s; the matrix cores are busy 56 % of the cycles at the 1.7
 // GHz that the power limit leaves (a library product of 8192 x 8192 x 8192: 1150).  64 rows of 32 heads behind 8192: 33.6 MB of keys
-// in 18 us, a start of 2, eleven until the last block is there, and the sums' way out.
+// in 19 us, a start of 2, eleven until the last block is there, and the sums' way out.
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) void prefix_lds_t;
@@ -556,7 +556,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_flash_bf16(PrefixArgs 
 // for all waves, under the products of the step before), and a step later are multiplied: one barrier a step.
 // p = 2^(s - m) with m raised where a step's maximum passes it by more than 8.  A step's products of V are added by themselves first:
 // chains of one step a sum across steps.
-// 1265 rows of 15 heads behind 1000 keys: 78 us (131 by the fp32 matrix cores), 1000 TFLOP/s of bf16 products with the tiles' unseen
+// 1265 rows of 15 heads behind 1000 keys: 79 us (131 by the fp32 matrix cores), 1000 TFLOP/s of bf16 products with the tiles' unseen
 // keys, the matrix cores busy 54 % of the cycles at 1.5 GHz; LDS is full (raw keys and planes, two stages each).
 constexpr int FRAW = 2 * 32 * PHD * 4;   // bytes of a step's K, then V^T, as they come
 constexpr int FPL = 32 * PHD * 2;        // of one plane of its K or V^T

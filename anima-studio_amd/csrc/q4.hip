@@ -641,8 +641,8 @@ __global__ __launch_bounds__(64 * QF_WAVES, 2) void q4_few_kernel(Q4Tile q) {
 // steps come in one load where rows of them allow it: each of a lane's own addresses costs the address unit as
 // much as 64 neighbouring bytes.  The LDS is held to half of a CU's (three stages for the largest tiles), so that one workgroup's
 // first copies and its epilogue pass under another's products: 8192 x 8192 x 2048, one term, gelu, 354 us by 256 x 256 tiles alone on
-// their CU and 336 by two of 128 x 256 (820 TFLOP/s; a library product of f16 matrices reaches 1110).  The matrix cores are busy 42 %
-// of the cycles at 1.8 GHz, the vector instructions (decode and gelu) take nearly as many.  2048 x 4096 x 1024 in two terms: 48 us,
+// their CU and 332 by two of 128 x 256 (828 TFLOP/s; a library product of f16 matrices reaches 1110).  The matrix cores are busy 45 %
+// of the cycles at 1.75 GHz, the vector instructions (decode and gelu) take nearly as many.  2048 x 4096 x 1024 in two terms: 48 us,
 // one round of tiles, of whose time the k loop takes 30 and the start and the epilogue the rest.
 template <int BM, int BN, int WM, int WN, int TERMS, int NST>
 __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void q4_tile_kernel(Q4Tile t) {

@@ -44,7 +44,7 @@ const isF8 = (l) => !!l.qkv && ["qkv", "o", "gate", "up", "down"].every((k) => l
 
 // The number of ids that all prompts begin with, or 0 where sharing them saves fewer than SHARE_ROWS rows: the
 // prefix costs two more calls a layer.  The 28 layers of 8 prompts with 77 shared ids and 40 of their own
-// (539 rows saved) take 4.6 ms shared and 5.4 apart, of 2 with 77 and 77 (77 rows) 4.1 and 3.6.
+// (539 rows saved) take 4.4 ms shared and 5.0 apart, of 2 with 77 and 77 (77 rows) 4.1 and 3.6.
 const SHARE_ROWS = 256;
 function commonPrefix(prompts) {
   let n = 0;
