@@ -380,7 +380,8 @@ __global__ __launch_bounds__(256) void q4_prep_kernel(Q4Prep a) {
       float mz = 0.0f;
       for (int g = lane; g < KG; g += 64) mz = fmaxf(mz, fabsf(bf16_f(a.gz[n * KG + g])));
       mz = wave_max(mz);
-      if (a.rn && mz != 0.0f) e = min(e, q4_exp(mz, 100));  // (middles of 2^107 scales: these have nothing to add)
+      // (beside middles of 2^78 scales these give way: 2^20 values of x below 2^15 and middles below 2^89 have finite sums)
+      if (a.rn && mz != 0.0f) e = min(e, q4_exp(mz, 88));
       for (int g = lane; g < a.KGp; g += 64) a.zp[n * a.KGp + g] = to_bf16(g < KG ? bf16_f(a.gz[n * KG + g]) * pow2f(e) : 0.0f);
     }
     if (a.rn && lane == 0) a.rn[n] = pow2f(-e);

@@ -518,9 +518,10 @@ typedef struct {
  * delta).
  * q4: r = alpha * sum_k x[m][k] w[n][k] of fp32 rows x (16-byte aligned, ldx % 4 == 0), with the products of
  * 32-bit accuracy or, on more than a few rows and with ANIMA_PREC_BF16, of x rounded to 11 bits.  A group_scale
- * below 2^-28 of the largest of its output n may be off by 2^-36 of that largest.  A row of x with an infinity or
- * a NaN gives no finite value.  M and N up to 2^29, K up to 2^20, ldx up to 2^22; as f8 in the rest (pooled
- * scratch, the order of sums by the sizes, no acc_out and no LoRA factors). */
+ * below 2^-28 of the largest of its output n (or 2^-105 of its largest group_mid) may be off by 2^-36 (2^-113)
+ * of that largest; from scales or middles of 2^88 in magnitude on, sums may become infinite where the result is
+ * not.  A row of x with an infinity or a NaN gives no finite value.  M and N up to 2^29, K up to 2^20, ldx up to
+ * 2^22; as f8 in the rest (pooled scratch, the order of sums by the sizes, no acc_out and no LoRA factors). */
 int anima_linear(anima_ctx* ctx, const anima_linear_desc* desc);
 
 /* The stacked QKV projection of a DiT block with the attention's operand preparation in its

@@ -45,3 +45,28 @@ def test_small_scales_alone(ctx, precision, M, N, K, g, name, apart):
         tol = tol + 2.0 ** -36 * s.max(1) * (np.abs(x64) @ np.abs(codes.astype(np.float64) - 8).T)
     err = np.abs(out.numpy() - want)
     assert np.all(err <= tol), (err / tol).max()
+
+
+@pytest.mark.parametrize("M,N,K,g,name", [(40, 100, 8192, 128, "gemm.q4.64"), (40, 100, 8192, 32, "gemm.q4.64"), (640, 1701, 4160, 32, "gemm.q4.128"), (1030, 3600, 8192, 32, "gemm.q4.128"),
+                                          (64, 1300, 1024, 64, "gemm.q4.few"), (4, 300, 8192, 32, "gemv.q4")])
+@pytest.mark.parametrize("power", [-60, -100, -120])
+def test_middles_beside_tiny_scales(ctx, M, N, K, g, name, power):
+    """Constant groups (a middle, no scale) beside one group of scales 2^power: sums of like signs as large as they can be stay finite.
+    The middles' part is bf16 values and three bf16 terms of a group's sum of x (2^-24 of it), so its bound is the product's."""
+    rng = np.random.default_rng(M + K)
+    W = ref.Q4(ctx, rng, N, K, g, True)
+    codes = np.stack([W.bufs[0].numpy() & 15, W.bufs[0].numpy() >> 4], 2).reshape(N, K)
+    s = np.zeros((N, K // g), np.float32)
+    s[:, 0] = 2.0 ** power
+    z = np.full((N, K // g), 1.9375, np.float32)
+    z[:, 0] = 0
+    W.bufs[1].write(ref.bf16(s))
+    W.bufs[2].write(ref.bf16(z))
+    w = ref.values(codes, s, z, g)
+    x = np.full((M, K), 1.9375, np.float32)
+    dx, out = ctx.upload(x), ctx.empty((M, N))
+    assert ran(ctx, lambda: ctx.linear(W.w, M, out, x=dx, precision=1)) == {name}
+    want = x.astype(np.float64) @ w.T
+    err = np.abs(out.numpy() - want)
+    tol = ref.bound(x.astype(np.float64), w, K, 1, False, want, want)
+    assert np.all(err <= tol), (err / tol).max()
