@@ -70,8 +70,7 @@ export class LatentPipeline {
 
   // Several prompts (as encode's) at once -> their conditionings, in order: those not cached pass the text
   // encoder together (Qwen3.encodeBatch: the tokens that they all begin with once).  They alone stay cached.
-  // A call that starts meanwhile
-  // leaves this one's conditionings alone; LoRAs attached meanwhile end it with an error.
+  // A call that starts meanwhile leaves this one's conditionings alone; LoRAs attached meanwhile end it with an error.
   async encodeBatch(prompts) {
     if (!this.te || !this.adapter) throw new Error("encodeBatch: the pipeline was built without opts.te / opts.adapter");
     const byKey = new Map(prompts.map((p) => [promptKey(p), p]));
