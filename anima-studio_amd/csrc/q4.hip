@@ -460,21 +460,20 @@ __global__ __launch_bounds__(256) void q4_prep_kernel(Q4Prep a) {
 }
 
 // Eight codes, times the scale pair s, in the order 0 4 1 5 2 6 3 7.  A code's bits in the mantissa of 1024 are 1024 + c, four places
-// further up 1024 + 16 c: less 1032, or a 16th of it less 72 in one instruction, is c - 8 exactly, and both meet the same s.
+// further up in that of 64 they are 64 + c: less 1032, or 72, it is c - 8 exactly, and both meet the same s.
 struct Q4Bits {  // (in registers: an instruction takes one constant of its own, and v_and_or two)
-  uint32_t even = 0x000f000fu, odd = 0x00f000f0u, big = 0x64006400u;
-  __device__ __forceinline__ Q4Bits() { asm("" : "+s"(even), "+s"(odd), "+v"(big)); }
+  uint32_t even = 0x000f000fu, odd = 0x00f000f0u, big = 0x64006400u, big_odd = 0x54005400u;
+  __device__ __forceinline__ Q4Bits() { asm("" : "+s"(even), "+s"(odd), "+v"(big), "+v"(big_odd)); }
 };
 __device__ __forceinline__ f16x8 q4_decode(const Q4Bits& b, uint32_t c, f16x2 s) {
-  const f16x2 off = {(_Float16)-1032.0f, (_Float16)-1032.0f}, off16 = {(_Float16)-72.0f, (_Float16)-72.0f},
-              part = {(_Float16)0.0625f, (_Float16)0.0625f};
+  const f16x2 off = {(_Float16)-1032.0f, (_Float16)-1032.0f}, off_odd = {(_Float16)-72.0f, (_Float16)-72.0f};
   f16x8 r;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    const f16x2 k = __builtin_bit_cast(f16x2, ((i < 2 ? c : c >> 8) & (i & 1 ? b.odd : b.even)) | b.big);
-    const f16x2 v = (i & 1 ? __builtin_elementwise_fma(k, part, off16) : k + off) * s;
-    r[2 * i] = v[0];
-    r[2 * i + 1] = v[1];
+    const uint32_t v = i < 2 ? c : c >> 8;
+    const f16x2 k = __builtin_bit_cast(f16x2, i & 1 ? (v & b.odd) | b.big_odd : (v & b.even) | b.big), w = (k + (i & 1 ? off_odd : off)) * s;
+    r[2 * i] = w[0];
+    r[2 * i + 1] = w[1];
   }
   return r;
 }
